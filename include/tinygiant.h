@@ -333,6 +333,66 @@ int tg_cuda_debug_div_check(long long n, unsigned seed, unsigned long long *mism
 int tg_cuda_matmul_q4k_noalloc(const uint8_t *q4_matrix, const float *input, float *output, int nrows, int ncols,
                                void *stream);
 
+/* ---- Attention on device tensors ---------------------------------------- *
+ * No counterpart in the reference: the attention of batched serving, for
+ * callers whose activations and caches live on the GPU.  Every pointer is
+ * caller-owned device memory on the current device; dtype 0 is bf16, 1 fp16
+ * (q, k, v, out alike); head_dim is a multiple of 8, at most 128; q, k, v and
+ * out start on 16-byte boundaries, their innermost dimension is contiguous and
+ * their strides (in elements) are positive multiples of 8.  Softmax
+ * statistics, accumulators and weights are fp32.  The calls enqueue on
+ * `stream` (a cudaStream_t), allocate nothing, keep nothing and can be
+ * captured in a graph; concurrent calls need workspaces of their own.  Return
+ * 0 when enqueued, else the error code that tg_cuda_last_error reports. */
+
+/* Causal attention of n_seqs sequences packed one after another.  Sequence s
+ * has the query rows cu_q[s] .. cu_q[s+1] and the keys cu_k[s] .. cu_k[s+1]
+ * (n_seqs + 1 ascending values from 0 to the total; values outside are read
+ * as the nearest one inside).  With nq queries and nk keys, query i is at
+ * position nk - nq + i and attends to the keys j up to it, with window > 0 to
+ * the last `window` of those.  sinks [n_heads] (or NULL): a logit per head
+ * that takes part in the softmax's sum without a value.  A query without a
+ * key gives zeros.  strides: token and head of q, k, v, out (8 values).
+ * max_k: an upper bound of the sequences' keys, for the workspace's size
+ * only.  workspace: 256-byte aligned, tg_attention_prompt_workspace bytes. */
+size_t tg_attention_prompt_workspace(int n_seqs, int total_q, int max_k, int n_heads, int n_kv_heads, int head_dim);
+int tg_attention_prompt(int dtype, const void *q, const void *k, const void *v, void *out, const int *cu_q,
+                        const int *cu_k, const float *sinks, int n_seqs, int total_q, int total_k, int max_k,
+                        int n_heads, int n_kv_heads, int head_dim, const int64_t *strides, int window, float scale,
+                        void *workspace, size_t workspace_bytes, void *stream);
+
+/* One new token of each of `batch` sequences: q [batch][n_heads] over the
+ * prefix that all share (prefix_k, prefix_v [n_kv_heads][prefix_len], at the
+ * positions 0 .. prefix_len - 1, read once for the batch) and the sequence's
+ * own keys k, v [batch][n_kv_heads][cap] behind it, lens[b] of them (values
+ * outside 0 .. max_len count as the nearest inside; max_len <= cap), its
+ * newest token's the last.  window, sinks: as above.  weights (or NULL)
+ * [batch][n_kv_heads][cap] fp32: each own key's softmax weight, summed over
+ * the query heads that share it, is added.  strides: q, out as above;
+ * in all: q (row, head), prefix_k (head, position), prefix_v, k (sequence,
+ * head, position), v, out (row, head), weights (sequence, head): 16 values.
+ * workspace: 256-byte aligned, tg_attention_shared_workspace bytes. */
+size_t tg_attention_shared_workspace(int batch, int prefix_len, int max_len, int n_heads, int n_kv_heads,
+                                     int head_dim, int with_weights);
+int tg_attention_shared(int dtype, const void *q, const void *prefix_k, const void *prefix_v, const void *k,
+                        const void *v, void *out, const int *lens, const float *sinks, float *weights, int batch,
+                        int prefix_len, int cap, int max_len, int n_heads, int n_kv_heads, int head_dim,
+                        const int64_t *strides, int window, float scale, void *workspace, size_t workspace_bytes,
+                        void *stream);
+
+/* Cuts a cache k, v [batch][n_kv_heads][cap][head_dim] (16-bit values of any
+ * type) down to `keep` positions.  Of the n = lens[b] positions of sequence b
+ * and each key head, min(n, keep) stay, in the order they had: the last
+ * `recent` of them and of the others those of the largest weight (equal
+ * weights: the earlier position; NaN above all numbers).  k_out, v_out
+ * [batch][n_kv_heads][keep][head_dim], weights_out and indices (the old
+ * positions) [batch][n_kv_heads][keep], lens_out [batch] are contiguous and
+ * overlap no input; behind a sequence's end they hold zeros and -1.  strides:
+ * k (sequence, head, position), v, weights (sequence, head): 8 values. */
+int tg_cache_evict(const void *k, const void *v, const float *weights, const int *lens, void *k_out, void *v_out,
+                   float *weights_out, int *lens_out, int *indices, int batch, int cap, int n_kv_heads, int head_dim,
+                   const int64_t *strides, int keep, int recent, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -89,6 +89,12 @@ EXT = {
     "tg_cuda_stream": ([], VP),
     "tg_cuda_synchronize": ([], CI),
     "tg_cuda_matmul_q4k_noalloc": ([VP, VP, VP, CI, CI, VP], CI),
+    "tg_attention_prompt_workspace": ([CI, CI, CI, CI, CI, CI], SZ),
+    "tg_attention_prompt": ([CI, VP, VP, VP, VP, VP, VP, VP, CI, CI, CI, CI, CI, CI, CI, VP, CI, CF, VP, SZ, VP], CI),
+    "tg_attention_shared_workspace": ([CI, CI, CI, CI, CI, CI, CI], SZ),
+    "tg_attention_shared": ([CI, VP, VP, VP, VP, VP, VP, VP, VP, VP, CI, CI, CI, CI, CI, CI, CI, VP, CI, CF, VP, SZ,
+                             VP], CI),
+    "tg_cache_evict": ([VP, VP, VP, VP, VP, VP, VP, VP, VP, CI, CI, CI, CI, VP, CI, CI, VP], CI),
 }
 
 

@@ -1,0 +1,88 @@
+// tg_attn.h — what the attention operators on device tensors share
+// (tg_attn_prompt.cu, tg_attn_shared.cu, tg_kv_evict.cu): element types,
+// argument checks of their C entries, conversions.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+
+#include "tg_runtime.h"
+
+namespace tg {
+
+enum { ATTN_BF16 = 0, ATTN_FP16 = 1 };
+constexpr int ATTN_MAX_HD = 128;   // head_dim limit of the operators, a multiple of 8
+constexpr float LOG2E = 1.4426950408889634f;
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T x);
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+
+// The checks of one C entry: the first failure records an error (code 3, bad
+// arguments; 2, no device) under the entry's name and sticks.
+struct ArgCheck {
+  const char* what;
+  int dev = -1;
+  int rc = 0;
+  explicit ArgCheck(const char* w) : what(w) {}
+  // A condition on the arguments; the text says what is wanted.
+  bool need(bool ok, const char* text) {
+    if (!ok && !rc) {
+      set_host_error(3, "%s: %s", what, text);
+      rc = 3;
+    }
+    return rc == 0;
+  }
+  bool device() {
+    if (rc) return false;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) {
+      set_host_error(2, "%s: no usable CUDA device (%s)", what, cudaGetErrorString(e));
+      rc = 2;
+    }
+    return rc == 0;
+  }
+  // Device memory of the current device, aligned to `align` bytes.
+  bool ptr(const void* p, unsigned align, const char* name) {
+    if (rc) return false;
+    cudaPointerAttributes a{};
+    const bool ok = p && cudaPointerGetAttributes(&a, p) == cudaSuccess &&
+                    (a.type == cudaMemoryTypeDevice || a.type == cudaMemoryTypeManaged) && a.device == dev;
+    if (!ok) {
+      cudaGetLastError();
+      set_host_error(3, "%s: %s must be device memory on the current device %d", what, name, dev);
+      rc = 3;
+    } else if ((uintptr_t)p % align) {
+      set_host_error(3, "%s: %s must be %u-byte aligned", what, name, align);
+      rc = 3;
+    }
+    return rc == 0;
+  }
+  // Strides in elements of a 16-bit tensor: positive multiples of 8 (16 bytes).
+  bool strides(const int64_t* s, int n) {
+    for (int i = 0; i < n && !rc; i++) need(s[i] > 0 && s[i] % 8 == 0 && s[i] < (1ll << 38), "strides must be positive multiples of 8 elements");
+    return rc == 0;
+  }
+  // The result of the launches.
+  int done(cudaError_t e) {
+    if (!rc && e != cudaSuccess) {
+      rc = 100 + (int)e;
+      set_host_error(rc, "%s: launch failed: %s", what, cudaGetErrorString(e));
+    }
+    return rc;
+  }
+};
+
+}  // namespace tg
