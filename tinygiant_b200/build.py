@@ -43,12 +43,21 @@ def _stale(target, deps):
     return any(d.stat().st_mtime > t for d in deps)
 
 
+# The attention operators on device tensors are bound by their tolerances, not
+# by another program's rounding: their products and sums may be fused.
+FUSED = {"tg_attn_prompt.cu", "tg_attn_shared.cu", "tg_kv_evict.cu"}
+
+
+def _flags(src):
+    return [f for f in NVCC_FLAGS if f != "--fmad=false" or src not in FUSED]
+
+
 def _compile(src, verbose):
     obj = BUILD / (src + ".o")
     deps = [CSRC / src] + HEADERS
     if not _stale(obj, deps):
         return obj, False
-    cmd = [nvcc()] + NVCC_FLAGS + ["-c", str(CSRC / src), "-o", str(obj)]
+    cmd = [nvcc()] + _flags(src) + ["-c", str(CSRC / src), "-o", str(obj)]
     if src.endswith(".cu"):
         cmd[1:1] = ["-x", "cu"]
     if verbose:

@@ -9,76 +9,234 @@
 //   o_i = sum_K e^(x_j) v_j / (sum_K e^(x_j) + e^sink).
 // Rows without a key give zeros.
 //
-// A warp per (row, query head): lanes take 32 keys at a time, a running
-// maximum m, sum l and accumulator; one pass over the keys.
+// Three launches.  plan_kernel (one CTA) reads the lengths on the device and
+// lists the units of work, longest first, splitting the keys of those that
+// cost more than an SM's share of the whole; the tensor-core kernel
+// (tg_attn_tc.cuh) works through the list; combine_kernel joins split units.
+#include <algorithm>
+
 #include "../../include/tinygiant.h"
-#include "tg_attn.h"
+#include "tg_attn_tc.cuh"
 
 namespace tg {
 
-struct PromptArgs {
-  const void *q, *k, *v;
-  void* out;
+constexpr int PLAN_THREADS = 1024;
+constexpr int PLAN_BUCKETS = 512;
+constexpr int MIN_PIECE = 4;    // key blocks of a split unit's piece, at least
+
+static __device__ DevStatus g_attn_status;
+
+DevStatus* attn_status() {
+  static DevStatus* at[64] = {};
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+  if (!at[dev] && cudaGetSymbolAddress((void**)&at[dev], g_attn_status) != cudaSuccess) cudaGetLastError();
+  return at[dev];
+}
+
+struct PlanArgs {
+  AttnHead* head;
+  AttnEntry* entries;
+  AttnSplit* splits;
   const int *cu_q, *cu_k;
-  const float* sinks;
-  int n_seqs, total_q, total_k, H, KH, hd, window;
-  long long sq[2], sk[2], sv[2], so[2];   // token and head strides, in elements
-  float scale;
+  int n_seqs, total_q, total_k, tpu, KH, window, sms;
+  int max_entries, max_slots;   // capacities (slots per key head)
 };
 
-template <typename T>
-__global__ void __launch_bounds__(128) prompt_rows_kernel(const PromptArgs a) {
-  __shared__ float qs[4][ATTN_MAX_HD];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const long long item = (long long)blockIdx.x * 4 + w;
-  if (item >= (long long)a.total_q * a.H) return;
-  const int row = (int)(item / a.H), h = (int)(item % a.H), kh = h / (a.H / a.KH);
-  int s = 0;
-  while (s < a.n_seqs && a.cu_q[s + 1] <= row) s++;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-  if (s < a.n_seqs && a.cu_q[s] <= row) {
-    const int k0 = max(0, a.cu_k[s]), nk = min(a.total_k, a.cu_k[s + 1]) - k0;
-    const int p = nk - (a.cu_q[s + 1] - row);
-    const int lo = a.window > 0 ? max(0, p - a.window + 1) : 0;
-    const T* q = (const T*)a.q + row * a.sq[0] + h * a.sq[1];
-    for (int d = lane; d < a.hd; d += 32) qs[w][d] = to_f32(q[d]);
-    __syncwarp();
-    for (int j0 = lo; j0 <= p; j0 += 32) {
-      const int j = j0 + lane;
-      float x = -INFINITY;
-      if (j <= p) {
-        const T* k = (const T*)a.k + (long long)(k0 + j) * a.sk[0] + kh * a.sk[1];
-        x = 0.f;
-        for (int d = 0; d < a.hd; d++) x = fmaf(qs[w][d], to_f32(k[d]), x);
-        x *= a.scale;
-      }
-      float t = x;
-      for (int o = 16; o; o >>= 1) t = fmaxf(t, __shfl_xor_sync(~0u, t, o));
-      const float mn = fmaxf(m, t), m0 = mn == -INFINITY ? 0.f : mn, c = expf(m - m0);
-      const float e = expf(x - m0);
-      float sum = e;
-      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-      l = l * c + sum;
-      m = mn;
-      for (int r = 0; r < 4; r++) acc[r] *= c;
-      for (int i = 0; i < 32 && j0 + i <= p; i++) {
-        const float ei = __shfl_sync(~0u, e, i);
-        const T* v = (const T*)a.v + (long long)(k0 + j0 + i) * a.sv[0] + kh * a.sv[1];
-        for (int r = 0; r < 4; r++)
-          if (lane + 32 * r < a.hd) acc[r] = fmaf(ei, to_f32(v[lane + 32 * r]), acc[r]);
+__global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const PlanArgs a) {
+  __shared__ int hist[PLAN_BUCKETS];
+  __shared__ unsigned long long s_total;
+  __shared__ int s_max, s_slots, s_splits, s_n;
+  pdl_trigger();
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  if (tid == 0) s_total = 0, s_max = 0, s_slots = 0, s_splits = 0;
+  for (int i = tid; i < PLAN_BUCKETS; i += PLAN_THREADS) hist[i] = 0;
+  __syncthreads();
+  // f(entry, cost) for every unit: a warp per sequence, or all threads one
+  // sequence after the other when there are few
+  auto each = [&](auto f) {
+    const bool few = a.n_seqs < PLAN_THREADS / 32;
+    for (int s = few ? 0 : w; s < a.n_seqs; s += few ? 1 : PLAN_THREADS / 32) {
+      const int q0 = min(max(a.cu_q[s], 0), a.total_q), nq = min(max(a.cu_q[s + 1], 0), a.total_q) - q0;
+      const int k0 = min(max(a.cu_k[s], 0), a.total_k), nk = max(0, min(max(a.cu_k[s + 1], 0), a.total_k) - k0);
+      for (int t0 = (few ? tid : lane) * a.tpu; t0 < nq; t0 += (few ? PLAN_THREADS : 32) * a.tpu) {
+        AttnEntry e;
+        e.q0 = q0 + t0;
+        e.ntok = min(a.tpu, nq - t0);
+        e.p0 = nk - nq + t0;
+        e.k0 = k0;
+        e.nk = nk;
+        const int hi = e.p0 + e.ntok, lo = a.window > 0 ? max(0, e.p0 + 1 - a.window) : 0;
+        e.kb0 = lo / AT_KEYS;
+        e.kb1 = hi > 0 ? (hi + AT_KEYS - 1) / AT_KEYS : e.kb0;
+        e.slot = -1;
+        f(e, e.kb1 - e.kb0);
       }
     }
-    if (a.sinks) {
-      const float sk = a.sinks[h], mn = fmaxf(m, sk), c = expf(m - mn);
-      if (m != -INFINITY) {
-        l = l * c + expf(sk - mn);
-        for (int r = 0; r < 4; r++) acc[r] *= c;
-      }
-    }
+  };
+  unsigned long long sum = 0;
+  int mx = 0;
+  each([&](const AttnEntry& e, int cost) {
+    sum += cost;
+    mx = max(mx, cost);
+  });
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+  mx = __reduce_max_sync(~0u, mx);
+  if (lane == 0) {
+    atomicAdd(&s_total, sum);
+    atomicMax(&s_max, mx);
   }
-  T* o = (T*)a.out + row * a.so[0] + h * a.so[1];
-  for (int r = 0; r < 4; r++)
-    if (lane + 32 * r < a.hd) o[lane + 32 * r] = from_f32<T>(l > 0.f ? acc[r] / l : 0.f);
+  __syncthreads();
+  // Units of more than `share` blocks are split into equal pieces of at most
+  // that.  There are at most 2 total / share such pieces, which bounds them
+  // by the capacity.
+  const unsigned long long total = s_total;
+  int share = 0x7fffffff;
+  if (a.max_slots > 0) {
+    const unsigned long long even = (total * a.KH + a.sms - 1) / a.sms, room = (2 * total + a.max_slots - 1) / a.max_slots;
+    share = (int)min((unsigned long long)0x7fffffff, max((unsigned long long)MIN_PIECE, max(even, room)));
+  }
+  auto pieces = [&](int cost) { return cost > share ? (cost + share - 1) / share : 1; };
+  const int top = max(1, min(s_max, share));
+  auto bucket = [&](int size) { return top < PLAN_BUCKETS ? top - size : (int)((long long)(top - size) * PLAN_BUCKETS / (top + 1)); };
+  each([&](const AttnEntry& e, int cost) {
+    const int n = pieces(cost);
+    atomicAdd(&hist[bucket((cost + n - 1) / n)], n);
+  });
+  __syncthreads();
+  if (w == 0) {   // exclusive sums: where each bucket starts
+    int run = 0;
+    for (int b0 = 0; b0 < PLAN_BUCKETS; b0 += 32) {
+      const int v = hist[b0 + lane];
+      int x = v;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(~0u, x, o);
+        if (lane >= o) x += y;
+      }
+      hist[b0 + lane] = run + x - v;
+      run += __shfl_sync(~0u, x, 31);
+    }
+    if (lane == 0) s_n = run;
+  }
+  __syncthreads();
+  each([&](const AttnEntry& e, int cost) {
+    const int n = pieces(cost);
+    int at = atomicAdd(&hist[bucket((cost + n - 1) / n)], n);
+    AttnEntry x = e;
+    if (n > 1) {
+      x.slot = atomicAdd(&s_slots, n);
+      const int i = atomicAdd(&s_splits, 1);
+      if (x.slot + n > a.max_slots) return;   // not reached: see the bound above
+      a.splits[i] = AttnSplit{e.q0, e.ntok, x.slot, n};
+    }
+    for (int i = 0; i < n; i++, at++) {
+      x.kb0 = e.kb0 + (int)((long long)cost * i / n);
+      x.kb1 = e.kb0 + (int)((long long)cost * (i + 1) / n);
+      if (at < a.max_entries) a.entries[at] = x;
+      x.slot += n > 1;
+    }
+  });
+  __syncthreads();
+  if (tid == 0) {
+    a.head->n_entries = min(s_n, a.max_entries);
+    a.head->counter = 0;
+    a.head->n_splits = min(s_splits, a.max_slots);
+  }
+}
+
+struct CombineArgs {
+  const AttnHead* head;
+  const AttnSplit* splits;
+  const float* po;
+  const float2* pml;
+  const float* sinks;
+  void* out;
+  long long so[2];
+  int G, KH, hd, tpt;
+};
+
+// A warp per (split unit, key head, tile row): the pieces' accumulators
+// weighted by 2^(c m - M), M the largest of the c m and the sink's.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
+  pdl_wait();
+  const int lane = threadIdx.x & 31, n = a.head->n_splits * a.KH * 2 * AT_ROWS;
+  for (int i = blockIdx.x * 8 + (threadIdx.x >> 5); i < n; i += gridDim.x * 8) {
+    const int row = i % AT_ROWS, t = i / AT_ROWS % 2, kh = i / (2 * AT_ROWS) % a.KH;
+    const AttnSplit s = a.splits[i / (2 * AT_ROWS * a.KH)];
+    const int tok = row / a.G, g = row - tok * a.G, tt = t * a.tpt + tok, h = kh * a.G + g;
+    if (tok >= a.tpt || tt >= s.ntok) continue;
+    auto at = [&](int p) { return ((size_t)(s.slot + p) * a.KH + kh) * (2 * AT_ROWS) + t * AT_ROWS + row; };
+    float M = -INFINITY;
+    for (int p = 0; p < s.n; p++) M = fmaxf(M, a.pml[at(p)].x);
+    float l = 0.f;
+    if (a.sinks && M != -INFINITY) {
+      const float sk = a.sinks[h] * LOG2E;
+      M = fmaxf(M, sk);
+      l = at_exp2(sk - M);
+    }
+    constexpr int E = HD / 32;
+    float o[E] = {};
+    for (int p = 0; p < s.n; p++) {
+      const float2 ml = a.pml[at(p)];
+      if (ml.y == 0.f) continue;   // a piece without keys for this row
+      const float f = at_exp2(ml.x - M);
+      l = fmaf(ml.y, f, l);
+      const float* po = a.po + at(p) * HD + lane * E;
+      if (E == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(po);
+        o[0] = fmaf(x.x, f, o[0]), o[1] = fmaf(x.y, f, o[1]), o[E - 2] = fmaf(x.z, f, o[E - 2]), o[E - 1] = fmaf(x.w, f, o[E - 1]);
+      } else {
+        const float2 x = *reinterpret_cast<const float2*>(po);
+        o[0] = fmaf(x.x, f, o[0]), o[1] = fmaf(x.y, f, o[1]);
+      }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* out = (T*)a.out + (s.q0 + tt) * a.so[0] + h * a.so[1] + lane * E;
+    if (lane * E < a.hd)
+      for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(out + e) = at_pack<T>(o[e] * inv, o[e + 1] * inv);
+  }
+}
+
+// The workspace: header, entries, splits, then the partial results.
+struct PromptSpace {
+  int max_entries, max_slots;
+  size_t entries, splits, pml, po, bytes;
+  PromptSpace(int n_seqs, int total_q, int max_k, int H, int KH, int hd) {
+    const long long tpu = 2 * (AT_ROWS / (H / KH)), units = (total_q + tpu - 1) / tpu + n_seqs;
+    const long long blocks = (max_k + AT_KEYS - 1) / AT_KEYS;
+    // pieces of split units per key head: two per SM, and no more than units of the longest sequence's keys make
+    const long long slots = blocks <= MIN_PIECE ? 0 : std::min((long long)(2 * attn_sms() / KH + 1), units * ((blocks + MIN_PIECE - 1) / MIN_PIECE));
+    max_slots = (int)slots;
+    max_entries = (int)std::min(units + slots, (long long)1 << 30);
+    auto take = [&](size_t n) {
+      const size_t o = bytes;
+      bytes = (bytes + n + 255) & ~(size_t)255;
+      return o;
+    };
+    bytes = 0;
+    take(sizeof(AttnHead));
+    entries = take(sizeof(AttnEntry) * max_entries);
+    splits = take(sizeof(AttnSplit) * max_slots);
+    const size_t rows = (size_t)max_slots * KH * 2 * AT_ROWS;
+    pml = take(sizeof(float2) * rows);
+    po = take(sizeof(float) * rows * (hd <= 64 ? 64 : 128));
+  }
+};
+
+template <typename T, int HD>
+static cudaError_t run_prompt(const PlanArgs& p, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const AttnTcArgs& a,
+                              const CombineArgs& c, long long units, cudaStream_t s) {
+  plan_kernel<<<1, PLAN_THREADS, 0, s>>>(p);
+  cudaError_t e = cudaGetLastError();
+  const long long work = (units + p.max_slots) * p.KH;
+  if (e == cudaSuccess) e = launch_attn_tc<T, HD, false>(qm, km, vm, a, (int)std::min((long long)p.sms, work), s);
+  count_launches(2);
+  if (e == cudaSuccess && p.max_slots > 0) {
+    e = launch_pdl(combine_kernel<T, HD>, dim3(2 * p.sms), 256, 0, s, c);
+    count_launches(1);
+  }
+  return e;
 }
 
 }  // namespace tg
@@ -87,7 +245,8 @@ using namespace tg;
 
 extern "C" size_t tg_attention_prompt_workspace(int n_seqs, int total_q, int max_k, int n_heads, int n_kv_heads,
                                                 int head_dim) {
-  return 0;
+  if (n_seqs < 0 || total_q < 0 || max_k < 0 || n_kv_heads <= 0 || n_heads < n_kv_heads || n_heads / n_kv_heads > AT_ROWS) return 0;
+  return PromptSpace(n_seqs, total_q, max_k, n_heads, n_kv_heads, head_dim).bytes;
 }
 
 extern "C" int tg_attention_prompt(int dtype, const void* q, const void* k, const void* v, void* out, const int* cu_q,
@@ -97,6 +256,7 @@ extern "C" int tg_attention_prompt(int dtype, const void* q, const void* k, cons
   ArgCheck c("tg_attention_prompt");
   c.need(dtype == ATTN_BF16 || dtype == ATTN_FP16, "dtype must be 0 (bf16) or 1 (fp16)");
   c.need(n_seqs >= 0 && total_q >= 0 && total_k >= 0 && max_k >= 0 && window >= 0, "counts must not be negative");
+  c.need(total_q < AT_NPOS && total_k < AT_NPOS, "too many rows");
   c.need(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && n_heads / n_kv_heads <= 128,
          "n_heads must be a multiple of n_kv_heads, at most 128 times it");
   c.need(head_dim > 0 && head_dim % 8 == 0 && head_dim <= ATTN_MAX_HD, "head_dim must be a multiple of 8, at most 128");
@@ -109,18 +269,38 @@ extern "C" int tg_attention_prompt(int dtype, const void* q, const void* k, cons
   c.ptr(q, 16, "q"), c.ptr(out, 16, "out"), c.ptr(cu_q, 4, "cu_q"), c.ptr(cu_k, 4, "cu_k");
   if (total_k > 0) c.ptr(k, 16, "k"), c.ptr(v, 16, "v");
   if (sinks) c.ptr(sinks, 4, "sinks");
+  const PromptSpace sp(n_seqs, total_q, max_k, n_heads, n_kv_heads, head_dim);
+  c.need(workspace_bytes >= sp.bytes, "the workspace is smaller than tg_attention_prompt_workspace says");
+  c.ptr(workspace, 256, "workspace");
   if (c.rc) return c.rc;
-  PromptArgs a{q, k, v, out, cu_q, cu_k, sinks, n_seqs, total_q, total_k, n_heads, n_kv_heads, head_dim, window,
-               {strides[0], strides[1]}, {strides[2], strides[3]}, {strides[4], strides[5]}, {strides[6], strides[7]},
-               scale};
-  const long long items = (long long)total_q * n_heads, grid = (items + 3) / 4;
-  c.need(grid < (1ll << 31), "too many rows");
+
+  const int G = n_heads / n_kv_heads, tpt = AT_ROWS / G;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  PlanArgs p{(AttnHead*)ws, (AttnEntry*)(ws + sp.entries), (AttnSplit*)(ws + sp.splits), cu_q, cu_k, n_seqs, total_q, total_k,
+             2 * tpt, n_kv_heads, window, attn_sms(), sp.max_entries, sp.max_slots};
+  AttnTcArgs a{};
+  a.head = p.head;
+  a.entries = p.entries;
+  a.out = out;
+  a.po = (float*)(ws + sp.po);
+  a.pml = (float2*)(ws + sp.pml);
+  a.sinks = sinks;
+  a.so[0] = strides[6], a.so[1] = strides[7];
+  a.G = G, a.KH = n_kv_heads, a.hd = head_dim, a.tpt = tpt, a.window = window, a.total_k = total_k;
+  a.c = scale * LOG2E;
+  a.st = attn_status();
+  CombineArgs cb{p.head, p.splits, a.po, a.pml, sinks, out, {strides[6], strides[7]}, G, n_kv_heads, head_dim, tpt};
+  CUtensorMap qm, km, vm;
+  c.need(attn_q_map(&qm, dtype, q, head_dim, n_heads, total_q, strides[0], strides[1], G, tpt) &&
+             attn_kv_map(&km, dtype, k, q, head_dim, n_kv_heads, total_k, strides[2], strides[3]) &&
+             attn_kv_map(&vm, dtype, v, q, head_dim, n_kv_heads, total_k, strides[4], strides[5]),
+         "the tensors' shapes and strides do not fit a tensor map");
   if (c.rc) return c.rc;
+  const long long units = (total_q + 2ll * tpt - 1) / (2 * tpt) + n_seqs;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == ATTN_BF16)
-    prompt_rows_kernel<__nv_bfloat16><<<(unsigned)grid, 128, 0, s>>>(a);
-  else
-    prompt_rows_kernel<__half><<<(unsigned)grid, 128, 0, s>>>(a);
-  count_launches(1);
-  return c.done(cudaGetLastError());
+  const bool bf = dtype == ATTN_BF16, small = head_dim <= 64;
+  return c.done(bf ? (small ? run_prompt<__nv_bfloat16, 64>(p, qm, km, vm, a, cb, units, s)
+                            : run_prompt<__nv_bfloat16, 128>(p, qm, km, vm, a, cb, units, s))
+                   : (small ? run_prompt<__half, 64>(p, qm, km, vm, a, cb, units, s)
+                            : run_prompt<__half, 128>(p, qm, km, vm, a, cb, units, s)));
 }
