@@ -40,7 +40,7 @@ namespace tg {
 
 constexpr int AT_ROWS = 128;       // query rows per tile (MMA M)
 constexpr int AT_KEYS = 128;       // keys per block (MMA N of S, K of P V)
-constexpr int AT_THREADS = 320;
+constexpr int AT_THREADS = 384;   // 12 warps, the last two idle: registers move between whole warpgroups
 constexpr int AT_NPOS = 0x3fffffff;
 
 // One piece of work of every key head.
@@ -284,6 +284,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
     return kh >= 0;
   };
 
+  // 168 registers a thread at launch (384 x 168 = 64,512): 216 for the eight
+  // softmax warps and 72 for the four others make the same sum.
+  if (wid >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   if (wid == 8) {
     // ---- loads
     const int tpu = 2 * a.tpt, nub = SHARED ? (a.B + tpu - 1) / tpu : 0;
@@ -435,7 +439,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
       }
     }
     __syncwarp();
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ---- softmax of tile t, a thread per row
     const int t = wid >> 2, row = tid & 127;
     const int tok = row / a.G, g = row - tok * a.G;
