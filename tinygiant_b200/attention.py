@@ -14,66 +14,88 @@ their workspace from torch's allocator, and can be captured in a CUDA graph.
 Tensors may be strided views: the last dimension is contiguous, the other
 strides are multiples of 8 elements, and data start on 16-byte boundaries.
 head_dim is a multiple of 8, at most 128.  Softmax statistics, accumulators
-and weights are fp32.  Bad arguments raise ValueError before anything runs;
-an error of the library raises TinyGiantCudaError.
+and weights are fp32.  Bad arguments raise ValueError before anything runs
+(ArgumentError, a TinyGiantCudaError too, where the library sees them); other
+errors of the library raise TinyGiantCudaError.
 """
 import ctypes
-import math
 
 import torch
 
 from . import TinyGiantCudaError, last_error, load
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+_I64x8, _I64x16 = ctypes.c_int64 * 8, ctypes.c_int64 * 16
+_raw_stream = torch._C._cuda_getCurrentRawStream   # torch.cuda.current_stream(i).cuda_stream, without its objects
 
 
-def _need(ok, text):
-    if not ok:
-        raise ValueError(text)
+class ArgumentError(TinyGiantCudaError, ValueError):
+    """Arguments that the library refused."""
 
 
-def _data(t, name, ndim, like=None):
-    """Checks a 16-bit tensor; its strides, with 8 in the place of those that no index uses."""
-    _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a CUDA tensor")
-    _need(t.dim() == ndim, f"{name} must have {ndim} dimensions, has {t.dim()}")
-    _need(t.dtype in _DTYPES if like is None else t.dtype == like.dtype,
-          f"{name} must be bfloat16 or float16, all of one type; is {t.dtype}")
-    _need(like is None or t.device == like.device, f"{name} must be on {like.device if like is not None else ''}")
-    shape, st = t.shape, t.stride()
-    _need(st[-1] == 1 or shape[-1] == 1, f"{name}'s last dimension must be contiguous")
-    out = []
-    for n, s in zip(shape[:-1], st[:-1]):
-        if n <= 1:
-            s = 8
-        elif s <= 0 or s % 8:
-            raise ValueError(f"{name}'s strides must be positive multiples of 8 elements, are {tuple(st)}")
-        out.append(s)
-    return out
-
-
-def _small(t, name, dtype, shape, like):
-    _need(isinstance(t, torch.Tensor) and t.device == like.device, f"{name} must be a tensor on {like.device}")
-    _need(t.dtype == dtype and tuple(t.shape) == tuple(shape) and t.is_contiguous(),
-          f"{name} must be contiguous {dtype} of shape {tuple(shape)}, is {t.dtype} {tuple(t.shape)}")
-
-
-def _heads(H, KH, hd):
-    _need(KH > 0 and H % KH == 0 and H // KH <= 128, f"{H} query heads do not share {KH} key heads (1 to 128 each)")
-    _need(0 < hd <= 128 and hd % 8 == 0, f"head_dim must be a multiple of 8, at most 128; is {hd}")
+def _call(device, fn, *args):
+    """One library call on torch's current stream of `device` (an index)."""
+    if device != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _call(device, fn, *args)
+    rc = fn(*args, _raw_stream(device))
+    if rc:
+        code, msg = last_error()
+        raise (ArgumentError if rc == 3 else TinyGiantCudaError)(f"[{code}] {msg}")
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _call(device, fn, *args):
-    """One library call on torch's current stream of `device`."""
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _call(device, fn, *args)
-    if fn(*args, torch.cuda.current_stream(device).cuda_stream):
-        code, msg = last_error()
-        raise TinyGiantCudaError(f"[{code}] {msg}")
+# The calls below test their tensors in one expression each, since their whole
+# host time is a few microseconds; _refuse says what is wrong when it fails.
+# What the library can see (strides, counts, alignment) it tests itself.
+
+def _refuse(named, heads=None, small=()):
+    """Raises the ValueError of the first tensor that does not fit.  named: (name, tensor, dimensions, shape or None);
+    heads: (H, KH, hd); small: (name, tensor, dtype, shape)."""
+    def need(ok, text):
+        if not ok:
+            raise ValueError(text)
+
+    _, first, _, _ = named[0]
+    for name, t, ndim, shape in named:
+        need(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a CUDA tensor")
+        need(t.dim() == ndim, f"{name} must have {ndim} dimensions, has {t.dim()}")
+        need(t.dtype in _DTYPES and t.dtype == first.dtype,
+             f"{name} must be bfloat16 or float16, all of one type; is {t.dtype}")
+        need(t.device == first.device, f"{name} must be on {first.device}, is on {t.device}")
+        need(t.stride(-1) == 1, f"{name}'s last dimension must be contiguous")
+    if heads:
+        H, KH, hd = heads
+        need(KH > 0 and H % KH == 0 and H // KH <= 128, f"{H} query heads do not share {KH} key heads (1 to 128 each)")
+        need(0 < hd <= 128 and hd % 8 == 0, f"head_dim must be a multiple of 8, at most 128; is {hd}")
+    for name, t, ndim, shape in named:
+        need(shape is None or tuple(t.shape) == tuple(shape), f"{name} {tuple(t.shape)} and the others do not fit: must be {shape}")
+    for name, t, dtype, shape in small:
+        if t is None:
+            continue
+        need(isinstance(t, torch.Tensor) and t.device == first.device, f"{name} must be a tensor on {first.device}")
+        need(t.dtype == dtype and tuple(t.shape) == tuple(shape), f"{name} must be {dtype} {tuple(shape)}, is {t.dtype} {tuple(t.shape)}")
+        need(t.is_contiguous() or (name == "weights" and t.stride(2) == 1), f"{name} must be contiguous")
+        need(name != "weights" or min(t.stride()) > 0, f"{name} must not be broadcast")
+    raise ValueError("the tensors do not fit one another")
+
+
+def _fits(t, device, dtype):
+    return t.get_device() == device and t.dtype is dtype and t.stride(-1) == 1
+
+
+def _heads_of(q, k):
+    """dtype, device index, shape of q and of k without its leading batch dimension (4-D caches)."""
+    if not (isinstance(q, torch.Tensor) and isinstance(k, torch.Tensor) and q.dtype in _DTYPES and q.is_cuda and q.dim() == 3
+            and k.dim() >= 3):
+        _refuse([("q", q, 3, None), ("k", k, 3, None)])
+    H, KH, hd = q.shape[1], k.shape[1], q.shape[2]
+    if KH == 0 or H % KH or H // KH > 128 or hd % 8 or not 0 < hd <= 128:
+        _refuse([("q", q, 3, None)], (H, KH, hd))
+    return q.dtype, q.get_device(), q.shape, k.shape[-3:] if k.dim() == 3 else (k.shape[0], KH, hd)
 
 
 def attention_prompt(q, k, v, cu_q, cu_k=None, *, max_k=None, window=0, sinks=None, scale=None, out=None):
@@ -90,35 +112,31 @@ def attention_prompt(q, k, v, cu_q, cu_k=None, *, max_k=None, window=0, sinks=No
     sequence, if known (default total_k); it sizes the workspace, and results
     do not depend on it.  Returns out [total_q, H, hd]; out must not overlap
     the inputs."""
-    sq, sk, sv = _data(q, "q", 3), _data(k, "k", 3, q), _data(v, "v", 3, q)
-    (tq, H, hd), (tk, KH, _) = q.shape, k.shape
-    _heads(H, KH, hd)
-    _need(k.shape == v.shape and k.shape[2] == hd, f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit q {tuple(q.shape)}")
-    _need(isinstance(cu_q, torch.Tensor) and cu_q.dim() == 1 and len(cu_q) >= 1, "cu_q must have one value more than there are sequences")
-    _small(cu_q, "cu_q", torch.int32, cu_q.shape, q)
+    dtype, dev, (tq, H, hd), (tk, KH, _) = _heads_of(q, k)
+    n = cu_q.shape[0] - 1 if isinstance(cu_q, torch.Tensor) and cu_q.dim() == 1 else -1
     if cu_k is None:
-        _need(tk == tq, "without cu_k there are as many keys as queries")
+        if tk != tq:
+            raise ValueError(f"without cu_k there are as many keys as queries; got {tk} and {tq}")
         cu_k = cu_q
-    else:
-        _small(cu_k, "cu_k", torch.int32, cu_q.shape, q)
-    if sinks is not None:
-        _small(sinks, "sinks", torch.float32, (H,), q)
-    _need(window >= 0, "window must not be negative")
-    max_k = tk if max_k is None else min(max_k, tk)
-    _need(max_k >= 0, "max_k must not be negative")
     if out is None:
-        out = torch.empty(tq, H, hd, dtype=q.dtype, device=q.device)
-    so = _data(out, "out", 3, q)
-    _need(out.shape == q.shape, f"out must have the shape of q, {tuple(q.shape)}")
-    if tq == 0:
-        return out
-    lib, n = load(), len(cu_q) - 1
+        out = torch.empty((tq, H, hd), dtype=dtype, device=q.device)
+    if not (dev >= 0 and n >= 0 and k.shape == v.shape and k.shape[2] == hd and out.shape == q.shape
+            and _fits(q, dev, dtype) and _fits(k, dev, dtype) and _fits(v, dev, dtype) and _fits(out, dev, dtype)
+            and _fits(cu_q, dev, torch.int32) and _fits(cu_k, dev, torch.int32) and cu_k.shape == cu_q.shape
+            and (sinks is None or (_fits(sinks, dev, torch.float32) and sinks.shape == (H,)))):
+        if out.shape != q.shape:
+            raise ValueError(f"out must have the shape of q, {tuple(q.shape)}")
+        _refuse([("q", q, 3, None), ("k", k, 3, (tk, KH, hd)), ("v", v, 3, (tk, KH, hd)), ("out", out, 3, None)], (H, KH, hd),
+                [("cu_q", cu_q, torch.int32, (max(n, 0) + 1,)), ("cu_k", cu_k, torch.int32, (max(n, 0) + 1,)),
+                 ("sinks", sinks, torch.float32, (H,))])
+    max_k = tk if max_k is None or max_k > tk else max_k
+    lib = load()
     nbytes = lib.tg_attention_prompt_workspace(n, tq, max_k, H, KH, hd)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _call(q.device, lib.tg_attention_prompt, _DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=q.device)
+    (q0, q1, _), (k0, k1, _), (v0, v1, _), (o0, o1, _) = q.stride(), k.stride(), v.stride(), out.stride()
+    _call(dev, lib.tg_attention_prompt, _DTYPES[dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
           cu_q.data_ptr(), cu_k.data_ptr(), _ptr(sinks), n, tq, tk, max_k, H, KH, hd,
-          (ctypes.c_int64 * 8)(*sq, *sk, *sv, *so), window, 1.0 / math.sqrt(hd) if scale is None else scale, _ptr(ws),
-          nbytes)
+          _I64x8(q0, q1, k0, k1, v0, v1, o0, o1), window, hd ** -0.5 if scale is None else scale, ws.data_ptr(), nbytes)
     return out
 
 
@@ -137,44 +155,41 @@ def attention_shared(q, prefix_k, prefix_v, k, v, lens, *, max_len=None, window=
     counts as max_len.  A sequence without a key gives zeros.  Rows of the
     caches behind lens are not read as values: they may hold anything.
     Returns out [B, H, hd]."""
-    sq, sk, sv = _data(q, "q", 3), _data(k, "k", 4, q), _data(v, "v", 4, q)
-    (B, H, hd), (_, KH, cap, _) = q.shape, k.shape
-    _heads(H, KH, hd)
-    _need(k.shape == v.shape and tuple(k.shape) == (B, KH, cap, hd),
-          f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit q {tuple(q.shape)}")
-    P, sp = 0, [8, 8, 8, 8]
-    if prefix_k is not None:
-        sp = _data(prefix_k, "prefix_k", 3, q)
-        P = prefix_k.shape[1]
-        _need(prefix_v is not None and prefix_k.shape == prefix_v.shape and tuple(prefix_k.shape) == (KH, P, hd),
-              f"prefix_k and prefix_v must both be [{KH}, P, {hd}]")
-        sp = sp + _data(prefix_v, "prefix_v", 3, q)
-    _small(lens, "lens", torch.int32, (B,), q)
-    if sinks is not None:
-        _small(sinks, "sinks", torch.float32, (H,), q)
-    sw = (1, 1)
-    if weights is not None:
-        _need(isinstance(weights, torch.Tensor) and weights.device == q.device and weights.dtype == torch.float32
-              and tuple(weights.shape) == (B, KH, cap) and (cap <= 1 or weights.stride(2) == 1),
-              f"weights must be float32 [{B}, {KH}, {cap}] with contiguous rows")
-        sw = [s if n > 1 else 1 for n, s in zip(weights.shape[:2], weights.stride()[:2])]
-        _need(min(sw) > 0, "weights must not be broadcast")
-    _need(window >= 0, "window must not be negative")
-    max_len = cap if max_len is None else min(max_len, cap)
-    _need(max_len >= 0, "max_len must not be negative")
+    dtype, dev, (B, H, hd), (_, KH, _) = _heads_of(q, k)
+    P = 0 if prefix_k is None else prefix_k.shape[1] if prefix_k.dim() == 3 else -1
     if out is None:
-        out = torch.empty(B, H, hd, dtype=q.dtype, device=q.device)
-    so = _data(out, "out", 3, q)
-    _need(out.shape == q.shape, f"out must have the shape of q, {tuple(q.shape)}")
-    if B == 0:
-        return out
+        out = torch.empty((B, H, hd), dtype=dtype, device=q.device)
+    if not (dev >= 0 and k.dim() == 4 and k.shape == v.shape and k.shape[0] == B and k.shape[3] == hd and out.shape == q.shape
+            and _fits(q, dev, dtype) and _fits(k, dev, dtype) and _fits(v, dev, dtype) and _fits(out, dev, dtype)
+            and (prefix_k is None if prefix_v is None else
+                 prefix_k is not None and prefix_k.shape == prefix_v.shape == (KH, P, hd) and _fits(prefix_k, dev, dtype)
+                 and _fits(prefix_v, dev, dtype))
+            and _fits(lens, dev, torch.int32) and lens.shape == (B,)
+            and (sinks is None or (_fits(sinks, dev, torch.float32) and sinks.shape == (H,)))
+            and (weights is None or (_fits(weights, dev, torch.float32) and weights.shape == k.shape[:3]
+                                     and min(weights.stride()) > 0))):
+        if out.shape != q.shape:
+            raise ValueError(f"out must have the shape of q, {tuple(q.shape)}")
+        cap = k.shape[2] if k.dim() == 4 else 0
+        named = [("q", q, 3, None), ("k", k, 4, (B, KH, cap, hd)), ("v", v, 4, (B, KH, cap, hd)), ("out", out, 3, None)]
+        if prefix_k is not None or prefix_v is not None:
+            if prefix_k is None or prefix_v is None or prefix_k.shape != prefix_v.shape or prefix_k.shape != (KH, P, hd):
+                raise ValueError(f"prefix_k and prefix_v must both be [{KH}, P, {hd}]")
+            named += [("prefix_k", prefix_k, 3, None), ("prefix_v", prefix_v, 3, None)]
+        _refuse(named, (H, KH, hd), [("lens", lens, torch.int32, (B,)), ("sinks", sinks, torch.float32, (H,)),
+                                     ("weights", weights, torch.float32, (B, KH, cap))])
+    cap = k.shape[2]
+    max_len = cap if max_len is None or max_len > cap else max_len
     lib = load()
     nbytes = lib.tg_attention_shared_workspace(B, P, max_len, H, KH, hd, weights is not None)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _call(q.device, lib.tg_attention_shared, _DTYPES[q.dtype], q.data_ptr(), _ptr(prefix_k), _ptr(prefix_v), k.data_ptr(),
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=q.device)
+    (q0, q1, _), (o0, o1, _), (k0, k1, k2, _), (v0, v1, v2, _) = q.stride(), out.stride(), k.stride(), v.stride()
+    (pk0, pk1, _), (pv0, pv1, _) = (prefix_k.stride(), prefix_v.stride()) if P else ((8, 8, 1), (8, 8, 1))
+    w0, w1, _ = weights.stride() if weights is not None else (1, 1, 1)
+    _call(dev, lib.tg_attention_shared, _DTYPES[dtype], q.data_ptr(), _ptr(prefix_k), _ptr(prefix_v), k.data_ptr(),
           v.data_ptr(), out.data_ptr(), lens.data_ptr(), _ptr(sinks), _ptr(weights), B, P, cap, max_len, H, KH, hd,
-          (ctypes.c_int64 * 16)(*sq, *sp, *sk, *sv, *so, *sw), window, 1.0 / math.sqrt(hd) if scale is None else scale,
-          _ptr(ws), nbytes)
+          _I64x16(q0, q1, pk0, pk1, pv0, pv1, k0, k1, k2, v0, v1, v2, o0, o1, w0, w1), window,
+          hd ** -0.5 if scale is None else scale, ws.data_ptr(), nbytes)
     return out
 
 
@@ -189,23 +204,26 @@ def cache_evict(k, v, weights, lens, keep, recent):
     Returns (k, v, weights, lens, indices): new tensors [B, KH, keep, hd],
     [B, KH, keep, hd], [B, KH, keep], [B] and the positions' old places
     [B, KH, keep] int32; behind a sequence's end they hold zeros and -1."""
-    sk, sv = _data(k, "k", 4), _data(v, "v", 4, k)
-    B, KH, cap, hd = k.shape
-    _heads(KH, KH, hd)
-    _need(k.shape == v.shape, f"k {tuple(k.shape)} and v {tuple(v.shape)} must have one shape")
-    _need(isinstance(weights, torch.Tensor) and weights.device == k.device and weights.dtype == torch.float32
-          and tuple(weights.shape) == (B, KH, cap) and (cap <= 1 or weights.stride(2) == 1),
-          f"weights must be float32 [{B}, {KH}, {cap}] with contiguous rows")
-    sw = [s if n > 1 else 1 for n, s in zip(weights.shape[:2], weights.stride()[:2])]
-    _need(min(sw) > 0, "weights must not be broadcast")
-    _small(lens, "lens", torch.int32, (B,), k)
-    _need(0 < keep <= cap and 0 <= recent <= keep, f"need 0 < keep <= {cap} and 0 <= recent <= keep; got {keep}, {recent}")
-    ko, vo = (torch.empty(B, KH, keep, hd, dtype=k.dtype, device=k.device) for _ in range(2))
-    wo = torch.empty(B, KH, keep, dtype=torch.float32, device=k.device)
-    idx = torch.empty(B, KH, keep, dtype=torch.int32, device=k.device)
-    lo = torch.empty(B, dtype=torch.int32, device=k.device)
-    if B:
-        _call(k.device, load().tg_cache_evict, k.data_ptr(), v.data_ptr(), weights.data_ptr(), lens.data_ptr(),
-              ko.data_ptr(), vo.data_ptr(), wo.data_ptr(), lo.data_ptr(), idx.data_ptr(), B, cap, KH, hd,
-              (ctypes.c_int64 * 8)(*sk, *sv, *sw), keep, recent)
+    shape = k.shape
+    if not (len(shape) == 4 and k.dtype in _DTYPES and k.is_cuda and shape == v.shape and weights.shape == shape[:3]
+            and _fits(k, k.get_device(), k.dtype) and _fits(v, k.get_device(), k.dtype)
+            and _fits(weights, k.get_device(), torch.float32) and min(weights.stride()) > 0
+            and _fits(lens, k.get_device(), torch.int32) and lens.shape == shape[:1]):
+        if k.shape != v.shape:
+            raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must have one shape")
+        _refuse([("k", k, 4, None), ("v", v, 4, None)], None, [("weights", weights, torch.float32, shape[:3]),
+                                                              ("lens", lens, torch.int32, shape[:1])])
+    B, KH, cap, hd = shape
+    dev, where = k.get_device(), k.device
+    if not (0 < keep <= cap and 0 <= recent <= keep):
+        raise ValueError(f"need 0 < keep <= {cap} and 0 <= recent <= keep; got {keep}, {recent}")
+    ko = torch.empty((B, KH, keep, hd), dtype=k.dtype, device=where)
+    vo = torch.empty((B, KH, keep, hd), dtype=k.dtype, device=where)
+    wo = torch.empty((B, KH, keep), dtype=torch.float32, device=where)
+    idx = torch.empty((B, KH, keep), dtype=torch.int32, device=where)
+    lo = torch.empty((B,), dtype=torch.int32, device=where)
+    (k0, k1, k2, _), (v0, v1, v2, _), (w0, w1, _) = k.stride(), v.stride(), weights.stride()
+    _call(dev, load().tg_cache_evict, k.data_ptr(), v.data_ptr(), weights.data_ptr(), lens.data_ptr(), ko.data_ptr(),
+          vo.data_ptr(), wo.data_ptr(), lo.data_ptr(), idx.data_ptr(), B, cap, KH, hd,
+          _I64x8(k0, k1, k2, v0, v1, v2, w0, w1), keep, recent)
     return ko, vo, wo, lo, idx

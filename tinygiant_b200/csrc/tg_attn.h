@@ -70,10 +70,12 @@ struct ArgCheck {
     }
     return rc == 0;
   }
-  // Strides in elements of a 16-bit tensor: positive multiples of 8 (16 bytes).
-  bool strides(const int64_t* s, int n) {
-    for (int i = 0; i < n && !rc; i++) need(s[i] > 0 && s[i] % 8 == 0 && s[i] < (1ll << 38), "strides must be positive multiples of 8 elements");
-    return rc == 0;
+  // The stride, in elements, of a 16-bit tensor's dimension of n values: a
+  // positive multiple of 8 (16 bytes).  One that no index uses may be anything.
+  long long stride(int64_t s, long long n) {
+    if (n <= 1) return 8;
+    need(s > 0 && s % 8 == 0 && s < (1ll << 38), "strides must be positive multiples of 8 elements");
+    return s;
   }
   // The result of the launches.
   int done(cudaError_t e) {

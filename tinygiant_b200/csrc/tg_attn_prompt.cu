@@ -13,6 +13,7 @@
 // lists the units of work, longest first, splitting the keys of those that
 // cost more than an SM's share of the whole; the tensor-core kernel
 // (tg_attn_tc.cuh) works through the list; combine_kernel joins split units.
+// Short sequences need neither plan nor joining.
 #include <algorithm>
 
 #include "../../include/tinygiant.h"
@@ -57,19 +58,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const PlanArgs a) {
   auto each = [&](auto f) {
     const bool few = a.n_seqs < PLAN_THREADS / 32;
     for (int s = few ? 0 : w; s < a.n_seqs; s += few ? 1 : PLAN_THREADS / 32) {
-      const int q0 = min(max(a.cu_q[s], 0), a.total_q), nq = min(max(a.cu_q[s + 1], 0), a.total_q) - q0;
-      const int k0 = min(max(a.cu_k[s], 0), a.total_k), nk = max(0, min(max(a.cu_k[s + 1], 0), a.total_k) - k0);
-      for (int t0 = (few ? tid : lane) * a.tpu; t0 < nq; t0 += (few ? PLAN_THREADS : 32) * a.tpu) {
-        AttnEntry e;
-        e.q0 = q0 + t0;
-        e.ntok = min(a.tpu, nq - t0);
-        e.p0 = nk - nq + t0;
-        e.k0 = k0;
-        e.nk = nk;
-        const int hi = e.p0 + e.ntok, lo = a.window > 0 ? max(0, e.p0 + 1 - a.window) : 0;
-        e.kb0 = lo / AT_KEYS;
-        e.kb1 = hi > 0 ? (hi + AT_KEYS - 1) / AT_KEYS : e.kb0;
-        e.slot = -1;
+      const AttnSeq q = attn_seq(a.cu_q, a.cu_k, s, a.total_q, a.total_k);
+      for (int t0 = (few ? tid : lane) * a.tpu; t0 < q.nq; t0 += (few ? PLAN_THREADS : 32) * a.tpu) {
+        const AttnEntry e = attn_unit(q, t0, a.tpu, a.window);
         f(e, e.kb1 - e.kb0);
       }
     }
@@ -227,11 +218,15 @@ struct PromptSpace {
 template <typename T, int HD>
 static cudaError_t run_prompt(const PlanArgs& p, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const AttnTcArgs& a,
                               const CombineArgs& c, long long units, cudaStream_t s) {
-  plan_kernel<<<1, PLAN_THREADS, 0, s>>>(p);
-  cudaError_t e = cudaGetLastError();
+  cudaError_t e = cudaSuccess;
+  if (a.entries) {
+    plan_kernel<<<1, PLAN_THREADS, 0, s>>>(p);
+    e = cudaGetLastError();
+    count_launches(1);
+  }
   const long long work = (units + p.max_slots) * p.KH;
   if (e == cudaSuccess) e = launch_attn_tc<T, HD, false>(qm, km, vm, a, (int)std::min((long long)p.sms, work), s);
-  count_launches(2);
+  count_launches(1);
   if (e == cudaSuccess && p.max_slots > 0) {
     e = launch_pdl(combine_kernel<T, HD>, dim3(2 * p.sms), 256, 0, s, c);
     count_launches(1);
@@ -255,15 +250,19 @@ extern "C" int tg_attention_prompt(int dtype, const void* q, const void* k, cons
                                    int window, float scale, void* workspace, size_t workspace_bytes, void* stream) {
   ArgCheck c("tg_attention_prompt");
   c.need(dtype == ATTN_BF16 || dtype == ATTN_FP16, "dtype must be 0 (bf16) or 1 (fp16)");
-  c.need(n_seqs >= 0 && total_q >= 0 && total_k >= 0 && max_k >= 0 && window >= 0, "counts must not be negative");
+  c.need(n_seqs >= 0 && total_q >= 0 && total_k >= 0 && max_k >= 0 && window >= 0, "counts and window must not be negative");
   c.need(total_q < AT_NPOS && total_k < AT_NPOS, "too many rows");
   c.need(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && n_heads / n_kv_heads <= 128,
          "n_heads must be a multiple of n_kv_heads, at most 128 times it");
   c.need(head_dim > 0 && head_dim % 8 == 0 && head_dim <= ATTN_MAX_HD, "head_dim must be a multiple of 8, at most 128");
   c.need(std::isfinite(scale) && scale > 0.f, "scale must be finite and positive");
   c.need(strides != nullptr, "strides is null");
-  if (c.rc || !c.strides(strides, 8)) return c.rc;
-  if (total_q == 0) return 0;
+  if (c.rc) return c.rc;
+  const long long n4[4] = {total_q, n_heads, total_k, n_kv_heads};
+  const int dim[8] = {0, 1, 2, 3, 2, 3, 0, 1};
+  long long st[8];
+  for (int i = 0; i < 8; i++) st[i] = c.stride(strides[i], n4[dim[i]]);
+  if (c.rc || total_q == 0) return c.rc;
   c.need(n_seqs > 0, "rows without a sequence");
   if (!c.device()) return c.rc;
   c.ptr(q, 16, "q"), c.ptr(out, 16, "out"), c.ptr(cu_q, 4, "cu_q"), c.ptr(cu_k, 4, "cu_k");
@@ -280,20 +279,24 @@ extern "C" int tg_attention_prompt(int dtype, const void* q, const void* k, cons
              2 * tpt, n_kv_heads, window, attn_sms(), sp.max_entries, sp.max_slots};
   AttnTcArgs a{};
   a.head = p.head;
-  a.entries = p.entries;
+  // Without splits (the longest sequence has no more keys than a split unit's
+  // piece) and with a lane for each sequence the units need no list: the
+  // plan's launch is saved.
+  a.entries = sp.max_slots == 0 && n_seqs <= 32 ? nullptr : p.entries;
+  a.cu_q = cu_q, a.cu_k = cu_k, a.n_seqs = n_seqs, a.total_q = total_q;
   a.out = out;
   a.po = (float*)(ws + sp.po);
   a.pml = (float2*)(ws + sp.pml);
   a.sinks = sinks;
-  a.so[0] = strides[6], a.so[1] = strides[7];
+  a.so[0] = st[6], a.so[1] = st[7];
   a.G = G, a.KH = n_kv_heads, a.hd = head_dim, a.tpt = tpt, a.window = window, a.total_k = total_k;
   a.c = scale * LOG2E;
   a.st = attn_status();
-  CombineArgs cb{p.head, p.splits, a.po, a.pml, sinks, out, {strides[6], strides[7]}, G, n_kv_heads, head_dim, tpt};
+  CombineArgs cb{p.head, p.splits, a.po, a.pml, sinks, out, {st[6], st[7]}, G, n_kv_heads, head_dim, tpt};
   CUtensorMap qm, km, vm;
-  c.need(attn_q_map(&qm, dtype, q, head_dim, n_heads, total_q, strides[0], strides[1], G, tpt) &&
-             attn_kv_map(&km, dtype, k, q, head_dim, n_kv_heads, total_k, strides[2], strides[3]) &&
-             attn_kv_map(&vm, dtype, v, q, head_dim, n_kv_heads, total_k, strides[4], strides[5]),
+  c.need(attn_q_map(&qm, dtype, q, head_dim, n_heads, total_q, st[0], st[1], G, tpt) &&
+             attn_kv_map(&km, dtype, k, q, head_dim, n_kv_heads, total_k, st[2], st[3]) &&
+             attn_kv_map(&vm, dtype, v, q, head_dim, n_kv_heads, total_k, st[4], st[5]),
          "the tensors' shapes and strides do not fit a tensor map");
   if (c.rc) return c.rc;
   const long long units = (total_q + 2ll * tpt - 1) / (2 * tpt) + n_seqs;

@@ -107,13 +107,17 @@ extern "C" int tg_attention_shared(int dtype, const void* q, const void* prefix_
   ArgCheck c("tg_attention_shared");
   c.need(dtype == ATTN_BF16 || dtype == ATTN_FP16, "dtype must be 0 (bf16) or 1 (fp16)");
   c.need(batch >= 0 && prefix_len >= 0 && cap >= 0 && max_len >= 0 && max_len <= cap && window >= 0,
-         "counts must not be negative, and max_len at most cap");
+         "counts and window must not be negative, and max_len at most cap");
   c.need(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && n_heads / n_kv_heads <= 128,
          "n_heads must be a multiple of n_kv_heads, at most 128 times it");
   c.need(head_dim > 0 && head_dim % 8 == 0 && head_dim <= ATTN_MAX_HD, "head_dim must be a multiple of 8, at most 128");
   c.need(std::isfinite(scale) && scale > 0.f, "scale must be finite and positive");
   c.need(strides != nullptr, "strides is null");
-  if (c.rc || !c.strides(strides, 14)) return c.rc;
+  if (c.rc) return c.rc;
+  const long long n5[5] = {batch, n_heads, n_kv_heads, prefix_len, cap};
+  const int dim[14] = {0, 1, 2, 3, 2, 3, 0, 2, 4, 0, 2, 4, 0, 1};
+  long long t[14];
+  for (int i = 0; i < 14; i++) t[i] = c.stride(strides[i], n5[dim[i]]);
   c.need(!weights || (strides[14] > 0 && strides[15] > 0), "strides of weights must be positive");
   if (c.rc || batch == 0) return c.rc;
   if (!c.device()) return c.rc;
@@ -123,10 +127,9 @@ extern "C" int tg_attention_shared(int dtype, const void* q, const void* prefix_
   if (sinks) c.ptr(sinks, 4, "sinks");
   if (weights) c.ptr(weights, 4, "weights");
   if (c.rc) return c.rc;
-  const int64_t* t = strides;
   SharedArgs a{q, prefix_k, prefix_v, k, v, out, lens, sinks, weights, batch, prefix_len, max_len, n_heads, n_kv_heads,
                head_dim, window, {t[0], t[1]}, {t[2], t[3]}, {t[4], t[5]}, {t[6], t[7], t[8]}, {t[9], t[10], t[11]},
-               {t[12], t[13]}, {weights ? t[14] : 0, weights ? t[15] : 0}, scale};
+               {t[12], t[13]}, {weights ? strides[14] : 0, weights ? strides[15] : 0}, scale};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == ATTN_BF16)
     shared_rows_kernel<__nv_bfloat16><<<batch * n_kv_heads, 32, 0, s>>>(a);

@@ -31,6 +31,7 @@
 #pragma once
 #include <cuda.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "tg_attn.h"
@@ -61,9 +62,38 @@ struct __align__(16) AttnSplit {
   int q0, ntok, slot, n;
 };
 
+// A sequence's query and key rows; offsets outside the tensors read as their ends.
+struct AttnSeq {
+  int q0, nq, k0, nk;
+};
+__device__ __forceinline__ AttnSeq attn_seq(const int* cu_q, const int* cu_k, int s, int total_q, int total_k) {
+  AttnSeq r;
+  r.q0 = min(max(cu_q[s], 0), total_q);
+  r.nq = max(0, min(max(cu_q[s + 1], 0), total_q) - r.q0);
+  r.k0 = min(max(cu_k[s], 0), total_k);
+  r.nk = max(0, min(max(cu_k[s + 1], 0), total_k) - r.k0);
+  return r;
+}
+// The unit of a sequence's tokens t0 .. t0 + tpu - 1.
+__device__ __forceinline__ AttnEntry attn_unit(const AttnSeq& s, int t0, int tpu, int window) {
+  AttnEntry e;
+  e.q0 = s.q0 + t0;
+  e.ntok = min(tpu, s.nq - t0);
+  e.p0 = s.nk - s.nq + t0;
+  e.k0 = s.k0;
+  e.nk = s.nk;
+  const int hi = e.p0 + e.ntok, lo = window > 0 ? max(0, e.p0 + 1 - window) : 0;
+  e.kb0 = lo / AT_KEYS;
+  e.kb1 = hi > 0 ? (hi + AT_KEYS - 1) / AT_KEYS : e.kb0;
+  e.slot = -1;
+  return e;
+}
+
 struct AttnTcArgs {
-  AttnHead* head;             // prompt: the plan's; shared: null
-  const AttnEntry* entries;   // prompt
+  AttnHead* head;             // prompt: the plan's
+  const AttnEntry* entries;   // prompt: the plan's, or null: at most 32 sequences, nothing split
+  const int *cu_q, *cu_k;     // prompt without a plan
+  int n_seqs, total_q;
   void* out;
   float* po;                  // partial results [slot * KH + kh][2 * 128][HD]
   float2* pml;                // their (c m, l) [slot * KH + kh][2 * 128]
@@ -252,9 +282,21 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
     if (!*abort) set_error(a.st, ERR_WAIT_TIMEOUT, site, blockIdx.x, u);
     *abort = 1;
   };
+  // Without a plan: lane s of the load warp has sequence s, of at most 32, and
+  // where its units end among those of all.
+  AttnSeq seq{};
+  int ends = 0;
   // Entry i of the work (every lane of the load warp calls it).
   auto unit_of = [&](int i) -> AttnEntry {
-    if (!SHARED) return a.entries[i];
+    if (!SHARED && a.entries) return a.entries[i];
+    if (!SHARED) {
+      const int s = __ffs(__ballot_sync(~0u, ends > i)) - 1;   // the sequence whose units end past i
+      AttnSeq q;
+      q.q0 = __shfl_sync(~0u, seq.q0, s), q.nq = __shfl_sync(~0u, seq.nq, s);
+      q.k0 = __shfl_sync(~0u, seq.k0, s), q.nk = __shfl_sync(~0u, seq.nk, s);
+      const int before = __shfl_sync(~0u, ends, s) - (q.nq + 2 * a.tpt - 1) / (2 * a.tpt);
+      return attn_unit(q, (i - before) * 2 * a.tpt, 2 * a.tpt, a.window);
+    }
     const int tpu = 2 * a.tpt, nblk = (a.P + AT_KEYS - 1) / AT_KEYS, sp = i % a.nsp;
     AttnEntry e{};
     e.q0 = i / a.nsp * tpu;
@@ -290,13 +332,23 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   if (wid == 8) {
     // ---- loads
-    const int tpu = 2 * a.tpt, nub = SHARED ? (a.B + tpu - 1) / tpu : 0;
-    const int n_work = (SHARED ? nub * a.nsp : a.head->n_entries) * a.KH;
+    const int tpu = 2 * a.tpt;
+    const bool fixed = SHARED || !a.entries;   // units dealt out in turn
+    if (!SHARED && !a.entries) {
+      if (lane < a.n_seqs) seq = attn_seq(a.cu_q, a.cu_k, lane, a.total_q, a.total_k);
+      ends = max(0, (seq.nq + tpu - 1) / tpu);
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(~0u, ends, o);
+        if (lane >= o) ends += y;
+      }
+    }
+    const int n_entries = SHARED ? (a.B + tpu - 1) / tpu * a.nsp : a.entries ? a.head->n_entries : __shfl_sync(~0u, ends, 31);
+    const int n_work = n_entries * a.KH;
     int issued = 0, qn = 0, auxn = 0;   // blocks, Q loads and corrected blocks so far
     bool ok = true;
     for (int it = 0; ok; it++) {
-      int w = SHARED ? (int)blockIdx.x + it * (int)gridDim.x : 0;
-      if (!SHARED) {
+      int w = (int)blockIdx.x + it * (int)gridDim.x;
+      if (!fixed) {
         if (lane == 0) w = atomicAdd(&a.head->counter, 1);
         w = __shfl_sync(~0u, w, 0);
       }
@@ -663,7 +715,13 @@ template <typename T, int HD, bool SHARED>
 inline cudaError_t launch_attn_tc(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const AttnTcArgs& a, int grid,
                                   cudaStream_t s) {
   const int smem = AttnTcShape<HD>::SMEM;
-  const cudaError_t e = cudaFuncSetAttribute(attn_tc_kernel<T, HD, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<unsigned long long> set{0};   // devices whose limit is raised
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !(set.load() >> dev & 1))) {
+    e = cudaFuncSetAttribute(attn_tc_kernel<T, HD, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess && dev < 64) set |= 1ull << dev;
+  }
   if (e != cudaSuccess) return e;
   return launch_pdl(attn_tc_kernel<T, HD, SHARED>, dim3(grid), AT_THREADS, smem, s, q, k, v, a);
 }

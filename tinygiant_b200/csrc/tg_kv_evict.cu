@@ -164,7 +164,10 @@ extern "C" int tg_cache_evict(const void* k, const void* v, const float* weights
   c.need(keep > 0 && keep <= cap && recent >= 0 && recent <= keep, "need 0 < keep <= cap and 0 <= recent <= keep");
   c.need(head_dim > 0 && head_dim % 8 == 0 && head_dim <= ATTN_MAX_HD, "head_dim must be a multiple of 8, at most 128");
   c.need(strides != nullptr, "strides is null");
-  if (c.rc || !c.strides(strides, 6)) return c.rc;
+  if (c.rc) return c.rc;
+  const long long n3[3] = {batch, n_kv_heads, cap};
+  long long t[6];
+  for (int i = 0; i < 6; i++) t[i] = c.stride(strides[i], n3[i % 3]);
   c.need(strides[6] > 0 && strides[7] > 0, "strides of weights must be positive");
   c.need((long long)batch * n_kv_heads <= 65535, "batch x n_kv_heads is at most 65535");
   c.need((long long)keep * head_dim < (1ll << 31), "keep x head_dim must be below 2^31");
@@ -176,10 +179,9 @@ extern "C" int tg_cache_evict(const void* k, const void* v, const float* weights
   c.need(k_out != k && k_out != v && v_out != v && v_out != k && weights_out != weights && lens_out != lens,
          "the outputs must not overlap the inputs");
   if (c.rc) return c.rc;
-  const int64_t* t = strides;
   EvictArgs a{(const uint4*)k, (const uint4*)v, weights, lens, (uint4*)k_out, (uint4*)v_out, weights_out, lens_out,
               indices, batch, n_kv_heads, cap, keep, recent, head_dim / 8,
-              {t[0] / 8, t[1] / 8, t[2] / 8}, {t[3] / 8, t[4] / 8, t[5] / 8}, {t[6], t[7]}};
+              {t[0] / 8, t[1] / 8, t[2] / 8}, {t[3] / 8, t[4] / 8, t[5] / 8}, {strides[6], strides[7]}};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int bh = batch * n_kv_heads, words = keep * (head_dim / 8);
   select_kernel<<<bh, EV_THREADS, 0, s>>>(a);
