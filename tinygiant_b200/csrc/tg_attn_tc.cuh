@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
 // ---------------------------------------------------------------------
 // Host side.
 
-inline CUresult attn_map(CUtensorMap* m, int dtype, const void* p, const cuuint64_t* dims, const cuuint64_t* strides,
+inline CUresult attn_map(CUtensorMap* m, int dtype, const void* p, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
                          const cuuint32_t* box) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -660,8 +660,8 @@ inline CUresult attn_map(CUtensorMap* m, int dtype, const void* p, const cuuint6
     return reinterpret_cast<Encode>(fn);
   }();
   if (!encode) return CUDA_ERROR_NOT_SUPPORTED;
-  const cuuint32_t es[3] = {1, 1, 1};
-  return encode(m, dtype == ATTN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(p),
+  const cuuint32_t es[4] = {1, 1, 1, 1};
+  return encode(m, dtype == ATTN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(p),
                 dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
@@ -672,7 +672,7 @@ inline bool attn_q_map(CUtensorMap* m, int dtype, const void* q, int hd, int H, 
   const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)H, (cuuint64_t)rows};
   const cuuint64_t st[2] = {(cuuint64_t)s_head * 2, (cuuint64_t)s_row * 2};
   const cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)tpt};
-  return attn_map(m, dtype, q, dims, st, box) == CUDA_SUCCESS;
+  return attn_map(m, dtype, q, 3, dims, st, box) == CUDA_SUCCESS;
 }
 
 // K or V as [heads][rows][hd] in boxes of 64 elements x 128 rows.  Without
@@ -682,7 +682,16 @@ inline bool attn_kv_map(CUtensorMap* m, int dtype, const void* p, const void* an
   const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)(rows > 0 ? rows : 1), (cuuint64_t)KH};
   const cuuint64_t st[2] = {(cuuint64_t)s_row * 2, (cuuint64_t)s_head * 2};
   const cuuint32_t box[3] = {64, AT_KEYS, 1};
-  return attn_map(m, dtype, rows > 0 ? p : any, dims, st, box) == CUDA_SUCCESS;
+  return attn_map(m, dtype, rows > 0 ? p : any, 3, dims, st, box) == CUDA_SUCCESS;
+}
+
+// A cache [sequences][heads][rows][hd] in boxes of 64 elements x `box_rows` rows.
+inline bool attn_cache_map(CUtensorMap* m, int dtype, const void* p, int hd, int rows, int KH, int B, long long s_row, long long s_head,
+                           long long s_seq, int box_rows) {
+  const cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)rows, (cuuint64_t)KH, (cuuint64_t)B};
+  const cuuint64_t st[3] = {(cuuint64_t)s_row * 2, (cuuint64_t)s_head * 2, (cuuint64_t)s_seq * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
+  return attn_map(m, dtype, p, 4, dims, st, box) == CUDA_SUCCESS;
 }
 
 // Launch with programmatic stream serialization: the kernel may start while
