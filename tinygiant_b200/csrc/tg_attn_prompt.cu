@@ -46,25 +46,53 @@ struct PlanArgs {
 
 __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const PlanArgs a) {
   __shared__ int hist[PLAN_BUCKETS];
+  __shared__ AttnSeq seqs[PLAN_THREADS];
+  __shared__ int ends[PLAN_THREADS];
+  __shared__ int sums[PLAN_THREADS / 32];
   __shared__ unsigned long long s_total;
   __shared__ int s_max, s_slots, s_splits, s_n;
   pdl_trigger();
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   if (tid == 0) s_total = 0, s_max = 0, s_slots = 0, s_splits = 0;
   for (int i = tid; i < PLAN_BUCKETS; i += PLAN_THREADS) hist[i] = 0;
-  __syncthreads();
-  // f(entry, cost) for every unit: a warp per sequence, or all threads one
-  // sequence after the other when there are few
+  // PLAN_THREADS sequences from s0 on in shared memory, with where their
+  // units end; returns the number of their units
+  auto load = [&](int s0) -> int {
+    __syncthreads();
+    AttnSeq q{};
+    if (s0 + tid < a.n_seqs) q = attn_seq(a.cu_q, a.cu_k, s0 + tid, a.total_q, a.total_k);
+    int x = (q.nq + a.tpu - 1) / a.tpu;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(~0u, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) sums[w] = x;
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int i = 0; i < PLAN_THREADS / 32; i++) {
+      if (i < w) before += sums[i];
+      all += sums[i];
+    }
+    seqs[tid] = q;
+    ends[tid] = before + x;
+    __syncthreads();
+    return all;
+  };
+  // f(entry, cost) for every unit
   auto each = [&](auto f) {
-    const bool few = a.n_seqs < PLAN_THREADS / 32;
-    for (int s = few ? 0 : w; s < a.n_seqs; s += few ? 1 : PLAN_THREADS / 32) {
-      const AttnSeq q = attn_seq(a.cu_q, a.cu_k, s, a.total_q, a.total_k);
-      for (int t0 = (few ? tid : lane) * a.tpu; t0 < q.nq; t0 += (few ? PLAN_THREADS : 32) * a.tpu) {
-        const AttnEntry e = attn_unit(q, t0, a.tpu, a.window);
-        f(e, e.kb1 - e.kb0);
+    for (int s0 = 0; s0 < a.n_seqs; s0 += PLAN_THREADS) {
+      const int n = a.n_seqs > PLAN_THREADS ? load(s0) : ends[PLAN_THREADS - 1];
+      for (int u = tid; u < n; u += PLAN_THREADS) {
+        int lo = 0;   // the first sequence whose units end past u
+        for (int step = PLAN_THREADS / 2; step; step >>= 1)
+          if (ends[lo + step - 1] <= u) lo += step;
+        const AttnSeq q = seqs[lo];
+        const AttnEntry e = attn_unit(q, (u - (ends[lo] - (q.nq + a.tpu - 1) / a.tpu)) * a.tpu, a.tpu, a.window);
+        f(e, e.nb);
       }
     }
   };
+  if (a.n_seqs <= PLAN_THREADS) load(0);
   unsigned long long sum = 0;
   int mx = 0;
   each([&](const AttnEntry& e, int cost) {
@@ -121,8 +149,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const PlanArgs a) {
       a.splits[i] = AttnSplit{e.q0, e.ntok, x.slot, n};
     }
     for (int i = 0; i < n; i++, at++) {
-      x.kb0 = e.kb0 + (int)((long long)cost * i / n);
-      x.kb1 = e.kb0 + (int)((long long)cost * (i + 1) / n);
+      const int b0 = (int)((long long)cost * i / n), b1 = (int)((long long)cost * (i + 1) / n);
+      x.ks = e.ks + b0 * AT_KEYS;
+      x.nb = b1 - b0;
       if (at < a.max_entries) a.entries[at] = x;
       x.slot += n > 1;
     }
@@ -146,46 +175,19 @@ struct CombineArgs {
   int G, KH, hd, tpt;
 };
 
-// A warp per (split unit, key head, tile row): the pieces' accumulators
-// weighted by 2^(c m - M), M the largest of the c m and the sink's.
+// A warp per (split unit, key head, tile row).
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
   pdl_wait();
-  const int lane = threadIdx.x & 31, n = a.head->n_splits * a.KH * 2 * AT_ROWS;
+  const int n = a.head->n_splits * a.KH * 2 * AT_ROWS;
   for (int i = blockIdx.x * 8 + (threadIdx.x >> 5); i < n; i += gridDim.x * 8) {
     const int row = i % AT_ROWS, t = i / AT_ROWS % 2, kh = i / (2 * AT_ROWS) % a.KH;
     const AttnSplit s = a.splits[i / (2 * AT_ROWS * a.KH)];
     const int tok = row / a.G, g = row - tok * a.G, tt = t * a.tpt + tok, h = kh * a.G + g;
     if (tok >= a.tpt || tt >= s.ntok) continue;
     auto at = [&](int p) { return ((size_t)(s.slot + p) * a.KH + kh) * (2 * AT_ROWS) + t * AT_ROWS + row; };
-    float M = -INFINITY;
-    for (int p = 0; p < s.n; p++) M = fmaxf(M, a.pml[at(p)].x);
-    float l = 0.f;
-    if (a.sinks && M != -INFINITY) {
-      const float sk = a.sinks[h] * LOG2E;
-      M = fmaxf(M, sk);
-      l = at_exp2(sk - M);
-    }
-    constexpr int E = HD / 32;
-    float o[E] = {};
-    for (int p = 0; p < s.n; p++) {
-      const float2 ml = a.pml[at(p)];
-      if (ml.y == 0.f) continue;   // a piece without keys for this row
-      const float f = at_exp2(ml.x - M);
-      l = fmaf(ml.y, f, l);
-      const float* po = a.po + at(p) * HD + lane * E;
-      if (E == 4) {
-        const float4 x = *reinterpret_cast<const float4*>(po);
-        o[0] = fmaf(x.x, f, o[0]), o[1] = fmaf(x.y, f, o[1]), o[E - 2] = fmaf(x.z, f, o[E - 2]), o[E - 1] = fmaf(x.w, f, o[E - 1]);
-      } else {
-        const float2 x = *reinterpret_cast<const float2*>(po);
-        o[0] = fmaf(x.x, f, o[0]), o[1] = fmaf(x.y, f, o[1]);
-      }
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    T* out = (T*)a.out + (s.q0 + tt) * a.so[0] + h * a.so[1] + lane * E;
-    if (lane * E < a.hd)
-      for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(out + e) = at_pack<T>(o[e] * inv, o[e + 1] * inv);
+    const float2 fin = join_scale(s.n, a.pml, a.sinks ? a.sinks[h] * LOG2E : -INFINITY, at);
+    join_row<T, HD>(s.n, a.pml, a.po, fin, at, (T*)a.out + (s.q0 + tt) * a.so[0] + h * a.so[1], a.hd);
   }
 }
 

@@ -16,14 +16,17 @@
 //   prefix  attn_tc_kernel (tg_attn_tc.cuh): the batch's queries of a key head
 //           are the rows of 128-row tiles, so the prefix is read once per tile
 //           pair and not once per sequence; pieces of its keys.
-//   own     own_kernel: each sequence's keys are read once, in pieces; bound
-//           by HBM.  G query heads share a key head, so S^T = K Q^T and
-//           O^T += V^T P^T with the heads as the 8 columns of mma.m16n8k16
-//           (few rows: the tensor memory path has 128).
+//   own     own_kernel: each sequence's keys are read once; bound by HBM.  G
+//           query heads share a key head, so S^T = K Q^T and O^T += V^T P^T
+//           with the heads as the 8 columns of mma.m16n8k16 (few rows: the
+//           tensor memory path has 128).  All sequences' keys in a row are cut
+//           evenly among the CTAs, so lengths may differ at will.
 //   join    join_kernel: weighted sum of the pieces, the sinks, the outputs;
 //           weights from the scores that own_kernel left, once the whole
 //           softmax's maximum and sum are known (their order is fixed: results
 //           are the same each time).
+// The prefix is bound by the tensor cores and the own keys by HBM, so the two
+// kernels run side by side, each on its share of the SMs.
 #include <algorithm>
 
 #include "../../include/tinygiant.h"
@@ -39,11 +42,12 @@ constexpr int OWN_THREADS = (OWN_WARPS + 1) * 32;
 struct OwnArgs {
   const void* q;
   const int* lens;
-  float* po;          // [(b KH + kh) nso + piece][G][HD]
-  float2* pml;        // [(b KH + kh) nso + piece][G]: (c m, l)
+  float* po;          // [segment][8 NT][HD], see OwnWalk
+  float2* pml;        // [segment][8 NT]: (c m, l)
+  int* starts;        // [batch + 1]: stages of a key head before each sequence
   float* scores;      // [b KH + kh][max_len][gp] c s, or null
   long long sq[2];
-  int B, KH, G, gp, hd, max_len, window, chunk, nso, ngc;   // ngc: groups of 8 NT heads per key head
+  int B, KH, G, gp, hd, max_len, window, ngc;   // ngc: groups of 8 NT heads per key head
   float c;
   DevStatus* st;
 };
@@ -95,19 +99,62 @@ __device__ __forceinline__ void mma16816<__half>(float (&d)[4], const uint32_t (
 struct OwnShared {
   uint64_t full[6], empty[6];
   float2 ml[OWN_WARPS][8];   // each warp's (m, l) of 8 heads
+  int sums[OWN_WARPS];
+  int b0, before;            // the CTA's first sequence, and the stages of a key head before it
   int abort;
 };
 
-// The keys [lo, hi) of piece `pc` of a sequence with len own keys.
-__device__ __forceinline__ void own_range(const OwnArgs& a, int len, int pc, int& lo, int& hi) {
-  lo = max(pc * a.chunk, a.window > 0 ? max(0, len - a.window) : 0);
-  hi = min((pc + 1) * a.chunk, len);
+// A sequence's own keys [lo, len) and the stages of 128 that they take.
+__device__ __forceinline__ int own_len(const int* lens, int b, int max_len) { return min(max(lens[b], 0), max_len); }
+__device__ __forceinline__ int own_first(int len, int window) { return window > 0 ? max(0, len - window) & ~15 : 0; }
+__device__ __forceinline__ int own_stages(int len, int window) {
+  return (len - own_first(len, window) + OWN_KEYS - 1) / OWN_KEYS;
 }
+// The CTA of n that stage x of `total` falls to: CTA i has the stages
+// [i total / n, (i + 1) total / n).
+__device__ __forceinline__ int own_cta(long long x, long long total, int n) { return (int)(((x + 1) * n - 1) / total); }
 
-// Persistent, one CTA per SM; item = ((b KH + kh) ngc + head group) nso +
-// piece.  Warp 8 loads stages ahead, across items; each of warps 0-7 takes 16
-// keys of a stage with a running maximum of its own, and the warps' partial
-// results join in shared memory at the end of the item.
+// The stages of a CTA, sequence by sequence, key head by key head (and group
+// of heads), as segments: consecutive stages of one (sequence, head).  A
+// segment's place among the partial results is its CTA's number plus the
+// number of its (sequence, head): two segments differ in one of them at least,
+// and neither ever falls.
+struct OwnWalk {
+  long long x, x1;
+  int b, hk, j, len, lo, n, j1;   // sequence, head, first stage; own keys, first key, stages; last stage + 1
+  __device__ void seq(const OwnArgs& a) {
+    len = own_len(a.lens, b, a.max_len);
+    lo = own_first(len, a.window);
+    n = own_stages(len, a.window);
+  }
+  __device__ void start(const OwnArgs& a, int b0, int before, long long x0, long long end) {
+    x = x0, x1 = end, b = b0;
+    if (x >= x1) return;
+    seq(a);
+    const long long r = x0 - (long long)before * (a.KH * a.ngc);
+    hk = (int)(r / n), j = (int)(r % n);
+    j1 = (int)min((long long)n, j + x1 - x);
+  }
+  __device__ bool more() const { return x < x1; }
+  __device__ void next(const OwnArgs& a) {
+    x += j1 - j;
+    if (x >= x1) return;
+    j = 0;
+    if (++hk == a.KH * a.ngc) {
+      hk = 0;
+      do {
+        b++;
+        seq(a);
+      } while (n == 0);   // x < x1: there is another sequence with keys
+    }
+    j1 = (int)min((long long)n, x1 - x);
+  }
+};
+
+// Persistent, one CTA per SM of its share.  Warp 8 loads stages ahead, across
+// segments; each of warps 0-7 takes 16 keys of a stage with a running maximum
+// of its own, and the warps' partial results join in shared memory at the end
+// of a segment.
 template <typename T, int HD, int NT>
 __global__ void __launch_bounds__(OWN_THREADS, 1) own_kernel(const __grid_constant__ CUtensorMap kmap,
                                                              const __grid_constant__ CUtensorMap vmap, const OwnArgs a) {
@@ -126,36 +173,78 @@ __global__ void __launch_bounds__(OWN_THREADS, 1) own_kernel(const __grid_consta
     sh.abort = 0;
     fence_mbar_init();
   }
-  __syncthreads();
   pdl_wait();
   pdl_trigger();
+  // The whole number of stages, then where this CTA's begin.  A thread has
+  // one of 256 sequences at a time; up to 256 stay in registers.
+  const int HK = a.KH * a.ngc;
+  int mine = 0, before = 0, round = 0;   // this thread's sequence: stages, those before it
+  auto scan = [&](int b0) {
+    const int b = b0 + tid;
+    mine = tid < OWN_WARPS * 32 && b < a.B ? own_stages(own_len(a.lens, b, a.max_len), a.window) : 0;
+    int y = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int z = __shfl_up_sync(~0u, y, o);
+      if (lane >= o) y += z;
+    }
+    __syncthreads();
+    if (lane == 31 && wid < OWN_WARPS) sh.sums[wid] = y;
+    __syncthreads();
+    before = round + y - mine;
+    for (int i = 0; i < OWN_WARPS; i++) {
+      if (i < wid) before += sh.sums[i];
+      round += sh.sums[i];
+    }
+  };
+  for (int b0 = 0; b0 < a.B; b0 += OWN_WARPS * 32) scan(b0);
+  const long long total = (long long)round * HK;
+  const long long ctas = min((long long)gridDim.x, total);   // those that get any: every CTA in between has a segment
+  const long long x0 = blockIdx.x < ctas ? total * blockIdx.x / ctas : total;
+  const long long x1 = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : total;
+  auto note = [&](int b0) {
+    const int b = b0 + tid;
+    if (tid >= OWN_WARPS * 32 || b >= a.B) return;
+    if ((long long)before * HK <= x0 && x0 < (long long)(before + mine) * HK) sh.b0 = b, sh.before = before;
+    if (blockIdx.x == 0) {
+      a.starts[b] = before;
+      if (b == a.B - 1) a.starts[a.B] = before + mine;
+    }
+  };
+  if (a.B <= OWN_WARPS * 32) {
+    note(0);
+  } else {
+    round = 0;
+    for (int b0 = 0; b0 < a.B; b0 += OWN_WARPS * 32) {
+      scan(b0);
+      note(b0);
+    }
+  }
+  __syncthreads();
   auto fail = [&](int site, int u) {
     if (!*abort) set_error(a.st, ERR_WAIT_TIMEOUT, site, blockIdx.x, u);
     *abort = 1;
   };
-  const int items = a.B * a.KH * a.ngc * a.nso;
+  OwnWalk wk;
   int n = 0;   // stages so far
 
   if (wid == OWN_WARPS) {
     bool ok = true;
-    for (int it = blockIdx.x; it < items && ok; it += gridDim.x) {
-      const int pc = it % a.nso, bk = it / (a.nso * a.ngc), kh = bk % a.KH, b = bk / a.KH;
-      int lo, hi;
-      own_range(a, min(max(a.lens[b], 0), a.max_len), pc, lo, hi);
-      for (int r0 = lo & ~15; r0 < hi; r0 += OWN_KEYS, n++) {
-        const int s = n % S::STAGES;
+    for (wk.start(a, sh.b0, sh.before, x0, x1); wk.more() && ok; wk.next(a)) {
+      const int kh = wk.hk / a.ngc;
+      for (int j = wk.j; j < wk.j1; j++, n++) {
+        const int s = n % S::STAGES, r0 = wk.lo + j * OWN_KEYS;
         if (n >= S::STAGES && !at_wait(&sh.empty[s], (n / S::STAGES - 1) & 1, abort)) {
-          if (lane == 0) fail(400, it);
+          if (lane == 0) fail(400, n);
           ok = false;
           break;
         }
-        const int boxes = min(OWN_KEYS, hi - r0 + OWN_BOX - 1) / OWN_BOX;   // of each column half of K and V
+        const int boxes = min(OWN_KEYS, wk.len - r0 + OWN_BOX - 1) / OWN_BOX;   // of each column half of K and V
         if (lane == 0) mbar_arrive_expect_tx(&sh.full[s], boxes * 2 * (HD / 64) * OWN_BOX * 128);
         __syncwarp();
         if (lane < boxes * 2 * (HD / 64)) {
           const int bx = lane % boxes, h = lane / boxes;   // h: K halves, then V halves
           tma_load_4d(stages + s * S::STAGE + h * S::HALF + bx * OWN_BOX * 128, h < HD / 64 ? &kmap : &vmap, 64 * (h % (HD / 64)),
-                      r0 + bx * OWN_BOX, kh, b, &sh.full[s]);
+                      r0 + bx * OWN_BOX, kh, wk.b, &sh.full[s]);
         }
       }
     }
@@ -168,11 +257,10 @@ __global__ void __launch_bounds__(OWN_THREADS, 1) own_kernel(const __grid_consta
   // this lane's ldmatrix rows within its 16 keys and its 16-byte column
   const int krow = wid * 16 + (lane & 15), kcol = lane >> 4;                                  // K: rows, then k halves
   const int vrow = wid * 16 + (lane & 7) + ((lane >> 4) << 3), vcol = (lane >> 3) & 1;        // V: d halves, then rows
-  for (int it = blockIdx.x; it < items; it += gridDim.x) {
-    const int pc = it % a.nso, gc = it / a.nso % a.ngc, bk = it / (a.nso * a.ngc), kh = bk % a.KH, b = bk / a.KH;
-    int lo, hi;
-    own_range(a, min(max(a.lens[b], 0), a.max_len), pc, lo, hi);
-    if (lo >= hi) continue;
+  for (wk.start(a, sh.b0, sh.before, x0, x1); wk.more(); wk.next(a)) {
+    const int b = wk.b, kh = wk.hk / a.ngc, gc = wk.hk % a.ngc, bk = b * a.KH + kh;
+    const int lo = a.window > 0 ? max(0, wk.len - a.window) : 0, hi = wk.len;
+    const size_t seg = (size_t)blockIdx.x + (size_t)b * HK + wk.hk;
     // Q^T as B fragments: heads are columns, absent ones and dimensions zero
     uint32_t qf[NT][HD / 16][2];
 #pragma unroll
@@ -195,10 +283,10 @@ __global__ void __launch_bounds__(OWN_THREADS, 1) own_kernel(const __grid_consta
 #pragma unroll
       for (int k = 0; k < HD / 16; k++) o[t][k][0] = o[t][k][1] = o[t][k][2] = o[t][k][3] = 0.f;
     }
-    for (int r0 = lo & ~15; r0 < hi; r0 += OWN_KEYS, n++) {
-      const int s = n % S::STAGES;
+    for (int j = wk.j; j < wk.j1; j++, n++) {
+      const int s = n % S::STAGES, r0 = wk.lo + j * OWN_KEYS;
       if (!at_wait(&sh.full[s], (n / S::STAGES) & 1, abort)) {
-        if (lane == 0) fail(401, it);
+        if (lane == 0) fail(401, n);
         break;   // on to the barriers below: every wait from here on fails at once
       }
       const int k0 = r0 + wid * 16;   // this warp's keys k0 .. k0 + 15
@@ -295,7 +383,6 @@ __global__ void __launch_bounds__(OWN_THREADS, 1) own_kernel(const __grid_consta
 #pragma unroll
         for (int z = 0; z < 4; z++) red[(wid * 8 + cc * 2 + (z & 1)) * HD + k * 16 + g + (z >> 1) * 8] = o[t][k][z];
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      const int h0 = (gc * NT + t) * 8;
       for (int i = tid; i < 8 * HD; i += OWN_WARPS * 32) {
         const int h = i / HD, d = i % HD;
         float M = -INFINITY, L = 0.f, v = 0.f;
@@ -309,11 +396,9 @@ __global__ void __launch_bounds__(OWN_THREADS, 1) own_kernel(const __grid_consta
           L = fmaf(ml.y, f, L);
           v = fmaf(red[(w * 8 + h) * HD + d], f, v);
         }
-        if (h0 + h < a.G) {
-          const size_t at = ((size_t)bk * a.nso + pc) * a.G + h0 + h;
-          a.po[at * HD + d] = v;
-          if (d == 0) a.pml[at] = make_float2(M, L);
-        }
+        const size_t at = seg * (8 * NT) + t * 8 + h;
+        a.po[at * HD + d] = v;
+        if (d == 0) a.pml[at] = make_float2(M, L);
       }
       asm volatile("bar.sync 1, 256;" ::: "memory");
     }
@@ -321,77 +406,56 @@ __global__ void __launch_bounds__(OWN_THREADS, 1) own_kernel(const __grid_consta
 }
 
 struct JoinArgs {
-  const int* lens;
+  const int *lens, *starts;
   const float* sinks;
   float* weights;
-  const float *ppo, *opo, *scores;
-  const float2 *ppml, *opml;
+  const float *po, *scores;
+  const float2* pml;
   void* out;
-  long long so[2], sw[2];
-  int B, KH, G, gp, hd, tpt, P, nsp, nso, chunk, max_len, window;
+  long long so[2], sw[2], own_row;   // own_row: the own segments' first row in pml and po
+  int B, KH, G, gp, hd, tpt, nsp, max_len, window, ngc, nt, own_ctas;
 };
 
 constexpr int JOIN_THREADS = 256;
-constexpr int JOIN_KEYS = 2048;   // own positions whose weights one block adds
+constexpr int JOIN_KEYS = 512;   // own positions whose weights one block adds
 
-// Block (b KH + kh, part): the (maximum, 1 / sum) of each head, then in part 0
-// the outputs and in every part the weights of JOIN_KEYS positions.
+// Block (b KH + kh, part): part 0 the outputs, a warp per head; the others
+// the weights of JOIN_KEYS own positions each.
 template <typename T, int HD>
 __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
-  __shared__ float2 fin[128];   // per head: M, 1 / L
+  __shared__ float2 fin[AT_ROWS];   // per head: M, 1 / the sum
   pdl_wait();
   const int bk = blockIdx.x, kh = bk % a.KH, b = bk / a.KH, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-  const int len = min(max(a.lens[b], 0), a.max_len), lo = a.window > 0 ? max(0, len - a.window) : 0;
-  const int p0 = lo / a.chunk, p1 = (len + a.chunk - 1) / a.chunk;   // own pieces with keys
-  const int j0 = blockIdx.y * JOIN_KEYS;
-  if (blockIdx.y > 0 && j0 >= len) return;
+  const int len = own_len(a.lens, b, a.max_len), lo = a.window > 0 ? max(0, len - a.window) : 0;
+  const int j0 = ((int)blockIdx.y - 1) * JOIN_KEYS;
+  if (blockIdx.y > 0 && (j0 >= len || j0 + JOIN_KEYS <= lo)) return;
   const int ub = b / (2 * a.tpt), r = b % (2 * a.tpt), t = r / a.tpt, tok = r % a.tpt;
-  auto pat = [&](int sp, int g) { return ((size_t)(ub * a.nsp + sp) * a.KH + kh) * (2 * AT_ROWS) + t * AT_ROWS + tok * a.G + g; };
-  auto oat = [&](int pc, int g) { return ((size_t)bk * a.nso + pc) * a.G + g; };
-  for (int g = wid; g < a.G; g += JOIN_THREADS / 32) {
-    float M = -INFINITY;
-    for (int i = lane; i < a.nsp; i += 32) M = fmaxf(M, a.ppml[pat(i, g)].x);
-    for (int i = p0 + lane; i < p1; i += 32) M = fmaxf(M, a.opml[oat(i, g)].x);
-    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, o));
-    const float sk = a.sinks ? a.sinks[kh * a.G + g] * LOG2E : -INFINITY;
-    const bool any = M != -INFINITY;
-    M = fmaxf(M, sk);
-    float L = 0.f;
-    for (int i = lane; i < a.nsp; i += 32) {
-      const float2 ml = a.ppml[pat(i, g)];
-      if (ml.y != 0.f) L = fmaf(ml.y, at_exp2(ml.x - M), L);
-    }
-    for (int i = p0 + lane; i < p1; i += 32) {
-      const float2 ml = a.opml[oat(i, g)];
-      if (ml.y != 0.f) L = fmaf(ml.y, at_exp2(ml.x - M), L);
-    }
-    for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(~0u, L, o);
-    const float inv = any && L != 0.f ? 1.f / (L + at_exp2(sk - M)) : L;   // L: 0, or NaN
-    if (lane == 0) fin[g] = make_float2(M, inv);
-    if (blockIdx.y == 0) {
-      constexpr int E = HD / 32;
-      float o[E] = {};
-      auto add = [&](const float2* pml, const float* po, size_t at) {
-        const float2 ml = pml[at];
-        if (ml.y == 0.f) return;
-        const float f = at_exp2(ml.x - M);
-        const float* x = po + at * HD + lane * E;
-        if (E == 4) {
-          const float4 v = *reinterpret_cast<const float4*>(x);
-          o[0] = fmaf(v.x, f, o[0]), o[1] = fmaf(v.y, f, o[1]), o[E - 2] = fmaf(v.z, f, o[E - 2]), o[E - 1] = fmaf(v.w, f, o[E - 1]);
-        } else {
-          const float2 v = *reinterpret_cast<const float2*>(x);
-          o[0] = fmaf(v.x, f, o[0]), o[1] = fmaf(v.y, f, o[1]);
-        }
-      };
-      for (int i = 0; i < a.nsp; i++) add(a.ppml, a.ppo, pat(i, g));
-      for (int i = p0; i < p1; i++) add(a.opml, a.opo, oat(i, g));
-      T* out = (T*)a.out + b * a.so[0] + (kh * a.G + g) * a.so[1] + lane * E;
-      if (lane * E < a.hd)
-        for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(out + e) = at_pack<T>(o[e] * inv, o[e + 1] * inv);
-    }
+  const int HK = a.KH * a.ngc, n = a.own_ctas ? own_stages(len, a.window) : 0;
+  long long total = 0, first = 0;
+  int ctas = 0;
+  if (n > 0) {
+    total = (long long)a.starts[a.B] * HK;
+    first = (long long)a.starts[b] * HK;
+    ctas = (int)min((long long)a.own_ctas, total);
   }
-  if (!a.weights) return;
+  for (int g = wid; g < a.G; g += JOIN_THREADS / 32) {
+    // pieces: the prefix's, then the segments of the CTAs c0 .. c1
+    const int hk = kh * a.ngc + g / (8 * a.nt), gl = g % (8 * a.nt);
+    int c0 = 0, pieces = a.nsp;
+    if (n > 0) {
+      c0 = own_cta(first + (long long)hk * n, total, ctas);
+      pieces += own_cta(first + (long long)(hk + 1) * n - 1, total, ctas) - c0 + 1;
+    }
+    auto row = [&](int i) -> long long {
+      if (i < a.nsp) return ((long long)(ub * a.nsp + i) * a.KH + kh) * (2 * AT_ROWS) + t * AT_ROWS + tok * a.G + g;
+      return a.own_row + ((long long)b * HK + hk + c0 + i - a.nsp) * (8 * a.nt) + gl;
+    };
+    const float2 f = join_scale(pieces, a.pml, a.sinks ? a.sinks[kh * a.G + g] * LOG2E : -INFINITY, row);
+    if (lane == 0) fin[g] = f;
+    if (blockIdx.y == 0)
+      join_row<T, HD>(pieces, a.pml, a.po, f, row, (T*)a.out + b * a.so[0] + (kh * a.G + g) * a.so[1], a.hd);
+  }
+  if (blockIdx.y == 0) return;
   __syncthreads();
   float* w = a.weights + b * a.sw[0] + kh * a.sw[1];
   for (int j = max(j0, lo) + tid; j < min(len, j0 + JOIN_KEYS); j += JOIN_THREADS) {
@@ -408,40 +472,48 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
   }
 }
 
-// How the work is cut, and the workspace: prefix and own partial results, scores.
+// How the work is cut, and the workspace: prefix pieces' and own segments'
+// partial results, the sequences' first stages, scores.
 struct SharedSpace {
-  int tpt, units, nsp, chunk, nso, gp;
-  size_t ppml, ppo, opml, opo, scores, bytes = 0;
+  int tpt, units, nsp, own_ctas, gp, nt, ngc;
+  long long own_row;
+  size_t pml, po, starts, scores, bytes = 0;
   SharedSpace(int B, int P, int max_len, int H, int KH, int hd, bool weights) {
     const int G = H / KH, sms = attn_sms(), HD = hd <= 64 ? 64 : 128;
     tpt = AT_ROWS / G;
     units = (B + 2 * tpt - 1) / (2 * tpt);
-    // Prefix: as many pieces as make the longest CTA's work least, counting
-    // two blocks' time for a piece's own start and end.
+    nt = G <= 8 ? 1 : 2;
+    ngc = (G + 8 * nt - 1) / (8 * nt);
+    gp = (G + 7) / 8 * 8;
     const int blocks = (P + AT_KEYS - 1) / AT_KEYS;
+    const long long HK = (long long)KH * ngc, stages = (long long)B * HK * ((max_len + OWN_KEYS - 1) / OWN_KEYS);
+    // The SMs' shares, by the time one SM would take: a block of two tiles of
+    // the prefix about 2 us at head_dim 128, a stage of own keys 0.65 us.
+    const double tp = 2.0 * units * KH * blocks, to = 0.65 * stages;
+    own_ctas = 0;
+    if (max_len > 0) {
+      own_ctas = blocks ? std::max(1, std::min(sms - 1, (int)(sms * to / (to + tp) + 0.5))) : sms;
+      own_ctas = (int)std::min((long long)own_ctas, stages);
+    }
+    // Prefix: as many pieces as make the last one end earliest, counting two
+    // blocks' time for a piece's own start and end.
     nsp = 0;
     long long best = 0;
     for (int n = 1; n <= std::min(blocks, 64); n++) {
       const long long rounds = ((long long)units * KH * n + sms - 1) / sms, cost = rounds * ((blocks + n - 1) / n + 2);
       if (!nsp || cost < best) nsp = n, best = cost;
     }
-    // Own keys: pieces of at least two stages, four for each SM if there are
-    // that many keys.
-    const long long heads = (long long)B * KH, want = (4ll * sms + heads - 1) / heads;
-    chunk = std::max(2 * OWN_KEYS, (int)(((max_len + want - 1) / want + OWN_KEYS - 1) / OWN_KEYS * OWN_KEYS));
-    nso = (max_len + chunk - 1) / chunk;
-    gp = (G + 7) / 8 * 8;
     auto take = [&](size_t n) {
       const size_t o = bytes;
       bytes = (bytes + n + 255) & ~(size_t)255;
       return o;
     };
-    const size_t pr = (size_t)units * nsp * KH * 2 * AT_ROWS, orows = (size_t)heads * nso * G;
-    ppml = take(8 * pr);
-    ppo = take(4 * pr * HD);
-    opml = take(8 * orows);
-    opo = take(4 * orows * HD);
-    scores = take(weights ? 4 * (size_t)heads * max_len * gp : 0);
+    own_row = (long long)units * nsp * KH * 2 * AT_ROWS;
+    const size_t rows = own_row + (own_ctas ? ((size_t)own_ctas + (size_t)B * HK) * 8 * nt : 0);
+    pml = take(8 * rows);
+    po = take(4 * rows * HD);
+    starts = take(own_ctas ? 4 * ((size_t)B + 1) : 0);
+    scores = take(weights ? 4 * (size_t)B * KH * max_len * gp : 0);
   }
 };
 
@@ -459,23 +531,25 @@ static cudaError_t launch_own(const CUtensorMap& k, const CUtensorMap& v, const 
   return launch_pdl(own_kernel<T, HD, NT>, dim3(grid), OWN_THREADS, smem, s, k, v, a);
 }
 
+// The own keys' kernel goes first and lets the prefix start beside it at once;
+// the prefix's CTAs, one for each piece, take the SMs that are left, and those
+// of the own keys once they are done.  The last of them waits for the own
+// keys' kernel, so that the join, which waits for the prefix, follows both.
 template <typename T, int HD>
-static cudaError_t run_shared(const CUtensorMap* m, const AttnTcArgs& ta, int prefix_grid, OwnArgs oa, JoinArgs ja, cudaStream_t s) {
+static cudaError_t run_shared(const CUtensorMap* m, AttnTcArgs ta, int pieces, const OwnArgs& oa, const JoinArgs& ja, cudaStream_t s) {
   cudaError_t e = cudaSuccess;
-  if (prefix_grid > 0) {
-    e = launch_attn_tc<T, HD, true>(m[0], m[1], m[2], ta, prefix_grid, s);
+  if (ja.own_ctas > 0) {
+    e = ja.nt == 1 ? launch_own<T, HD, 1>(m[3], m[4], oa, ja.own_ctas, s) : launch_own<T, HD, 2>(m[3], m[4], oa, ja.own_ctas, s);
     count_launches(1);
   }
-  if (e == cudaSuccess && oa.nso > 0) {
-    const int nt = oa.G <= 8 ? 1 : 2;
-    oa.ngc = (oa.G + 8 * nt - 1) / (8 * nt);
-    const int grid = (int)std::min((long long)attn_sms(), (long long)oa.B * oa.KH * oa.ngc * oa.nso);
-    e = nt == 1 ? launch_own<T, HD, 1>(m[3], m[4], oa, grid, s) : launch_own<T, HD, 2>(m[3], m[4], oa, grid, s);
+  ta.beside = ja.own_ctas > 0;
+  if (e == cudaSuccess && pieces > 0) {
+    e = launch_attn_tc<T, HD, true>(m[0], m[1], m[2], ta, pieces, s);
     count_launches(1);
   }
   if (e == cudaSuccess) {
-    const int parts = ja.weights ? std::max(1, (oa.max_len + JOIN_KEYS - 1) / JOIN_KEYS) : 1;
-    e = launch_pdl(join_kernel<T, HD>, dim3(oa.B * oa.KH, parts), JOIN_THREADS, 0, s, ja);
+    const dim3 grid(ja.B * ja.KH, 1 + (ja.weights ? (ja.max_len + JOIN_KEYS - 1) / JOIN_KEYS : 0));
+    e = launch_pdl(join_kernel<T, HD>, grid, JOIN_THREADS, 0, s, ja);
     count_launches(1);
   }
   return e;
@@ -521,7 +595,7 @@ extern "C" int tg_attention_shared(int dtype, const void* q, const void* prefix_
   if (sinks) c.ptr(sinks, 4, "sinks");
   if (weights) c.ptr(weights, 4, "weights");
   const SharedSpace sp(batch, prefix_len, max_len, n_heads, n_kv_heads, head_dim, weights != nullptr);
-  c.need((long long)batch * n_kv_heads * std::max(1, sp.nso) * 16 < 0x7fffffff, "too many positions");
+  c.need((long long)sp.units * sp.nsp * n_kv_heads < 0x7fffffff && max_len / JOIN_KEYS < 65535, "too many positions");
   c.need(workspace_bytes >= sp.bytes, "the workspace is smaller than tg_attention_shared_workspace says");
   if (sp.bytes > 0) c.ptr(workspace, 256, "workspace");
   if (c.rc) return c.rc;
@@ -530,22 +604,25 @@ extern "C" int tg_attention_shared(int dtype, const void* q, const void* prefix_
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   AttnTcArgs a{};
   a.out = out;
-  a.po = (float*)(ws + sp.ppo);
-  a.pml = (float2*)(ws + sp.ppml);
+  a.po = (float*)(ws + sp.po);
+  a.pml = (float2*)(ws + sp.pml);
   a.lens = lens;
   a.G = G, a.KH = n_kv_heads, a.hd = head_dim, a.tpt = sp.tpt, a.window = window, a.total_k = prefix_len;
   a.P = prefix_len, a.B = batch, a.nsp = sp.nsp, a.max_len = max_len;
   a.c = scale * LOG2E;
   a.st = attn_status();
-  OwnArgs o{q, lens, (float*)(ws + sp.opo), (float2*)(ws + sp.opml), weights ? (float*)(ws + sp.scores) : nullptr, {t[0], t[1]},
-            batch, n_kv_heads, G, sp.gp, head_dim, max_len, window, sp.chunk, sp.nso, 1, a.c, a.st};
-  JoinArgs j{lens, sinks, weights, a.po, o.po, o.scores, a.pml, o.pml, out, {t[12], t[13]}, {weights ? strides[14] : 0, weights ? strides[15] : 0},
-             batch, n_kv_heads, G, sp.gp, head_dim, sp.tpt, prefix_len, sp.nsp, sp.nso, sp.chunk, max_len, window};
+  int* starts = (int*)(ws + sp.starts);
+  OwnArgs o{q, lens, a.po + sp.own_row * (head_dim <= 64 ? 64 : 128), a.pml + sp.own_row, starts,
+            weights ? (float*)(ws + sp.scores) : nullptr, {t[0], t[1]}, batch, n_kv_heads, G, sp.gp, head_dim, max_len, window, sp.ngc,
+            a.c, a.st};
+  JoinArgs j{lens, starts, sinks, weights, a.po, o.scores, a.pml, out, {t[12], t[13]},
+             {weights ? strides[14] : 0, weights ? strides[15] : 0}, sp.own_row, batch, n_kv_heads, G, sp.gp, head_dim, sp.tpt, sp.nsp,
+             max_len, window, sp.ngc, sp.nt, sp.own_ctas};
   CUtensorMap m[5];
   bool maps = true;
-  int grid = 0;
+  int pieces = 0;
   if (prefix_len > 0) {
-    grid = (int)std::min((long long)attn_sms(), (long long)sp.units * sp.nsp * n_kv_heads);
+    pieces = sp.units * sp.nsp * n_kv_heads;
     maps = attn_q_map(&m[0], dtype, q, head_dim, n_heads, batch, t[0], t[1], G, sp.tpt) &&
            attn_kv_map(&m[1], dtype, prefix_k, q, head_dim, n_kv_heads, prefix_len, t[3], t[2]) &&
            attn_kv_map(&m[2], dtype, prefix_v, q, head_dim, n_kv_heads, prefix_len, t[5], t[4]);
@@ -557,6 +634,6 @@ extern "C" int tg_attention_shared(int dtype, const void* q, const void* prefix_
   if (c.rc) return c.rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf = dtype == ATTN_BF16, small = head_dim <= 64;
-  return c.done(bf ? (small ? run_shared<__nv_bfloat16, 64>(m, a, grid, o, j, s) : run_shared<__nv_bfloat16, 128>(m, a, grid, o, j, s))
-                   : (small ? run_shared<__half, 64>(m, a, grid, o, j, s) : run_shared<__half, 128>(m, a, grid, o, j, s)));
+  return c.done(bf ? (small ? run_shared<__nv_bfloat16, 64>(m, a, pieces, o, j, s) : run_shared<__nv_bfloat16, 128>(m, a, pieces, o, j, s))
+                   : (small ? run_shared<__half, 64>(m, a, pieces, o, j, s) : run_shared<__half, 128>(m, a, pieces, o, j, s)));
 }

@@ -18,14 +18,18 @@
 // (token, query head of the group) pairs, token-major, so a group of G heads
 // fills a tile with 128 / G tokens: K and V tiles are used by the whole group,
 // short sequences fill tiles, and the masked corner of the causal diagonal is
-// a few tokens wide.  Its keys are the blocks [kb0, kb1).
+// a few tokens wide.  Its keys are nb blocks from key ks on.
 //
-// Warps: 0-3 and 4-7 the softmax of tile 0 and 1 (a thread per row), 8 the TMA
-// loads, 9 the MMAs.  Tensor memory: S (128 columns of fp32) and O per tile;
-// the 16-bit P overwrites S.  While one tile's softmax runs, the tensor cores
-// work on the other tile: P V of its block, then S of its next block.
+// Warps: 0-7 and 8-15 the softmax of tile 0 and 1, two threads per row with 64
+// of a block's keys each, who exchange their maxima (with one thread per row
+// and 128 keys in registers a warp's own latencies bound the kernel: 490 us
+// against the 8,192-token figure below); 16 the TMA loads, 17 the S products,
+// 18 the P V.  Tensor memory (512 columns): O of both tiles, the 16-bit P of
+// both, and S, one buffer of 128 columns for both tiles at head_dim 128, one
+// for each at 64.  A softmax warp takes its S into registers at once and frees
+// the buffer, so the next S is computed while it works on its exponentials.
 // Persistent CTAs, one per SM; units come from an atomic counter, longest
-// first, so loads and the first S of the next unit overlap the last epilogue.
+// first.
 // Every wait is bounded; a role that gives up records the error and the others
 // stop waiting.
 #pragma once
@@ -41,15 +45,18 @@ namespace tg {
 
 constexpr int AT_ROWS = 128;       // query rows per tile (MMA M)
 constexpr int AT_KEYS = 128;       // keys per block (MMA N of S, K of P V)
-constexpr int AT_THREADS = 384;   // 12 warps, the last two idle: registers move between whole warpgroups
+#ifndef NH_OF
+#define NH_OF(HD) 1
+#endif
 constexpr int AT_NPOS = 0x3fffffff;
+constexpr int AT_UNITS = 4;        // units announced ahead
 
 // One piece of work of every key head.
 struct __align__(16) AttnEntry {
   int q0, ntok;   // first query row (token) and tokens, at most 2 * (128 / G)
   int p0;         // position of the first token among its sequence's keys
   int k0, nk;     // the sequence's first key row and its keys
-  int kb0, kb1;   // key blocks of this piece
+  int ks, nb;     // this piece's first key and blocks of keys
   int slot;       // -1: writes the outputs; else the piece's place among the partial results
 };
 
@@ -83,8 +90,8 @@ __device__ __forceinline__ AttnEntry attn_unit(const AttnSeq& s, int t0, int tpu
   e.k0 = s.k0;
   e.nk = s.nk;
   const int hi = e.p0 + e.ntok, lo = window > 0 ? max(0, e.p0 + 1 - window) : 0;
-  e.kb0 = lo / AT_KEYS;
-  e.kb1 = hi > 0 ? (hi + AT_KEYS - 1) / AT_KEYS : e.kb0;
+  e.ks = lo;
+  e.nb = hi > lo ? (hi - lo + AT_KEYS - 1) / AT_KEYS : 0;
   e.slot = -1;
   return e;
 }
@@ -103,6 +110,7 @@ struct AttnTcArgs {
   int G, KH, hd, tpt, window;
   int total_k;                // rows of k and v
   int P, B, nsp, max_len;     // shared: prefix keys, sequences, pieces per unit, bound of lens
+  int beside;                 // shared: launched beside a kernel that it does not wait for
   float c;                    // scale log2(e)
   DevStatus* st;
 };
@@ -150,12 +158,10 @@ __device__ __forceinline__ void at_ld32(uint32_t taddr, uint32_t* r) {
       : AT_R4(r, 0), AT_R4(r, 4), AT_R4(r, 8), AT_R4(r, 12), AT_R4(r, 16), AT_R4(r, 20), AT_R4(r, 24), AT_R4(r, 28)
       : "r"(taddr));
 }
-__device__ __forceinline__ void at_st32(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::AT_W4(r, 0),
-      AT_W4(r, 4), AT_W4(r, 8), AT_W4(r, 12), AT_W4(r, 16), AT_W4(r, 20), AT_W4(r, 24), AT_W4(r, 28), "r"(taddr)
-      : "memory");
+__device__ __forceinline__ void at_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : AT_R4(r, 0), AT_R4(r, 4), AT_R4(r, 8), AT_R4(r, 12)
+               : "r"(taddr));
 }
 __device__ __forceinline__ void at_st16(uint32_t taddr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::AT_W4(r, 0),
@@ -174,10 +180,21 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
                : "memory");
 }
 
+// The thread's number, read anew: nothing computed from it stays in registers.
+__device__ __forceinline__ int at_tid() {
+  int x;
+  asm volatile("mov.u32 %0, %%tid.x;" : "=r"(x));
+  return x;
+}
 __device__ __forceinline__ float at_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ __forceinline__ float at_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 template <typename T>
 __device__ __forceinline__ uint32_t at_pack(float lo, float hi);
@@ -210,17 +227,54 @@ __device__ __forceinline__ float2 at_add2(float2 a, float2 b) {
   return d;
 }
 
+// 2^x of a pair on the FMA units, x >= -126 (less counts as that): x = n + f
+// with f in [-1/2, 1/2], 2^f by the degree-4 polynomial of least relative
+// error there (2.6e-6, fitted by reweighted least squares), n added to the
+// exponent.
+__device__ __forceinline__ float2 at_exp2_poly(float2 x) {
+  const float2 magic = make_float2(12582912.f, 12582912.f), minus = make_float2(-12582912.f, -12582912.f);   // 1.5 2^23
+  auto two = [](float v) { return make_float2(v, v); };
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
+  const float2 t = at_add2(x, magic);
+  const float2 n = at_add2(t, minus);
+  const float2 f = at_fma2(n, two(-1.f), x);
+  float2 p = at_fma2(two(0.009570101276f), f, two(0.05591785908f));
+  p = at_fma2(p, f, two(0.2402474433f));
+  p = at_fma2(p, f, two(0.6931217909f));
+  p = at_fma2(p, f, two(0.9999992847f));
+  p.x = __int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23));
+  p.y = __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23));
+  return p;
+}
+
 template <int HD>
 struct AttnTcShape {
+  static constexpr int NH = NH_OF(HD);                    // threads of the softmax per row
+  static constexpr int SOFT = 8 * NH;                     // its warps
+  static constexpr int THREADS = (SOFT + 4) * 32;         // and those of loads and products; the last idles
+  // registers: (65,536 / THREADS) at launch, moved between whole warpgroups
+  static constexpr int R_SOFT = NH == 1 ? 216 : 104, R_REST = NH == 1 ? 72 : 64;
   static constexpr int TILE = 128 * HD * 2;               // bytes of a Q tile, a K or a V block
-  static constexpr int STAGES = HD == 128 ? 5 : 8;        // K and V blocks in flight
-  static constexpr int SMEM = 2 * TILE + STAGES * TILE + 1024;
+  // One pair of exponentials in POLY_OF goes to the FMA units: the special
+  // function unit gives 4 values a clock to each quarter of the SM, as long for
+  // a block's 128 x 128 as the tensor cores take for both its products (none:
+  // 445 us at 8,192 tokens, 1 in 8 431, 1 in 4 440; at head_dim 64, where the
+  // products are half as long, 117, 106 and 107 us at 4,096).
+  static constexpr int POLY_OF = HD == 128 ? 8 : 4;
+  static constexpr int NQ = HD == 128 ? 1 : 2;            // units whose Q is there or on its way
+  static constexpr int STAGES = HD == 64 ? 8 : NH == 1 ? 5 : 4;        // K and V blocks in flight
+  static constexpr int SMEM = (2 * NQ + STAGES) * TILE + 1024;
 };
 
+template <int NH>
 struct AttnTcShared {
-  uint64_t q_full, q_empty, kv_full[8], kv_empty[8], s_full[2], p_full[2], o_full[2], unit_full[2], unit_empty[2], aux, drain;
-  AttnEntry unit[2];
-  int unit_kh[2];             // -1: no more work
+  uint64_t q_full[2], q_empty[2], kv_full[8], kv_empty[8], s_full[2], s_loaded[2], p_full[2], p_empty[2], pair[8], unit_full[AT_UNITS],
+      unit_empty[AT_UNITS], aux, drain[2];
+  AttnEntry unit[AT_UNITS];
+  int unit_kh[AT_UNITS];      // -1: no more work
+  int4 edge[8 * NH];               // a softmax warp's lo0, hi1, lo1, hi0 (below)
+  float row[NH == 1 ? 1 : 2][2][2][NH == 1 ? 1 : AT_ROWS];   // a row's two halves' numbers: [turn][tile][half][row]
   uint32_t tmem;
   int abort;
 };
@@ -229,46 +283,52 @@ struct AttnTcShared {
 // role has.
 __device__ __forceinline__ bool at_wait(uint64_t* bar, uint32_t parity, const volatile int* abort) {
   if (mbar_try_wait(bar, parity)) return true;
-  const long long t0 = clock64();
+  const uint32_t t0 = clock();   // 32 bits: a second is half of their range
   while (!mbar_try_wait(bar, parity))
-    if (*abort || clock64() - t0 > (1ll << 31)) return false;
+    if (*abort || (uint32_t)clock() - t0 > 1u << 31) return false;
   return true;
 }
 
 template <typename T, int HD, bool SHARED>
-__global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_constant__ CUtensorMap qmap,
+__global__ void __launch_bounds__(AttnTcShape<HD>::THREADS, 1) attn_tc_kernel(const __grid_constant__ CUtensorMap qmap,
                                                                 const __grid_constant__ CUtensorMap kmap,
                                                                 const __grid_constant__ CUtensorMap vmap, const AttnTcArgs a) {
   using S = AttnTcShape<HD>;
-  constexpr int NST = S::STAGES, TILE = S::TILE;
-  constexpr int TM_O = 2 * AT_KEYS;   // tensor memory: S of tile t at 128 t, O at 256 + HD t
+  constexpr int NST = S::STAGES, TILE = S::TILE, NQ = S::NQ, NH = S::NH, HK = AT_KEYS / NH, OD = HD / NH, W0 = S::SOFT;
+  // tensor memory: S buffers of 128 columns, P of 64 for each tile, O of HD for each
+  constexpr int NS = HD == 128 ? 1 : 2, TM_P = NS * AT_KEYS, TM_O = TM_P + AT_KEYS;
   extern __shared__ uint8_t dsm[];
-  __shared__ AttnTcShared sh;
+  __shared__ AttnTcShared<S::NH> sh;
   const int tid = threadIdx.x, wid = tid >> 5, lane = tid & 31;
   uint8_t* qs = dsm + ((1024u - (smem_u32(dsm) & 1023u)) & 1023u);
-  uint8_t* kvs = qs + 2 * TILE;
+  uint8_t* kvs = qs + 2 * NQ * TILE;
   volatile int* abort = &sh.abort;
 
-  if (wid == 8) {
+  if (wid == W0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  if (tid == 288) {
-    mbar_init(&sh.q_full, 1);
-    mbar_init(&sh.q_empty, 1);
+  if (tid == W0 * 32 + 32) {
     for (int i = 0; i < NST; i++) {
       mbar_init(&sh.kv_full[i], 1);
       mbar_init(&sh.kv_empty[i], 1);
     }
     for (int i = 0; i < 2; i++) {
+      mbar_init(&sh.q_full[i], 1);
+      mbar_init(&sh.q_empty[i], 1);
       mbar_init(&sh.s_full[i], 1);
-      mbar_init(&sh.p_full[i], 4);
-      mbar_init(&sh.o_full[i], 1);
-      mbar_init(&sh.unit_full[i], 1);
-      mbar_init(&sh.unit_empty[i], 9);
+      mbar_init(&sh.s_loaded[i], W0 / 2);
+      mbar_init(&sh.p_full[i], W0 / 2);
+      mbar_init(&sh.p_empty[i], 1);
     }
+    for (int i = 0; i < AT_UNITS; i++) {
+      mbar_init(&sh.unit_full[i], 1);
+      mbar_init(&sh.unit_empty[i], W0 + 2);
+    }
+    for (int i = 0; i < 8; i++) mbar_init(&sh.pair[i], 2);
     mbar_init(&sh.aux, 1);
-    mbar_init(&sh.drain, 1);
+    mbar_init(&sh.drain[0], 1);
+    mbar_init(&sh.drain[1], 1);
     sh.abort = 0;
     fence_mbar_init();
   }
@@ -276,8 +336,12 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
   __syncthreads();
   at_fence_after();
   const uint32_t tmem = sh.tmem;
-  pdl_wait();   // the plan comes from the preceding kernel
-  pdl_trigger();
+  // The plan comes from the preceding kernel; a prefix beside the own keys'
+  // kernel depends on nothing that runs.
+  if (!SHARED || !a.beside) {
+    pdl_wait();
+    pdl_trigger();
+  }
   auto fail = [&](int site, int u) {
     if (!*abort) set_error(a.st, ERR_WAIT_TIMEOUT, site, blockIdx.x, u);
     *abort = 1;
@@ -302,22 +366,25 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
     e.q0 = i / a.nsp * tpu;
     e.ntok = min(tpu, a.B - e.q0);
     e.nk = a.P;
-    e.kb0 = (int)((long long)nblk * sp / a.nsp);
-    e.kb1 = (int)((long long)nblk * (sp + 1) / a.nsp);
+    const int b0 = (int)((long long)nblk * sp / a.nsp), b1 = (int)((long long)nblk * (sp + 1) / a.nsp);
+    e.ks = b0 * AT_KEYS;
+    e.nb = b1 - b0;
     e.slot = i;
     if (a.window > 0) {   // without the keys that no row of the unit sees
       int lo = a.P;
       for (int r = lane; r < e.ntok; r += 32) lo = min(lo, max(0, a.P + min(max(a.lens[e.q0 + r], 0), a.max_len) - a.window));
       lo = __reduce_min_sync(~0u, lo);
-      e.kb0 = lo >= a.P ? e.kb1 : min(e.kb1, max(e.kb0, lo / AT_KEYS));
+      const int skip = lo >= a.P ? e.nb : min(e.nb, max(0, (lo - e.ks) / AT_KEYS));
+      e.ks += skip * AT_KEYS;
+      e.nb -= skip;
     }
     return e;
   };
   // The next unit, as the load warp announced it; false at the end.
   int un = 0;
   auto next_unit = [&](AttnEntry& e, int& kh) -> bool {
-    const int i = un & 1;
-    if (!at_wait(&sh.unit_full[i], (un >> 1) & 1, abort)) {
+    const int i = un % AT_UNITS;
+    if (!at_wait(&sh.unit_full[i], (un / AT_UNITS) & 1, abort)) {
       fail(300, un);
       return false;
     }
@@ -326,11 +393,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
     return kh >= 0;
   };
 
-  // 168 registers a thread at launch (384 x 168 = 64,512): 216 for the eight
-  // softmax warps and 72 for the four others make the same sum.
-  if (wid >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-  if (wid == 8) {
+  if (wid >= W0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::R_REST));
+  if (wid == W0) {
     // ---- loads
     const int tpu = 2 * a.tpt;
     const bool fixed = SHARED || !a.entries;   // units dealt out in turn
@@ -355,8 +420,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
       AttnEntry e{};
       const int kh = w < n_work ? w % a.KH : -1;
       if (kh >= 0) e = unit_of(w / a.KH);
-      const int us = it & 1;
-      if (it >= 2 && !at_wait(&sh.unit_empty[us], ((it >> 1) - 1) & 1, abort)) {
+      const int us = it % AT_UNITS;
+      if (it >= AT_UNITS && !at_wait(&sh.unit_empty[us], (it / AT_UNITS - 1) & 1, abort)) {
         if (lane == 0) fail(301, it);
         break;
       }
@@ -366,21 +431,22 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
         mbar_arrive(&sh.unit_full[us]);
       }
       if (kh < 0) break;
-      if (e.kb0 >= e.kb1) continue;
+      if (e.nb <= 0) continue;
       const int ntile = e.ntok > a.tpt ? 2 : 1;
-      if (qn > 0 && !at_wait(&sh.q_empty, (qn - 1) & 1, abort)) {
+      const int qb = qn % NQ;
+      if (qn >= NQ && !at_wait(&sh.q_empty[qb], (qn / NQ - 1) & 1, abort)) {
         if (lane == 0) fail(302, it);
         break;
       }
       qn++;
       if (lane == 0) {
-        mbar_arrive_expect_tx(&sh.q_full, ntile * (HD / 64) * a.G * a.tpt * 128);
+        mbar_arrive_expect_tx(&sh.q_full[qb], ntile * (HD / 64) * a.G * a.tpt * 128);
         for (int t = 0; t < ntile; t++)
           for (int c = 0; c < HD / 64; c++)
-            tma_load_3d(qs + t * TILE + c * 16384, &qmap, 64 * c, kh * a.G, e.q0 + t * a.tpt, &sh.q_full);
+            tma_load_3d(qs + (2 * qb + t) * TILE + c * 16384, &qmap, 64 * c, kh * a.G, e.q0 + t * a.tpt, &sh.q_full[qb]);
       }
-      for (int i = 0; i < 2 * (e.kb1 - e.kb0); i++) {
-        const int s = issued % NST, row = (e.kb0 + (i >> 1)) * AT_KEYS;
+      for (int i = 0; i < 2 * e.nb; i++) {
+        const int s = issued % NST, row = e.ks + (i >> 1) * AT_KEYS;
         const bool v = i & 1;
         if (issued >= NST && !at_wait(&sh.kv_empty[s], (issued / NST - 1) & 1, abort)) {
           if (lane == 0) fail(303, it);
@@ -418,99 +484,140 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
     }
     if (*abort && lane == 0) {   // no copy of this CTA may still be in flight
       for (int i = max(0, issued - NST); i < issued; i++) mbar_wait(&sh.kv_full[i % NST], (i / NST) & 1);
-      if (qn > 0) mbar_wait(&sh.q_full, (qn - 1) & 1);
+      for (int i = max(0, qn - NQ); i < qn; i++) mbar_wait(&sh.q_full[i % NQ], (i / NQ) & 1);
     }
-  } else if (wid == 9) {
-    // ---- MMAs, issued by one thread
+  } else if (wid == W0 + 1 || wid == W0 + 2) {
+    // ---- products, each kind issued by a thread of its own: what one has to
+    // do between two products does not keep the tensor cores from the other's
     if (lane == 0) {
-      constexpr uint32_t idesc_s = idesc_f16<T>(AT_KEYS, false), idesc_o = idesc_f16<T>(HD, true);
-      const uint32_t q0 = smem_u32(qs), kv0 = smem_u32(kvs);
-      auto mma_s = [&](int t, int s) {   // S_t = Q_t K^T
-#pragma unroll
-        for (int k = 0; k < HD / 16; k++) {
-          const uint32_t o = (k / 4) * 16384 + (k % 4) * 32;
-          at_mma_ss(tmem + t * AT_KEYS, desc_kmajor(q0 + t * TILE + o), desc_kmajor(kv0 + s * TILE + o), idesc_s, k > 0);
-        }
-        at_commit(&sh.s_full[t]);
-      };
-      int kvn = 0, qn = 0, pn[2] = {0, 0};
-      bool ok = true;
+      bool ok = true, issued = false;
       auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
-        if (ok && !at_wait(bar, parity, abort)) {
+        if (!at_wait(bar, parity & 1, abort)) {
           fail(site, un);
           ok = false;
         }
         return ok;
       };
-      auto kv_wait = [&](int i, int site) { return wait(&sh.kv_full[i % NST], (i / NST) & 1, site); };
-      for (; ok; un++) {
-        AttnEntry e;
-        int kh;
-        if (!next_unit(e, kh)) break;
-        mbar_arrive(&sh.unit_empty[un & 1]);
-        const int nb = e.kb1 - e.kb0, ntile = e.ntok > a.tpt ? 2 : 1;
+      // A place in a ring and its phase, counted on without divisions.
+      struct Ring {
+        uint32_t s, ph;
+        __device__ __forceinline__ void add(uint32_t k, uint32_t n) {
+          s += k;
+          if (s >= n) s -= n, ph ^= 1;
+        }
+      };
+      Ring unit{0, 0}, qr{0, 0}, kv{wid == W0 + 1 ? 0u : 1u, 0};   // kv: K and V take turns
+      // Parities of the tiles' S (or P), a bit each (an indexed array would
+      // live in local memory).
+      uint32_t bits = 0, last = 0;
+      for (;; un++) {
+        if (!wait(&sh.unit_full[unit.s], unit.ph, 300)) break;
+        const int nb = sh.unit[unit.s].nb, ntile = sh.unit[unit.s].ntok > a.tpt ? 2 : 1;
+        if (sh.unit_kh[unit.s] < 0) break;
+        mbar_arrive(&sh.unit_empty[unit.s]);
+        unit.add(1, AT_UNITS);
         if (nb <= 0) continue;
-        if (!wait(&sh.q_full, qn & 1, 310) || !kv_wait(kvn, 311)) break;
-        qn++;
-        at_fence_after();
-        for (int t = 0; t < ntile; t++) mma_s(t, kvn % NST);
-        at_commit(&sh.kv_empty[kvn % NST]);
-        if (nb == 1) at_commit(&sh.q_empty);
-        kvn++;
-        for (int j = 0; j < nb && ok; j++) {
-          const bool more = j + 1 < nb;
-          const int vs = kvn % NST, ks = (kvn + 1) % NST;
-          if (!kv_wait(kvn, 312)) break;
-          for (int t = 0; t < ntile; t++) {
-            if (!wait(&sh.p_full[t], pn[t] & 1, 313)) break;
-            pn[t]++;
-            at_fence_after();
+        issued = true;
+        if (wid == W0 + 1) {
+          constexpr uint32_t idesc = idesc_f16<T>(AT_KEYS, false);
+          const uint64_t dq = desc_kmajor(smem_u32(qs) + qr.s * 2 * TILE), dk = desc_kmajor(smem_u32(kvs));
+          if (!wait(&sh.q_full[qr.s], qr.ph, 310)) break;
+          for (int j = 0; j < nb && ok; j++) {
+            if (!wait(&sh.kv_full[kv.s], kv.ph, 311)) break;
+            const uint64_t bk = dk + kv.s * (TILE / 16);
+            for (uint32_t t = 0; t < ntile; t++) {
+              // The buffer is free once the softmax has loaded what was in it
+              // (a barrier's phase before its first counts as complete).
+              const uint32_t was = NS == 1 ? last : t;
+              if (!wait(&sh.s_loaded[was], (bits >> was) + 1, 312)) break;
+              at_fence_after();
+              const uint64_t aq = dq + t * (TILE / 16);
 #pragma unroll
-            for (int k = 0; k < AT_KEYS / 16; k++)   // O_t += P_t V
-              at_mma_ts(tmem + TM_O + t * HD, tmem + t * AT_KEYS + k * 8, desc_mnmajor(kv0 + vs * TILE + k * 2048), idesc_o,
-                        j > 0 || k > 0);
-            if (more) {
-              if (t == 0 && !kv_wait(kvn + 1, 314)) break;
-              mma_s(t, ks);
-            } else {
-              at_commit(&sh.o_full[t]);
+              for (int k = 0; k < HD / 16; k++) {   // S_t = Q_t K^T
+                const uint32_t o = ((k / 4) * 16384 + (k % 4) * 32) / 16;
+                at_mma_ss(tmem + (NS == 1 ? 0 : t * AT_KEYS), aq + o, bk + o, idesc, k > 0);
+              }
+              at_commit(&sh.s_full[t]);
+              bits ^= 1u << t;
+              last = t;
             }
+            at_commit(&sh.kv_empty[kv.s]);
+            kv.add(2, NST);
           }
           if (!ok) break;
-          at_commit(&sh.kv_empty[vs]);
-          if (more) {
-            at_commit(&sh.kv_empty[ks]);
-            if (j + 2 == nb) at_commit(&sh.q_empty);
+          at_commit(&sh.q_empty[qr.s]);
+          qr.add(1, NQ);
+        } else {
+          constexpr uint32_t idesc = idesc_f16<T>(HD, true);
+          const uint64_t dv = desc_mnmajor(smem_u32(kvs));
+          for (int j = 0; j < nb && ok; j++) {
+            if (!wait(&sh.kv_full[kv.s], kv.ph, 313)) break;
+            const uint64_t bv = dv + kv.s * (TILE / 16);
+            for (uint32_t t = 0; t < ntile; t++) {
+              const uint32_t d = tmem + TM_O + t * HD, pa = tmem + TM_P + t * (AT_KEYS / 2), par = bits >> t;
+              if (!wait(&sh.p_full[t], par, 315)) break;
+              at_fence_after();
+#pragma unroll
+              for (int k = 0; k < AT_KEYS / 16; k++)   // O_t += P_t V
+                at_mma_ts(d, pa + k * 8, bv + k * (2048 / 16), idesc, j > 0 || k > 0);
+              at_commit(&sh.p_empty[t]);
+              bits ^= 1u << t;
+            }
+            at_commit(&sh.kv_empty[kv.s]);
+            kv.add(2, NST);
           }
-          kvn += more ? 2 : 1;
+          if (!ok) break;
         }
       }
-      if (*abort) {   // no MMA of this CTA may still be in flight
-        at_commit(&sh.drain);
-        mbar_wait(&sh.drain, 0);
+      if (*abort && issued) {   // no MMA of this CTA may still be in flight
+        at_commit(&sh.drain[wid - W0 - 1]);
+        mbar_wait(&sh.drain[wid - W0 - 1], 0);
       }
     }
     __syncwarp();
   }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    // ---- softmax of tile t, a thread per row
-    const int t = wid >> 2, row = tid & 127;
-    const int tok = row / a.G, g = row - tok * a.G;
-    const uint32_t lanes = (uint32_t)(wid & 3) << 21;   // this warp's 32 lanes of tensor memory
-    const uint32_t ts = tmem + t * AT_KEYS + lanes, to = tmem + TM_O + t * HD + lanes;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::R_SOFT));
+    // ---- softmax of tile t: half `hf` of a row's keys and of its outputs.
+    // What a block does not need is kept in shared memory and computed again
+    // from the thread's number: a spilled register costs more, since next to
+    // 200 KB of shared memory there is hardly an L1 for it.
+    const int t = wid / (4 * NH);
+    auto tile_of = [](int x) { return x / (128 * NH); };
+    auto half_of = [](int x) { return NH == 1 ? 0 : x >> 7 & 1; };
+    // tensor memory of this warp's 32 lanes: its half of S, of P, of O
+    auto ts = [&](int x) { return tmem + ((x >> 5 & 3) << 21) + (NS == 1 ? 0 : tile_of(x) * AT_KEYS) + half_of(x) * HK; };
+    auto tp = [&](int x) { return tmem + ((x >> 5 & 3) << 21) + TM_P + (tile_of(x) * NH + half_of(x)) * (HK / 2); };
+    auto to = [&](int x) { return tmem + ((x >> 5 & 3) << 21) + TM_O + (tile_of(x) * NH + half_of(x)) * OD; };
     const float c = a.c;
-    int sn = 0, on = 0;
-    for (;; un++) {
-      AttnEntry e;
-      int kh;
-      if (!next_unit(e, kh)) break;
+    uint32_t par = 0;   // bit 0: blocks so far, bit 1: exchanges so far, modulo 2
+    // The other half's number for this row, in exchange for this one's.
+    auto exchange = [&](float mine, float& other) -> bool {
+      if (NH == 1) {
+        other = mine;
+        return true;
+      }
+      const int x = at_tid(), i = par >> 1 & 1;
+      float* r = &sh.row[i][x >> 8 & 1][0][(x & 31) + (x >> 5 & 3) * 32];
+      r[(x >> 7 & 1) * AT_ROWS] = mine;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.unit_empty[un & 1]);
-      const int tt = t * a.tpt + tok, nb = e.kb1 - e.kb0;
-      if (t * a.tpt >= e.ntok) continue;
+      uint64_t* bar = &sh.pair[(x >> 8) * 4 + (x >> 5 & 3)];
+      if ((x & 31) == 0) mbar_arrive(bar);
+      if (!at_wait(bar, i, abort)) {
+        fail(326, un);
+        return false;
+      }
+      other = r[((x >> 7 & 1) ^ 1) * AT_ROWS];
+      par ^= 2;
+      return true;
+    };
+    // The row's keys [lo, hi), from its unit; whether it has any.
+    auto row_keys = [&](const AttnEntry& e, int& tt, int& g, int& lo, int& hi) -> bool {
+      const int x = at_tid(), row = (x & 31) + (x >> 5 & 3) * 32, tok = row / a.G;
+      g = row - tok * a.G;
+      tt = tile_of(x) * a.tpt + tok;
       const bool valid = tok < a.tpt && tt < e.ntok;
-      int hi, lo = 0;   // the row's keys
+      lo = 0;
       if (SHARED) {
         hi = a.P;
         if (a.window > 0 && valid) lo = max(0, a.P + min(max(a.lens[e.q0 + tt], 0), a.max_len) - a.window);
@@ -518,129 +625,301 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
         hi = e.p0 + tt + 1;
         if (a.window > 0) lo = max(0, hi - a.window);
       }
-      const int wlo = __reduce_max_sync(~0u, valid ? lo : 0), whi = __reduce_min_sync(~0u, valid ? hi : AT_NPOS);
-      float m = -INFINITY, l = 0.f;
+      return valid;
+    };
+    for (;; un++) {
+      {
+        AttnEntry e;
+        int kh;
+        if (!next_unit(e, kh)) break;
+      }
+      const volatile AttnEntry* ev = &sh.unit[un % AT_UNITS];   // handed back at the unit's end
+      auto entry = [&]() {
+        AttnEntry e;
+        e.q0 = ev->q0, e.ntok = ev->ntok, e.p0 = ev->p0, e.ks = ev->ks, e.nb = ev->nb, e.slot = ev->slot;
+        return e;
+      };
+      const int nb = ev->nb;
+      float m = -INFINITY, l = 0.f, sink2 = -INFINITY;
       bool ok = true;
-      for (int j = 0; j < nb; j++) {
-        if (!at_wait(&sh.s_full[t], sn & 1, abort)) {
-          if (lane == 0) fail(320 + t, un);
+      const bool mine = t * a.tpt < ev->ntok;   // the tile has rows
+      if (mine) {
+        const AttnEntry e = entry();
+        int tt, g, lo, hi;
+        const bool valid = row_keys(e, tt, g, lo, hi);
+        // over the warp's rows: keys that some see, and keys that all see
+        const int lo0 = __reduce_min_sync(~0u, valid ? lo : AT_NPOS), hi1 = __reduce_max_sync(~0u, valid ? hi : 0);
+        const int lo1 = __reduce_max_sync(~0u, valid ? lo : 0), hi0 = __reduce_min_sync(~0u, valid ? hi : AT_NPOS);
+        if (lane == 0) sh.edge[wid] = make_int4(lo0, hi1, lo1, hi0);
+        __syncwarp();
+        if (!SHARED && a.sinks && valid && e.slot < 0) sink2 = a.sinks[sh.unit_kh[un % AT_UNITS] * a.G + g] * LOG2E;
+      }
+      for (int j = 0; mine && j < nb; j++) {
+        if (!at_wait(&sh.s_full[t], par & 1, abort)) {
+          fail(320 + t, un);
           ok = false;
           break;
         }
-        sn++;
         at_fence_after();
-        uint32_t r[128];
+        uint32_t r[HK];
+        const uint32_t sa = ts(at_tid());
 #pragma unroll
-        for (int i = 0; i < 4; i++) at_ld32(ts + 32 * i, r + 32 * i);
+        for (int i = 0; i < HK / 32; i++) at_ld32(sa + 32 * i, r + 32 * i);
         at_wait_ld();
+        at_fence_before();
+        __syncwarp();
+        if ((at_tid() & 31) == 0) mbar_arrive(&sh.s_loaded[t]);
         float* s = reinterpret_cast<float*>(r);
-        const int base = (e.kb0 + j) * AT_KEYS;
-        if (base < wlo || base + AT_KEYS > whi) {
-          const int l0 = lo - base, h0 = hi - base;
+        // Masked blocks go by chunks of 32 keys: those that no row of the warp
+        // sees (dead) need no exponential, and only those at an edge a test
+        // for each key.
+        unsigned dead = 0;
+        bool clean = true;
+        {
+          const int x = at_tid(), base = ev->ks + j * AT_KEYS + half_of(x) * HK;
+          const volatile int* edge = &sh.edge[x >> 5].x;
+          if (base < edge[2] || base + HK > edge[3]) {
+            clean = false;
+            int tt, g, lo, hi;
+            row_keys(entry(), tt, g, lo, hi);
+            const int lo0 = edge[0], hi1 = edge[1], lo1 = edge[2], hi0 = edge[3];
 #pragma unroll
-          for (int i = 0; i < 128; i++) s[i] = i >= l0 && i < h0 ? s[i] : -INFINITY;
+            for (int i = 0; i < HK / 32; i++) {
+              const int cb = base + 32 * i;
+              if (cb >= hi1 || cb + 32 <= lo0) {
+                dead |= 1u << i;
+#pragma unroll
+                for (int q = 0; q < 32; q++) s[32 * i + q] = -INFINITY;
+              } else if (cb < lo1 || cb + 32 > hi0) {
+                const int l0 = lo - cb, h0 = hi - cb;
+                unsigned see = h0 >= 32 ? ~0u : h0 <= 0 ? 0u : (1u << h0) - 1;
+                see &= l0 <= 0 ? ~0u : l0 >= 32 ? 0u : ~0u << l0;
+#pragma unroll
+                for (int q = 0; q < 32; q++) s[32 * i + q] = see & (1u << q) ? s[32 * i + q] : -INFINITY;
+              }
+            }
+          }
         }
-        float mx[4] = {s[0], s[1], s[2], s[3]};
+        float mx[4];
 #pragma unroll
-        for (int i = 4; i < 128; i++) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
-        const float mn = fmaxf(fmaxf(m, fmaxf(mx[0], mx[1])), fmaxf(mx[2], mx[3]));
+        for (int i = 0; i < 4; i++) mx[i] = at_max3(s[i], s[i + 4], s[i + 8]);
+#pragma unroll
+        for (int i = 12; i < HK - 4; i += 8)
+#pragma unroll
+          for (int q = 0; q < 4; q++) mx[q] = at_max3(mx[q], s[i + q], s[i + q + 4]);
+#pragma unroll
+        for (int q = 0; q < 4; q++) mx[q] = fmaxf(mx[q], s[HK - 4 + q]);
+        float mn = fmaxf(at_max3(m, mx[0], mx[1]), fmaxf(mx[2], mx[3])), other;
+        if (!exchange(mn, other)) {
+          ok = false;
+          break;
+        }
+        mn = fmaxf(mn, other);
+        // P V of the block before: its P may be overwritten, its O scaled (a
+        // barrier's phase before its first counts as complete)
+        if (!at_wait(&sh.p_empty[t], (par & 1) ^ 1, abort)) {
+          fail(324 + t, un);
+          ok = false;
+          break;
+        }
+        par ^= 1;
+        at_fence_after();
         if (j == 0) {
           m = mn;
         } else {
           const float d = (mn - m) * c;
           const bool up = d > 8.f;
-          if (__any_sync(~0u, up)) {   // P V of the block before is complete: S came behind it
+          if (__any_sync(~0u, up)) {
+            const uint32_t oa = to(at_tid());
             const float f = up ? at_exp2(-d) : 1.f;
             if (up) m = mn;
             l *= f;
 #pragma unroll
-            for (int i = 0; i < HD / 32; i++) {
-              uint32_t o[32];
-              at_ld32(to + 32 * i, o);
+            for (int i = 0; i < OD / 16; i++) {
+              uint32_t o[16];
+              at_ld16(oa + 16 * i, o);
               at_wait_ld();
 #pragma unroll
-              for (int q = 0; q < 32; q++) o[q] = __float_as_uint(__uint_as_float(o[q]) * f);
-              at_st32(to + 32 * i, o);
+              for (int q = 0; q < 16; q++) o[q] = __float_as_uint(__uint_as_float(o[q]) * f);
+              at_st16(oa + 16 * i, o);
             }
           }
         }
+        const uint32_t pa = tp(at_tid());
         const float cm = m == -INFINITY ? 0.f : -c * m;
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        auto scaled = [&](int i) {   // c s - c m of the pair i
+          return at_fma2(make_float2(s[2 * i], s[2 * i + 1]), make_float2(c, c), make_float2(cm, cm));
+        };
+        if (clean) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          uint32_t p[16];
+          for (int i = 0; i < HK / 32; i++) {
+            uint32_t p[16];
 #pragma unroll
-          for (int q = 0; q < 16; q++) {
-            float2 x = at_fma2(make_float2(s[32 * i + 2 * q], s[32 * i + 2 * q + 1]), make_float2(c, c), make_float2(cm, cm));
-            x.x = at_exp2(x.x);
-            x.y = at_exp2(x.y);
-            sum[q & 1] = at_add2(sum[q & 1], x);
-            p[q] = at_pack<T>(x.x, x.y);
+            for (int q = 0; q < 16; q++) {
+              float2 x = scaled(16 * i + q);
+              if (q % S::POLY_OF == S::POLY_OF - 1) {
+                x = at_exp2_poly(x);
+              } else {
+                x.x = at_exp2(x.x);
+                x.y = at_exp2(x.y);
+              }
+              sum[q & 1] = at_add2(sum[q & 1], x);
+              p[q] = at_pack<T>(x.x, x.y);
+            }
+            at_st16(pa + 16 * i, p);
           }
-          at_st16(ts + 16 * i, p);
+        } else {   // -inf has to give 0 here
+#pragma unroll
+          for (int i = 0; i < HK / 32; i++) {
+            uint32_t p[16];
+            if (dead >> i & 1) {
+#pragma unroll
+              for (int q = 0; q < 16; q++) p[q] = 0;
+            } else {
+#pragma unroll
+              for (int q = 0; q < 16; q++) {
+                float2 x = scaled(16 * i + q);
+                x.x = at_exp2(x.x);
+                x.y = at_exp2(x.y);
+                sum[q & 1] = at_add2(sum[q & 1], x);
+                p[q] = at_pack<T>(x.x, x.y);
+              }
+            }
+            at_st16(pa + 16 * i, p);
+          }
         }
         at_wait_st();
         at_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.p_full[t]);
+        if ((at_tid() & 31) == 0) mbar_arrive(&sh.p_full[t]);
         sum[0] = at_add2(sum[0], sum[1]);
         l += sum[0].x + sum[0].y;
       }
       if (!ok) break;
-      if (nb > 0) {
-        if (!at_wait(&sh.o_full[t], on & 1, abort)) {
-          if (lane == 0) fail(322 + t, un);
-          break;
-        }
-        on++;
-        at_fence_after();
-      }
-      const int h = kh * a.G + g;
-      const bool part = SHARED || e.slot >= 0;
-      const size_t pr = ((size_t)e.slot * a.KH + kh) * (2 * AT_ROWS) + t * AT_ROWS + row;
-      float inv = 1.f;
-      if (part) {
-        if (valid) a.pml[pr] = make_float2(l == 0.f ? -INFINITY : c * m, l);
-      } else {
-        if (a.sinks && valid && l != 0.f) l += at_exp2(a.sinks[h] * LOG2E - c * m);
-        inv = l == 0.f ? 0.f : 1.f / l;
-      }
-      T* out = (T*)a.out + (e.q0 + tt) * a.so[0] + h * a.so[1];
-      float* po = a.po + pr * HD;
-#pragma unroll
-      for (int i = 0; i < HD / 32; i++) {
-        uint32_t o[32];
+      if (mine) {
         if (nb > 0) {
-          at_ld32(to + 32 * i, o);
-          at_wait_ld();
-        } else {
-#pragma unroll
-          for (int q = 0; q < 32; q++) o[q] = 0;
+          float other;
+          if (!exchange(l, other)) break;
+          if (NH == 2) l = half_of(at_tid()) ? other + l : l + other;
+          if (!at_wait(&sh.p_empty[t], (par & 1) ^ 1, abort)) {   // the last P V: O is whole
+            fail(322 + t, un);
+            break;
+          }
+          at_fence_after();
         }
-        if (!valid) continue;
+        const AttnEntry e = entry();
+        int tt, g, lo, hi;
+        const bool valid = row_keys(e, tt, g, lo, hi);
+        const int hf = half_of(at_tid()), kh = *(volatile int*)&sh.unit_kh[un % AT_UNITS];
+        const bool part = SHARED || e.slot >= 0;
+        float inv = 1.f;
+        char* at;   // this thread's outputs, or its part of the partial result
         if (part) {
-          if (nb <= 0) continue;   // l = 0: not read
-#pragma unroll
-          for (int q = 0; q < 32; q += 4)
-            *reinterpret_cast<uint4*>(po + 32 * i + q) = make_uint4(o[q], o[q + 1], o[q + 2], o[q + 3]);
+          const size_t pr = ((size_t)e.slot * a.KH + kh) * (2 * AT_ROWS) + tile_of(at_tid()) * AT_ROWS + (at_tid() & 127);
+          if (valid && hf == 0) a.pml[pr] = make_float2(l == 0.f ? -INFINITY : c * m, l);
+          at = (char*)(a.po + pr * HD + hf * OD);
         } else {
+          if (l != 0.f) l += at_exp2(sink2 - c * m);
+          inv = l == 0.f ? 0.f : 1.f / l;
+          at = (char*)((T*)a.out + (e.q0 + tt) * a.so[0] + (kh * a.G + g) * a.so[1] + hf * OD);
+        }
 #pragma unroll
-          for (int q = 0; q < 32; q += 8) {
-            uint4 x;
-            uint32_t* xs = &x.x;
+        for (int i = 0; i < OD / 32; i++) {
+          uint32_t o[32];
+          if (nb > 0) {
+            at_ld32(to(at_tid()) + 32 * i, o);
+            at_wait_ld();
+          } else {
 #pragma unroll
-            for (int z = 0; z < 4; z++)
-              xs[z] = at_pack<T>(__uint_as_float(o[q + 2 * z]) * inv, __uint_as_float(o[q + 2 * z + 1]) * inv);
-            if (32 * i + q < a.hd) *reinterpret_cast<uint4*>(out + 32 * i + q) = x;
+            for (int q = 0; q < 32; q++) o[q] = 0;
+          }
+          if (!valid || (part && nb <= 0)) continue;   // a partial result without keys, l = 0, is not read
+          if (part) {
+#pragma unroll
+            for (int q = 0; q < 32; q += 4) reinterpret_cast<uint4*>(at)[8 * i + q / 4] = make_uint4(o[q], o[q + 1], o[q + 2], o[q + 3]);
+          } else {
+#pragma unroll
+            for (int q = 0; q < 32; q += 8) {
+              uint32_t x[4];
+#pragma unroll
+              for (int z = 0; z < 4; z++) x[z] = at_pack<T>(__uint_as_float(o[q + 2 * z]) * inv, __uint_as_float(o[q + 2 * z + 1]) * inv);
+              if (hf * OD + 32 * i + q < a.hd) reinterpret_cast<uint4*>(at)[4 * i + q / 8] = make_uint4(x[0], x[1], x[2], x[3]);
+            }
           }
         }
+        at_fence_before();
       }
-      at_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.unit_empty[un % AT_UNITS]);
     }
   }
   at_fence_before();
   __syncthreads();
-  if (wid == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  if (wid == W0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  if (SHARED && a.beside && blockIdx.x == gridDim.x - 1) pdl_wait();   // this grid ends after the one beside it
+}
+
+// ---------------------------------------------------------------------
+// Joining partial results.  A row's pieces have (c m, l) in pml and their
+// accumulators of HD values in po; row(i) is the place of piece i of n.
+//   M = max(c m_i, sink),  f_i = 2^(c m_i - M),
+//   o = sum f_i o_i / (sum f_i l_i + 2^(sink - M)).
+// A warp per row: its lanes weigh 32 pieces at a time, then add them up four
+// at a time with HD / 32 dimensions each.  Pieces without a key (l = 0) have
+// no accumulator.  Returns (M, 1 / the whole sum), 0 without keys.
+template <typename F>
+__device__ __forceinline__ float2 join_scale(int n, const float2* pml, float sink2, F row) {
+  const int lane = threadIdx.x & 31;
+  float M = -INFINITY, L = 0.f;
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const float2 ml = i0 + lane < n ? pml[row(i0 + lane)] : make_float2(-INFINITY, 0.f);
+    float m = ml.x;
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    m = fmaxf(M, m);
+    float l = ml.y == 0.f ? 0.f : ml.y * at_exp2(ml.x - m);
+    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
+    L = (L == 0.f ? 0.f : L * at_exp2(M - m)) + l;
+    M = m;
+  }
+  if (L == 0.f) return make_float2(0.f, 0.f);
+  const float m = fmaxf(M, sink2);
+  return make_float2(m, 1.f / (L * at_exp2(M - m) + at_exp2(sink2 - m)));
+}
+template <typename T, int HD, typename F>
+__device__ __forceinline__ void join_row(int n, const float2* pml, const float* po, float2 fin, F row, T* out, int hd) {
+  constexpr int E = HD / 32;
+  const int lane = threadIdx.x & 31;
+  float o[E] = {};
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const long long r = i0 + lane < n ? (long long)row(i0 + lane) : 0;
+    const float2 ml = i0 + lane < n ? pml[r] : make_float2(0.f, 0.f);
+    const float f = ml.y == 0.f ? 0.f : at_exp2(ml.x - fin.x) * fin.y;
+    unsigned todo = __ballot_sync(~0u, ml.y != 0.f);
+    while (todo) {
+      float fj[4], x[4][E];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int i = todo ? __ffs(todo) - 1 : -1;
+        todo &= todo - 1;
+        fj[j] = __shfl_sync(~0u, f, i & 31);
+        const long long ri = __shfl_sync(~0u, r, i & 31);
+        if (i < 0) fj[j] = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const float2 v = i < 0 ? make_float2(0.f, 0.f) : *reinterpret_cast<const float2*>(po + ri * HD + lane * E + e);
+          x[j][e] = v.x, x[j][e + 1] = v.y;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] = fmaf(x[j][e], fj[j], o[e]);
+    }
+  }
+  if (lane * E < hd)
+#pragma unroll
+    for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(out + lane * E + e) = at_pack<T>(o[e], o[e + 1]);
 }
 
 // ---------------------------------------------------------------------
@@ -732,7 +1011,7 @@ inline cudaError_t launch_attn_tc(const CUtensorMap& q, const CUtensorMap& k, co
     if (e == cudaSuccess && dev < 64) set |= 1ull << dev;
   }
   if (e != cudaSuccess) return e;
-  return launch_pdl(attn_tc_kernel<T, HD, SHARED>, dim3(grid), AT_THREADS, smem, s, q, k, v, a);
+  return launch_pdl(attn_tc_kernel<T, HD, SHARED>, dim3(grid), AttnTcShape<HD>::THREADS, smem, s, q, k, v, a);
 }
 
 DevStatus* attn_status();   // the operators' device error record on the current device, or null (tg_attn_prompt.cu)
