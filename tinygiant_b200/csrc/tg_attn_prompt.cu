@@ -292,6 +292,7 @@ extern "C" int tg_attention_prompt(int dtype, const void* q, const void* k, cons
   a.sinks = sinks;
   a.so[0] = st[6], a.so[1] = st[7];
   a.G = G, a.KH = n_kv_heads, a.hd = head_dim, a.tpt = tpt, a.window = window, a.total_k = total_k;
+  a.wide = head_dim % 16 == 0 && (uintptr_t)out % 32 == 0 && st[6] % 16 == 0 && st[7] % 16 == 0;
   a.c = scale * LOG2E;
   a.st = attn_status();
   CombineArgs cb{p.head, p.splits, a.po, a.pml, sinks, out, {st[6], st[7]}, G, n_kv_heads, head_dim, tpt};

@@ -20,14 +20,12 @@
 // short sequences fill tiles, and the masked corner of the causal diagonal is
 // a few tokens wide.  Its keys are nb blocks from key ks on.
 //
-// Warps: 0-7 and 8-15 the softmax of tile 0 and 1, two threads per row with 64
-// of a block's keys each, who exchange their maxima (with one thread per row
-// and 128 keys in registers a warp's own latencies bound the kernel: 490 us
-// against the 8,192-token figure below); 16 the TMA loads, 17 the S products,
-// 18 the P V.  Tensor memory (512 columns): O of both tiles, the 16-bit P of
-// both, and S, one buffer of 128 columns for both tiles at head_dim 128, one
-// for each at 64.  A softmax warp takes its S into registers at once and frees
-// the buffer, so the next S is computed while it works on its exponentials.
+// Warps: 0-3 and 4-7 the softmax of tile 0 and 1 (a thread per row), 8 the TMA
+// loads, 9 the S products, 10 the P V.  Tensor memory (512 columns): O of both
+// tiles, the 16-bit P of both, and S, one buffer of 128 columns for both tiles
+// at head_dim 128, one for each at 64.  A softmax warp takes its S into
+// registers at once and frees the buffer, so the next S is computed while it
+// works on its exponentials.
 // Persistent CTAs, one per SM; units come from an atomic counter, longest
 // first.
 // Every wait is bounded; a role that gives up records the error and the others
@@ -45,9 +43,8 @@ namespace tg {
 
 constexpr int AT_ROWS = 128;       // query rows per tile (MMA M)
 constexpr int AT_KEYS = 128;       // keys per block (MMA N of S, K of P V)
-#ifndef NH_OF
-#define NH_OF(HD) 1
-#endif
+constexpr int AT_SOFT = 8;         // softmax warps; then one each for loads, S, P V, and an idle one:
+constexpr int AT_THREADS = 384;    // registers move between whole warpgroups
 constexpr int AT_NPOS = 0x3fffffff;
 constexpr int AT_UNITS = 4;        // units announced ahead
 
@@ -110,6 +107,7 @@ struct AttnTcArgs {
   int G, KH, hd, tpt, window;
   int total_k;                // rows of k and v
   int P, B, nsp, max_len;     // shared: prefix keys, sequences, pieces per unit, bound of lens
+  int wide;                   // outputs in 32-byte pieces: head_dim a multiple of 16, rows 32-byte aligned
   int beside;                 // shared: launched beside a kernel that it does not wait for
   float c;                    // scale log2(e)
   DevStatus* st;
@@ -180,6 +178,11 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
                : "memory");
 }
 
+// 32 aligned bytes in one store: a warp's rows are far apart, and each store
+// takes the load/store unit a cycle for every row.
+__device__ __forceinline__ void at_store8(void* p, const uint32_t* r) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), AT_W4(r, 0), AT_W4(r, 4) : "memory");
+}
 // The thread's number, read anew: nothing computed from it stays in registers.
 __device__ __forceinline__ int at_tid() {
   int x;
@@ -250,11 +253,6 @@ __device__ __forceinline__ float2 at_exp2_poly(float2 x) {
 
 template <int HD>
 struct AttnTcShape {
-  static constexpr int NH = NH_OF(HD);                    // threads of the softmax per row
-  static constexpr int SOFT = 8 * NH;                     // its warps
-  static constexpr int THREADS = (SOFT + 4) * 32;         // and those of loads and products; the last idles
-  // registers: (65,536 / THREADS) at launch, moved between whole warpgroups
-  static constexpr int R_SOFT = NH == 1 ? 216 : 104, R_REST = NH == 1 ? 72 : 64;
   static constexpr int TILE = 128 * HD * 2;               // bytes of a Q tile, a K or a V block
   // One pair of exponentials in POLY_OF goes to the FMA units: the special
   // function unit gives 4 values a clock to each quarter of the SM, as long for
@@ -263,18 +261,15 @@ struct AttnTcShape {
   // products are half as long, 117, 106 and 107 us at 4,096).
   static constexpr int POLY_OF = HD == 128 ? 8 : 4;
   static constexpr int NQ = HD == 128 ? 1 : 2;            // units whose Q is there or on its way
-  static constexpr int STAGES = HD == 64 ? 8 : NH == 1 ? 5 : 4;        // K and V blocks in flight
+  static constexpr int STAGES = HD == 128 ? 5 : 8;        // K and V blocks in flight
   static constexpr int SMEM = (2 * NQ + STAGES) * TILE + 1024;
 };
 
-template <int NH>
 struct AttnTcShared {
-  uint64_t q_full[2], q_empty[2], kv_full[8], kv_empty[8], s_full[2], s_loaded[2], p_full[2], p_empty[2], pair[8], unit_full[AT_UNITS],
+  uint64_t q_full[2], q_empty[2], kv_full[8], kv_empty[8], s_full[2], s_loaded[2], p_full[2], p_empty[2], unit_full[AT_UNITS],
       unit_empty[AT_UNITS], aux, drain[2];
   AttnEntry unit[AT_UNITS];
   int unit_kh[AT_UNITS];      // -1: no more work
-  int4 edge[8 * NH];               // a softmax warp's lo0, hi1, lo1, hi0 (below)
-  float row[NH == 1 ? 1 : 2][2][2][NH == 1 ? 1 : AT_ROWS];   // a row's two halves' numbers: [turn][tile][half][row]
   uint32_t tmem;
   int abort;
 };
@@ -290,15 +285,15 @@ __device__ __forceinline__ bool at_wait(uint64_t* bar, uint32_t parity, const vo
 }
 
 template <typename T, int HD, bool SHARED>
-__global__ void __launch_bounds__(AttnTcShape<HD>::THREADS, 1) attn_tc_kernel(const __grid_constant__ CUtensorMap qmap,
+__global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_constant__ CUtensorMap qmap,
                                                                 const __grid_constant__ CUtensorMap kmap,
                                                                 const __grid_constant__ CUtensorMap vmap, const AttnTcArgs a) {
   using S = AttnTcShape<HD>;
-  constexpr int NST = S::STAGES, TILE = S::TILE, NQ = S::NQ, NH = S::NH, HK = AT_KEYS / NH, OD = HD / NH, W0 = S::SOFT;
+  constexpr int NST = S::STAGES, TILE = S::TILE, NQ = S::NQ, W0 = AT_SOFT;
   // tensor memory: S buffers of 128 columns, P of 64 for each tile, O of HD for each
   constexpr int NS = HD == 128 ? 1 : 2, TM_P = NS * AT_KEYS, TM_O = TM_P + AT_KEYS;
   extern __shared__ uint8_t dsm[];
-  __shared__ AttnTcShared<S::NH> sh;
+  __shared__ AttnTcShared sh;
   const int tid = threadIdx.x, wid = tid >> 5, lane = tid & 31;
   uint8_t* qs = dsm + ((1024u - (smem_u32(dsm) & 1023u)) & 1023u);
   uint8_t* kvs = qs + 2 * NQ * TILE;
@@ -325,7 +320,6 @@ __global__ void __launch_bounds__(AttnTcShape<HD>::THREADS, 1) attn_tc_kernel(co
       mbar_init(&sh.unit_full[i], 1);
       mbar_init(&sh.unit_empty[i], W0 + 2);
     }
-    for (int i = 0; i < 8; i++) mbar_init(&sh.pair[i], 2);
     mbar_init(&sh.aux, 1);
     mbar_init(&sh.drain[0], 1);
     mbar_init(&sh.drain[1], 1);
@@ -393,8 +387,11 @@ __global__ void __launch_bounds__(AttnTcShape<HD>::THREADS, 1) attn_tc_kernel(co
     return kh >= 0;
   };
 
+  // 168 registers a thread at launch (384 x 168 = 64,512): 216 for the eight
+  // softmax warps and 72 for the four others make the same sum.
   if (wid >= W0) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::R_REST));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  }
   if (wid == W0) {
     // ---- loads
     const int tpu = 2 * a.tpt;
@@ -575,84 +572,43 @@ __global__ void __launch_bounds__(AttnTcShape<HD>::THREADS, 1) attn_tc_kernel(co
       }
     }
     __syncwarp();
-  }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::R_SOFT));
-    // ---- softmax of tile t: half `hf` of a row's keys and of its outputs.
-    // What a block does not need is kept in shared memory and computed again
-    // from the thread's number: a spilled register costs more, since next to
-    // 200 KB of shared memory there is hardly an L1 for it.
-    const int t = wid / (4 * NH);
-    auto tile_of = [](int x) { return x / (128 * NH); };
-    auto half_of = [](int x) { return NH == 1 ? 0 : x >> 7 & 1; };
-    // tensor memory of this warp's 32 lanes: its half of S, of P, of O
-    auto ts = [&](int x) { return tmem + ((x >> 5 & 3) << 21) + (NS == 1 ? 0 : tile_of(x) * AT_KEYS) + half_of(x) * HK; };
-    auto tp = [&](int x) { return tmem + ((x >> 5 & 3) << 21) + TM_P + (tile_of(x) * NH + half_of(x)) * (HK / 2); };
-    auto to = [&](int x) { return tmem + ((x >> 5 & 3) << 21) + TM_O + (tile_of(x) * NH + half_of(x)) * OD; };
+  } else if (wid < W0) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    // ---- softmax of tile t, a thread per row.  What a block does not need is
+    // read or computed again at the unit's end: a spilled register costs more,
+    // since next to 200 KB of shared memory there is hardly an L1 for it.
+    const int t = wid >> 2;
+    // tensor memory of this warp's 32 lanes: S, P, O of its tile
+    const uint32_t lanes = tmem + ((uint32_t)(wid & 3) << 21);
+    const uint32_t ts = lanes + (NS == 1 ? 0 : t * AT_KEYS), tp = lanes + TM_P + t * (AT_KEYS / 2), to = lanes + TM_O + t * HD;
     const float c = a.c;
-    uint32_t par = 0;   // bit 0: blocks so far, bit 1: exchanges so far, modulo 2
-    // The other half's number for this row, in exchange for this one's.
-    auto exchange = [&](float mine, float& other) -> bool {
-      if (NH == 1) {
-        other = mine;
-        return true;
-      }
-      const int x = at_tid(), i = par >> 1 & 1;
-      float* r = &sh.row[i][x >> 8 & 1][0][(x & 31) + (x >> 5 & 3) * 32];
-      r[(x >> 7 & 1) * AT_ROWS] = mine;
-      __syncwarp();
-      uint64_t* bar = &sh.pair[(x >> 8) * 4 + (x >> 5 & 3)];
-      if ((x & 31) == 0) mbar_arrive(bar);
-      if (!at_wait(bar, i, abort)) {
-        fail(326, un);
-        return false;
-      }
-      other = r[((x >> 7 & 1) ^ 1) * AT_ROWS];
-      par ^= 2;
-      return true;
-    };
-    // The row's keys [lo, hi), from its unit; whether it has any.
-    auto row_keys = [&](const AttnEntry& e, int& tt, int& g, int& lo, int& hi) -> bool {
-      const int x = at_tid(), row = (x & 31) + (x >> 5 & 3) * 32, tok = row / a.G;
-      g = row - tok * a.G;
-      tt = tile_of(x) * a.tpt + tok;
-      const bool valid = tok < a.tpt && tt < e.ntok;
-      lo = 0;
-      if (SHARED) {
-        hi = a.P;
-        if (a.window > 0 && valid) lo = max(0, a.P + min(max(a.lens[e.q0 + tt], 0), a.max_len) - a.window);
-      } else {
-        hi = e.p0 + tt + 1;
-        if (a.window > 0) lo = max(0, hi - a.window);
-      }
-      return valid;
-    };
+    uint32_t par = 0;   // blocks so far, modulo 2
     for (;; un++) {
+      const volatile AttnEntry* e = &sh.unit[un % AT_UNITS];   // handed back at the unit's end
       {
-        AttnEntry e;
+        AttnEntry first;
         int kh;
-        if (!next_unit(e, kh)) break;
+        if (!next_unit(first, kh)) break;
       }
-      const volatile AttnEntry* ev = &sh.unit[un % AT_UNITS];   // handed back at the unit's end
-      auto entry = [&]() {
-        AttnEntry e;
-        e.q0 = ev->q0, e.ntok = ev->ntok, e.p0 = ev->p0, e.ks = ev->ks, e.nb = ev->nb, e.slot = ev->slot;
-        return e;
-      };
-      const int nb = ev->nb;
-      float m = -INFINITY, l = 0.f, sink2 = -INFINITY;
-      bool ok = true;
-      const bool mine = t * a.tpt < ev->ntok;   // the tile has rows
+      const int nb = e->nb;
+      float m = -INFINITY, l = 0.f, sink = -INFINITY;
+      int lo = 0, hi = 0;                            // the row's keys
+      int lo0 = 0, hi1 = 0, lo1 = 0, hi0 = 0;        // over the warp's rows: keys that some see, keys that all see
+      bool valid = false, ok = true;
+      const bool mine = t * a.tpt < e->ntok;         // the tile has rows
       if (mine) {
-        const AttnEntry e = entry();
-        int tt, g, lo, hi;
-        const bool valid = row_keys(e, tt, g, lo, hi);
-        // over the warp's rows: keys that some see, and keys that all see
-        const int lo0 = __reduce_min_sync(~0u, valid ? lo : AT_NPOS), hi1 = __reduce_max_sync(~0u, valid ? hi : 0);
-        const int lo1 = __reduce_max_sync(~0u, valid ? lo : 0), hi0 = __reduce_min_sync(~0u, valid ? hi : AT_NPOS);
-        if (lane == 0) sh.edge[wid] = make_int4(lo0, hi1, lo1, hi0);
-        __syncwarp();
-        if (!SHARED && a.sinks && valid && e.slot < 0) sink2 = a.sinks[sh.unit_kh[un % AT_UNITS] * a.G + g] * LOG2E;
+        const int x = at_tid(), tok = (x & 127) / a.G, tt = (x >> 7) * a.tpt + tok;
+        valid = tok < a.tpt && tt < e->ntok;
+        if (SHARED) {
+          hi = a.P;
+          if (a.window > 0 && valid) lo = max(0, a.P + min(max(a.lens[e->q0 + tt], 0), a.max_len) - a.window);
+        } else {
+          hi = e->p0 + tt + 1;
+          if (a.window > 0) lo = max(0, hi - a.window);
+          if (a.sinks && valid && e->slot < 0) sink = a.sinks[sh.unit_kh[un % AT_UNITS] * a.G + (x & 127) - tok * a.G];   // used at the end
+        }
+        lo0 = __reduce_min_sync(~0u, valid ? lo : AT_NPOS), hi1 = __reduce_max_sync(~0u, valid ? hi : 0);
+        lo1 = __reduce_max_sync(~0u, valid ? lo : 0), hi0 = __reduce_min_sync(~0u, valid ? hi : AT_NPOS);
       }
       for (int j = 0; mine && j < nb; j++) {
         if (!at_wait(&sh.s_full[t], par & 1, abort)) {
@@ -661,42 +617,34 @@ __global__ void __launch_bounds__(AttnTcShape<HD>::THREADS, 1) attn_tc_kernel(co
           break;
         }
         at_fence_after();
-        uint32_t r[HK];
-        const uint32_t sa = ts(at_tid());
+        uint32_t r[AT_KEYS];
 #pragma unroll
-        for (int i = 0; i < HK / 32; i++) at_ld32(sa + 32 * i, r + 32 * i);
+        for (int i = 0; i < 4; i++) at_ld32(ts + 32 * i, r + 32 * i);
         at_wait_ld();
         at_fence_before();
         __syncwarp();
-        if ((at_tid() & 31) == 0) mbar_arrive(&sh.s_loaded[t]);
+        if (lane == 0) mbar_arrive(&sh.s_loaded[t]);
         float* s = reinterpret_cast<float*>(r);
         // Masked blocks go by chunks of 32 keys: those that no row of the warp
         // sees (dead) need no exponential, and only those at an edge a test
         // for each key.
+        const int base = e->ks + j * AT_KEYS;
         unsigned dead = 0;
-        bool clean = true;
-        {
-          const int x = at_tid(), base = ev->ks + j * AT_KEYS + half_of(x) * HK;
-          const volatile int* edge = &sh.edge[x >> 5].x;
-          if (base < edge[2] || base + HK > edge[3]) {
-            clean = false;
-            int tt, g, lo, hi;
-            row_keys(entry(), tt, g, lo, hi);
-            const int lo0 = edge[0], hi1 = edge[1], lo1 = edge[2], hi0 = edge[3];
+        const bool clean = base >= lo1 && base + AT_KEYS <= hi0;
+        if (!clean) {
 #pragma unroll
-            for (int i = 0; i < HK / 32; i++) {
-              const int cb = base + 32 * i;
-              if (cb >= hi1 || cb + 32 <= lo0) {
-                dead |= 1u << i;
+          for (int i = 0; i < 4; i++) {
+            const int cb = base + 32 * i;
+            if (cb >= hi1 || cb + 32 <= lo0) {
+              dead |= 1u << i;
 #pragma unroll
-                for (int q = 0; q < 32; q++) s[32 * i + q] = -INFINITY;
-              } else if (cb < lo1 || cb + 32 > hi0) {
-                const int l0 = lo - cb, h0 = hi - cb;
-                unsigned see = h0 >= 32 ? ~0u : h0 <= 0 ? 0u : (1u << h0) - 1;
-                see &= l0 <= 0 ? ~0u : l0 >= 32 ? 0u : ~0u << l0;
+              for (int q = 0; q < 32; q++) s[32 * i + q] = -INFINITY;
+            } else if (cb < lo1 || cb + 32 > hi0) {
+              const int l0 = lo - cb, h0 = hi - cb;
+              unsigned see = h0 >= 32 ? ~0u : h0 <= 0 ? 0u : (1u << h0) - 1;
+              see &= l0 <= 0 ? ~0u : l0 >= 32 ? 0u : ~0u << l0;
 #pragma unroll
-                for (int q = 0; q < 32; q++) s[32 * i + q] = see & (1u << q) ? s[32 * i + q] : -INFINITY;
-              }
+              for (int q = 0; q < 32; q++) s[32 * i + q] = see & (1u << q) ? s[32 * i + q] : -INFINITY;
             }
           }
         }
@@ -704,17 +652,12 @@ __global__ void __launch_bounds__(AttnTcShape<HD>::THREADS, 1) attn_tc_kernel(co
 #pragma unroll
         for (int i = 0; i < 4; i++) mx[i] = at_max3(s[i], s[i + 4], s[i + 8]);
 #pragma unroll
-        for (int i = 12; i < HK - 4; i += 8)
+        for (int i = 12; i < AT_KEYS - 4; i += 8)
 #pragma unroll
           for (int q = 0; q < 4; q++) mx[q] = at_max3(mx[q], s[i + q], s[i + q + 4]);
 #pragma unroll
-        for (int q = 0; q < 4; q++) mx[q] = fmaxf(mx[q], s[HK - 4 + q]);
-        float mn = fmaxf(at_max3(m, mx[0], mx[1]), fmaxf(mx[2], mx[3])), other;
-        if (!exchange(mn, other)) {
-          ok = false;
-          break;
-        }
-        mn = fmaxf(mn, other);
+        for (int q = 0; q < 4; q++) mx[q] = fmaxf(mx[q], s[AT_KEYS - 4 + q]);
+        const float mn = fmaxf(at_max3(m, mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         // P V of the block before: its P may be overwritten, its O scaled (a
         // barrier's phase before its first counts as complete)
         if (!at_wait(&sh.p_empty[t], (par & 1) ^ 1, abort)) {
@@ -730,22 +673,20 @@ __global__ void __launch_bounds__(AttnTcShape<HD>::THREADS, 1) attn_tc_kernel(co
           const float d = (mn - m) * c;
           const bool up = d > 8.f;
           if (__any_sync(~0u, up)) {
-            const uint32_t oa = to(at_tid());
             const float f = up ? at_exp2(-d) : 1.f;
             if (up) m = mn;
             l *= f;
 #pragma unroll
-            for (int i = 0; i < OD / 16; i++) {
+            for (int i = 0; i < HD / 16; i++) {
               uint32_t o[16];
-              at_ld16(oa + 16 * i, o);
+              at_ld16(to + 16 * i, o);
               at_wait_ld();
 #pragma unroll
               for (int q = 0; q < 16; q++) o[q] = __float_as_uint(__uint_as_float(o[q]) * f);
-              at_st16(oa + 16 * i, o);
+              at_st16(to + 16 * i, o);
             }
           }
         }
-        const uint32_t pa = tp(at_tid());
         const float cm = m == -INFINITY ? 0.f : -c * m;
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         auto scaled = [&](int i) {   // c s - c m of the pair i
@@ -753,7 +694,7 @@ __global__ void __launch_bounds__(AttnTcShape<HD>::THREADS, 1) attn_tc_kernel(co
         };
         if (clean) {
 #pragma unroll
-          for (int i = 0; i < HK / 32; i++) {
+          for (int i = 0; i < 4; i++) {
             uint32_t p[16];
 #pragma unroll
             for (int q = 0; q < 16; q++) {
@@ -767,11 +708,11 @@ __global__ void __launch_bounds__(AttnTcShape<HD>::THREADS, 1) attn_tc_kernel(co
               sum[q & 1] = at_add2(sum[q & 1], x);
               p[q] = at_pack<T>(x.x, x.y);
             }
-            at_st16(pa + 16 * i, p);
+            at_st16(tp + 16 * i, p);
           }
         } else {   // -inf has to give 0 here
 #pragma unroll
-          for (int i = 0; i < HK / 32; i++) {
+          for (int i = 0; i < 4; i++) {
             uint32_t p[16];
             if (dead >> i & 1) {
 #pragma unroll
@@ -786,49 +727,44 @@ __global__ void __launch_bounds__(AttnTcShape<HD>::THREADS, 1) attn_tc_kernel(co
                 p[q] = at_pack<T>(x.x, x.y);
               }
             }
-            at_st16(pa + 16 * i, p);
+            at_st16(tp + 16 * i, p);
           }
         }
         at_wait_st();
         at_fence_before();
         __syncwarp();
-        if ((at_tid() & 31) == 0) mbar_arrive(&sh.p_full[t]);
+        if (lane == 0) mbar_arrive(&sh.p_full[t]);
         sum[0] = at_add2(sum[0], sum[1]);
         l += sum[0].x + sum[0].y;
       }
       if (!ok) break;
       if (mine) {
         if (nb > 0) {
-          float other;
-          if (!exchange(l, other)) break;
-          if (NH == 2) l = half_of(at_tid()) ? other + l : l + other;
           if (!at_wait(&sh.p_empty[t], (par & 1) ^ 1, abort)) {   // the last P V: O is whole
             fail(322 + t, un);
             break;
           }
           at_fence_after();
         }
-        const AttnEntry e = entry();
-        int tt, g, lo, hi;
-        const bool valid = row_keys(e, tt, g, lo, hi);
-        const int hf = half_of(at_tid()), kh = *(volatile int*)&sh.unit_kh[un % AT_UNITS];
-        const bool part = SHARED || e.slot >= 0;
+        const int x = at_tid(), tok = (x & 127) / a.G, g = (x & 127) - tok * a.G, kh = *(volatile int*)&sh.unit_kh[un % AT_UNITS];
+        const int slot = e->slot;
+        const bool part = SHARED || slot >= 0;
         float inv = 1.f;
         char* at;   // this thread's outputs, or its part of the partial result
         if (part) {
-          const size_t pr = ((size_t)e.slot * a.KH + kh) * (2 * AT_ROWS) + tile_of(at_tid()) * AT_ROWS + (at_tid() & 127);
-          if (valid && hf == 0) a.pml[pr] = make_float2(l == 0.f ? -INFINITY : c * m, l);
-          at = (char*)(a.po + pr * HD + hf * OD);
+          const size_t pr = ((size_t)slot * a.KH + kh) * (2 * AT_ROWS) + x;
+          if (valid) a.pml[pr] = make_float2(l == 0.f ? -INFINITY : c * m, l);
+          at = (char*)(a.po + pr * HD);
         } else {
-          if (l != 0.f) l += at_exp2(sink2 - c * m);
+          if (l != 0.f) l += at_exp2(fmaf(sink, LOG2E, -c * m));
           inv = l == 0.f ? 0.f : 1.f / l;
-          at = (char*)((T*)a.out + (e.q0 + tt) * a.so[0] + (kh * a.G + g) * a.so[1] + hf * OD);
+          at = (char*)((T*)a.out + (e->q0 + (x >> 7) * a.tpt + tok) * a.so[0] + (kh * a.G + g) * a.so[1]);
         }
 #pragma unroll
-        for (int i = 0; i < OD / 32; i++) {
+        for (int i = 0; i < HD / 32; i++) {
           uint32_t o[32];
           if (nb > 0) {
-            at_ld32(to(at_tid()) + 32 * i, o);
+            at_ld32(to + 32 * i, o);
             at_wait_ld();
           } else {
 #pragma unroll
@@ -837,14 +773,19 @@ __global__ void __launch_bounds__(AttnTcShape<HD>::THREADS, 1) attn_tc_kernel(co
           if (!valid || (part && nb <= 0)) continue;   // a partial result without keys, l = 0, is not read
           if (part) {
 #pragma unroll
-            for (int q = 0; q < 32; q += 4) reinterpret_cast<uint4*>(at)[8 * i + q / 4] = make_uint4(o[q], o[q + 1], o[q + 2], o[q + 3]);
+            for (int q = 0; q < 32; q += 8) at_store8(at + 128 * i + 4 * q, o + q);
           } else {
+            uint32_t y[16];
 #pragma unroll
-            for (int q = 0; q < 32; q += 8) {
-              uint32_t x[4];
+            for (int z = 0; z < 16; z++) y[z] = at_pack<T>(__uint_as_float(o[2 * z]) * inv, __uint_as_float(o[2 * z + 1]) * inv);
+            // 32 bytes at a time where they are whole and aligned
+            if (a.wide) {
+              if (32 * i < a.hd) at_store8(at + 64 * i, y);
+              if (32 * i + 16 < a.hd) at_store8(at + 64 * i + 32, y + 8);
+            } else {
 #pragma unroll
-              for (int z = 0; z < 4; z++) x[z] = at_pack<T>(__uint_as_float(o[q + 2 * z]) * inv, __uint_as_float(o[q + 2 * z + 1]) * inv);
-              if (hf * OD + 32 * i + q < a.hd) reinterpret_cast<uint4*>(at)[4 * i + q / 8] = make_uint4(x[0], x[1], x[2], x[3]);
+              for (int q = 0; q < 4; q++)
+                if (32 * i + 8 * q < a.hd) reinterpret_cast<uint4*>(at)[4 * i + q] = make_uint4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
             }
           }
         }
@@ -1011,7 +952,7 @@ inline cudaError_t launch_attn_tc(const CUtensorMap& q, const CUtensorMap& k, co
     if (e == cudaSuccess && dev < 64) set |= 1ull << dev;
   }
   if (e != cudaSuccess) return e;
-  return launch_pdl(attn_tc_kernel<T, HD, SHARED>, dim3(grid), AttnTcShape<HD>::THREADS, smem, s, q, k, v, a);
+  return launch_pdl(attn_tc_kernel<T, HD, SHARED>, dim3(grid), AT_THREADS, smem, s, q, k, v, a);
 }
 
 DevStatus* attn_status();   // the operators' device error record on the current device, or null (tg_attn_prompt.cu)
