@@ -106,17 +106,18 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const PlanArgs a) {
     atomicMax(&s_max, mx);
   }
   __syncthreads();
-  // Units of more than `share` blocks are split into equal pieces of at most
-  // that.  There are at most 2 total / share such pieces, which bounds them
-  // by the capacity.
+  // Units of more than twice `share` blocks are split into equal pieces of at
+  // most `share` (a piece costs a partial result; taken first, a unit of up to
+  // twice an SM's share delays the end by less than that).  There are at most
+  // 2 total / share pieces, which bounds them by the capacity.
   const unsigned long long total = s_total;
   int share = 0x7fffffff;
   if (a.max_slots > 0) {
     const unsigned long long even = (total * a.KH + a.sms - 1) / a.sms, room = (2 * total + a.max_slots - 1) / a.max_slots;
     share = (int)min((unsigned long long)0x7fffffff, max((unsigned long long)MIN_PIECE, max(even, room)));
   }
-  auto pieces = [&](int cost) { return cost > share ? (cost + share - 1) / share : 1; };
-  const int top = max(1, min(s_max, share));
+  auto pieces = [&](int cost) { return cost > 2ll * share ? (cost + share - 1) / share : 1; };
+  const int top = max(1, (int)min((long long)s_max, 2ll * share));
   auto bucket = [&](int size) { return top < PLAN_BUCKETS ? top - size : (int)((long long)(top - size) * PLAN_BUCKETS / (top + 1)); };
   each([&](const AttnEntry& e, int cost) {
     const int n = pieces(cost);
@@ -230,7 +231,7 @@ static cudaError_t run_prompt(const PlanArgs& p, const CUtensorMap& qm, const CU
   if (e == cudaSuccess) e = launch_attn_tc<T, HD, false>(qm, km, vm, a, (int)std::min((long long)p.sms, work), s);
   count_launches(1);
   if (e == cudaSuccess && p.max_slots > 0) {
-    e = launch_pdl(combine_kernel<T, HD>, dim3(2 * p.sms), 256, 0, s, c);
+    e = launch_pdl(combine_kernel<T, HD>, dim3(8 * p.sms), 256, 0, s, c);
     count_launches(1);
   }
   return e;

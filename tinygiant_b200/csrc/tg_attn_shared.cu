@@ -34,9 +34,9 @@
 
 namespace tg {
 
-constexpr int OWN_KEYS = 128;       // keys per stage: 16 for each consumer warp
+constexpr int OWN_KEYS = 128;       // keys per stage: 32 for each warp of a group
 constexpr int OWN_BOX = 32;         // rows per TMA box: a sequence's last stage reads at most 31 rows too many
-constexpr int OWN_WARPS = 8;
+constexpr int OWN_WARPS = 8;        // two groups of four that take stages in turn
 constexpr int OWN_THREADS = (OWN_WARPS + 1) * 32;
 
 struct OwnArgs {
@@ -56,8 +56,9 @@ template <int HD>
 struct OwnShape {
   static constexpr int HALF = OWN_KEYS * 128;             // bytes of 64 columns of a stage's K or V
   static constexpr int STAGE = 2 * (HD / 64) * HALF;      // K and V
-  static constexpr int STAGES = HD == 128 ? 3 : 6;
-  static constexpr int RED = OWN_WARPS * 8 * HD * 4;      // the warps' accumulators of 8 heads
+  static constexpr int STAGES = HD == 128 ? 3 : 6, BARS = 2 * STAGES;
+  static constexpr int RP = HD + 4;                       // row pitch of the next: lanes with other heads on other banks
+  static constexpr int RED = OWN_WARPS * 8 * RP * 4;      // the warps' accumulators of 8 heads
   static constexpr int SMEM = STAGES * STAGE + RED + 1024;
 };
 
@@ -96,8 +97,11 @@ __device__ __forceinline__ void mma16816<__half>(float (&d)[4], const uint32_t (
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Barriers go by the stage's number modulo twice the ring: then a barrier
+// belongs to one group, which sees each of its phases (a wait by parity passes
+// if the barrier is a whole phase behind).
 struct OwnShared {
-  uint64_t full[6], empty[6];
+  uint64_t full[12], empty[12];
   float2 ml[OWN_WARPS][8];   // each warp's (m, l) of 8 heads
   int sums[OWN_WARPS];
   int b0, before;            // the CTA's first sequence, and the stages of a key head before it
@@ -152,9 +156,13 @@ struct OwnWalk {
 };
 
 // Persistent, one CTA per SM of its share.  Warp 8 loads stages ahead, across
-// segments; each of warps 0-7 takes 16 keys of a stage with a running maximum
-// of its own, and the warps' partial results join in shared memory at the end
-// of a segment.
+// segments.  Warps 0-3 and 4-7 take stages in turn, each warp 32 keys with a
+// reference m of its own (moved, as in attn_tc_kernel, only when a score
+// exceeds it by 8 in base 2: one vote in the common case); the warps' partial
+// results join in shared memory at the end of a segment.  A step's latencies
+// (matrix loads, dependent products, exponentials) are what a warp waits for:
+// two tiles of 16 keys in flight and two groups of warps took an SM from 46 to
+// the figure below of GB/s.
 template <typename T, int HD, int NT>
 __global__ void __launch_bounds__(OWN_THREADS, 1) own_kernel(const __grid_constant__ CUtensorMap kmap,
                                                              const __grid_constant__ CUtensorMap vmap, const OwnArgs a) {
@@ -166,9 +174,9 @@ __global__ void __launch_bounds__(OWN_THREADS, 1) own_kernel(const __grid_consta
   float* red = reinterpret_cast<float*>(stages + S::STAGES * S::STAGE);
   volatile int* abort = &sh.abort;
   if (tid == 0) {
-    for (int i = 0; i < S::STAGES; i++) {
+    for (int i = 0; i < S::BARS; i++) {
       mbar_init(&sh.full[i], 1);
-      mbar_init(&sh.empty[i], OWN_WARPS);
+      mbar_init(&sh.empty[i], OWN_WARPS / 2);
     }
     sh.abort = 0;
     fence_mbar_init();
@@ -232,31 +240,38 @@ __global__ void __launch_bounds__(OWN_THREADS, 1) own_kernel(const __grid_consta
     for (wk.start(a, sh.b0, sh.before, x0, x1); wk.more() && ok; wk.next(a)) {
       const int kh = wk.hk / a.ngc;
       for (int j = wk.j; j < wk.j1; j++, n++) {
-        const int s = n % S::STAGES, r0 = wk.lo + j * OWN_KEYS;
-        if (n >= S::STAGES && !at_wait(&sh.empty[s], (n / S::STAGES - 1) & 1, abort)) {
+        const int s = n % S::STAGES, r0 = wk.lo + j * OWN_KEYS, old = n - S::STAGES;
+        uint64_t* full = &sh.full[n % S::BARS];
+        if (old >= 0 && !at_wait(&sh.empty[old % S::BARS], (old / S::BARS) & 1, abort)) {
           if (lane == 0) fail(400, n);
           ok = false;
           break;
         }
         const int boxes = min(OWN_KEYS, wk.len - r0 + OWN_BOX - 1) / OWN_BOX;   // of each column half of K and V
-        if (lane == 0) mbar_arrive_expect_tx(&sh.full[s], boxes * 2 * (HD / 64) * OWN_BOX * 128);
+        if (lane == 0) mbar_arrive_expect_tx(full, boxes * 2 * (HD / 64) * OWN_BOX * 128);
         __syncwarp();
         if (lane < boxes * 2 * (HD / 64)) {
           const int bx = lane % boxes, h = lane / boxes;   // h: K halves, then V halves
           tma_load_4d(stages + s * S::STAGE + h * S::HALF + bx * OWN_BOX * 128, h < HD / 64 ? &kmap : &vmap, 64 * (h % (HD / 64)),
-                      r0 + bx * OWN_BOX, kh, wk.b, &sh.full[s]);
+                      r0 + bx * OWN_BOX, kh, wk.b, full);
         }
       }
     }
     if (*abort && lane == 0)   // no copy of this CTA may still be in flight
-      for (int i = max(0, n - S::STAGES); i < n; i++) mbar_wait(&sh.full[i % S::STAGES], (i / S::STAGES) & 1);
+      for (int i = max(0, n - S::STAGES); i < n; i++) mbar_wait(&sh.full[i % S::BARS], (i / S::BARS) & 1);
     return;
   }
 
-  const int g = lane >> 2, cc = lane & 3;
-  // this lane's ldmatrix rows within its 16 keys and its 16-byte column
-  const int krow = wid * 16 + (lane & 15), kcol = lane >> 4;                                  // K: rows, then k halves
-  const int vrow = wid * 16 + (lane & 7) + ((lane >> 4) << 3), vcol = (lane >> 3) & 1;        // V: d halves, then rows
+  const int g = lane >> 2, cc = lane & 3, wq = wid & 3;
+  // this lane's ldmatrix row and 16-byte column of the warp's first 16 keys,
+  // for columns 0-15 of each 16: K rows then halves of k, V halves of d then rows
+  const int krow = wq * 32 + (lane & 15), vrow = wq * 32 + (lane & 7) + ((lane >> 4) << 3);
+  uint32_t ko[4], vo[4];   // byte offsets of the four 16-column groups of a half, swizzled
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    ko[k] = krow * 128 + (((k * 2 + (lane >> 4)) ^ (krow & 7)) << 4);
+    vo[k] = vrow * 128 + (((k * 2 + ((lane >> 3) & 1)) ^ (vrow & 7)) << 4);
+  }
   for (wk.start(a, sh.b0, sh.before, x0, x1); wk.more(); wk.next(a)) {
     const int b = wk.b, kh = wk.hk / a.ngc, gc = wk.hk % a.ngc, bk = b * a.KH + kh;
     const int lo = a.window > 0 ? max(0, wk.len - a.window) : 0, hi = wk.len;
@@ -284,52 +299,60 @@ __global__ void __launch_bounds__(OWN_THREADS, 1) own_kernel(const __grid_consta
       for (int k = 0; k < HD / 16; k++) o[t][k][0] = o[t][k][1] = o[t][k][2] = o[t][k][3] = 0.f;
     }
     for (int j = wk.j; j < wk.j1; j++, n++) {
+      if ((n & 1) != wid >> 2) continue;
       const int s = n % S::STAGES, r0 = wk.lo + j * OWN_KEYS;
-      if (!at_wait(&sh.full[s], (n / S::STAGES) & 1, abort)) {
+      if (!at_wait(&sh.full[n % S::BARS], (n / S::BARS) & 1, abort)) {
         if (lane == 0) fail(401, n);
         break;   // on to the barriers below: every wait from here on fails at once
       }
-      const int k0 = r0 + wid * 16;   // this warp's keys k0 .. k0 + 15
+      const int k0 = r0 + wq * 32;   // this warp's keys k0 .. k0 + 31
       if (k0 < hi) {
         const uint32_t kb = smem_u32(stages + s * S::STAGE), vb = kb + (HD / 64) * S::HALF;
-        float x[NT][4];
+        float x[2][NT][4];
 #pragma unroll
-        for (int t = 0; t < NT; t++) x[t][0] = x[t][1] = x[t][2] = x[t][3] = 0.f;
+        for (int u = 0; u < 2; u++)
 #pragma unroll
-        for (int k = 0; k < HD / 16; k++) {
-          uint32_t f[4];
-          ldsm4(f, kb + (k / 4) * S::HALF + krow * 128 + ((((k % 4) * 2 + kcol) ^ (krow & 7)) << 4));
+          for (int t = 0; t < NT; t++) x[u][t][0] = x[u][t][1] = x[u][t][2] = x[u][t][3] = 0.f;
 #pragma unroll
-          for (int t = 0; t < NT; t++) mma16816<T>(x[t], f, qf[t][k][0], qf[t][k][1]);
-        }
-        const bool in0 = k0 + g >= lo && k0 + g < hi, in1 = k0 + g + 8 >= lo && k0 + g + 8 < hi;
-        uint32_t p[NT][2];
+        for (int k = 0; k < HD / 16; k++)
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
+          for (int u = 0; u < 2; u++) {
+            uint32_t f[4];
+            ldsm4(f, kb + (k / 4) * S::HALF + u * 2048 + ko[k % 4]);
 #pragma unroll
-          for (int z = 0; z < 4; z++) x[t][z] = (z < 2 ? in0 : in1) ? x[t][z] * a.c : -INFINITY;
-          if (a.scores) {
-            float* sc = a.scores + ((size_t)bk * a.max_len + k0 + g) * a.gp + (gc * NT + t) * 8 + cc * 2;
-            if ((gc * NT + t) * 8 < a.gp) {
-              if (in0) *reinterpret_cast<float2*>(sc) = make_float2(x[t][0], x[t][1]);
-              if (in1) *reinterpret_cast<float2*>(sc + 8 * a.gp) = make_float2(x[t][2], x[t][3]);
+            for (int t = 0; t < NT; t++) mma16816<T>(x[u][t], f, qf[t][k][0], qf[t][k][1]);
+          }
+        // scores in base 2; -inf outside the sequence's keys
+        const bool whole = k0 >= lo && k0 + 32 <= hi;
+        bool up = false;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          const int ka = k0 + 16 * u + g;
+          const bool in0 = whole || (ka >= lo && ka < hi), in1 = whole || (ka + 8 >= lo && ka + 8 < hi);
+#pragma unroll
+          for (int t = 0; t < NT; t++) {
+#pragma unroll
+            for (int z = 0; z < 4; z++) {
+              x[u][t][z] = (z < 2 ? in0 : in1) ? x[u][t][z] * a.c : -INFINITY;
+              up |= x[u][t][z] > m[t][z & 1] + 8.f;
+            }
+            if (a.scores && (gc * NT + t) * 8 < a.gp) {
+              float* sc = a.scores + ((size_t)bk * a.max_len + ka) * a.gp + (gc * NT + t) * 8 + cc * 2;
+              if (in0) *reinterpret_cast<float2*>(sc) = make_float2(x[u][t][0], x[u][t][1]);
+              if (in1) *reinterpret_cast<float2*>(sc + 8 * a.gp) = make_float2(x[u][t][2], x[u][t][3]);
             }
           }
-          float mn[2];
-          bool up = false;
+        }
+        if (__any_sync(~0u, up)) {
 #pragma unroll
-          for (int z = 0; z < 2; z++) {
-            float v = fmaxf(x[t][z], x[t][z + 2]);
-#pragma unroll
-            for (int sft = 4; sft < 32; sft <<= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, sft));
-            mn[z] = fmaxf(m[t][z], v);
-            up |= mn[z] > m[t][z];
-          }
-          if (__any_sync(~0u, up)) {
+          for (int t = 0; t < NT; t++)
 #pragma unroll
             for (int z = 0; z < 2; z++) {
-              const float f = mn[z] > m[t][z] ? at_exp2(m[t][z] - mn[z]) : 1.f;
-              m[t][z] = mn[z];
+              float v = fmaxf(fmaxf(x[0][t][z], x[0][t][z + 2]), fmaxf(x[1][t][z], x[1][t][z + 2]));
+#pragma unroll
+              for (int sft = 4; sft < 32; sft <<= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, sft));
+              const float mn = fmaxf(m[t][z], v), f = mn > m[t][z] ? at_exp2(m[t][z] - mn) : 1.f;
+              m[t][z] = mn;
               l[t][z] *= f;
 #pragma unroll
               for (int k = 0; k < HD / 16; k++) {
@@ -337,37 +360,45 @@ __global__ void __launch_bounds__(OWN_THREADS, 1) own_kernel(const __grid_consta
                 o[t][k][z + 2] *= f;
               }
             }
-          }
-          float e[4];
-#pragma unroll
-          for (int z = 0; z < 4; z++) {
-            const float mz = m[t][z & 1];
-            e[z] = at_exp2(x[t][z] - (mz == -INFINITY ? 0.f : mz));
-            l[t][z & 1] += e[z];
-          }
-          p[t][0] = movm(at_pack<T>(e[0], e[1]));
-          p[t][1] = movm(at_pack<T>(e[2], e[3]));
         }
+        uint32_t p[2][NT][2];
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int t = 0; t < NT; t++) {
+            float e[4];
+#pragma unroll
+            for (int z = 0; z < 4; z++) {
+              const float mz = m[t][z & 1];
+              e[z] = at_exp2(x[u][t][z] - (mz == -INFINITY ? 0.f : mz));
+              l[t][z & 1] += e[z];
+            }
+            p[u][t][0] = movm(at_pack<T>(e[0], e[1]));
+            p[u][t][1] = movm(at_pack<T>(e[2], e[3]));
+          }
         // V rows outside [lo, hi) may hold anything, infinities and NaN too:
         // their bits are cleared (a register has two keys of one dimension)
-        const bool whole = k0 >= lo && k0 + 16 <= hi;
-        uint32_t vm[2];
+        uint32_t vm[2][2];
 #pragma unroll
-        for (int z = 0; z < 2; z++) {
-          const int kk = k0 + z * 8 + cc * 2;
-          vm[z] = (kk >= lo && kk < hi ? 0x0000ffffu : 0u) | (kk + 1 >= lo && kk + 1 < hi ? 0xffff0000u : 0u);
-        }
+        for (int u = 0; u < 2; u++)
 #pragma unroll
-        for (int k = 0; k < HD / 16; k++) {
-          uint32_t f[4];
-          ldsm4t(f, vb + (k / 4) * S::HALF + vrow * 128 + ((((k % 4) * 2 + vcol) ^ (vrow & 7)) << 4));
-          if (!whole) f[0] &= vm[0], f[1] &= vm[0], f[2] &= vm[1], f[3] &= vm[1];
+          for (int z = 0; z < 2; z++) {
+            const int kk = k0 + 16 * u + z * 8 + cc * 2;
+            vm[u][z] = (kk >= lo && kk < hi ? 0x0000ffffu : 0u) | (kk + 1 >= lo && kk + 1 < hi ? 0xffff0000u : 0u);
+          }
 #pragma unroll
-          for (int t = 0; t < NT; t++) mma16816<T>(o[t][k], f, p[t][0], p[t][1]);
-        }
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int k = 0; k < HD / 16; k++) {
+            uint32_t f[4];
+            ldsm4t(f, vb + (k / 4) * S::HALF + u * 2048 + vo[k % 4]);
+            if (!whole) f[0] &= vm[u][0], f[1] &= vm[u][0], f[2] &= vm[u][1], f[3] &= vm[u][1];
+#pragma unroll
+            for (int t = 0; t < NT; t++) mma16816<T>(o[t][k], f, p[u][t][0], p[u][t][1]);
+          }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.empty[s]);
+      if (lane == 0) mbar_arrive(&sh.empty[n % S::BARS]);
     }
     // join the warps, 8 heads at a time
 #pragma unroll
@@ -381,7 +412,7 @@ __global__ void __launch_bounds__(OWN_THREADS, 1) own_kernel(const __grid_consta
 #pragma unroll
       for (int k = 0; k < HD / 16; k++)
 #pragma unroll
-        for (int z = 0; z < 4; z++) red[(wid * 8 + cc * 2 + (z & 1)) * HD + k * 16 + g + (z >> 1) * 8] = o[t][k][z];
+        for (int z = 0; z < 4; z++) red[(wid * 8 + cc * 2 + (z & 1)) * S::RP + k * 16 + g + (z >> 1) * 8] = o[t][k][z];
       asm volatile("bar.sync 1, 256;" ::: "memory");
       for (int i = tid; i < 8 * HD; i += OWN_WARPS * 32) {
         const int h = i / HD, d = i % HD;
@@ -394,7 +425,7 @@ __global__ void __launch_bounds__(OWN_THREADS, 1) own_kernel(const __grid_consta
           if (ml.y == 0.f) continue;   // a warp without keys
           const float f = at_exp2(ml.x - M);
           L = fmaf(ml.y, f, L);
-          v = fmaf(red[(w * 8 + h) * HD + d], f, v);
+          v = fmaf(red[(w * 8 + h) * S::RP + d], f, v);
         }
         const size_t at = seg * (8 * NT) + t * 8 + h;
         a.po[at * HD + d] = v;
@@ -417,17 +448,17 @@ struct JoinArgs {
 };
 
 constexpr int JOIN_THREADS = 256;
-constexpr int JOIN_KEYS = 512;   // own positions whose weights one block adds
+constexpr int JOIN_KEYS = 2048;  // own positions whose weights one block adds
 
-// Block (b KH + kh, part): part 0 the outputs, a warp per head; the others
-// the weights of JOIN_KEYS own positions each.
+// Block (b KH + kh, part): the weights of JOIN_KEYS own positions, and in part
+// 0 the outputs, a warp per head.
 template <typename T, int HD>
 __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
   __shared__ float2 fin[AT_ROWS];   // per head: M, 1 / the sum
   pdl_wait();
   const int bk = blockIdx.x, kh = bk % a.KH, b = bk / a.KH, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const int len = own_len(a.lens, b, a.max_len), lo = a.window > 0 ? max(0, len - a.window) : 0;
-  const int j0 = ((int)blockIdx.y - 1) * JOIN_KEYS;
+  const int j0 = (int)blockIdx.y * JOIN_KEYS;
   if (blockIdx.y > 0 && (j0 >= len || j0 + JOIN_KEYS <= lo)) return;
   const int ub = b / (2 * a.tpt), r = b % (2 * a.tpt), t = r / a.tpt, tok = r % a.tpt;
   const int HK = a.KH * a.ngc, n = a.own_ctas ? own_stages(len, a.window) : 0;
@@ -455,7 +486,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
     if (blockIdx.y == 0)
       join_row<T, HD>(pieces, a.pml, a.po, f, row, (T*)a.out + b * a.so[0] + (kh * a.G + g) * a.so[1], a.hd);
   }
-  if (blockIdx.y == 0) return;
+  if (!a.weights) return;
   __syncthreads();
   float* w = a.weights + b * a.sw[0] + kh * a.sw[1];
   for (int j = max(j0, lo) + tid; j < min(len, j0 + JOIN_KEYS); j += JOIN_THREADS) {
@@ -548,7 +579,7 @@ static cudaError_t run_shared(const CUtensorMap* m, AttnTcArgs ta, int pieces, c
     count_launches(1);
   }
   if (e == cudaSuccess) {
-    const dim3 grid(ja.B * ja.KH, 1 + (ja.weights ? (ja.max_len + JOIN_KEYS - 1) / JOIN_KEYS : 0));
+    const dim3 grid(ja.B * ja.KH, ja.weights ? std::max(1, (ja.max_len + JOIN_KEYS - 1) / JOIN_KEYS) : 1);
     e = launch_pdl(join_kernel<T, HD>, grid, JOIN_THREADS, 0, s, ja);
     count_launches(1);
   }

@@ -183,12 +183,6 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
 __device__ __forceinline__ void at_store8(void* p, const uint32_t* r) {
   asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), AT_W4(r, 0), AT_W4(r, 4) : "memory");
 }
-// The thread's number, read anew: nothing computed from it stays in registers.
-__device__ __forceinline__ int at_tid() {
-  int x;
-  asm volatile("mov.u32 %0, %%tid.x;" : "=r"(x));
-  return x;
-}
 __device__ __forceinline__ float at_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -261,12 +255,16 @@ struct AttnTcShape {
   // products are half as long, 117, 106 and 107 us at 4,096).
   static constexpr int POLY_OF = HD == 128 ? 8 : 4;
   static constexpr int NQ = HD == 128 ? 1 : 2;            // units whose Q is there or on its way
-  static constexpr int STAGES = HD == 128 ? 5 : 8;        // K and V blocks in flight
+  static constexpr int STAGES = HD == 128 ? 5 : 8;        // K and V blocks in flight, in turn
+  // Their barriers: an even number, so that each is K's or V's alone and its
+  // waiter sees every phase (a wait by parity passes if the barrier is a whole
+  // phase behind).
+  static constexpr int BARS = STAGES % 2 ? 2 * STAGES : STAGES;
   static constexpr int SMEM = (2 * NQ + STAGES) * TILE + 1024;
 };
 
 struct AttnTcShared {
-  uint64_t q_full[2], q_empty[2], kv_full[8], kv_empty[8], s_full[2], s_loaded[2], p_full[2], p_empty[2], unit_full[AT_UNITS],
+  uint64_t q_full[2], q_empty[2], kv_full[10], kv_empty[10], s_full[2], s_loaded[2], p_full[2], p_empty[2], unit_full[AT_UNITS],
       unit_empty[AT_UNITS], aux, drain[2];
   AttnEntry unit[AT_UNITS];
   int unit_kh[AT_UNITS];      // -1: no more work
@@ -289,7 +287,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
                                                                 const __grid_constant__ CUtensorMap kmap,
                                                                 const __grid_constant__ CUtensorMap vmap, const AttnTcArgs a) {
   using S = AttnTcShape<HD>;
-  constexpr int NST = S::STAGES, TILE = S::TILE, NQ = S::NQ, W0 = AT_SOFT;
+  constexpr int NST = S::STAGES, NBAR = S::BARS, TILE = S::TILE, NQ = S::NQ, W0 = AT_SOFT;
   // tensor memory: S buffers of 128 columns, P of 64 for each tile, O of HD for each
   constexpr int NS = HD == 128 ? 1 : 2, TM_P = NS * AT_KEYS, TM_O = TM_P + AT_KEYS;
   extern __shared__ uint8_t dsm[];
@@ -304,7 +302,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   if (tid == W0 * 32 + 32) {
-    for (int i = 0; i < NST; i++) {
+    for (int i = 0; i < NBAR; i++) {
       mbar_init(&sh.kv_full[i], 1);
       mbar_init(&sh.kv_empty[i], 1);
     }
@@ -445,7 +443,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
       for (int i = 0; i < 2 * e.nb; i++) {
         const int s = issued % NST, row = e.ks + (i >> 1) * AT_KEYS;
         const bool v = i & 1;
-        if (issued >= NST && !at_wait(&sh.kv_empty[s], (issued / NST - 1) & 1, abort)) {
+        const int old = issued - NST;   // the block that was there before
+        if (old >= 0 && !at_wait(&sh.kv_empty[old % NBAR], (old / NBAR) & 1, abort)) {
           if (lane == 0) fail(303, it);
           ok = false;
           break;
@@ -456,7 +455,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
         // (Keys need nothing: their scores are replaced.)
         const int end = e.nk - row;
         const bool fix = v && end < AT_KEYS && e.k0 + e.nk < a.total_k;
-        uint64_t* bar = fix ? &sh.aux : &sh.kv_full[s];
+        uint64_t* full = &sh.kv_full[issued % NBAR];
+        uint64_t* bar = fix ? &sh.aux : full;
         if (lane == 0) {
           mbar_arrive_expect_tx(bar, TILE);
           for (int c = 0; c < HD / 64; c++)
@@ -474,13 +474,13 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
               reinterpret_cast<uint4*>(dst + c * 16384)[o] = make_uint4(0, 0, 0, 0);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.kv_full[s]);
+          if (lane == 0) mbar_arrive(full);
         }
         issued++;
       }
     }
     if (*abort && lane == 0) {   // no copy of this CTA may still be in flight
-      for (int i = max(0, issued - NST); i < issued; i++) mbar_wait(&sh.kv_full[i % NST], (i / NST) & 1);
+      for (int i = max(0, issued - NST); i < issued; i++) mbar_wait(&sh.kv_full[i % NBAR], (i / NBAR) & 1);
       for (int i = max(0, qn - NQ); i < qn; i++) mbar_wait(&sh.q_full[i % NQ], (i / NQ) & 1);
     }
   } else if (wid == W0 + 1 || wid == W0 + 2) {
@@ -503,7 +503,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
           if (s >= n) s -= n, ph ^= 1;
         }
       };
-      Ring unit{0, 0}, qr{0, 0}, kv{wid == W0 + 1 ? 0u : 1u, 0};   // kv: K and V take turns
+      Ring unit{0, 0}, qr{0, 0}, kv{wid == W0 + 1 ? 0u : 1u, 0};   // kv: the barrier; K and V take turns
       // Parities of the tiles' S (or P), a bit each (an indexed array would
       // live in local memory).
       uint32_t bits = 0, last = 0;
@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
           if (!wait(&sh.q_full[qr.s], qr.ph, 310)) break;
           for (int j = 0; j < nb && ok; j++) {
             if (!wait(&sh.kv_full[kv.s], kv.ph, 311)) break;
-            const uint64_t bk = dk + kv.s * (TILE / 16);
+            const uint64_t bk = dk + (kv.s < NST ? kv.s : kv.s - NST) * (TILE / 16);
             for (uint32_t t = 0; t < ntile; t++) {
               // The buffer is free once the softmax has loaded what was in it
               // (a barrier's phase before its first counts as complete).
@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
               last = t;
             }
             at_commit(&sh.kv_empty[kv.s]);
-            kv.add(2, NST);
+            kv.add(2, NBAR);
           }
           if (!ok) break;
           at_commit(&sh.q_empty[qr.s]);
@@ -549,7 +549,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
           const uint64_t dv = desc_mnmajor(smem_u32(kvs));
           for (int j = 0; j < nb && ok; j++) {
             if (!wait(&sh.kv_full[kv.s], kv.ph, 313)) break;
-            const uint64_t bv = dv + kv.s * (TILE / 16);
+            const uint64_t bv = dv + (kv.s < NST ? kv.s : kv.s - NST) * (TILE / 16);
             for (uint32_t t = 0; t < ntile; t++) {
               const uint32_t d = tmem + TM_O + t * HD, pa = tmem + TM_P + t * (AT_KEYS / 2), par = bits >> t;
               if (!wait(&sh.p_full[t], par, 315)) break;
@@ -561,12 +561,12 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
               bits ^= 1u << t;
             }
             at_commit(&sh.kv_empty[kv.s]);
-            kv.add(2, NST);
+            kv.add(2, NBAR);
           }
           if (!ok) break;
         }
       }
-      if (*abort && issued) {   // no MMA of this CTA may still be in flight
+      if (issued) {   // no product or commit of this CTA may still be in flight at its end
         at_commit(&sh.drain[wid - W0 - 1]);
         mbar_wait(&sh.drain[wid - W0 - 1], 0);
       }
@@ -582,6 +582,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
     const uint32_t lanes = tmem + ((uint32_t)(wid & 3) << 21);
     const uint32_t ts = lanes + (NS == 1 ? 0 : t * AT_KEYS), tp = lanes + TM_P + t * (AT_KEYS / 2), to = lanes + TM_O + t * HD;
     const float c = a.c;
+    const int tok = (tid & 127) / a.G, g = (tid & 127) - tok * a.G;   // the row's token and query head
     uint32_t par = 0;   // blocks so far, modulo 2
     for (;; un++) {
       const volatile AttnEntry* e = &sh.unit[un % AT_UNITS];   // handed back at the unit's end
@@ -597,7 +598,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
       bool valid = false, ok = true;
       const bool mine = t * a.tpt < e->ntok;         // the tile has rows
       if (mine) {
-        const int x = at_tid(), tok = (x & 127) / a.G, tt = (x >> 7) * a.tpt + tok;
+        const int tt = t * a.tpt + tok;
         valid = tok < a.tpt && tt < e->ntok;
         if (SHARED) {
           hi = a.P;
@@ -605,7 +606,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
         } else {
           hi = e->p0 + tt + 1;
           if (a.window > 0) lo = max(0, hi - a.window);
-          if (a.sinks && valid && e->slot < 0) sink = a.sinks[sh.unit_kh[un % AT_UNITS] * a.G + (x & 127) - tok * a.G];   // used at the end
+          if (a.sinks && valid && e->slot < 0) sink = a.sinks[sh.unit_kh[un % AT_UNITS] * a.G + g];   // used at the end
         }
         lo0 = __reduce_min_sync(~0u, valid ? lo : AT_NPOS), hi1 = __reduce_max_sync(~0u, valid ? hi : 0);
         lo1 = __reduce_max_sync(~0u, valid ? lo : 0), hi0 = __reduce_min_sync(~0u, valid ? hi : AT_NPOS);
@@ -631,15 +632,16 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
         const int base = e->ks + j * AT_KEYS;
         unsigned dead = 0;
         const bool clean = base >= lo1 && base + AT_KEYS <= hi0;
-        if (!clean) {
+        float mx[4] = {m, m, m, m};
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const int cb = base + 32 * i;
+        for (int i = 0; i < 4; i++) {
+          const int cb = base + 32 * i;
+          if (!clean) {
             if (cb >= hi1 || cb + 32 <= lo0) {
               dead |= 1u << i;
-#pragma unroll
-              for (int q = 0; q < 32; q++) s[32 * i + q] = -INFINITY;
-            } else if (cb < lo1 || cb + 32 > hi0) {
+              continue;
+            }
+            if (cb < lo1 || cb + 32 > hi0) {
               const int l0 = lo - cb, h0 = hi - cb;
               unsigned see = h0 >= 32 ? ~0u : h0 <= 0 ? 0u : (1u << h0) - 1;
               see &= l0 <= 0 ? ~0u : l0 >= 32 ? 0u : ~0u << l0;
@@ -647,17 +649,12 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
               for (int q = 0; q < 32; q++) s[32 * i + q] = see & (1u << q) ? s[32 * i + q] : -INFINITY;
             }
           }
+#pragma unroll
+          for (int q = 0; q < 32; q += 8)
+#pragma unroll
+            for (int z = 0; z < 4; z++) mx[z] = at_max3(mx[z], s[32 * i + q + z], s[32 * i + q + z + 4]);
         }
-        float mx[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) mx[i] = at_max3(s[i], s[i + 4], s[i + 8]);
-#pragma unroll
-        for (int i = 12; i < AT_KEYS - 4; i += 8)
-#pragma unroll
-          for (int q = 0; q < 4; q++) mx[q] = at_max3(mx[q], s[i + q], s[i + q + 4]);
-#pragma unroll
-        for (int q = 0; q < 4; q++) mx[q] = fmaxf(mx[q], s[AT_KEYS - 4 + q]);
-        const float mn = fmaxf(at_max3(m, mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         // P V of the block before: its P may be overwritten, its O scaled (a
         // barrier's phase before its first counts as complete)
         if (!at_wait(&sh.p_empty[t], (par & 1) ^ 1, abort)) {
@@ -746,19 +743,19 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
           }
           at_fence_after();
         }
-        const int x = at_tid(), tok = (x & 127) / a.G, g = (x & 127) - tok * a.G, kh = *(volatile int*)&sh.unit_kh[un % AT_UNITS];
+        const int kh = *(volatile int*)&sh.unit_kh[un % AT_UNITS];
         const int slot = e->slot;
         const bool part = SHARED || slot >= 0;
         float inv = 1.f;
         char* at;   // this thread's outputs, or its part of the partial result
         if (part) {
-          const size_t pr = ((size_t)slot * a.KH + kh) * (2 * AT_ROWS) + x;
+          const size_t pr = ((size_t)slot * a.KH + kh) * (2 * AT_ROWS) + tid;
           if (valid) a.pml[pr] = make_float2(l == 0.f ? -INFINITY : c * m, l);
           at = (char*)(a.po + pr * HD);
         } else {
           if (l != 0.f) l += at_exp2(fmaf(sink, LOG2E, -c * m));
           inv = l == 0.f ? 0.f : 1.f / l;
-          at = (char*)((T*)a.out + (e->q0 + (x >> 7) * a.tpt + tok) * a.so[0] + (kh * a.G + g) * a.so[1]);
+          at = (char*)((T*)a.out + (e->q0 + t * a.tpt + tok) * a.so[0] + (kh * a.G + g) * a.so[1]);
         }
 #pragma unroll
         for (int i = 0; i < HD / 32; i++) {
