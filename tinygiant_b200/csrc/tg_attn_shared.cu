@@ -35,7 +35,10 @@
 namespace tg {
 
 constexpr int OWN_KEYS = 128;       // keys per stage: 32 for each warp of a group
-constexpr int OWN_BOX = 32;         // rows per TMA box: a sequence's last stage reads at most 31 rows too many
+// Rows per TMA box: whole stages come in boxes of 128 rows, a sequence's last
+// 64 rows and less in boxes of 32 (a box takes about 85 clocks to issue: with
+// 16 boxes of 32 rows in every stage the issuing bound an SM to 46 GB/s).
+constexpr int OWN_BOX = 32;
 constexpr int OWN_WARPS = 8;        // two groups of four that take stages in turn
 constexpr int OWN_THREADS = (OWN_WARPS + 1) * 32;
 
@@ -165,7 +168,9 @@ struct OwnWalk {
 // the figure below of GB/s.
 template <typename T, int HD, int NT>
 __global__ void __launch_bounds__(OWN_THREADS, 1) own_kernel(const __grid_constant__ CUtensorMap kmap,
-                                                             const __grid_constant__ CUtensorMap vmap, const OwnArgs a) {
+                                                             const __grid_constant__ CUtensorMap vmap,
+                                                             const __grid_constant__ CUtensorMap kend,
+                                                             const __grid_constant__ CUtensorMap vend, const OwnArgs a) {
   using S = OwnShape<HD>;
   extern __shared__ uint8_t dsm[];
   __shared__ OwnShared sh;
@@ -247,13 +252,14 @@ __global__ void __launch_bounds__(OWN_THREADS, 1) own_kernel(const __grid_consta
           ok = false;
           break;
         }
-        const int boxes = min(OWN_KEYS, wk.len - r0 + OWN_BOX - 1) / OWN_BOX;   // of each column half of K and V
-        if (lane == 0) mbar_arrive_expect_tx(full, boxes * 2 * (HD / 64) * OWN_BOX * 128);
+        const bool all = wk.len - r0 > OWN_KEYS / 2;
+        const int rows = all ? OWN_KEYS : OWN_BOX, boxes = all ? 1 : (wk.len - r0 + OWN_BOX - 1) / OWN_BOX;   // of each column half of K and V
+        if (lane == 0) mbar_arrive_expect_tx(full, boxes * 2 * (HD / 64) * rows * 128);
         __syncwarp();
         if (lane < boxes * 2 * (HD / 64)) {
           const int bx = lane % boxes, h = lane / boxes;   // h: K halves, then V halves
-          tma_load_4d(stages + s * S::STAGE + h * S::HALF + bx * OWN_BOX * 128, h < HD / 64 ? &kmap : &vmap, 64 * (h % (HD / 64)),
-                      r0 + bx * OWN_BOX, kh, wk.b, full);
+          const CUtensorMap* map = h < HD / 64 ? (all ? &kmap : &kend) : (all ? &vmap : &vend);
+          tma_load_4d(stages + s * S::STAGE + h * S::HALF + bx * OWN_BOX * 128, map, 64 * (h % (HD / 64)), r0 + bx * OWN_BOX, kh, wk.b, full);
         }
       }
     }
@@ -549,7 +555,7 @@ struct SharedSpace {
 };
 
 template <typename T, int HD, int NT>
-static cudaError_t launch_own(const CUtensorMap& k, const CUtensorMap& v, const OwnArgs& a, int grid, cudaStream_t s) {
+static cudaError_t launch_own(const CUtensorMap* m, const OwnArgs& a, int grid, cudaStream_t s) {
   const int smem = OwnShape<HD>::SMEM;
   static std::atomic<unsigned long long> set{0};   // devices whose limit is raised
   int dev = 0;
@@ -559,7 +565,7 @@ static cudaError_t launch_own(const CUtensorMap& k, const CUtensorMap& v, const 
     if (e == cudaSuccess && dev < 64) set |= 1ull << dev;
   }
   if (e != cudaSuccess) return e;
-  return launch_pdl(own_kernel<T, HD, NT>, dim3(grid), OWN_THREADS, smem, s, k, v, a);
+  return launch_pdl(own_kernel<T, HD, NT>, dim3(grid), OWN_THREADS, smem, s, m[0], m[1], m[2], m[3], a);
 }
 
 // The own keys' kernel goes first and lets the prefix start beside it at once;
@@ -570,7 +576,7 @@ template <typename T, int HD>
 static cudaError_t run_shared(const CUtensorMap* m, AttnTcArgs ta, int pieces, const OwnArgs& oa, const JoinArgs& ja, cudaStream_t s) {
   cudaError_t e = cudaSuccess;
   if (ja.own_ctas > 0) {
-    e = ja.nt == 1 ? launch_own<T, HD, 1>(m[3], m[4], oa, ja.own_ctas, s) : launch_own<T, HD, 2>(m[3], m[4], oa, ja.own_ctas, s);
+    e = ja.nt == 1 ? launch_own<T, HD, 1>(m + 3, oa, ja.own_ctas, s) : launch_own<T, HD, 2>(m + 3, oa, ja.own_ctas, s);
     count_launches(1);
   }
   ta.beside = ja.own_ctas > 0;
@@ -649,7 +655,7 @@ extern "C" int tg_attention_shared(int dtype, const void* q, const void* prefix_
   JoinArgs j{lens, starts, sinks, weights, a.po, o.scores, a.pml, out, {t[12], t[13]},
              {weights ? strides[14] : 0, weights ? strides[15] : 0}, sp.own_row, batch, n_kv_heads, G, sp.gp, head_dim, sp.tpt, sp.nsp,
              max_len, window, sp.ngc, sp.nt, sp.own_ctas};
-  CUtensorMap m[5];
+  CUtensorMap m[7];
   bool maps = true;
   int pieces = 0;
   if (prefix_len > 0) {
@@ -659,8 +665,11 @@ extern "C" int tg_attention_shared(int dtype, const void* q, const void* prefix_
            attn_kv_map(&m[2], dtype, prefix_v, q, head_dim, n_kv_heads, prefix_len, t[5], t[4]);
   }
   if (max_len > 0)
-    maps = maps && attn_cache_map(&m[3], dtype, k, head_dim, cap, n_kv_heads, batch, t[8], t[7], t[6], OWN_BOX) &&
-           attn_cache_map(&m[4], dtype, v, head_dim, cap, n_kv_heads, batch, t[11], t[10], t[9], OWN_BOX);
+    for (int i = 0; i < 2; i++) {
+      const int rows = i ? OWN_BOX : OWN_KEYS;
+      maps = maps && attn_cache_map(&m[3 + 2 * i], dtype, k, head_dim, cap, n_kv_heads, batch, t[8], t[7], t[6], rows) &&
+             attn_cache_map(&m[4 + 2 * i], dtype, v, head_dim, cap, n_kv_heads, batch, t[11], t[10], t[9], rows);
+    }
   c.need(maps, "the tensors' shapes and strides do not fit a tensor map");
   if (c.rc) return c.rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
