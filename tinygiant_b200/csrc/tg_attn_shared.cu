@@ -162,10 +162,8 @@ struct OwnWalk {
 // segments.  Warps 0-3 and 4-7 take stages in turn, each warp 32 keys with a
 // reference m of its own (moved, as in attn_tc_kernel, only when a score
 // exceeds it by 8 in base 2: one vote in the common case); the warps' partial
-// results join in shared memory at the end of a segment.  A step's latencies
-// (matrix loads, dependent products, exponentials) are what a warp waits for:
-// two tiles of 16 keys in flight and two groups of warps took an SM from 46 to
-// the figure below of GB/s.
+// results join in shared memory at the end of a segment.  Bound by HBM: 442 MB
+// in 76 us on all SMs (batch 256, 768 keys on average), 0.89 of measured.
 template <typename T, int HD, int NT>
 __global__ void __launch_bounds__(OWN_THREADS, 1) own_kernel(const __grid_constant__ CUtensorMap kmap,
                                                              const __grid_constant__ CUtensorMap vmap,
@@ -524,9 +522,11 @@ struct SharedSpace {
     gp = (G + 7) / 8 * 8;
     const int blocks = (P + AT_KEYS - 1) / AT_KEYS;
     const long long HK = (long long)KH * ngc, stages = (long long)B * HK * ((max_len + OWN_KEYS - 1) / OWN_KEYS);
-    // The SMs' shares, by the time one SM would take: a block of two tiles of
-    // the prefix about 2 us at head_dim 128, a stage of own keys 0.65 us.
-    const double tp = 2.0 * units * KH * blocks, to = 0.65 * stages;
+    // The SMs' shares, by the time that one SM takes: a block of two tiles of
+    // the prefix about 2 us at head_dim 128, a stage of own keys (64 KB, at the
+    // 54 GB/s that an SM loads) 1.1 us.  Batch 256 on 16,384 keys with up to
+    // 1,024 own ones: 138 us at 80 CTAs for these, 156 at 60, 154 at 148.
+    const double tp = 2.0 * units * KH * blocks, to = 1.1 * stages;
     own_ctas = 0;
     if (max_len > 0) {
       own_ctas = blocks ? std::max(1, std::min(sms - 1, (int)(sms * to / (to + tp) + 0.5))) : sms;

@@ -7,17 +7,21 @@
 // keeps its order.  Weights compare as numbers (-0 equals 0), NaN above all.
 //
 // select_kernel, a block per (sequence, key head), finds the threshold (the
-// (m - r)-th largest weight) by three radix passes of 11, 11 and 10 bits over
-// the weights' order-preserving integers, then one pass in position order
-// that numbers what stays.  gather_kernel moves the rows.
+// (m - r)-th largest weight) by radix passes of 11, 11 and 10 bits over the
+// weights' order-preserving integers, kept in shared memory where they fit,
+// then numbers what stays in position order: counts by ballot for every 32
+// positions, one prefix sum over the warps.  gather_kernel moves the rows:
+// bound by HBM, 2 rows read and written per position.
 #include <algorithm>
 
 #include "../../include/tinygiant.h"
-#include "tg_attn.h"
+#include "tg_attn_tc.cuh"
 
 namespace tg {
 
-constexpr int EV_THREADS = 512;
+constexpr int EV_THREADS = 1024;
+constexpr int EV_WARPS = EV_THREADS / 32;
+constexpr int EV_CACHED = 40960;   // weights of a row kept in shared memory, at most (160 KB)
 
 struct EvictArgs {
   const uint4 *k, *v;
@@ -49,79 +53,28 @@ __device__ __forceinline__ int block_excl_sum(int v, int* red, int* total) {
   __syncthreads();
   if (lane == 31) red[w] = x;
   __syncthreads();
-  int base = 0, sum = 0;
-  for (int i = 0; i < EV_THREADS / 32; i++) {
-    if (i < w) base += red[i];
-    sum += red[i];
-  }
-  *total = sum;
+  const int mine = red[lane];   // EV_WARPS = 32
+  const int base = __reduce_add_sync(~0u, lane < w ? mine : 0);
+  *total = __reduce_add_sync(~0u, mine);
   return base + x - v;
 }
 
-__global__ void __launch_bounds__(EV_THREADS) select_kernel(const EvictArgs a) {
+// keys(i): the order key of position i, from shared memory if `cached`.
+__global__ void __launch_bounds__(EV_THREADS) select_kernel(const EvictArgs a, int cached) {
+  static_assert(EV_WARPS == 32, "block_excl_sum");
+  extern __shared__ uint32_t sk[];
   __shared__ int hist[2048];
-  __shared__ int red[EV_THREADS / 32];
+  __shared__ int red[EV_WARPS];
   __shared__ uint32_t s_bin;
   __shared__ int s_need;
-  const int t = threadIdx.x, b = blockIdx.x / a.KH, h = blockIdx.x % a.KH;
+  pdl_trigger();
+  const int t = threadIdx.x, lane = t & 31, wp = t >> 5, b = blockIdx.x / a.KH, h = blockIdx.x % a.KH;
   const int n = min(max(a.lens[b], 0), a.cap), m = min(n, a.keep), r = min(a.recent, m);
   const float* w = a.w + b * a.sw[0] + h * a.sw[1];
   int* idx = a.idx + (size_t)blockIdx.x * a.keep;
   float* wo = a.wo + (size_t)blockIdx.x * a.keep;
   if (h == 0 && t == 0) a.lens_out[b] = m;
   const int cand = n - r, want = m - r;       // want <= cand
-  uint32_t thr = 0;                           // keys above thr stay, and need of those equal to it
-  int need = want;
-  if (want > 0 && want < cand) {
-    int shift = 32;
-    for (int pass = 0; pass < 3; pass++) {
-      const int bits = pass < 2 ? 11 : 10;
-      shift -= bits;
-      for (int i = t; i < 2048; i += EV_THREADS) hist[i] = 0;
-      __syncthreads();
-      for (int i = t; i < cand; i += EV_THREADS) {
-        const uint32_t u = order_key(w[i]);
-        if (pass == 0 || (u >> (shift + bits)) == (thr >> (shift + bits))) atomicAdd(&hist[(u >> shift) & ((1 << bits) - 1)], 1);
-      }
-      __syncthreads();
-      // the bin, from the top, in which the need-th key lies
-      const int nb = 1 << bits, per = nb / EV_THREADS;   // 4 or 2 bins a thread
-      int c = 0;
-      for (int i = 0; i < per; i++) c += hist[nb - 1 - (t * per + i)];
-      int total;
-      int above = block_excl_sum(c, red, &total);
-      if (above < need && above + c >= need)
-        for (int i = 0; i < per; i++) {
-          const int bin = nb - 1 - (t * per + i);
-          if (above + hist[bin] >= need) {
-            s_bin = bin;
-            s_need = need - above;
-            break;
-          }
-          above += hist[bin];
-        }
-      __syncthreads();
-      thr |= s_bin << shift;
-      need = s_need;
-      __syncthreads();
-    }
-  }
-  int kept = 0, equal = 0;
-  for (int i0 = 0; i0 < cand && want > 0; i0 += EV_THREADS) {
-    const int i = i0 + t;
-    const float x = i < cand ? w[i] : 0.f;
-    const uint32_t u = order_key(x);
-    int eq = want < cand && i < cand && u == thr, sum;
-    const int er = equal + block_excl_sum(eq, red, &sum);
-    equal += sum;
-    const int stay = i < cand && (want == cand || u > thr || (eq && er < need));
-    const int at = kept + block_excl_sum(stay, red, &sum);
-    kept += sum;
-    if (stay) {
-      idx[at] = i;
-      wo[at] = x;
-    }
-  }
   for (int i = t; i < r; i += EV_THREADS) {
     idx[want + i] = cand + i;
     wo[want + i] = w[cand + i];
@@ -130,11 +83,89 @@ __global__ void __launch_bounds__(EV_THREADS) select_kernel(const EvictArgs a) {
     idx[i] = -1;
     wo[i] = 0.f;
   }
+  if (want == 0) return;
+  if (want == cand) {   // all of them
+    for (int i = t; i < cand; i += EV_THREADS) {
+      idx[i] = i;
+      wo[i] = w[i];
+    }
+    return;
+  }
+  auto key = [&](int i) { return cached ? sk[i] : order_key(w[i]); };
+  uint32_t thr = 0;                           // keys above thr stay, and need of those equal to it
+  int need = want, shift = 32;
+  for (int pass = 0; pass < 3; pass++) {
+    const int bits = pass < 2 ? 11 : 10;
+    shift -= bits;
+    for (int i = t; i < 2048; i += EV_THREADS) hist[i] = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (int i = t; i < cand; i += EV_THREADS) {
+      uint32_t u;
+      if (pass == 0) {
+        u = order_key(w[i]);
+        if (cached) sk[i] = u;
+      } else {
+        u = key(i);
+      }
+      if (pass == 0 || (u >> (shift + bits)) == (thr >> (shift + bits))) atomicAdd(&hist[(u >> shift) & ((1 << bits) - 1)], 1);
+    }
+    __syncthreads();
+    // the bin, from the top, in which the need-th key lies
+    const int nb = 1 << bits, per = nb / EV_THREADS;   // 2 bins a thread, or 1
+    int c = 0;
+    for (int i = 0; i < per; i++) c += hist[nb - 1 - (t * per + i)];
+    int total;
+    int above = block_excl_sum(c, red, &total);
+    if (above < need && above + c >= need)
+      for (int i = 0; i < per; i++) {
+        const int bin = nb - 1 - (t * per + i);
+        if (above + hist[bin] >= need) {
+          s_bin = bin;
+          s_need = need - above;
+          break;
+        }
+        above += hist[bin];
+      }
+    __syncthreads();
+    thr |= s_bin << shift;
+    need = s_need;
+  }
+  // Each warp has a run of whole 32s; the numbers of kept keys before it, and
+  // of keys equal to the threshold, whose first `need` stay, by prefix sums.
+  const int groups = (cand + 31) / 32, per = (groups + EV_WARPS - 1) / EV_WARPS;
+  const int g0 = min(groups, wp * per), g1 = min(groups, g0 + per);
+  int above = 0, equal = 0;
+  for (int g = g0; g < g1; g++) {
+    const int i = g * 32 + lane;
+    const uint32_t u = i < cand ? key(i) : 0;
+    above += __popc(__ballot_sync(~0u, i < cand && u > thr));
+    equal += __popc(__ballot_sync(~0u, i < cand && u == thr));
+  }
+  int total;
+  const int eq0 = __shfl_sync(~0u, block_excl_sum(lane == 0 ? equal : 0, red, &total), 0);
+  const int ab0 = __shfl_sync(~0u, block_excl_sum(lane == 0 ? above : 0, red, &total), 0);
+  int at = ab0 + min(eq0, need), eqs = eq0;   // kept before this warp's run; equal ones before it
+  for (int g = g0; g < g1; g++) {
+    const int i = g * 32 + lane;
+    const uint32_t u = i < cand ? key(i) : 0;
+    const unsigned before = (1u << lane) - 1, em = __ballot_sync(~0u, i < cand && u == thr);
+    const bool stay = i < cand && (u > thr || (u == thr && eqs + __popc(em & before) < need));
+    const unsigned sm = __ballot_sync(~0u, stay);
+    if (stay) {
+      const int o = at + __popc(sm & before);
+      idx[o] = i;
+      wo[o] = w[i];
+    }
+    at += __popc(sm);
+    eqs += __popc(em);
+  }
 }
 
 // Rows of one (sequence, key head): word c of output row j from row idx[j],
 // zeros behind the sequence's end.
 __global__ void __launch_bounds__(256) gather_kernel(const EvictArgs a) {
+  pdl_wait();   // the choice
   const int bh = blockIdx.y, b = bh / a.KH, h = bh % a.KH;
   const uint4* k = a.k + b * a.sk[0] + h * a.sk[1];
   const uint4* v = a.v + b * a.sv[0] + h * a.sv[1];
@@ -184,8 +215,15 @@ extern "C" int tg_cache_evict(const void* k, const void* v, const float* weights
               {t[0] / 8, t[1] / 8, t[2] / 8}, {t[3] / 8, t[4] / 8, t[5] / 8}, {strides[6], strides[7]}};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int bh = batch * n_kv_heads, words = keep * (head_dim / 8);
-  select_kernel<<<bh, EV_THREADS, 0, s>>>(a);
-  gather_kernel<<<dim3(std::min(64, (words + 255) / 256), bh), 256, 0, s>>>(a);
+  const int cached = cap <= EV_CACHED;
+  const size_t smem = cached ? 4 * (size_t)cap : 0;
+  cudaError_t e = cudaSuccess;
+  if (smem > 32768) e = cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess) {
+    select_kernel<<<bh, EV_THREADS, smem, s>>>(a, cached);
+    e = cudaGetLastError();
+  }
+  if (e == cudaSuccess) e = launch_pdl(gather_kernel, dim3(std::min(64, (words + 255) / 256), bh), 256, 0, s, a);
   count_launches(2);
-  return c.done(cudaGetLastError());
+  return c.done(e);
 }
