@@ -23,6 +23,7 @@ namespace tg {
 
 constexpr int PLAN_THREADS = 1024;
 constexpr int PLAN_BUCKETS = 512;
+constexpr int PLAN_SPLITS = 256;   // split units, at most: each costs over twice an SM's share
 constexpr int MIN_PIECE = 4;    // key blocks of a split unit's piece, at least
 
 static __device__ DevStatus g_attn_status;
@@ -49,8 +50,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const PlanArgs a) {
   __shared__ AttnSeq seqs[PLAN_THREADS];
   __shared__ int ends[PLAN_THREADS];
   __shared__ int sums[PLAN_THREADS / 32];
+  __shared__ AttnEntry split[PLAN_SPLITS];
+  __shared__ int split_at[PLAN_SPLITS], split_n[PLAN_SPLITS];
   __shared__ unsigned long long s_total;
   __shared__ int s_max, s_slots, s_splits, s_n;
+  pdl_wait();
   pdl_trigger();
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   if (tid == 0) s_total = 0, s_max = 0, s_slots = 0, s_splits = 0;
@@ -68,11 +72,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const PlanArgs a) {
     }
     if (lane == 31) sums[w] = x;
     __syncthreads();
-    int before = 0, all = 0;
-    for (int i = 0; i < PLAN_THREADS / 32; i++) {
-      if (i < w) before += sums[i];
-      all += sums[i];
-    }
+    static_assert(PLAN_THREADS == 1024, "a lane for each warp's sum");
+    const int s = sums[lane], before = __reduce_add_sync(~0u, lane < w ? s : 0), all = __reduce_add_sync(~0u, s);
     seqs[tid] = q;
     ends[tid] = before + x;
     __syncthreads();
@@ -126,7 +127,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const PlanArgs a) {
   __syncthreads();
   if (w == 0) {   // exclusive sums: where each bucket starts
     int run = 0;
-    for (int b0 = 0; b0 < PLAN_BUCKETS; b0 += 32) {
+    for (int b0 = 0; b0 <= min(top, PLAN_BUCKETS - 1); b0 += 32) {
       const int v = hist[b0 + lane];
       int x = v;
       for (int o = 1; o < 32; o <<= 1) {
@@ -140,28 +141,38 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const PlanArgs a) {
   }
   __syncthreads();
   each([&](const AttnEntry& e, int cost) {
-    const int n = pieces(cost);
-    int at = atomicAdd(&hist[bucket((cost + n - 1) / n)], n);
-    AttnEntry x = e;
-    if (n > 1) {
-      x.slot = atomicAdd(&s_slots, n);
-      const int i = atomicAdd(&s_splits, 1);
-      if (x.slot + n > a.max_slots) return;   // not reached: see the bound above
-      a.splits[i] = AttnSplit{e.q0, e.ntok, x.slot, n};
+    const int n = pieces(cost), at = atomicAdd(&hist[bucket((cost + n - 1) / n)], n);
+    if (n == 1) {
+      if (at < a.max_entries) a.entries[at] = e;
+      return;
     }
-    for (int i = 0; i < n; i++, at++) {
-      const int b0 = (int)((long long)cost * i / n), b1 = (int)((long long)cost * (i + 1) / n);
+    AttnEntry x = e;
+    x.slot = atomicAdd(&s_slots, n);
+    const int i = atomicAdd(&s_splits, 1);
+    if (x.slot + n > a.max_slots || i >= PLAN_SPLITS) return;   // not reached: see the bound above
+    a.splits[i] = AttnSplit{e.q0, e.ntok, x.slot, n};
+    split[i] = x;
+    split_at[i] = at;
+    split_n[i] = n;
+  });
+  __syncthreads();
+  for (int i = w; i < min(s_splits, PLAN_SPLITS); i += PLAN_THREADS / 32) {   // a warp per split unit, a lane per piece
+    const AttnEntry e = split[i];
+    const int n = split_n[i];
+    for (int p = lane; p < n; p += 32) {
+      AttnEntry x = e;
+      const int b0 = (int)((long long)e.nb * p / n), b1 = (int)((long long)e.nb * (p + 1) / n);
       x.ks = e.ks + b0 * AT_KEYS;
       x.nb = b1 - b0;
-      if (at < a.max_entries) a.entries[at] = x;
-      x.slot += n > 1;
+      x.slot = e.slot + p;
+      if (split_at[i] + p < a.max_entries) a.entries[split_at[i] + p] = x;
     }
-  });
+  }
   __syncthreads();
   if (tid == 0) {
     a.head->n_entries = min(s_n, a.max_entries);
     a.head->counter = 0;
-    a.head->n_splits = min(s_splits, a.max_slots);
+    a.head->n_splits = min(min(s_splits, a.max_slots), PLAN_SPLITS);
   }
 }
 
@@ -223,8 +234,7 @@ static cudaError_t run_prompt(const PlanArgs& p, const CUtensorMap& qm, const CU
                               const CombineArgs& c, long long units, cudaStream_t s) {
   cudaError_t e = cudaSuccess;
   if (a.entries) {
-    plan_kernel<<<1, PLAN_THREADS, 0, s>>>(p);
-    e = cudaGetLastError();
+    e = launch_pdl(plan_kernel, dim3(1), PLAN_THREADS, 0, s, p);
     count_launches(1);
   }
   const long long work = (units + p.max_slots) * p.KH;

@@ -803,7 +803,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
 // accumulators of HD values in po; row(i) is the place of piece i of n.
 //   M = max(c m_i, sink),  f_i = 2^(c m_i - M),
 //   o = sum f_i o_i / (sum f_i l_i + 2^(sink - M)).
-// A warp per row: its lanes weigh 32 pieces at a time, then add them up four
+// A warp per row: its lanes weigh 32 pieces at a time, then add them up eight
 // at a time with HD / 32 dimensions each.  Pieces without a key (l = 0) have
 // no accumulator.  Returns (M, 1 / the whole sum), 0 without keys.
 template <typename F>
@@ -835,9 +835,9 @@ __device__ __forceinline__ void join_row(int n, const float2* pml, const float* 
     const float f = ml.y == 0.f ? 0.f : at_exp2(ml.x - fin.x) * fin.y;
     unsigned todo = __ballot_sync(~0u, ml.y != 0.f);
     while (todo) {
-      float fj[4], x[4][E];
+      float fj[8], x[8][E];
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
+      for (int j = 0; j < 8; j++) {
         const int i = todo ? __ffs(todo) - 1 : -1;
         todo &= todo - 1;
         fj[j] = __shfl_sync(~0u, f, i & 31);
@@ -850,7 +850,7 @@ __device__ __forceinline__ void join_row(int n, const float2* pml, const float* 
         }
       }
 #pragma unroll
-      for (int j = 0; j < 4; j++)
+      for (int j = 0; j < 8; j++)
 #pragma unroll
         for (int e = 0; e < E; e++) o[e] = fmaf(x[j][e], fj[j], o[e]);
     }

@@ -67,6 +67,7 @@ __global__ void __launch_bounds__(EV_THREADS) select_kernel(const EvictArgs a, i
   __shared__ int red[EV_WARPS];
   __shared__ uint32_t s_bin;
   __shared__ int s_need;
+  pdl_wait();
   pdl_trigger();
   const int t = threadIdx.x, lane = t & 31, wp = t >> 5, b = blockIdx.x / a.KH, h = blockIdx.x % a.KH;
   const int n = min(max(a.lens[b], 0), a.cap), m = min(n, a.keep), r = min(a.recent, m);
@@ -220,8 +221,7 @@ extern "C" int tg_cache_evict(const void* k, const void* v, const float* weights
   cudaError_t e = cudaSuccess;
   if (smem > 32768) e = cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e == cudaSuccess) {
-    select_kernel<<<bh, EV_THREADS, smem, s>>>(a, cached);
-    e = cudaGetLastError();
+    e = launch_pdl(select_kernel, dim3(bh), EV_THREADS, smem, s, a, cached);
   }
   if (e == cudaSuccess) e = launch_pdl(gather_kernel, dim3(std::min(64, (words + 255) / 256), bh), 256, 0, s, a);
   count_launches(2);
