@@ -489,3 +489,13 @@ def test_c_entries_refuse_host_memory(gpu):
     assert lib.tg_attention_prompt(*args(d, None)) == 3 and "device memory" in tg.last_error(lib)[1]
     rc = lib.tg_cache_evict(d, d, d, d, d, d + 4096, d + 8192, d + 12288, d + 16384, 1, 8, 1, 64, st, 4, 1, None)
     assert rc == 3 and "overlap" in tg.last_error(lib)[1]
+
+
+def test_serving_example(gpu):
+    """Prompts, decoding, evictions and the experts' steps through examples/serve_batch.py, the last attention checked."""
+    import importlib.util
+    from pathlib import Path
+    spec = importlib.util.spec_from_file_location("serve_batch", Path(__file__).resolve().parents[1] / "examples" / "serve_batch.py")
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    assert mod.main(["--batch", "5", "--prefix", "130", "--steps", "30", "--cap", "130", "--keep", "100", "--recent", "20"]) < 2e-2
