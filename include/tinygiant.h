@@ -343,7 +343,13 @@ int tg_cuda_matmul_q4k_noalloc(const uint8_t *q4_matrix, const float *input, flo
  * statistics, accumulators and weights are fp32.  The calls enqueue on
  * `stream` (a cudaStream_t), allocate nothing, keep nothing and can be
  * captured in a graph; concurrent calls need workspaces of their own.  Return
- * 0 when enqueued, else the error code that tg_cuda_last_error reports. */
+ * 0 when enqueued, else the error code that tg_cuda_last_error reports.  A
+ * kernel's wait that runs out (after about a second: a fault of the kernel)
+ * leaves the outputs undefined; tg_cuda_synchronize, called when the stream is
+ * done, reports it.  Keys and values of other sequences, behind a sequence's
+ * end or of evicted positions may hold anything, infinities and NaN too; a
+ * value that is not finite at one of a prompt's own later positions may reach
+ * the outputs of up to 127 positions before it. */
 
 /* Causal attention of n_seqs sequences packed one after another.  Sequence s
  * has the query rows cu_q[s] .. cu_q[s+1] and the keys cu_k[s] .. cu_k[s+1]
@@ -352,7 +358,8 @@ int tg_cuda_matmul_q4k_noalloc(const uint8_t *q4_matrix, const float *input, flo
  * position nk - nq + i and attends to the keys j up to it, with window > 0 to
  * the last `window` of those.  sinks [n_heads] (or NULL): a logit per head
  * that takes part in the softmax's sum without a value.  A query without a
- * key gives zeros.  strides: token and head of q, k, v, out (8 values).
+ * key gives zeros; rows of no sequence are not written.  strides: token and
+ * head of q, k, v, out (8 values).  n_heads / n_kv_heads is at most 128.
  * max_k: an upper bound of the sequences' keys, for the workspace's size
  * only.  workspace: 256-byte aligned, tg_attention_prompt_workspace bytes. */
 size_t tg_attention_prompt_workspace(int n_seqs, int total_q, int max_k, int n_heads, int n_kv_heads, int head_dim);

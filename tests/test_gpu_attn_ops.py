@@ -362,6 +362,7 @@ EVICT = [     # kv heads, head_dim, cap, lens, keep, recent
     (1, 40, 5000, [5000, 4097], 1, 1),
     (1, 96, 5000, [5000, 4097], 1, 0),
     (2, 64, 40000, [40000, 33333], 10001, 77),
+    (1, 8, 50000, [50000, 41000], 20000, 300),     # more weights than shared memory holds
 ]
 
 
@@ -476,6 +477,15 @@ def test_refusals(A):
     no("weights", E, c, c, w[:, :1], n, 4, 1)
     no("one shape", E, c, c[:, :, :7], w, n, 4, 1)
     assert not bool(P(q, k, k, cu).any())      # and the next good call runs
+
+
+def test_no_device_error_is_pending(A, gpu):
+    """tg_cuda_synchronize reports the operators' device errors; good calls leave none."""
+    g = gen(31)
+    q, k, v = rand(g, 300, 8, 128, dtype=torch.bfloat16), *(rand(g, 300, 2, 128, dtype=torch.bfloat16) for _ in range(2))
+    A.attention_prompt(q, k, v, ends([300]))
+    torch.cuda.synchronize()
+    assert gpu.tg_cuda_synchronize() == 0, tg.last_error(gpu)
 
 
 def test_c_entries_refuse_host_memory(gpu):

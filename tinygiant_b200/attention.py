@@ -13,8 +13,12 @@ All are asynchronous on torch's current stream of the tensors' device, take
 their workspace from torch's allocator, and can be captured in a CUDA graph.
 Tensors may be strided views: the last dimension is contiguous, the other
 strides are multiples of 8 elements, and data start on 16-byte boundaries.
-head_dim is a multiple of 8, at most 128.  Softmax statistics, accumulators
-and weights are fp32.  Bad arguments raise ValueError before anything runs
+head_dim is a multiple of 8, at most 128, and up to 128 query heads share a
+key head.  Softmax statistics, accumulators and weights are fp32; the softmax
+weights are rounded to the tensors' type for their product with the values.
+A value that is not finite at one of a prompt's own later positions may reach
+the outputs of up to 127 positions before it; other sequences' rows and what
+lies behind a cache's lengths may hold anything.  Bad arguments raise ValueError before anything runs
 (ArgumentError, a TinyGiantCudaError too, where the library sees them); other
 errors of the library raise TinyGiantCudaError.
 """

@@ -36,6 +36,21 @@ DevStatus* attn_status() {
   return at[dev];
 }
 
+// Reports a wait that ran out in one of the operators' kernels on the current
+// device since the last call, and clears the record.
+bool attn_finish(const char* what) {
+  DevStatus *d = attn_status(), st{};
+  if (!d) return true;
+  if (cudaMemcpy(&st, d, sizeof st, cudaMemcpyDeviceToHost) != cudaSuccess) {
+    set_host_error(100, "%s: reading the attention operators' status failed", what);
+    return false;
+  }
+  if (st.code == 0) return true;
+  cudaMemset(d, 0, sizeof st);
+  set_host_error(200 + st.code, "%s: device error %d at site %d of an attention operator (%d, %d)", what, st.code, st.where, st.a, st.b);
+  return false;
+}
+
 struct PlanArgs {
   AttnHead* head;
   AttnEntry* entries;

@@ -772,7 +772,8 @@ void* tg_cuda_stream(void) {
 int tg_cuda_synchronize(void) {
   std::lock_guard<std::recursive_mutex> lk(ctx_mutex());
   if (!ensure_init()) return -1;
-  return finish("tg_cuda_synchronize") ? 0 : -1;
+  const bool ok = finish("tg_cuda_synchronize");
+  return attn_finish("tg_cuda_synchronize") && ok ? 0 : -1;
 }
 
 }  // extern "C"

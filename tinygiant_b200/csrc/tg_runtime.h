@@ -44,5 +44,7 @@ void unregister_counters(void* p);
 // Attention decode's KV-cache mirrors (tg_attention.cu), dropped with the registry.
 void kv_mirror_forget(const void* host);
 void kv_mirror_clear();
+// Errors of the attention operators on device tensors (tg_attn_prompt.cu).
+bool attn_finish(const char* what);
 
 }  // namespace tg
