@@ -30,6 +30,7 @@ from . import TinyGiantCudaError, last_error, load
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _I64x8, _I64x16 = ctypes.c_int64 * 8, ctypes.c_int64 * 16
+_empty = torch.empty_strided                       # less host time than torch.empty
 _raw_stream = torch._C._cuda_getCurrentRawStream   # torch.cuda.current_stream(i).cuda_stream, without its objects
 
 
@@ -88,7 +89,7 @@ def _refuse(named, heads=None, small=()):
 
 
 def _fits(t, device, dtype):
-    return t.get_device() == device and t.dtype is dtype and t.stride(-1) == 1
+    return t.get_device() == device and t.dtype is dtype and t.stride()[-1] == 1
 
 
 def _heads_of(q, k):
@@ -123,7 +124,7 @@ def attention_prompt(q, k, v, cu_q, cu_k=None, *, max_k=None, window=0, sinks=No
             raise ValueError(f"without cu_k there are as many keys as queries; got {tk} and {tq}")
         cu_k = cu_q
     if out is None:
-        out = torch.empty((tq, H, hd), dtype=dtype, device=q.device)
+        out = _empty((tq, H, hd), (H * hd, hd, 1), dtype=dtype, device=q.device)
     if not (dev >= 0 and n >= 0 and k.shape == v.shape and k.shape[2] == hd and out.shape == q.shape
             and _fits(q, dev, dtype) and _fits(k, dev, dtype) and _fits(v, dev, dtype) and _fits(out, dev, dtype)
             and _fits(cu_q, dev, torch.int32) and _fits(cu_k, dev, torch.int32) and cu_k.shape == cu_q.shape
@@ -136,11 +137,11 @@ def attention_prompt(q, k, v, cu_q, cu_k=None, *, max_k=None, window=0, sinks=No
     max_k = tk if max_k is None or max_k > tk else max_k
     lib = load()
     nbytes = lib.tg_attention_prompt_workspace(n, tq, max_k, H, KH, hd)
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=q.device)
+    ws = _empty((nbytes,), (1,), dtype=torch.uint8, device=q.device) if nbytes else None
     (q0, q1, _), (k0, k1, _), (v0, v1, _), (o0, o1, _) = q.stride(), k.stride(), v.stride(), out.stride()
     _call(dev, lib.tg_attention_prompt, _DTYPES[dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
           cu_q.data_ptr(), cu_k.data_ptr(), _ptr(sinks), n, tq, tk, max_k, H, KH, hd,
-          _I64x8(q0, q1, k0, k1, v0, v1, o0, o1), window, hd ** -0.5 if scale is None else scale, ws.data_ptr(), nbytes)
+          _I64x8(q0, q1, k0, k1, v0, v1, o0, o1), window, hd ** -0.5 if scale is None else scale, _ptr(ws), nbytes)
     return out
 
 
@@ -162,7 +163,7 @@ def attention_shared(q, prefix_k, prefix_v, k, v, lens, *, max_len=None, window=
     dtype, dev, (B, H, hd), (_, KH, _) = _heads_of(q, k)
     P = 0 if prefix_k is None else prefix_k.shape[1] if prefix_k.dim() == 3 else -1
     if out is None:
-        out = torch.empty((B, H, hd), dtype=dtype, device=q.device)
+        out = _empty((B, H, hd), (H * hd, hd, 1), dtype=dtype, device=q.device)
     if not (dev >= 0 and k.dim() == 4 and k.shape == v.shape and k.shape[0] == B and k.shape[3] == hd and out.shape == q.shape
             and _fits(q, dev, dtype) and _fits(k, dev, dtype) and _fits(v, dev, dtype) and _fits(out, dev, dtype)
             and (prefix_k is None if prefix_v is None else
@@ -186,14 +187,14 @@ def attention_shared(q, prefix_k, prefix_v, k, v, lens, *, max_len=None, window=
     max_len = cap if max_len is None or max_len > cap else max_len
     lib = load()
     nbytes = lib.tg_attention_shared_workspace(B, P, max_len, H, KH, hd, weights is not None)
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=q.device)
+    ws = _empty((nbytes,), (1,), dtype=torch.uint8, device=q.device) if nbytes else None
     (q0, q1, _), (o0, o1, _), (k0, k1, k2, _), (v0, v1, v2, _) = q.stride(), out.stride(), k.stride(), v.stride()
     (pk0, pk1, _), (pv0, pv1, _) = (prefix_k.stride(), prefix_v.stride()) if P else ((8, 8, 1), (8, 8, 1))
     w0, w1, _ = weights.stride() if weights is not None else (1, 1, 1)
     _call(dev, lib.tg_attention_shared, _DTYPES[dtype], q.data_ptr(), _ptr(prefix_k), _ptr(prefix_v), k.data_ptr(),
           v.data_ptr(), out.data_ptr(), lens.data_ptr(), _ptr(sinks), _ptr(weights), B, P, cap, max_len, H, KH, hd,
           _I64x16(q0, q1, pk0, pk1, pv0, pv1, k0, k1, k2, v0, v1, v2, o0, o1, w0, w1), window,
-          hd ** -0.5 if scale is None else scale, ws.data_ptr(), nbytes)
+          hd ** -0.5 if scale is None else scale, _ptr(ws), nbytes)
     return out
 
 
@@ -208,24 +209,24 @@ def cache_evict(k, v, weights, lens, keep, recent):
     Returns (k, v, weights, lens, indices): new tensors [B, KH, keep, hd],
     [B, KH, keep, hd], [B, KH, keep], [B] and the positions' old places
     [B, KH, keep] int32; behind a sequence's end they hold zeros and -1."""
-    shape = k.shape
-    if not (len(shape) == 4 and k.dtype in _DTYPES and k.is_cuda and shape == v.shape and weights.shape == shape[:3]
-            and _fits(k, k.get_device(), k.dtype) and _fits(v, k.get_device(), k.dtype)
-            and _fits(weights, k.get_device(), torch.float32) and min(weights.stride()) > 0
-            and _fits(lens, k.get_device(), torch.int32) and lens.shape == shape[:1]):
+    shape, dtype, dev = k.shape, k.dtype, k.get_device()
+    if not (len(shape) == 4 and dtype in _DTYPES and dev >= 0 and shape == v.shape and weights.shape == shape[:3]
+            and _fits(k, dev, dtype) and _fits(v, dev, dtype) and _fits(weights, dev, torch.float32)
+            and min(weights.stride()) > 0 and _fits(lens, dev, torch.int32) and lens.shape == shape[:1]):
         if k.shape != v.shape:
             raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must have one shape")
         _refuse([("k", k, 4, None), ("v", v, 4, None)], None, [("weights", weights, torch.float32, shape[:3]),
                                                               ("lens", lens, torch.int32, shape[:1])])
     B, KH, cap, hd = shape
-    dev, where = k.get_device(), k.device
+    where = k.device
     if not (0 < keep <= cap and 0 <= recent <= keep):
         raise ValueError(f"need 0 < keep <= {cap} and 0 <= recent <= keep; got {keep}, {recent}")
-    ko = torch.empty((B, KH, keep, hd), dtype=k.dtype, device=where)
-    vo = torch.empty((B, KH, keep, hd), dtype=k.dtype, device=where)
-    wo = torch.empty((B, KH, keep), dtype=torch.float32, device=where)
-    idx = torch.empty((B, KH, keep), dtype=torch.int32, device=where)
-    lo = torch.empty((B,), dtype=torch.int32, device=where)
+    rows = KH * keep
+    ko = _empty((B, KH, keep, hd), (rows * hd, keep * hd, hd, 1), dtype=dtype, device=where)
+    vo = torch.empty_like(ko)
+    wo = _empty((B, KH, keep), (rows, keep, 1), dtype=torch.float32, device=where)
+    idx = _empty((B, KH, keep), (rows, keep, 1), dtype=torch.int32, device=where)
+    lo = _empty((B,), (1,), dtype=torch.int32, device=where)
     (k0, k1, k2, _), (v0, v1, v2, _), (w0, w1, _) = k.stride(), v.stride(), weights.stride()
     _call(dev, load().tg_cache_evict, k.data_ptr(), v.data_ptr(), weights.data_ptr(), lens.data_ptr(), ko.data_ptr(),
           vo.data_ptr(), wo.data_ptr(), lo.data_ptr(), idx.data_ptr(), B, cap, KH, hd,

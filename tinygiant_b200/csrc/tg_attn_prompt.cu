@@ -221,6 +221,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
 // The workspace: header, entries, splits, then the partial results.
 struct PromptSpace {
   int max_entries, max_slots;
+  bool plan;   // without splits (no sequence has more keys than a piece) and with a lane for each sequence the units need no list
   size_t entries, splits, pml, po, bytes;
   PromptSpace(int n_seqs, int total_q, int max_k, int H, int KH, int hd) {
     const long long tpu = 2 * (AT_ROWS / (H / KH)), units = (total_q + tpu - 1) / tpu + n_seqs;
@@ -235,6 +236,9 @@ struct PromptSpace {
       return o;
     };
     bytes = 0;
+    entries = splits = pml = po = 0;
+    plan = max_slots > 0 || n_seqs > 32;
+    if (!plan) return;
     take(sizeof(AttnHead));
     entries = take(sizeof(AttnEntry) * max_entries);
     splits = take(sizeof(AttnSplit) * max_slots);
@@ -298,7 +302,7 @@ extern "C" int tg_attention_prompt(int dtype, const void* q, const void* k, cons
   if (sinks) c.ptr(sinks, 4, "sinks");
   const PromptSpace sp(n_seqs, total_q, max_k, n_heads, n_kv_heads, head_dim);
   c.need(workspace_bytes >= sp.bytes, "the workspace is smaller than tg_attention_prompt_workspace says");
-  c.ptr(workspace, 256, "workspace");
+  if (sp.bytes > 0) c.ptr(workspace, 256, "workspace");
   if (c.rc) return c.rc;
 
   const int G = n_heads / n_kv_heads, tpt = AT_ROWS / G;
@@ -307,10 +311,7 @@ extern "C" int tg_attention_prompt(int dtype, const void* q, const void* k, cons
              2 * tpt, n_kv_heads, window, attn_sms(), sp.max_entries, sp.max_slots};
   AttnTcArgs a{};
   a.head = p.head;
-  // Without splits (the longest sequence has no more keys than a split unit's
-  // piece) and with a lane for each sequence the units need no list: the
-  // plan's launch is saved.
-  a.entries = sp.max_slots == 0 && n_seqs <= 32 ? nullptr : p.entries;
+  a.entries = sp.plan ? p.entries : nullptr;   // null: dealt out in turn
   a.cu_q = cu_q, a.cu_k = cu_k, a.n_seqs = n_seqs, a.total_q = total_q;
   a.out = out;
   a.po = (float*)(ws + sp.po);
