@@ -28,6 +28,7 @@
 // The prefix is bound by the tensor cores and the own keys by HBM, so the two
 // kernels run side by side, each on its share of the SMs.
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/tinygiant.h"
 #include "tg_attn_tc.cuh"
@@ -51,7 +52,7 @@ struct OwnArgs {
   float* scores;      // [b KH + kh][max_len][gp] c s, or null
   long long sq[2];
   int B, KH, G, gp, hd, max_len, window, ngc;   // ngc: groups of 8 NT heads per key head
-  float c;
+  float c, inv_c;     // scale log2(e), and 1 / that
   DevStatus* st;
 };
 
@@ -129,15 +130,17 @@ __device__ __forceinline__ int own_cta(long long x, long long total, int n) { re
 struct OwnWalk {
   long long x, x1;
   int b, hk, j, len, lo, n, j1;   // sequence, head, first stage; own keys, first key, stages; last stage + 1
-  __device__ void seq(const OwnArgs& a) {
-    len = own_len(a.lens, b, a.max_len);
+  int ahead;                      // the next sequence's own keys, read a sequence early
+  __device__ void seq(const OwnArgs& a, int keys) {
+    len = keys;
     lo = own_first(len, a.window);
     n = own_stages(len, a.window);
+    ahead = b + 1 < a.B ? own_len(a.lens, b + 1, a.max_len) : 0;
   }
   __device__ void start(const OwnArgs& a, int b0, int before, long long x0, long long end) {
     x = x0, x1 = end, b = b0;
     if (x >= x1) return;
-    seq(a);
+    seq(a, own_len(a.lens, b, a.max_len));
     const long long r = x0 - (long long)before * (a.KH * a.ngc);
     hk = (int)(r / n), j = (int)(r % n);
     j1 = (int)min((long long)n, j + x1 - x);
@@ -151,7 +154,7 @@ struct OwnWalk {
       hk = 0;
       do {
         b++;
-        seq(a);
+        seq(a, ahead);
       } while (n == 0);   // x < x1: there is another sequence with keys
     }
     j1 = (int)min((long long)n, x1 - x);
@@ -276,6 +279,8 @@ __global__ void __launch_bounds__(OWN_THREADS, 1) own_kernel(const __grid_consta
     ko[k] = krow * 128 + (((k * 2 + (lane >> 4)) ^ (krow & 7)) << 4);
     vo[k] = vrow * 128 + (((k * 2 + ((lane >> 3) & 1)) ^ (vrow & 7)) << 4);
   }
+  int turn = 0;                              // the next stage's group
+  uint32_t stage = 0, bar = 0, phase = 0;    // and its place, barrier and phase
   for (wk.start(a, sh.b0, sh.before, x0, x1); wk.more(); wk.next(a)) {
     const int b = wk.b, kh = wk.hk / a.ngc, gc = wk.hk % a.ngc, bk = b * a.KH + kh;
     const int lo = a.window > 0 ? max(0, wk.len - a.window) : 0, hi = wk.len;
@@ -302,107 +307,124 @@ __global__ void __launch_bounds__(OWN_THREADS, 1) own_kernel(const __grid_consta
 #pragma unroll
       for (int k = 0; k < HD / 16; k++) o[t][k][0] = o[t][k][1] = o[t][k][2] = o[t][k][3] = 0.f;
     }
-    for (int j = wk.j; j < wk.j1; j++, n++) {
-      if ((n & 1) != wid >> 2) continue;
-      const int s = n % S::STAGES, r0 = wk.lo + j * OWN_KEYS;
-      if (!at_wait(&sh.full[n % S::BARS], (n / S::BARS) & 1, abort)) {
-        if (lane == 0) fail(401, n);
-        break;   // on to the barriers below: every wait from here on fails at once
-      }
-      const int k0 = r0 + wq * 32;   // this warp's keys k0 .. k0 + 31
-      if (k0 < hi) {
-        const uint32_t kb = smem_u32(stages + s * S::STAGE), vb = kb + (HD / 64) * S::HALF;
-        float x[2][NT][4];
+    // reference m in base 2, as -m and as the score that exceeds it by 8
+    float nm[NT][2], lim[NT][2];
 #pragma unroll
-        for (int u = 0; u < 2; u++)
+    for (int t = 0; t < NT; t++) nm[t][0] = nm[t][1] = 0.f, lim[t][0] = lim[t][1] = -INFINITY;
+    float* scores = a.scores ? a.scores + (size_t)bk * a.max_len * a.gp + gc * NT * 8 + cc * 2 : nullptr;
+    // One step: this warp's keys k0 .. k0 + 31 of a stage.  WHOLE: all of them
+    // are the sequence's.
+    auto step = [&](auto whole, uint32_t kb, int k0) {
+      constexpr bool WHOLE = decltype(whole)::value;
+      const uint32_t vb = kb + (HD / 64) * S::HALF;
+      float x[2][NT][4];
 #pragma unroll
-          for (int t = 0; t < NT; t++) x[u][t][0] = x[u][t][1] = x[u][t][2] = x[u][t][3] = 0.f;
+      for (int u = 0; u < 2; u++)
 #pragma unroll
-        for (int k = 0; k < HD / 16; k++)
+        for (int t = 0; t < NT; t++) x[u][t][0] = x[u][t][1] = x[u][t][2] = x[u][t][3] = 0.f;
 #pragma unroll
-          for (int u = 0; u < 2; u++) {
-            uint32_t f[4];
-            ldsm4(f, kb + (k / 4) * S::HALF + u * 2048 + ko[k % 4]);
-#pragma unroll
-            for (int t = 0; t < NT; t++) mma16816<T>(x[u][t], f, qf[t][k][0], qf[t][k][1]);
-          }
-        // scores in base 2; -inf outside the sequence's keys
-        const bool whole = k0 >= lo && k0 + 32 <= hi;
-        bool up = false;
+      for (int k = 0; k < HD / 16; k++)
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-          const int ka = k0 + 16 * u + g;
-          const bool in0 = whole || (ka >= lo && ka < hi), in1 = whole || (ka + 8 >= lo && ka + 8 < hi);
+          uint32_t f[4];
+          ldsm4(f, kb + ko[k % 4] + (k / 4) * S::HALF + u * 2048);
 #pragma unroll
-          for (int t = 0; t < NT; t++) {
+          for (int t = 0; t < NT; t++) mma16816<T>(x[u][t], f, qf[t][k][0], qf[t][k][1]);
+        }
+      bool up = false;
 #pragma unroll
-            for (int z = 0; z < 4; z++) {
-              x[u][t][z] = (z < 2 ? in0 : in1) ? x[u][t][z] * a.c : -INFINITY;
-              up |= x[u][t][z] > m[t][z & 1] + 8.f;
-            }
-            if (a.scores && (gc * NT + t) * 8 < a.gp) {
-              float* sc = a.scores + ((size_t)bk * a.max_len + ka) * a.gp + (gc * NT + t) * 8 + cc * 2;
-              if (in0) *reinterpret_cast<float2*>(sc) = make_float2(x[u][t][0], x[u][t][1]);
-              if (in1) *reinterpret_cast<float2*>(sc + 8 * a.gp) = make_float2(x[u][t][2], x[u][t][3]);
-            }
+      for (int u = 0; u < 2; u++) {
+        const int ka = k0 + 16 * u + g;
+        const bool in0 = WHOLE || (ka >= lo && ka < hi), in1 = WHOLE || (ka + 8 >= lo && ka + 8 < hi);
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+#pragma unroll
+          for (int z = 0; z < 4; z++) {
+            if (!WHOLE && !(z < 2 ? in0 : in1)) x[u][t][z] = -INFINITY;
+            up |= x[u][t][z] > lim[t][z & 1];
+          }
+          if (a.scores && (gc * NT + t) * 8 < a.gp) {
+            float* sc = scores + (size_t)ka * a.gp + t * 8;
+            if (in0) *reinterpret_cast<float2*>(sc) = make_float2(x[u][t][0] * a.c, x[u][t][1] * a.c);
+            if (in1) *reinterpret_cast<float2*>(sc + 8 * a.gp) = make_float2(x[u][t][2] * a.c, x[u][t][3] * a.c);
           }
         }
-        if (__any_sync(~0u, up)) {
+      }
+      if (__any_sync(~0u, up)) {
 #pragma unroll
-          for (int t = 0; t < NT; t++)
+        for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int z = 0; z < 2; z++) {
-              float v = fmaxf(fmaxf(x[0][t][z], x[0][t][z + 2]), fmaxf(x[1][t][z], x[1][t][z + 2]));
+          for (int z = 0; z < 2; z++) {
+            float v = fmaxf(fmaxf(x[0][t][z], x[0][t][z + 2]), fmaxf(x[1][t][z], x[1][t][z + 2]));
 #pragma unroll
-              for (int sft = 4; sft < 32; sft <<= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, sft));
-              const float mn = fmaxf(m[t][z], v), f = mn > m[t][z] ? at_exp2(m[t][z] - mn) : 1.f;
-              m[t][z] = mn;
-              l[t][z] *= f;
+            for (int sft = 4; sft < 32; sft <<= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, sft));
+            const float mn = fmaxf(m[t][z], v * a.c), f = mn > m[t][z] ? at_exp2(m[t][z] - mn) : 1.f;
+            m[t][z] = mn;
+            nm[t][z] = mn == -INFINITY ? 0.f : -mn;
+            lim[t][z] = (mn + 8.f) * a.inv_c;
+            l[t][z] *= f;
 #pragma unroll
-              for (int k = 0; k < HD / 16; k++) {
-                o[t][k][z] *= f;
-                o[t][k][z + 2] *= f;
-              }
+            for (int k = 0; k < HD / 16; k++) {
+              o[t][k][z] *= f;
+              o[t][k][z + 2] *= f;
             }
-        }
-        uint32_t p[2][NT][2];
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-          for (int t = 0; t < NT; t++) {
-            float e[4];
-#pragma unroll
-            for (int z = 0; z < 4; z++) {
-              const float mz = m[t][z & 1];
-              e[z] = at_exp2(x[u][t][z] - (mz == -INFINITY ? 0.f : mz));
-              l[t][z & 1] += e[z];
-            }
-            p[u][t][0] = movm(at_pack<T>(e[0], e[1]));
-            p[u][t][1] = movm(at_pack<T>(e[2], e[3]));
           }
+      }
+      uint32_t p[2][NT][2];
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+          float e[4];
+#pragma unroll
+          for (int z = 0; z < 4; z++) {
+            e[z] = at_exp2(fmaf(x[u][t][z], a.c, nm[t][z & 1]));
+            l[t][z & 1] += e[z];
+          }
+          p[u][t][0] = movm(at_pack<T>(e[0], e[1]));
+          p[u][t][1] = movm(at_pack<T>(e[2], e[3]));
+        }
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
         // V rows outside [lo, hi) may hold anything, infinities and NaN too:
         // their bits are cleared (a register has two keys of one dimension)
-        uint32_t vm[2][2];
-#pragma unroll
-        for (int u = 0; u < 2; u++)
+        uint32_t vm[2] = {~0u, ~0u};
+        if (!WHOLE)
 #pragma unroll
           for (int z = 0; z < 2; z++) {
             const int kk = k0 + 16 * u + z * 8 + cc * 2;
-            vm[u][z] = (kk >= lo && kk < hi ? 0x0000ffffu : 0u) | (kk + 1 >= lo && kk + 1 < hi ? 0xffff0000u : 0u);
+            vm[z] = (kk >= lo && kk < hi ? 0x0000ffffu : 0u) | (kk + 1 >= lo && kk + 1 < hi ? 0xffff0000u : 0u);
           }
 #pragma unroll
-        for (int u = 0; u < 2; u++)
+        for (int k = 0; k < HD / 16; k++) {
+          uint32_t f[4];
+          ldsm4t(f, vb + vo[k % 4] + (k / 4) * S::HALF + u * 2048);
+          if (!WHOLE) f[0] &= vm[0], f[1] &= vm[0], f[2] &= vm[1], f[3] &= vm[1];
 #pragma unroll
-          for (int k = 0; k < HD / 16; k++) {
-            uint32_t f[4];
-            ldsm4t(f, vb + (k / 4) * S::HALF + u * 2048 + vo[k % 4]);
-            if (!whole) f[0] &= vm[u][0], f[1] &= vm[u][0], f[2] &= vm[u][1], f[3] &= vm[u][1];
-#pragma unroll
-            for (int t = 0; t < NT; t++) mma16816<T>(o[t][k], f, p[u][t][0], p[u][t][1]);
-          }
+          for (int t = 0; t < NT; t++) mma16816<T>(o[t][k], f, p[u][t][0], p[u][t][1]);
+        }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.empty[n % S::BARS]);
+    };
+    for (int j = wk.j; j < wk.j1; j++) {
+      if (turn == wid >> 2) {
+        if (!at_wait(&sh.full[bar], phase, abort)) {
+          if (lane == 0) fail(401, bar);
+          break;   // on to the barriers below: every wait from here on fails at once
+        }
+        const int k0 = wk.lo + j * OWN_KEYS + wq * 32;
+        if (k0 < hi) {
+          const uint32_t kb = smem_u32(stages) + stage * S::STAGE;
+          if (k0 >= lo && k0 + 32 <= hi)
+            step(std::true_type{}, kb, k0);
+          else
+            step(std::false_type{}, kb, k0);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.empty[bar]);
+      }
+      turn ^= 1;
+      if (++stage == S::STAGES) stage = 0;
+      if (++bar == S::BARS) bar = 0, phase ^= 1;
     }
     // join the warps, 8 heads at a time
 #pragma unroll
@@ -651,7 +673,7 @@ extern "C" int tg_attention_shared(int dtype, const void* q, const void* prefix_
   int* starts = (int*)(ws + sp.starts);
   OwnArgs o{q, lens, a.po + sp.own_row * (head_dim <= 64 ? 64 : 128), a.pml + sp.own_row, starts,
             weights ? (float*)(ws + sp.scores) : nullptr, {t[0], t[1]}, batch, n_kv_heads, G, sp.gp, head_dim, max_len, window, sp.ngc,
-            a.c, a.st};
+            a.c, 1.f / a.c, a.st};
   JoinArgs j{lens, starts, sinks, weights, a.po, o.scores, a.pml, out, {t[12], t[13]},
              {weights ? strides[14] : 0, weights ? strides[15] : 0}, sp.own_row, batch, n_kv_heads, G, sp.gp, head_dim, sp.tpt, sp.nsp,
              max_len, window, sp.ngc, sp.nt, sp.own_ctas};
