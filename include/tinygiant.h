@@ -346,10 +346,9 @@ int tg_cuda_matmul_q4k_noalloc(const uint8_t *q4_matrix, const float *input, flo
  * 0 when enqueued, else the error code that tg_cuda_last_error reports.  A
  * kernel's wait that runs out (after about a second: a fault of the kernel)
  * leaves the outputs undefined; tg_cuda_synchronize, called when the stream is
- * done, reports it.  Keys and values of other sequences, behind a sequence's
- * end or of evicted positions may hold anything, infinities and NaN too; a
- * value that is not finite at one of a prompt's own later positions may reach
- * the outputs of up to 127 positions before it. */
+ * done, reports it.  What a query does not attend to (later positions, those
+ * before its window, other sequences, rows behind a cache's lengths) may hold
+ * anything, infinities and NaN too. */
 
 /* Causal attention of n_seqs sequences packed one after another.  Sequence s
  * has the query rows cu_q[s] .. cu_q[s+1] and the keys cu_k[s] .. cu_k[s+1]

@@ -170,6 +170,50 @@ def test_prompt_sequences_do_not_touch(A, poison):
     assert torch.equal(got[:70], clean[:70]) and torch.equal(got[160:], clean[160:])
 
 
+@pytest.mark.parametrize("poison", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("H,KH,hd,nq,nk,window", [(8, 2, 64, [300, 40], None, 0), (2, 2, 128, [500], None, 100),
+                                                  (8, 1, 128, [8, 3], [3000, 260], 0), (4, 4, 96, [260], [700], 150)])
+def test_prompt_values_do_not_reach_rows_that_do_not_see_them(A, H, KH, hd, nq, nk, window, poison):
+    """A value row that is not finite changes the rows that attend to its key and no other; those get it in its dimension."""
+    g, dt = gen(32), torch.bfloat16
+    nk = nk or nq
+    q, k, v = rand(g, sum(nq), H, hd, dtype=dt), *(rand(g, sum(nk), KH, hd, dtype=dt) for _ in range(2))
+    run = lambda: A.attention_prompt(q, k, v, ends(nq), ends(nk), window=window)  # noqa: E731
+    clean = run()
+    n, m = nq[0], nk[0]
+    at = [m - 1, m - 2 if n > 2 else m - 1, max(0, m - n + n // 2)]      # the last keys and one amid the queries
+    dim = [3, hd - 1, 0]
+    for j, d in zip(at, dim):
+        v[j, KH - 1, d] = poison
+    got = run()
+    want = clean.clone()
+    i = torch.arange(n, device="cuda") + (m - n)
+    for j, d in zip(at, dim):
+        sees = (i >= j) & ((i - j < window) if window else True)
+        heads = range(H - H // KH, H)
+        for h in heads:
+            want[:n, h, d] = torch.where(sees, torch.tensor(poison, dtype=dt, device="cuda"), want[:n, h, d])
+    same = (got == want) | (torch.isnan(got) & torch.isnan(want))
+    # a weight that is 0 in the type makes a NaN of an infinity: rows that see the key may have that instead
+    same |= torch.isnan(got) & torch.isinf(want)
+    assert bool(same.all()), int((~same).sum())
+
+
+def test_shared_prefix_values_outside_the_window(A):
+    """A prefix value that is not finite, before the window of some sequences: those do not see it."""
+    g, dt, H, KH, hd, P = gen(33), torch.bfloat16, 8, 2, 64, 300
+    q = rand(g, 3, H, hd, dtype=dt)
+    pk, pv = (rand(g, KH, P, hd, dtype=dt) for _ in range(2))
+    k, v = (rand(g, 3, KH, 64, hd, dtype=dt) for _ in range(2))
+    n = torch.tensor([60, 5, 55], dtype=torch.int32, device="cuda")
+    run = lambda: A.attention_shared(q, pk, pv, k, v, n, window=100)  # noqa: E731
+    clean = run()
+    pv[:, 250, 7] = math.inf            # seen from position 304 (back to 205), not from 359 (260) and 354 (255)
+    got = run()
+    assert torch.equal(got[0], clean[0]) and torch.equal(got[2], clean[2])
+    assert bool(torch.isinf(got[1, :, 7]).all()) and torch.equal(got[1, :, :7], clean[1, :, :7])
+
+
 def test_prompt_on_another_stream_and_in_a_graph(A):
     g, nq = gen(6), [100, 28]
     q, k, v = rand(g, 128, 8, 64, dtype=torch.bfloat16), *(rand(g, 128, 2, 64, dtype=torch.bfloat16) for _ in range(2))

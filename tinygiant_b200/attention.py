@@ -16,9 +16,9 @@ strides are multiples of 8 elements, and data start on 16-byte boundaries.
 head_dim is a multiple of 8, at most 128, and up to 128 query heads share a
 key head.  Softmax statistics, accumulators and weights are fp32; the softmax
 weights are rounded to the tensors' type for their product with the values.
-A value that is not finite at one of a prompt's own later positions may reach
-the outputs of up to 127 positions before it; other sequences' rows and what
-lies behind a cache's lengths may hold anything.  Bad arguments raise ValueError before anything runs
+What a query does not attend to (later positions, those before its window,
+other sequences, rows behind a cache's lengths) may hold anything, infinities
+and NaN too.  Bad arguments raise ValueError before anything runs
 (ArgumentError, a TinyGiantCudaError too, where the library sees them); other
 errors of the library raise TinyGiantCudaError.
 """

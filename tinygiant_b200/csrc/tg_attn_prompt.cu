@@ -318,6 +318,7 @@ extern "C" int tg_attention_prompt(int dtype, const void* q, const void* k, cons
   a.pml = (float2*)(ws + sp.pml);
   a.sinks = sinks;
   a.so[0] = st[6], a.so[1] = st[7];
+  a.v = v, a.sv[0] = st[4], a.sv[1] = st[5];
   a.G = G, a.KH = n_kv_heads, a.hd = head_dim, a.tpt = tpt, a.window = window, a.total_k = total_k;
   a.wide = head_dim % 16 == 0 && (uintptr_t)out % 32 == 0 && st[6] % 16 == 0 && st[7] % 16 == 0;
   a.c = scale * LOG2E;

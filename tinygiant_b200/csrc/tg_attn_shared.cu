@@ -666,6 +666,7 @@ extern "C" int tg_attention_shared(int dtype, const void* q, const void* prefix_
   a.po = (float*)(ws + sp.po);
   a.pml = (float2*)(ws + sp.pml);
   a.lens = lens;
+  a.v = prefix_v, a.sv[0] = t[5], a.sv[1] = t[4];
   a.G = G, a.KH = n_kv_heads, a.hd = head_dim, a.tpt = sp.tpt, a.window = window, a.total_k = prefix_len;
   a.P = prefix_len, a.B = batch, a.nsp = sp.nsp, a.max_len = max_len;
   a.c = scale * LOG2E;

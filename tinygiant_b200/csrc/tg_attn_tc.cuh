@@ -21,7 +21,7 @@
 // a few tokens wide.  Its keys are nb blocks from key ks on.
 //
 // Warps: 0-3 and 4-7 the softmax of tile 0 and 1 (a thread per row), 8 the TMA
-// loads, 9 the S products, 10 the P V.  Tensor memory (512 columns): O of both
+// loads, 9 the S products, 10 the P V, 11 the values that not all rows see.  Tensor memory (512 columns): O of both
 // tiles, the 16-bit P of both, and S, one buffer of 128 columns for both tiles
 // at head_dim 128, one for each at 64.  A softmax warp takes its S into
 // registers at once and frees the buffer, so the next S is computed while it
@@ -43,10 +43,11 @@ namespace tg {
 
 constexpr int AT_ROWS = 128;       // query rows per tile (MMA M)
 constexpr int AT_KEYS = 128;       // keys per block (MMA N of S, K of P V)
-constexpr int AT_SOFT = 8;         // softmax warps; then one each for loads, S, P V, and an idle one:
-constexpr int AT_THREADS = 384;    // registers move between whole warpgroups
+constexpr int AT_SOFT = 8;         // softmax warps; then one each for loads, S, P V and edges
+constexpr int AT_THREADS = 384;
 constexpr int AT_NPOS = 0x3fffffff;
 constexpr int AT_UNITS = 4;        // units announced ahead
+constexpr int AT_EDGES = 8;        // a unit's blocks that some rows see in part, at most (2 tiles of 128 tokens, both ends)
 
 // One piece of work of every key head.
 struct __align__(16) AttnEntry {
@@ -54,6 +55,7 @@ struct __align__(16) AttnEntry {
   int p0;         // position of the first token among its sequence's keys
   int k0, nk;     // the sequence's first key row and its keys
   int ks, nb;     // this piece's first key and blocks of keys
+  int el, eh;     // the keys [el, eh) are those that all rows see
   int slot;       // -1: writes the outputs; else the piece's place among the partial results
 };
 
@@ -88,6 +90,8 @@ __device__ __forceinline__ AttnEntry attn_unit(const AttnSeq& s, int t0, int tpu
   e.nk = s.nk;
   const int hi = e.p0 + e.ntok, lo = window > 0 ? max(0, e.p0 + 1 - window) : 0;
   e.ks = lo;
+  e.el = window > 0 ? max(0, hi - window) : 0;
+  e.eh = e.p0 + 1;
   e.nb = hi > lo ? (hi - lo + AT_KEYS - 1) / AT_KEYS : 0;
   e.slot = -1;
   return e;
@@ -104,6 +108,8 @@ struct AttnTcArgs {
   const float* sinks;
   const int* lens;            // shared: own keys of each sequence
   long long so[2];
+  const void* v;              // the values, and their strides of rows and heads
+  long long sv[2];
   int G, KH, hd, tpt, window;
   int total_k;                // rows of k and v
   int P, B, nsp, max_len;     // shared: prefix keys, sequences, pieces per unit, bound of lens
@@ -265,9 +271,13 @@ struct AttnTcShape {
 
 struct AttnTcShared {
   uint64_t q_full[2], q_empty[2], kv_full[10], kv_empty[10], s_full[2], s_loaded[2], p_full[2], p_empty[2], unit_full[AT_UNITS],
-      unit_empty[AT_UNITS], aux, drain[2];
+      unit_empty[AT_UNITS], edge[10], drain[2];
   AttnEntry unit[AT_UNITS];
   int unit_kh[AT_UNITS];      // -1: no more work
+  // Edge blocks with values that are not finite: 16 times the unit's number
+  // and how many; each one's block and its keys, a bit each.
+  int bad[AT_UNITS], bad_block[AT_UNITS][AT_EDGES];
+  uint32_t bad_keys[AT_UNITS][AT_EDGES][4];
   uint32_t tmem;
   int abort;
 };
@@ -280,6 +290,54 @@ __device__ __forceinline__ bool at_wait(uint64_t* bar, uint32_t parity, const vo
   while (!mbar_try_wait(bar, parity))
     if (*abort || (uint32_t)clock() - t0 > 1u << 31) return false;
   return true;
+}
+
+// The same for a warp that has time: it polls a few times in a microsecond, so
+// that its quarter of the SM's softmax keeps the issue slots.
+__device__ __forceinline__ bool at_wait_idle(uint64_t* bar, uint32_t parity, const volatile int* abort) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint32_t t0 = clock();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*abort || (uint32_t)clock() - t0 > 1u << 31) return false;
+    __nanosleep(200);
+  }
+  return true;
+}
+
+// A place in a ring and its phase, counted on without divisions.
+struct AttnRing {
+  uint32_t s, ph;
+  __device__ __forceinline__ void add(uint32_t k, uint32_t n) {
+    s += k;
+    if (s >= n) s -= n, ph ^= 1;
+  }
+};
+
+// Adds to a row's O in tensor memory the values that are not finite of the
+// noted keys in [lo, hi) (numbers from the unit's first key on, whose values
+// start at v).  All lanes of the warp call it.
+template <typename T, int HD>
+__device__ __noinline__ void attn_add_odd(uint32_t to, const char* v, long long stride, int hd, int blocks, const int* block,
+                                          const uint32_t (*keys)[4], int lo, int hi) {
+  for (int i = 0; i < HD / 16; i++) {
+    uint32_t o[16];
+    at_ld16(to + 16 * i, o);
+    at_wait_ld();
+    for (int r = 0; r < blocks; r++)
+      for (int k = 0; k < AT_KEYS; k++) {
+        const int key = block[r] * AT_KEYS + k;
+        if (!(keys[r][k / 32] >> (k % 32) & 1) || key < lo || key >= hi) continue;
+        const T* x = (const T*)v + key * stride + 16 * i;
+#pragma unroll
+        for (int q = 0; q < 16; q++) {
+          const float y = 16 * i + q < hd ? to_f32(x[q]) : 0.f;
+          if (!isfinite(y)) o[q] = __float_as_uint(__uint_as_float(o[q]) + y);
+        }
+      }
+    __syncwarp();
+    at_st16(to + 16 * i, o);
+    at_wait_st();
+  }
 }
 
 template <typename T, int HD, bool SHARED>
@@ -305,6 +363,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
     for (int i = 0; i < NBAR; i++) {
       mbar_init(&sh.kv_full[i], 1);
       mbar_init(&sh.kv_empty[i], 1);
+      mbar_init(&sh.edge[i], 1);
     }
     for (int i = 0; i < 2; i++) {
       mbar_init(&sh.q_full[i], 1);
@@ -316,9 +375,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
     }
     for (int i = 0; i < AT_UNITS; i++) {
       mbar_init(&sh.unit_full[i], 1);
-      mbar_init(&sh.unit_empty[i], W0 + 2);
+      mbar_init(&sh.unit_empty[i], W0 + 3);
     }
-    mbar_init(&sh.aux, 1);
+    for (int i = 0; i < AT_UNITS; i++) sh.bad[i] = -1;
     mbar_init(&sh.drain[0], 1);
     mbar_init(&sh.drain[1], 1);
     sh.abort = 0;
@@ -362,10 +421,15 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
     e.ks = b0 * AT_KEYS;
     e.nb = b1 - b0;
     e.slot = i;
+    e.eh = AT_NPOS;       // behind the prefix there are zeros
     if (a.window > 0) {   // without the keys that no row of the unit sees
-      int lo = a.P;
-      for (int r = lane; r < e.ntok; r += 32) lo = min(lo, max(0, a.P + min(max(a.lens[e.q0 + r], 0), a.max_len) - a.window));
+      int lo = a.P, most = 0;
+      for (int r = lane; r < e.ntok; r += 32) {
+        const int first = max(0, a.P + min(max(a.lens[e.q0 + r], 0), a.max_len) - a.window);
+        lo = min(lo, first), most = max(most, first);
+      }
       lo = __reduce_min_sync(~0u, lo);
+      e.el = __reduce_max_sync(~0u, most);
       const int skip = lo >= a.P ? e.nb : min(e.nb, max(0, (lo - e.ks) / AT_KEYS));
       e.ks += skip * AT_KEYS;
       e.nb -= skip;
@@ -374,6 +438,11 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
   };
   // The next unit, as the load warp announced it; false at the end.
   int un = 0;
+  // Whether some row sees the block from key `row` on only in part, or it
+  // reaches behind the sequence's keys into others'.
+  auto on_edge = [&](const AttnEntry& e, int row) {
+    return row < e.el || row + AT_KEYS > e.eh || (e.nk - row < AT_KEYS && e.k0 + e.nk < a.total_k);
+  };
   auto next_unit = [&](AttnEntry& e, int& kh) -> bool {
     const int i = un % AT_UNITS;
     if (!at_wait(&sh.unit_full[i], (un / AT_UNITS) & 1, abort)) {
@@ -404,7 +473,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
     }
     const int n_entries = SHARED ? (a.B + tpu - 1) / tpu * a.nsp : a.entries ? a.head->n_entries : __shfl_sync(~0u, ends, 31);
     const int n_work = n_entries * a.KH;
-    int issued = 0, qn = 0, auxn = 0;   // blocks, Q loads and corrected blocks so far
+    int issued = 0, qn = 0;   // blocks and Q loads so far
     bool ok = true;
     for (int it = 0; ok; it++) {
       int w = (int)blockIdx.x + it * (int)gridDim.x;
@@ -450,31 +519,12 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
           break;
         }
         uint8_t* dst = kvs + s * TILE;
-        // Values behind the sequence's end belong to others: p = 0 does not
-        // silence an infinity or NaN there, so those rows are zeroed first.
-        // (Keys need nothing: their scores are replaced.)
-        const int end = e.nk - row;
-        const bool fix = v && end < AT_KEYS && e.k0 + e.nk < a.total_k;
-        uint64_t* full = &sh.kv_full[issued % NBAR];
-        uint64_t* bar = fix ? &sh.aux : full;
+        // a V block that not all rows see whole goes through the edge warp
+        uint64_t* bar = v && on_edge(e, row) ? &sh.edge[issued % NBAR] : &sh.kv_full[issued % NBAR];
         if (lane == 0) {
           mbar_arrive_expect_tx(bar, TILE);
           for (int c = 0; c < HD / 64; c++)
             tma_load_3d(dst + c * 16384, v ? &vmap : &kmap, 64 * c, e.k0 + row, kh, bar);
-        }
-        if (fix) {
-          if (!at_wait(&sh.aux, auxn & 1, abort)) {
-            if (lane == 0) fail(304, it);
-            ok = false;
-            break;
-          }
-          auxn++;
-          for (int c = 0; c < HD / 64; c++)
-            for (int o = max(end, 0) * 8 + lane; o < AT_KEYS * 8; o += 32)
-              reinterpret_cast<uint4*>(dst + c * 16384)[o] = make_uint4(0, 0, 0, 0);
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) mbar_arrive(full);
         }
         issued++;
       }
@@ -495,15 +545,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
         }
         return ok;
       };
-      // A place in a ring and its phase, counted on without divisions.
-      struct Ring {
-        uint32_t s, ph;
-        __device__ __forceinline__ void add(uint32_t k, uint32_t n) {
-          s += k;
-          if (s >= n) s -= n, ph ^= 1;
-        }
-      };
-      Ring unit{0, 0}, qr{0, 0}, kv{wid == W0 + 1 ? 0u : 1u, 0};   // kv: the barrier; K and V take turns
+      AttnRing unit{0, 0}, qr{0, 0}, kv{wid == W0 + 1 ? 0u : 1u, 0};   // kv: the barrier; K and V take turns
       // Parities of the tiles' S (or P), a bit each (an indexed array would
       // live in local memory).
       uint32_t bits = 0, last = 0;
@@ -572,6 +614,76 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
       }
     }
     __syncwarp();
+  } else if (wid == W0 + 3) {
+    // ---- edges: p = 0 does not silence an infinity or NaN among the values
+    // that a row must not see.  Rows behind the sequence's end are zeroed, and
+    // such values among the sequence's own rows that not all rows see; those
+    // are noted, and the softmax adds them at the end to the rows that do.
+    AttnRing kv{1, 0}, unit{0, 0};
+    uint32_t bits = 0;   // parities of the edge barriers' next phases
+    bool ok = true;
+    for (; ok; un++) {
+      if (!at_wait_idle(&sh.unit_full[unit.s], unit.ph, abort)) {
+        if (lane == 0) fail(330, un);
+        break;
+      }
+      const AttnEntry e = sh.unit[unit.s];
+      if (sh.unit_kh[unit.s] < 0) break;
+      int nbad = 0;
+      for (int j = 0; j < e.nb; j++, kv.add(2, NBAR)) {
+        const int row = e.ks + j * AT_KEYS;
+        if (!on_edge(e, row)) continue;
+        if (!at_wait_idle(&sh.edge[kv.s], bits >> kv.s & 1, abort)) {
+          if (lane == 0) fail(331, un);
+          ok = false;
+          break;
+        }
+        bits ^= 1u << kv.s;
+        uint8_t* dst = kvs + (kv.s < NST ? kv.s : kv.s - NST) * TILE;
+        const int end = e.k0 + e.nk < a.total_k ? min(AT_KEYS, max(0, e.nk - row)) : AT_KEYS;
+        const int r1 = min(end, max(0, e.el - row)), r2 = min(end, max(r1, e.eh - row));   // not all see [0, r1) and [r2, end)
+        // exponent bits all ones: 1 added to the exponent reaches the sign bit
+        constexpr uint32_t EXP = std::is_same<T, __nv_bfloat16>::value ? 0x7f807f80u : 0x7c007c00u;
+        constexpr uint32_t ONE = std::is_same<T, __nv_bfloat16>::value ? 0x00800080u : 0x04000400u;
+        auto odd = [&](uint32_t x) { return ((x & EXP) + ONE) & 0x80008000u; };
+        auto odd4 = [&](uint4 x) { return odd(x.x) | odd(x.y) | odd(x.z) | odd(x.w); };
+        uint32_t any = 0;
+        for (int c = 0; c < HD / 64; c++) {
+          uint4* p = reinterpret_cast<uint4*>(dst + c * 16384);   // 8 words of 16 bytes a row
+          for (int o = end * 8 + lane; o < AT_KEYS * 8; o += 32) p[o] = make_uint4(0, 0, 0, 0);
+#pragma unroll 4
+          for (int o = lane; o < r1 * 8; o += 32) any |= odd4(p[o]);
+#pragma unroll 4
+          for (int o = r2 * 8 + lane; o < end * 8; o += 32) any |= odd4(p[o]);
+        }
+        if (__any_sync(~0u, any != 0)) {
+          for (int w = 0; w < 4; w++) {   // a lane per row
+            const int r = w * 32 + lane;
+            uint32_t x = 0;
+            if (r < r1 || (r >= r2 && r < end))
+              for (int i = 0; i < HD / 2; i++) {
+                uint32_t* p = reinterpret_cast<uint32_t*>(dst + i / 32 * 16384) + r * 32 + i % 32;
+                const uint32_t m = odd(*p);
+                x |= m;
+                if (m) *p &= ~((m >> 31) * 0xffff0000u | (m >> 15 & 1) * 0xffffu);
+              }
+            const uint32_t rows = __ballot_sync(~0u, x != 0);
+            if (lane == 0 && nbad < AT_EDGES) sh.bad_keys[unit.s][nbad][w] = rows;
+          }
+          if (lane == 0 && nbad < AT_EDGES) {
+            sh.bad_block[unit.s][nbad] = j;
+            sh.bad[unit.s] = un * 16 + nbad + 1;
+          }
+          nbad++;
+        }
+        if (end < AT_KEYS || __any_sync(~0u, any != 0)) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // written to
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.kv_full[kv.s]);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.unit_empty[unit.s]);
+      unit.add(1, AT_UNITS);
+    }
   } else if (wid < W0) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ---- softmax of tile t, a thread per row.  What a block does not need is
@@ -744,8 +856,13 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
           at_fence_after();
         }
         const int kh = *(volatile int*)&sh.unit_kh[un % AT_UNITS];
-        const int slot = e->slot;
+        const int slot = e->slot, us = un % AT_UNITS;
         const bool part = SHARED || slot >= 0;
+        const int noted = *(volatile int*)&sh.bad[us], bad = noted >> 4 == un ? noted & 15 : 0;
+        if (bad && nb > 0) {
+          const char* v = (const char*)((const T*)a.v + (e->k0 + e->ks) * a.sv[0] + kh * a.sv[1]);
+          attn_add_odd<T, HD>(to, v, a.sv[0], a.hd, bad, sh.bad_block[us], sh.bad_keys[us], valid ? lo - e->ks : 1, valid ? hi - e->ks : 0);
+        }
         float inv = 1.f;
         char* at;   // this thread's outputs, or its part of the partial result
         if (part) {
