@@ -121,6 +121,19 @@ def test_prompt_matches_definition(A, case, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_prompt_of_many_sequences(A, dtype):
+    """More sequences than the plan holds at a time, and one long one among them that is split."""
+    rng, g, dt, H, KH, hd = np.random.default_rng(41), gen(41), DT[dtype], 4, 2, 64
+    nq = [int(n) for n in rng.integers(0, 6, 1500)]
+    nk = [n + int(c) for n, c in zip(nq, rng.integers(0, 9, 1500))]
+    nq[1200], nk[1200] = 3, 20000
+    q = rand(g, sum(nq), H, hd, dtype=dt, scale=1.5)
+    k, v = (rand(g, sum(nk), KH, hd, dtype=dt) for _ in range(2))
+    got = A.attention_prompt(q, k, v, ends(nq), ends(nk), max_k=20000)
+    check(got, *prompt_ref(q, k, v, nq, nk, 0, None, 1 / 8))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 def test_prompt_strided_views(A, dtype):
     """Views of one fused q/k/v tensor, of head-major tensors, and a strided output."""
     g, dt, H, KH, hd, nq = gen(2), DT[dtype], 8, 2, 64, [150, 33]
@@ -295,6 +308,7 @@ SHARED = [    # heads, kv heads, head_dim, prefix, cap, lens, window, sinks
     (8, 2, 64, 200, 100, [50, 7], 1, False),
     (32, 4, 128, 5000, 2000, [2000, 1111], 0, False),
     (8, 1, 128, 0, 9000, [9000], 0, True),
+    (4, 2, 64, 40, 300, [(i * 37) % 301 for i in range(300)], 0, False),     # more sequences than a scan takes at once
 ]
 
 
