@@ -369,7 +369,8 @@ int tg_attention_prompt(int dtype, const void *q, const void *k, const void *v, 
 
 /* One new token of each of `batch` sequences: q [batch][n_heads] over the
  * prefix that all share (prefix_k, prefix_v [n_kv_heads][prefix_len], at the
- * positions 0 .. prefix_len - 1, read once for the batch) and the sequence's
+ * positions 0 .. prefix_len - 1, read once for every 256 query rows of a key
+ * head: 32 sequences of 8 heads each) and the sequence's
  * own keys k, v [batch][n_kv_heads][cap] behind it, lens[b] of them (values
  * outside 0 .. max_len count as the nearest inside; max_len <= cap), its
  * newest token's the last.  window, sinks: as above.  weights (or NULL)

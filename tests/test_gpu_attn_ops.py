@@ -255,6 +255,20 @@ def test_prompt_twice_gives_the_same_bits(A):
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
 
 
+def test_empty_calls(A):
+    """No rows, no keys, no sequences: nothing, or zeros."""
+    bf = torch.bfloat16
+    q, k = torch.ones(6, 4, 64, dtype=bf, device="cuda"), torch.ones(0, 2, 64, dtype=bf, device="cuda")
+    assert A.attention_prompt(q[:0], k, k, ends([0]), ends([0])).shape == (0, 4, 64)
+    assert not bool(A.attention_prompt(q, k, k, ends([4, 2]), ends([0, 0])).any())
+    c, n = torch.ones(6, 2, 0, 64, dtype=bf, device="cuda"), torch.zeros(6, dtype=torch.int32, device="cuda")
+    w = torch.zeros(6, 2, 0, device="cuda")
+    assert not bool(A.attention_shared(q, None, None, c, c, n, weights=w).any())
+    assert A.attention_shared(q[:0], None, None, c[:0], c[:0], n[:0]).shape == (0, 4, 64)
+    p = torch.ones(2, 3, 64, dtype=bf, device="cuda")
+    assert bool((A.attention_shared(q, p, p, c, c, n) == 1).all())      # the prefix alone: the mean of ones
+
+
 def test_prompt_offsets_past_the_rows_stay_inside(A):
     """Offsets beyond the tensors read as their ends: no access outside, other sequences unharmed."""
     g = gen(8)

@@ -150,9 +150,9 @@ def attention_shared(q, prefix_k, prefix_v, k, v, lens, *, max_len=None, window=
     """One new token of each sequence over a shared prefix and its own cache.
 
     q [B, H, hd]; prefix_k, prefix_v [KH, P, hd] (None: no prefix), read once
-    for the whole batch; k, v [B, KH, cap, hd]; lens [B] int32 on the device:
-    the own positions of each sequence, its newest token's key the last of
-    them.  The prefix is at the positions 0 .. P - 1, the own keys behind it.
+    for every 256 query rows of a key head (32 sequences of 8 heads); k, v
+    [B, KH, cap, hd]; lens [B] int32 on the device: the own positions of each
+    sequence, its newest token's key the last of them.  The prefix is at the positions 0 .. P - 1, the own keys behind it.
     window > 0: only the last `window` positions.  sinks, scale: as
     attention_prompt.  weights [B, KH, cap] fp32: each own key's softmax
     weight, summed over the query heads that share it, is added in place.
