@@ -28,6 +28,7 @@
 // The prefix is bound by the tensor cores and the own keys by HBM, so the two
 // kernels run side by side, each on its share of the SMs.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "../../include/tinygiant.h"
@@ -546,23 +547,40 @@ struct SharedSpace {
     gp = (G + 7) / 8 * 8;
     const int blocks = (P + AT_KEYS - 1) / AT_KEYS;
     const long long HK = (long long)KH * ngc, stages = (long long)B * HK * ((max_len + OWN_KEYS - 1) / OWN_KEYS);
-    // The SMs' shares, by the time that one SM takes: a block of two tiles of
-    // the prefix about 2 us at head_dim 128, a stage of own keys (64 KB, at the
-    // 54 GB/s that an SM loads) 1.1 us.  Batch 256 on 16,384 keys with up to
-    // 1,024 own ones: 138 us at 80 CTAs for these, 156 at 60, 154 at 148.
-    const double tp = 2.0 * units * KH * blocks, to = 1.1 * stages;
-    own_ctas = 0;
-    if (max_len > 0) {
-      own_ctas = blocks ? std::max(1, std::min(sms - 1, (int)(sms * to / (to + tp) + 0.5))) : sms;
-      own_ctas = (int)std::min((long long)own_ctas, stages);
-    }
-    // Prefix: as many pieces as make the last one end earliest, counting two
-    // blocks' time for a piece's own start and end.
+    // The SMs' shares and the prefix's pieces: those whose end is earliest by
+    // this count (us, measured at head_dim 128 / 64).  A piece takes 1.9 / 1.1 a
+    // block of two tiles and 8 for its start and end; the own keys 8, and an SM
+    // 1.1 / 0.9 a stage (three quarters of the bound max_len, no faster than HBM)
+    // and 1.7 a sequence and head, after which their SMs take pieces too.  Batch 256 on 16,384 keys with up to
+    // 1,024 own ones: 131 us with 72 SMs and 2 pieces, 171 with 78 and 3, 211
+    // with 90 and 2; with up to 256 own ones 105 with 72 and 6, 149 with 32 and 4.
+    own_ctas = max_len > 0 ? (int)std::min((long long)sms, stages) : 0;
     nsp = 0;
-    long long best = 0;
-    for (int n = 1; n <= std::min(blocks, 64); n++) {
-      const long long rounds = ((long long)units * KH * n + sms - 1) / sms, cost = rounds * ((blocks + n - 1) / n + 2);
-      if (!nsp || cost < best) nsp = n, best = cost;
+    const double tb = HD == 128 ? 1.9 : 1.1, ts = 0.75 * (HD == 128 ? 1.1 : 0.9), th = 0.75 * OWN_KEYS * HD * 4 / 6.0e6;
+    const int step = std::max(1, sms / 8), most = max_len > 0 && blocks ? std::max(1, sms - step) : 0;
+    double best = 0;
+    for (int own = std::min(most, step); blocks && own <= most; own += step) {
+      const double free = most ? 8 + std::max((ts * stages + 1.7 * B * HK) / std::min((long long)own, stages), th * stages) : 0;
+      for (int n : {1, 2, 3, 4, 5, 6, 8, 12, 16, 32, 64}) {
+        if (n > blocks) break;
+        const double d = tb * ((blocks + n - 1) / n) + 8;
+        const long long m = (long long)units * KH * n;
+        const double about = std::max(0.0, (m * d + own * free) / sms);
+        double one = std::floor(about / d) * d, two = free + std::max(0.0, std::floor((about - free) / d)) * d;   // both groups' ends
+        long long done = (long long)(one / d + 0.5) * (sms - own) + (long long)((two - free) / d + 0.5) * own;
+        double end = std::max(one, done > 0 && two > free ? two : 0.0);
+        while (done < m) {
+          if (!own || one <= two)
+            end = std::max(end, one += d), done += sms - own;
+          else
+            end = std::max(end, two += d), done += own;
+        }
+        end = std::max(end, free) + 0.5 * n;
+        if (!nsp || end < best) {
+          best = end, nsp = n;
+          if (most) own_ctas = (int)std::min((long long)own, stages);
+        }
+      }
     }
     auto take = [&](size_t n) {
       const size_t o = bytes;
