@@ -1,0 +1,112 @@
+"""Attention operators where the numbers or the calls are unusual: scores
+that are not finite, weights far below the row's largest, windows beyond any
+position, prefix values that are not finite under many window edges.
+
+Tolerances are those of test_gpu_attn_ops.  A weight of more than 2^-25 of
+its row's largest is a normal number in either 16-bit type, so its rounding
+is the unit roundoff that the tolerance has; the weights below are such.
+"""
+import math
+
+import pytest
+
+import tinygiant_b200 as tg
+from test_gpu_attn_ops import DT, attend, check, ends, gen, prompt_ref, rand, shared_ref
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module")
+def A(gpu):
+    from tinygiant_b200 import attention
+    return attention
+
+
+# ---- scores that are not finite: the definition's softmax is NaN for a row
+# that attends to a score of NaN or +inf, and gives a key of -inf no weight.
+# 32 key heads hold one odd key each, at every place among 32, in a block of
+# keys that later rows see whole.
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("poison", [math.nan, math.inf, -math.inf])
+def test_prompt_scores_that_are_not_finite(A, poison, hd, dtype):
+    g, dt, n, KH, H = gen(51), DT[dtype], 420, 32, 64
+    q = rand(g, n, H, hd, dtype=dt)
+    q[..., 0] = q[..., 0].abs() + 0.125                       # an infinity keeps its sign
+    k, v = (rand(g, n, KH, hd, dtype=dt) for _ in range(2))
+    clean = A.attention_prompt(q, k, v, ends([n]))
+    at = 128 + 32 + torch.arange(KH, device="cuda")
+    k[at, torch.arange(KH, device="cuda"), 0] = poison
+    got = A.attention_prompt(q, k, v, ends([n]))
+    sees = (torch.arange(n, device="cuda")[:, None] >= at).repeat_interleave(2, 1)      # [n, H]
+    assert torch.equal(got[~sees], clean[~sees])
+    if poison == -math.inf:                                   # as if the key were not there
+        for kh in (0, 1, 7, 14, 15, 30, 31):
+            rest = torch.arange(n, device="cuda") != at[kh]
+            for h in (2 * kh, 2 * kh + 1):
+                i, j = torch.arange(n, device="cuda")[:, None], torch.arange(n, device="cuda")
+                kk = torch.where(rest[:, None], k[:, kh], 0.0)
+                o, _, a, d = attend(q[:, h], kk, v[:, kh], (j <= i) & rest, hd ** -0.5, None)
+                check(got[:, h], o, a, d)
+        assert not bool(torch.isnan(got).any())
+    else:
+        assert bool(torch.isnan(got[sees]).all()), int((~torch.isnan(got[sees])).any(-1).sum())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("poison", [math.nan, math.inf, -math.inf])
+def test_prefix_scores_that_are_not_finite(A, poison, hd, dtype):
+    g, dt, P, KH, H, lens = gen(52), DT[dtype], 384, 32, 64, [9, 0, 40]
+    q = rand(g, 3, H, hd, dtype=dt)
+    q[..., 0] = q[..., 0].abs() + 0.125
+    pk, pv = (rand(g, KH, P, hd, dtype=dt) for _ in range(2))
+    k, v = (rand(g, 3, KH, 40, hd, dtype=dt) for _ in range(2))
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    heads = torch.arange(KH, device="cuda")
+    pk[heads, 128 + 64 + heads, 0] = poison
+    w = torch.zeros(3, KH, 40, device="cuda")
+    got = A.attention_shared(q, pk, pv, k, v, n, weights=w)
+    if poison == -math.inf:
+        keep = torch.stack([torch.cat([torch.arange(192 + h), torch.arange(193 + h, P)]) for h in range(KH)]).cuda()
+        at = keep[..., None].expand(KH, P - 1, hd)
+        out, a, delta, ww, wd = shared_ref(q, torch.gather(pk, 1, at), torch.gather(pv, 1, at), k, v, lens, 0, None, hd ** -0.5)
+        check(got, out, a, delta)
+        assert bool(((w.double() - ww).abs() <= 1.05 * wd + ww * 2.0 ** -22).all())
+    else:
+        assert bool(torch.isnan(got).all()), int((~torch.isnan(got)).sum())
+        there = torch.arange(40, device="cuda") < n[:, None]
+        assert bool(torch.isnan(w.transpose(1, 2)[there]).all()) and not bool(w.transpose(1, 2)[~there].any())
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_rows_whose_scores_are_all_minus_infinity(A, hd):
+    """No key has any weight: zeros, as for a row without a key; a later finite score takes everything."""
+    g, n, H, KH = gen(53), 600, 4, 2
+    q, k, v = rand(g, n, H, hd, dtype=torch.bfloat16), *(rand(g, n, KH, hd, dtype=torch.bfloat16) for _ in range(2))
+    q[..., 0] = 1
+    k[:, 0, 0] = -math.inf
+    k[:400, 1, 0] = -math.inf
+    got = A.attention_prompt(q, k, v, ends([n]))
+    assert not bool(got[:, :2].any()) and not bool(got[:400, 2:].any())
+    check(got[400:, 2:], *prompt_ref(q[400:, 2:], k[400:, 1:], v[400:, 1:], [200], [200], 0, None, hd ** -0.5))
+    sinks = torch.zeros(H, device="cuda")
+    assert not bool(A.attention_prompt(q, k, v, ends([n]), sinks=sinks)[:, :2].any())
+    pk, pv = k.transpose(0, 1).contiguous(), v.transpose(0, 1).contiguous()
+    c = torch.zeros(2, KH, 8, hd, dtype=torch.bfloat16, device="cuda")
+    got = A.attention_shared(q[:2], pk[:, :384], pv[:, :384], c, c, torch.zeros(2, dtype=torch.int32, device="cuda"))
+    assert not bool(got.any())
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_a_query_that_is_not_finite_stays_in_its_row(A, hd):
+    g, n, H, KH = gen(54), 700, 4, 2
+    q, k, v = rand(g, n, H, hd, dtype=torch.bfloat16), *(rand(g, n, KH, hd, dtype=torch.bfloat16) for _ in range(2))
+    clean = A.attention_prompt(q, k, v, ends([n]))
+    q[5, 1, 3], q[333, 2, 0], q[699, 0, 1] = math.nan, math.inf, -math.inf
+    got = A.attention_prompt(q, k, v, ends([n]))
+    bad = torch.zeros(n, H, dtype=torch.bool, device="cuda")
+    bad[5, 1] = bad[333, 2] = bad[699, 0] = True
+    assert torch.equal(got[~bad], clean[~bad]) and bool(torch.isnan(got[bad]).all())

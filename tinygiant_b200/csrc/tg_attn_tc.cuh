@@ -202,9 +202,15 @@ __device__ __forceinline__ float at_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Maxima that are NaN if an operand is.
 __device__ __forceinline__ float at_max3(float a, float b, float c) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float at_max2(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
 template <typename T>
@@ -238,7 +244,8 @@ __device__ __forceinline__ float2 at_add2(float2 a, float2 b) {
   return d;
 }
 
-// 2^x of a pair on the FMA units, x >= -126 (less counts as that): x = n + f
+// 2^x of a pair on the FMA units, x >= -126 (less, and NaN, counts as that; a
+// row with a score of NaN or +inf becomes NaN by its other keys, see cm): x = n + f
 // with f in [-1/2, 1/2], 2^f by the degree-4 polynomial of least relative
 // error there (2.6e-6, fitted by reweighted least squares), n added to the
 // exponent.
@@ -774,7 +781,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
 #pragma unroll
             for (int z = 0; z < 4; z++) mx[z] = at_max3(mx[z], s[32 * i + q + z], s[32 * i + q + z + 4]);
         }
-        const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        const float mn = at_max3(mx[0], mx[1], at_max2(mx[2], mx[3]));
         // P V of the block before: its P may be overwritten, its O scaled (a
         // barrier's phase before its first counts as complete)
         if (!at_wait(&sh.p_empty[t], (par & 1) ^ 1, abort)) {
@@ -804,7 +811,11 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
             }
           }
         }
-        const float cm = m == -INFINITY ? 0.f : -c * m;
+        // Not finite: a score of NaN or +inf makes mn NaN or +inf, then cm and
+        // with it every p of the special function unit NaN, as the softmax is.
+        // While all scores are -inf, m is too: their p count as 0 (those of the
+        // FMA units are 2^-126; a first larger score scales them, and l, by 0).
+        const float cm = mn == -INFINITY ? 0.f : fmaf(m, -c, mn - mn);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         auto scaled = [&](int i) {   // c s - c m of the pair i
           return at_fma2(make_float2(s[2 * i], s[2 * i + 1]), make_float2(c, c), make_float2(cm, cm));
@@ -856,6 +867,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
       }
       if (!ok) break;
       if (mine) {
+        if (m == -INFINITY) l *= 0.f;   // no key, or none above -inf; NaN stays
         const int us = un % AT_UNITS, kh = *(volatile int*)&sh.unit_kh[us], slot = e->slot;
         const bool part = SHARED || slot >= 0;
         float inv = 1.f;
