@@ -110,3 +110,28 @@ def test_a_query_that_is_not_finite_stays_in_its_row(A, hd):
     bad = torch.zeros(n, H, dtype=torch.bool, device="cuda")
     bad[5, 1] = bad[333, 2] = bad[699, 0] = True
     assert torch.equal(got[~bad], clean[~bad]) and bool(torch.isnan(got[bad]).all())
+
+
+# ---- values that are not finite in more partly seen blocks than a unit notes
+
+@pytest.mark.parametrize("poison", [math.inf, math.nan])
+def test_prefix_values_under_many_window_edges(A, poison):
+    """Sequences whose windows begin all over the prefix, an odd value in each block: those that see it get it."""
+    g, dt, H, KH, hd, P, cap, window = gen(55), torch.bfloat16, 16, 16, 64, 4000, 2048, 4100
+    lens = [100, 1999, 400, 700, 1000, 1300, 1600, 1900]      # first keys seen: len - 100
+    q = rand(g, 8, H, hd, dtype=dt)
+    pk, pv = (rand(g, KH, P, hd, dtype=dt) for _ in range(2))
+    k, v = (rand(g, 8, KH, cap, hd, dtype=dt) for _ in range(2))
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    clean = A.attention_shared(q, pk, pv, k, v, n, window=window)
+    at = list(range(60, 2000, 64))                            # two in every block that some see in part
+    for i, j in enumerate(at):
+        pv[3, j, i] = poison
+    got = A.attention_shared(q, pk, pv, k, v, n, window=window)
+    want = clean.clone()
+    for i, j in enumerate(at):
+        for b, m in enumerate(lens):
+            if j >= P + m - window:
+                want[b, 3, i] = poison
+    same = (got == want) | (torch.isnan(got) & (torch.isnan(want) | torch.isinf(want)))   # 0 times infinity may be NaN
+    assert bool(same.all()), int((~same).sum())

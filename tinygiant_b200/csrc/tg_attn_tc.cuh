@@ -55,7 +55,10 @@ constexpr int AT_SOFT = 8;         // softmax warps; then one each for loads, S,
 constexpr int AT_THREADS = 384;
 constexpr int AT_NPOS = 0x3fffffff;
 constexpr int AT_UNITS = 4;        // units announced ahead
-constexpr int AT_EDGES = 8;        // a unit's blocks that some rows see in part, at most (2 tiles of 128 tokens, both ends)
+// A unit's noted blocks of values that not all rows see.  A prompt's unit has no
+// more (2 tiles of 128 tokens, both ends); a prefix's may, as its sequences'
+// windows begin wherever their lengths put them: then all are looked through.
+constexpr int AT_EDGES = 8;
 
 // One piece of work of every key head.
 struct __align__(16) AttnEntry {
@@ -290,7 +293,8 @@ struct AttnTcShared {
   AttnEntry unit[AT_UNITS];
   int unit_kh[AT_UNITS];      // -1: no more work
   // Edge blocks with values that are not finite: 16 times the unit's number
-  // and how many; each one's block and its keys, a bit each.
+  // and how many (AT_EDGES + 1: more than are noted); each one's block and its
+  // keys, a bit each.
   int bad[AT_UNITS], bad_block[AT_UNITS][AT_EDGES];
   uint32_t bad_keys[AT_UNITS][AT_EDGES][4];
   uint32_t tmem;
@@ -352,6 +356,50 @@ __device__ __noinline__ void attn_add_odd(uint32_t to, const char* v, long long 
     __syncwarp();
     at_st16(to + 16 * i, o);
     at_wait_st();
+  }
+}
+
+// Whether a pair of 16-bit values has one that is not finite, a bit for each:
+// its exponent bits are all ones, so 1 added to the exponent reaches the sign.
+template <typename T>
+__device__ __forceinline__ uint32_t at_odd(uint32_t x) {
+  constexpr uint32_t EXP = std::is_same<T, __nv_bfloat16>::value ? 0x7f807f80u : 0x7c007c00u;
+  constexpr uint32_t ONE = std::is_same<T, __nv_bfloat16>::value ? 0x00800080u : 0x04000400u;
+  return ((x & EXP) + ONE) & 0x80008000u;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t at_odd4(uint4 x) {
+  return at_odd<T>(x.x) | at_odd<T>(x.y) | at_odd<T>(x.z) | at_odd<T>(x.w);
+}
+
+// The same for more blocks than are noted: the unit's first n keys, which not
+// all rows see, are read again, a lane per key.
+template <typename T, int HD>
+__device__ __noinline__ void attn_add_odd_front(uint32_t to, const char* v, long long stride, int hd, int n, int lo, int hi) {
+  const int lane = threadIdx.x & 31;
+  for (int k0 = 0; k0 < n; k0 += 32) {
+    uint32_t odd = 0;
+    if (k0 + lane < n) {
+      const uint4* x = (const uint4*)((const T*)v + (k0 + lane) * stride);
+      for (int i = 0; i < hd / 8; i++) odd |= at_odd4<T>(x[i]);
+    }
+    for (uint32_t keys = __ballot_sync(~0u, odd != 0); keys; keys &= keys - 1) {
+      const int key = k0 + __ffs(keys) - 1;
+      const T* x = (const T*)v + key * stride;
+      for (int i = 0; i < HD / 16; i++) {
+        uint32_t o[16];
+        at_ld16(to + 16 * i, o);
+        at_wait_ld();
+#pragma unroll
+        for (int q = 0; q < 16; q++) {
+          const float y = key >= lo && key < hi && 16 * i + q < hd ? to_f32(x[16 * i + q]) : 0.f;
+          if (!isfinite(y)) o[q] = __float_as_uint(__uint_as_float(o[q]) + y);
+        }
+        __syncwarp();
+        at_st16(to + 16 * i, o);
+        at_wait_st();
+      }
+    }
   }
 }
 
@@ -657,19 +705,14 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
         uint8_t* dst = kvs + (kv.s < NST ? kv.s : kv.s - NST) * TILE;
         const int end = e.k0 + e.nk < a.total_k ? min(AT_KEYS, max(0, e.nk - row)) : AT_KEYS;
         const int r1 = min(end, max(0, e.el - row)), r2 = min(end, max(r1, e.eh - row));   // not all see [0, r1) and [r2, end)
-        // exponent bits all ones: 1 added to the exponent reaches the sign bit
-        constexpr uint32_t EXP = std::is_same<T, __nv_bfloat16>::value ? 0x7f807f80u : 0x7c007c00u;
-        constexpr uint32_t ONE = std::is_same<T, __nv_bfloat16>::value ? 0x00800080u : 0x04000400u;
-        auto odd = [&](uint32_t x) { return ((x & EXP) + ONE) & 0x80008000u; };
-        auto odd4 = [&](uint4 x) { return odd(x.x) | odd(x.y) | odd(x.z) | odd(x.w); };
         uint32_t any = 0;
         for (int c = 0; c < HD / 64; c++) {
           uint4* p = reinterpret_cast<uint4*>(dst + c * 16384);   // 8 words of 16 bytes a row
           for (int o = end * 8 + lane; o < AT_KEYS * 8; o += 32) p[o] = make_uint4(0, 0, 0, 0);
 #pragma unroll 4
-          for (int o = lane; o < r1 * 8; o += 32) any |= odd4(p[o]);
+          for (int o = lane; o < r1 * 8; o += 32) any |= at_odd4<T>(p[o]);
 #pragma unroll 4
-          for (int o = r2 * 8 + lane; o < end * 8; o += 32) any |= odd4(p[o]);
+          for (int o = r2 * 8 + lane; o < end * 8; o += 32) any |= at_odd4<T>(p[o]);
         }
         if (__any_sync(~0u, any != 0)) {
           for (int w = 0; w < 4; w++) {   // a lane per row
@@ -678,16 +721,16 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
             if (r < r1 || (r >= r2 && r < end))
               for (int i = 0; i < HD / 2; i++) {
                 uint32_t* p = reinterpret_cast<uint32_t*>(dst + i / 32 * 16384) + r * 32 + i % 32;
-                const uint32_t m = odd(*p);
+                const uint32_t m = at_odd<T>(*p);
                 x |= m;
                 if (m) *p &= ~((m >> 31) * 0xffff0000u | (m >> 15 & 1) * 0xffffu);
               }
             const uint32_t rows = __ballot_sync(~0u, x != 0);
             if (lane == 0 && nbad < AT_EDGES) sh.bad_keys[unit.s][nbad][w] = rows;
           }
-          if (lane == 0 && nbad < AT_EDGES) {
-            sh.bad_block[unit.s][nbad] = j;
-            sh.bad[unit.s] = un * 16 + nbad + 1;
+          if (lane == 0) {
+            if (nbad < AT_EDGES) sh.bad_block[unit.s][nbad] = j;
+            sh.bad[unit.s] = un * 16 + min(nbad, AT_EDGES) + 1;
           }
           nbad++;
         }
@@ -890,7 +933,11 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
           const int noted = *(volatile int*)&sh.bad[us], bad = noted >> 4 == un ? noted & 15 : 0;
           if (bad) {
             const char* v = (const char*)((const T*)a.v + (e->k0 + e->ks) * a.sv[0] + kh * a.sv[1]);
-            attn_add_odd<T, HD>(to, v, a.sv[0], a.hd, bad, sh.bad_block[us], sh.bad_keys[us], valid ? lo - e->ks : 1, valid ? hi - e->ks : 0);
+            const int from = valid ? lo - e->ks : 1, end = valid ? hi - e->ks : 0;
+            if (bad <= AT_EDGES)
+              attn_add_odd<T, HD>(to, v, a.sv[0], a.hd, bad, sh.bad_block[us], sh.bad_keys[us], from, end);
+            else if (SHARED)
+              attn_add_odd_front<T, HD>(to, v, a.sv[0], a.hd, min(min(e->el, e->nk) - e->ks, nb * AT_KEYS), from, end);
           }
         }
 #pragma unroll
