@@ -135,3 +135,41 @@ def test_prefix_values_under_many_window_edges(A, poison):
                 want[b, 3, i] = poison
     same = (got == want) | (torch.isnan(got) & (torch.isnan(want) | torch.isinf(want)))   # 0 times infinity may be NaN
     assert bool(same.all()), int((~same).sum())
+
+
+# ---- weights far below the largest that together matter
+
+def rare_heavy(g, n, KH, hd, dt, low):
+    """Keys with a score of 0 and no value at every 32nd place, the others at `low` with values about 1000."""
+    k = torch.zeros(n, KH, hd, device="cuda")
+    k[..., 0] = low
+    v = 1000 + 50 * torch.randn(n, KH, hd, generator=g, device="cuda")
+    k[::32, :, 0] = 0
+    v[::32] = 0
+    return k.to(dt), v.to(dt)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("low", [-12, -17])
+def test_weights_far_below_the_largest(A, low, hd, dtype):
+    """exp(-17) = 2^-24.5: below what an fp16 number resolves beside 1, yet all of the output."""
+    g, dt, n, H, KH = gen(56), DT[dtype], 6400, 4, 2
+    k, v = rare_heavy(g, n, KH, hd, dt, low)
+    q = torch.zeros(8, H, hd, device="cuda")
+    q[..., 0] = 1
+    q = q.to(dt)
+    check(A.attention_prompt(q, k, v, ends([8]), ends([n]), scale=1.0), *prompt_ref(q, k, v, [8], [n], 0, None, 1.0))
+    sinks = torch.tensor([-math.inf, 0.0, 3.0, -20.0], device="cuda")
+    got = A.attention_prompt(q, k, v, ends([8]), ends([n]), scale=1.0, sinks=sinks)
+    check(got, *prompt_ref(q, k, v, [8], [n], 0, sinks, 1.0))
+    kh, vh = k.transpose(0, 1)[None].expand(2, KH, n, hd).contiguous(), v.transpose(0, 1)[None].expand(2, KH, n, hd).contiguous()
+    lens = [n, 3201]
+    nn = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    for pk, pv in ((None, None), (kh[0, :, :3200].contiguous(), vh[0, :, :3200].contiguous())):
+        w = torch.zeros(2, KH, n, device="cuda")
+        out, a, delta, ww, wd = shared_ref(q[:2], pk, pv, kh, vh, lens, 0, sinks, 1.0)
+        check(A.attention_shared(q[:2], pk, pv, kh, vh, nn, scale=1.0, sinks=sinks, weights=w), out, a, delta)
+        assert bool(((w.double() - ww).abs() <= 1.05 * wd + ww * 2.0 ** -22).all())
+    out, a, delta, _, _ = shared_ref(q[:2], pk, pv, kh, vh, [0, 0], 0, None, 1.0)
+    check(A.attention_shared(q[:2], pk, pv, kh, vh, nn * 0, scale=1.0), out, a, delta)

@@ -48,7 +48,7 @@ struct OwnArgs {
   const void* q;
   const int* lens;
   float* po;          // [segment][8 NT][HD], see OwnWalk
-  float2* pml;        // [segment][8 NT]: (c m, l)
+  float2* pml;        // [segment][8 NT]: (c m - OFF, l)
   int* starts;        // [batch + 1]: stages of a key head before each sequence
   float* scores;      // [b KH + kh][max_len][gp] c s, or null
   long long sq[2];
@@ -165,7 +165,7 @@ struct OwnWalk {
 // Persistent, one CTA per SM of its share.  Warp 8 loads stages ahead, across
 // segments.  Warps 0-3 and 4-7 take stages in turn, each warp 32 keys with a
 // reference m of its own (moved, as in attn_tc_kernel, only when a score
-// exceeds it by 8 in base 2: one vote in the common case); the warps' partial
+// exceeds it by LIFT in base 2: one vote in the common case); the warps' partial
 // results join in shared memory at the end of a segment.  Bound by HBM: 442 MB
 // in 76 us on all SMs (batch 256, 768 keys on average), 0.89 of measured.
 template <typename T, int HD, int NT>
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(OWN_THREADS, 1) own_kernel(const __grid_consta
 #pragma unroll
       for (int k = 0; k < HD / 16; k++) o[t][k][0] = o[t][k][1] = o[t][k][2] = o[t][k][3] = 0.f;
     }
-    // reference m in base 2, as -m and as the score that exceeds it by 8
+    // reference m in base 2, as OFF - m and as the score that exceeds it by LIFT
     float nm[NT][2], lim[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; t++) nm[t][0] = nm[t][1] = 0.f, lim[t][0] = lim[t][1] = -INFINITY;
@@ -361,8 +361,8 @@ __global__ void __launch_bounds__(OWN_THREADS, 1) own_kernel(const __grid_consta
             for (int sft = 4; sft < 32; sft <<= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, sft));
             const float mn = fmaxf(m[t][z], v * a.c), f = mn > m[t][z] ? at_exp2(m[t][z] - mn) : 1.f;
             m[t][z] = mn;
-            nm[t][z] = mn == -INFINITY ? 0.f : -mn;
-            lim[t][z] = (mn + 8.f) * a.inv_c;
+            nm[t][z] = mn == -INFINITY ? 0.f : AttnRange<T>::OFF - mn;
+            lim[t][z] = (mn + AttnRange<T>::LIFT) * a.inv_c;
             l[t][z] *= f;
 #pragma unroll
             for (int k = 0; k < HD / 16; k++) {
@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(OWN_THREADS, 1) own_kernel(const __grid_consta
       for (int z = 0; z < 2; z++) {
 #pragma unroll
         for (int sft = 4; sft < 32; sft <<= 1) l[t][z] += __shfl_xor_sync(~0u, l[t][z], sft);
-        if (g == 0) sh.ml[wid][cc * 2 + z] = make_float2(m[t][z], l[t][z]);
+        if (g == 0) sh.ml[wid][cc * 2 + z] = make_float2(m[t][z] - AttnRange<T>::OFF, l[t][z]);
       }
 #pragma unroll
       for (int k = 0; k < HD / 16; k++)

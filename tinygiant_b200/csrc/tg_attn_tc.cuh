@@ -7,12 +7,12 @@
 //   p_j = 2^(c s_j - c m),  l += p_j,  o += p_j v_j;   result o / l.
 // m starts as the first block's maximum.  It moves (with l and o scaled by
 // 2^(c m_old - c m_new)) only when a block's maximum exceeds it by more than
-// 2^8 in the exponent's base: results do not depend on the reference, fp32
-// sums and 16-bit p_j hold 2^8 as well as 1, and o is then rarely touched.
-// p_j is rounded to the inputs' type for the second product, as tcgen05 wants
-// both operands of one type; its error there is that of rounding v once more
-// (unit roundoff 2^-8 or 2^-11 of the weighted mean of |v|), the order of the
-// output's own rounding.  l sums the unrounded p_j.
+// 2^8 (fp16: 2^4) in the exponent's base: results do not depend on the
+// reference, and o is then rarely touched.  p_j is rounded to the inputs' type
+// for the second product, as tcgen05 wants both operands of one type; its error
+// there is that of rounding v once more (unit roundoff 2^-8 or 2^-11 of the
+// weighted mean of |v|), the order of the output's own rounding; fp16's range
+// is used whole for that (AttnRange).  l sums the unrounded p_j.
 //
 // Work unit: one key head, two tiles of 128 query rows.  A tile's rows are
 // (token, query head of the group) pairs, token-major, so a group of G heads
@@ -115,7 +115,7 @@ struct AttnTcArgs {
   int n_seqs, total_q;
   void* out;
   float* po;                  // partial results [slot * KH + kh][2 * 128][HD]
-  float2* pml;                // their (c m, l) [slot * KH + kh][2 * 128]
+  float2* pml;                // their (c m - OFF, l) [slot * KH + kh][2 * 128]
   const float* sinks;
   const int* lens;            // shared: own keys of each sequence
   long long so[2];
@@ -838,7 +838,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
           m = mn;
         } else {
           const float d = (mn - m) * c;
-          const bool up = d > 8.f;
+          const bool up = d > AttnRange<T>::LIFT;
           if (__any_sync(~0u, up)) {
             const float f = up ? at_exp2(-d) : 1.f;
             if (up) m = mn;
@@ -858,9 +858,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
         // with it every p of the special function unit NaN, as the softmax is.
         // While all scores are -inf, m is too: their p count as 0 (those of the
         // FMA units are 2^-126; a first larger score scales them, and l, by 0).
-        const float cm = mn == -INFINITY ? 0.f : fmaf(m, -c, mn - mn);
+        const float cm = mn == -INFINITY ? 0.f : fmaf(m, -c, mn - mn + AttnRange<T>::OFF);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        auto scaled = [&](int i) {   // c s - c m of the pair i
+        auto scaled = [&](int i) {   // c s - c m + OFF of the pair i
           return at_fma2(make_float2(s[2 * i], s[2 * i + 1]), make_float2(c, c), make_float2(cm, cm));
         };
         if (clean) {
@@ -917,10 +917,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
         char* at;   // this thread's outputs, or its part of the partial result
         if (part) {
           const size_t pr = ((size_t)slot * a.KH + kh) * (2 * AT_ROWS) + tid;
-          if (valid) a.pml[pr] = make_float2(l == 0.f ? -INFINITY : c * m, l);
+          if (valid) a.pml[pr] = make_float2(l == 0.f ? -INFINITY : c * m - AttnRange<T>::OFF, l);
           at = (char*)(a.po + pr * HD);
         } else {
-          if (l != 0.f) l += at_exp2(fmaf(sink, LOG2E, -c * m));
+          if (l != 0.f) l += at_exp2(fmaf(sink, LOG2E, AttnRange<T>::OFF - c * m));
           inv = l == 0.f ? 0.f : 1.f / l;
           at = (char*)((T*)a.out + (e->q0 + t * a.tpt + tok) * a.so[0] + (kh * a.G + g) * a.so[1]);
         }
@@ -984,9 +984,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
 }
 
 // ---------------------------------------------------------------------
-// Joining partial results.  A row's pieces have (c m, l) in pml and their
-// accumulators of HD values in po; row(i) is the place of piece i of n.
-//   M = max(c m_i, sink),  f_i = 2^(c m_i - M),
+// Joining partial results.  A row's pieces have (m_i, l_i) in pml, m_i = c m -
+// OFF (the factor 2^OFF of their sums taken out), and their accumulators of HD
+// values in po; row(i) is the place of piece i of n.
+//   M = max(m_i, sink),  f_i = 2^(m_i - M),
 //   o = sum f_i o_i / (sum f_i l_i + 2^(sink - M)).
 // A warp per row: its lanes weigh 32 pieces at a time, then add them up eight
 // at a time with HD / 32 dimensions each.  Pieces without a key (l = 0) have
