@@ -173,3 +173,27 @@ def test_weights_far_below_the_largest(A, low, hd, dtype):
         assert bool(((w.double() - ww).abs() <= 1.05 * wd + ww * 2.0 ** -22).all())
     out, a, delta, _, _ = shared_ref(q[:2], pk, pv, kh, vh, [0, 0], 0, None, 1.0)
     check(A.attention_shared(q[:2], pk, pv, kh, vh, nn * 0, scale=1.0), out, a, delta)
+
+
+# ---- windows beyond any position
+
+@pytest.mark.parametrize("window", [2 ** 30, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5, 2 ** 40])
+def test_windows_beyond_any_position(A, window):
+    """They are no window, also where queries precede the first key."""
+    g, dt = gen(57), torch.bfloat16
+    q, k, v = rand(g, 40, 4, 64, dtype=dt), *(rand(g, 20, 2, 64, dtype=dt) for _ in range(2))
+    want = A.attention_prompt(q, k, v, ends([40]), ends([20]))
+    check(want, *prompt_ref(q, k, v, [40], [20], 0, None, 1 / 8))
+    assert torch.equal(A.attention_prompt(q, k, v, ends([40]), ends([20]), window=window), want)
+    c, n = rand(g, 4, 2, 8, 64, dtype=dt), torch.tensor([8, 0, 3, 5], dtype=torch.int32, device="cuda")
+    p = rand(g, 2, 300, 64, dtype=dt)
+    check(A.attention_shared(q[:4], p, p, c, c, n, window=window), *shared_ref(q[:4], p, p, c, c, [8, 0, 3, 5], 0, None, 1 / 8)[:3])
+
+
+def test_windows_below_zero_are_refused(A):
+    q, c = torch.zeros(4, 4, 64, dtype=torch.bfloat16, device="cuda"), torch.zeros(4, 2, 8, 64, dtype=torch.bfloat16, device="cuda")
+    for window in (-1, -2 ** 31, -2 ** 32, 1 - 2 ** 32):
+        with pytest.raises(ValueError, match="window"):
+            A.attention_prompt(q, c[:, :, 0], c[:, :, 0], ends([4]), window=window)
+        with pytest.raises(ValueError, match="window"):
+            A.attention_shared(q, None, None, c, c, ends([1] * 3), window=window)

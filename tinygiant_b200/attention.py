@@ -30,6 +30,7 @@ from . import TinyGiantCudaError, last_error, load
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _I64x8, _I64x16 = ctypes.c_int64 * 8, ctypes.c_int64 * 16
+_MOST = 0x7fffffff                                 # no position is beyond it
 _empty = torch.empty_strided                       # less host time than torch.empty
 _raw_stream = torch._C._cuda_getCurrentRawStream   # torch.cuda.current_stream(i).cuda_stream, without its objects
 
@@ -47,6 +48,13 @@ def _call(device, fn, *args):
     if rc:
         code, msg = last_error()
         raise (ArgumentError if rc == 3 else TinyGiantCudaError)(f"[{code}] {msg}")
+
+
+def _window(n):
+    """A window as the library's 32-bit argument: one beyond any position is as good as the largest."""
+    if n < 0:
+        raise ValueError(f"window must not be negative; is {n}")
+    return n if n < _MOST else _MOST
 
 
 def _ptr(t):
@@ -141,7 +149,7 @@ def attention_prompt(q, k, v, cu_q, cu_k=None, *, max_k=None, window=0, sinks=No
     (q0, q1, _), (k0, k1, _), (v0, v1, _), (o0, o1, _) = q.stride(), k.stride(), v.stride(), out.stride()
     _call(dev, lib.tg_attention_prompt, _DTYPES[dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
           cu_q.data_ptr(), cu_k.data_ptr(), _ptr(sinks), n, tq, tk, max_k, H, KH, hd,
-          _I64x8(q0, q1, k0, k1, v0, v1, o0, o1), window, hd ** -0.5 if scale is None else scale, _ptr(ws), nbytes)
+          _I64x8(q0, q1, k0, k1, v0, v1, o0, o1), _window(window), hd ** -0.5 if scale is None else scale, _ptr(ws), nbytes)
     return out
 
 
@@ -193,7 +201,7 @@ def attention_shared(q, prefix_k, prefix_v, k, v, lens, *, max_len=None, window=
     w0, w1, _ = weights.stride() if weights is not None else (1, 1, 1)
     _call(dev, lib.tg_attention_shared, _DTYPES[dtype], q.data_ptr(), _ptr(prefix_k), _ptr(prefix_v), k.data_ptr(),
           v.data_ptr(), out.data_ptr(), lens.data_ptr(), _ptr(sinks), _ptr(weights), B, P, cap, max_len, H, KH, hd,
-          _I64x16(q0, q1, pk0, pk1, pv0, pv1, k0, k1, k2, v0, v1, v2, o0, o1, w0, w1), window,
+          _I64x16(q0, q1, pk0, pk1, pv0, pv1, k0, k1, k2, v0, v1, v2, o0, o1, w0, w1), _window(window),
           hd ** -0.5 if scale is None else scale, _ptr(ws), nbytes)
     return out
 

@@ -304,6 +304,7 @@ extern "C" int tg_attention_prompt(int dtype, const void* q, const void* k, cons
   for (int i = 0; i < 8; i++) st[i] = c.stride(strides[i], n4[dim[i]]);
   if (c.rc || total_q == 0) return c.rc;
   c.need(n_seqs > 0, "rows without a sequence");
+  window = std::min(window, AT_NPOS);   // beyond any position: position - window stays an int
   if (!c.device()) return c.rc;
   c.ptr(q, 16, "q"), c.ptr(out, 16, "out"), c.ptr(cu_q, 4, "cu_q"), c.ptr(cu_k, 4, "cu_k");
   if (total_k > 0) c.ptr(k, 16, "k"), c.ptr(v, 16, "v");
