@@ -197,3 +197,56 @@ def test_windows_below_zero_are_refused(A):
             A.attention_prompt(q, c[:, :, 0], c[:, :, 0], ends([4]), window=window)
         with pytest.raises(ValueError, match="window"):
             A.attention_shared(q, None, None, c, c, ends([1] * 3), window=window)
+
+
+# ---- evictions of caches of different lengths at the same time
+
+def evict_args(cap, keep):
+    g = gen(58)
+    k = rand(g, 1, 1, cap, 8, dtype=torch.bfloat16)
+    return k, k, torch.rand(1, 1, cap, generator=g, device="cuda"), torch.tensor([cap], dtype=torch.int32, device="cuda"), keep, 3
+
+
+def test_a_shorter_eviction_leaves_a_captured_longer_one(A):
+    """A smaller cache's call between the capture of a larger one's and its instantiation."""
+    big, small = evict_args(40000, 100), evict_args(9000, 50)
+    want, less = A.cache_evict(*big), A.cache_evict(*small)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = A.cache_evict(*big)
+        got2 = A.cache_evict(*small)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, want)) and all(torch.equal(x, y) for x, y in zip(got2, less))
+
+
+def test_evictions_from_two_threads(gpu):
+    """Long and short caches cut down at the same time, many times, through the C entry (Python leaves its lock meanwhile)."""
+    import ctypes
+    import threading
+    refused = []
+
+    def args_of(cap, stream):
+        k, _, w, n, keep, recent = evict_args(cap, 64)
+        outs = [torch.zeros(keep * 8, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+        outs += [torch.zeros(keep, device="cuda"), *(torch.zeros(m, dtype=torch.int32, device="cuda") for m in (1, keep))]
+        strides = (ctypes.c_int64 * 8)(cap * 8, cap * 8, 8, cap * 8, cap * 8, 8, cap, cap)
+        return (k, w, n, outs, strides), (k.data_ptr(), k.data_ptr(), w.data_ptr(), n.data_ptr(), *(x.data_ptr() for x in outs), 1, cap, 1,
+                                          8, ctypes.addressof(strides), keep, recent, stream.cuda_stream)
+
+    def loop(args):
+        for _ in range(30000):
+            if gpu.tg_cache_evict(*args):
+                refused.append(tg.last_error(gpu))
+                return
+
+    keep, args = zip(*(args_of(cap, torch.cuda.Stream()) for cap in (40000, 9000)))
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=loop, args=(a,)) for a in args]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not refused, refused
+    del keep

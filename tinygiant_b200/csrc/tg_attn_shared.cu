@@ -599,13 +599,8 @@ struct SharedSpace {
 template <typename T, int HD, int NT>
 static cudaError_t launch_own(const CUtensorMap* m, const OwnArgs& a, int grid, cudaStream_t s) {
   const int smem = OwnShape<HD>::SMEM;
-  static std::atomic<unsigned long long> set{0};   // devices whose limit is raised
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess && (dev >= 64 || !(set.load() >> dev & 1))) {
-    e = cudaFuncSetAttribute(own_kernel<T, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess && dev < 64) set |= 1ull << dev;
-  }
+  static std::atomic<unsigned long long> set{0};
+  const cudaError_t e = attn_smem(own_kernel<T, HD, NT>, smem, set);
   if (e != cudaSuccess) return e;
   return launch_pdl(own_kernel<T, HD, NT>, dim3(grid), OWN_THREADS, smem, s, m[0], m[1], m[2], m[3], a);
 }

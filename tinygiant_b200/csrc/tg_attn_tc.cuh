@@ -1123,17 +1123,26 @@ inline int attn_sms() {   // SMs of the current device
   return sms[dev];
 }
 
+// Raises a kernel's dynamic shared-memory limit on the current device, once, to
+// the most that any launch of it asks for: a limit set for each launch could be
+// lowered by another thread's before the launch.  set: the devices that have it.
+template <typename K>
+inline cudaError_t attn_smem(K kernel, int most, std::atomic<unsigned long long>& set) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !(set.load() >> dev & 1))) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e == cudaSuccess && dev < 64) set |= 1ull << dev;
+  }
+  return e;
+}
+
 template <typename T, int HD, bool SHARED>
 inline cudaError_t launch_attn_tc(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const AttnTcArgs& a, int grid,
                                   cudaStream_t s) {
   const int smem = AttnTcShape<HD>::SMEM;
-  static std::atomic<unsigned long long> set{0};   // devices whose limit is raised
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess && (dev >= 64 || !(set.load() >> dev & 1))) {
-    e = cudaFuncSetAttribute(attn_tc_kernel<T, HD, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess && dev < 64) set |= 1ull << dev;
-  }
+  static std::atomic<unsigned long long> set{0};
+  const cudaError_t e = attn_smem(attn_tc_kernel<T, HD, SHARED>, smem, set);
   if (e != cudaSuccess) return e;
   return launch_pdl(attn_tc_kernel<T, HD, SHARED>, dim3(grid), AT_THREADS, smem, s, q, k, v, a);
 }

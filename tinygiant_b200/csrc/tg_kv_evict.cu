@@ -220,11 +220,9 @@ extern "C" int tg_cache_evict(const void* k, const void* v, const float* weights
   const int bh = batch * n_kv_heads, words = keep * (head_dim / 8);
   const int cached = cap <= EV_CACHED;
   const size_t smem = cached ? 4 * (size_t)cap : 0;
-  cudaError_t e = cudaSuccess;
-  if (smem > 32768) e = cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e == cudaSuccess) {
-    e = launch_pdl(select_kernel, dim3(bh), EV_THREADS, smem, s, a, cached);
-  }
+  static std::atomic<unsigned long long> set{0};
+  cudaError_t e = attn_smem(select_kernel, 4 * EV_CACHED, set);
+  if (e == cudaSuccess) e = launch_pdl(select_kernel, dim3(bh), EV_THREADS, smem, s, a, cached);
   if (e == cudaSuccess) e = launch_pdl(gather_kernel, dim3(std::min(64, (words + 255) / 256), bh), 256, 0, s, a);
   count_launches(2);
   return c.done(e);
