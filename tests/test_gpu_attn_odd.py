@@ -250,3 +250,51 @@ def test_evictions_from_two_threads(gpu):
     torch.cuda.synchronize()
     assert not refused, refused
     del keep
+
+
+# ---- what tg_cuda_synchronize waits for
+
+def test_synchronize_waits_for_the_librarys_stream_alone(A, gpu):
+    """Work on the default stream goes on."""
+    q, k = torch.ones(4, 4, 64, dtype=torch.bfloat16, device="cuda"), torch.ones(4, 2, 64, dtype=torch.bfloat16, device="cuda")
+    A.attention_prompt(q, k, k, ends([4]))
+    gpu.tg_cuda_set_stream(None)
+    assert gpu.tg_cuda_synchronize() == 0
+    torch.cuda.synchronize()
+    torch.cuda._sleep(1_000_000_000)                          # half a second on the legacy default stream
+    done = torch.cuda.Event()
+    done.record()
+    assert gpu.tg_cuda_synchronize() == 0
+    assert not done.query()
+    torch.cuda.synchronize()
+
+
+FIRST = """
+import sys
+sys.path.insert(0, {root!r})
+import torch
+from tinygiant_b200 import attention as A
+bf = torch.bfloat16
+q, k = torch.ones(3, 4, 64, dtype=bf, device="cuda"), torch.ones(3, 2, 64, dtype=bf, device="cuda")
+cu = torch.tensor([0, 1, 3], dtype=torch.int32, device="cuda")
+c, n = torch.ones(3, 2, 600, 64, dtype=bf, device="cuda"), torch.tensor([600, 1, 5], dtype=torch.int32, device="cuda")
+w = torch.zeros(3, 2, 600, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    a = A.attention_prompt(q, k, k, cu)
+    b = A.attention_shared(q, c[0], c[0], c, c, n, weights=w)
+    e = A.cache_evict(c, c, w, n, 40, 4)
+g.replay()
+torch.cuda.synchronize()
+assert bool((a == 1).all()) and bool((b == 1).all()) and e[3].tolist() == [40, 1, 5]
+"""
+
+
+def test_first_calls_of_a_process_can_be_captured(gpu):
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = FIRST.format(root=str(Path(__file__).resolve().parents[1]))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]

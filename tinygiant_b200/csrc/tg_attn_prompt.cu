@@ -15,6 +15,7 @@
 // (tg_attn_tc.cuh) works through the list; combine_kernel joins split units.
 // Short sequences need neither plan nor joining.
 #include <algorithm>
+#include <atomic>
 
 #include "../../include/tinygiant.h"
 #include "tg_attn_tc.cuh"
@@ -30,27 +31,50 @@ constexpr int MIN_PIECE = 4;
 
 static __device__ DevStatus g_attn_status;
 
+// The record's address on each device where an operator with waits was called.
+static std::atomic<DevStatus*> g_status_at[ATTN_DEVICES];
+
 DevStatus* attn_status() {
-  static DevStatus* at[64] = {};
   int dev = -1;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
-  if (!at[dev] && cudaGetSymbolAddress((void**)&at[dev], g_attn_status) != cudaSuccess) cudaGetLastError();
-  return at[dev];
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= ATTN_DEVICES) return nullptr;
+  DevStatus* at = g_status_at[dev].load();
+  if (!at) {
+    if (cudaGetSymbolAddress((void**)&at, g_attn_status) != cudaSuccess) {
+      cudaGetLastError();
+      return nullptr;
+    }
+    g_status_at[dev] = at;
+  }
+  return at;
 }
 
-// Reports a wait that ran out in one of the operators' kernels on the current
-// device since the last call, and clears the record.
-bool attn_finish(const char* what) {
-  DevStatus *d = attn_status(), st{};
-  if (!d) return true;
-  if (cudaMemcpy(&st, d, sizeof st, cudaMemcpyDeviceToHost) != cudaSuccess) {
-    set_host_error(100, "%s: reading the attention operators' status failed", what);
-    return false;
+// Reports waits that ran out in the operators' kernels, on any device, since
+// the last report, and clears the records.  In two steps around the library
+// stream's synchronisation, with copies on that stream into pinned memory: no
+// other stream is waited for, and where no operator ran nothing is done.
+bool attn_status_copy_async(cudaStream_t s, const char* what) {
+  for (int i = 0; i < ATTN_DEVICES; i++)
+    if (const DevStatus* at = g_status_at[i].load()) {
+      const cudaError_t e = cudaMemcpyAsync(attn_status_host() + i, at, sizeof *at, cudaMemcpyDeviceToHost, s);
+      if (e != cudaSuccess) {
+        set_host_error(100 + (int)e, "%s: reading the attention operators' status failed (%s)", what, cudaGetErrorString(e));
+        return false;
+      }
+    }
+  return true;
+}
+bool attn_finish_copied(cudaStream_t s, const char* what) {
+  bool ok = true;
+  for (int i = 0; i < ATTN_DEVICES; i++) {
+    DevStatus *at = g_status_at[i].load(), *h = attn_status_host() + i;
+    if (!at || h->code == 0) continue;
+    cudaMemsetAsync(at, 0, sizeof *at, s);
+    cudaStreamSynchronize(s);
+    set_host_error(200 + h->code, "%s: device error %d at site %d of an attention operator (%d, %d)", what, h->code, h->where, h->a, h->b);
+    h->code = 0;
+    ok = false;
   }
-  if (st.code == 0) return true;
-  cudaMemset(d, 0, sizeof st);
-  set_host_error(200 + st.code, "%s: device error %d at site %d of an attention operator (%d, %d)", what, st.code, st.where, st.a, st.b);
-  return false;
+  return ok;
 }
 
 struct PlanArgs {

@@ -772,8 +772,9 @@ void* tg_cuda_stream(void) {
 int tg_cuda_synchronize(void) {
   std::lock_guard<std::recursive_mutex> lk(ctx_mutex());
   if (!ensure_init()) return -1;
-  const bool ok = finish("tg_cuda_synchronize");
-  return attn_finish("tg_cuda_synchronize") && ok ? 0 : -1;
+  const char* what = "tg_cuda_synchronize";
+  const bool copied = attn_status_copy_async(stream(), what), ok = finish(what);
+  return copied && ok && attn_finish_copied(stream(), what) ? 0 : -1;
 }
 
 }  // extern "C"

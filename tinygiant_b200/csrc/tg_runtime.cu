@@ -147,7 +147,7 @@ struct Ctx {
   cudaStream_t user_stream = nullptr;
   bool user_stream_set = false;
   DevStatus* d_status = nullptr;
-  DevStatus* h_status = nullptr;  // pinned
+  DevStatus* h_status = nullptr;  // pinned; behind it the attention operators' records
   unsigned int* d_arrived = nullptr;   // deliver_kernel's CTA count (zero between launches)
   DevBuf d_stage, d_xq8, d_hidden, d_hq8, d_tmp, d_counters, d_parts;
   PinBuf h_up, h_down;
@@ -175,6 +175,7 @@ void unregister_counters(void* p) {
     }
 }
 DevStatus* status_ptr() { return g.d_status; }
+DevStatus* attn_status_host() { return g.h_status + 1; }
 void count_launches(int n) { g_launches += n; }
 void* pinned_up(size_t n) { return g.h_up.reserve(n) ? g.h_up.p : nullptr; }
 void* pinned_down(size_t n) { return g.h_down.reserve(n) ? g.h_down.p : nullptr; }
@@ -213,13 +214,14 @@ bool ensure_init() {
   }
   if (!cuda_ok(cudaStreamCreateWithFlags(&g.own_stream, cudaStreamNonBlocking), "cudaStreamCreate") ||
       !cuda_ok(cudaMalloc(&g.d_status, sizeof(DevStatus)), "cudaMalloc(status)") ||
-      !cuda_ok(cudaMallocHost(&g.h_status, sizeof(DevStatus)), "cudaMallocHost(status)") ||
+      !cuda_ok(cudaMallocHost(&g.h_status, (1 + ATTN_DEVICES) * sizeof(DevStatus)), "cudaMallocHost(status)") ||
       !cuda_ok(cudaMemset(g.d_status, 0, sizeof(DevStatus)), "cudaMemset(status)") ||
       !cuda_ok(cudaMalloc(&g.d_arrived, sizeof(unsigned int)), "cudaMalloc(arrivals)") ||
       !cuda_ok(cudaMemset(g.d_arrived, 0, sizeof(unsigned int)), "cudaMemset(arrivals)")) {
     g.init_failed = true;
     return false;
   }
+  for (int i = 0; i <= ATTN_DEVICES; i++) g.h_status[i] = DevStatus{};
   register_counters(g.d_arrived, sizeof(unsigned int));   // cleared again after a device error
   g.inited = true;
   return true;

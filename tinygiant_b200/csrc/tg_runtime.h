@@ -44,7 +44,12 @@ void unregister_counters(void* p);
 // Attention decode's KV-cache mirrors (tg_attention.cu), dropped with the registry.
 void kv_mirror_forget(const void* host);
 void kv_mirror_clear();
-// Errors of the attention operators on device tensors (tg_attn_prompt.cu).
-bool attn_finish(const char* what);
+// Errors of the attention operators on device tensors (tg_attn_prompt.cu):
+// copies of their records enqueued before the stream is synchronised, and
+// looked at after; attn_status_host: pinned memory for one of each device.
+constexpr int ATTN_DEVICES = 64;
+DevStatus* attn_status_host();
+bool attn_status_copy_async(cudaStream_t s, const char* what);
+bool attn_finish_copied(cudaStream_t s, const char* what);
 
 }  // namespace tg
