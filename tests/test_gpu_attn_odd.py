@@ -298,3 +298,13 @@ def test_first_calls_of_a_process_can_be_captured(gpu):
     code = FIRST.format(root=str(Path(__file__).resolve().parents[1]))
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+# ---- empty batches
+
+def test_an_empty_batch_with_a_prefix_and_a_cache(A):
+    bf = torch.bfloat16
+    q, p, c = torch.ones(0, 32, 128, dtype=bf, device="cuda"), torch.ones(4, 16384, 128, dtype=bf, device="cuda"), \
+        torch.ones(0, 4, 1024, 128, dtype=bf, device="cuda")
+    n, w = torch.zeros(0, dtype=torch.int32, device="cuda"), torch.zeros(0, 4, 1024, device="cuda")
+    assert A.attention_shared(q, p, p, c, c, n, weights=w).shape == (0, 32, 128)

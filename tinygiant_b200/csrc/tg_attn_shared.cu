@@ -32,11 +32,11 @@
 #include <type_traits>
 
 #include "../../include/tinygiant.h"
+#include "tg_attn_split.h"
 #include "tg_attn_tc.cuh"
 
 namespace tg {
 
-constexpr int OWN_KEYS = 128;       // keys per stage: 32 for each warp of a group
 // Rows per TMA box: whole stages come in boxes of 128 rows, a sequence's last
 // 64 rows and less in boxes of 32 (a box takes about 85 clocks to issue: with
 // 16 boxes of 32 rows in every stage the issuing bound an SM to 46 GB/s).
@@ -532,56 +532,14 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
   }
 }
 
-// How the work is cut, and the workspace: prefix pieces' and own segments'
-// partial results, the sequences' first stages, scores.
-struct SharedSpace {
-  int tpt, units, nsp, own_ctas, gp, nt, ngc;
+// The workspace of the cut work (tg_attn_split.h): prefix pieces' and own
+// segments' partial results, the sequences' first stages, scores.
+struct SharedSpace : SharedSplit {
   long long own_row;
   size_t pml, po, starts, scores, bytes = 0;
-  SharedSpace(int B, int P, int max_len, int H, int KH, int hd, bool weights) {
-    const int G = H / KH, sms = attn_sms(), HD = hd <= 64 ? 64 : 128;
-    tpt = AT_ROWS / G;
-    units = (B + 2 * tpt - 1) / (2 * tpt);
-    nt = G <= 8 ? 1 : 2;
-    ngc = (G + 8 * nt - 1) / (8 * nt);
-    gp = (G + 7) / 8 * 8;
-    const int blocks = (P + AT_KEYS - 1) / AT_KEYS;
-    const long long HK = (long long)KH * ngc, stages = (long long)B * HK * ((max_len + OWN_KEYS - 1) / OWN_KEYS);
-    // The SMs' shares and the prefix's pieces: those whose end is earliest by
-    // this count (us, measured at head_dim 128 / 64).  A piece takes 1.9 / 1.1 a
-    // block of two tiles and 8 for its start and end; the own keys 8, and an SM
-    // 1.1 / 0.9 a stage (three quarters of the bound max_len, no faster than HBM)
-    // and 1.7 a sequence and head, after which their SMs take pieces too.  Batch 256 on 16,384 keys with up to
-    // 1,024 own ones: 131 us with 72 SMs and 2 pieces, 171 with 78 and 3, 211
-    // with 90 and 2; with up to 256 own ones 105 with 72 and 6, 149 with 32 and 4.
-    own_ctas = max_len > 0 ? (int)std::min((long long)sms, stages) : 0;
-    nsp = 0;
-    const double tb = HD == 128 ? 1.9 : 1.1, ts = 0.75 * (HD == 128 ? 1.1 : 0.9), th = 0.75 * OWN_KEYS * HD * 4 / 6.0e6;
-    const int step = std::max(1, sms / 8), most = max_len > 0 && blocks ? std::max(1, sms - step) : 0;
-    double best = 0;
-    for (int own = std::min(most, step); blocks && own <= most; own += step) {
-      const double free = most ? 8 + std::max((ts * stages + 1.7 * B * HK) / std::min((long long)own, stages), th * stages) : 0;
-      for (int n : {1, 2, 3, 4, 5, 6, 8, 12, 16, 32, 64}) {
-        if (n > blocks) break;
-        const double d = tb * ((blocks + n - 1) / n) + 8;
-        const long long m = (long long)units * KH * n;
-        const double about = std::max(0.0, (m * d + own * free) / sms);
-        double one = std::floor(about / d) * d, two = free + std::max(0.0, std::floor((about - free) / d)) * d;   // both groups' ends
-        long long done = (long long)(one / d + 0.5) * (sms - own) + (long long)((two - free) / d + 0.5) * own;
-        double end = std::max(one, done > 0 && two > free ? two : 0.0);
-        while (done < m) {
-          if (!own || one <= two)
-            end = std::max(end, one += d), done += sms - own;
-          else
-            end = std::max(end, two += d), done += own;
-        }
-        end = std::max(end, free) + 0.5 * n;
-        if (!nsp || end < best) {
-          best = end, nsp = n;
-          if (most) own_ctas = (int)std::min((long long)own, stages);
-        }
-      }
-    }
+  SharedSpace(int B, int P, int max_len, int H, int KH, int hd, bool weights) : SharedSplit(B, P, max_len, H, KH, hd, attn_sms()) {
+    const int HD = hd <= 64 ? 64 : 128;
+    const long long HK = (long long)KH * ngc;
     auto take = [&](size_t n) {
       const size_t o = bytes;
       bytes = (bytes + n + 255) & ~(size_t)255;

@@ -45,12 +45,11 @@
 #include <type_traits>
 
 #include "tg_attn.h"
+#include "tg_attn_split.h"
 #include "tg_ptx.cuh"
 
 namespace tg {
 
-constexpr int AT_ROWS = 128;       // query rows per tile (MMA M)
-constexpr int AT_KEYS = 128;       // keys per block (MMA N of S, K of P V)
 constexpr int AT_SOFT = 8;         // softmax warps; then one each for loads, S, P V and edges
 constexpr int AT_THREADS = 384;
 constexpr int AT_NPOS = 0x3fffffff;
