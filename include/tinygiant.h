@@ -311,6 +311,10 @@ int tg_cuda_debug_row_isums(int fmt, const void *mat, int nrows, int ncols, cons
  * the IEEE division on n pseudo-random operand pairs; writes the number of
  * results that differ (0 expected).  Returns 0, or -1 on error. */
 int tg_cuda_debug_div_check(long long n, unsigned seed, unsigned long long *mismatches);
+/* Test hook: the attention operators' bounded waits on a barrier that nothing
+ * arrives at (about a second on the library's stream); they record a timeout
+ * in the operators' status.  Returns 0 when enqueued, or -1 on error. */
+int tg_cuda_debug_attn_wait(void);
 
 /* ---- Allocation-free matvec -------------------------------------------- *
  * No counterpart in the reference: an extension for callers that cannot

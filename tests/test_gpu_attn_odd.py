@@ -308,3 +308,19 @@ def test_an_empty_batch_with_a_prefix_and_a_cache(A):
         torch.ones(0, 4, 1024, 128, dtype=bf, device="cuda")
     n, w = torch.zeros(0, dtype=torch.int32, device="cuda"), torch.zeros(0, 4, 1024, device="cuda")
     assert A.attention_shared(q, p, p, c, c, n, weights=w).shape == (0, 32, 128)
+
+
+# ---- waits that run out
+
+def test_a_wait_that_runs_out_is_reported_once(A, gpu):
+    """The operators' waits end by themselves; tg_cuda_synchronize says so, and the next call is a good one."""
+    assert gpu.tg_cuda_synchronize() == 0
+    assert gpu.tg_cuda_debug_attn_wait() == 0
+    assert gpu.tg_cuda_synchronize() == -1
+    code, text = tg.last_error(gpu)
+    assert code == 202 and "site 399 of an attention operator (3, 0)" in text, text
+    assert gpu.tg_cuda_synchronize() == 0
+    q, k = torch.ones(4, 4, 64, dtype=torch.bfloat16, device="cuda"), torch.ones(4, 2, 64, dtype=torch.bfloat16, device="cuda")
+    assert bool((A.attention_prompt(q, k, k, ends([4])) == 1).all())
+    torch.cuda.synchronize()
+    assert gpu.tg_cuda_synchronize() == 0

@@ -78,6 +78,7 @@ EXT = {
     "tg_cuda_step_trace_warps": ([], CI),
     "tg_cuda_tc_trace": ([VP], CI),
     "tg_cuda_debug_step_fault": ([CI, CI], CI),
+    "tg_cuda_debug_attn_wait": ([], CI),
     "tg_cuda_debug_tc_isums": ([VP, VP], CI),
     "tg_layer_forward": ([VP, VP, VP, CI, CI], CI),
     "tg_layer_last_routing": ([VP, CI, VP, VP], CI),

@@ -77,6 +77,30 @@ bool attn_finish_copied(cudaStream_t s, const char* what) {
   return ok;
 }
 
+// The operators' waits, by a warp, a warp that has time and a thread, for a
+// barrier that nothing arrives at; records how many gave up.
+__global__ void __launch_bounds__(96) debug_wait_kernel(DevStatus* st) {
+  __shared__ uint64_t bar;
+  __shared__ int abort, gave_up;
+  if (threadIdx.x == 0) {
+    mbar_init(&bar, 1);
+    abort = gave_up = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  const int w = threadIdx.x / 32, lane = threadIdx.x % 32;
+  bool ok = true;
+  if (w == 0)
+    ok = at_wait(&bar, 0, &abort);
+  else if (w == 1)
+    ok = at_wait_idle(&bar, 0, &abort);
+  else if (lane == 0)
+    ok = at_wait(&bar, 0, &abort);
+  if (!ok && lane == 0) atomicAdd(&gave_up, 1);
+  __syncthreads();
+  if (threadIdx.x == 0 && gave_up) set_error(st, ERR_WAIT_TIMEOUT, 399, gave_up);
+}
+
 struct PlanArgs {
   AttnHead* head;
   AttnEntry* entries;
@@ -301,6 +325,18 @@ static cudaError_t run_prompt(const PlanArgs& p, const CUtensorMap& qm, const CU
 }  // namespace tg
 
 using namespace tg;
+
+extern "C" int tg_cuda_debug_attn_wait(void) {
+  std::lock_guard<std::recursive_mutex> lk(ctx_mutex());
+  if (!ensure_init()) return -1;
+  DevStatus* st = attn_status();
+  if (!st) return -1;
+  debug_wait_kernel<<<1, 96, 0, stream()>>>(st);
+  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) return 0;
+  set_host_error(100 + (int)e, "tg_cuda_debug_attn_wait: %s", cudaGetErrorString(e));
+  return -1;
+}
 
 extern "C" size_t tg_attention_prompt_workspace(int n_seqs, int total_q, int max_k, int n_heads, int n_kv_heads,
                                                 int head_dim) {

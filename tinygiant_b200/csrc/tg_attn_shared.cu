@@ -265,7 +265,8 @@ __global__ void __launch_bounds__(OWN_THREADS, 1) own_kernel(const __grid_consta
         }
       }
     }
-    if (*abort && lane == 0)   // no copy of this CTA may still be in flight
+    __syncthreads();   // the other warps are done
+    if (*abort && lane == 0)   // some warp gave up: no copy of this CTA may still be in flight at its end
       for (int i = max(0, n - S::STAGES); i < n; i++) mbar_wait(&sh.full[i % S::BARS], (i / S::BARS) & 1);
     return;
   }
@@ -461,6 +462,7 @@ __global__ void __launch_bounds__(OWN_THREADS, 1) own_kernel(const __grid_consta
       asm volatile("bar.sync 1, 256;" ::: "memory");
     }
   }
+  __syncthreads();   // with the load warp's
 }
 
 struct JoinArgs {

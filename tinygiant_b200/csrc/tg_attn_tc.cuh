@@ -298,10 +298,16 @@ struct AttnTcShared {
   uint32_t bad_keys[AT_UNITS][AT_EDGES][4];
   uint32_t tmem;
   int abort;
+  // Copies of the load warp, for the end of a CTA that gave up: blocks and Q
+  // loads so far, and of each K / V barrier's last block whether it went
+  // through the edge barrier (is) and that barrier's next phase (par).
+  int issued, q_issued;
+  uint32_t edge_is, edge_par;
 };
 
 // Waits for phase `parity`; gives up after about a second, or once another
-// role has.
+// role has.  A warp comes here converged, so a poll is one instruction for all
+// its lanes and they leave together (a vote on it costs 1 % at 8,192 tokens).
 __device__ __forceinline__ bool at_wait(uint64_t* bar, uint32_t parity, const volatile int* abort) {
   if (mbar_try_wait(bar, parity)) return true;
   const uint32_t t0 = clock();   // 32 bits: a second is half of their range
@@ -536,6 +542,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
     const int n_entries = SHARED ? (a.B + tpu - 1) / tpu * a.nsp : a.entries ? a.head->n_entries : __shfl_sync(~0u, ends, 31);
     const int n_work = n_entries * a.KH;
     int issued = 0, qn = 0;   // blocks and Q loads so far
+    uint32_t edge_is = 0, edge_par = 0;
     bool ok = true;
     for (int it = 0; ok; it++) {
       int w = (int)blockIdx.x + it * (int)gridDim.x;
@@ -582,7 +589,11 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
         }
         uint8_t* dst = kvs + s * TILE;
         // a V block that not all rows see whole goes through the edge warp
-        uint64_t* bar = v && on_edge(e, row) ? &sh.edge[issued % NBAR] : &sh.kv_full[issued % NBAR];
+        const int b = issued % NBAR;
+        const bool edge = v && on_edge(e, row);
+        edge_is = edge_is & ~(1u << b) | (uint32_t)edge << b;
+        edge_par ^= (uint32_t)edge << b;
+        uint64_t* bar = edge ? &sh.edge[b] : &sh.kv_full[b];
         if (lane == 0) {
           mbar_arrive_expect_tx(bar, TILE);
           for (int c = 0; c < HD / 64; c++)
@@ -591,10 +602,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
         issued++;
       }
     }
-    if (*abort && lane == 0) {   // no copy of this CTA may still be in flight
-      for (int i = max(0, issued - NST); i < issued; i++) mbar_wait(&sh.kv_full[i % NBAR], (i / NBAR) & 1);
-      for (int i = max(0, qn - NQ); i < qn; i++) mbar_wait(&sh.q_full[i % NQ], (i / NQ) & 1);
-    }
+    if (lane == 0) sh.issued = issued, sh.q_issued = qn, sh.edge_is = edge_is, sh.edge_par = edge_par;
   } else if (wid == W0 + 1 || wid == W0 + 2) {
     // ---- products, each kind issued by a thread of its own: what one has to
     // do between two products does not keep the tensor cores from the other's
@@ -978,6 +986,17 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tc_kernel(const __grid_con
   }
   at_fence_before();
   __syncthreads();
+  if (*abort && tid == W0 * 32) {   // some role gave up: no copy of this CTA may still be in flight at its end
+    for (int i = max(0, sh.issued - NST); i < sh.issued; i++) {
+      const int b = i % NBAR;
+      if (sh.edge_is >> b & 1)
+        mbar_wait(&sh.edge[b], (sh.edge_par >> b & 1) ^ 1);
+      else
+        mbar_wait(&sh.kv_full[b], (i / NBAR) & 1);
+    }
+    for (int i = max(0, sh.q_issued - NQ); i < sh.q_issued; i++) mbar_wait(&sh.q_full[i % NQ], (i / NQ) & 1);
+  }
+  __syncwarp();
   if (wid == W0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
   if (SHARED && a.beside && blockIdx.x == gridDim.x - 1) pdl_wait();   // this grid ends after the one beside it
 }
