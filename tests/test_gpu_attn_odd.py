@@ -300,6 +300,42 @@ def test_first_calls_of_a_process_can_be_captured(gpu):
     assert r.returncode == 0, r.stderr[-2000:]
 
 
+# ---- arguments that are no tensors
+
+def test_arguments_that_are_no_tensors_are_value_errors(A):
+    bf, cu = torch.bfloat16, ends([4])
+    q, k = torch.zeros(4, 4, 64, dtype=bf, device="cuda"), torch.zeros(4, 2, 64, dtype=bf, device="cuda")
+    c, n, w = torch.zeros(4, 2, 8, 64, dtype=bf, device="cuda"), ends([1] * 3), torch.zeros(4, 2, 8, device="cuda")
+
+    def no(text, fn, *args, **kw):
+        with pytest.raises(ValueError, match=text):
+            fn(*args, **kw)
+
+    P, S, E = A.attention_prompt, A.attention_shared, A.cache_evict
+    no("q must", P, None, k, k, cu)
+    no("k must", P, q, None, k, cu)
+    no("v must", P, q, k, None, cu)
+    no("cu_q", P, q, k, k, [0, 4])
+    no("cu_k", P, q, k, k, cu, [0, 4])
+    no("sinks", P, q, k, k, cu, sinks=[0.0] * 4)
+    no("out must", P, q, k, k, cu, out=7)
+    no("k must have 3", P, q, c, c, cu)
+    no("k must have 4", S, q, None, None, k[:, 0], k[:, 0], n)
+    no("v must", S, q, None, None, c, None, n)
+    no("lens", S, q, None, None, c, c, [1] * 4)
+    no("lens", S, q, None, None, c, c, None)
+    no("lens", S, q[:1], None, None, c[:1], c[:1], n[0])
+    no("prefix", S, q, 1, 1, c, c, n)
+    no("weights", S, q, None, None, c, c, n, weights=[1.0])
+    no("sinks", S, q, None, None, c, c, n, sinks=0.5)
+    no("out must", S, q, None, None, c, c, n, out="out")
+    no("k must", E, None, c, w, n, 4, 1)
+    no("v must", E, c, None, w, n, 4, 1)
+    no("weights", E, c, c, None, n, 4, 1)
+    no("lens", E, c, c, w, None, 4, 1)
+    no("CUDA tensor", E, c.cpu(), c.cpu(), w.cpu(), n.cpu(), 4, 1)
+
+
 # ---- empty batches
 
 def test_an_empty_batch_with_a_prefix_and_a_cache(A):

@@ -29,6 +29,7 @@ import torch
 from . import TinyGiantCudaError, last_error, load
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+_NO_TENSOR = (AttributeError, IndexError)          # of what is no tensor, or has no dimension
 _I64x8, _I64x16 = ctypes.c_int64 * 8, ctypes.c_int64 * 16
 _MOST = 0x7fffffff                                 # no position is beyond it
 _empty = torch.empty_strided                       # less host time than torch.empty
@@ -67,7 +68,7 @@ def _ptr(t):
 
 def _refuse(named, heads=None, small=()):
     """Raises the ValueError of the first tensor that does not fit.  named: (name, tensor, dimensions, shape or None);
-    heads: (H, KH, hd); small: (name, tensor, dtype, shape)."""
+    heads: (H, KH, hd); small: (name, tensor, dtype, shape), None where a call may leave the tensor out."""
     def need(ok, text):
         if not ok:
             raise ValueError(text)
@@ -86,9 +87,7 @@ def _refuse(named, heads=None, small=()):
         need(0 < hd <= 128 and hd % 8 == 0, f"head_dim must be a multiple of 8, at most 128; is {hd}")
     for name, t, ndim, shape in named:
         need(shape is None or tuple(t.shape) == tuple(shape), f"{name} {tuple(t.shape)} and the others do not fit: must be {shape}")
-    for name, t, dtype, shape in small:
-        if t is None:
-            continue
+    for name, t, dtype, shape in filter(None, small):
         need(isinstance(t, torch.Tensor) and t.device == first.device, f"{name} must be a tensor on {first.device}")
         need(t.dtype == dtype and tuple(t.shape) == tuple(shape), f"{name} must be {dtype} {tuple(shape)}, is {t.dtype} {tuple(t.shape)}")
         need(t.is_contiguous() or (name == "weights" and t.stride(2) == 1), f"{name} must be contiguous")
@@ -100,15 +99,20 @@ def _fits(t, device, dtype):
     return t.get_device() == device and t.dtype is dtype and t.stride()[-1] == 1
 
 
-def _heads_of(q, k):
-    """dtype, device index, shape of q and of k without its leading batch dimension (4-D caches)."""
+def _heads_of(q, k, dims):
+    """dtype, device index, shape of q and (rows, heads, head_dim) of k, which has `dims` dimensions."""
     if not (isinstance(q, torch.Tensor) and isinstance(k, torch.Tensor) and q.dtype in _DTYPES and q.is_cuda and q.dim() == 3
-            and k.dim() >= 3):
-        _refuse([("q", q, 3, None), ("k", k, 3, None)])
+            and k.dim() == dims):
+        _refuse([("q", q, 3, None), ("k", k, dims, None)])
     H, KH, hd = q.shape[1], k.shape[1], q.shape[2]
     if KH == 0 or H % KH or H // KH > 128 or hd % 8 or not 0 < hd <= 128:
         _refuse([("q", q, 3, None)], (H, KH, hd))
-    return q.dtype, q.get_device(), q.shape, k.shape[-3:] if k.dim() == 3 else (k.shape[0], KH, hd)
+    return q.dtype, q.get_device(), q.shape, (k.shape[0], KH, hd)
+
+
+def _need_out(out, q):
+    if not isinstance(out, torch.Tensor) or out.shape != q.shape:
+        raise ValueError(f"out must have the shape of q, {tuple(q.shape)}")
 
 
 def attention_prompt(q, k, v, cu_q, cu_k=None, *, max_k=None, window=0, sinks=None, scale=None, out=None):
@@ -125,7 +129,7 @@ def attention_prompt(q, k, v, cu_q, cu_k=None, *, max_k=None, window=0, sinks=No
     sequence, if known (default total_k); it sizes the workspace, and results
     do not depend on it.  Returns out [total_q, H, hd]; out must not overlap
     the inputs."""
-    dtype, dev, (tq, H, hd), (tk, KH, _) = _heads_of(q, k)
+    dtype, dev, (tq, H, hd), (tk, KH, _) = _heads_of(q, k, 3)
     n = cu_q.shape[0] - 1 if isinstance(cu_q, torch.Tensor) and cu_q.dim() == 1 else -1
     if cu_k is None:
         if tk != tq:
@@ -133,15 +137,18 @@ def attention_prompt(q, k, v, cu_q, cu_k=None, *, max_k=None, window=0, sinks=No
         cu_k = cu_q
     if out is None:
         out = _empty((tq, H, hd), (H * hd, hd, 1), dtype=dtype, device=q.device)
-    if not (dev >= 0 and n >= 0 and k.shape == v.shape and k.shape[2] == hd and out.shape == q.shape
-            and _fits(q, dev, dtype) and _fits(k, dev, dtype) and _fits(v, dev, dtype) and _fits(out, dev, dtype)
-            and _fits(cu_q, dev, torch.int32) and _fits(cu_k, dev, torch.int32) and cu_k.shape == cu_q.shape
-            and (sinks is None or (_fits(sinks, dev, torch.float32) and sinks.shape == (H,)))):
-        if out.shape != q.shape:
-            raise ValueError(f"out must have the shape of q, {tuple(q.shape)}")
+    try:
+        fit = (dev >= 0 and n >= 0 and k.shape == v.shape and k.shape[2] == hd and out.shape == q.shape
+               and _fits(q, dev, dtype) and _fits(k, dev, dtype) and _fits(v, dev, dtype) and _fits(out, dev, dtype)
+               and _fits(cu_q, dev, torch.int32) and _fits(cu_k, dev, torch.int32) and cu_k.shape == cu_q.shape
+               and (sinks is None or (_fits(sinks, dev, torch.float32) and sinks.shape == (H,))))
+    except _NO_TENSOR:
+        fit = False
+    if not fit:
+        _need_out(out, q)
         _refuse([("q", q, 3, None), ("k", k, 3, (tk, KH, hd)), ("v", v, 3, (tk, KH, hd)), ("out", out, 3, None)], (H, KH, hd),
                 [("cu_q", cu_q, torch.int32, (max(n, 0) + 1,)), ("cu_k", cu_k, torch.int32, (max(n, 0) + 1,)),
-                 ("sinks", sinks, torch.float32, (H,))])
+                 sinks is not None and ("sinks", sinks, torch.float32, (H,))])
     max_k = tk if max_k is None or max_k > tk else max_k
     lib = load()
     nbytes = lib.tg_attention_prompt_workspace(n, tq, max_k, H, KH, hd)
@@ -168,29 +175,32 @@ def attention_shared(q, prefix_k, prefix_v, k, v, lens, *, max_len=None, window=
     counts as max_len.  A sequence without a key gives zeros.  Rows of the
     caches behind lens are not read as values: they may hold anything.
     Returns out [B, H, hd]."""
-    dtype, dev, (B, H, hd), (_, KH, _) = _heads_of(q, k)
-    P = 0 if prefix_k is None else prefix_k.shape[1] if prefix_k.dim() == 3 else -1
+    dtype, dev, (B, H, hd), (_, KH, _) = _heads_of(q, k, 4)
+    P = 0 if prefix_k is None else prefix_k.shape[1] if isinstance(prefix_k, torch.Tensor) and prefix_k.dim() == 3 else -1
     if out is None:
         out = _empty((B, H, hd), (H * hd, hd, 1), dtype=dtype, device=q.device)
-    if not (dev >= 0 and k.dim() == 4 and k.shape == v.shape and k.shape[0] == B and k.shape[3] == hd and out.shape == q.shape
-            and _fits(q, dev, dtype) and _fits(k, dev, dtype) and _fits(v, dev, dtype) and _fits(out, dev, dtype)
-            and (prefix_k is None if prefix_v is None else
-                 prefix_k is not None and prefix_k.shape == prefix_v.shape == (KH, P, hd) and _fits(prefix_k, dev, dtype)
-                 and _fits(prefix_v, dev, dtype))
-            and _fits(lens, dev, torch.int32) and lens.shape == (B,)
-            and (sinks is None or (_fits(sinks, dev, torch.float32) and sinks.shape == (H,)))
-            and (weights is None or (_fits(weights, dev, torch.float32) and weights.shape == k.shape[:3]
-                                     and min(weights.stride()) > 0))):
-        if out.shape != q.shape:
-            raise ValueError(f"out must have the shape of q, {tuple(q.shape)}")
-        cap = k.shape[2] if k.dim() == 4 else 0
+    try:
+        fit = (dev >= 0 and k.shape == v.shape and k.shape[0] == B and k.shape[3] == hd and out.shape == q.shape
+               and _fits(q, dev, dtype) and _fits(k, dev, dtype) and _fits(v, dev, dtype) and _fits(out, dev, dtype)
+               and (prefix_k is None if prefix_v is None else
+                    prefix_k is not None and prefix_k.shape == prefix_v.shape == (KH, P, hd) and _fits(prefix_k, dev, dtype)
+                    and _fits(prefix_v, dev, dtype))
+               and _fits(lens, dev, torch.int32) and lens.shape == (B,)
+               and (sinks is None or (_fits(sinks, dev, torch.float32) and sinks.shape == (H,)))
+               and (weights is None or (_fits(weights, dev, torch.float32) and weights.shape == k.shape[:3]
+                                        and min(weights.stride()) > 0)))
+    except _NO_TENSOR:
+        fit = False
+    if not fit:
+        _need_out(out, q)
+        cap = k.shape[2]
         named = [("q", q, 3, None), ("k", k, 4, (B, KH, cap, hd)), ("v", v, 4, (B, KH, cap, hd)), ("out", out, 3, None)]
         if prefix_k is not None or prefix_v is not None:
-            if prefix_k is None or prefix_v is None or prefix_k.shape != prefix_v.shape or prefix_k.shape != (KH, P, hd):
+            if not all(isinstance(t, torch.Tensor) and t.shape == (KH, P, hd) for t in (prefix_k, prefix_v)):
                 raise ValueError(f"prefix_k and prefix_v must both be [{KH}, P, {hd}]")
             named += [("prefix_k", prefix_k, 3, None), ("prefix_v", prefix_v, 3, None)]
-        _refuse(named, (H, KH, hd), [("lens", lens, torch.int32, (B,)), ("sinks", sinks, torch.float32, (H,)),
-                                     ("weights", weights, torch.float32, (B, KH, cap))])
+        _refuse(named, (H, KH, hd), [("lens", lens, torch.int32, (B,)), sinks is not None and ("sinks", sinks, torch.float32, (H,)),
+                                     weights is not None and ("weights", weights, torch.float32, (B, KH, cap))])
     cap = k.shape[2]
     max_len = cap if max_len is None or max_len > cap else max_len
     lib = load()
@@ -217,14 +227,19 @@ def cache_evict(k, v, weights, lens, keep, recent):
     Returns (k, v, weights, lens, indices): new tensors [B, KH, keep, hd],
     [B, KH, keep, hd], [B, KH, keep], [B] and the positions' old places
     [B, KH, keep] int32; behind a sequence's end they hold zeros and -1."""
-    shape, dtype, dev = k.shape, k.dtype, k.get_device()
-    if not (len(shape) == 4 and dtype in _DTYPES and dev >= 0 and shape == v.shape and weights.shape == shape[:3]
-            and _fits(k, dev, dtype) and _fits(v, dev, dtype) and _fits(weights, dev, torch.float32)
-            and min(weights.stride()) > 0 and _fits(lens, dev, torch.int32) and lens.shape == shape[:1]):
-        if k.shape != v.shape:
+    try:
+        shape, dtype, dev = k.shape, k.dtype, k.get_device()
+        fit = (len(shape) == 4 and dtype in _DTYPES and dev >= 0 and shape == v.shape and weights.shape == shape[:3]
+               and _fits(k, dev, dtype) and _fits(v, dev, dtype) and _fits(weights, dev, torch.float32)
+               and min(weights.stride()) > 0 and _fits(lens, dev, torch.int32) and lens.shape == shape[:1])
+    except _NO_TENSOR:
+        fit = False
+    if not fit:
+        tensors = isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor)
+        if tensors and k.shape != v.shape:
             raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must have one shape")
-        _refuse([("k", k, 4, None), ("v", v, 4, None)], None, [("weights", weights, torch.float32, shape[:3]),
-                                                              ("lens", lens, torch.int32, shape[:1])])
+        _refuse([("k", k, 4, None), ("v", v, 4, None)], None,
+                [("weights", weights, torch.float32, k.shape[:3]), ("lens", lens, torch.int32, k.shape[:1])] if tensors else ())
     B, KH, cap, hd = shape
     where = k.device
     if not (0 < keep <= cap and 0 <= recent <= keep):
