@@ -336,6 +336,43 @@ def test_arguments_that_are_no_tensors_are_value_errors(A):
     no("CUDA tensor", E, c.cpu(), c.cpu(), w.cpu(), n.cpu(), 4, 1)
 
 
+# ---- gradients
+
+def test_gradients_are_refused_and_writes_in_place_are_counted(A):
+    """The operators have no backward pass: where one would be recorded they say so."""
+    bf, cu = torch.bfloat16, ends([4])
+    q, k = torch.ones(4, 4, 64, dtype=bf, device="cuda"), torch.ones(4, 2, 64, dtype=bf, device="cuda")
+    c, n, w = torch.ones(4, 2, 8, 64, dtype=bf, device="cuda"), ends([1] * 3), torch.zeros(4, 2, 8, device="cuda")
+    sinks = torch.zeros(4, device="cuda", requires_grad=True)
+    for i in range(3):
+        args = [q, k, k]
+        args[i] = args[i].clone().requires_grad_()
+        with pytest.raises(ValueError, match="no backward"):
+            A.attention_prompt(*args, cu)
+        with torch.no_grad():
+            assert bool((A.attention_prompt(*args, cu) == 1).all())
+        args = [q, c, c]
+        args[i] = args[i].clone().requires_grad_()
+        with pytest.raises(ValueError, match="no backward"):
+            A.attention_shared(args[0], None, None, args[1], args[2], n)
+    with pytest.raises(ValueError, match="no backward"):
+        A.attention_prompt(q, k, k, cu, sinks=sinks)
+    with pytest.raises(ValueError, match="no backward"):
+        A.attention_shared(q, c[0].clone().requires_grad_(), c[0], c, c, n)
+    with pytest.raises(ValueError, match="no backward"):
+        A.cache_evict(c.clone().requires_grad_(), c, w, n, 4, 1)
+    with pytest.raises(ValueError, match="no backward"):
+        A.cache_evict(c, c, w.clone().requires_grad_(), n, 4, 1)
+    before, out = w._version, torch.zeros_like(q)
+    A.attention_shared(q, None, None, c, c, n, weights=w, out=out)
+    assert w._version > before and out._version > 0
+    before = out._version
+    A.attention_prompt(q, k, k, cu, out=out)
+    assert out._version > before
+    with torch.inference_mode():
+        A.attention_shared(q, None, None, c, c, n, weights=torch.zeros(4, 2, 8, device="cuda"), out=torch.zeros_like(q))
+
+
 # ---- empty batches
 
 def test_an_empty_batch_with_a_prefix_and_a_cache(A):

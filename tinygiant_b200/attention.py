@@ -20,7 +20,9 @@ What a query does not attend to (later positions, those before its window,
 other sequences, rows behind a cache's lengths) may hold anything, infinities
 and NaN too.  Bad arguments raise ValueError before anything runs
 (ArgumentError, a TinyGiantCudaError too, where the library sees them); other
-errors of the library raise TinyGiantCudaError.
+errors of the library raise TinyGiantCudaError.  There is no backward pass:
+where autograd would record the call (gradients on, and a tensor that requires
+them), it is refused.  Writes into out and weights count as changes in place.
 """
 import ctypes
 
@@ -33,6 +35,8 @@ _NO_TENSOR = (AttributeError, IndexError)          # of what is no tensor, or ha
 _I64x8, _I64x16 = ctypes.c_int64 * 8, ctypes.c_int64 * 16
 _MOST = 0x7fffffff                                 # no position is beyond it
 _empty = torch.empty_strided                       # less host time than torch.empty
+_recording = torch.is_grad_enabled
+_written = torch.autograd.graph.increment_version  # of tensors written in place
 _raw_stream = torch._C._cuda_getCurrentRawStream   # torch.cuda.current_stream(i).cuda_stream, without its objects
 
 
@@ -110,6 +114,11 @@ def _heads_of(q, k, dims):
     return q.dtype, q.get_device(), q.shape, (k.shape[0], KH, hd)
 
 
+def _no_backward():
+    if _recording():
+        raise ValueError("the attention operators have no backward pass: call them under torch.no_grad(), or detach the tensors")
+
+
 def _need_out(out, q):
     if not isinstance(out, torch.Tensor) or out.shape != q.shape:
         raise ValueError(f"out must have the shape of q, {tuple(q.shape)}")
@@ -135,7 +144,8 @@ def attention_prompt(q, k, v, cu_q, cu_k=None, *, max_k=None, window=0, sinks=No
         if tk != tq:
             raise ValueError(f"without cu_k there are as many keys as queries; got {tk} and {tq}")
         cu_k = cu_q
-    if out is None:
+    given = out is not None
+    if not given:
         out = _empty((tq, H, hd), (H * hd, hd, 1), dtype=dtype, device=q.device)
     try:
         fit = (dev >= 0 and n >= 0 and k.shape == v.shape and k.shape[2] == hd and out.shape == q.shape
@@ -149,6 +159,9 @@ def attention_prompt(q, k, v, cu_q, cu_k=None, *, max_k=None, window=0, sinks=No
         _refuse([("q", q, 3, None), ("k", k, 3, (tk, KH, hd)), ("v", v, 3, (tk, KH, hd)), ("out", out, 3, None)], (H, KH, hd),
                 [("cu_q", cu_q, torch.int32, (max(n, 0) + 1,)), ("cu_k", cu_k, torch.int32, (max(n, 0) + 1,)),
                  sinks is not None and ("sinks", sinks, torch.float32, (H,))])
+    if (q.requires_grad or k.requires_grad or v.requires_grad or (given and out.requires_grad)
+            or (sinks is not None and sinks.requires_grad)):
+        _no_backward()
     max_k = tk if max_k is None or max_k > tk else max_k
     lib = load()
     nbytes = lib.tg_attention_prompt_workspace(n, tq, max_k, H, KH, hd)
@@ -157,6 +170,8 @@ def attention_prompt(q, k, v, cu_q, cu_k=None, *, max_k=None, window=0, sinks=No
     _call(dev, lib.tg_attention_prompt, _DTYPES[dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
           cu_q.data_ptr(), cu_k.data_ptr(), _ptr(sinks), n, tq, tk, max_k, H, KH, hd,
           _I64x8(q0, q1, k0, k1, v0, v1, o0, o1), _window(window), hd ** -0.5 if scale is None else scale, _ptr(ws), nbytes)
+    if given:
+        _written(out)
     return out
 
 
@@ -177,7 +192,8 @@ def attention_shared(q, prefix_k, prefix_v, k, v, lens, *, max_len=None, window=
     Returns out [B, H, hd]."""
     dtype, dev, (B, H, hd), (_, KH, _) = _heads_of(q, k, 4)
     P = 0 if prefix_k is None else prefix_k.shape[1] if isinstance(prefix_k, torch.Tensor) and prefix_k.dim() == 3 else -1
-    if out is None:
+    given = out is not None
+    if not given:
         out = _empty((B, H, hd), (H * hd, hd, 1), dtype=dtype, device=q.device)
     try:
         fit = (dev >= 0 and k.shape == v.shape and k.shape[0] == B and k.shape[3] == hd and out.shape == q.shape
@@ -201,6 +217,10 @@ def attention_shared(q, prefix_k, prefix_v, k, v, lens, *, max_len=None, window=
             named += [("prefix_k", prefix_k, 3, None), ("prefix_v", prefix_v, 3, None)]
         _refuse(named, (H, KH, hd), [("lens", lens, torch.int32, (B,)), sinks is not None and ("sinks", sinks, torch.float32, (H,)),
                                      weights is not None and ("weights", weights, torch.float32, (B, KH, cap))])
+    if (q.requires_grad or k.requires_grad or v.requires_grad or (given and out.requires_grad)
+            or (P and (prefix_k.requires_grad or prefix_v.requires_grad)) or (sinks is not None and sinks.requires_grad)
+            or (weights is not None and weights.requires_grad)):
+        _no_backward()
     cap = k.shape[2]
     max_len = cap if max_len is None or max_len > cap else max_len
     lib = load()
@@ -213,6 +233,10 @@ def attention_shared(q, prefix_k, prefix_v, k, v, lens, *, max_len=None, window=
           v.data_ptr(), out.data_ptr(), lens.data_ptr(), _ptr(sinks), _ptr(weights), B, P, cap, max_len, H, KH, hd,
           _I64x16(q0, q1, pk0, pk1, pv0, pv1, k0, k1, k2, v0, v1, v2, o0, o1, w0, w1), _window(window),
           hd ** -0.5 if scale is None else scale, _ptr(ws), nbytes)
+    if given:
+        _written(out)
+    if weights is not None:
+        _written(weights)
     return out
 
 
@@ -240,6 +264,8 @@ def cache_evict(k, v, weights, lens, keep, recent):
             raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must have one shape")
         _refuse([("k", k, 4, None), ("v", v, 4, None)], None,
                 [("weights", weights, torch.float32, k.shape[:3]), ("lens", lens, torch.int32, k.shape[:1])] if tensors else ())
+    if k.requires_grad or v.requires_grad or weights.requires_grad:
+        _no_backward()
     B, KH, cap, hd = shape
     where = k.device
     if not (0 < keep <= cap and 0 <= recent <= keep):
