@@ -40,12 +40,6 @@ template <>
 __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
 template <>
 __device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
-template <typename T>
-__device__ __forceinline__ T from_f32(float x);
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 
 // The checks of one C entry: the first failure records an error (code 3, bad
 // arguments; 2, no device) under the entry's name and sticks.
