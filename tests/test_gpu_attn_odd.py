@@ -2,9 +2,10 @@
 that are not finite, weights far below the row's largest, windows beyond any
 position, prefix values that are not finite under many window edges.
 
-Tolerances are those of test_gpu_attn_ops.  A weight of more than 2^-25 of
-its row's largest is a normal number in either 16-bit type, so its rounding
-is the unit roundoff that the tolerance has; the weights below are such.
+Tolerances are those of test_gpu_attn_ops.  A weight of 2^-24 of its row's
+largest or more is a normal number in either 16-bit type, so its rounding is
+the unit roundoff u that the tolerance has; at 2^-24.5 it is at most 1.5 u, and
+what the tolerance leaves for the scores (0.6 u at least there) covers that.
 """
 import math
 

@@ -7,7 +7,7 @@
 //   p_j = 2^(c s_j - c m),  l += p_j,  o += p_j v_j;   result o / l.
 // m starts as the first block's maximum.  It moves (with l and o scaled by
 // 2^(c m_old - c m_new)) only when a block's maximum exceeds it by more than
-// 2^8 (fp16: 2^4) in the exponent's base: results do not depend on the
+// 2^8 (fp16: 2^5) in the exponent's base: results do not depend on the
 // reference, and o is then rarely touched.  p_j is rounded to the inputs' type
 // for the second product, as tcgen05 wants both operands of one type; its error
 // there is that of rounding v once more (unit roundoff 2^-8 or 2^-11 of the
