@@ -361,10 +361,11 @@ int tg_cuda_matmul_q4k_noalloc(const uint8_t *q4_matrix, const float *input, flo
  * position nk - nq + i and attends to the keys j up to it, with window > 0 to
  * the last `window` of those.  sinks [n_heads] (or NULL): a logit per head
  * that takes part in the softmax's sum without a value.  A query without a
- * key gives zeros; rows of no sequence are not written.  strides: token and
+ * key gives zeros, and so does one whose scores are all -inf; a NaN or +inf
+ * among them gives NaN.  Rows of no sequence are not written.  strides: token and
  * head of q, k, v, out (8 values).  n_heads / n_kv_heads is at most 128.
- * max_k: an upper bound of the sequences' keys, for the workspace's size
- * only.  workspace: 256-byte aligned, tg_attention_prompt_workspace bytes. */
+ * max_k: an upper bound of the sequences' keys, for the workspace's size and
+ * for how far long axes are split (a smaller value is no error).  workspace: 256-byte aligned, tg_attention_prompt_workspace bytes. */
 size_t tg_attention_prompt_workspace(int n_seqs, int total_q, int max_k, int n_heads, int n_kv_heads, int head_dim);
 int tg_attention_prompt(int dtype, const void *q, const void *k, const void *v, void *out, const int *cu_q,
                         const int *cu_k, const float *sinks, int n_seqs, int total_q, int total_k, int max_k,
@@ -377,7 +378,9 @@ int tg_attention_prompt(int dtype, const void *q, const void *k, const void *v, 
  * head: 32 sequences of 8 heads each) and the sequence's
  * own keys k, v [batch][n_kv_heads][cap] behind it, lens[b] of them (values
  * outside 0 .. max_len count as the nearest inside; max_len <= cap), its
- * newest token's the last.  window, sinks: as above.  weights (or NULL)
+ * newest token's the last; they are read once for every 16 query heads of a
+ * key head.  window (in rows of the cache, whatever an eviction took out
+ * before), sinks: as above.  weights (or NULL)
  * [batch][n_kv_heads][cap] fp32: each own key's softmax weight, summed over
  * the query heads that share it, is added.  strides: q, out as above;
  * in all: q (row, head), prefix_k (head, position), prefix_v, k (sequence,
@@ -399,7 +402,8 @@ int tg_attention_shared(int dtype, const void *q, const void *prefix_k, const vo
  * [batch][n_kv_heads][keep][head_dim], weights_out and indices (the old
  * positions) [batch][n_kv_heads][keep], lens_out [batch] are contiguous and
  * overlap no input; behind a sequence's end they hold zeros and -1.  strides:
- * k (sequence, head, position), v, weights (sequence, head): 8 values. */
+ * k (sequence, head, position), v, weights (sequence, head): 8 values.
+ * batch x n_kv_heads is at most 65535. */
 int tg_cache_evict(const void *k, const void *v, const float *weights, const int *lens, void *k_out, void *v_out,
                    float *weights_out, int *lens_out, int *indices, int batch, int cap, int n_kv_heads, int head_dim,
                    const int64_t *strides, int keep, int recent, void *stream);

@@ -136,8 +136,10 @@ def attention_prompt(q, k, v, cu_q, cu_k=None, *, max_k=None, window=0, sinks=No
     adds a logit without a value to each softmax.  scale: 1 / sqrt(hd).  A
     query without a key gives zeros.  max_k: the largest number of keys of a
     sequence, if known (default total_k); it sizes the workspace, and results
-    do not depend on it.  Returns out [total_q, H, hd]; out must not overlap
-    the inputs."""
+    depend on it by no more than the order of their fp32 sums (it decides how
+    long axes are split).  A query whose scores have a NaN or +inf among its
+    keys gives NaN, one whose scores are all -inf zeros.  Returns
+    out [total_q, H, hd]; out must not overlap the inputs."""
     dtype, dev, (tq, H, hd), (tk, KH, _) = _heads_of(q, k, 3)
     n = cu_q.shape[0] - 1 if isinstance(cu_q, torch.Tensor) and cu_q.dim() == 1 else -1
     if cu_k is None:
@@ -181,10 +183,12 @@ def attention_shared(q, prefix_k, prefix_v, k, v, lens, *, max_len=None, window=
 
     q [B, H, hd]; prefix_k, prefix_v [KH, P, hd] (None: no prefix), read once
     for every 256 query rows of a key head (32 sequences of 8 heads); k, v
-    [B, KH, cap, hd]; lens [B] int32 on the device: the own positions of each
-    sequence, its newest token's key the last of them.  The prefix is at the positions 0 .. P - 1, the own keys behind it.
-    window > 0: only the last `window` positions.  sinks, scale: as
-    attention_prompt.  weights [B, KH, cap] fp32: each own key's softmax
+    [B, KH, cap, hd], read once for every 16 query heads of a key head; lens
+    [B] int32 on the device: the own positions of each sequence, its newest
+    token's key the last of them.  The prefix is at the positions 0 .. P - 1,
+    the own keys behind it.  window > 0: only the last `window` positions, as
+    rows of the cache count them: after cache_evict has closed the gaps that is
+    not the last `window` tokens.  sinks, scale: as attention_prompt.  weights [B, KH, cap] fp32: each own key's softmax
     weight, summed over the query heads that share it, is added in place.
     max_len: an upper bound of lens (default cap); a larger value in lens
     counts as max_len.  A sequence without a key gives zeros.  Rows of the
@@ -247,7 +251,10 @@ def cache_evict(k, v, weights, lens, keep, recent):
     gathers them; lens [B] int32 on the device.  Of a sequence's n positions
     min(n, keep) stay: the last `recent` of them, and of the others those of
     the largest weight (equal weights: the earlier position; NaN counts as the
-    largest).  Each key head keeps its own choice, in the order they had.
+    largest).  Weights come from decoded tokens: straight after a prompt they
+    are all zero, and the earliest positions stay.  Each key head keeps its own
+    choice, in the order they had; rows are moved together, so windows of later
+    calls count kept rows, not tokens.  B x KH is at most 65535.
     Returns (k, v, weights, lens, indices): new tensors [B, KH, keep, hd],
     [B, KH, keep, hd], [B, KH, keep], [B] and the positions' old places
     [B, KH, keep] int32; behind a sequence's end they hold zeros and -1."""

@@ -16,8 +16,9 @@
 //   prefix  attn_tc_kernel (tg_attn_tc.cuh): the batch's queries of a key head
 //           are the rows of 128-row tiles, so the prefix is read once per tile
 //           pair and not once per sequence; pieces of its keys.
-//   own     own_kernel: each sequence's keys are read once; bound by HBM.  G
-//           query heads share a key head, so S^T = K Q^T and O^T += V^T P^T
+//   own     own_kernel: each sequence's keys are read once for every 16 query
+//           heads of their key head (its registers hold that many), once in
+//           all for up to 16; bound by HBM.  S^T = K Q^T and O^T += V^T P^T
 //           with the heads as the 8 columns of mma.m16n8k16 (few rows: the
 //           tensor memory path has 128).  All sequences' keys in a row are cut
 //           evenly among the CTAs, so lengths may differ at will.

@@ -36,8 +36,9 @@
 // 2,048 clocks at head_dim 128 and the exponentials 1,792 of the special
 // function unit; a softmax warp needs about 3,100 for its block (load 430,
 // maximum 350, exponentials and P 1,600, waits).  8,192 tokens, 32 / 4 heads of
-// 128, bf16: 427 us, 1.29 PFLOP/s, 0.78 of measured (0.80 of the sustained rate
-// in a long loop); 4,096 at head_dim 64: 110 us.
+// 128, bf16: 427 us, 1.29 PFLOP/s, 0.78 of measured (in a long loop, under the
+// power cap, 489 to 501, 0.79 to 0.81 of the sustained rate); fp16 445 (see
+// AttnRange); 4,096 at head_dim 64: 116 us.
 #pragma once
 #include <cuda.h>
 
