@@ -365,7 +365,8 @@ int tg_cuda_matmul_q4k_noalloc(const uint8_t *q4_matrix, const float *input, flo
  * among them gives NaN.  Rows of no sequence are not written.  strides: token and
  * head of q, k, v, out (8 values).  n_heads / n_kv_heads is at most 128.
  * max_k: an upper bound of the sequences' keys, for the workspace's size and
- * for how far long axes are split (a smaller value is no error).  workspace: 256-byte aligned, tg_attention_prompt_workspace bytes. */
+ * for how far long axes are split (a smaller value is no error).  workspace:
+ * 256-byte aligned, tg_attention_prompt_workspace bytes. */
 size_t tg_attention_prompt_workspace(int n_seqs, int total_q, int max_k, int n_heads, int n_kv_heads, int head_dim);
 int tg_attention_prompt(int dtype, const void *q, const void *k, const void *v, void *out, const int *cu_q,
                         const int *cu_k, const float *sinks, int n_seqs, int total_q, int total_k, int max_k,

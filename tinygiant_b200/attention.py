@@ -188,8 +188,8 @@ def attention_shared(q, prefix_k, prefix_v, k, v, lens, *, max_len=None, window=
     token's key the last of them.  The prefix is at the positions 0 .. P - 1,
     the own keys behind it.  window > 0: only the last `window` positions, as
     rows of the cache count them: after cache_evict has closed the gaps that is
-    not the last `window` tokens.  sinks, scale: as attention_prompt.  weights [B, KH, cap] fp32: each own key's softmax
-    weight, summed over the query heads that share it, is added in place.
+    not the last `window` tokens.  sinks, scale: as attention_prompt.  weights
+    [B, KH, cap] fp32: each own key's softmax weight, summed over the query heads that share it, is added in place.
     max_len: an upper bound of lens (default cap); a larger value in lens
     counts as max_len.  A sequence without a key gives zeros.  Rows of the
     caches behind lens are not read as values: they may hold anything.
