@@ -409,6 +409,78 @@ int tg_cache_evict(const void *k, const void *v, const float *weights, const int
                    float *weights_out, int *lens_out, int *indices, int batch, int cap, int n_kv_heads, int head_dim,
                    const int64_t *strides, int keep, int recent, void *stream);
 
+/* ---- A paged cache on device tensors ------------------------------------ *
+ * No counterpart in the reference.  Pointers, types, streams, alignment and
+ * errors as for the attention above; strides in elements, positive multiples
+ * of 16 bytes but for scales and tables.
+ *
+ * A cache is k_pages, v_pages [n_pages][n_kv_heads][page][head_dim], page a power
+ * of two of at least 16, and tables [batch][table_cols]: position p of sequence
+ * b is row p % page of page tables[b][p / page].  A position below zero or
+ * behind the table and a page outside 0 .. n_pages - 1 is no place: nothing is
+ * read or written there.  page_bits 16: values of dtype; 8: e4m3 codes
+ * (head_dim a multiple of 16) with scales k_scales, v_scales
+ * [n_pages][n_kv_heads][page / 16] fp32, a value its code times the scale of its
+ * 16 positions.  The strides of a cache are k_pages (page, head, row), v_pages,
+ * k_scales (page, head, block), v_scales, tables (row): 13 values. */
+
+/* q_out, k_out = q [n_tokens][n_heads], k [n_tokens][n_kv_heads] rotated by
+ * positions [n_tokens].  Pair j < n_freqs of a head is its dimensions (j, j +
+ * n_freqs), or (2 j, 2 j + 1) if interleaved; it turns by position x freqs[j]
+ * radians and is multiplied by amplitude; dimensions from 2 n_freqs on stay.
+ * q_norm, k_norm [head_dim] (or NULL): each head is first divided by
+ * sqrt(mean(x^2) + eps) and multiplied by these.  q_out and k_out may be q and k.
+ * n_heads or n_kv_heads may be 0.  strides: q, k, q_out, k_out (token, head): 8
+ * values. */
+int tg_rotary(int dtype, const void *q, const void *k, void *q_out, void *k_out, const int *positions,
+              const double *freqs, const float *q_norm, const float *k_norm, int n_tokens, int n_heads,
+              int n_kv_heads, int head_dim, int n_freqs, int interleaved, float amplitude, float eps,
+              const int64_t *strides, void *stream);
+
+/* Writes the keys (normed and rotated as above) and values of new tokens
+ * k, v [n_tokens][n_kv_heads], packed sequence by sequence, to their pages, and
+ * rotates q [n_tokens][n_heads] into q_out (n_heads 0: none).  Sequence b has the
+ * rows cu[b] .. cu[b+1] (batch + 1 ascending values; NULL: n_tokens / batch
+ * each), at its last positions before lens[b].  positions [n_tokens] (or NULL:
+ * the place in the cache): what to rotate by.  Tokens without a place are not
+ * written, rows of no sequence are left out.  With page_bits 8 a block's scale is
+ * the least power of two (2^-117 at least) under which its values are at most
+ * 448, or larger if its earlier tokens' is; if it grows, their codes are
+ * rounded again; a block's first token starts it anew.  Values that are not
+ * finite become NaN.  No place may be written twice in a call, and no 8-bit block
+ * by two sequences.  strides: q, k, v, q_out (token, head), then the cache's: 21
+ * values. */
+int tg_paged_append(int dtype, int page_bits, const void *q, const void *k, const void *v, void *q_out, void *k_pages,
+                    void *v_pages, float *k_scales, float *v_scales, const int *tables, const int *lens, const int *cu,
+                    const int *positions, const double *freqs, const float *q_norm, const float *k_norm, int n_tokens,
+                    int batch, int n_pages, int page, int table_cols, int n_heads, int n_kv_heads, int head_dim,
+                    int n_freqs, int interleaved, float amplitude, float eps, const int64_t *strides, void *stream);
+
+/* The n_queries newest tokens of each sequence, q [batch][n_queries][n_heads],
+ * over its pages: query i is at position lens[b] - n_queries + i and attends to
+ * the positions up to it, with window > 0 to the last `window` of those.
+ * lens[b] outside 0 .. max_len counts as the nearest inside; max_len is at
+ * most table_cols x page.  sinks, and queries without a key: as
+ * tg_attention_prompt.  With page_bits 8 the softmax weights meet the codes in
+ * fp16.  strides: q, out (sequence, token, head), then the cache's: 19 values.
+ * workspace: 256-byte aligned, tg_attention_paged_workspace bytes. */
+size_t tg_attention_paged_workspace(int page_bits, int batch, int n_queries, int max_len, int n_heads, int n_kv_heads,
+                                    int head_dim);
+int tg_attention_paged(int dtype, int page_bits, const void *q, const void *k_pages, const void *v_pages,
+                       const float *k_scales, const float *v_scales, void *out, const int *tables, const int *lens,
+                       const float *sinks, int batch, int n_queries, int n_pages, int page, int table_cols, int max_len,
+                       int n_heads, int n_kv_heads, int head_dim, const int64_t *strides, int window, float scale,
+                       void *workspace, size_t workspace_bytes, void *stream);
+
+/* k_out, v_out [total][n_kv_heads] = the first positions of each sequence,
+ * sequence b's in the rows cu[b] .. cu[b+1].  dtype: the outputs' (page_bits 16:
+ * the pages' too).  What is no place reads as zeros; rows of no sequence are not
+ * written.  strides: k_out, v_out (token, head), then the cache's: 17 values. */
+int tg_paged_gather(int dtype, int page_bits, const void *k_pages, const void *v_pages, const float *k_scales,
+                    const float *v_scales, const int *tables, const int *cu, void *k_out, void *v_out, int total,
+                    int batch, int n_pages, int page, int table_cols, int n_kv_heads, int head_dim,
+                    const int64_t *strides, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,604 @@
+// tg_paged_cache.cu — what stands around attention over a paged cache:
+//   tg_rotary        queries and keys rotated by their positions
+//   tg_paged_append  new tokens' keys (rotated) and values written to their pages
+//   tg_paged_gather  pages read back as packed rows
+//
+// Norm:      x <- x / sqrt(mean x^2 + eps) w over a head's dimensions, where
+//            weights are given.
+// Rotation:  a head's first 2 n dimensions are n pairs, (j, j + n) or
+//            (2 j, 2 j + 1); pair j of position p turns by p f_j:
+//            a <- s (a cos - b sin), b <- s (b cos + a sin).
+// All in fp32 and rounded once.  The angle is taken in turns in 64 bits,
+// reduced there to an eighth of a turn: in 32 bits a position of 100,000 would
+// leave a sine 7 bits.
+//
+// Pages of 8 bits (e4m3) have a scale for each key head and block of 16 tokens,
+// a power of two: e4m3 keeps 4 bits of every value whatever the factor, so a
+// finer scale gains nothing but the exact top of its range, and a block whose
+// scale grows when a larger token comes keeps its earlier codes' bits (but for
+// those that fall below the format's least normal value).
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+
+#include "../../include/tinygiant.h"
+#include "tg_attn_tc.cuh"
+#include "tg_paged.h"
+
+namespace tg {
+
+constexpr int PC_THREADS = 256;
+constexpr int PC_WARPS = PC_THREADS / 32;
+constexpr int PC_CU = 1024;       // sequences whose offsets are kept in shared memory
+constexpr int PC_WINDOW = 8;      // packed tokens that a CTA looks through for blocks' first ones, where sequences bring many
+constexpr int PC_GATHER = 16;     // rows of a gather CTA
+constexpr int PC_IN_FLIGHT = 4;   // rows that a thread has loaded before it works on the first
+
+enum { PC_ROTARY, PC_PAGES16, PC_PAGES8 };
+
+struct CacheArgs {
+  const void *q, *k, *v;
+  void *qo, *ko;              // rotated q (append: if q is there) and k (tg_rotary)
+  uint8_t *kp, *vp;           // pages
+  float *ks, *vs;             // scales of 8-bit pages
+  const int *tables, *lens, *cu, *positions;
+  const double* freqs;
+  const float *qw, *kw;       // weights of the norms, or null
+  long long sq[2], sk[2], sv[2], sqo[2], sko[2];   // token, head; elements
+  long long skp[3], svp[3];   // page, head, row; bytes
+  long long sks[3], svs[3];   // page, head, block
+  long long st;               // tables' row
+  int T, B, per, H, KH, hd, nf, n_pages, cols, shift, run_ctas, window;
+  int interleaved;
+  float amp, eps;
+};
+
+// cos and sin of p f radians, times amp.
+__device__ __forceinline__ float2 rope_angle(int p, double f, float amp) {
+  const double t = (double)p * (f * 0.15915494309189533577);   // turns
+  const double n = rint(4.0 * t);
+  float s, c;
+  sincospif(2.f * (float)(t - 0.25 * n), &s, &c);   // at most a quarter of pi
+  const int quarter = (int)((long long)n & 3);
+  const float cs = quarter & 1 ? -s : c, sn = quarter & 1 ? c : s;
+  return quarter & 2 ? make_float2(-cs * amp, -sn * amp) : make_float2(cs * amp, sn * amp);
+}
+
+// Eight values of a row as four pairs (x[2 i], x[2 i + 1]), the lane's pairs
+// 4 c .. 4 c + 3 of the row's hd / 2: pair j < nf is (j, j + nf), or neighbours if
+// interleaved; pairs behind those are neighbours.  VEC: nf is a multiple of 4
+// or pairs are neighbours, so that four values of a row lie together.
+struct LanePairs {
+  int c, hd, nf;
+  bool split;   // (j, j + nf)
+  __device__ LanePairs(const CacheArgs& a, int lane_of_row) : c(lane_of_row), hd(a.hd), nf(a.nf), split(!a.interleaved && 4 * lane_of_row < a.nf) {}
+  __device__ bool any() const { return 8 * c < hd; }
+  __device__ int low(int i) const {
+    const int j = 4 * c + i;
+    return split && j < nf ? j : 2 * j;
+  }
+  __device__ int high(int i) const {
+    const int j = 4 * c + i;
+    return split && j < nf ? j + nf : 2 * j + 1;
+  }
+};
+template <bool VEC>
+struct Raw {
+  uint32_t w[4];
+};
+template <bool VEC>
+__device__ __forceinline__ void load_pairs(Raw<VEC>& r, const LanePairs& m, const void* row) {
+  const uint16_t* p = static_cast<const uint16_t*>(row);
+  if (VEC) {
+    const uint2 lo = *reinterpret_cast<const uint2*>(p + (m.split ? 4 * m.c : 8 * m.c));
+    const uint2 hi = *reinterpret_cast<const uint2*>(p + (m.split ? m.nf + 4 * m.c : 8 * m.c + 4));
+    r.w[0] = lo.x, r.w[1] = lo.y, r.w[2] = hi.x, r.w[3] = hi.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) r.w[i] = (uint32_t)p[m.low(i)] | (uint32_t)p[m.high(i)] << 16;
+  }
+}
+template <typename T>
+__device__ __forceinline__ float half_of(uint32_t w, int i) {
+  const uint16_t h = i ? w >> 16 : w & 0xffffu;
+  return to_f32<T>(*reinterpret_cast<const T*>(&h));
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void unpack_pairs(float (&x)[8], const Raw<VEC>& r, const LanePairs& m) {
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    if (VEC && m.split) {
+      x[2 * i] = half_of<T>(r.w[i / 2], i & 1);
+      x[2 * i + 1] = half_of<T>(r.w[2 + i / 2], i & 1);
+    } else {
+      x[2 * i] = half_of<T>(r.w[i], 0);
+      x[2 * i + 1] = half_of<T>(r.w[i], 1);
+    }
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_pairs(void* row, const LanePairs& m, const float (&x)[8]) {
+  uint16_t* p = static_cast<uint16_t*>(row);
+  if (VEC) {
+    uint2 lo, hi;
+    if (m.split) {
+      lo = make_uint2(at_pack<T>(x[0], x[2]), at_pack<T>(x[4], x[6]));
+      hi = make_uint2(at_pack<T>(x[1], x[3]), at_pack<T>(x[5], x[7]));
+    } else {
+      lo = make_uint2(at_pack<T>(x[0], x[1]), at_pack<T>(x[2], x[3]));
+      hi = make_uint2(at_pack<T>(x[4], x[5]), at_pack<T>(x[6], x[7]));
+    }
+    *reinterpret_cast<uint2*>(p + (m.split ? 4 * m.c : 8 * m.c)) = lo;
+    *reinterpret_cast<uint2*>(p + (m.split ? m.nf + 4 * m.c : 8 * m.c + 4)) = hi;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t w = at_pack<T>(x[2 * i], x[2 * i + 1]);
+      p[m.low(i)] = (uint16_t)w;
+      p[m.high(i)] = (uint16_t)(w >> 16);
+    }
+  }
+}
+// e4m3 codes of a pair, the first in the low byte; NaN where a value is not finite.
+__device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
+  uint16_t d;
+  lo = fabsf(lo) <= FLT_MAX ? lo : NAN;
+  hi = fabsf(hi) <= FLT_MAX ? hi : NAN;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+__device__ __forceinline__ float2 e4m3_values(uint32_t two) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)two));
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+template <bool VEC>
+__device__ __forceinline__ void store_codes(uint8_t* p, const LanePairs& m, const float (&x)[8]) {
+  uint32_t lo, hi;
+  if (VEC && m.split) {
+    lo = e4m3_pair(x[0], x[2]) | e4m3_pair(x[4], x[6]) << 16;
+    hi = e4m3_pair(x[1], x[3]) | e4m3_pair(x[5], x[7]) << 16;
+  } else {
+    lo = e4m3_pair(x[0], x[1]) | e4m3_pair(x[2], x[3]) << 16;
+    hi = e4m3_pair(x[4], x[5]) | e4m3_pair(x[6], x[7]) << 16;
+  }
+  if (VEC) {
+    *reinterpret_cast<uint32_t*>(p + (m.split ? 4 * m.c : 8 * m.c)) = lo;
+    *reinterpret_cast<uint32_t*>(p + (m.split ? m.nf + 4 * m.c : 8 * m.c + 4)) = hi;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t two = (i < 2 ? lo : hi) >> 16 * (i & 1);
+      p[m.low(i)] = (uint8_t)two;
+      p[m.high(i)] = (uint8_t)(two >> 8);
+    }
+  }
+}
+
+// The lane's weights of a norm, in its pairs' order.
+__device__ __forceinline__ void load_weights(float (&w)[8], const LanePairs& m, const float* p) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    w[2 * i] = p && m.any() ? p[m.low(i)] : 1.f;
+    w[2 * i + 1] = p && m.any() ? p[m.high(i)] : 1.f;
+  }
+}
+// The norm over the LPR lanes of a row; lanes without values have zeros.
+template <int LPR>
+__device__ __forceinline__ void norm_row(float (&x)[8], const float (&w)[8], int hd, float eps) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; i++) s = fmaf(x[i], x[i], s);
+#pragma unroll
+  for (int o = LPR / 2; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+  const float r = 1.f / sqrtf(s / hd + eps);
+#pragma unroll
+  for (int i = 0; i < 8; i++) x[i] = x[i] * r * w[i];
+}
+// Pairs j < nf turned; the others stay as they are, whatever their neighbours hold.
+__device__ __forceinline__ void rotate_pairs(float (&x)[8], const float2 (&cs)[4], const LanePairs& m) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if (4 * m.c + i >= m.nf) continue;
+    const float a = x[2 * i], b = x[2 * i + 1];
+    x[2 * i] = fmaf(a, cs[i].x, -(b * cs[i].y));
+    x[2 * i + 1] = fmaf(b, cs[i].x, a * cs[i].y);
+  }
+}
+
+// Offsets of the sequences, in shared memory where they fit.
+__device__ __forceinline__ const int* keep_offsets(const int* cu, int B, int* s_cu) {
+  if (!cu || B > PC_CU) return cu;
+  for (int i = threadIdx.x; i <= B; i += PC_THREADS) s_cu[i] = cu[i];
+  return s_cu;
+}
+
+struct CacheShared {
+  int cu[PC_CU + 1];
+  float2 turn[(PC_WINDOW + PAGED_BLOCK - 1) * (ATTN_MAX_HD / 2)];   // cos, sin of tokens' pairs
+  int at[PC_WINDOW + PAGED_BLOCK - 1];                              // tokens' positions for the rotation
+  int run[PC_WINDOW], len[PC_WINDOW], page[PC_WINDOW], row[PC_WINDOW];   // runs: first token, tokens, page, first row
+  int runs, cover;
+};
+
+// One token's rows: q, and (tg_rotary, 16-bit pages) k and v.  A row is LPR
+// lanes of 8 values.
+template <typename T, int LPR, bool VEC, int MODE>
+__device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, int t) {
+  const int tid = threadIdx.x, g = tid / LPR;
+  constexpr int ROWS = PC_THREADS / LPR;
+  const LanePairs m(a, tid % LPR);
+  const int rows = a.H + (MODE == PC_PAGES8 ? 0 : a.KH) + (MODE == PC_PAGES16 ? a.KH : 0);
+  auto source = [&](int r) -> const T* {
+    if (r < a.H) return (const T*)a.q + t * a.sq[0] + r * a.sq[1];
+    if (r < a.H + a.KH) return (const T*)a.k + t * a.sk[0] + (r - a.H) * a.sk[1];
+    return (const T*)a.v + t * a.sv[0] + (r - a.H - a.KH) * a.sv[1];
+  };
+  Raw<VEC> raw[PC_IN_FLIGHT];
+#pragma unroll
+  for (int i = 0; i < PC_IN_FLIGHT; i++)
+    if (g + i * ROWS < rows && m.any()) load_pairs(raw[i], m, source(g + i * ROWS));
+  int pos, page = -1;
+  if (MODE == PC_ROTARY) {
+    pos = a.positions[t];
+  } else {
+    const int* cu = keep_offsets(a.cu, a.B, sh.cu);
+    if (a.cu) __syncthreads();
+    const PagedToken k = paged_token(cu, a.B, a.per, a.T, t);
+    if (k.seq < 0) return;   // of no sequence: the whole CTA, all threads have the same token
+    const int p = paged_position(a.lens[k.seq], k.end, t);
+    pos = a.positions ? a.positions[t] : p;
+    if (MODE == PC_PAGES16) {
+      page = paged_page(a.tables + k.seq * a.st, a.cols, p, a.shift, a.n_pages);
+      if (tid == 0) sh.row[0] = p & ((1 << a.shift) - 1);
+    }
+  }
+  for (int i = tid; i < a.nf; i += PC_THREADS) sh.turn[i] = rope_angle(pos, a.freqs[i], a.amp);
+  float qw[8], kw[8];
+  load_weights(qw, m, a.qw);
+  load_weights(kw, m, a.kw);
+  __syncthreads();
+  float2 cs[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) cs[i] = 4 * m.c + i < a.nf ? sh.turn[4 * m.c + i] : make_float2(1.f, 0.f);
+  for (int r0 = 0; r0 < rows; r0 += PC_IN_FLIGHT * ROWS) {
+#pragma unroll
+    for (int i = 0; i < PC_IN_FLIGHT; i++) {
+      const int r = r0 + g + i * ROWS;
+      if (r0 + i * ROWS >= rows) break;   // the same for the whole CTA
+      float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (r < rows && m.any()) unpack_pairs<T>(x, raw[i], m);
+      if (a.qw || a.kw) {   // lanes of rows that have none take part in the sums
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = x[e];
+        norm_row<LPR>(y, r < a.H ? qw : kw, a.hd, a.eps);
+        if (r < a.H ? a.qw != nullptr : r < a.H + a.KH && a.kw)
+#pragma unroll
+          for (int e = 0; e < 8; e++) x[e] = y[e];
+      }
+      if (r < a.H + a.KH) rotate_pairs(x, cs, m);
+      if (r < rows && m.any()) {
+        T* to = nullptr;
+        if (r < a.H)
+          to = (T*)a.qo + t * a.sqo[0] + r * a.sqo[1];
+        else if (MODE == PC_ROTARY)
+          to = (T*)a.ko + t * a.sko[0] + (r - a.H) * a.sko[1];
+        else if (page >= 0)
+          to = r < a.H + a.KH ? (T*)(a.kp + page * a.skp[0] + (r - a.H) * a.skp[1] + sh.row[0] * a.skp[2])
+                              : (T*)(a.vp + page * a.svp[0] + (r - a.H - a.KH) * a.svp[1] + sh.row[0] * a.svp[2]);
+        if (to) store_pairs<T, VEC>(to, m, x);
+      }
+      const int next = r + PC_IN_FLIGHT * ROWS;
+      if (next < rows && m.any()) load_pairs(raw[i], m, source(next));
+    }
+  }
+}
+
+// Runs of 8-bit blocks whose first token is one of the `window` packed tokens
+// from t0 on: a warp has one run's keys or values of a key head.
+template <typename T, int LPR, bool VEC>
+__device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& sh, int t0) {
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+  constexpr int RPP = 32 / LPR, PASSES = PAGED_BLOCK / RPP;
+  const int* cu = keep_offsets(a.cu, a.B, sh.cu);
+  __syncthreads();
+  if (wid == 0) {
+    const int t = t0 + lane;
+    int n = 0, p = 0;
+    PagedToken k;
+    k.seq = -1;
+    if (lane < a.window + PAGED_BLOCK - 1 && t < a.T) {
+      k = paged_token(cu, a.B, a.per, a.T, t);
+      p = k.seq >= 0 ? paged_position(a.lens[k.seq], k.end, t) : 0;
+      sh.at[lane] = k.seq >= 0 && a.positions ? a.positions[t] : p;
+      n = lane < a.window ? paged_run(k, t, p) : 0;
+    }
+    const int page = n ? paged_page(a.tables + k.seq * a.st, a.cols, p, a.shift, a.n_pages) : -1;
+    const unsigned mine = __ballot_sync(~0u, page >= 0);
+    if (page >= 0) {
+      const int i = __popc(mine & ((1u << lane) - 1));
+      sh.run[i] = lane, sh.len[i] = n, sh.page[i] = page, sh.row[i] = p & ((1 << a.shift) - 1);
+    }
+    const int cover = __reduce_max_sync(~0u, page >= 0 ? lane + n : 0);
+    if (lane == 0) sh.runs = __popc(mine), sh.cover = cover;
+  }
+  __syncthreads();
+  if (!sh.runs) return;
+  for (int i = tid; i < sh.cover * a.nf; i += PC_THREADS) sh.turn[i] = rope_angle(sh.at[i / a.nf], a.freqs[i % a.nf], a.amp);
+  const LanePairs m(a, lane % LPR);
+  float kw[8];
+  load_weights(kw, m, a.kw);
+  __syncthreads();
+  for (int item = wid; item < sh.runs * 2 * a.KH; item += PC_WARPS) {
+    const int i = item / (2 * a.KH), kh = item % (2 * a.KH) >> 1, is_v = item & 1;
+    const int j0 = sh.run[i], n = sh.len[i], off = sh.row[i] % PAGED_BLOCK, block = sh.row[i] / PAGED_BLOCK;
+    uint8_t* rows = is_v ? a.vp + sh.page[i] * a.svp[0] + kh * a.svp[1] + (long long)block * PAGED_BLOCK * a.svp[2]
+                         : a.kp + sh.page[i] * a.skp[0] + kh * a.skp[1] + (long long)block * PAGED_BLOCK * a.skp[2];
+    const long long pitch = is_v ? a.svp[2] : a.skp[2];
+    float* scale_at = is_v ? a.vs + sh.page[i] * a.svs[0] + kh * a.svs[1] + block * a.svs[2]
+                           : a.ks + sh.page[i] * a.sks[0] + kh * a.sks[1] + block * a.sks[2];
+    const float before = off ? *scale_at : 0.f;
+    Raw<VEC> raw[PASSES];
+#pragma unroll
+    for (int u = 0; u < PASSES; u++) {
+      const int j = u * RPP + lane / LPR;
+      if (j < n && m.any()) {
+        const long long t = t0 + j0 + j;
+        load_pairs(raw[u], m, is_v ? (const T*)a.v + t * a.sv[0] + kh * a.sv[1] : (const T*)a.k + t * a.sk[0] + kh * a.sk[1]);
+      }
+    }
+    float x[PASSES][8];
+    uint32_t amax = 0;   // bits of the largest finite magnitude
+#pragma unroll
+    for (int u = 0; u < PASSES; u++) {
+      if (u * RPP >= n) break;
+      const int j = u * RPP + lane / LPR;
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[u][e] = 0.f;
+      if (j < n && m.any()) unpack_pairs<T>(x[u], raw[u], m);
+      if (!is_v) {
+        if (a.kw) norm_row<LPR>(x[u], kw, a.hd, a.eps);
+        if (j < n && m.any()) {
+          float2 cs[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) cs[e] = 4 * m.c + e < a.nf ? sh.turn[(j0 + j) * a.nf + 4 * m.c + e] : make_float2(1.f, 0.f);
+          rotate_pairs(x[u], cs, m);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        if (fabsf(x[u][e]) <= FLT_MAX) amax = max(amax, __float_as_uint(x[u][e]) & 0x7fffffffu);
+    }
+    amax = __reduce_max_sync(~0u, amax);
+    const float need = __uint_as_float((uint32_t)(paged_scale_exp(amax) + 127) << 23);
+    const float scale = fmaxf(need, before), inv = 1.f / scale;
+    if (off && scale > before) {   // the earlier tokens' codes under the larger scale
+      const float again = before * inv;
+      for (int i8 = lane; i8 < off * (a.hd / 8); i8 += 32) {
+        uint2* at = reinterpret_cast<uint2*>(rows + i8 / (a.hd / 8) * pitch + i8 % (a.hd / 8) * 8);
+        const uint2 w = *at;
+        auto four = [&](uint32_t c) {
+          const float2 lo = e4m3_values(c), hi = e4m3_values(c >> 16);
+          return e4m3_pair(lo.x * again, lo.y * again) | e4m3_pair(hi.x * again, hi.y * again) << 16;
+        };
+        *at = make_uint2(four(w.x), four(w.y));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < PASSES; u++) {
+      const int j = u * RPP + lane / LPR;
+      if (j < n && m.any()) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[u][e] *= inv;
+        store_codes<VEC>(rows + (off + j) * pitch, m, x[u]);
+      }
+    }
+    if (lane == 0) *scale_at = scale;
+  }
+}
+
+template <typename T, int LPR, bool VEC, int MODE>
+__global__ void __launch_bounds__(PC_THREADS) cache_kernel(const CacheArgs a) {
+  __shared__ CacheShared sh;
+  pdl_wait();
+  if (MODE == PC_PAGES8 && blockIdx.x < a.run_ctas)
+    runs_of_blocks<T, LPR, VEC>(a, sh, blockIdx.x * a.window);
+  else
+    token_rows<T, LPR, VEC, MODE>(a, sh, blockIdx.x - (MODE == PC_PAGES8 ? a.run_ctas : 0));
+}
+
+struct GatherArgs {
+  const uint8_t *kp, *vp;
+  const float *ks, *vs;
+  const int *tables, *cu;
+  void *ko, *vo;
+  long long skp[3], svp[3], sks[3], svs[3], sko[2], svo[2], st;
+  int T, B, KH, hd, n_pages, cols, shift;
+};
+
+// Rows of the packed outputs: 16 bytes of a page's row at a time.
+template <typename T, bool CODES>
+__global__ void __launch_bounds__(PC_THREADS) gather_pages_kernel(const GatherArgs a, int lpr) {
+  __shared__ int s_cu[PC_CU + 1], s_page[PC_GATHER], s_row[PC_GATHER];
+  pdl_wait();
+  const int tid = threadIdx.x, t0 = blockIdx.x * PC_GATHER;
+  const int* cu = keep_offsets(a.cu, a.B, s_cu);
+  __syncthreads();
+  if (tid < PC_GATHER && t0 + tid < a.T) {
+    const PagedToken k = paged_token(cu, a.B, 1, a.T, t0 + tid);
+    const int p = t0 + tid - k.first;
+    s_page[tid] = k.seq < 0 ? -2 : paged_page(a.tables + k.seq * a.st, a.cols, p, a.shift, a.n_pages);   // -2: of no sequence
+    s_row[tid] = p & ((1 << a.shift) - 1);
+  }
+  __syncthreads();
+  const int c = tid % lpr, chunks = a.hd / (CODES ? 16 : 8);
+  if (c >= chunks) return;
+  const int rows = min(PC_GATHER, a.T - t0) * 2 * a.KH;
+#pragma unroll 4
+  for (int r = tid / lpr; r < rows; r += PC_THREADS / lpr) {
+    const int j = r / (2 * a.KH), kh = r % (2 * a.KH) % a.KH, is_v = r % (2 * a.KH) >= a.KH, page = s_page[j];
+    if (page == -2) continue;
+    uint4 w = make_uint4(0, 0, 0, 0);
+    float scale = 0.f;
+    if (page >= 0) {
+      const long long* s = is_v ? a.svp : a.skp;
+      w = *reinterpret_cast<const uint4*>((is_v ? a.vp : a.kp) + page * s[0] + kh * s[1] + s_row[j] * s[2] + c * 16);
+      if (CODES) scale = is_v ? a.vs[page * a.svs[0] + kh * a.svs[1] + s_row[j] / PAGED_BLOCK * a.svs[2]]
+                              : a.ks[page * a.sks[0] + kh * a.sks[1] + s_row[j] / PAGED_BLOCK * a.sks[2]];
+    }
+    T* to = (is_v ? (T*)a.vo + (t0 + j) * a.svo[0] + kh * a.svo[1] : (T*)a.ko + (t0 + j) * a.sko[0] + kh * a.sko[1]) + c * (CODES ? 16 : 8);
+    if (!CODES) {
+      *reinterpret_cast<uint4*>(to) = w;
+    } else {
+      auto two = [&](uint32_t code) {
+        const float2 v = e4m3_values(code);
+        return page >= 0 ? at_pack<T>(v.x * scale, v.y * scale) : 0u;
+      };
+      reinterpret_cast<uint4*>(to)[0] = make_uint4(two(w.x), two(w.x >> 16), two(w.y), two(w.y >> 16));
+      reinterpret_cast<uint4*>(to)[1] = make_uint4(two(w.z), two(w.z >> 16), two(w.w), two(w.w >> 16));
+    }
+  }
+}
+
+template <typename T, int MODE>
+static cudaError_t launch_cache(const CacheArgs& a, int grid, cudaStream_t s) {
+  const bool vec = a.interleaved || a.nf % 4 == 0, narrow = a.hd <= 64;
+  count_launches(1);
+  if (narrow)
+    return vec ? launch_pdl(cache_kernel<T, 8, true, MODE>, dim3(grid), PC_THREADS, 0, s, a)
+               : launch_pdl(cache_kernel<T, 8, false, MODE>, dim3(grid), PC_THREADS, 0, s, a);
+  return vec ? launch_pdl(cache_kernel<T, 16, true, MODE>, dim3(grid), PC_THREADS, 0, s, a)
+             : launch_pdl(cache_kernel<T, 16, false, MODE>, dim3(grid), PC_THREADS, 0, s, a);
+}
+
+}  // namespace tg
+
+using namespace tg;
+
+extern "C" int tg_rotary(int dtype, const void* q, const void* k, void* q_out, void* k_out, const int* positions,
+                         const double* freqs, const float* q_norm, const float* k_norm, int n_tokens, int n_heads,
+                         int n_kv_heads, int head_dim, int n_freqs, int interleaved, float amplitude, float eps,
+                         const int64_t* strides, void* stream) {
+  ArgCheck c("tg_rotary");
+  c.need(dtype == ATTN_BF16 || dtype == ATTN_FP16, "dtype must be 0 (bf16) or 1 (fp16)");
+  c.need(n_tokens >= 0 && n_heads >= 0 && n_kv_heads >= 0, "counts must not be negative");
+  c.need(head_dim > 0 && head_dim % 8 == 0 && head_dim <= ATTN_MAX_HD, "head_dim must be a multiple of 8, at most 128");
+  c.need(n_freqs >= 0 && 2 * (long long)n_freqs <= head_dim, "at most head_dim / 2 frequencies");
+  c.need(std::isfinite(amplitude), "amplitude must be finite");
+  c.need(std::isfinite(eps) && eps >= 0.f, "eps must be finite and not negative");
+  c.need(strides != nullptr, "strides is null");
+  if (c.rc) return c.rc;
+  long long t[8];
+  for (int i = 0; i < 8; i++) t[i] = c.stride(strides[i], i % 2 == 0 ? n_tokens : i / 2 % 2 == 0 ? n_heads : n_kv_heads);
+  if (c.rc || n_tokens == 0 || n_heads + n_kv_heads == 0) return c.rc;
+  if (!c.device()) return c.rc;
+  if (n_heads) c.ptr(q, 16, "q"), c.ptr(q_out, 16, "q_out");
+  if (n_kv_heads) c.ptr(k, 16, "k"), c.ptr(k_out, 16, "k_out");
+  c.ptr(positions, 4, "positions");
+  if (n_freqs) c.ptr(freqs, 8, "freqs");
+  if (q_norm) c.ptr(q_norm, 4, "q_norm");
+  if (k_norm) c.ptr(k_norm, 4, "k_norm");
+  if (c.rc) return c.rc;
+  CacheArgs a{};
+  a.q = q, a.k = k, a.qo = q_out, a.ko = k_out, a.positions = positions, a.freqs = freqs, a.qw = q_norm, a.kw = k_norm;
+  for (int i = 0; i < 2; i++) a.sq[i] = t[i], a.sk[i] = t[2 + i], a.sqo[i] = t[4 + i], a.sko[i] = t[6 + i];
+  a.T = n_tokens, a.H = n_heads, a.KH = n_kv_heads, a.hd = head_dim, a.nf = n_freqs;
+  a.interleaved = interleaved != 0, a.amp = amplitude, a.eps = eps;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return c.done(dtype == ATTN_BF16 ? launch_cache<__nv_bfloat16, PC_ROTARY>(a, n_tokens, s)
+                                   : launch_cache<__half, PC_ROTARY>(a, n_tokens, s));
+}
+
+extern "C" int tg_paged_append(int dtype, int page_bits, const void* q, const void* k, const void* v, void* q_out,
+                               void* k_pages, void* v_pages, float* k_scales, float* v_scales, const int* tables,
+                               const int* lens, const int* cu, const int* positions, const double* freqs,
+                               const float* q_norm, const float* k_norm, int n_tokens, int batch, int n_pages, int page,
+                               int table_cols, int n_heads, int n_kv_heads, int head_dim, int n_freqs, int interleaved,
+                               float amplitude, float eps, const int64_t* strides, void* stream) {
+  ArgCheck c("tg_paged_append");
+  c.need(dtype == ATTN_BF16 || dtype == ATTN_FP16, "dtype must be 0 (bf16) or 1 (fp16)");
+  c.need(n_tokens >= 0 && batch >= 0 && n_heads >= 0 && n_kv_heads > 0, "n_kv_heads must be positive, the other counts not negative");
+  c.need(head_dim > 0 && head_dim % 8 == 0 && head_dim <= ATTN_MAX_HD, "head_dim must be a multiple of 8, at most 128");
+  c.need(n_freqs >= 0 && 2 * (long long)n_freqs <= head_dim, "at most head_dim / 2 frequencies");
+  c.need(std::isfinite(amplitude), "amplitude must be finite");
+  c.need(std::isfinite(eps) && eps >= 0.f, "eps must be finite and not negative");
+  c.need(n_tokens == 0 || batch > 0, "tokens without a sequence");
+  c.need(cu || batch == 0 || n_tokens % batch == 0, "without cu there are as many tokens of each sequence");
+  c.need(n_tokens < 1 << 30, "too many tokens");
+  c.need(strides != nullptr, "strides is null");
+  if (c.rc) return c.rc;
+  const PoolCheck pool(c, page_bits, n_pages, page, table_cols, batch, n_kv_heads, head_dim, strides + 8);
+  long long t[8];
+  for (int i = 0; i < 8; i++)   // q, k, v, q_out
+    t[i] = c.stride(strides[i], i % 2 == 0 ? n_tokens : i / 2 == 0 || i / 2 == 3 ? n_heads : n_kv_heads);
+  if (c.rc || n_tokens == 0) return c.rc;
+  if (!c.device()) return c.rc;
+  c.ptr(k, 16, "k"), c.ptr(v, 16, "v"), c.ptr(lens, 4, "lens");
+  if (table_cols) c.ptr(tables, 4, "tables");
+  if (n_pages) c.ptr(k_pages, 16, "k_pages"), c.ptr(v_pages, 16, "v_pages");
+  if (n_pages && page_bits == 8) c.ptr(k_scales, 4, "k_scales"), c.ptr(v_scales, 4, "v_scales");
+  if (n_heads) c.ptr(q, 16, "q"), c.ptr(q_out, 16, "q_out");
+  if (cu) c.ptr(cu, 4, "cu");
+  if (positions) c.ptr(positions, 4, "positions");
+  if (n_freqs) c.ptr(freqs, 8, "freqs");
+  if (q_norm) c.ptr(q_norm, 4, "q_norm");
+  if (k_norm) c.ptr(k_norm, 4, "k_norm");
+  if (c.rc) return c.rc;
+  CacheArgs a{};
+  a.q = q, a.k = k, a.v = v, a.qo = q_out, a.kp = (uint8_t*)k_pages, a.vp = (uint8_t*)v_pages, a.ks = k_scales, a.vs = v_scales;
+  a.tables = tables, a.lens = lens, a.cu = cu, a.positions = positions, a.freqs = freqs, a.qw = q_norm, a.kw = k_norm;
+  for (int i = 0; i < 2; i++) a.sq[i] = t[i], a.sk[i] = t[2 + i], a.sv[i] = t[4 + i], a.sqo[i] = t[6 + i];
+  for (int i = 0; i < 3; i++) a.skp[i] = pool.kp[i], a.svp[i] = pool.vp[i], a.sks[i] = pool.ks[i], a.svs[i] = pool.vs[i];
+  a.st = pool.st;
+  a.T = n_tokens, a.B = batch, a.per = n_tokens / batch, a.H = n_heads, a.KH = n_kv_heads, a.hd = head_dim, a.nf = n_freqs;
+  a.n_pages = n_pages, a.cols = table_cols, a.shift = pool.shift, a.interleaved = interleaved != 0, a.amp = amplitude, a.eps = eps;
+  int grid = n_tokens;
+  if (page_bits == 8) {
+    a.window = n_tokens / batch >= PC_WINDOW ? PC_WINDOW : 1;
+    a.run_ctas = (n_tokens + a.window - 1) / a.window;
+    grid = a.run_ctas + (n_heads ? n_tokens : 0);
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool bf = dtype == ATTN_BF16;
+  if (page_bits == 16)
+    return c.done(bf ? launch_cache<__nv_bfloat16, PC_PAGES16>(a, grid, s) : launch_cache<__half, PC_PAGES16>(a, grid, s));
+  return c.done(bf ? launch_cache<__nv_bfloat16, PC_PAGES8>(a, grid, s) : launch_cache<__half, PC_PAGES8>(a, grid, s));
+}
+
+extern "C" int tg_paged_gather(int dtype, int page_bits, const void* k_pages, const void* v_pages, const float* k_scales,
+                               const float* v_scales, const int* tables, const int* cu, void* k_out, void* v_out,
+                               int total, int batch, int n_pages, int page, int table_cols, int n_kv_heads, int head_dim,
+                               const int64_t* strides, void* stream) {
+  ArgCheck c("tg_paged_gather");
+  c.need(dtype == ATTN_BF16 || dtype == ATTN_FP16, "dtype must be 0 (bf16) or 1 (fp16)");
+  c.need(total >= 0 && batch >= 0 && n_kv_heads > 0, "n_kv_heads must be positive, the other counts not negative");
+  c.need(n_kv_heads < 1 << 20, "too many heads");
+  c.need(head_dim > 0 && head_dim % 8 == 0 && head_dim <= ATTN_MAX_HD, "head_dim must be a multiple of 8, at most 128");
+  c.need(strides != nullptr, "strides is null");
+  if (c.rc) return c.rc;
+  const PoolCheck pool(c, page_bits, n_pages, page, table_cols, batch, n_kv_heads, head_dim, strides + 4);
+  long long t[4];
+  for (int i = 0; i < 4; i++) t[i] = c.stride(strides[i], i % 2 == 0 ? total : n_kv_heads);
+  if (c.rc || total == 0 || batch == 0) return c.rc;
+  if (!c.device()) return c.rc;
+  c.ptr(cu, 4, "cu"), c.ptr(k_out, 16, "k_out"), c.ptr(v_out, 16, "v_out");
+  if (table_cols) c.ptr(tables, 4, "tables");
+  if (n_pages) c.ptr(k_pages, 16, "k_pages"), c.ptr(v_pages, 16, "v_pages");
+  if (n_pages && page_bits == 8) c.ptr(k_scales, 4, "k_scales"), c.ptr(v_scales, 4, "v_scales");
+  if (c.rc) return c.rc;
+  GatherArgs a{};
+  a.kp = (const uint8_t*)k_pages, a.vp = (const uint8_t*)v_pages, a.ks = k_scales, a.vs = v_scales, a.tables = tables, a.cu = cu;
+  a.ko = k_out, a.vo = v_out;
+  for (int i = 0; i < 3; i++) a.skp[i] = pool.kp[i], a.svp[i] = pool.vp[i], a.sks[i] = pool.ks[i], a.svs[i] = pool.vs[i];
+  for (int i = 0; i < 2; i++) a.sko[i] = t[i], a.svo[i] = t[2 + i];
+  a.st = pool.st, a.T = total, a.B = batch, a.KH = n_kv_heads, a.hd = head_dim, a.n_pages = n_pages, a.cols = table_cols, a.shift = pool.shift;
+  int lpr = 1;
+  while (lpr < head_dim / (page_bits == 8 ? 16 : 8)) lpr *= 2;
+  const dim3 grid((total + PC_GATHER - 1) / PC_GATHER);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool bf = dtype == ATTN_BF16;
+  count_launches(1);
+  if (page_bits == 16) return c.done(launch_pdl(gather_pages_kernel<__half, false>, grid, PC_THREADS, 0, s, a, lpr));
+  return c.done(bf ? launch_pdl(gather_pages_kernel<__nv_bfloat16, true>, grid, PC_THREADS, 0, s, a, lpr)
+                   : launch_pdl(gather_pages_kernel<__half, true>, grid, PC_THREADS, 0, s, a, lpr));
+}

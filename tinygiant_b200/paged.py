@@ -1,0 +1,406 @@
+"""A paged key/value cache on device tensors, and positions: what a server of
+batched steps has between its layer steps when sequences come and go.
+
+  rotary_frequencies   angles per position, scaled for long contexts
+  rotary               queries and keys rotated by their positions (tg_rotary)
+  cache_append         new tokens' keys and values into their pages, rotated
+                       on the way (tg_paged_append)
+  attention_paged      the newest tokens of each sequence over its pages
+                       (tg_attention_paged)
+  cache_gather         pages read back as packed keys and values, for
+                       attention.attention_prompt (tg_paged_gather)
+
+A cache is two pools of pages, k_pages and v_pages [n_pages, KH, page, hd], and
+a table of page numbers for each sequence, tables [B, columns] int32: position
+p of sequence b is row p % page of the page tables[b, p // page].  page is a
+power of two, at least 16.  Numbers outside the pool (-1, say) are no pages:
+what would lie there is not written, has no weight, and reads as zeros, so
+pages behind a window can be given back.  Sequences may share pages that
+neither writes.
+
+Pages are of the tensors' own type, bfloat16 or float16, or of 8 bits,
+torch.float8_e4m3fn with scales k_scales and v_scales [n_pages, KH, page // 16]
+fp32: a value is its code times the scale of its block of 16 positions and key
+head.  cache_append makes scales that are powers of two, the least (but 2^-117
+at least) under which a block's values reach no further than 448; a larger
+token raises its block's scale, and the codes before it in the block are
+rounded again.  A first token of a block starts its scale anew, whatever was
+there.  attention_paged and cache_gather take any positive scales.
+
+As in tinygiant_b200.attention: calls are asynchronous on torch's current
+stream of the tensors' device, take workspace and outputs from torch's
+allocator, can be captured in a CUDA graph, give the same bits each time, and
+read lengths and tables on the device.  Tensors may be strided views: the last
+dimension is contiguous, the other strides are multiples of 16 bytes (scales
+and tables: any), and data start on 16-byte boundaries.  head_dim is a
+multiple of 8 (16 for pages of 8 bits), at most 128.  Norms, angles, rotations,
+softmax statistics and accumulators are fp32 or more.  Bad arguments raise
+ValueError before anything runs; there is no backward pass.
+"""
+import ctypes
+import math
+
+import torch
+
+from . import load
+from .attention import (_DTYPES, _NO_TENSOR, ArgumentError, _call, _empty, _fits, _no_backward, _ptr, _recording, _window,
+                        _written)
+
+__all__ = ["rotary_frequencies", "rotary", "cache_append", "attention_paged", "cache_gather", "ArgumentError"]
+
+_CODES = torch.float8_e4m3fn
+_I64x17, _I64x19, _I64x21 = ctypes.c_int64 * 17, ctypes.c_int64 * 19, ctypes.c_int64 * 21
+_I64x8 = ctypes.c_int64 * 8
+
+
+def rotary_frequencies(dim, theta=10000.0, *, scaling=None, factor=1.0, original_len=None, beta_fast=32.0, beta_slow=1.0,
+                       truncate=True, device=None):
+    """The angles per position of `dim` rotated dimensions, and the amplitude.
+
+    Pair j of dim // 2 turns by theta^(-2 j / dim) radians a position.  scaling,
+    for contexts `factor` times as long: "linear" divides all by factor; "ntk"
+    raises theta by factor^(dim / (dim - 2)); "yarn" divides those that turn
+    less than beta_slow times in original_len positions, leaves those that turn
+    more than beta_fast times, goes evenly over the pairs between (whose ends
+    are whole pairs if truncate), and has the amplitude 0.1 ln(factor) + 1.
+    Returns (fp64 tensor [dim // 2], float)."""
+    if dim <= 0 or dim % 2 or not theta > 1 or not factor >= 1:
+        raise ValueError(f"need an even dim > 0, theta > 1 and factor >= 1; got {dim}, {theta}, {factor}")
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise ValueError(f"scaling must be None, 'linear', 'ntk' or 'yarn'; is {scaling!r}")
+    if scaling == "ntk":
+        if dim <= 2:
+            raise ValueError("'ntk' needs more than one pair")
+        theta = theta * factor ** (dim / (dim - 2))
+    f = [theta ** (-2 * j / dim) for j in range(dim // 2)]
+    amplitude = 1.0
+    if scaling == "linear":
+        f = [x / factor for x in f]
+    if scaling == "yarn":
+        if not original_len or original_len < 1 or not beta_fast >= beta_slow > 0:
+            raise ValueError("'yarn' needs original_len >= 1 and beta_fast >= beta_slow > 0")
+        low, high = (dim * math.log(original_len / (n * 2 * math.pi)) / (2 * math.log(theta)) for n in (beta_fast, beta_slow))
+        if truncate:
+            low, high = math.floor(low), math.ceil(high)
+        low, high = max(low, 0), min(high, dim - 1)
+        less = [min(1.0, max(0.0, (j - low) / max(high - low, 0.001))) for j in range(dim // 2)]
+        f = [x / factor * w + x * (1 - w) for x, w in zip(f, less)]
+        amplitude = 0.1 * math.log(factor) + 1
+    return torch.tensor(f, dtype=torch.float64, device=device), amplitude
+
+
+# As in tinygiant_b200.attention, each call tests its tensors in one
+# expression, and _refuse says what is wrong when that fails.
+
+def _refuse(first, *named):
+    """Raises the ValueError of the first tensor that does not fit.  named: (name, tensor, dtypes, shape), a shape's -1 for any
+    number, None for what a call may leave out; first: the tensor that the others go by."""
+    for name, t, dtypes, shape in filter(None, named):
+        if not (isinstance(t, torch.Tensor) and t.is_cuda):
+            raise ValueError(f"{name} must be a CUDA tensor")
+        if t.device != first.device:
+            raise ValueError(f"{name} must be on {first.device}, is on {t.device}")
+        if t.dtype not in dtypes:
+            raise ValueError(f"{name} must be {' or '.join(str(d)[6:] for d in dtypes)}; is {t.dtype}")
+        if t.dim() != len(shape) or any(n not in (-1, m) for n, m in zip(shape, t.shape)):
+            raise ValueError(f"{name} {tuple(t.shape)} and the others do not fit: must be {tuple(shape)}")
+        if t.stride(-1) != 1 and not name.endswith("scales"):
+            raise ValueError(f"{name}'s last dimension must be contiguous")
+    raise ValueError("the tensors do not fit one another")
+
+
+def _vector(t, dev, dtype, n):
+    """A contiguous vector of n values, or None."""
+    return t is None or (_fits(t, dev, dtype) and t.shape == (n,))
+
+
+def _pool_fits(dev, dtype, k_pages, v_pages, tables, k_scales, v_scales, KH, hd):
+    """Whether pools, scales and tables fit key heads of `dtype`; AttributeError or IndexError for what is no tensor."""
+    N, kh, page, d = k_pages.shape
+    kind = k_pages.dtype
+    return (kh == KH and d == hd and v_pages.shape == k_pages.shape and kind in (dtype, _CODES)
+            and _fits(k_pages, dev, kind) and _fits(v_pages, dev, kind) and tables.dim() == 2 and _fits(tables, dev, torch.int32)
+            and (k_scales is None and v_scales is None if kind is dtype else
+                 k_scales.shape == v_scales.shape == (N, KH, page // 16) and k_scales.dtype is v_scales.dtype is torch.float32
+                 and k_scales.get_device() == v_scales.get_device() == dev))
+
+
+def _pool_named(dtype, k_pages, v_pages, tables, k_scales, v_scales, B, KH, hd):
+    """The same for _refuse; what it cannot say is raised here."""
+    kinds = (dtype, _CODES)
+    shape = tuple(k_pages.shape) if isinstance(k_pages, torch.Tensor) and k_pages.dim() == 4 else (-1, -1, -1, -1)
+    codes = isinstance(k_pages, torch.Tensor) and k_pages.dtype is _CODES
+    if not codes and (k_scales is not None or v_scales is not None):
+        raise ValueError("pages of 16 bits have no scales")
+    if codes and (k_scales is None or v_scales is None):
+        raise ValueError("pages of 8 bits need k_scales and v_scales")
+    return [("k_pages", k_pages, kinds, (shape[0], KH, shape[2], hd)),
+            ("v_pages", v_pages, (k_pages.dtype,) if isinstance(k_pages, torch.Tensor) else kinds, shape),
+            codes and ("k_scales", k_scales, (torch.float32,), (shape[0], KH, shape[2] // 16)),
+            codes and ("v_scales", v_scales, (torch.float32,), (shape[0], KH, shape[2] // 16)),
+            ("tables", tables, (torch.int32,), (B, -1))]
+
+
+def _pool_strides(k_pages, v_pages, tables, k_scales, v_scales):
+    k, v = k_pages.stride(), v_pages.stride()
+    ks, vs = ((1, 1, 1), (1, 1, 1)) if k_scales is None else (k_scales.stride(), v_scales.stride())
+    return (*k[:3], *v[:3], *ks, *vs, tables.stride()[0])
+
+
+def _bits(k_pages):
+    return 8 if k_pages.dtype is _CODES else 16
+
+
+def rotary(q, k, positions, freqs, *, interleaved=False, amplitude=1.0, q_norm=None, k_norm=None, eps=1e-6, out=None):
+    """Queries and keys rotated by their tokens' positions.
+
+    q [T, H, hd] and k [T, KH, hd] (or None); positions [T] int32; freqs [n]
+    fp64, the angles per position in radians (rotary_frequencies), 2 n <= hd.
+    Pair j of a head is its dimensions (j, j + n), or (2 j, 2 j + 1) if
+    interleaved; dimensions from 2 n on stay as they are.  The pairs are
+    multiplied by amplitude.  q_norm, k_norm [hd] fp32: each head is first
+    divided by sqrt(mean(x^2) + eps) and multiplied by these.
+    out: (q, k) to write, which may be q and k themselves but must not overlap
+    them in any other way.  Returns (q, k), k None if it was."""
+    try:
+        dtype, dev, (T, H, hd) = q.dtype, q.get_device(), q.shape
+        KH = 0 if k is None else k.shape[1]
+        n = freqs.shape[0]
+        given = out is not None
+        qo, ko = out if given else (_empty((T, H, hd), (H * hd, hd, 1), dtype=dtype, device=q.device),
+                                    None if k is None else _empty((T, KH, hd), (KH * hd, hd, 1), dtype=dtype, device=q.device))
+        fit = (dtype in _DTYPES and dev >= 0 and _fits(q, dev, dtype) and qo.shape == q.shape and _fits(qo, dev, dtype)
+               and (ko is None if k is None else
+                    k.shape == ko.shape == (T, KH, hd) and _fits(k, dev, dtype) and _fits(ko, dev, dtype))
+               and _vector(positions, dev, torch.int32, T) and positions is not None
+               and freqs.dim() == 1 and _fits(freqs, dev, torch.float64)
+               and _vector(q_norm, dev, torch.float32, hd) and _vector(k_norm, dev, torch.float32, hd))
+    except (*_NO_TENSOR, ValueError, TypeError):
+        fit = False
+    if not fit:
+        _refuse_rotary(q, k, positions, freqs, q_norm, k_norm, out)
+    if (q.requires_grad or (k is not None and k.requires_grad) or freqs.requires_grad
+            or (q_norm is not None and q_norm.requires_grad) or (k_norm is not None and k_norm.requires_grad)
+            or (given and (qo.requires_grad or (ko is not None and ko.requires_grad)))):
+        _no_backward()
+    (q0, q1, _), (qo0, qo1, _) = q.stride(), qo.stride()
+    (k0, k1, _), (ko0, ko1, _) = (k.stride(), ko.stride()) if k is not None else ((8, 8, 1), (8, 8, 1))
+    _call(dev, load().tg_rotary, _DTYPES[dtype], q.data_ptr(), _ptr(k), qo.data_ptr(), _ptr(ko), positions.data_ptr(),
+          freqs.data_ptr(), _ptr(q_norm), _ptr(k_norm), T, H, KH, hd, n, interleaved, amplitude, eps,
+          _I64x8(q0, q1, k0, k1, qo0, qo1, ko0, ko1))
+    if given:
+        _written(qo)
+        if ko is not None:
+            _written(ko)
+    return qo, ko
+
+
+def _refuse_rotary(q, k, positions, freqs, q_norm, k_norm, out):
+    kinds, f32 = tuple(_DTYPES), (torch.float32,)
+    if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.dtype not in kinds:
+        _refuse(q, ("q", q, kinds, (-1, -1, -1)))
+    T, H, hd = q.shape
+    same = (q.dtype,)
+    qo, ko = (None, None) if out is None else out if isinstance(out, (tuple, list)) and len(out) == 2 else (out, out)
+    _refuse(q, ("q", q, kinds, (T, H, hd)), k is not None and ("k", k, same, (T, -1, hd)),
+            ("positions", positions, (torch.int32,), (T,)), ("freqs", freqs, (torch.float64,), (-1,)),
+            q_norm is not None and ("q_norm", q_norm, f32, (hd,)), k_norm is not None and ("k_norm", k_norm, f32, (hd,)),
+            out is not None and ("out[0]", qo, same, (T, H, hd)),
+            out is not None and (k is not None or ko is not None) and ("out[1]", ko, same, tuple(k.shape) if k is not None else (0,)))
+
+
+def cache_append(k, v, k_pages, v_pages, tables, lens, cu=None, *, k_scales=None, v_scales=None, freqs=None, positions=None,
+                 interleaved=False, amplitude=1.0, q=None, q_norm=None, k_norm=None, eps=1e-6, out=None):
+    """New tokens' keys, rotated on the way, and values written to their pages.
+
+    k, v [T, KH, hd]: the new tokens of all sequences packed one after another,
+    sequence b's the rows cu[b] .. cu[b + 1] (int32 on the device, B + 1
+    ascending values; None: T / B of each).  lens [B] int32: the positions of
+    each sequence with its new tokens, which are its last.  freqs, interleaved,
+    amplitude, q_norm, k_norm and eps: as rotary; without freqs nothing is
+    rotated.  positions [T] int32: what to rotate by, if it is not the place in
+    the cache.  q [T, H, hd]: rotated as well and returned, in out if given
+    (which may be q itself).  A token whose place is no place (a position below
+    zero or behind the table, a page outside the pool) is not written there;
+    its query is rotated all the same.  Rows of no sequence are left out, the
+    query's too.  No place may be written twice in a call, and in pages of 8
+    bits no two sequences may write to one block: its values would be undefined.
+    A value that is not finite becomes NaN in 8 bits and does not count for
+    the scale.  Returns the rotated q, or None."""
+    given = out is not None
+    try:
+        dtype, dev, (T, KH, hd) = k.dtype, k.get_device(), k.shape
+        B = lens.shape[0]
+        n = 0 if freqs is None else freqs.shape[0]
+        H = 0 if q is None else q.shape[1]
+        if q is not None and not given:
+            out = _empty((T, H, hd), (H * hd, hd, 1), dtype=dtype, device=k.device)
+        fit = (dtype in _DTYPES and dev >= 0 and _fits(k, dev, dtype) and v.shape == k.shape and _fits(v, dev, dtype)
+               and _pool_fits(dev, dtype, k_pages, v_pages, tables, k_scales, v_scales, KH, hd)
+               and tables.shape[0] == B and _vector(lens, dev, torch.int32, B) and _vector(cu, dev, torch.int32, B + 1)
+               and (cu is not None or (T % B == 0 if B else T == 0)) and _vector(positions, dev, torch.int32, T)
+               and (freqs is None or (freqs.dim() == 1 and _fits(freqs, dev, torch.float64)))
+               and (out is None if q is None else
+                    q.shape == out.shape == (T, H, hd) and _fits(q, dev, dtype) and _fits(out, dev, dtype))
+               and _vector(q_norm, dev, torch.float32, hd) and _vector(k_norm, dev, torch.float32, hd))
+    except (*_NO_TENSOR, ValueError, TypeError):
+        fit = False
+    if not fit:
+        _refuse_append(k, v, k_pages, v_pages, tables, lens, cu, k_scales, v_scales, freqs, positions, q, q_norm, k_norm,
+                       out if given else None)
+    if _recording() and any(t is not None and t.requires_grad for t in (k, v, k_pages, v_pages, k_scales, v_scales, freqs, q,
+                                                                        q_norm, k_norm, out)):
+        _no_backward()
+    (k0, k1, _), (v0, v1, _) = k.stride(), v.stride()
+    (q0, q1, _), (o0, o1, _) = (q.stride(), out.stride()) if q is not None else ((8, 8, 1), (8, 8, 1))
+    N, _, page, _ = k_pages.shape
+    _call(dev, load().tg_paged_append, _DTYPES[dtype], _bits(k_pages), _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(out),
+          k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales), tables.data_ptr(), lens.data_ptr(), _ptr(cu),
+          _ptr(positions), _ptr(freqs), _ptr(q_norm), _ptr(k_norm), T, B, N, page, tables.shape[1], H, KH, hd, n, interleaved,
+          amplitude, eps,
+          _I64x21(q0, q1, k0, k1, v0, v1, o0, o1, *_pool_strides(k_pages, v_pages, tables, k_scales, v_scales)))
+    _written(k_pages)
+    _written(v_pages)
+    if k_scales is not None:
+        _written(k_scales)
+        _written(v_scales)
+    if given:
+        _written(out)
+    return out
+
+
+def _refuse_append(k, v, k_pages, v_pages, tables, lens, cu, k_scales, v_scales, freqs, positions, q, q_norm, k_norm, out):
+    kinds, i32, f32 = tuple(_DTYPES), (torch.int32,), (torch.float32,)
+    if not isinstance(k, torch.Tensor) or k.dim() != 3 or k.dtype not in kinds:
+        _refuse(k, ("k", k, kinds, (-1, -1, -1)))
+    if not isinstance(lens, torch.Tensor) or lens.dim() != 1:
+        _refuse(k, ("lens", lens, i32, (-1,)))
+    (T, KH, hd), B, same = k.shape, lens.shape[0], (k.dtype,)
+    if cu is None and (T % B if B else T):
+        raise ValueError(f"without cu there are as many tokens of each sequence; got {T} of {B}")
+    if q is None and out is not None:
+        raise ValueError("out is for q")
+    _refuse(k, ("k", k, kinds, (T, KH, hd)), ("v", v, same, (T, KH, hd)), ("lens", lens, i32, (B,)),
+            *_pool_named(k.dtype, k_pages, v_pages, tables, k_scales, v_scales, B, KH, hd),
+            cu is not None and ("cu", cu, i32, (B + 1,)), positions is not None and ("positions", positions, i32, (T,)),
+            freqs is not None and ("freqs", freqs, (torch.float64,), (-1,)), q is not None and ("q", q, same, (T, -1, hd)),
+            out is not None and ("out", out, same, tuple(q.shape)),
+            q_norm is not None and ("q_norm", q_norm, f32, (hd,)), k_norm is not None and ("k_norm", k_norm, f32, (hd,)))
+
+
+def attention_paged(q, k_pages, v_pages, tables, lens, *, k_scales=None, v_scales=None, max_len=None, window=0, sinks=None,
+                    scale=None, out=None):
+    """The newest tokens of each sequence over its pages, causal.
+
+    q [B, H, hd], one token each, or [B, n, H, hd], the n newest of each (a
+    few drafted tokens; a whole prompt is faster through cache_gather and
+    attention.attention_prompt); H a multiple of KH, up to 128 heads share a key
+    head.  lens [B] int32: the positions of each sequence, its newest tokens'
+    keys among them: query i of n is at lens - n + i and attends to the
+    positions up to it, the last `window` of them if window > 0.  max_len: an
+    upper bound of lens, if known (default: all that the tables hold); a larger
+    value in lens counts as max_len.  sinks, scale: as attention.attention_prompt.
+    A query without a key gives zeros.  Rows behind lens or before every
+    query's window are not read, and nothing that a query does not attend to
+    reaches it, infinities and NaN neither; a score of NaN or +inf among its keys
+    makes its outputs NaN, one of -inf has no weight.  With pages of 8 bits the
+    softmax weights meet the codes in fp16, else in the tensors' type.
+    Returns out, of q's shape."""
+    given = out is not None
+    try:
+        dtype, dev, shape = q.dtype, q.get_device(), q.shape
+        few = len(shape) == 4
+        B, H, hd = shape[0], shape[-2], shape[-1]
+        n = shape[1] if few else 1
+        KH = k_pages.shape[1]
+        if not given:
+            out = torch.empty(shape, dtype=dtype, device=q.device)
+        fit = (dtype in _DTYPES and dev >= 0 and (few or len(shape) == 3) and _fits(q, dev, dtype) and out.shape == shape
+               and _fits(out, dev, dtype) and _pool_fits(dev, dtype, k_pages, v_pages, tables, k_scales, v_scales, KH, hd)
+               and tables.shape[0] == B and _vector(lens, dev, torch.int32, B) and lens is not None
+               and _vector(sinks, dev, torch.float32, H))
+    except (*_NO_TENSOR, ValueError, TypeError):
+        fit = False
+    if not fit:
+        _refuse_paged(q, k_pages, v_pages, tables, lens, k_scales, v_scales, sinks, out if given else None)
+    if _recording() and any(t is not None and t.requires_grad for t in (q, k_pages, v_pages, k_scales, v_scales, sinks, out)):
+        _no_backward()
+    N, _, page, _ = k_pages.shape
+    cols = tables.shape[1]
+    most = cols * page
+    max_len = most if max_len is None or max_len > most else max_len
+    lib, bits = load(), _bits(k_pages)
+    nbytes = lib.tg_attention_paged_workspace(bits, B, n, max_len, H, KH, hd)
+    ws = _empty((nbytes,), (1,), dtype=torch.uint8, device=q.device) if nbytes else None
+    qs, os = q.stride(), out.stride()
+    q3, o3 = (qs[:3], os[:3]) if few else ((qs[0], 8, qs[1]), (os[0], 8, os[1]))
+    _call(dev, lib.tg_attention_paged, _DTYPES[dtype], bits, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales),
+          _ptr(v_scales), out.data_ptr(), tables.data_ptr(), lens.data_ptr(), _ptr(sinks), B, n, N, page, cols, max_len, H, KH, hd,
+          _I64x19(*q3, *o3, *_pool_strides(k_pages, v_pages, tables, k_scales, v_scales)), _window(window),
+          hd ** -0.5 if scale is None else scale, _ptr(ws), nbytes)
+    if given:
+        _written(out)
+    return out
+
+
+def _refuse_paged(q, k_pages, v_pages, tables, lens, k_scales, v_scales, sinks, out):
+    kinds = tuple(_DTYPES)
+    if not isinstance(q, torch.Tensor) or q.dim() not in (3, 4) or q.dtype not in kinds:
+        _refuse(q, ("q", q, kinds, (-1, -1, -1)))
+    B, H, hd = q.shape[0], q.shape[-2], q.shape[-1]
+    _refuse(q, ("q", q, kinds, tuple(q.shape)), ("lens", lens, (torch.int32,), (B,)),
+            *_pool_named(q.dtype, k_pages, v_pages, tables, k_scales, v_scales, B, -1, hd),
+            sinks is not None and ("sinks", sinks, (torch.float32,), (H,)),
+            out is not None and ("out", out, (q.dtype,), tuple(q.shape)))
+
+
+def cache_gather(k_pages, v_pages, tables, cu, total, *, k_scales=None, v_scales=None, dtype=None, out=None):
+    """The first positions of each sequence read back from its pages, packed.
+
+    Sequence b's are the rows cu[b] .. cu[b + 1] (int32 on the device, B + 1
+    ascending values) of the outputs [total, KH, hd], as attention.attention_prompt
+    takes them with cu_k=cu.  dtype: the outputs' type for pages of 8 bits
+    (bfloat16 unless out says otherwise); pages of 16 bits keep theirs.  Rows on a
+    page outside the pool or behind the table read as zeros; rows of no
+    sequence are not written.  out: (k, v) to write.  Returns (k, v)."""
+    given = out is not None
+    try:
+        kind, dev = k_pages.dtype, k_pages.get_device()
+        KH, hd = k_pages.shape[1], k_pages.shape[3]
+        dtype = (out[0].dtype if given else torch.bfloat16 if kind is _CODES else kind) if dtype is None else dtype
+        B = tables.shape[0]
+        ko, vo = out if given else (_empty((total, KH, hd), (KH * hd, hd, 1), dtype=dtype, device=k_pages.device) for _ in range(2))
+        fit = (dtype in _DTYPES and dev >= 0 and total >= 0 and ko.shape == vo.shape == (total, KH, hd) and _fits(ko, dev, dtype)
+               and _fits(vo, dev, dtype) and _pool_fits(dev, dtype, k_pages, v_pages, tables, k_scales, v_scales, KH, hd)
+               and _vector(cu, dev, torch.int32, B + 1) and cu is not None)
+    except (*_NO_TENSOR, ValueError, TypeError, RuntimeError):
+        fit = False
+    if not fit:
+        _refuse_gather(k_pages, v_pages, tables, cu, total, k_scales, v_scales, dtype, out if given else None)
+    if _recording() and any(t is not None and t.requires_grad for t in (k_pages, v_pages, k_scales, v_scales, ko, vo)):
+        _no_backward()
+    (k0, k1, _), (v0, v1, _), (N, _, page, _) = ko.stride(), vo.stride(), k_pages.shape
+    _call(dev, load().tg_paged_gather, _DTYPES[dtype], _bits(k_pages), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales),
+          _ptr(v_scales), tables.data_ptr(), cu.data_ptr(), ko.data_ptr(), vo.data_ptr(), total, B, N, page, tables.shape[1], KH, hd,
+          _I64x17(k0, k1, v0, v1, *_pool_strides(k_pages, v_pages, tables, k_scales, v_scales)))
+    if given:
+        _written(ko)
+        _written(vo)
+    return ko, vo
+
+
+def _refuse_gather(k_pages, v_pages, tables, cu, total, k_scales, v_scales, dtype, out):
+    if not isinstance(k_pages, torch.Tensor) or k_pages.dim() != 4:
+        _refuse(k_pages, ("k_pages", k_pages, (*_DTYPES, _CODES), (-1, -1, -1, -1)))
+    if not isinstance(total, int) or total < 0:
+        raise ValueError(f"total must be a number of rows; is {total!r}")
+    if dtype not in _DTYPES:
+        raise ValueError(f"dtype must be bfloat16 or float16; is {dtype}")
+    if k_pages.dtype not in (dtype, _CODES):
+        raise ValueError(f"pages of {k_pages.dtype} are not read as {dtype}")
+    KH, hd = k_pages.shape[1], k_pages.shape[3]
+    B = tables.shape[0] if isinstance(tables, torch.Tensor) and tables.dim() else -1
+    ko, vo = (None, None) if out is None else out if isinstance(out, (tuple, list)) and len(out) == 2 else (out, out)
+    _refuse(k_pages, *_pool_named(dtype, k_pages, v_pages, tables, k_scales, v_scales, B, KH, hd),
+            ("cu", cu, (torch.int32,), (B + 1,)), out is not None and ("out[0]", ko, (dtype,), (total, KH, hd)),
+            out is not None and ("out[1]", vo, (dtype,), (total, KH, hd)))
