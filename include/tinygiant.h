@@ -464,8 +464,8 @@ int tg_paged_append(int dtype, int page_bits, const void *q, const void *k, cons
  * tg_attention_prompt.  With page_bits 8 the softmax weights meet the codes in
  * fp16.  strides: q, out (sequence, token, head), then the cache's: 19 values.
  * workspace: 256-byte aligned, tg_attention_paged_workspace bytes. */
-size_t tg_attention_paged_workspace(int page_bits, int batch, int n_queries, int max_len, int n_heads, int n_kv_heads,
-                                    int head_dim);
+size_t tg_attention_paged_workspace(int page_bits, int batch, int n_queries, int max_len, int window, int n_heads,
+                                    int n_kv_heads, int head_dim);
 int tg_attention_paged(int dtype, int page_bits, const void *q, const void *k_pages, const void *v_pages,
                        const float *k_scales, const float *v_scales, void *out, const int *tables, const int *lens,
                        const float *sinks, int batch, int n_queries, int n_pages, int page, int table_cols, int max_len,

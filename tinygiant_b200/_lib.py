@@ -99,7 +99,7 @@ EXT = {
     "tg_rotary": ([CI, VP, VP, VP, VP, VP, VP, VP, VP, CI, CI, CI, CI, CI, CI, CF, CF, VP, VP], CI),
     "tg_paged_append": ([CI, CI, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, CI, CI, CI, CI, CI, CI, CI, CI,
                          CI, CI, CF, CF, VP, VP], CI),
-    "tg_attention_paged_workspace": ([CI, CI, CI, CI, CI, CI, CI], SZ),
+    "tg_attention_paged_workspace": ([CI, CI, CI, CI, CI, CI, CI, CI], SZ),
     "tg_attention_paged": ([CI, CI, VP, VP, VP, VP, VP, VP, VP, VP, VP, CI, CI, CI, CI, CI, CI, CI, CI, CI, VP, CI, CF, VP, SZ,
                             VP], CI),
     "tg_paged_gather": ([CI, CI, VP, VP, VP, VP, VP, VP, VP, VP, CI, CI, CI, CI, CI, CI, CI, VP, VP], CI),

@@ -329,14 +329,14 @@ def attention_paged(q, k_pages, v_pages, tables, lens, *, k_scales=None, v_scale
     cols = tables.shape[1]
     most = cols * page
     max_len = most if max_len is None or max_len > most else max_len
-    lib, bits = load(), _bits(k_pages)
-    nbytes = lib.tg_attention_paged_workspace(bits, B, n, max_len, H, KH, hd)
+    lib, bits, window = load(), _bits(k_pages), _window(window)
+    nbytes = lib.tg_attention_paged_workspace(bits, B, n, max_len, window, H, KH, hd)
     ws = _empty((nbytes,), (1,), dtype=torch.uint8, device=q.device) if nbytes else None
     qs, os = q.stride(), out.stride()
     q3, o3 = (qs[:3], os[:3]) if few else ((qs[0], 8, qs[1]), (os[0], 8, os[1]))
     _call(dev, lib.tg_attention_paged, _DTYPES[dtype], bits, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales),
           _ptr(v_scales), out.data_ptr(), tables.data_ptr(), lens.data_ptr(), _ptr(sinks), B, n, N, page, cols, max_len, H, KH, hd,
-          _I64x19(*q3, *o3, *_pool_strides(k_pages, v_pages, tables, k_scales, v_scales)), _window(window),
+          _I64x19(*q3, *o3, *_pool_strides(k_pages, v_pages, tables, k_scales, v_scales)), window,
           hd ** -0.5 if scale is None else scale, _ptr(ws), nbytes)
     if given:
         _written(out)
