@@ -50,8 +50,8 @@ struct PagedArgs {
   float4* pml;    // [2 group + slot][rows of a unit]: m, l, r
   int4* desc;     // [group]: sequence (-1: no unit begins here and ends later), head unit, last group
   long long sq[3], so[3];     // sequence, token, head
-  long long skp[3], svp[3];   // page, head, row; bytes
-  long long sks[3], svs[3];   // page, head, block
+  unsigned skp[3], svp[3];    // page, head, row; 16-byte words
+  unsigned sks[3], svs[3];    // page, head, block
   long long st;
   int B, n, rows, rt, KH, G, hd, cols, n_pages, shift, max_len, window;
   unsigned by_g;  // 2^32 / G, rounded up (G > 1)
@@ -107,11 +107,11 @@ __device__ __forceinline__ uint32_t paged_result(float2 v, float L, float up) {
   auto one = [&](float x) { return L == 0.f ? 0.f : x == 0.f ? x / L : x / L * s; };
   return at_pack<T>(one(v.x), one(v.y));
 }
-// Two e4m3 codes, the lower byte first, as fp16.
-__device__ __forceinline__ uint32_t pg_codes(uint32_t two) {
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)two));
-  return h;
+// Four e4m3 codes, the lowest byte first, as two pairs of fp16.
+__device__ __forceinline__ void pg_codes(uint32_t four, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(four));
 }
 
 // T: type of q and out; CODES: pages of 8 bits; HD: 64 or 128; NT: groups of 8
@@ -198,7 +198,9 @@ struct PagedShared {
   int b0[PG_MOST];                                         // and that
 };
 
-template <typename T, bool CODES, int HD, int NT>
+// MANY: more than one query of a sequence (the code that keeps apart what some
+// see, although it is hardly ever run, takes 100 instructions of each tile's 880).
+template <typename T, bool CODES, int HD, int NT, bool MANY>
 __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) paged_kernel(const PagedArgs a) {
   using S = PagedShape<T, CODES, HD, NT>;
   using M = typename S::M;
@@ -296,50 +298,77 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
   constexpr int PER = 32 / S::CH;             // rows of a warp's load
   const int r0 = lane / S::CH, c0 = lane % S::CH;
   const bool col = c0 * 16 < a.hd * (CODES ? 1 : 2);
-  const long long k_lane = r0 * a.skp[2] + c0 * 16, v_lane = r0 * a.svp[2] + c0 * 16;
+  const uint32_t to0 = S::at(r0, c0);         // this lane's word of row r0; of row r0 + i: i rows on, and bits 4 to 6 differ by i & 6
+  const uint8_t *lk = nullptr, *lv = nullptr;   // this lane's words of the unit's key head
+  const float* ls = nullptr;                    // lanes 0 .. 2 U - 1: the scales of K and V of part lane / 2
+  const unsigned s_page = lane & 1 ? a.svs[0] : a.sks[0], s_block = lane & 1 ? a.svs[2] : a.sks[2];
+  auto head = [&]() {
+    if (!lw.more()) return;
+    lk = a.kp + 16 * ((uint64_t)lw.kh * a.skp[1] + (uint64_t)r0 * a.skp[2] + c0);
+    lv = a.vp + 16 * ((uint64_t)lw.kh * a.svp[1] + (uint64_t)r0 * a.svp[2] + c0);
+    if (CODES) ls = lane & 1 ? a.vs + (uint64_t)lw.kh * a.svs[1] : a.ks + (uint64_t)lw.kh * a.sks[1];
+  };
   auto load = [&]() {
     if (lw.more()) {
       const uint32_t slot = ring32 + put * S::SLOT;
+      const int key0 = (lw.lo & ~15) + lj * KEYS;
+      int there = 0;
 #pragma unroll
       for (int u = 0; u < S::U; u++) {
-        const int key = (lw.lo & ~15) + lj * KEYS + 16 * u, row = key & ((1 << a.shift) - 1);
-        const bool there = ids[u] >= 0 && ids[u] < a.n_pages;
-        const int page = there ? ids[u] : 0, lo = lw.lo - key, n = there && col ? lw.len - lw.lo : 0;   // rows [lo, lo + n) of the part's
-        const uint8_t* k = a.kp + page * a.skp[0] + lw.kh * a.skp[1] + row * a.skp[2] + k_lane;
-        const uint8_t* v = a.vp + page * a.svp[0] + lw.kh * a.svp[1] + row * a.svp[2] + v_lane;
+        const int key = key0 + 16 * u;
+        const unsigned row = key & ((1 << a.shift) - 1);
+        const bool ok = (unsigned)ids[u] < (unsigned)a.n_pages;
+        const unsigned page = ok ? ids[u] : 0;
+        const int lo = lw.lo - key - r0, n = ok && col ? lw.len - lw.lo : 0;   // rows [lo, lo + n) from this lane's first on are there
+        there |= (int)ok << u;
+        const uint8_t* k = lk + 16 * ((uint64_t)page * a.skp[0] + (uint64_t)row * a.skp[2]);
+        const uint8_t* v = lv + 16 * ((uint64_t)page * a.svp[0] + (uint64_t)row * a.svp[2]);
 #pragma unroll
         for (int i = 0; i < 16; i += PER) {
-          const bool in = (unsigned)(i + r0 - lo) < (unsigned)n;
-          const uint32_t to = slot + S::at(16 * u + i + r0, c0);
-          cp16(to, k + i * a.skp[2], in);
-          cp16(to + S::HALF, v + i * a.svp[2], in);
+          const bool in = (unsigned)(i - lo) < (unsigned)n;
+          const uint32_t to = slot + (16 * u + i) * S::RB + (to0 ^ (i & 6) << 4);
+          cp16(to, k, in);
+          cp16(to + S::HALF, v, in);
+          k += PER * 16 * (uint64_t)a.skp[2];
+          v += PER * 16 * (uint64_t)a.svp[2];
         }
-        if (CODES && lane < 2) {
-          const int block = row / PAGED_BLOCK;
-          const float* s = lane ? a.vs + page * a.svs[0] + lw.kh * a.svs[1] + block * a.svs[2] : a.ks + page * a.sks[0] + lw.kh * a.sks[1] + block * a.sks[2];
-          cp4(slot + 2 * S::HALF + (2 * u + lane) * 4, s, there);
-        }
-        if (lane == 0) *reinterpret_cast<int*>(ring + put * S::SLOT + 2 * S::HALF + 16 + 4 * u) = there;
       }
+      if (CODES && lane < 2 * S::U) {
+        const int u = lane >> 1, id = S::U > 1 && u ? ids[S::U - 1] : ids[0];
+        const bool ok = (unsigned)id < (unsigned)a.n_pages;
+        const unsigned block = ((key0 + 16 * u) & ((1 << a.shift) - 1)) / PAGED_BLOCK;
+        cp4(slot + 2 * S::HALF + 4 * lane, ls + (uint64_t)(ok ? id : 0) * s_page + (uint64_t)block * s_block, ok);
+      }
+      if (lane == 0) *reinterpret_cast<int*>(ring + put * S::SLOT + 2 * S::HALF + 16) = there;
       if (++put == S::D) put = 0;
       lj += a.team;
     }
     cp_commit();
   };
   // On to the next tile, and its pages, whose numbers have until the next load to come.
-  auto look = [&]() {
-    while (lw.more() && lj >= lw.j1) {   // tiles behind the segment's end are the next one's
-      const int over = lj - lw.j1;
-      lw.next<KEYS>(a);
-      lj = lw.j + over;
+  const int* row_of = nullptr;
+  auto look = [&](bool again) {
+    while (lw.more() && (again || lj >= lw.j1)) {   // tiles behind the segment's end are the next one's
+      if (!again) {
+        const int over = lj - lw.j1;
+        lw.next<KEYS>(a);
+        lj = lw.j + over;
+      }
+      again = false;
+      row_of = a.tables + (long long)lw.b * a.st;
+      head();
     }
 #pragma unroll
     for (int u = 0; u < S::U; u++) {
       const int key = (lw.lo & ~15) + lj * KEYS + 16 * u;
-      ids[u] = lw.more() && key < lw.len && (key >> a.shift) < a.cols ? a.tables[lw.b * a.st + (key >> a.shift)] : -1;
+      ids[u] = lw.more() && key < lw.len && (key >> a.shift) < a.cols ? row_of[key >> a.shift] : -1;
     }
   };
   int tj = wk.j + mate, get = 0;
+  // this lane's words in the ring: K of key g, words t4 and t4 + 4; V of the keys 2 t4 and 2 t4 + 1
+  const uint32_t ko0 = S::at(g, t4), ko1 = S::KC > 1 ? S::at(g, t4 + 4) : 0;
+  const uint32_t vo0 = S::RB == 64 ? S::at(2 * t4, g >> 1) + (g & 1) * 8 : S::at(2 * t4, g);
+  const uint32_t vo1 = S::RB == 64 ? S::at(2 * t4 + 1, g >> 1) + (g & 1) * 8 : S::at(2 * t4 + 1, g);
   uint32_t qf[NT][S::STEPS][2];
   float f[NT][2];      // scale log2(e) of this lane's columns' scores, over the power of two in q
   int tok[NT][2];      // their queries
@@ -407,14 +436,15 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
       for (int t = 0; t < NT; t++) x[u][t][0] = x[u][t][1] = x[u][t][2] = x[u][t][3] = 0.f;
 #pragma unroll
       for (int w = 0; w < S::KC; w++) {
-        const uint4 lo4 = lds16(kb + S::at(16 * u + g, t4 + 4 * w)), hi4 = lds16(kb + S::at(16 * u + g + 8, t4 + 4 * w));
+        const uint32_t from = kb + 16 * u * S::RB + w / 2 * 128 + (w % 2 ? ko1 : ko0);
+        const uint4 lo4 = lds16(from), hi4 = lds16(from + 8 * S::RB);
         const uint32_t lo[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, hi[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
         constexpr int PW = S::STEPS / S::KC;
 #pragma unroll
         for (int s = 0; s < PW; s++) {
           uint32_t fr[4];
           if (CODES)
-            fr[0] = pg_codes(lo[s]), fr[1] = pg_codes(hi[s]), fr[2] = pg_codes(lo[s] >> 16), fr[3] = pg_codes(hi[s] >> 16);
+            pg_codes(lo[s], fr[0], fr[2]), pg_codes(hi[s], fr[1], fr[3]);
           else
             fr[0] = lo[2 * s & 3], fr[1] = hi[2 * s & 3], fr[2] = lo[2 * s + 1 & 3], fr[3] = hi[2 * s + 1 & 3];
 #pragma unroll
@@ -422,20 +452,22 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
         }
       }
     }
-    // scores in base 2; those that a row does not see: -inf
-    bool part = k0 < (a.window > 0 ? wk.len - a.window : 0) || k0 + KEYS > base + 1;   // not all rows see all keys
-    float lv[S::U];
-    bool there[S::U];
+    // scores in base 2, and (CODES) what they become with the values' scale; those that a row does not see: -inf
+    const int there = reinterpret_cast<const int*>(extra)[4];
+    const bool part = there != (1 << S::U) - 1 || k0 < (a.window > 0 ? wk.len - a.window : 0) || k0 + KEYS > base + 1;   // not all rows see all keys
+    float y[CODES ? S::U : 1][NT][4];
 #pragma unroll
     for (int u = 0; u < S::U; u++) {
-      const float sk = CODES ? extra[2 * u] : 1.f;
-      lv[u] = CODES ? __log2f(extra[2 * u + 1]) : 0.f;
-      there[u] = reinterpret_cast<const int*>(extra)[4 + u];
-      part |= !there[u];
+      const float sk = CODES ? extra[2 * u] : 1.f, lv = CODES ? __log2f(extra[2 * u + 1]) : 0.f;
 #pragma unroll
-      for (int t = 0; t < NT; t++)
+      for (int t = 0; t < NT; t++) {
+        const float ft[2] = {CODES ? f[t][0] * sk : f[t][0], CODES ? f[t][1] * sk : f[t][1]};
 #pragma unroll
-        for (int z = 0; z < 4; z++) x[u][t][z] *= CODES ? f[t][z & 1] * sk : f[t][z & 1];
+        for (int z = 0; z < 4; z++) {
+          x[u][t][z] *= ft[z & 1];
+          if (CODES) y[u][t][z] = x[u][t][z] + lv;
+        }
+      }
     }
     if (part) {
 #pragma unroll
@@ -448,29 +480,34 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
 #pragma unroll
             for (int h = 0; h < 2; h++) {
               const int key = k0 + 16 * u + g + h * 8;
-              if (!there[u] || key > hi || key < lo) x[u][t][z + 2 * h] = -INFINITY;
+              if (!(there >> u & 1) || key > hi || key < lo) {
+                x[u][t][z + 2 * h] = -INFINITY;
+                if (CODES) y[u][t][z + 2 * h] = -INFINITY;
+              }
             }
         }
     }
+    float top[NT][2], topy[NT][2];   // of the lane's keys; NaN where no score is a number, which counts as none
     bool up = false;
 #pragma unroll
-    for (int u = 0; u < S::U; u++)
+    for (int t = 0; t < NT; t++)
 #pragma unroll
-      for (int t = 0; t < NT; t++)
-#pragma unroll
-        for (int z = 0; z < 4; z++) up |= x[u][t][z] > limm[t][z & 1] || (CODES && x[u][t][z] + lv[u] > limr[t][z & 1]);
+      for (int z = 0; z < 2; z++) {
+        top[t][z] = fmaxf(x[0][t][z], x[0][t][z + 2]);
+        if (S::U > 1) top[t][z] = fmaxf(top[t][z], fmaxf(x[S::U - 1][t][z], x[S::U - 1][t][z + 2]));
+        up |= top[t][z] > limm[t][z];
+        if (CODES) {
+          topy[t][z] = fmaxf(y[0][t][z], y[0][t][z + 2]);
+          if (S::U > 1) topy[t][z] = fmaxf(topy[t][z], fmaxf(y[S::U - 1][t][z], y[S::U - 1][t][z + 2]));
+          up |= topy[t][z] > limr[t][z];
+        }
+      }
     if (__any_sync(~0u, up)) {
 #pragma unroll
       for (int t = 0; t < NT; t++)
 #pragma unroll
         for (int z = 0; z < 2; z++) {
-          float v = -INFINITY, w = -INFINITY;
-#pragma unroll
-          for (int u = 0; u < S::U; u++) {
-            const float y = fmaxf(x[u][t][z], x[u][t][z + 2]);
-            v = fmaxf(v, y);
-            if (CODES) w = fmaxf(w, y + lv[u]);
-          }
+          float v = top[t][z], w = CODES ? topy[t][z] : 0.f;
 #pragma unroll
           for (int sft = 4; sft < 32; sft <<= 1) {
             v = fmaxf(v, __shfl_xor_sync(~0u, v, sft));
@@ -499,10 +536,9 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
         float e[4];
 #pragma unroll
         for (int z = 0; z < 4; z++) {
-          const float y = at_exp2(x[u][t][z] + nm[t][z & 1]);
-          l[t][z & 1] += y;
-          // where the row does not see the key, whatever its scale holds
-          e[z] = !CODES ? y : x[u][t][z] == -INFINITY ? 0.f : at_exp2(x[u][t][z] + lv[u] + nr[t][z & 1]);
+          e[z] = at_exp2(x[u][t][z] + nm[t][z & 1]);
+          l[t][z & 1] += e[z];
+          if (CODES) e[z] = at_exp2(y[u][t][z] + nr[t][z & 1]);
         }
         p[u][t][0] = pg_movm(at_pack<M>(e[0], e[1]));
         p[u][t][1] = pg_movm(at_pack<M>(e[2], e[3]));
@@ -515,14 +551,14 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
       uint32_t v[4][W];
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const int row = 16 * u + 2 * t4 + (i & 1) + (i >> 1) * 8;
+        const uint32_t from = vb + (16 * u + 8 * (i >> 1)) * S::RB + (i & 1 ? vo1 : vo0);
         if (W == 2) {
-          const uint2 y = lds8(vb + S::at(row, g >> 1) + (g & 1) * 8);
+          const uint2 y = lds8(from);
           v[i][0] = y.x, v[i][W - 1] = y.y;
         } else {
 #pragma unroll
           for (int h = 0; h < W / 4; h++) {
-            const uint4 y = lds16(vb + S::at(row, g + 8 * h));
+            const uint4 y = lds16(from + 128 * h);
             v[i][4 * h] = y.x, v[i][4 * h + 1] = y.y, v[i][4 * h + 2] = y.z, v[i][4 * h + 3] = y.w;
           }
         }
@@ -530,8 +566,8 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
       auto part_of = [&](int k, uint32_t (&fr)[4]) {   // dimensions 2 k and 2 k + 1 of the lane's
         if (CODES) {
           const uint32_t sel = k & 1 ? 0x7362u : 0x5140u;
-          const uint32_t y0 = __byte_perm(v[0][k / 2], v[1][k / 2], sel), y1 = __byte_perm(v[2][k / 2], v[3][k / 2], sel);
-          fr[0] = pg_codes(y0), fr[1] = pg_codes(y0 >> 16), fr[2] = pg_codes(y1), fr[3] = pg_codes(y1 >> 16);
+          pg_codes(__byte_perm(v[0][k / 2], v[1][k / 2], sel), fr[0], fr[1]);
+          pg_codes(__byte_perm(v[2][k / 2], v[3][k / 2], sel), fr[2], fr[3]);
         } else {
           const int w = k % W;
           fr[0] = __byte_perm(v[0][w], v[1][w], 0x5410), fr[1] = __byte_perm(v[0][w], v[1][w], 0x7632);
@@ -539,7 +575,7 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
         }
       };
       uint32_t odd = 0;   // values that are not finite, where some rows may see a key and others not: 0 x NaN must not reach those
-      if (part && a.n > 1) {
+      if (MANY && part) {
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -550,7 +586,7 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
           }
         odd = __any_sync(~0u, odd != 0);
       }
-      if (!odd) {
+      if (!MANY || !odd) {
 #pragma unroll
         for (int k = 0; k < S::STEPS; k++) {
           uint32_t fr[4];
@@ -651,7 +687,7 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
   // time: 256 sequences 403 us).
   int ahead = 0;
   bool fresh = true;   // a segment that has not begun
-  look();
+  look(true);
 #pragma unroll 1
   while (wk.more()) {
     if (++ahead >= S::D) {
@@ -668,7 +704,7 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
       if (fresh) break;   // no more segments
     }
     load();
-    look();
+    look(false);
     if (ahead < S::D) continue;
     cp_wait<S::D - 1>();
     __syncwarp();
@@ -764,12 +800,12 @@ struct PagedSpace {
   }
 };
 
-template <typename T, bool CODES, int HD, int NT>
+template <typename T, bool CODES, int HD, int NT, bool MANY>
 static cudaError_t run_paged(const PagedArgs& a, const PagedSpace& sp, cudaStream_t s) {
   const int smem = PagedShape<T, CODES, HD, NT>::SMEM;
   static std::atomic<unsigned long long> set{0};
-  cudaError_t e = attn_smem(paged_kernel<T, CODES, HD, NT>, smem, set);
-  if (e == cudaSuccess) e = launch_pdl(paged_kernel<T, CODES, HD, NT>, dim3(sp.grid), PagedShape<T, CODES, HD, NT>::THREADS, smem, s, a);
+  cudaError_t e = attn_smem(paged_kernel<T, CODES, HD, NT, MANY>, smem, set);
+  if (e == cudaSuccess) e = launch_pdl(paged_kernel<T, CODES, HD, NT, MANY>, dim3(sp.grid), PagedShape<T, CODES, HD, NT>::THREADS, smem, s, a);
   count_launches(1);
   if (e == cudaSuccess && !a.whole && sp.groups > 1) {
     e = launch_pdl(paged_join_kernel<T, CODES, HD, NT>, dim3(sp.groups - 1), PG_JOIN_THREADS, 0, s, a);
@@ -779,8 +815,13 @@ static cudaError_t run_paged(const PagedArgs& a, const PagedSpace& sp, cudaStrea
 }
 template <typename T, bool CODES>
 static cudaError_t run_paged(const PagedArgs& a, const PagedSpace& sp, cudaStream_t s) {
-  if (a.hd <= 64) return sp.nt == 1 ? run_paged<T, CODES, 64, 1>(a, sp, s) : run_paged<T, CODES, 64, 2>(a, sp, s);
-  return sp.nt == 1 ? run_paged<T, CODES, 128, 1>(a, sp, s) : run_paged<T, CODES, 128, 2>(a, sp, s);
+  const bool many = a.n > 1;
+  if (a.hd <= 64) {
+    if (sp.nt == 1) return many ? run_paged<T, CODES, 64, 1, true>(a, sp, s) : run_paged<T, CODES, 64, 1, false>(a, sp, s);
+    return many ? run_paged<T, CODES, 64, 2, true>(a, sp, s) : run_paged<T, CODES, 64, 2, false>(a, sp, s);
+  }
+  if (sp.nt == 1) return many ? run_paged<T, CODES, 128, 1, true>(a, sp, s) : run_paged<T, CODES, 128, 1, false>(a, sp, s);
+  return many ? run_paged<T, CODES, 128, 2, true>(a, sp, s) : run_paged<T, CODES, 128, 2, false>(a, sp, s);
 }
 
 }  // namespace tg
@@ -836,7 +877,8 @@ extern "C" int tg_attention_paged(int dtype, int page_bits, const void* q, const
   a.po = (float*)(ws + sp.po), a.pml = (float4*)(ws + sp.pml), a.desc = (int4*)(ws + sp.desc);
   for (int i = 0; i < 3; i++) {
     a.sq[i] = t[i], a.so[i] = t[3 + i];
-    a.skp[i] = pool.kp[i], a.svp[i] = pool.vp[i], a.sks[i] = pool.ks[i], a.svs[i] = pool.vs[i];
+    a.skp[i] = (unsigned)(pool.kp[i] / 16), a.svp[i] = (unsigned)(pool.vp[i] / 16);
+    a.sks[i] = (unsigned)pool.ks[i], a.svs[i] = (unsigned)pool.vs[i];
   }
   a.st = pool.st, a.B = batch, a.n = n_queries, a.G = n_heads / n_kv_heads, a.KH = n_kv_heads, a.rows = n_queries * a.G, a.rt = sp.rt;
   a.by_g = (unsigned)(((1ull << 32) + a.G - 1) / a.G);

@@ -111,7 +111,8 @@ struct PoolCheck {
     for (int i = 0; i < 6; i++) {
       long long s = t[i];
       if (n[i % 3] > 1) {
-        c.need(s > 0 && s * bits / 8 % 16 == 0 && s < (1ll << 38), "strides of pages must be positive multiples of 16 bytes");
+        c.need(s > 0 && s < (1ll << 36) / (bits / 8) && s * bits / 8 % 16 == 0,
+               "strides of pages must be positive multiples of 16 bytes, below 2^36 bytes");
       } else {
         s = 0;
       }
@@ -120,7 +121,7 @@ struct PoolCheck {
     for (int i = 0; bits == 8 && i < 6; i++) {
       long long s = t[6 + i];
       if (nb[i % 3] > 1)
-        c.need(s > 0 && s < (1ll << 38), "strides of scales must be positive");
+        c.need(s > 0 && s < 1ll << 31, "strides of scales must be positive and below 2^31");
       else
         s = 0;
       (i < 3 ? ks[i] : vs[i - 3]) = s;

@@ -31,8 +31,8 @@ constexpr int PC_THREADS = 256;
 constexpr int PC_WARPS = PC_THREADS / 32;
 constexpr int PC_CU = 1024;       // sequences whose offsets are kept in shared memory
 constexpr int PC_WINDOW = 8;      // packed tokens that a CTA looks through for blocks' first ones, where sequences bring many
-constexpr int PC_GATHER = 16;     // rows of a gather CTA
-constexpr int PC_IN_FLIGHT = 4;   // rows that a thread has loaded before it works on the first
+constexpr int PC_GATHER = 64;     // tokens of a gather CTA, at most
+constexpr int PC_IN_FLIGHT = 3;   // rows that a thread has loaded before it works on the first
 
 enum { PC_ROTARY, PC_PAGES16, PC_PAGES8 };
 
@@ -53,15 +53,16 @@ struct CacheArgs {
   float amp, eps;
 };
 
-// cos and sin of p f radians, times amp.
+// cos and sin of p f radians, times amp, rounded once: Taylor's series at an
+// eighth of a turn at most, off by 2^-33.
 __device__ __forceinline__ float2 rope_angle(int p, double f, float amp) {
   const double t = (double)p * (f * 0.15915494309189533577);   // turns
-  const double n = rint(4.0 * t);
-  float s, c;
-  sincospif(2.f * (float)(t - 0.25 * n), &s, &c);   // at most a quarter of pi
+  const double n = rint(4.0 * t), x = 6.2831853071795864769 * (t - 0.25 * n), y = x * x;
+  const double s = amp * x * (1 + y * (-1.0 / 6 + y * (1.0 / 120 + y * (-1.0 / 5040 + y * (1.0 / 362880)))));
+  const double c = amp * (1 + y * (-1.0 / 2 + y * (1.0 / 24 + y * (-1.0 / 720 + y * (1.0 / 40320 - y * (1.0 / 3628800))))));
   const int quarter = (int)((long long)n & 3);
-  const float cs = quarter & 1 ? -s : c, sn = quarter & 1 ? c : s;
-  return quarter & 2 ? make_float2(-cs * amp, -sn * amp) : make_float2(cs * amp, sn * amp);
+  const float cs = (float)(quarter & 1 ? -s : c), sn = (float)(quarter & 1 ? c : s);
+  return quarter & 2 ? make_float2(-cs, -sn) : make_float2(cs, sn);
 }
 
 // Eight values of a row as four pairs (x[2 i], x[2 i + 1]), the lane's pairs
@@ -174,25 +175,19 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const LanePairs& m, cons
   }
 }
 
-// The lane's weights of a norm, in its pairs' order.
-__device__ __forceinline__ void load_weights(float (&w)[8], const LanePairs& m, const float* p) {
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    w[2 * i] = p && m.any() ? p[m.low(i)] : 1.f;
-    w[2 * i + 1] = p && m.any() ? p[m.high(i)] : 1.f;
-  }
-}
-// The norm over the LPR lanes of a row; lanes without values have zeros.
+// The norm over the LPR lanes of a row; lanes without values have zeros.  w: the
+// weights in the lanes' order.
 template <int LPR>
-__device__ __forceinline__ void norm_row(float (&x)[8], const float (&w)[8], int hd, float eps) {
+__device__ __forceinline__ void norm_row(float (&x)[8], const float* w, int hd, float eps) {
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; i++) s = fmaf(x[i], x[i], s);
 #pragma unroll
   for (int o = LPR / 2; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
   const float r = 1.f / sqrtf(s / hd + eps);
-#pragma unroll
-  for (int i = 0; i < 8; i++) x[i] = x[i] * r * w[i];
+  const float4 a = reinterpret_cast<const float4*>(w)[0], b = reinterpret_cast<const float4*>(w)[1];
+  x[0] *= r * a.x, x[1] *= r * a.y, x[2] *= r * a.z, x[3] *= r * a.w;
+  x[4] *= r * b.x, x[5] *= r * b.y, x[6] *= r * b.z, x[7] *= r * b.w;
 }
 // Pairs j < nf turned; the others stay as they are, whatever their neighbours hold.
 __device__ __forceinline__ void rotate_pairs(float (&x)[8], const float2 (&cs)[4], const LanePairs& m) {
@@ -214,15 +209,28 @@ __device__ __forceinline__ const int* keep_offsets(const int* cu, int B, int* s_
 
 struct CacheShared {
   int cu[PC_CU + 1];
-  float2 turn[(PC_WINDOW + PAGED_BLOCK - 1) * (ATTN_MAX_HD / 2)];   // cos, sin of tokens' pairs
+  alignas(16) float w[2][ATTN_MAX_HD];                              // norms' weights of q and k, in the lanes' order; 1 where there are none
+  alignas(16) float2 turn[PC_WINDOW + PAGED_BLOCK - 1][ATTN_MAX_HD / 2];   // cos, sin of tokens' pairs that turn
   int at[PC_WINDOW + PAGED_BLOCK - 1];                              // tokens' positions for the rotation
   int run[PC_WINDOW], len[PC_WINDOW], page[PC_WINDOW], row[PC_WINDOW];   // runs: first token, tokens, page, first row
   int runs, cover;
 };
+__device__ __forceinline__ void keep_weights(const CacheArgs& a, CacheShared& sh) {
+  for (int i = threadIdx.x; i < a.hd; i += PC_THREADS) {   // value i & 1 of pair i / 2
+    const int j = i >> 1, d = j >= a.nf || a.interleaved ? i : i & 1 ? j + a.nf : j;
+    sh.w[0][i] = a.qw ? a.qw[d] : 1.f;
+    sh.w[1][i] = a.kw ? a.kw[d] : 1.f;
+  }
+}
+__device__ __forceinline__ void load_turns(float2 (&cs)[4], const float2* turn, const LanePairs& m) {
+  const float4 a = *reinterpret_cast<const float4*>(turn + 4 * m.c), b = *reinterpret_cast<const float4*>(turn + 4 * m.c + 2);
+  cs[0] = make_float2(a.x, a.y), cs[1] = make_float2(a.z, a.w), cs[2] = make_float2(b.x, b.y), cs[3] = make_float2(b.z, b.w);
+}
 
 // One token's rows: q, and (tg_rotary, 16-bit pages) k and v.  A row is LPR
-// lanes of 8 values.
-template <typename T, int LPR, bool VEC, int MODE>
+// lanes of 8 values; a thread has PC_IN_FLIGHT rows loaded while the angles are
+// made.
+template <typename T, int LPR, bool VEC, int MODE, bool NORM>
 __device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, int t) {
   const int tid = threadIdx.x, g = tid / LPR;
   constexpr int ROWS = PC_THREADS / LPR;
@@ -237,7 +245,7 @@ __device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, 
 #pragma unroll
   for (int i = 0; i < PC_IN_FLIGHT; i++)
     if (g + i * ROWS < rows && m.any()) load_pairs(raw[i], m, source(g + i * ROWS));
-  int pos, page = -1;
+  int pos, page = -1, row = 0;
   if (MODE == PC_ROTARY) {
     pos = a.positions[t];
   } else {
@@ -249,43 +257,43 @@ __device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, 
     pos = a.positions ? a.positions[t] : p;
     if (MODE == PC_PAGES16) {
       page = paged_page(a.tables + k.seq * a.st, a.cols, p, a.shift, a.n_pages);
-      if (tid == 0) sh.row[0] = p & ((1 << a.shift) - 1);
+      row = p & ((1 << a.shift) - 1);
     }
   }
-  for (int i = tid; i < a.nf; i += PC_THREADS) sh.turn[i] = rope_angle(pos, a.freqs[i], a.amp);
-  float qw[8], kw[8];
-  load_weights(qw, m, a.qw);
-  load_weights(kw, m, a.kw);
+  for (int i = tid; i < a.nf; i += PC_THREADS) sh.turn[0][i] = rope_angle(pos, a.freqs[i], a.amp);
+  if (NORM) keep_weights(a, sh);
   __syncthreads();
-  float2 cs[4];
-#pragma unroll
-  for (int i = 0; i < 4; i++) cs[i] = 4 * m.c + i < a.nf ? sh.turn[4 * m.c + i] : make_float2(1.f, 0.f);
   for (int r0 = 0; r0 < rows; r0 += PC_IN_FLIGHT * ROWS) {
 #pragma unroll
     for (int i = 0; i < PC_IN_FLIGHT; i++) {
-      const int r = r0 + g + i * ROWS;
       if (r0 + i * ROWS >= rows) break;   // the same for the whole CTA
+      const int r = r0 + g + i * ROWS;
+      const bool is_q = r < a.H, is_v = r >= a.H + a.KH;
       float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       if (r < rows && m.any()) unpack_pairs<T>(x, raw[i], m);
-      if (a.qw || a.kw) {   // lanes of rows that have none take part in the sums
+      if (NORM) {   // lanes of rows that have none take part in the sums
         float y[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) y[e] = x[e];
-        norm_row<LPR>(y, r < a.H ? qw : kw, a.hd, a.eps);
-        if (r < a.H ? a.qw != nullptr : r < a.H + a.KH && a.kw)
+        norm_row<LPR>(y, sh.w[!is_q] + (m.any() ? 8 * m.c : 0), a.hd, a.eps);
+        if (is_q ? a.qw != nullptr : !is_v && a.kw)
 #pragma unroll
           for (int e = 0; e < 8; e++) x[e] = y[e];
       }
-      if (r < a.H + a.KH) rotate_pairs(x, cs, m);
       if (r < rows && m.any()) {
+        if (!is_v) {
+          float2 cs[4];
+          load_turns(cs, sh.turn[0], m);
+          rotate_pairs(x, cs, m);
+        }
         T* to = nullptr;
-        if (r < a.H)
+        if (is_q)
           to = (T*)a.qo + t * a.sqo[0] + r * a.sqo[1];
         else if (MODE == PC_ROTARY)
           to = (T*)a.ko + t * a.sko[0] + (r - a.H) * a.sko[1];
         else if (page >= 0)
-          to = r < a.H + a.KH ? (T*)(a.kp + page * a.skp[0] + (r - a.H) * a.skp[1] + sh.row[0] * a.skp[2])
-                              : (T*)(a.vp + page * a.svp[0] + (r - a.H - a.KH) * a.svp[1] + sh.row[0] * a.svp[2]);
+          to = is_v ? (T*)(a.vp + page * a.svp[0] + (r - a.H - a.KH) * a.svp[1] + row * a.svp[2])
+                    : (T*)(a.kp + page * a.skp[0] + (r - a.H) * a.skp[1] + row * a.skp[2]);
         if (to) store_pairs<T, VEC>(to, m, x);
       }
       const int next = r + PC_IN_FLIGHT * ROWS;
@@ -295,12 +303,15 @@ __device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, 
 }
 
 // Runs of 8-bit blocks whose first token is one of the `window` packed tokens
-// from t0 on: a warp has one run's keys or values of a key head.
-template <typename T, int LPR, bool VEC>
+// from t0 on: a warp has one run's keys or values of a key head.  Its values are
+// worked out twice, for the largest and for the codes: kept in fp32 they would
+// take 64 registers of a thread, and the warps of a CTA half as many an SM.
+template <typename T, int LPR, bool VEC, bool NORM>
 __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& sh, int t0) {
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   constexpr int RPP = 32 / LPR, PASSES = PAGED_BLOCK / RPP;
   const int* cu = keep_offsets(a.cu, a.B, sh.cu);
+  if (NORM) keep_weights(a, sh);
   __syncthreads();
   if (wid == 0) {
     const int t = t0 + lane;
@@ -324,12 +335,22 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
   }
   __syncthreads();
   if (!sh.runs) return;
-  for (int i = tid; i < sh.cover * a.nf; i += PC_THREADS) sh.turn[i] = rope_angle(sh.at[i / a.nf], a.freqs[i % a.nf], a.amp);
   const LanePairs m(a, lane % LPR);
-  float kw[8];
-  load_weights(kw, m, a.kw);
+  const int items = sh.runs * 2 * a.KH;
+  Raw<VEC> raw[PASSES];
+  auto load = [&](int item) {
+    const int i = item / (2 * a.KH), kh = item % (2 * a.KH) >> 1, j0 = sh.run[i];
+    const T* from = item & 1 ? (const T*)a.v + (long long)(t0 + j0) * a.sv[0] + kh * a.sv[1] : (const T*)a.k + (long long)(t0 + j0) * a.sk[0] + kh * a.sk[1];
+#pragma unroll
+    for (int u = 0; u < PASSES; u++) {
+      const int j = u * RPP + lane / LPR;
+      if (j < sh.len[i] && m.any()) load_pairs(raw[u], m, from + j * (item & 1 ? a.sv[0] : a.sk[0]));
+    }
+  };
+  if (wid < items) load(wid);
+  for (int i = tid; i < sh.cover * a.nf; i += PC_THREADS) sh.turn[i / a.nf][i % a.nf] = rope_angle(sh.at[i / a.nf], a.freqs[i % a.nf], a.amp);
   __syncthreads();
-  for (int item = wid; item < sh.runs * 2 * a.KH; item += PC_WARPS) {
+  for (int item = wid; item < items; item += PC_WARPS) {
     const int i = item / (2 * a.KH), kh = item % (2 * a.KH) >> 1, is_v = item & 1;
     const int j0 = sh.run[i], n = sh.len[i], off = sh.row[i] % PAGED_BLOCK, block = sh.row[i] / PAGED_BLOCK;
     uint8_t* rows = is_v ? a.vp + sh.page[i] * a.svp[0] + kh * a.svp[1] + (long long)block * PAGED_BLOCK * a.svp[2]
@@ -338,36 +359,30 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
     float* scale_at = is_v ? a.vs + sh.page[i] * a.svs[0] + kh * a.svs[1] + block * a.svs[2]
                            : a.ks + sh.page[i] * a.sks[0] + kh * a.sks[1] + block * a.sks[2];
     const float before = off ? *scale_at : 0.f;
-    Raw<VEC> raw[PASSES];
-#pragma unroll
-    for (int u = 0; u < PASSES; u++) {
+    auto values = [&](int u, float (&x)[8]) {   // of row u RPP + lane / LPR; zeros where there is none
       const int j = u * RPP + lane / LPR;
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = 0.f;
+      if (j < n && m.any()) unpack_pairs<T>(x, raw[u], m);
+      if (is_v) return;
+      if (NORM && a.kw) norm_row<LPR>(x, sh.w[1] + (m.any() ? 8 * m.c : 0), a.hd, a.eps);
       if (j < n && m.any()) {
-        const long long t = t0 + j0 + j;
-        load_pairs(raw[u], m, is_v ? (const T*)a.v + t * a.sv[0] + kh * a.sv[1] : (const T*)a.k + t * a.sk[0] + kh * a.sk[1]);
+        float2 cs[4];
+        load_turns(cs, sh.turn[j0 + j], m);
+        rotate_pairs(x, cs, m);
       }
-    }
-    float x[PASSES][8];
+    };
     uint32_t amax = 0;   // bits of the largest finite magnitude
 #pragma unroll
     for (int u = 0; u < PASSES; u++) {
       if (u * RPP >= n) break;
-      const int j = u * RPP + lane / LPR;
+      float x[8];
+      values(u, x);
 #pragma unroll
-      for (int e = 0; e < 8; e++) x[u][e] = 0.f;
-      if (j < n && m.any()) unpack_pairs<T>(x[u], raw[u], m);
-      if (!is_v) {
-        if (a.kw) norm_row<LPR>(x[u], kw, a.hd, a.eps);
-        if (j < n && m.any()) {
-          float2 cs[4];
-#pragma unroll
-          for (int e = 0; e < 4; e++) cs[e] = 4 * m.c + e < a.nf ? sh.turn[(j0 + j) * a.nf + 4 * m.c + e] : make_float2(1.f, 0.f);
-          rotate_pairs(x[u], cs, m);
-        }
+      for (int e = 0; e < 8; e++) {
+        const uint32_t y = __float_as_uint(x[e]) & 0x7fffffffu;
+        amax = max(amax, y < 0x7f800000u ? y : 0u);
       }
-#pragma unroll
-      for (int e = 0; e < 8; e++)
-        if (fabsf(x[u][e]) <= FLT_MAX) amax = max(amax, __float_as_uint(x[u][e]) & 0x7fffffffu);
     }
     amax = __reduce_max_sync(~0u, amax);
     const float need = __uint_as_float((uint32_t)(paged_scale_exp(amax) + 127) << 23);
@@ -386,25 +401,29 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
     }
 #pragma unroll
     for (int u = 0; u < PASSES; u++) {
+      if (u * RPP >= n) break;
       const int j = u * RPP + lane / LPR;
+      float x[8];
+      values(u, x);
       if (j < n && m.any()) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[u][e] *= inv;
-        store_codes<VEC>(rows + (off + j) * pitch, m, x[u]);
+        for (int e = 0; e < 8; e++) x[e] *= inv;
+        store_codes<VEC>(rows + (off + j) * pitch, m, x);
       }
     }
     if (lane == 0) *scale_at = scale;
+    if (item + PC_WARPS < items) load(item + PC_WARPS);
   }
 }
 
-template <typename T, int LPR, bool VEC, int MODE>
-__global__ void __launch_bounds__(PC_THREADS) cache_kernel(const CacheArgs a) {
+template <typename T, int LPR, bool VEC, int MODE, bool NORM>
+__global__ void __launch_bounds__(PC_THREADS, MODE == PC_PAGES8 ? 3 : 4) cache_kernel(const CacheArgs a) {
   __shared__ CacheShared sh;
   pdl_wait();
   if (MODE == PC_PAGES8 && blockIdx.x < a.run_ctas)
-    runs_of_blocks<T, LPR, VEC>(a, sh, blockIdx.x * a.window);
+    runs_of_blocks<T, LPR, VEC, NORM>(a, sh, blockIdx.x * a.window);
   else
-    token_rows<T, LPR, VEC, MODE>(a, sh, blockIdx.x - (MODE == PC_PAGES8 ? a.run_ctas : 0));
+    token_rows<T, LPR, VEC, MODE, NORM>(a, sh, blockIdx.x - (MODE == PC_PAGES8 ? a.run_ctas : 0));
 }
 
 struct GatherArgs {
@@ -416,15 +435,17 @@ struct GatherArgs {
   int T, B, KH, hd, n_pages, cols, shift;
 };
 
-// Rows of the packed outputs: 16 bytes of a page's row at a time.
+// Rows of the packed outputs, 16 bytes of a page's row at a time, four of them
+// loaded before the first is stored.  A CTA has `per` tokens.
 template <typename T, bool CODES>
-__global__ void __launch_bounds__(PC_THREADS) gather_pages_kernel(const GatherArgs a, int lpr) {
+__global__ void __launch_bounds__(PC_THREADS) gather_pages_kernel(const GatherArgs a, int lpr, int per) {
+  constexpr int N = 4;
   __shared__ int s_cu[PC_CU + 1], s_page[PC_GATHER], s_row[PC_GATHER];
   pdl_wait();
-  const int tid = threadIdx.x, t0 = blockIdx.x * PC_GATHER;
+  const int tid = threadIdx.x, t0 = blockIdx.x * per;
   const int* cu = keep_offsets(a.cu, a.B, s_cu);
   __syncthreads();
-  if (tid < PC_GATHER && t0 + tid < a.T) {
+  if (tid < per && t0 + tid < a.T) {
     const PagedToken k = paged_token(cu, a.B, 1, a.T, t0 + tid);
     const int p = t0 + tid - k.first;
     s_page[tid] = k.seq < 0 ? -2 : paged_page(a.tables + k.seq * a.st, a.cols, p, a.shift, a.n_pages);   // -2: of no sequence
@@ -433,42 +454,57 @@ __global__ void __launch_bounds__(PC_THREADS) gather_pages_kernel(const GatherAr
   __syncthreads();
   const int c = tid % lpr, chunks = a.hd / (CODES ? 16 : 8);
   if (c >= chunks) return;
-  const int rows = min(PC_GATHER, a.T - t0) * 2 * a.KH;
-#pragma unroll 4
-  for (int r = tid / lpr; r < rows; r += PC_THREADS / lpr) {
-    const int j = r / (2 * a.KH), kh = r % (2 * a.KH) % a.KH, is_v = r % (2 * a.KH) >= a.KH, page = s_page[j];
-    if (page == -2) continue;
-    uint4 w = make_uint4(0, 0, 0, 0);
-    float scale = 0.f;
-    if (page >= 0) {
-      const long long* s = is_v ? a.svp : a.skp;
-      w = *reinterpret_cast<const uint4*>((is_v ? a.vp : a.kp) + page * s[0] + kh * s[1] + s_row[j] * s[2] + c * 16);
-      if (CODES) scale = is_v ? a.vs[page * a.svs[0] + kh * a.svs[1] + s_row[j] / PAGED_BLOCK * a.svs[2]]
-                              : a.ks[page * a.sks[0] + kh * a.sks[1] + s_row[j] / PAGED_BLOCK * a.sks[2]];
+  const int rows = min(per, a.T - t0) * 2 * a.KH, step = PC_THREADS / lpr;
+  for (int r0 = tid / lpr; r0 < rows; r0 += N * step) {
+    uint4 w[N];
+    float scale[N];
+    T* to[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const int r = r0 + i * step;
+      to[i] = nullptr;
+      w[i] = make_uint4(0, 0, 0, 0);
+      scale[i] = 0.f;
+      if (r >= rows) continue;
+      const int j = r / (2 * a.KH), h = r % (2 * a.KH), is_v = h >= a.KH, kh = is_v ? h - a.KH : h, page = s_page[j], row = s_row[j];
+      if (page == -2) continue;
+      to[i] = (is_v ? (T*)a.vo + (t0 + j) * a.svo[0] + kh * a.svo[1] : (T*)a.ko + (t0 + j) * a.sko[0] + kh * a.sko[1]) + c * (CODES ? 16 : 8);
+      if (page < 0) continue;
+      w[i] = *reinterpret_cast<const uint4*>(is_v ? a.vp + page * a.svp[0] + kh * a.svp[1] + row * a.svp[2] + c * 16
+                                                  : a.kp + page * a.skp[0] + kh * a.skp[1] + row * a.skp[2] + c * 16);
+      if (CODES) scale[i] = is_v ? a.vs[page * a.svs[0] + kh * a.svs[1] + row / PAGED_BLOCK * a.svs[2]]
+                                 : a.ks[page * a.sks[0] + kh * a.sks[1] + row / PAGED_BLOCK * a.sks[2]];
     }
-    T* to = (is_v ? (T*)a.vo + (t0 + j) * a.svo[0] + kh * a.svo[1] : (T*)a.ko + (t0 + j) * a.sko[0] + kh * a.sko[1]) + c * (CODES ? 16 : 8);
-    if (!CODES) {
-      *reinterpret_cast<uint4*>(to) = w;
-    } else {
-      auto two = [&](uint32_t code) {
-        const float2 v = e4m3_values(code);
-        return page >= 0 ? at_pack<T>(v.x * scale, v.y * scale) : 0u;
-      };
-      reinterpret_cast<uint4*>(to)[0] = make_uint4(two(w.x), two(w.x >> 16), two(w.y), two(w.y >> 16));
-      reinterpret_cast<uint4*>(to)[1] = make_uint4(two(w.z), two(w.z >> 16), two(w.w), two(w.w >> 16));
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      if (!to[i]) continue;
+      if (!CODES) {
+        *reinterpret_cast<uint4*>(to[i]) = w[i];
+      } else {
+        auto two = [&](uint32_t code) {
+          const float2 v = e4m3_values(code);
+          return at_pack<T>(v.x * scale[i], v.y * scale[i]);
+        };
+        reinterpret_cast<uint4*>(to[i])[0] = make_uint4(two(w[i].x), two(w[i].x >> 16), two(w[i].y), two(w[i].y >> 16));
+        reinterpret_cast<uint4*>(to[i])[1] = make_uint4(two(w[i].z), two(w[i].z >> 16), two(w[i].w), two(w[i].w >> 16));
+      }
     }
   }
 }
 
-template <typename T, int MODE>
+template <typename T, int MODE, bool NORM>
 static cudaError_t launch_cache(const CacheArgs& a, int grid, cudaStream_t s) {
   const bool vec = a.interleaved || a.nf % 4 == 0, narrow = a.hd <= 64;
-  count_launches(1);
   if (narrow)
-    return vec ? launch_pdl(cache_kernel<T, 8, true, MODE>, dim3(grid), PC_THREADS, 0, s, a)
-               : launch_pdl(cache_kernel<T, 8, false, MODE>, dim3(grid), PC_THREADS, 0, s, a);
-  return vec ? launch_pdl(cache_kernel<T, 16, true, MODE>, dim3(grid), PC_THREADS, 0, s, a)
-             : launch_pdl(cache_kernel<T, 16, false, MODE>, dim3(grid), PC_THREADS, 0, s, a);
+    return vec ? launch_pdl(cache_kernel<T, 8, true, MODE, NORM>, dim3(grid), PC_THREADS, 0, s, a)
+               : launch_pdl(cache_kernel<T, 8, false, MODE, NORM>, dim3(grid), PC_THREADS, 0, s, a);
+  return vec ? launch_pdl(cache_kernel<T, 16, true, MODE, NORM>, dim3(grid), PC_THREADS, 0, s, a)
+             : launch_pdl(cache_kernel<T, 16, false, MODE, NORM>, dim3(grid), PC_THREADS, 0, s, a);
+}
+template <typename T, int MODE>
+static cudaError_t launch_cache(const CacheArgs& a, int grid, cudaStream_t s) {
+  count_launches(1);
+  return a.qw || a.kw ? launch_cache<T, MODE, true>(a, grid, s) : launch_cache<T, MODE, false>(a, grid, s);
 }
 
 }  // namespace tg
@@ -594,11 +630,12 @@ extern "C" int tg_paged_gather(int dtype, int page_bits, const void* k_pages, co
   a.st = pool.st, a.T = total, a.B = batch, a.KH = n_kv_heads, a.hd = head_dim, a.n_pages = n_pages, a.cols = table_cols, a.shift = pool.shift;
   int lpr = 1;
   while (lpr < head_dim / (page_bits == 8 ? 16 : 8)) lpr *= 2;
-  const dim3 grid((total + PC_GATHER - 1) / PC_GATHER);
+  const int per = total >= 64 * attn_sms() * 4 ? 64 : 16;   // tokens of a CTA
+  const dim3 grid((total + per - 1) / per);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf = dtype == ATTN_BF16;
   count_launches(1);
-  if (page_bits == 16) return c.done(launch_pdl(gather_pages_kernel<__half, false>, grid, PC_THREADS, 0, s, a, lpr));
-  return c.done(bf ? launch_pdl(gather_pages_kernel<__nv_bfloat16, true>, grid, PC_THREADS, 0, s, a, lpr)
-                   : launch_pdl(gather_pages_kernel<__half, true>, grid, PC_THREADS, 0, s, a, lpr));
+  if (page_bits == 16) return c.done(launch_pdl(gather_pages_kernel<__half, false>, grid, PC_THREADS, 0, s, a, lpr, per));
+  return c.done(bf ? launch_pdl(gather_pages_kernel<__nv_bfloat16, true>, grid, PC_THREADS, 0, s, a, lpr, per)
+                   : launch_pdl(gather_pages_kernel<__half, true>, grid, PC_THREADS, 0, s, a, lpr, per));
 }
