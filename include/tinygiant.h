@@ -481,6 +481,14 @@ int tg_paged_gather(int dtype, int page_bits, const void *k_pages, const void *v
                     int batch, int n_pages, int page, int table_cols, int n_kv_heads, int head_dim,
                     const int64_t *strides, void *stream);
 
+/* The four calls above for bindings whose calls cost by the argument: one
+ * record of 64-bit words (integers, pointers, doubles for floats): 0 tg_rotary, 1
+ * tg_paged_append, 2 tg_attention_paged or 3 tg_paged_gather, then that entry's
+ * arguments in their order, the words of strides in place of its pointer; in
+ * tg_attention_paged window stands before them.  Pointers are taken for device
+ * memory of the current device without asking the driver. */
+int tg_paged_call(const void *record);
+
 #ifdef __cplusplus
 }
 #endif

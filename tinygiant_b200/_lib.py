@@ -102,6 +102,7 @@ EXT = {
     "tg_attention_paged_workspace": ([CI, CI, CI, CI, CI, CI, CI, CI], SZ),
     "tg_attention_paged": ([CI, CI, VP, VP, VP, VP, VP, VP, VP, VP, VP, CI, CI, CI, CI, CI, CI, CI, CI, CI, VP, CI, CF, VP, SZ,
                             VP], CI),
+    "tg_paged_call": ([ctypes.c_char_p], CI),
     "tg_paged_gather": ([CI, CI, VP, VP, VP, VP, VP, VP, VP, VP, CI, CI, CI, CI, CI, CI, CI, VP, VP], CI),
 }
 

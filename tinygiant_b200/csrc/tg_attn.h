@@ -48,7 +48,8 @@ struct ArgCheck {
   const char* what;
   int dev = -1;
   int rc = 0;
-  explicit ArgCheck(const char* w) : what(w) {}
+  bool known;   // pointers are known to be null or device memory of the current device
+  explicit ArgCheck(const char* w, bool k = false) : what(w), known(k) {}
   // A condition on the arguments; the text says what is wanted.
   bool need(bool ok, const char* text) {
     if (!ok && !rc) {
@@ -70,8 +71,8 @@ struct ArgCheck {
   bool ptr(const void* p, unsigned align, const char* name) {
     if (rc) return false;
     cudaPointerAttributes a{};
-    const bool ok = p && cudaPointerGetAttributes(&a, p) == cudaSuccess &&
-                    (a.type == cudaMemoryTypeDevice || a.type == cudaMemoryTypeManaged) && a.device == dev;
+    const bool ok = p && (known || (cudaPointerGetAttributes(&a, p) == cudaSuccess &&
+                                    (a.type == cudaMemoryTypeDevice || a.type == cudaMemoryTypeManaged) && a.device == dev));
     if (!ok) {
       cudaGetLastError();
       set_host_error(3, "%s: %s must be device memory on the current device %d", what, name, dev);

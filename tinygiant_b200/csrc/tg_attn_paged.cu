@@ -830,9 +830,59 @@ using namespace tg;
 
 extern "C" size_t tg_attention_paged_workspace(int page_bits, int batch, int n_queries, int max_len, int window,
                                                int n_heads, int n_kv_heads, int head_dim) {
-  if (batch <= 0 || n_queries <= 0 || max_len <= 0 || n_kv_heads <= 0 || n_heads < n_kv_heads || n_heads / n_kv_heads > 128 || head_dim <= 0) return 0;
+  if (batch <= 0 || n_queries <= 0 || max_len <= 0 || max_len >= AT_NPOS || window < 0 || n_kv_heads <= 0 || n_heads < n_kv_heads || n_heads / n_kv_heads > 128 || head_dim <= 0) return 0;
   if ((long long)n_queries * n_heads >= 1 << 24) return 0;
   return PagedSpace(page_bits, batch, n_queries, max_len, window, n_heads, n_kv_heads, head_dim, attn_sms()).bytes;
+}
+
+int tg::attention_paged(ArgCheck& c, const AttendRecord& r) {
+  c.need(r.dtype == ATTN_BF16 || r.dtype == ATTN_FP16, "dtype must be 0 (bf16) or 1 (fp16)");
+  c.need(r.max_len < AT_NPOS, "too many positions");
+  need_ints(c, &r.batch, 10);
+  c.need(r.batch >= 0 && r.n_queries >= 0 && r.max_len >= 0 && r.window >= 0, "counts and window must not be negative");
+  c.need(r.n_heads > 0 && r.n_kv_heads > 0 && r.n_heads % r.n_kv_heads == 0 && r.n_heads / r.n_kv_heads <= 128,
+         "n_heads must be a multiple of n_kv_heads, at most 128 times it");
+  c.need(r.n_queries * r.n_heads < 1 << 24 && r.batch * r.n_queries * r.n_heads < 1ll << 31, "too many query rows");
+  c.need(r.head_dim > 0 && r.head_dim % 8 == 0 && r.head_dim <= ATTN_MAX_HD, "head_dim must be a multiple of 8, at most 128");
+  c.need(std::isfinite((float)r.scale) && (float)r.scale > 0.f, "scale must be finite and positive");
+  if (c.rc) return c.rc;
+  const int batch = (int)r.batch, queries = (int)r.n_queries, H = (int)r.n_heads, KH = (int)r.n_kv_heads, hd = (int)r.head_dim;
+  const PoolCheck pool(c, (int)r.page_bits, (int)r.n_pages, (int)r.page, (int)r.table_cols, batch, KH, hd, r.strides + 6);
+  const long long n3[3] = {batch, queries, H};
+  long long t[6];
+  for (int i = 0; i < 6; i++) t[i] = c.stride(r.strides[i], n3[i % 3]);
+  c.need(r.max_len <= r.table_cols * r.page, "max_len must be at most table_cols x page");
+  if (c.rc || batch == 0 || queries == 0) return c.rc;
+  const int max_len = r.n_pages == 0 ? 0 : (int)r.max_len;
+  if (!c.device()) return c.rc;
+  c.ptr(r.q, 16, "q"), c.ptr(r.out, 16, "out"), c.ptr(r.lens, 4, "lens");
+  if (max_len > 0) {
+    c.ptr(r.k_pages, 16, "k_pages"), c.ptr(r.v_pages, 16, "v_pages"), c.ptr(r.tables, 4, "tables");
+    if (r.page_bits == 8) c.ptr(r.k_scales, 4, "k_scales"), c.ptr(r.v_scales, 4, "v_scales");
+  }
+  if (r.sinks) c.ptr(r.sinks, 4, "sinks");
+  const PagedSpace sp((int)r.page_bits, batch, queries, max_len, (int)r.window, H, KH, hd, attn_sms());
+  c.need(r.workspace_bytes >= (int64_t)sp.bytes, "the workspace is smaller than tg_attention_paged_workspace says");
+  if (sp.bytes > 0) c.ptr(r.workspace, 256, "workspace");
+  if (c.rc) return c.rc;
+  uint8_t* ws = static_cast<uint8_t*>(r.workspace);
+  PagedArgs a{};
+  a.q = r.q, a.kp = (const uint8_t*)r.k_pages, a.vp = (const uint8_t*)r.v_pages, a.ks = (const float*)r.k_scales, a.vs = (const float*)r.v_scales;
+  a.tables = (const int*)r.tables, a.lens = (const int*)r.lens, a.sinks = (const float*)r.sinks, a.out = r.out;
+  a.po = (float*)(ws + sp.po), a.pml = (float4*)(ws + sp.pml), a.desc = (int4*)(ws + sp.desc);
+  for (int i = 0; i < 3; i++) {
+    a.sq[i] = t[i], a.so[i] = t[3 + i];
+    a.skp[i] = (unsigned)(pool.kp[i] / 16), a.svp[i] = (unsigned)(pool.vp[i] / 16);
+    a.sks[i] = (unsigned)pool.ks[i], a.svs[i] = (unsigned)pool.vs[i];
+  }
+  a.st = pool.st, a.B = batch, a.n = queries, a.G = H / KH, a.KH = KH, a.rows = queries * a.G, a.rt = sp.rt;
+  a.by_g = (unsigned)(((1ull << 32) + a.G - 1) / a.G);
+  a.hd = hd, a.cols = (int)r.table_cols, a.n_pages = (int)r.n_pages, a.shift = pool.shift, a.max_len = max_len, a.window = (int)r.window;
+  a.whole = sp.whole, a.team = sp.team, a.c = (float)r.scale * LOG2E;
+  cudaStream_t s = static_cast<cudaStream_t>(r.stream);
+  if (r.dtype == ATTN_BF16)
+    return c.done(r.page_bits == 8 ? run_paged<__nv_bfloat16, true>(a, sp, s) : run_paged<__nv_bfloat16, false>(a, sp, s));
+  return c.done(r.page_bits == 8 ? run_paged<__half, true>(a, sp, s) : run_paged<__half, false>(a, sp, s));
 }
 
 extern "C" int tg_attention_paged(int dtype, int page_bits, const void* q, const void* k_pages, const void* v_pages,
@@ -842,50 +892,9 @@ extern "C" int tg_attention_paged(int dtype, int page_bits, const void* q, const
                                   const int64_t* strides, int window, float scale, void* workspace,
                                   size_t workspace_bytes, void* stream) {
   ArgCheck c("tg_attention_paged");
-  c.need(dtype == ATTN_BF16 || dtype == ATTN_FP16, "dtype must be 0 (bf16) or 1 (fp16)");
-  c.need(batch >= 0 && n_queries >= 0 && max_len >= 0 && window >= 0, "counts and window must not be negative");
-  c.need(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && n_heads / n_kv_heads <= 128,
-         "n_heads must be a multiple of n_kv_heads, at most 128 times it");
-  c.need((long long)n_queries * n_heads < 1 << 24 && (long long)batch * n_queries * n_heads < 1ll << 31, "too many query rows");
-  c.need(head_dim > 0 && head_dim % 8 == 0 && head_dim <= ATTN_MAX_HD, "head_dim must be a multiple of 8, at most 128");
-  c.need(std::isfinite(scale) && scale > 0.f, "scale must be finite and positive");
-  c.need(strides != nullptr, "strides is null");
-  if (c.rc) return c.rc;
-  const PoolCheck pool(c, page_bits, n_pages, page, table_cols, batch, n_kv_heads, head_dim, strides + 6);
-  const long long n3[3] = {batch, n_queries, n_heads};
-  long long t[6];
-  for (int i = 0; i < 6; i++) t[i] = c.stride(strides[i], n3[i % 3]);
-  c.need(max_len <= (long long)table_cols * page, "max_len must be at most table_cols x page");
-  c.need(max_len < AT_NPOS, "too many positions");
-  if (c.rc || batch == 0 || n_queries == 0) return c.rc;
-  if (n_pages == 0) max_len = 0;
-  if (!c.device()) return c.rc;
-  c.ptr(q, 16, "q"), c.ptr(out, 16, "out"), c.ptr(lens, 4, "lens");
-  if (max_len > 0) {
-    c.ptr(k_pages, 16, "k_pages"), c.ptr(v_pages, 16, "v_pages"), c.ptr(tables, 4, "tables");
-    if (page_bits == 8) c.ptr(k_scales, 4, "k_scales"), c.ptr(v_scales, 4, "v_scales");
-  }
-  if (sinks) c.ptr(sinks, 4, "sinks");
-  const PagedSpace sp(page_bits, batch, n_queries, max_len, window, n_heads, n_kv_heads, head_dim, attn_sms());
-  c.need(workspace_bytes >= sp.bytes, "the workspace is smaller than tg_attention_paged_workspace says");
-  if (sp.bytes > 0) c.ptr(workspace, 256, "workspace");
-  if (c.rc) return c.rc;
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
-  PagedArgs a{};
-  a.q = q, a.kp = (const uint8_t*)k_pages, a.vp = (const uint8_t*)v_pages, a.ks = k_scales, a.vs = v_scales;
-  a.tables = tables, a.lens = lens, a.sinks = sinks, a.out = out;
-  a.po = (float*)(ws + sp.po), a.pml = (float4*)(ws + sp.pml), a.desc = (int4*)(ws + sp.desc);
-  for (int i = 0; i < 3; i++) {
-    a.sq[i] = t[i], a.so[i] = t[3 + i];
-    a.skp[i] = (unsigned)(pool.kp[i] / 16), a.svp[i] = (unsigned)(pool.vp[i] / 16);
-    a.sks[i] = (unsigned)pool.ks[i], a.svs[i] = (unsigned)pool.vs[i];
-  }
-  a.st = pool.st, a.B = batch, a.n = n_queries, a.G = n_heads / n_kv_heads, a.KH = n_kv_heads, a.rows = n_queries * a.G, a.rt = sp.rt;
-  a.by_g = (unsigned)(((1ull << 32) + a.G - 1) / a.G);
-  a.hd = head_dim, a.cols = table_cols, a.n_pages = n_pages, a.shift = pool.shift, a.max_len = max_len, a.window = window;
-  a.whole = sp.whole, a.team = sp.team, a.c = scale * LOG2E;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == ATTN_BF16)
-    return c.done(page_bits == 8 ? run_paged<__nv_bfloat16, true>(a, sp, s) : run_paged<__nv_bfloat16, false>(a, sp, s));
-  return c.done(page_bits == 8 ? run_paged<__half, true>(a, sp, s) : run_paged<__half, false>(a, sp, s));
+  if (!c.need(strides != nullptr, "strides is null")) return c.rc;
+  AttendRecord r{2, dtype, page_bits, q, k_pages, v_pages, k_scales, v_scales, out, tables, lens, sinks, batch, n_queries, n_pages, page,
+                 table_cols, max_len, n_heads, n_kv_heads, head_dim, window, {}, scale, workspace, (int64_t)workspace_bytes, stream};
+  std::copy(strides, strides + 19, r.strides);
+  return attention_paged(c, r);
 }

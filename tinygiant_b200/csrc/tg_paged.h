@@ -132,6 +132,50 @@ struct PoolCheck {
     }
   }
 };
+
+// The entries' arguments as one record of 64-bit words, as tg_paged_call takes
+// them; the pointers are the caller's word for device memory.
+struct RotaryRecord {
+  int64_t op, dtype;
+  const void *q, *k;
+  void *q_out, *k_out;
+  const void *positions, *freqs, *q_norm, *k_norm;
+  int64_t n_tokens, n_heads, n_kv_heads, head_dim, n_freqs, interleaved, strides[8];
+  double amplitude, eps;
+  void* stream;
+};
+struct AppendRecord {
+  int64_t op, dtype, page_bits;
+  const void *q, *k, *v;
+  void *q_out, *k_pages, *v_pages, *k_scales, *v_scales;
+  const void *tables, *lens, *cu, *positions, *freqs, *q_norm, *k_norm;
+  int64_t n_tokens, batch, n_pages, page, table_cols, n_heads, n_kv_heads, head_dim, n_freqs, interleaved, strides[21];
+  double amplitude, eps;
+  void* stream;
+};
+struct AttendRecord {
+  int64_t op, dtype, page_bits;
+  const void *q, *k_pages, *v_pages, *k_scales, *v_scales;
+  void* out;
+  const void *tables, *lens, *sinks;
+  int64_t batch, n_queries, n_pages, page, table_cols, max_len, n_heads, n_kv_heads, head_dim, window, strides[19];
+  double scale;
+  void* workspace;
+  int64_t workspace_bytes;
+  void* stream;
+};
+struct GatherRecord {
+  int64_t op, dtype, page_bits;
+  const void *k_pages, *v_pages, *k_scales, *v_scales, *tables, *cu;
+  void *k_out, *v_out;
+  int64_t total, batch, n_pages, page, table_cols, n_kv_heads, head_dim, strides[17];
+  void* stream;
+};
+// Counts of a record: the n words from `at` on, which have to be 32-bit numbers.
+inline void need_ints(ArgCheck& c, const int64_t* at, int n) {
+  for (int i = 0; i < n; i++) c.need(at[i] >= INT32_MIN && at[i] <= INT32_MAX, "a count does not fit 32 bits");
+}
+int attention_paged(ArgCheck& c, const AttendRecord& r);   // tg_attn_paged.cu
 #endif
 
 }  // namespace tg

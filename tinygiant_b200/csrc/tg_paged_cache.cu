@@ -511,38 +511,143 @@ static cudaError_t launch_cache(const CacheArgs& a, int grid, cudaStream_t s) {
 
 using namespace tg;
 
+namespace tg {
+
+static int rotary(ArgCheck& c, const RotaryRecord& r) {
+  const int64_t* strides = r.strides;
+  c.need(r.dtype == ATTN_BF16 || r.dtype == ATTN_FP16, "dtype must be 0 (bf16) or 1 (fp16)");
+  need_ints(c, &r.n_tokens, 6);
+  c.need(r.n_tokens >= 0 && r.n_heads >= 0 && r.n_kv_heads >= 0, "counts must not be negative");
+  c.need(r.n_heads < 1 << 24 && r.n_kv_heads < 1 << 24, "too many heads");
+  c.need(r.head_dim > 0 && r.head_dim % 8 == 0 && r.head_dim <= ATTN_MAX_HD, "head_dim must be a multiple of 8, at most 128");
+  c.need(r.n_freqs >= 0 && 2 * r.n_freqs <= r.head_dim, "at most head_dim / 2 frequencies");
+  c.need(std::isfinite((float)r.amplitude), "amplitude must be finite");
+  c.need(std::isfinite((float)r.eps) && r.eps >= 0, "eps must be finite and not negative");
+  if (c.rc) return c.rc;
+  long long t[8];
+  for (int i = 0; i < 8; i++) t[i] = c.stride(strides[i], i % 2 == 0 ? r.n_tokens : i / 2 % 2 == 0 ? r.n_heads : r.n_kv_heads);
+  if (c.rc || r.n_tokens == 0 || r.n_heads + r.n_kv_heads == 0) return c.rc;
+  if (!c.device()) return c.rc;
+  if (r.n_heads) c.ptr(r.q, 16, "q"), c.ptr(r.q_out, 16, "q_out");
+  if (r.n_kv_heads) c.ptr(r.k, 16, "k"), c.ptr(r.k_out, 16, "k_out");
+  c.ptr(r.positions, 4, "positions");
+  if (r.n_freqs) c.ptr(r.freqs, 8, "freqs");
+  if (r.q_norm) c.ptr(r.q_norm, 4, "q_norm");
+  if (r.k_norm) c.ptr(r.k_norm, 4, "k_norm");
+  if (c.rc) return c.rc;
+  CacheArgs a{};
+  a.q = r.q, a.k = r.k, a.qo = r.q_out, a.ko = r.k_out, a.positions = (const int*)r.positions, a.freqs = (const double*)r.freqs;
+  a.qw = (const float*)r.q_norm, a.kw = (const float*)r.k_norm;
+  for (int i = 0; i < 2; i++) a.sq[i] = t[i], a.sk[i] = t[2 + i], a.sqo[i] = t[4 + i], a.sko[i] = t[6 + i];
+  a.T = (int)r.n_tokens, a.H = (int)r.n_heads, a.KH = (int)r.n_kv_heads, a.hd = (int)r.head_dim, a.nf = (int)r.n_freqs;
+  a.interleaved = r.interleaved != 0, a.amp = (float)r.amplitude, a.eps = (float)r.eps;
+  cudaStream_t s = static_cast<cudaStream_t>(r.stream);
+  return c.done(r.dtype == ATTN_BF16 ? launch_cache<__nv_bfloat16, PC_ROTARY>(a, a.T, s) : launch_cache<__half, PC_ROTARY>(a, a.T, s));
+}
+
+static int append(ArgCheck& c, const AppendRecord& r) {
+  c.need(r.dtype == ATTN_BF16 || r.dtype == ATTN_FP16, "dtype must be 0 (bf16) or 1 (fp16)");
+  need_ints(c, &r.n_tokens, 10);
+  c.need(r.n_tokens >= 0 && r.batch >= 0 && r.n_heads >= 0 && r.n_kv_heads > 0, "n_kv_heads must be positive, the other counts not negative");
+  c.need(r.n_heads < 1 << 24 && r.n_kv_heads < 1 << 24, "too many heads");
+  c.need(r.head_dim > 0 && r.head_dim % 8 == 0 && r.head_dim <= ATTN_MAX_HD, "head_dim must be a multiple of 8, at most 128");
+  c.need(r.n_freqs >= 0 && 2 * r.n_freqs <= r.head_dim, "at most head_dim / 2 frequencies");
+  c.need(std::isfinite((float)r.amplitude), "amplitude must be finite");
+  c.need(std::isfinite((float)r.eps) && r.eps >= 0, "eps must be finite and not negative");
+  c.need(r.n_tokens == 0 || r.batch > 0, "tokens without a sequence");
+  c.need(r.cu || r.batch == 0 || r.n_tokens % r.batch == 0, "without cu there are as many tokens of each sequence");
+  c.need(r.n_tokens < 1 << 30, "too many tokens");
+  if (c.rc) return c.rc;
+  const PoolCheck pool(c, (int)r.page_bits, (int)r.n_pages, (int)r.page, (int)r.table_cols, (int)r.batch, (int)r.n_kv_heads, (int)r.head_dim,
+                       r.strides + 8);
+  long long t[8];
+  for (int i = 0; i < 8; i++)   // q, k, v, q_out
+    t[i] = c.stride(r.strides[i], i % 2 == 0 ? r.n_tokens : i / 2 == 0 || i / 2 == 3 ? r.n_heads : r.n_kv_heads);
+  if (c.rc || r.n_tokens == 0) return c.rc;
+  if (!c.device()) return c.rc;
+  c.ptr(r.k, 16, "k"), c.ptr(r.v, 16, "v"), c.ptr(r.lens, 4, "lens");
+  if (r.table_cols) c.ptr(r.tables, 4, "tables");
+  if (r.n_pages) c.ptr(r.k_pages, 16, "k_pages"), c.ptr(r.v_pages, 16, "v_pages");
+  if (r.n_pages && r.page_bits == 8) c.ptr(r.k_scales, 4, "k_scales"), c.ptr(r.v_scales, 4, "v_scales");
+  if (r.n_heads) c.ptr(r.q, 16, "q"), c.ptr(r.q_out, 16, "q_out");
+  if (r.cu) c.ptr(r.cu, 4, "cu");
+  if (r.positions) c.ptr(r.positions, 4, "positions");
+  if (r.n_freqs) c.ptr(r.freqs, 8, "freqs");
+  if (r.q_norm) c.ptr(r.q_norm, 4, "q_norm");
+  if (r.k_norm) c.ptr(r.k_norm, 4, "k_norm");
+  if (c.rc) return c.rc;
+  CacheArgs a{};
+  a.q = r.q, a.k = r.k, a.v = r.v, a.qo = r.q_out, a.kp = (uint8_t*)r.k_pages, a.vp = (uint8_t*)r.v_pages;
+  a.ks = (float*)r.k_scales, a.vs = (float*)r.v_scales, a.tables = (const int*)r.tables, a.lens = (const int*)r.lens, a.cu = (const int*)r.cu;
+  a.positions = (const int*)r.positions, a.freqs = (const double*)r.freqs, a.qw = (const float*)r.q_norm, a.kw = (const float*)r.k_norm;
+  for (int i = 0; i < 2; i++) a.sq[i] = t[i], a.sk[i] = t[2 + i], a.sv[i] = t[4 + i], a.sqo[i] = t[6 + i];
+  for (int i = 0; i < 3; i++) a.skp[i] = pool.kp[i], a.svp[i] = pool.vp[i], a.sks[i] = pool.ks[i], a.svs[i] = pool.vs[i];
+  a.st = pool.st;
+  a.T = (int)r.n_tokens, a.B = (int)r.batch, a.per = a.T / a.B, a.H = (int)r.n_heads, a.KH = (int)r.n_kv_heads, a.hd = (int)r.head_dim;
+  a.nf = (int)r.n_freqs, a.n_pages = (int)r.n_pages, a.cols = (int)r.table_cols, a.shift = pool.shift;
+  a.interleaved = r.interleaved != 0, a.amp = (float)r.amplitude, a.eps = (float)r.eps;
+  int grid = a.T;
+  if (r.page_bits == 8) {
+    a.window = a.T / a.B >= PC_WINDOW ? PC_WINDOW : 1;
+    a.run_ctas = (a.T + a.window - 1) / a.window;
+    grid = a.run_ctas + (a.H ? a.T : 0);
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(r.stream);
+  const bool bf = r.dtype == ATTN_BF16;
+  if (r.page_bits == 16)
+    return c.done(bf ? launch_cache<__nv_bfloat16, PC_PAGES16>(a, grid, s) : launch_cache<__half, PC_PAGES16>(a, grid, s));
+  return c.done(bf ? launch_cache<__nv_bfloat16, PC_PAGES8>(a, grid, s) : launch_cache<__half, PC_PAGES8>(a, grid, s));
+}
+
+static int gather(ArgCheck& c, const GatherRecord& r) {
+  c.need(r.dtype == ATTN_BF16 || r.dtype == ATTN_FP16, "dtype must be 0 (bf16) or 1 (fp16)");
+  need_ints(c, &r.total, 7);
+  c.need(r.total >= 0 && r.batch >= 0 && r.n_kv_heads > 0, "n_kv_heads must be positive, the other counts not negative");
+  c.need(r.n_kv_heads < 1 << 20, "too many heads");
+  c.need(r.head_dim > 0 && r.head_dim % 8 == 0 && r.head_dim <= ATTN_MAX_HD, "head_dim must be a multiple of 8, at most 128");
+  if (c.rc) return c.rc;
+  const PoolCheck pool(c, (int)r.page_bits, (int)r.n_pages, (int)r.page, (int)r.table_cols, (int)r.batch, (int)r.n_kv_heads, (int)r.head_dim,
+                       r.strides + 4);
+  long long t[4];
+  for (int i = 0; i < 4; i++) t[i] = c.stride(r.strides[i], i % 2 == 0 ? r.total : r.n_kv_heads);
+  if (c.rc || r.total == 0 || r.batch == 0) return c.rc;
+  if (!c.device()) return c.rc;
+  c.ptr(r.cu, 4, "cu"), c.ptr(r.k_out, 16, "k_out"), c.ptr(r.v_out, 16, "v_out");
+  if (r.table_cols) c.ptr(r.tables, 4, "tables");
+  if (r.n_pages) c.ptr(r.k_pages, 16, "k_pages"), c.ptr(r.v_pages, 16, "v_pages");
+  if (r.n_pages && r.page_bits == 8) c.ptr(r.k_scales, 4, "k_scales"), c.ptr(r.v_scales, 4, "v_scales");
+  if (c.rc) return c.rc;
+  GatherArgs a{};
+  a.kp = (const uint8_t*)r.k_pages, a.vp = (const uint8_t*)r.v_pages, a.ks = (const float*)r.k_scales, a.vs = (const float*)r.v_scales;
+  a.tables = (const int*)r.tables, a.cu = (const int*)r.cu, a.ko = r.k_out, a.vo = r.v_out;
+  for (int i = 0; i < 3; i++) a.skp[i] = pool.kp[i], a.svp[i] = pool.vp[i], a.sks[i] = pool.ks[i], a.svs[i] = pool.vs[i];
+  for (int i = 0; i < 2; i++) a.sko[i] = t[i], a.svo[i] = t[2 + i];
+  a.st = pool.st, a.T = (int)r.total, a.B = (int)r.batch, a.KH = (int)r.n_kv_heads, a.hd = (int)r.head_dim, a.n_pages = (int)r.n_pages;
+  a.cols = (int)r.table_cols, a.shift = pool.shift;
+  int lpr = 1;
+  while (lpr < a.hd / (r.page_bits == 8 ? 16 : 8)) lpr *= 2;
+  const int per = a.T >= 64 * attn_sms() * 4 ? 64 : 16;   // tokens of a CTA
+  const dim3 grid((a.T + per - 1) / per);
+  cudaStream_t s = static_cast<cudaStream_t>(r.stream);
+  const bool bf = r.dtype == ATTN_BF16;
+  count_launches(1);
+  if (r.page_bits == 16) return c.done(launch_pdl(gather_pages_kernel<__half, false>, grid, PC_THREADS, 0, s, a, lpr, per));
+  return c.done(bf ? launch_pdl(gather_pages_kernel<__nv_bfloat16, true>, grid, PC_THREADS, 0, s, a, lpr, per)
+                   : launch_pdl(gather_pages_kernel<__half, true>, grid, PC_THREADS, 0, s, a, lpr, per));
+}
+
+}  // namespace tg
+
 extern "C" int tg_rotary(int dtype, const void* q, const void* k, void* q_out, void* k_out, const int* positions,
                          const double* freqs, const float* q_norm, const float* k_norm, int n_tokens, int n_heads,
                          int n_kv_heads, int head_dim, int n_freqs, int interleaved, float amplitude, float eps,
                          const int64_t* strides, void* stream) {
   ArgCheck c("tg_rotary");
-  c.need(dtype == ATTN_BF16 || dtype == ATTN_FP16, "dtype must be 0 (bf16) or 1 (fp16)");
-  c.need(n_tokens >= 0 && n_heads >= 0 && n_kv_heads >= 0, "counts must not be negative");
-  c.need(head_dim > 0 && head_dim % 8 == 0 && head_dim <= ATTN_MAX_HD, "head_dim must be a multiple of 8, at most 128");
-  c.need(n_freqs >= 0 && 2 * (long long)n_freqs <= head_dim, "at most head_dim / 2 frequencies");
-  c.need(std::isfinite(amplitude), "amplitude must be finite");
-  c.need(std::isfinite(eps) && eps >= 0.f, "eps must be finite and not negative");
-  c.need(strides != nullptr, "strides is null");
-  if (c.rc) return c.rc;
-  long long t[8];
-  for (int i = 0; i < 8; i++) t[i] = c.stride(strides[i], i % 2 == 0 ? n_tokens : i / 2 % 2 == 0 ? n_heads : n_kv_heads);
-  if (c.rc || n_tokens == 0 || n_heads + n_kv_heads == 0) return c.rc;
-  if (!c.device()) return c.rc;
-  if (n_heads) c.ptr(q, 16, "q"), c.ptr(q_out, 16, "q_out");
-  if (n_kv_heads) c.ptr(k, 16, "k"), c.ptr(k_out, 16, "k_out");
-  c.ptr(positions, 4, "positions");
-  if (n_freqs) c.ptr(freqs, 8, "freqs");
-  if (q_norm) c.ptr(q_norm, 4, "q_norm");
-  if (k_norm) c.ptr(k_norm, 4, "k_norm");
-  if (c.rc) return c.rc;
-  CacheArgs a{};
-  a.q = q, a.k = k, a.qo = q_out, a.ko = k_out, a.positions = positions, a.freqs = freqs, a.qw = q_norm, a.kw = k_norm;
-  for (int i = 0; i < 2; i++) a.sq[i] = t[i], a.sk[i] = t[2 + i], a.sqo[i] = t[4 + i], a.sko[i] = t[6 + i];
-  a.T = n_tokens, a.H = n_heads, a.KH = n_kv_heads, a.hd = head_dim, a.nf = n_freqs;
-  a.interleaved = interleaved != 0, a.amp = amplitude, a.eps = eps;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return c.done(dtype == ATTN_BF16 ? launch_cache<__nv_bfloat16, PC_ROTARY>(a, n_tokens, s)
-                                   : launch_cache<__half, PC_ROTARY>(a, n_tokens, s));
+  if (!c.need(strides != nullptr, "strides is null")) return c.rc;
+  RotaryRecord r{0, dtype, q, k, q_out, k_out, positions, freqs, q_norm, k_norm, n_tokens, n_heads, n_kv_heads, head_dim, n_freqs,
+                 interleaved, {}, amplitude, eps, stream};
+  std::copy(strides, strides + 8, r.strides);
+  return rotary(c, r);
 }
 
 extern "C" int tg_paged_append(int dtype, int page_bits, const void* q, const void* k, const void* v, void* q_out,
@@ -552,53 +657,12 @@ extern "C" int tg_paged_append(int dtype, int page_bits, const void* q, const vo
                                int table_cols, int n_heads, int n_kv_heads, int head_dim, int n_freqs, int interleaved,
                                float amplitude, float eps, const int64_t* strides, void* stream) {
   ArgCheck c("tg_paged_append");
-  c.need(dtype == ATTN_BF16 || dtype == ATTN_FP16, "dtype must be 0 (bf16) or 1 (fp16)");
-  c.need(n_tokens >= 0 && batch >= 0 && n_heads >= 0 && n_kv_heads > 0, "n_kv_heads must be positive, the other counts not negative");
-  c.need(head_dim > 0 && head_dim % 8 == 0 && head_dim <= ATTN_MAX_HD, "head_dim must be a multiple of 8, at most 128");
-  c.need(n_freqs >= 0 && 2 * (long long)n_freqs <= head_dim, "at most head_dim / 2 frequencies");
-  c.need(std::isfinite(amplitude), "amplitude must be finite");
-  c.need(std::isfinite(eps) && eps >= 0.f, "eps must be finite and not negative");
-  c.need(n_tokens == 0 || batch > 0, "tokens without a sequence");
-  c.need(cu || batch == 0 || n_tokens % batch == 0, "without cu there are as many tokens of each sequence");
-  c.need(n_tokens < 1 << 30, "too many tokens");
-  c.need(strides != nullptr, "strides is null");
-  if (c.rc) return c.rc;
-  const PoolCheck pool(c, page_bits, n_pages, page, table_cols, batch, n_kv_heads, head_dim, strides + 8);
-  long long t[8];
-  for (int i = 0; i < 8; i++)   // q, k, v, q_out
-    t[i] = c.stride(strides[i], i % 2 == 0 ? n_tokens : i / 2 == 0 || i / 2 == 3 ? n_heads : n_kv_heads);
-  if (c.rc || n_tokens == 0) return c.rc;
-  if (!c.device()) return c.rc;
-  c.ptr(k, 16, "k"), c.ptr(v, 16, "v"), c.ptr(lens, 4, "lens");
-  if (table_cols) c.ptr(tables, 4, "tables");
-  if (n_pages) c.ptr(k_pages, 16, "k_pages"), c.ptr(v_pages, 16, "v_pages");
-  if (n_pages && page_bits == 8) c.ptr(k_scales, 4, "k_scales"), c.ptr(v_scales, 4, "v_scales");
-  if (n_heads) c.ptr(q, 16, "q"), c.ptr(q_out, 16, "q_out");
-  if (cu) c.ptr(cu, 4, "cu");
-  if (positions) c.ptr(positions, 4, "positions");
-  if (n_freqs) c.ptr(freqs, 8, "freqs");
-  if (q_norm) c.ptr(q_norm, 4, "q_norm");
-  if (k_norm) c.ptr(k_norm, 4, "k_norm");
-  if (c.rc) return c.rc;
-  CacheArgs a{};
-  a.q = q, a.k = k, a.v = v, a.qo = q_out, a.kp = (uint8_t*)k_pages, a.vp = (uint8_t*)v_pages, a.ks = k_scales, a.vs = v_scales;
-  a.tables = tables, a.lens = lens, a.cu = cu, a.positions = positions, a.freqs = freqs, a.qw = q_norm, a.kw = k_norm;
-  for (int i = 0; i < 2; i++) a.sq[i] = t[i], a.sk[i] = t[2 + i], a.sv[i] = t[4 + i], a.sqo[i] = t[6 + i];
-  for (int i = 0; i < 3; i++) a.skp[i] = pool.kp[i], a.svp[i] = pool.vp[i], a.sks[i] = pool.ks[i], a.svs[i] = pool.vs[i];
-  a.st = pool.st;
-  a.T = n_tokens, a.B = batch, a.per = n_tokens / batch, a.H = n_heads, a.KH = n_kv_heads, a.hd = head_dim, a.nf = n_freqs;
-  a.n_pages = n_pages, a.cols = table_cols, a.shift = pool.shift, a.interleaved = interleaved != 0, a.amp = amplitude, a.eps = eps;
-  int grid = n_tokens;
-  if (page_bits == 8) {
-    a.window = n_tokens / batch >= PC_WINDOW ? PC_WINDOW : 1;
-    a.run_ctas = (n_tokens + a.window - 1) / a.window;
-    grid = a.run_ctas + (n_heads ? n_tokens : 0);
-  }
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool bf = dtype == ATTN_BF16;
-  if (page_bits == 16)
-    return c.done(bf ? launch_cache<__nv_bfloat16, PC_PAGES16>(a, grid, s) : launch_cache<__half, PC_PAGES16>(a, grid, s));
-  return c.done(bf ? launch_cache<__nv_bfloat16, PC_PAGES8>(a, grid, s) : launch_cache<__half, PC_PAGES8>(a, grid, s));
+  if (!c.need(strides != nullptr, "strides is null")) return c.rc;
+  AppendRecord r{1, dtype, page_bits, q, k, v, q_out, k_pages, v_pages, k_scales, v_scales, tables, lens, cu, positions, freqs, q_norm,
+                 k_norm, n_tokens, batch, n_pages, page, table_cols, n_heads, n_kv_heads, head_dim, n_freqs, interleaved, {}, amplitude,
+                 eps, stream};
+  std::copy(strides, strides + 21, r.strides);
+  return append(c, r);
 }
 
 extern "C" int tg_paged_gather(int dtype, int page_bits, const void* k_pages, const void* v_pages, const float* k_scales,
@@ -606,36 +670,21 @@ extern "C" int tg_paged_gather(int dtype, int page_bits, const void* k_pages, co
                                int total, int batch, int n_pages, int page, int table_cols, int n_kv_heads, int head_dim,
                                const int64_t* strides, void* stream) {
   ArgCheck c("tg_paged_gather");
-  c.need(dtype == ATTN_BF16 || dtype == ATTN_FP16, "dtype must be 0 (bf16) or 1 (fp16)");
-  c.need(total >= 0 && batch >= 0 && n_kv_heads > 0, "n_kv_heads must be positive, the other counts not negative");
-  c.need(n_kv_heads < 1 << 20, "too many heads");
-  c.need(head_dim > 0 && head_dim % 8 == 0 && head_dim <= ATTN_MAX_HD, "head_dim must be a multiple of 8, at most 128");
-  c.need(strides != nullptr, "strides is null");
-  if (c.rc) return c.rc;
-  const PoolCheck pool(c, page_bits, n_pages, page, table_cols, batch, n_kv_heads, head_dim, strides + 4);
-  long long t[4];
-  for (int i = 0; i < 4; i++) t[i] = c.stride(strides[i], i % 2 == 0 ? total : n_kv_heads);
-  if (c.rc || total == 0 || batch == 0) return c.rc;
-  if (!c.device()) return c.rc;
-  c.ptr(cu, 4, "cu"), c.ptr(k_out, 16, "k_out"), c.ptr(v_out, 16, "v_out");
-  if (table_cols) c.ptr(tables, 4, "tables");
-  if (n_pages) c.ptr(k_pages, 16, "k_pages"), c.ptr(v_pages, 16, "v_pages");
-  if (n_pages && page_bits == 8) c.ptr(k_scales, 4, "k_scales"), c.ptr(v_scales, 4, "v_scales");
-  if (c.rc) return c.rc;
-  GatherArgs a{};
-  a.kp = (const uint8_t*)k_pages, a.vp = (const uint8_t*)v_pages, a.ks = k_scales, a.vs = v_scales, a.tables = tables, a.cu = cu;
-  a.ko = k_out, a.vo = v_out;
-  for (int i = 0; i < 3; i++) a.skp[i] = pool.kp[i], a.svp[i] = pool.vp[i], a.sks[i] = pool.ks[i], a.svs[i] = pool.vs[i];
-  for (int i = 0; i < 2; i++) a.sko[i] = t[i], a.svo[i] = t[2 + i];
-  a.st = pool.st, a.T = total, a.B = batch, a.KH = n_kv_heads, a.hd = head_dim, a.n_pages = n_pages, a.cols = table_cols, a.shift = pool.shift;
-  int lpr = 1;
-  while (lpr < head_dim / (page_bits == 8 ? 16 : 8)) lpr *= 2;
-  const int per = total >= 64 * attn_sms() * 4 ? 64 : 16;   // tokens of a CTA
-  const dim3 grid((total + per - 1) / per);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool bf = dtype == ATTN_BF16;
-  count_launches(1);
-  if (page_bits == 16) return c.done(launch_pdl(gather_pages_kernel<__half, false>, grid, PC_THREADS, 0, s, a, lpr, per));
-  return c.done(bf ? launch_pdl(gather_pages_kernel<__nv_bfloat16, true>, grid, PC_THREADS, 0, s, a, lpr, per)
-                   : launch_pdl(gather_pages_kernel<__half, true>, grid, PC_THREADS, 0, s, a, lpr, per));
+  if (!c.need(strides != nullptr, "strides is null")) return c.rc;
+  GatherRecord r{3, dtype, page_bits, k_pages, v_pages, k_scales, v_scales, tables, cu, k_out, v_out, total, batch, n_pages, page,
+                 table_cols, n_kv_heads, head_dim, {}, stream};
+  std::copy(strides, strides + 17, r.strides);
+  return gather(c, r);
+}
+
+extern "C" int tg_paged_call(const void* record) {
+  const int64_t op = record ? *static_cast<const int64_t*>(record) : -1;
+  static const char* const names[4] = {"tg_rotary", "tg_paged_append", "tg_attention_paged", "tg_paged_gather"};
+  ArgCheck c(op >= 0 && op < 4 ? names[op] : "tg_paged_call", true);
+  if (op == 0) return rotary(c, *static_cast<const RotaryRecord*>(record));
+  if (op == 1) return append(c, *static_cast<const AppendRecord*>(record));
+  if (op == 2) return attention_paged(c, *static_cast<const AttendRecord*>(record));
+  if (op == 3) return gather(c, *static_cast<const GatherRecord*>(record));
+  c.need(false, "the record's first word must be 0 to 3");
+  return c.rc;
 }

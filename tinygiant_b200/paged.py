@@ -37,20 +37,39 @@ multiple of 8 (16 for pages of 8 bits), at most 128.  Norms, angles, rotations,
 softmax statistics and accumulators are fp32 or more.  Bad arguments raise
 ValueError before anything runs; there is no backward pass.
 """
-import ctypes
 import math
+import struct
 
 import torch
 
-from . import load
-from .attention import (_DTYPES, _NO_TENSOR, ArgumentError, _call, _empty, _fits, _no_backward, _ptr, _recording, _window,
-                        _written)
+from . import TinyGiantCudaError, last_error, load
+from .attention import _DTYPES, _MOST, _NO_TENSOR, ArgumentError, _empty, _fits, _no_backward, _raw_stream, _window, _written
 
 __all__ = ["rotary_frequencies", "rotary", "cache_append", "attention_paged", "cache_gather", "ArgumentError"]
 
 _CODES = torch.float8_e4m3fn
-_I64x17, _I64x19, _I64x21 = ctypes.c_int64 * 17, ctypes.c_int64 * 19, ctypes.c_int64 * 21
-_I64x8 = ctypes.c_int64 * 8
+# The calls' arguments as tg_paged_call's records: a call of 30 arguments through ctypes takes 7 us, a record of them 1.
+_ROTARY, _APPEND, _ATTEND, _GATHER = (struct.Struct(f).pack for f in ("24q2dq", "49q2dq", "41qd3q", "36q"))
+
+
+def _run(device, pack, *args):
+    """One library call on torch's current stream of `device` (an index)."""
+    if device != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return _run(device, pack, *args)
+    try:
+        record = pack(*args, _raw_stream(device))
+    except struct.error as e:                      # a number that is none, or beyond 64 bits
+        raise ValueError(f"bad argument: {e}") from None
+    rc = load().tg_paged_call(record)
+    if rc:
+        code, msg = last_error()
+        raise (ArgumentError if rc == 3 else TinyGiantCudaError)(f"[{code}] {msg}")
+
+
+def _at(t):
+    """Where a tensor lies, or 0."""
+    return 0 if t is None else t.data_ptr()
 
 
 def rotary_frequencies(dim, theta=10000.0, *, scaling=None, factor=1.0, original_len=None, beta_fast=32.0, beta_slow=1.0,
@@ -143,8 +162,9 @@ def _pool_named(dtype, k_pages, v_pages, tables, k_scales, v_scales, B, KH, hd):
 
 def _pool_strides(k_pages, v_pages, tables, k_scales, v_scales):
     k, v = k_pages.stride(), v_pages.stride()
-    ks, vs = ((1, 1, 1), (1, 1, 1)) if k_scales is None else (k_scales.stride(), v_scales.stride())
-    return (*k[:3], *v[:3], *ks, *vs, tables.stride()[0])
+    if k_scales is None:
+        return (*k[:3], *v[:3], 1, 1, 1, 1, 1, 1, tables.stride()[0])
+    return (*k[:3], *v[:3], *k_scales.stride(), *v_scales.stride(), tables.stride()[0])
 
 
 def _bits(k_pages):
@@ -185,9 +205,8 @@ def rotary(q, k, positions, freqs, *, interleaved=False, amplitude=1.0, q_norm=N
         _no_backward()
     (q0, q1, _), (qo0, qo1, _) = q.stride(), qo.stride()
     (k0, k1, _), (ko0, ko1, _) = (k.stride(), ko.stride()) if k is not None else ((8, 8, 1), (8, 8, 1))
-    _call(dev, load().tg_rotary, _DTYPES[dtype], q.data_ptr(), _ptr(k), qo.data_ptr(), _ptr(ko), positions.data_ptr(),
-          freqs.data_ptr(), _ptr(q_norm), _ptr(k_norm), T, H, KH, hd, n, interleaved, amplitude, eps,
-          _I64x8(q0, q1, k0, k1, qo0, qo1, ko0, ko1))
+    _run(dev, _ROTARY, 0, _DTYPES[dtype], q.data_ptr(), _at(k), qo.data_ptr(), _at(ko), positions.data_ptr(), freqs.data_ptr(),
+         _at(q_norm), _at(k_norm), T, H, KH, hd, n, interleaved, q0, q1, k0, k1, qo0, qo1, ko0, ko1, amplitude, eps)
     if given:
         _written(qo)
         if ko is not None:
@@ -248,17 +267,18 @@ def cache_append(k, v, k_pages, v_pages, tables, lens, cu=None, *, k_scales=None
     if not fit:
         _refuse_append(k, v, k_pages, v_pages, tables, lens, cu, k_scales, v_scales, freqs, positions, q, q_norm, k_norm,
                        out if given else None)
-    if _recording() and any(t is not None and t.requires_grad for t in (k, v, k_pages, v_pages, k_scales, v_scales, freqs, q,
-                                                                        q_norm, k_norm, out)):
+    if (k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad
+            or (k_scales is not None and (k_scales.requires_grad or v_scales.requires_grad)) or (freqs is not None and freqs.requires_grad)
+            or (q is not None and (q.requires_grad or out.requires_grad)) or (q_norm is not None and q_norm.requires_grad)
+            or (k_norm is not None and k_norm.requires_grad)):
         _no_backward()
     (k0, k1, _), (v0, v1, _) = k.stride(), v.stride()
     (q0, q1, _), (o0, o1, _) = (q.stride(), out.stride()) if q is not None else ((8, 8, 1), (8, 8, 1))
     N, _, page, _ = k_pages.shape
-    _call(dev, load().tg_paged_append, _DTYPES[dtype], _bits(k_pages), _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(out),
-          k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales), tables.data_ptr(), lens.data_ptr(), _ptr(cu),
-          _ptr(positions), _ptr(freqs), _ptr(q_norm), _ptr(k_norm), T, B, N, page, tables.shape[1], H, KH, hd, n, interleaved,
-          amplitude, eps,
-          _I64x21(q0, q1, k0, k1, v0, v1, o0, o1, *_pool_strides(k_pages, v_pages, tables, k_scales, v_scales)))
+    _run(dev, _APPEND, 1, _DTYPES[dtype], _bits(k_pages), _at(q), k.data_ptr(), v.data_ptr(), _at(out), k_pages.data_ptr(),
+         v_pages.data_ptr(), _at(k_scales), _at(v_scales), tables.data_ptr(), lens.data_ptr(), _at(cu), _at(positions), _at(freqs),
+         _at(q_norm), _at(k_norm), T, B, N, page, tables.shape[1], H, KH, hd, n, interleaved, q0, q1, k0, k1, v0, v1, o0, o1,
+         *_pool_strides(k_pages, v_pages, tables, k_scales, v_scales), amplitude, eps)
     _written(k_pages)
     _written(v_pages)
     if k_scales is not None:
@@ -323,21 +343,21 @@ def attention_paged(q, k_pages, v_pages, tables, lens, *, k_scales=None, v_scale
         fit = False
     if not fit:
         _refuse_paged(q, k_pages, v_pages, tables, lens, k_scales, v_scales, sinks, out if given else None)
-    if _recording() and any(t is not None and t.requires_grad for t in (q, k_pages, v_pages, k_scales, v_scales, sinks, out)):
+    if (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad or out.requires_grad
+            or (k_scales is not None and (k_scales.requires_grad or v_scales.requires_grad)) or (sinks is not None and sinks.requires_grad)):
         _no_backward()
     N, _, page, _ = k_pages.shape
     cols = tables.shape[1]
     most = cols * page
     max_len = most if max_len is None or max_len > most else max_len
-    lib, bits, window = load(), _bits(k_pages), _window(window)
-    nbytes = lib.tg_attention_paged_workspace(bits, B, n, max_len, window, H, KH, hd)
+    bits, window = _bits(k_pages), _window(window)
+    nbytes = load().tg_attention_paged_workspace(bits, B, n, max_len, window, H, KH, hd) if 0 < max_len < _MOST else 0
     ws = _empty((nbytes,), (1,), dtype=torch.uint8, device=q.device) if nbytes else None
     qs, os = q.stride(), out.stride()
     q3, o3 = (qs[:3], os[:3]) if few else ((qs[0], 8, qs[1]), (os[0], 8, os[1]))
-    _call(dev, lib.tg_attention_paged, _DTYPES[dtype], bits, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales),
-          _ptr(v_scales), out.data_ptr(), tables.data_ptr(), lens.data_ptr(), _ptr(sinks), B, n, N, page, cols, max_len, H, KH, hd,
-          _I64x19(*q3, *o3, *_pool_strides(k_pages, v_pages, tables, k_scales, v_scales)), window,
-          hd ** -0.5 if scale is None else scale, _ptr(ws), nbytes)
+    _run(dev, _ATTEND, 2, _DTYPES[dtype], bits, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _at(k_scales), _at(v_scales),
+         out.data_ptr(), tables.data_ptr(), lens.data_ptr(), _at(sinks), B, n, N, page, cols, max_len, H, KH, hd, window, *q3, *o3,
+         *_pool_strides(k_pages, v_pages, tables, k_scales, v_scales), hd ** -0.5 if scale is None else scale, _at(ws), nbytes)
     if given:
         _written(out)
     return out
@@ -377,12 +397,13 @@ def cache_gather(k_pages, v_pages, tables, cu, total, *, k_scales=None, v_scales
         fit = False
     if not fit:
         _refuse_gather(k_pages, v_pages, tables, cu, total, k_scales, v_scales, dtype, out if given else None)
-    if _recording() and any(t is not None and t.requires_grad for t in (k_pages, v_pages, k_scales, v_scales, ko, vo)):
+    if (k_pages.requires_grad or v_pages.requires_grad or ko.requires_grad or vo.requires_grad
+            or (k_scales is not None and (k_scales.requires_grad or v_scales.requires_grad))):
         _no_backward()
     (k0, k1, _), (v0, v1, _), (N, _, page, _) = ko.stride(), vo.stride(), k_pages.shape
-    _call(dev, load().tg_paged_gather, _DTYPES[dtype], _bits(k_pages), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales),
-          _ptr(v_scales), tables.data_ptr(), cu.data_ptr(), ko.data_ptr(), vo.data_ptr(), total, B, N, page, tables.shape[1], KH, hd,
-          _I64x17(k0, k1, v0, v1, *_pool_strides(k_pages, v_pages, tables, k_scales, v_scales)))
+    _run(dev, _GATHER, 3, _DTYPES[dtype], _bits(k_pages), k_pages.data_ptr(), v_pages.data_ptr(), _at(k_scales), _at(v_scales),
+         tables.data_ptr(), cu.data_ptr(), ko.data_ptr(), vo.data_ptr(), total, B, N, page, tables.shape[1], KH, hd, k0, k1, v0, v1,
+         *_pool_strides(k_pages, v_pages, tables, k_scales, v_scales))
     if given:
         _written(ko)
         _written(vo)
