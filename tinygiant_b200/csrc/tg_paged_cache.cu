@@ -31,6 +31,7 @@ constexpr int PC_THREADS = 256;
 constexpr int PC_WARPS = PC_THREADS / 32;
 constexpr int PC_CU = 1024;       // sequences whose offsets are kept in shared memory
 constexpr int PC_WINDOW = 8;      // packed tokens that a CTA looks through for blocks' first ones, where sequences bring many
+constexpr int PC_TOKENS = 16;     // tokens of a CTA that rotates, at most
 constexpr int PC_GATHER = 64;     // tokens of a gather CTA, at most
 constexpr int PC_IN_FLIGHT = 3;   // rows that a thread has loaded before it works on the first
 
@@ -48,7 +49,7 @@ struct CacheArgs {
   long long skp[3], svp[3];   // page, head, row; bytes
   long long sks[3], svs[3];   // page, head, block
   long long st;               // tables' row
-  int T, B, per, H, KH, hd, nf, n_pages, cols, shift, run_ctas, window;
+  int T, B, per, H, KH, hd, nf, n_pages, cols, shift, run_ctas, window, tokens;
   int interleaved;
   float amp, eps;
 };
@@ -212,7 +213,7 @@ struct CacheShared {
   alignas(16) float w[2][ATTN_MAX_HD];                              // norms' weights of q and k, in the lanes' order; 1 where there are none
   alignas(16) float2 turn[PC_WINDOW + PAGED_BLOCK - 1][ATTN_MAX_HD / 2];   // cos, sin of tokens' pairs that turn
   int at[PC_WINDOW + PAGED_BLOCK - 1];                              // tokens' positions for the rotation
-  int run[PC_WINDOW], len[PC_WINDOW], page[PC_WINDOW], row[PC_WINDOW];   // runs: first token, tokens, page, first row
+  int run[PC_WINDOW], len[PC_WINDOW], page[PC_TOKENS], row[PC_TOKENS];   // runs: first token, tokens; runs' or tokens' page and (first) row
   int runs, cover;
 };
 __device__ __forceinline__ void keep_weights(const CacheArgs& a, CacheShared& sh) {
@@ -227,47 +228,65 @@ __device__ __forceinline__ void load_turns(float2 (&cs)[4], const float2* turn, 
   cs[0] = make_float2(a.x, a.y), cs[1] = make_float2(a.z, a.w), cs[2] = make_float2(b.x, b.y), cs[3] = make_float2(b.z, b.w);
 }
 
-// One token's rows: q, and (tg_rotary, 16-bit pages) k and v.  A row is LPR
-// lanes of 8 values; a thread has PC_IN_FLIGHT rows loaded while the angles are
-// made.
+// The rows of nt tokens from t0 on: q, and (tg_rotary, 16-bit pages) k and v.  A
+// row is LPR lanes of 8 values; the rows of all tokens follow one another, and a
+// thread has PC_IN_FLIGHT of them loaded ahead.  A token's angles are made while
+// the one before it is turned.
 template <typename T, int LPR, bool VEC, int MODE, bool NORM>
-__device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, int t) {
+__device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, int t0, int nt) {
   const int tid = threadIdx.x, g = tid / LPR;
   constexpr int ROWS = PC_THREADS / LPR;
   const LanePairs m(a, tid % LPR);
-  const int rows = a.H + (MODE == PC_PAGES8 ? 0 : a.KH) + (MODE == PC_PAGES16 ? a.KH : 0);
-  auto source = [&](int r) -> const T* {
-    if (r < a.H) return (const T*)a.q + t * a.sq[0] + r * a.sq[1];
-    if (r < a.H + a.KH) return (const T*)a.k + t * a.sk[0] + (r - a.H) * a.sk[1];
-    return (const T*)a.v + t * a.sv[0] + (r - a.H - a.KH) * a.sv[1];
-  };
+  const int rows = a.H + (MODE == PC_PAGES8 ? 0 : a.KH) + (MODE == PC_PAGES16 ? a.KH : 0), passes = (rows + ROWS - 1) / ROWS;
   Raw<VEC> raw[PC_IN_FLIGHT];
+  int ltok = 0, lpass = 0;   // the next row to load
+  auto load = [&](Raw<VEC>& to) {
+    if (ltok >= nt) return;
+    const int r = g + lpass * ROWS;
+    const long long t = t0 + ltok;
+    if (r < rows && m.any())
+      load_pairs(to, m, r < a.H          ? (const T*)a.q + t * a.sq[0] + r * a.sq[1]
+                        : r < a.H + a.KH ? (const T*)a.k + t * a.sk[0] + (r - a.H) * a.sk[1]
+                                         : (const T*)a.v + t * a.sv[0] + (r - a.H - a.KH) * a.sv[1]);
+    if (++lpass == passes) lpass = 0, ltok++;
+  };
 #pragma unroll
-  for (int i = 0; i < PC_IN_FLIGHT; i++)
-    if (g + i * ROWS < rows && m.any()) load_pairs(raw[i], m, source(g + i * ROWS));
-  int pos, page = -1, row = 0;
-  if (MODE == PC_ROTARY) {
-    pos = a.positions[t];
-  } else {
-    const int* cu = keep_offsets(a.cu, a.B, sh.cu);
-    if (a.cu) __syncthreads();
-    const PagedToken k = paged_token(cu, a.B, a.per, a.T, t);
-    if (k.seq < 0) return;   // of no sequence: the whole CTA, all threads have the same token
-    const int p = paged_position(a.lens[k.seq], k.end, t);
-    pos = a.positions ? a.positions[t] : p;
-    if (MODE == PC_PAGES16) {
-      page = paged_page(a.tables + k.seq * a.st, a.cols, p, a.shift, a.n_pages);
-      row = p & ((1 << a.shift) - 1);
-    }
-  }
-  for (int i = tid; i < a.nf; i += PC_THREADS) sh.turn[0][i] = rope_angle(pos, a.freqs[i], a.amp);
+  for (int i = 0; i < PC_IN_FLIGHT; i++) load(raw[i]);
+  const int* cu = MODE == PC_ROTARY ? nullptr : keep_offsets(a.cu, a.B, sh.cu);
   if (NORM) keep_weights(a, sh);
+  if (MODE != PC_ROTARY) __syncthreads();
+  if (tid < nt) {
+    int pos = 0, page = -1, row = 0;
+    if (MODE == PC_ROTARY) {
+      pos = a.positions[t0 + tid];
+    } else {
+      const PagedToken k = paged_token(cu, a.B, a.per, a.T, t0 + tid);
+      page = -2;   // of no sequence
+      if (k.seq >= 0) {
+        const int p = paged_position(a.lens[k.seq], k.end, t0 + tid);
+        pos = a.positions ? a.positions[t0 + tid] : p;
+        page = MODE == PC_PAGES16 ? paged_page(a.tables + k.seq * a.st, a.cols, p, a.shift, a.n_pages) : -1;
+        row = p & ((1 << a.shift) - 1);
+      }
+    }
+    sh.at[tid] = pos, sh.page[tid] = page, sh.row[tid] = row;
+  }
+  auto angles = [&](int i) {
+    for (int j = tid; j < a.nf; j += PC_THREADS) sh.turn[i & 1][j] = rope_angle(sh.at[i], a.freqs[j], a.amp);
+  };
   __syncthreads();
-  for (int r0 = 0; r0 < rows; r0 += PC_IN_FLIGHT * ROWS) {
+  angles(0);
+  int tok = 0, pass = 0;
+  for (int k0 = 0; k0 < nt * passes; k0 += PC_IN_FLIGHT) {
 #pragma unroll
     for (int i = 0; i < PC_IN_FLIGHT; i++) {
-      if (r0 + i * ROWS >= rows) break;   // the same for the whole CTA
-      const int r = r0 + g + i * ROWS;
+      if (tok >= nt) break;   // the same for the whole CTA
+      if (pass == 0) {
+        __syncthreads();
+        if (tok + 1 < nt) angles(tok + 1);
+      }
+      const int r = g + pass * ROWS, page = MODE == PC_ROTARY ? -1 : sh.page[tok];
+      const long long t = t0 + tok;
       const bool is_q = r < a.H, is_v = r >= a.H + a.KH;
       float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       if (r < rows && m.any()) unpack_pairs<T>(x, raw[i], m);
@@ -280,10 +299,10 @@ __device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, 
 #pragma unroll
           for (int e = 0; e < 8; e++) x[e] = y[e];
       }
-      if (r < rows && m.any()) {
+      if (r < rows && m.any() && page != -2) {
         if (!is_v) {
           float2 cs[4];
-          load_turns(cs, sh.turn[0], m);
+          load_turns(cs, sh.turn[tok & 1], m);
           rotate_pairs(x, cs, m);
         }
         T* to = nullptr;
@@ -292,12 +311,12 @@ __device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, 
         else if (MODE == PC_ROTARY)
           to = (T*)a.ko + t * a.sko[0] + (r - a.H) * a.sko[1];
         else if (page >= 0)
-          to = is_v ? (T*)(a.vp + page * a.svp[0] + (r - a.H - a.KH) * a.svp[1] + row * a.svp[2])
-                    : (T*)(a.kp + page * a.skp[0] + (r - a.H) * a.skp[1] + row * a.skp[2]);
+          to = is_v ? (T*)(a.vp + page * a.svp[0] + (r - a.H - a.KH) * a.svp[1] + sh.row[tok] * a.svp[2])
+                    : (T*)(a.kp + page * a.skp[0] + (r - a.H) * a.skp[1] + sh.row[tok] * a.skp[2]);
         if (to) store_pairs<T, VEC>(to, m, x);
       }
-      const int next = r + PC_IN_FLIGHT * ROWS;
-      if (next < rows && m.any()) load_pairs(raw[i], m, source(next));
+      load(raw[i]);
+      if (++pass == passes) pass = 0, tok++;
     }
   }
 }
@@ -422,8 +441,10 @@ __global__ void __launch_bounds__(PC_THREADS, MODE == PC_PAGES8 ? 3 : 4) cache_k
   pdl_wait();
   if (MODE == PC_PAGES8 && blockIdx.x < a.run_ctas)
     runs_of_blocks<T, LPR, VEC, NORM>(a, sh, blockIdx.x * a.window);
-  else
-    token_rows<T, LPR, VEC, MODE, NORM>(a, sh, blockIdx.x - (MODE == PC_PAGES8 ? a.run_ctas : 0));
+  else {
+    const int t0 = (blockIdx.x - (MODE == PC_PAGES8 ? a.run_ctas : 0)) * a.tokens;
+    token_rows<T, LPR, VEC, MODE, NORM>(a, sh, t0, min(a.tokens, a.T - t0));
+  }
 }
 
 struct GatherArgs {
@@ -433,6 +454,7 @@ struct GatherArgs {
   void *ko, *vo;
   long long skp[3], svp[3], sks[3], svs[3], sko[2], svo[2], st;
   int T, B, KH, hd, n_pages, cols, shift;
+  int wide;   // outputs in 32-byte pieces: rows start on 32-byte boundaries
 };
 
 // Rows of the packed outputs, 16 bytes of a page's row at a time, four of them
@@ -485,8 +507,14 @@ __global__ void __launch_bounds__(PC_THREADS) gather_pages_kernel(const GatherAr
           const float2 v = e4m3_values(code);
           return at_pack<T>(v.x * scale[i], v.y * scale[i]);
         };
-        reinterpret_cast<uint4*>(to[i])[0] = make_uint4(two(w[i].x), two(w[i].x >> 16), two(w[i].y), two(w[i].y >> 16));
-        reinterpret_cast<uint4*>(to[i])[1] = make_uint4(two(w[i].z), two(w[i].z >> 16), two(w[i].w), two(w[i].w >> 16));
+        const uint32_t y[8] = {two(w[i].x), two(w[i].x >> 16), two(w[i].y), two(w[i].y >> 16),
+                               two(w[i].z), two(w[i].z >> 16), two(w[i].w), two(w[i].w >> 16)};
+        if (a.wide) {
+          at_store8(to[i], y);
+        } else {
+          reinterpret_cast<uint4*>(to[i])[0] = make_uint4(y[0], y[1], y[2], y[3]);
+          reinterpret_cast<uint4*>(to[i])[1] = make_uint4(y[4], y[5], y[6], y[7]);
+        }
       }
     }
   }
@@ -512,6 +540,13 @@ static cudaError_t launch_cache(const CacheArgs& a, int grid, cudaStream_t s) {
 using namespace tg;
 
 namespace tg {
+
+// Tokens of a CTA, so that all CTAs are there at once where PC_TOKENS allow it; the CTAs.
+static int token_ctas(CacheArgs& a, int per_sm) {
+  const int most = attn_sms() * per_sm;
+  a.tokens = std::min(PC_TOKENS, (a.T + most - 1) / most);
+  return (a.T + a.tokens - 1) / a.tokens;
+}
 
 static int rotary(ArgCheck& c, const RotaryRecord& r) {
   const int64_t* strides = r.strides;
@@ -542,7 +577,8 @@ static int rotary(ArgCheck& c, const RotaryRecord& r) {
   a.T = (int)r.n_tokens, a.H = (int)r.n_heads, a.KH = (int)r.n_kv_heads, a.hd = (int)r.head_dim, a.nf = (int)r.n_freqs;
   a.interleaved = r.interleaved != 0, a.amp = (float)r.amplitude, a.eps = (float)r.eps;
   cudaStream_t s = static_cast<cudaStream_t>(r.stream);
-  return c.done(r.dtype == ATTN_BF16 ? launch_cache<__nv_bfloat16, PC_ROTARY>(a, a.T, s) : launch_cache<__half, PC_ROTARY>(a, a.T, s));
+  const int grid = token_ctas(a, 4);
+  return c.done(r.dtype == ATTN_BF16 ? launch_cache<__nv_bfloat16, PC_ROTARY>(a, grid, s) : launch_cache<__half, PC_ROTARY>(a, grid, s));
 }
 
 static int append(ArgCheck& c, const AppendRecord& r) {
@@ -586,11 +622,11 @@ static int append(ArgCheck& c, const AppendRecord& r) {
   a.T = (int)r.n_tokens, a.B = (int)r.batch, a.per = a.T / a.B, a.H = (int)r.n_heads, a.KH = (int)r.n_kv_heads, a.hd = (int)r.head_dim;
   a.nf = (int)r.n_freqs, a.n_pages = (int)r.n_pages, a.cols = (int)r.table_cols, a.shift = pool.shift;
   a.interleaved = r.interleaved != 0, a.amp = (float)r.amplitude, a.eps = (float)r.eps;
-  int grid = a.T;
+  int grid = token_ctas(a, r.page_bits == 8 ? 3 : 4);
   if (r.page_bits == 8) {
     a.window = a.T / a.B >= PC_WINDOW ? PC_WINDOW : 1;
     a.run_ctas = (a.T + a.window - 1) / a.window;
-    grid = a.run_ctas + (a.H ? a.T : 0);
+    grid = a.run_ctas + (a.H ? grid : 0);
   }
   cudaStream_t s = static_cast<cudaStream_t>(r.stream);
   const bool bf = r.dtype == ATTN_BF16;
@@ -624,6 +660,7 @@ static int gather(ArgCheck& c, const GatherRecord& r) {
   for (int i = 0; i < 2; i++) a.sko[i] = t[i], a.svo[i] = t[2 + i];
   a.st = pool.st, a.T = (int)r.total, a.B = (int)r.batch, a.KH = (int)r.n_kv_heads, a.hd = (int)r.head_dim, a.n_pages = (int)r.n_pages;
   a.cols = (int)r.table_cols, a.shift = pool.shift;
+  a.wide = ((uintptr_t)r.k_out | (uintptr_t)r.v_out) % 32 == 0 && (t[0] | t[1] | t[2] | t[3]) % 16 == 0;
   int lpr = 1;
   while (lpr < a.hd / (r.page_bits == 8 ? 16 : 8)) lpr *= 2;
   const int per = a.T >= 64 * attn_sms() * 4 ? 64 : 16;   // tokens of a CTA

@@ -43,11 +43,12 @@ import struct
 import torch
 
 from . import TinyGiantCudaError, last_error, load
-from .attention import _DTYPES, _MOST, _NO_TENSOR, ArgumentError, _empty, _fits, _no_backward, _raw_stream, _window, _written
+from .attention import _DTYPES, _MOST, ArgumentError, _empty, _no_backward, _raw_stream, _window, _written
 
 __all__ = ["rotary_frequencies", "rotary", "cache_append", "attention_paged", "cache_gather", "ArgumentError"]
 
 _CODES = torch.float8_e4m3fn
+_MISFITS = (AttributeError, IndexError, KeyError, TypeError, ValueError)   # of what is no tensor, or of other dimensions
 # The calls' arguments as tg_paged_call's records: a call of 30 arguments through ctypes takes 7 us, a record of them 1.
 _ROTARY, _APPEND, _ATTEND, _GATHER = (struct.Struct(f).pack for f in ("24q2dq", "49q2dq", "41qd3q", "36q"))
 
@@ -129,19 +130,29 @@ def _refuse(first, *named):
 
 
 def _vector(t, dev, dtype, n):
-    """A contiguous vector of n values, or None."""
-    return t is None or (_fits(t, dev, dtype) and t.shape == (n,))
+    """Whether t is a contiguous vector of n values."""
+    return t.dtype is dtype and t.get_device() == dev and t.shape == (n,) and (n < 2 or t.stride() == (1,))
 
 
-def _pool_fits(dev, dtype, k_pages, v_pages, tables, k_scales, v_scales, KH, hd):
-    """Whether pools, scales and tables fit key heads of `dtype`; AttributeError or IndexError for what is no tensor."""
-    N, kh, page, d = k_pages.shape
-    kind = k_pages.dtype
-    return (kh == KH and d == hd and v_pages.shape == k_pages.shape and kind in (dtype, _CODES)
-            and _fits(k_pages, dev, kind) and _fits(v_pages, dev, kind) and tables.dim() == 2 and _fits(tables, dev, torch.int32)
-            and (k_scales is None and v_scales is None if kind is dtype else
-                 k_scales.shape == v_scales.shape == (N, KH, page // 16) and k_scales.dtype is v_scales.dtype is torch.float32
-                 and k_scales.get_device() == v_scales.get_device() == dev))
+def _pool(dev, dtype, k_pages, v_pages, tables, k_scales, v_scales, KH, hd):
+    """The cache's strides as the library takes them, or None where pools, scales and tables do not fit key heads of `dtype`;
+    AttributeError, IndexError or ValueError for what is no tensor, or of other dimensions."""
+    shape, kind = k_pages.shape, k_pages.dtype
+    N, kh, page, d = shape
+    k0, k1, k2, k3 = k_pages.stride()
+    v0, v1, v2, v3 = v_pages.stride()
+    t0, t1 = tables.stride()
+    if not (kh == KH and d == hd and v_pages.shape == shape and v_pages.dtype is kind and k3 == v3 == t1 == 1
+            and tables.dtype is torch.int32 and k_pages.get_device() == v_pages.get_device() == tables.get_device() == dev):
+        return None
+    if kind is _CODES:
+        if not (k_scales.shape == v_scales.shape == (N, kh, page // 16) and k_scales.dtype is v_scales.dtype is torch.float32
+                and k_scales.get_device() == v_scales.get_device() == dev):
+            return None
+        return (k0, k1, k2, v0, v1, v2, *k_scales.stride(), *v_scales.stride(), t0)
+    if kind is not dtype or k_scales is not None or v_scales is not None:
+        return None
+    return (k0, k1, k2, v0, v1, v2, 1, 1, 1, 1, 1, 1, t0)
 
 
 def _pool_named(dtype, k_pages, v_pages, tables, k_scales, v_scales, B, KH, hd):
@@ -160,13 +171,6 @@ def _pool_named(dtype, k_pages, v_pages, tables, k_scales, v_scales, B, KH, hd):
             ("tables", tables, (torch.int32,), (B, -1))]
 
 
-def _pool_strides(k_pages, v_pages, tables, k_scales, v_scales):
-    k, v = k_pages.stride(), v_pages.stride()
-    if k_scales is None:
-        return (*k[:3], *v[:3], 1, 1, 1, 1, 1, 1, tables.stride()[0])
-    return (*k[:3], *v[:3], *k_scales.stride(), *v_scales.stride(), tables.stride()[0])
-
-
 def _bits(k_pages):
     return 8 if k_pages.dtype is _CODES else 16
 
@@ -182,31 +186,41 @@ def rotary(q, k, positions, freqs, *, interleaved=False, amplitude=1.0, q_norm=N
     divided by sqrt(mean(x^2) + eps) and multiplied by these.
     out: (q, k) to write, which may be q and k themselves but must not overlap
     them in any other way.  Returns (q, k), k None if it was."""
+    given = out is not None
     try:
-        dtype, dev, (T, H, hd) = q.dtype, q.get_device(), q.shape
-        KH = 0 if k is None else k.shape[1]
-        n = freqs.shape[0]
-        given = out is not None
-        qo, ko = out if given else (_empty((T, H, hd), (H * hd, hd, 1), dtype=dtype, device=q.device),
-                                    None if k is None else _empty((T, KH, hd), (KH * hd, hd, 1), dtype=dtype, device=q.device))
-        fit = (dtype in _DTYPES and dev >= 0 and _fits(q, dev, dtype) and qo.shape == q.shape and _fits(qo, dev, dtype)
-               and (ko is None if k is None else
-                    k.shape == ko.shape == (T, KH, hd) and _fits(k, dev, dtype) and _fits(ko, dev, dtype))
-               and _vector(positions, dev, torch.int32, T) and positions is not None
-               and freqs.dim() == 1 and _fits(freqs, dev, torch.float64)
-               and _vector(q_norm, dev, torch.float32, hd) and _vector(k_norm, dev, torch.float32, hd))
-    except (*_NO_TENSOR, ValueError, TypeError):
+        dtype, dev, (T, H, hd), (q0, q1, q2) = q.dtype, q.get_device(), q.shape, q.stride()
+        kind = _DTYPES[dtype]
+        if given:
+            qo, ko = out
+            o0, o1, o2 = qo.stride()
+            fit = qo.dtype is dtype and qo.get_device() == dev and qo.shape == q.shape
+        else:
+            o0, o1, o2 = max(H, 1) * hd, hd, 1
+            qo, ko, fit = _empty((T, H, hd), (o0, o1, 1), dtype=dtype, device=q.device), None, True
+        if k is None:
+            KH, k0, k1, k2, p0, p1, p2, fit = 0, 8, 8, 1, 8, 8, 1, fit and ko is None
+        else:
+            (k0, k1, k2), KH = k.stride(), k.shape[1]
+            if given:
+                p0, p1, p2 = ko.stride()
+                fit = fit and ko.dtype is dtype and ko.get_device() == dev and ko.shape == k.shape
+            else:
+                p0, p1, p2 = max(KH, 1) * hd, hd, 1
+                ko = _empty((T, KH, hd), (p0, p1, 1), dtype=dtype, device=q.device)
+            fit = fit and k.dtype is dtype and k.get_device() == dev and k.shape == (T, KH, hd)
+        n, = freqs.shape
+        fit = (fit and dev >= 0 and q2 == k2 == o2 == p2 == 1 and positions is not None and _vector(positions, dev, torch.int32, T)
+               and _vector(freqs, dev, torch.float64, n) and (q_norm is None or _vector(q_norm, dev, torch.float32, hd))
+               and (k_norm is None or _vector(k_norm, dev, torch.float32, hd)))
+    except _MISFITS:
         fit = False
     if not fit:
         _refuse_rotary(q, k, positions, freqs, q_norm, k_norm, out)
-    if (q.requires_grad or (k is not None and k.requires_grad) or freqs.requires_grad
-            or (q_norm is not None and q_norm.requires_grad) or (k_norm is not None and k_norm.requires_grad)
-            or (given and (qo.requires_grad or (ko is not None and ko.requires_grad)))):
+    if (q.requires_grad or (k is not None and (k.requires_grad or ko.requires_grad)) or freqs.requires_grad or qo.requires_grad
+            or (q_norm is not None and q_norm.requires_grad) or (k_norm is not None and k_norm.requires_grad)):
         _no_backward()
-    (q0, q1, _), (qo0, qo1, _) = q.stride(), qo.stride()
-    (k0, k1, _), (ko0, ko1, _) = (k.stride(), ko.stride()) if k is not None else ((8, 8, 1), (8, 8, 1))
-    _run(dev, _ROTARY, 0, _DTYPES[dtype], q.data_ptr(), _at(k), qo.data_ptr(), _at(ko), positions.data_ptr(), freqs.data_ptr(),
-         _at(q_norm), _at(k_norm), T, H, KH, hd, n, interleaved, q0, q1, k0, k1, qo0, qo1, ko0, ko1, amplitude, eps)
+    _run(dev, _ROTARY, 0, kind, q.data_ptr(), _at(k), qo.data_ptr(), _at(ko), positions.data_ptr(), freqs.data_ptr(), _at(q_norm),
+         _at(k_norm), T, H, KH, hd, n, interleaved, q0, q1, k0, k1, o0, o1, p0, p1, amplitude, eps)
     if given:
         _written(qo)
         if ko is not None:
@@ -248,21 +262,33 @@ def cache_append(k, v, k_pages, v_pages, tables, lens, cu=None, *, k_scales=None
     the scale.  Returns the rotated q, or None."""
     given = out is not None
     try:
-        dtype, dev, (T, KH, hd) = k.dtype, k.get_device(), k.shape
-        B = lens.shape[0]
-        n = 0 if freqs is None else freqs.shape[0]
-        H = 0 if q is None else q.shape[1]
-        if q is not None and not given:
-            out = _empty((T, H, hd), (H * hd, hd, 1), dtype=dtype, device=k.device)
-        fit = (dtype in _DTYPES and dev >= 0 and _fits(k, dev, dtype) and v.shape == k.shape and _fits(v, dev, dtype)
-               and _pool_fits(dev, dtype, k_pages, v_pages, tables, k_scales, v_scales, KH, hd)
-               and tables.shape[0] == B and _vector(lens, dev, torch.int32, B) and _vector(cu, dev, torch.int32, B + 1)
-               and (cu is not None or (T % B == 0 if B else T == 0)) and _vector(positions, dev, torch.int32, T)
-               and (freqs is None or (freqs.dim() == 1 and _fits(freqs, dev, torch.float64)))
-               and (out is None if q is None else
-                    q.shape == out.shape == (T, H, hd) and _fits(q, dev, dtype) and _fits(out, dev, dtype))
-               and _vector(q_norm, dev, torch.float32, hd) and _vector(k_norm, dev, torch.float32, hd))
-    except (*_NO_TENSOR, ValueError, TypeError):
+        dtype, dev, shape, (k0, k1, k2), (v0, v1, v2) = k.dtype, k.get_device(), k.shape, k.stride(), v.stride()
+        kind, (T, KH, hd) = _DTYPES[dtype], shape
+        B, = lens.shape
+        pool = _pool(dev, dtype, k_pages, v_pages, tables, k_scales, v_scales, KH, hd)
+        N, _, page, _ = k_pages.shape
+        rows, cols = tables.shape
+        fit = (pool and dev >= 0 and k2 == v2 == 1 and v.shape == shape and v.dtype is dtype and v.get_device() == dev and rows == B
+               and _vector(lens, dev, torch.int32, B)
+               and ((T % B == 0 if B else T == 0) if cu is None else _vector(cu, dev, torch.int32, B + 1)))
+        if q is None:
+            H, q0, q1, o0, o1, fit = 0, 8, 8, 8, 8, fit and out is None
+        else:
+            (q0, q1, q2), H = q.stride(), q.shape[1]
+            if given:
+                o0, o1, o2 = out.stride()
+                fit = fit and o2 == 1 and out.dtype is dtype and out.get_device() == dev and out.shape == q.shape
+            else:
+                o0, o1 = max(H, 1) * hd, hd
+                out = _empty((T, H, hd), (o0, o1, 1), dtype=dtype, device=k.device)
+            fit = fit and q2 == 1 and q.dtype is dtype and q.get_device() == dev and q.shape == (T, H, hd)
+        n = 0
+        if freqs is not None:
+            n, = freqs.shape
+            fit = fit and _vector(freqs, dev, torch.float64, n)
+        fit = (fit and (positions is None or _vector(positions, dev, torch.int32, T))
+               and (q_norm is None or _vector(q_norm, dev, torch.float32, hd)) and (k_norm is None or _vector(k_norm, dev, torch.float32, hd)))
+    except _MISFITS:
         fit = False
     if not fit:
         _refuse_append(k, v, k_pages, v_pages, tables, lens, cu, k_scales, v_scales, freqs, positions, q, q_norm, k_norm,
@@ -272,18 +298,10 @@ def cache_append(k, v, k_pages, v_pages, tables, lens, cu=None, *, k_scales=None
             or (q is not None and (q.requires_grad or out.requires_grad)) or (q_norm is not None and q_norm.requires_grad)
             or (k_norm is not None and k_norm.requires_grad)):
         _no_backward()
-    (k0, k1, _), (v0, v1, _) = k.stride(), v.stride()
-    (q0, q1, _), (o0, o1, _) = (q.stride(), out.stride()) if q is not None else ((8, 8, 1), (8, 8, 1))
-    N, _, page, _ = k_pages.shape
-    _run(dev, _APPEND, 1, _DTYPES[dtype], _bits(k_pages), _at(q), k.data_ptr(), v.data_ptr(), _at(out), k_pages.data_ptr(),
-         v_pages.data_ptr(), _at(k_scales), _at(v_scales), tables.data_ptr(), lens.data_ptr(), _at(cu), _at(positions), _at(freqs),
-         _at(q_norm), _at(k_norm), T, B, N, page, tables.shape[1], H, KH, hd, n, interleaved, q0, q1, k0, k1, v0, v1, o0, o1,
-         *_pool_strides(k_pages, v_pages, tables, k_scales, v_scales), amplitude, eps)
-    _written(k_pages)
-    _written(v_pages)
-    if k_scales is not None:
-        _written(k_scales)
-        _written(v_scales)
+    _run(dev, _APPEND, 1, kind, _bits(k_pages), _at(q), k.data_ptr(), v.data_ptr(), _at(out), k_pages.data_ptr(), v_pages.data_ptr(),
+         _at(k_scales), _at(v_scales), tables.data_ptr(), lens.data_ptr(), _at(cu), _at(positions), _at(freqs), _at(q_norm), _at(k_norm),
+         T, B, N, page, cols, H, KH, hd, n, interleaved, q0, q1, k0, k1, v0, v1, o0, o1, *pool, amplitude, eps)
+    _written((k_pages, v_pages) if k_scales is None else (k_pages, v_pages, k_scales, v_scales))
     if given:
         _written(out)
     return out
@@ -329,35 +347,38 @@ def attention_paged(q, k_pages, v_pages, tables, lens, *, k_scales=None, v_scale
     given = out is not None
     try:
         dtype, dev, shape = q.dtype, q.get_device(), q.shape
-        few = len(shape) == 4
-        B, H, hd = shape[0], shape[-2], shape[-1]
-        n = shape[1] if few else 1
-        KH = k_pages.shape[1]
-        if not given:
-            out = torch.empty(shape, dtype=dtype, device=q.device)
-        fit = (dtype in _DTYPES and dev >= 0 and (few or len(shape) == 3) and _fits(q, dev, dtype) and out.shape == shape
-               and _fits(out, dev, dtype) and _pool_fits(dev, dtype, k_pages, v_pages, tables, k_scales, v_scales, KH, hd)
-               and tables.shape[0] == B and _vector(lens, dev, torch.int32, B) and lens is not None
-               and _vector(sinks, dev, torch.float32, H))
-    except (*_NO_TENSOR, ValueError, TypeError):
+        kind = _DTYPES[dtype]
+        if len(shape) == 4:
+            (B, n, H, hd), (q0, q1, q2, q3) = shape, q.stride()
+            if not given:
+                out = _empty(shape, (max(n * H, 1) * hd, max(H, 1) * hd, hd, 1), dtype=dtype, device=q.device)
+            o0, o1, o2, o3 = out.stride()
+        else:
+            (B, H, hd), (q0, q2, q3), n, q1, o1 = shape, q.stride(), 1, 8, 8
+            if not given:
+                out = _empty(shape, (H * hd, hd, 1), dtype=dtype, device=q.device)
+            o0, o2, o3 = out.stride()
+        N, KH, page, _ = k_pages.shape
+        pool = _pool(dev, dtype, k_pages, v_pages, tables, k_scales, v_scales, KH, hd)
+        rows, cols = tables.shape
+        fit = (pool and dev >= 0 and q3 == o3 == 1 and rows == B and lens is not None and _vector(lens, dev, torch.int32, B)
+               and (not given or (out.shape == shape and out.dtype is dtype and out.get_device() == dev))
+               and (sinks is None or _vector(sinks, dev, torch.float32, H)))
+    except _MISFITS:
         fit = False
     if not fit:
         _refuse_paged(q, k_pages, v_pages, tables, lens, k_scales, v_scales, sinks, out if given else None)
     if (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad or out.requires_grad
             or (k_scales is not None and (k_scales.requires_grad or v_scales.requires_grad)) or (sinks is not None and sinks.requires_grad)):
         _no_backward()
-    N, _, page, _ = k_pages.shape
-    cols = tables.shape[1]
     most = cols * page
     max_len = most if max_len is None or max_len > most else max_len
     bits, window = _bits(k_pages), _window(window)
     nbytes = load().tg_attention_paged_workspace(bits, B, n, max_len, window, H, KH, hd) if 0 < max_len < _MOST else 0
     ws = _empty((nbytes,), (1,), dtype=torch.uint8, device=q.device) if nbytes else None
-    qs, os = q.stride(), out.stride()
-    q3, o3 = (qs[:3], os[:3]) if few else ((qs[0], 8, qs[1]), (os[0], 8, os[1]))
-    _run(dev, _ATTEND, 2, _DTYPES[dtype], bits, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _at(k_scales), _at(v_scales),
-         out.data_ptr(), tables.data_ptr(), lens.data_ptr(), _at(sinks), B, n, N, page, cols, max_len, H, KH, hd, window, *q3, *o3,
-         *_pool_strides(k_pages, v_pages, tables, k_scales, v_scales), hd ** -0.5 if scale is None else scale, _at(ws), nbytes)
+    _run(dev, _ATTEND, 2, kind, bits, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _at(k_scales), _at(v_scales),
+         out.data_ptr(), tables.data_ptr(), lens.data_ptr(), _at(sinks), B, n, N, page, cols, max_len, H, KH, hd, window, q0, q1, q2,
+         o0, o1, o2, *pool, hd ** -0.5 if scale is None else scale, _at(ws), nbytes)
     if given:
         _written(out)
     return out
@@ -385,25 +406,32 @@ def cache_gather(k_pages, v_pages, tables, cu, total, *, k_scales=None, v_scales
     sequence are not written.  out: (k, v) to write.  Returns (k, v)."""
     given = out is not None
     try:
-        kind, dev = k_pages.dtype, k_pages.get_device()
-        KH, hd = k_pages.shape[1], k_pages.shape[3]
-        dtype = (out[0].dtype if given else torch.bfloat16 if kind is _CODES else kind) if dtype is None else dtype
-        B = tables.shape[0]
-        ko, vo = out if given else (_empty((total, KH, hd), (KH * hd, hd, 1), dtype=dtype, device=k_pages.device) for _ in range(2))
-        fit = (dtype in _DTYPES and dev >= 0 and total >= 0 and ko.shape == vo.shape == (total, KH, hd) and _fits(ko, dev, dtype)
-               and _fits(vo, dev, dtype) and _pool_fits(dev, dtype, k_pages, v_pages, tables, k_scales, v_scales, KH, hd)
-               and _vector(cu, dev, torch.int32, B + 1) and cu is not None)
-    except (*_NO_TENSOR, ValueError, TypeError, RuntimeError):
+        pages, dev, (N, KH, page, hd) = k_pages.dtype, k_pages.get_device(), k_pages.shape
+        if dtype is None:
+            dtype = out[0].dtype if given else torch.bfloat16 if pages is _CODES else pages
+        kind, shape = _DTYPES[dtype], (total, KH, hd)
+        if given:
+            ko, vo = out
+            (k0, k1, k2), (v0, v1, v2) = ko.stride(), vo.stride()
+            fit = (ko.shape == vo.shape == shape and ko.dtype is vo.dtype is dtype and ko.get_device() == vo.get_device() == dev
+                   and k2 == v2 == 1)
+        else:
+            k0, k1 = v0, v1 = strides = KH * hd, hd
+            where = k_pages.device
+            ko, vo = _empty(shape, (*strides, 1), dtype=dtype, device=where), _empty(shape, (*strides, 1), dtype=dtype, device=where)
+            fit = True
+        pool = _pool(dev, dtype, k_pages, v_pages, tables, k_scales, v_scales, KH, hd)
+        B, cols = tables.shape
+        fit = fit and pool and dev >= 0 and cu is not None and _vector(cu, dev, torch.int32, B + 1)
+    except (*_MISFITS, RuntimeError):
         fit = False
     if not fit:
         _refuse_gather(k_pages, v_pages, tables, cu, total, k_scales, v_scales, dtype, out if given else None)
     if (k_pages.requires_grad or v_pages.requires_grad or ko.requires_grad or vo.requires_grad
             or (k_scales is not None and (k_scales.requires_grad or v_scales.requires_grad))):
         _no_backward()
-    (k0, k1, _), (v0, v1, _), (N, _, page, _) = ko.stride(), vo.stride(), k_pages.shape
-    _run(dev, _GATHER, 3, _DTYPES[dtype], _bits(k_pages), k_pages.data_ptr(), v_pages.data_ptr(), _at(k_scales), _at(v_scales),
-         tables.data_ptr(), cu.data_ptr(), ko.data_ptr(), vo.data_ptr(), total, B, N, page, tables.shape[1], KH, hd, k0, k1, v0, v1,
-         *_pool_strides(k_pages, v_pages, tables, k_scales, v_scales))
+    _run(dev, _GATHER, 3, kind, _bits(k_pages), k_pages.data_ptr(), v_pages.data_ptr(), _at(k_scales), _at(v_scales), tables.data_ptr(),
+         cu.data_ptr(), ko.data_ptr(), vo.data_ptr(), total, B, N, page, cols, KH, hd, k0, k1, v0, v1, *pool)
     if given:
         _written(ko)
         _written(vo)
