@@ -29,11 +29,13 @@ namespace tg {
 
 constexpr int PC_THREADS = 256;
 constexpr int PC_WARPS = PC_THREADS / 32;
+constexpr int PC_PAIRS = ATTN_MAX_HD / 2;   // pairs of a head, at most
+static_assert(PC_THREADS == 4 * PC_PAIRS, "angles of four tokens at a time");
 constexpr int PC_CU = 1024;       // sequences whose offsets are kept in shared memory
 constexpr int PC_WINDOW = 8;      // packed tokens that a CTA looks through for blocks' first ones, where sequences bring many
 constexpr int PC_TOKENS = 16;     // tokens of a CTA that rotates, at most
 constexpr int PC_GATHER = 64;     // tokens of a gather CTA, at most
-constexpr int PC_IN_FLIGHT = 3;   // rows that a thread has loaded before it works on the first
+constexpr int PC_ROWS = 3;        // rows of a token that a thread has
 
 enum { PC_ROTARY, PC_PAGES16, PC_PAGES8 };
 
@@ -49,9 +51,9 @@ struct CacheArgs {
   long long skp[3], svp[3];   // page, head, row; bytes
   long long sks[3], svs[3];   // page, head, block
   long long st;               // tables' row
-  int T, B, per, H, KH, hd, nf, n_pages, cols, shift, run_ctas, window, tokens;
+  int T, B, per, H, KH, hd, nf, n_pages, cols, shift, run_ctas, window, tokens, parts;
   int interleaved;
-  float amp, eps;
+  float amp, eps, inv_hd;   // inv_hd: 1 / hd
 };
 
 // cos and sin of p f radians, times amp, rounded once: Taylor's series at an
@@ -176,19 +178,22 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const LanePairs& m, cons
   }
 }
 
-// The norm over the LPR lanes of a row; lanes without values have zeros.  w: the
-// weights in the lanes' order.
+// The norm over the LPR lanes of a row (lanes without values have zeros), where
+// `on`; w: the weights in the lanes' order, ones where the norm is off.
 template <int LPR>
-__device__ __forceinline__ void norm_row(float (&x)[8], const float* w, int hd, float eps) {
+__device__ __forceinline__ void norm_row(float (&x)[8], const float* w, const CacheArgs& a, bool on) {
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; i++) s = fmaf(x[i], x[i], s);
 #pragma unroll
   for (int o = LPR / 2; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-  const float r = 1.f / sqrtf(s / hd + eps);
-  const float4 a = reinterpret_cast<const float4*>(w)[0], b = reinterpret_cast<const float4*>(w)[1];
-  x[0] *= r * a.x, x[1] *= r * a.y, x[2] *= r * a.z, x[3] *= r * a.w;
-  x[4] *= r * b.x, x[5] *= r * b.y, x[6] *= r * b.z, x[7] *= r * b.w;
+  s = fmaf(s, a.inv_hd, a.eps);
+  float r = rsqrtf(s);
+  r = s > 0.f && r < INFINITY ? fmaf(0.5f * r, fmaf(-s * r, r, 1.f), r) : r;   // a Newton step: half an ulp more exact
+  r = on ? r : 1.f;
+  const float4 u = reinterpret_cast<const float4*>(w)[0], v = reinterpret_cast<const float4*>(w)[1];
+  x[0] *= r * u.x, x[1] *= r * u.y, x[2] *= r * u.z, x[3] *= r * u.w;
+  x[4] *= r * v.x, x[5] *= r * v.y, x[6] *= r * v.z, x[7] *= r * v.w;
 }
 // Pairs j < nf turned; the others stay as they are, whatever their neighbours hold.
 __device__ __forceinline__ void rotate_pairs(float (&x)[8], const float2 (&cs)[4], const LanePairs& m) {
@@ -210,7 +215,7 @@ __device__ __forceinline__ const int* keep_offsets(const int* cu, int B, int* s_
 
 struct CacheShared {
   int cu[PC_CU + 1];
-  alignas(16) float w[2][ATTN_MAX_HD];                              // norms' weights of q and k, in the lanes' order; 1 where there are none
+  alignas(16) float w[3][ATTN_MAX_HD];                              // norms' weights of q and k, in the lanes' order; 1 where there are none, and for v
   alignas(16) float2 turn[PC_WINDOW + PAGED_BLOCK - 1][ATTN_MAX_HD / 2];   // cos, sin of tokens' pairs that turn
   int at[PC_WINDOW + PAGED_BLOCK - 1];                              // tokens' positions for the rotation
   int run[PC_WINDOW], len[PC_WINDOW], page[PC_TOKENS], row[PC_TOKENS];   // runs: first token, tokens; runs' or tokens' page and (first) row
@@ -221,6 +226,7 @@ __device__ __forceinline__ void keep_weights(const CacheArgs& a, CacheShared& sh
     const int j = i >> 1, d = j >= a.nf || a.interleaved ? i : i & 1 ? j + a.nf : j;
     sh.w[0][i] = a.qw ? a.qw[d] : 1.f;
     sh.w[1][i] = a.kw ? a.kw[d] : 1.f;
+    sh.w[2][i] = 1.f;
   }
 }
 __device__ __forceinline__ void load_turns(float2 (&cs)[4], const float2* turn, const LanePairs& m) {
@@ -228,30 +234,37 @@ __device__ __forceinline__ void load_turns(float2 (&cs)[4], const float2* turn, 
   cs[0] = make_float2(a.x, a.y), cs[1] = make_float2(a.z, a.w), cs[2] = make_float2(b.x, b.y), cs[3] = make_float2(b.z, b.w);
 }
 
-// The rows of nt tokens from t0 on: q, and (tg_rotary, 16-bit pages) k and v.  A
-// row is LPR lanes of 8 values; the rows of all tokens follow one another, and a
-// thread has PC_IN_FLIGHT of them loaded ahead.  A token's angles are made while
-// the one before it is turned.
+// Rows of nt tokens from t0 on: q, and (tg_rotary, 16-bit pages) k and v.  A row
+// is LPR lanes of 8 values; a thread has the same PC_ROWS rows of every token, of
+// the `part`-th share of a token's rows, and loads the next token's as it turns
+// this one's.  The angles of four tokens are made together, by all threads, while
+// the four before are turned.
 template <typename T, int LPR, bool VEC, int MODE, bool NORM>
-__device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, int t0, int nt) {
-  const int tid = threadIdx.x, g = tid / LPR;
+__device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, int t0, int nt, int part) {
+  const int tid = threadIdx.x;
   constexpr int ROWS = PC_THREADS / LPR;
   const LanePairs m(a, tid % LPR);
-  const int rows = a.H + (MODE == PC_PAGES8 ? 0 : a.KH) + (MODE == PC_PAGES16 ? a.KH : 0), passes = (rows + ROWS - 1) / ROWS;
-  Raw<VEC> raw[PC_IN_FLIGHT];
-  int ltok = 0, lpass = 0;   // the next row to load
-  auto load = [&](Raw<VEC>& to) {
-    if (ltok >= nt) return;
-    const int r = g + lpass * ROWS;
-    const long long t = t0 + ltok;
-    if (r < rows && m.any())
-      load_pairs(to, m, r < a.H          ? (const T*)a.q + t * a.sq[0] + r * a.sq[1]
-                        : r < a.H + a.KH ? (const T*)a.k + t * a.sk[0] + (r - a.H) * a.sk[1]
-                                         : (const T*)a.v + t * a.sv[0] + (r - a.H - a.KH) * a.sv[1]);
-    if (++lpass == passes) lpass = 0, ltok++;
-  };
+  const int rows = a.H + (MODE == PC_PAGES8 ? 0 : a.KH) + (MODE == PC_PAGES16 ? a.KH : 0);
+  const int first = part * PC_ROWS * ROWS + tid / LPR;   // its rows: first, first + ROWS, ..
+  const T* from[PC_ROWS];
+  T* to[PC_ROWS];   // q, tg_rotary's k; the head's place in a page
+  Raw<VEC> raw[PC_ROWS];
 #pragma unroll
-  for (int i = 0; i < PC_IN_FLIGHT; i++) load(raw[i]);
+  for (int i = 0; i < PC_ROWS; i++) {
+    const int r = first + i * ROWS;
+    const long long t = t0;
+    if (r < a.H) {
+      from[i] = (const T*)a.q + t * a.sq[0] + r * a.sq[1];
+      to[i] = (T*)a.qo + t * a.sqo[0] + r * a.sqo[1];
+    } else if (r < a.H + a.KH) {
+      from[i] = (const T*)a.k + t * a.sk[0] + (r - a.H) * a.sk[1];
+      to[i] = MODE == PC_ROTARY ? (T*)a.ko + t * a.sko[0] + (r - a.H) * a.sko[1] : (T*)(a.kp + (r - a.H) * a.skp[1]);
+    } else {
+      from[i] = (const T*)a.v + t * a.sv[0] + (r - a.H - a.KH) * a.sv[1];
+      to[i] = (T*)(a.vp + (r - a.H - a.KH) * a.svp[1]);
+    }
+    if (r < rows && m.any()) load_pairs(raw[i], m, from[i]);
+  }
   const int* cu = MODE == PC_ROTARY ? nullptr : keep_offsets(a.cu, a.B, sh.cu);
   if (NORM) keep_weights(a, sh);
   if (MODE != PC_ROTARY) __syncthreads();
@@ -271,64 +284,56 @@ __device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, 
     }
     sh.at[tid] = pos, sh.page[tid] = page, sh.row[tid] = row;
   }
-  auto angles = [&](int i) {
-    for (int j = tid; j < a.nf; j += PC_THREADS) sh.turn[i & 1][j] = rope_angle(sh.at[i], a.freqs[j], a.amp);
+  const int pair = tid % PC_PAIRS, quarter = tid / PC_PAIRS;
+  auto angles = [&](int t) {   // of four tokens from t on
+    if (t + quarter < nt && pair < a.nf) sh.turn[(t & 4) + quarter][pair] = rope_angle(sh.at[t + quarter], a.freqs[pair], a.amp);
   };
   __syncthreads();
   angles(0);
-  int tok = 0, pass = 0;
-  for (int k0 = 0; k0 < nt * passes; k0 += PC_IN_FLIGHT) {
+#pragma unroll 1
+  for (int t = 0; t < nt; t++) {
+    if (t % 4 == 0) {
+      __syncthreads();
+      angles(t + 4);
+    }
+    float2 cs[4];
+    load_turns(cs, sh.turn[t & 7], m);
+    const int page = MODE == PC_ROTARY ? -1 : sh.page[t];
 #pragma unroll
-    for (int i = 0; i < PC_IN_FLIGHT; i++) {
-      if (tok >= nt) break;   // the same for the whole CTA
-      if (pass == 0) {
-        __syncthreads();
-        if (tok + 1 < nt) angles(tok + 1);
-      }
-      const int r = g + pass * ROWS, page = MODE == PC_ROTARY ? -1 : sh.page[tok];
-      const long long t = t0 + tok;
-      const bool is_q = r < a.H, is_v = r >= a.H + a.KH;
+    for (int i = 0; i < PC_ROWS; i++) {
+      const int r = first + i * ROWS;
+      const bool is_q = r < a.H, is_v = r >= a.H + a.KH, here = r < rows && m.any();
       float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (r < rows && m.any()) unpack_pairs<T>(x, raw[i], m);
-      if (NORM) {   // lanes of rows that have none take part in the sums
-        float y[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) y[e] = x[e];
-        norm_row<LPR>(y, sh.w[!is_q] + (m.any() ? 8 * m.c : 0), a.hd, a.eps);
-        if (is_q ? a.qw != nullptr : !is_v && a.kw)
-#pragma unroll
-          for (int e = 0; e < 8; e++) x[e] = y[e];
+      if (here) {
+        unpack_pairs<T>(x, raw[i], m);
+        from[i] += is_q ? a.sq[0] : is_v ? a.sv[0] : a.sk[0];
+        if (t + 1 < nt) load_pairs(raw[i], m, from[i]);
       }
-      if (r < rows && m.any() && page != -2) {
-        if (!is_v) {
-          float2 cs[4];
-          load_turns(cs, sh.turn[tok & 1], m);
-          rotate_pairs(x, cs, m);
+      if (NORM)   // lanes of rows that have none take part in the sums
+        norm_row<LPR>(x, sh.w[is_q ? 0 : is_v ? 2 : 1] + (m.any() ? 8 * m.c : 0), a, is_q ? a.qw != nullptr : !is_v && a.kw);
+      if (here) {
+        if (MODE != PC_PAGES16 || !is_v) rotate_pairs(x, cs, m);
+        if (MODE != PC_PAGES16 || is_q) {
+          if (page != -2) store_pairs<T, VEC>(to[i], m, x);
+          to[i] += is_q ? a.sqo[0] : a.sko[0];
+        } else if (page >= 0) {
+          const long long at = is_v ? page * a.svp[0] + sh.row[t] * a.svp[2] : page * a.skp[0] + sh.row[t] * a.skp[2];
+          store_pairs<T, VEC>((uint8_t*)to[i] + at, m, x);
         }
-        T* to = nullptr;
-        if (is_q)
-          to = (T*)a.qo + t * a.sqo[0] + r * a.sqo[1];
-        else if (MODE == PC_ROTARY)
-          to = (T*)a.ko + t * a.sko[0] + (r - a.H) * a.sko[1];
-        else if (page >= 0)
-          to = is_v ? (T*)(a.vp + page * a.svp[0] + (r - a.H - a.KH) * a.svp[1] + sh.row[tok] * a.svp[2])
-                    : (T*)(a.kp + page * a.skp[0] + (r - a.H) * a.skp[1] + sh.row[tok] * a.skp[2]);
-        if (to) store_pairs<T, VEC>(to, m, x);
       }
-      load(raw[i]);
-      if (++pass == passes) pass = 0, tok++;
     }
   }
 }
 
 // Runs of 8-bit blocks whose first token is one of the `window` packed tokens
 // from t0 on: a warp has one run's keys or values of a key head.  Its values are
-// worked out twice, for the largest and for the codes: kept in fp32 they would
-// take 64 registers of a thread, and the warps of a CTA half as many an SM.
+// read (the second time from the L1 cache) and worked out twice, for the largest
+// and for the codes: kept in registers they leave room for one CTA of an SM
+// instead of four (8,192 tokens with q 171 us).
 template <typename T, int LPR, bool VEC, bool NORM>
 __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& sh, int t0) {
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-  constexpr int RPP = 32 / LPR, PASSES = PAGED_BLOCK / RPP;
+  constexpr int RPP = 32 / LPR;   // rows of a warp at a time
   const int* cu = keep_offsets(a.cu, a.B, sh.cu);
   if (NORM) keep_weights(a, sh);
   __syncthreads();
@@ -356,18 +361,10 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
   if (!sh.runs) return;
   const LanePairs m(a, lane % LPR);
   const int items = sh.runs * 2 * a.KH;
-  Raw<VEC> raw[PASSES];
-  auto load = [&](int item) {
-    const int i = item / (2 * a.KH), kh = item % (2 * a.KH) >> 1, j0 = sh.run[i];
-    const T* from = item & 1 ? (const T*)a.v + (long long)(t0 + j0) * a.sv[0] + kh * a.sv[1] : (const T*)a.k + (long long)(t0 + j0) * a.sk[0] + kh * a.sk[1];
-#pragma unroll
-    for (int u = 0; u < PASSES; u++) {
-      const int j = u * RPP + lane / LPR;
-      if (j < sh.len[i] && m.any()) load_pairs(raw[u], m, from + j * (item & 1 ? a.sv[0] : a.sk[0]));
-    }
-  };
-  if (wid < items) load(wid);
-  for (int i = tid; i < sh.cover * a.nf; i += PC_THREADS) sh.turn[i / a.nf][i % a.nf] = rope_angle(sh.at[i / a.nf], a.freqs[i % a.nf], a.amp);
+  if (tid % PC_PAIRS < a.nf) {
+    const double f = a.freqs[tid % PC_PAIRS];
+    for (int j = tid / PC_PAIRS; j < sh.cover; j += PC_THREADS / PC_PAIRS) sh.turn[j][tid % PC_PAIRS] = rope_angle(sh.at[j], f, a.amp);
+  }
   __syncthreads();
   for (int item = wid; item < items; item += PC_WARPS) {
     const int i = item / (2 * a.KH), kh = item % (2 * a.KH) >> 1, is_v = item & 1;
@@ -378,29 +375,38 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
     float* scale_at = is_v ? a.vs + sh.page[i] * a.svs[0] + kh * a.svs[1] + block * a.svs[2]
                            : a.ks + sh.page[i] * a.sks[0] + kh * a.sks[1] + block * a.sks[2];
     const float before = off ? *scale_at : 0.f;
-    auto values = [&](int u, float (&x)[8]) {   // of row u RPP + lane / LPR; zeros where there is none
-      const int j = u * RPP + lane / LPR;
+    const long long step = is_v ? a.sv[0] : a.sk[0];
+    const T* from = (is_v ? (const T*)a.v + kh * a.sv[1] : (const T*)a.k + kh * a.sk[1]) + (t0 + j0 + lane / LPR) * step;
+    auto values = [&](int j, const Raw<VEC>& raw, float (&x)[8]) {   // of row j; zeros where there is none
+      const bool here = j < n && m.any();
 #pragma unroll
       for (int e = 0; e < 8; e++) x[e] = 0.f;
-      if (j < n && m.any()) unpack_pairs<T>(x, raw[u], m);
+      if (here) unpack_pairs<T>(x, raw, m);
       if (is_v) return;
-      if (NORM && a.kw) norm_row<LPR>(x, sh.w[1] + (m.any() ? 8 * m.c : 0), a.hd, a.eps);
-      if (j < n && m.any()) {
+      if (NORM) norm_row<LPR>(x, sh.w[1] + (m.any() ? 8 * m.c : 0), a, a.kw != nullptr);
+      if (here) {
         float2 cs[4];
         load_turns(cs, sh.turn[j0 + j], m);
         rotate_pairs(x, cs, m);
       }
     };
     uint32_t amax = 0;   // bits of the largest finite magnitude
+#pragma unroll 1
+    for (int u = 0; u * RPP < n; u += 4) {
+      Raw<VEC> raw[4];
 #pragma unroll
-    for (int u = 0; u < PASSES; u++) {
-      if (u * RPP >= n) break;
-      float x[8];
-      values(u, x);
+      for (int i4 = 0; i4 < 4; i4++)
+        if ((u + i4) * RPP + lane / LPR < n && m.any()) load_pairs(raw[i4], m, from + (u + i4) * RPP * step);
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const uint32_t y = __float_as_uint(x[e]) & 0x7fffffffu;
-        amax = max(amax, y < 0x7f800000u ? y : 0u);
+      for (int i4 = 0; i4 < 4; i4++) {
+        if ((u + i4) * RPP >= n) break;
+        float x[8];
+        values((u + i4) * RPP + lane / LPR, raw[i4], x);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const uint32_t y = __float_as_uint(x[e]) & 0x7fffffffu;
+          amax = max(amax, y < 0x7f800000u ? y : 0u);
+        }
       }
     }
     amax = __reduce_max_sync(~0u, amax);
@@ -418,12 +424,13 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
         *at = make_uint2(four(w.x), four(w.y));
       }
     }
-#pragma unroll
-    for (int u = 0; u < PASSES; u++) {
-      if (u * RPP >= n) break;
+#pragma unroll 2
+    for (int u = 0; u * RPP < n; u++) {
       const int j = u * RPP + lane / LPR;
+      Raw<VEC> raw;
+      if (j < n && m.any()) load_pairs(raw, m, from + u * RPP * step);
       float x[8];
-      values(u, x);
+      values(j, raw, x);
       if (j < n && m.any()) {
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] *= inv;
@@ -431,19 +438,18 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
       }
     }
     if (lane == 0) *scale_at = scale;
-    if (item + PC_WARPS < items) load(item + PC_WARPS);
   }
 }
 
 template <typename T, int LPR, bool VEC, int MODE, bool NORM>
-__global__ void __launch_bounds__(PC_THREADS, MODE == PC_PAGES8 ? 3 : 4) cache_kernel(const CacheArgs a) {
+__global__ void __launch_bounds__(PC_THREADS, 4) cache_kernel(const CacheArgs a) {
   __shared__ CacheShared sh;
   pdl_wait();
   if (MODE == PC_PAGES8 && blockIdx.x < a.run_ctas)
     runs_of_blocks<T, LPR, VEC, NORM>(a, sh, blockIdx.x * a.window);
   else {
-    const int t0 = (blockIdx.x - (MODE == PC_PAGES8 ? a.run_ctas : 0)) * a.tokens;
-    token_rows<T, LPR, VEC, MODE, NORM>(a, sh, t0, min(a.tokens, a.T - t0));
+    const int i = blockIdx.x - (MODE == PC_PAGES8 ? a.run_ctas : 0), t0 = i / a.parts * a.tokens;
+    token_rows<T, LPR, VEC, MODE, NORM>(a, sh, t0, min(a.tokens, a.T - t0), i % a.parts);
   }
 }
 
@@ -541,19 +547,21 @@ using namespace tg;
 
 namespace tg {
 
-// Tokens of a CTA, so that all CTAs are there at once where PC_TOKENS allow it; the CTAs.
-static int token_ctas(CacheArgs& a, int per_sm) {
-  const int most = attn_sms() * per_sm;
-  a.tokens = std::min(PC_TOKENS, (a.T + most - 1) / most);
-  return (a.T + a.tokens - 1) / a.tokens;
+// The CTAs that rotate: shares of `rows` rows of a token, and tokens of a CTA so
+// that all of them are there at once where PC_TOKENS allow it.
+static long long token_ctas(CacheArgs& a, long long rows, int per_sm) {
+  const int share = PC_ROWS * PC_THREADS / (a.hd <= 64 ? 8 : 16), most = attn_sms() * per_sm;
+  a.parts = (int)((rows + share - 1) / share);
+  a.tokens = (int)std::min((long long)PC_TOKENS, ((long long)a.T * a.parts + most - 1) / most);
+  return (long long)((a.T + a.tokens - 1) / a.tokens) * a.parts;
 }
 
 static int rotary(ArgCheck& c, const RotaryRecord& r) {
   const int64_t* strides = r.strides;
   c.need(r.dtype == ATTN_BF16 || r.dtype == ATTN_FP16, "dtype must be 0 (bf16) or 1 (fp16)");
   need_ints(c, &r.n_tokens, 6);
-  c.need(r.n_tokens >= 0 && r.n_heads >= 0 && r.n_kv_heads >= 0, "counts must not be negative");
-  c.need(r.n_heads < 1 << 24 && r.n_kv_heads < 1 << 24, "too many heads");
+  c.need(r.n_tokens >= 0 && r.n_tokens < 1 << 30 && r.n_heads >= 0 && r.n_kv_heads >= 0, "counts must not be negative, and tokens below 2^30");
+  c.need(r.n_heads < 1 << 16 && r.n_kv_heads < 1 << 16, "too many heads");
   c.need(r.head_dim > 0 && r.head_dim % 8 == 0 && r.head_dim <= ATTN_MAX_HD, "head_dim must be a multiple of 8, at most 128");
   c.need(r.n_freqs >= 0 && 2 * r.n_freqs <= r.head_dim, "at most head_dim / 2 frequencies");
   c.need(std::isfinite((float)r.amplitude), "amplitude must be finite");
@@ -575,17 +583,18 @@ static int rotary(ArgCheck& c, const RotaryRecord& r) {
   a.qw = (const float*)r.q_norm, a.kw = (const float*)r.k_norm;
   for (int i = 0; i < 2; i++) a.sq[i] = t[i], a.sk[i] = t[2 + i], a.sqo[i] = t[4 + i], a.sko[i] = t[6 + i];
   a.T = (int)r.n_tokens, a.H = (int)r.n_heads, a.KH = (int)r.n_kv_heads, a.hd = (int)r.head_dim, a.nf = (int)r.n_freqs;
-  a.interleaved = r.interleaved != 0, a.amp = (float)r.amplitude, a.eps = (float)r.eps;
+  a.interleaved = r.interleaved != 0, a.amp = (float)r.amplitude, a.eps = (float)r.eps, a.inv_hd = 1.f / a.hd;
   cudaStream_t s = static_cast<cudaStream_t>(r.stream);
-  const int grid = token_ctas(a, 4);
-  return c.done(r.dtype == ATTN_BF16 ? launch_cache<__nv_bfloat16, PC_ROTARY>(a, grid, s) : launch_cache<__half, PC_ROTARY>(a, grid, s));
+  const long long grid = token_ctas(a, (long long)a.H + a.KH, 4);
+  if (!c.need(grid < 1ll << 31, "too many rows")) return c.rc;
+  return c.done(r.dtype == ATTN_BF16 ? launch_cache<__nv_bfloat16, PC_ROTARY>(a, (int)grid, s) : launch_cache<__half, PC_ROTARY>(a, (int)grid, s));
 }
 
 static int append(ArgCheck& c, const AppendRecord& r) {
   c.need(r.dtype == ATTN_BF16 || r.dtype == ATTN_FP16, "dtype must be 0 (bf16) or 1 (fp16)");
   need_ints(c, &r.n_tokens, 10);
   c.need(r.n_tokens >= 0 && r.batch >= 0 && r.n_heads >= 0 && r.n_kv_heads > 0, "n_kv_heads must be positive, the other counts not negative");
-  c.need(r.n_heads < 1 << 24 && r.n_kv_heads < 1 << 24, "too many heads");
+  c.need(r.n_heads < 1 << 16 && r.n_kv_heads < 1 << 16, "too many heads");
   c.need(r.head_dim > 0 && r.head_dim % 8 == 0 && r.head_dim <= ATTN_MAX_HD, "head_dim must be a multiple of 8, at most 128");
   c.need(r.n_freqs >= 0 && 2 * r.n_freqs <= r.head_dim, "at most head_dim / 2 frequencies");
   c.need(std::isfinite((float)r.amplitude), "amplitude must be finite");
@@ -621,13 +630,15 @@ static int append(ArgCheck& c, const AppendRecord& r) {
   a.st = pool.st;
   a.T = (int)r.n_tokens, a.B = (int)r.batch, a.per = a.T / a.B, a.H = (int)r.n_heads, a.KH = (int)r.n_kv_heads, a.hd = (int)r.head_dim;
   a.nf = (int)r.n_freqs, a.n_pages = (int)r.n_pages, a.cols = (int)r.table_cols, a.shift = pool.shift;
-  a.interleaved = r.interleaved != 0, a.amp = (float)r.amplitude, a.eps = (float)r.eps;
-  int grid = token_ctas(a, r.page_bits == 8 ? 3 : 4);
+  a.interleaved = r.interleaved != 0, a.amp = (float)r.amplitude, a.eps = (float)r.eps, a.inv_hd = 1.f / a.hd;
+  long long ctas = r.page_bits == 16 ? token_ctas(a, (long long)a.H + 2 * a.KH, 4) : a.H ? token_ctas(a, a.H, 4) : 0;
   if (r.page_bits == 8) {
     a.window = a.T / a.B >= PC_WINDOW ? PC_WINDOW : 1;
     a.run_ctas = (a.T + a.window - 1) / a.window;
-    grid = a.run_ctas + (a.H ? grid : 0);
+    ctas += a.run_ctas;
   }
+  if (!c.need(ctas < 1ll << 31, "too many rows")) return c.rc;
+  const int grid = (int)ctas;
   cudaStream_t s = static_cast<cudaStream_t>(r.stream);
   const bool bf = r.dtype == ATTN_BF16;
   if (r.page_bits == 16)
