@@ -18,7 +18,6 @@
 // scale grows when a larger token comes keeps its earlier codes' bits (but for
 // those that fall below the format's least normal value).
 #include <algorithm>
-#include <cfloat>
 #include <cmath>
 
 #include "../../include/tinygiant.h"
@@ -29,13 +28,17 @@ namespace tg {
 
 constexpr int PC_THREADS = 256;
 constexpr int PC_WARPS = PC_THREADS / 32;
+constexpr int PC_PER_SM = 3;      // CTAs of an SM (4 leave 64 registers, and norms spill: 8,192 tokens x 32 heads rotated in 25 us instead of 22, with norms 37 instead of 33)
 constexpr int PC_PAIRS = ATTN_MAX_HD / 2;   // pairs of a head, at most
 static_assert(PC_THREADS == 4 * PC_PAIRS, "angles of four tokens at a time");
 constexpr int PC_CU = 1024;       // sequences whose offsets are kept in shared memory
-constexpr int PC_WINDOW = 8;      // packed tokens that a CTA looks through for blocks' first ones, where sequences bring many
-constexpr int PC_TOKENS = 16;     // tokens of a CTA that rotates, at most
+constexpr int PC_WINDOW = 16;     // packed tokens that a CTA looks through for blocks' first ones, at most
+constexpr int PC_TOKENS = 32;     // tokens of a CTA that rotates, at most
 constexpr int PC_GATHER = 64;     // tokens of a gather CTA, at most
 constexpr int PC_ROWS = 3;        // rows of a token that a thread has
+constexpr int PC_AHEAD = 3;       // tokens whose rows are there or on their way
+constexpr int PC_RING = PC_AHEAD * PC_ROWS * 2 * 8 * PC_THREADS;
+static_assert(PC_RING >= PAGED_BLOCK * ATTN_MAX_HD * 2 * PC_WARPS, "a warp's run of a head");
 
 enum { PC_ROTARY, PC_PAGES16, PC_PAGES8 };
 
@@ -51,7 +54,7 @@ struct CacheArgs {
   long long skp[3], svp[3];   // page, head, row; bytes
   long long sks[3], svs[3];   // page, head, block
   long long st;               // tables' row
-  int T, B, per, H, KH, hd, nf, n_pages, cols, shift, run_ctas, window, tokens, parts;
+  int T, B, per, H, KH, hd, nf, n_pages, cols, shift, token_ctas, window, tokens, parts;
   int interleaved;
   float amp, eps, inv_hd;   // inv_hd: 1 / hd
 };
@@ -68,24 +71,30 @@ __device__ __forceinline__ float2 rope_angle(int p, double f, float amp) {
   return quarter & 2 ? make_float2(-cs, -sn) : make_float2(cs, sn);
 }
 
-// Eight values of a row as four pairs (x[2 i], x[2 i + 1]), the lane's pairs
-// 4 c .. 4 c + 3 of the row's hd / 2: pair j < nf is (j, j + nf), or neighbours if
-// interleaved; pairs behind those are neighbours.  VEC: nf is a multiple of 4
-// or pairs are neighbours, so that four values of a row lie together.
+// Eight values of a row are a lane's: the pairs 4 c .. 4 c + 3 of the row's hd / 2.
+// Pair j < nf is the dimensions (j, j + nf), or neighbours if interleaved; pairs
+// behind those are neighbours and do not turn.  VEC: nf is a multiple of 4, so a
+// lane's pairs turn all or none and four values lie together.
 struct LanePairs {
   int c, hd, nf;
   bool split;   // (j, j + nf)
   __device__ LanePairs(const CacheArgs& a, int lane_of_row) : c(lane_of_row), hd(a.hd), nf(a.nf), split(!a.interleaved && 4 * lane_of_row < a.nf) {}
   __device__ bool any() const { return 8 * c < hd; }
-  __device__ int low(int i) const {
-    const int j = 4 * c + i;
-    return split && j < nf ? j : 2 * j;
-  }
-  __device__ int high(int i) const {
-    const int j = 4 * c + i;
-    return split && j < nf ? j + nf : 2 * j + 1;
-  }
+  __device__ bool turns(int i) const { return 4 * c + i < nf; }
+  __device__ int low(int i) const { return split && turns(i) ? 4 * c + i : 8 * c + 2 * i; }
+  __device__ int high(int i) const { return split && turns(i) ? 4 * c + i + nf : 8 * c + 2 * i + 1; }
 };
+// The pairs' first and second values, for the FMA units' two at a time.
+struct Pairs {
+  float2 a[2], b[2];
+};
+__device__ __forceinline__ float2 pc_mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
 template <bool VEC>
 struct Raw {
   uint32_t w[4];
@@ -103,50 +112,45 @@ __device__ __forceinline__ void load_pairs(Raw<VEC>& r, const LanePairs& m, cons
   }
 }
 template <typename T>
-__device__ __forceinline__ float half_of(uint32_t w, int i) {
-  const uint16_t h = i ? w >> 16 : w & 0xffffu;
-  return to_f32<T>(*reinterpret_cast<const T*>(&h));
+__device__ __forceinline__ float2 halves(uint32_t w) {
+  const uint16_t lo = w & 0xffffu, hi = w >> 16;
+  return make_float2(to_f32<T>(*reinterpret_cast<const T*>(&lo)), to_f32<T>(*reinterpret_cast<const T*>(&hi)));
 }
 template <typename T, bool VEC>
-__device__ __forceinline__ void unpack_pairs(float (&x)[8], const Raw<VEC>& r, const LanePairs& m) {
-#pragma unroll
-  for (int i = 0; i < 4; i++)
-    if (VEC && m.split) {
-      x[2 * i] = half_of<T>(r.w[i / 2], i & 1);
-      x[2 * i + 1] = half_of<T>(r.w[2 + i / 2], i & 1);
-    } else {
-      x[2 * i] = half_of<T>(r.w[i], 0);
-      x[2 * i + 1] = half_of<T>(r.w[i], 1);
-    }
-}
-template <typename T, bool VEC>
-__device__ __forceinline__ void store_pairs(void* row, const LanePairs& m, const float (&x)[8]) {
-  uint16_t* p = static_cast<uint16_t*>(row);
-  if (VEC) {
-    uint2 lo, hi;
-    if (m.split) {
-      lo = make_uint2(at_pack<T>(x[0], x[2]), at_pack<T>(x[4], x[6]));
-      hi = make_uint2(at_pack<T>(x[1], x[3]), at_pack<T>(x[5], x[7]));
-    } else {
-      lo = make_uint2(at_pack<T>(x[0], x[1]), at_pack<T>(x[2], x[3]));
-      hi = make_uint2(at_pack<T>(x[4], x[5]), at_pack<T>(x[6], x[7]));
-    }
-    *reinterpret_cast<uint2*>(p + (m.split ? 4 * m.c : 8 * m.c)) = lo;
-    *reinterpret_cast<uint2*>(p + (m.split ? m.nf + 4 * m.c : 8 * m.c + 4)) = hi;
+__device__ __forceinline__ void unpack_pairs(Pairs& x, const Raw<VEC>& r, const LanePairs& m) {
+  const float2 y[4] = {halves<T>(r.w[0]), halves<T>(r.w[1]), halves<T>(r.w[2]), halves<T>(r.w[3])};
+  if (VEC && m.split) {
+    x.a[0] = y[0], x.a[1] = y[1], x.b[0] = y[2], x.b[1] = y[3];
   } else {
+    x.a[0] = make_float2(y[0].x, y[1].x), x.b[0] = make_float2(y[0].y, y[1].y);
+    x.a[1] = make_float2(y[2].x, y[3].x), x.b[1] = make_float2(y[2].y, y[3].y);
+  }
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_pairs(void* row, const LanePairs& m, const Pairs& x) {
+  uint16_t* p = static_cast<uint16_t*>(row);
+  if (VEC && m.split) {
+    *reinterpret_cast<uint2*>(p + 4 * m.c) = make_uint2(at_pack<T>(x.a[0].x, x.a[0].y), at_pack<T>(x.a[1].x, x.a[1].y));
+    *reinterpret_cast<uint2*>(p + m.nf + 4 * m.c) = make_uint2(at_pack<T>(x.b[0].x, x.b[0].y), at_pack<T>(x.b[1].x, x.b[1].y));
+  } else {
+    const uint32_t w[4] = {at_pack<T>(x.a[0].x, x.b[0].x), at_pack<T>(x.a[0].y, x.b[0].y), at_pack<T>(x.a[1].x, x.b[1].x), at_pack<T>(x.a[1].y, x.b[1].y)};
+    if (VEC) {
+      *reinterpret_cast<uint2*>(p + 8 * m.c) = make_uint2(w[0], w[1]);
+      *reinterpret_cast<uint2*>(p + 8 * m.c + 4) = make_uint2(w[2], w[3]);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const uint32_t w = at_pack<T>(x[2 * i], x[2 * i + 1]);
-      p[m.low(i)] = (uint16_t)w;
-      p[m.high(i)] = (uint16_t)(w >> 16);
+      for (int i = 0; i < 4; i++) {
+        p[m.low(i)] = (uint16_t)w[i];
+        p[m.high(i)] = (uint16_t)(w[i] >> 16);
+      }
     }
   }
 }
 // e4m3 codes of a pair, the first in the low byte; NaN where a value is not finite.
 __device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
   uint16_t d;
-  lo = fabsf(lo) <= FLT_MAX ? lo : NAN;
-  hi = fabsf(hi) <= FLT_MAX ? hi : NAN;
+  lo = lo - lo == 0.f ? lo : NAN;
+  hi = hi - hi == 0.f ? hi : NAN;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(hi), "f"(lo));
   return d;
 }
@@ -156,24 +160,22 @@ __device__ __forceinline__ float2 e4m3_values(uint32_t two) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 template <bool VEC>
-__device__ __forceinline__ void store_codes(uint8_t* p, const LanePairs& m, const float (&x)[8]) {
-  uint32_t lo, hi;
+__device__ __forceinline__ void store_codes(uint8_t* p, const LanePairs& m, const Pairs& x) {
   if (VEC && m.split) {
-    lo = e4m3_pair(x[0], x[2]) | e4m3_pair(x[4], x[6]) << 16;
-    hi = e4m3_pair(x[1], x[3]) | e4m3_pair(x[5], x[7]) << 16;
+    *reinterpret_cast<uint32_t*>(p + 4 * m.c) = e4m3_pair(x.a[0].x, x.a[0].y) | e4m3_pair(x.a[1].x, x.a[1].y) << 16;
+    *reinterpret_cast<uint32_t*>(p + m.nf + 4 * m.c) = e4m3_pair(x.b[0].x, x.b[0].y) | e4m3_pair(x.b[1].x, x.b[1].y) << 16;
   } else {
-    lo = e4m3_pair(x[0], x[1]) | e4m3_pair(x[2], x[3]) << 16;
-    hi = e4m3_pair(x[4], x[5]) | e4m3_pair(x[6], x[7]) << 16;
-  }
-  if (VEC) {
-    *reinterpret_cast<uint32_t*>(p + (m.split ? 4 * m.c : 8 * m.c)) = lo;
-    *reinterpret_cast<uint32_t*>(p + (m.split ? m.nf + 4 * m.c : 8 * m.c + 4)) = hi;
-  } else {
+    const uint32_t w[2] = {e4m3_pair(x.a[0].x, x.b[0].x) | e4m3_pair(x.a[0].y, x.b[0].y) << 16,
+                           e4m3_pair(x.a[1].x, x.b[1].x) | e4m3_pair(x.a[1].y, x.b[1].y) << 16};
+    if (VEC) {
+      *reinterpret_cast<uint2*>(p + 8 * m.c) = make_uint2(w[0], w[1]);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const uint32_t two = (i < 2 ? lo : hi) >> 16 * (i & 1);
-      p[m.low(i)] = (uint8_t)two;
-      p[m.high(i)] = (uint8_t)(two >> 8);
+      for (int i = 0; i < 4; i++) {
+        const uint32_t two = w[i / 2] >> 16 * (i & 1);
+        p[m.low(i)] = (uint8_t)two;
+        p[m.high(i)] = (uint8_t)(two >> 8);
+      }
     }
   }
 }
@@ -181,29 +183,53 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const LanePairs& m, cons
 // The norm over the LPR lanes of a row (lanes without values have zeros), where
 // `on`; w: the weights in the lanes' order, ones where the norm is off.
 template <int LPR>
-__device__ __forceinline__ void norm_row(float (&x)[8], const float* w, const CacheArgs& a, bool on) {
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; i++) s = fmaf(x[i], x[i], s);
+__device__ __forceinline__ void norm_row(Pairs& x, const float* w, const CacheArgs& a, bool on) {
+  float2 q = pc_mul2(x.a[0], x.a[0]);
+  q = at_fma2(x.a[1], x.a[1], q);
+  q = at_fma2(x.b[0], x.b[0], q);
+  q = at_fma2(x.b[1], x.b[1], q);
+  float s = q.x + q.y;
 #pragma unroll
   for (int o = LPR / 2; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
   s = fmaf(s, a.inv_hd, a.eps);
   float r = rsqrtf(s);
   r = s > 0.f && r < INFINITY ? fmaf(0.5f * r, fmaf(-s * r, r, 1.f), r) : r;   // a Newton step: half an ulp more exact
   r = on ? r : 1.f;
+  const float2 rr = make_float2(r, r);
   const float4 u = reinterpret_cast<const float4*>(w)[0], v = reinterpret_cast<const float4*>(w)[1];
-  x[0] *= r * u.x, x[1] *= r * u.y, x[2] *= r * u.z, x[3] *= r * u.w;
-  x[4] *= r * v.x, x[5] *= r * v.y, x[6] *= r * v.z, x[7] *= r * v.w;
+  x.a[0] = pc_mul2(x.a[0], pc_mul2(rr, make_float2(u.x, u.y)));
+  x.a[1] = pc_mul2(x.a[1], pc_mul2(rr, make_float2(u.z, u.w)));
+  x.b[0] = pc_mul2(x.b[0], pc_mul2(rr, make_float2(v.x, v.y)));
+  x.b[1] = pc_mul2(x.b[1], pc_mul2(rr, make_float2(v.z, v.w)));
 }
-// Pairs j < nf turned; the others stay as they are, whatever their neighbours hold.
-__device__ __forceinline__ void rotate_pairs(float (&x)[8], const float2 (&cs)[4], const LanePairs& m) {
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    if (4 * m.c + i >= m.nf) continue;
-    const float a = x[2 * i], b = x[2 * i + 1];
-    x[2 * i] = fmaf(a, cs[i].x, -(b * cs[i].y));
-    x[2 * i + 1] = fmaf(b, cs[i].x, a * cs[i].y);
+// cos and sin of a lane's four pairs.
+struct Turns {
+  float2 c[2], s[2];
+  __device__ __forceinline__ Turns(const float (*turn)[PC_PAIRS], const LanePairs& m) {
+    const float4 u = *reinterpret_cast<const float4*>(&turn[0][4 * m.c]), v = *reinterpret_cast<const float4*>(&turn[1][4 * m.c]);
+    c[0] = make_float2(u.x, u.y), c[1] = make_float2(u.z, u.w), s[0] = make_float2(v.x, v.y), s[1] = make_float2(v.z, v.w);
   }
+};
+// Pairs j < nf turned; the others stay as they are, whatever their neighbours hold.
+template <bool VEC>
+__device__ __forceinline__ void rotate_pairs(Pairs& x, const Turns& t, const LanePairs& m) {
+  if (VEC && !m.turns(0)) return;
+  const Pairs y = x;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    x.a[i] = at_fma2(y.a[i], t.c[i], pc_mul2(y.b[i], make_float2(-t.s[i].x, -t.s[i].y)));
+    x.b[i] = at_fma2(y.b[i], t.c[i], pc_mul2(y.a[i], t.s[i]));
+  }
+  if (!VEC) {
+    if (!m.turns(0)) x.a[0].x = y.a[0].x, x.b[0].x = y.b[0].x;
+    if (!m.turns(1)) x.a[0].y = y.a[0].y, x.b[0].y = y.b[0].y;
+    if (!m.turns(2)) x.a[1].x = y.a[1].x, x.b[1].x = y.b[1].x;
+    if (!m.turns(3)) x.a[1].y = y.a[1].y, x.b[1].y = y.b[1].y;
+  }
+}
+__device__ __forceinline__ Pairs no_pairs() {
+  const float2 z = make_float2(0.f, 0.f);
+  return Pairs{{z, z}, {z, z}};
 }
 
 // Offsets of the sequences, in shared memory where they fit.
@@ -213,32 +239,38 @@ __device__ __forceinline__ const int* keep_offsets(const int* cu, int B, int* s_
   return s_cu;
 }
 
+__device__ __forceinline__ void cp8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+static_assert(PC_TOKENS >= PC_WINDOW + PAGED_BLOCK - 1, "both kinds of CTAs' tokens");
 struct CacheShared {
   int cu[PC_CU + 1];
   alignas(16) float w[3][ATTN_MAX_HD];                              // norms' weights of q and k, in the lanes' order; 1 where there are none, and for v
-  alignas(16) float2 turn[PC_WINDOW + PAGED_BLOCK - 1][ATTN_MAX_HD / 2];   // cos, sin of tokens' pairs that turn
-  int at[PC_WINDOW + PAGED_BLOCK - 1];                              // tokens' positions for the rotation
+  alignas(16) float turn[PC_WINDOW + PAGED_BLOCK - 1][2][PC_PAIRS];   // cos, sin of tokens' pairs that turn
+  int at[PC_TOKENS];                                                // tokens' positions for the rotation
   int run[PC_WINDOW], len[PC_WINDOW], page[PC_TOKENS], row[PC_TOKENS];   // runs: first token, tokens; runs' or tokens' page and (first) row
   int runs, cover;
 };
 __device__ __forceinline__ void keep_weights(const CacheArgs& a, CacheShared& sh) {
-  for (int i = threadIdx.x; i < a.hd; i += PC_THREADS) {   // value i & 1 of pair i / 2
-    const int j = i >> 1, d = j >= a.nf || a.interleaved ? i : i & 1 ? j + a.nf : j;
+  for (int i = threadIdx.x; i < a.hd; i += PC_THREADS) {   // value i % 8 of lane i / 8: four first ones, four second
+    const int j = i / 8 * 4 + i % 4, second = i % 8 / 4, d = j >= a.nf || a.interleaved ? 2 * j + second : second ? j + a.nf : j;
     sh.w[0][i] = a.qw ? a.qw[d] : 1.f;
     sh.w[1][i] = a.kw ? a.kw[d] : 1.f;
     sh.w[2][i] = 1.f;
   }
 }
-__device__ __forceinline__ void load_turns(float2 (&cs)[4], const float2* turn, const LanePairs& m) {
-  const float4 a = *reinterpret_cast<const float4*>(turn + 4 * m.c), b = *reinterpret_cast<const float4*>(turn + 4 * m.c + 2);
-  cs[0] = make_float2(a.x, a.y), cs[1] = make_float2(a.z, a.w), cs[2] = make_float2(b.x, b.y), cs[3] = make_float2(b.z, b.w);
+__device__ __forceinline__ void keep_turn(float (*turn)[PC_PAIRS], int pair, int pos, double f, float amp) {
+  const float2 t = rope_angle(pos, f, amp);
+  turn[0][pair] = t.x, turn[1][pair] = t.y;
 }
 
 // Rows of nt tokens from t0 on: q, and (tg_rotary, 16-bit pages) k and v.  A row
 // is LPR lanes of 8 values; a thread has the same PC_ROWS rows of every token, of
-// the `part`-th share of a token's rows, and loads the next token's as it turns
-// this one's.  The angles of four tokens are made together, by all threads, while
-// the four before are turned.
+// the `part`-th share of a token's rows, and copies those of the next tokens into
+// its own places of a ring in shared memory as it turns this one's.  The angles
+// of four tokens are made together, by all threads, while the four before are
+// turned.
+extern __shared__ uint2 pc_ring[];   // [token % PC_AHEAD][row][half][thread]
 template <typename T, int LPR, bool VEC, int MODE, bool NORM>
 __device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, int t0, int nt, int part) {
   const int tid = threadIdx.x;
@@ -248,7 +280,27 @@ __device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, 
   const int first = part * PC_ROWS * ROWS + tid / LPR;   // its rows: first, first + ROWS, ..
   const T* from[PC_ROWS];
   T* to[PC_ROWS];   // q, tg_rotary's k; the head's place in a page
-  Raw<VEC> raw[PC_ROWS];
+  auto fetch = [&](int t) {
+    if (t < nt)
+#pragma unroll
+      for (int i = 0; i < PC_ROWS; i++) {
+        const int r = first + i * ROWS;
+        if (r < rows && m.any()) {
+          const uint32_t at = smem_u32(pc_ring + ((t % PC_AHEAD * PC_ROWS + i) * 2) * PC_THREADS + tid);
+          if (VEC) {
+            cp8(at, from[i] + (m.split ? 4 * m.c : 8 * m.c));
+            cp8(at + 8 * PC_THREADS, from[i] + (m.split ? m.nf + 4 * m.c : 8 * m.c + 4));
+          } else {   // in 2-byte pieces
+            Raw<VEC> raw;
+            load_pairs(raw, m, from[i]);
+            pc_ring[((t % PC_AHEAD * PC_ROWS + i) * 2) * PC_THREADS + tid] = make_uint2(raw.w[0], raw.w[1]);
+            pc_ring[((t % PC_AHEAD * PC_ROWS + i) * 2 + 1) * PC_THREADS + tid] = make_uint2(raw.w[2], raw.w[3]);
+          }
+        }
+        from[i] += r < a.H ? a.sq[0] : r < a.H + a.KH ? a.sk[0] : a.sv[0];
+      }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
 #pragma unroll
   for (int i = 0; i < PC_ROWS; i++) {
     const int r = first + i * ROWS;
@@ -263,8 +315,9 @@ __device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, 
       from[i] = (const T*)a.v + t * a.sv[0] + (r - a.H - a.KH) * a.sv[1];
       to[i] = (T*)(a.vp + (r - a.H - a.KH) * a.svp[1]);
     }
-    if (r < rows && m.any()) load_pairs(raw[i], m, from[i]);
   }
+#pragma unroll
+  for (int t = 0; t < PC_AHEAD - 1; t++) fetch(t);
   const int* cu = MODE == PC_ROTARY ? nullptr : keep_offsets(a.cu, a.B, sh.cu);
   if (NORM) keep_weights(a, sh);
   if (MODE != PC_ROTARY) __syncthreads();
@@ -285,8 +338,9 @@ __device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, 
     sh.at[tid] = pos, sh.page[tid] = page, sh.row[tid] = row;
   }
   const int pair = tid % PC_PAIRS, quarter = tid / PC_PAIRS;
+  const double f = pair < a.nf ? a.freqs[pair] : 0.0;
   auto angles = [&](int t) {   // of four tokens from t on
-    if (t + quarter < nt && pair < a.nf) sh.turn[(t & 4) + quarter][pair] = rope_angle(sh.at[t + quarter], a.freqs[pair], a.amp);
+    if (t + quarter < nt && pair < a.nf) keep_turn(sh.turn[(t & 4) + quarter], pair, sh.at[t + quarter], f, a.amp);
   };
   __syncthreads();
   angles(0);
@@ -296,23 +350,24 @@ __device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, 
       __syncthreads();
       angles(t + 4);
     }
-    float2 cs[4];
-    load_turns(cs, sh.turn[t & 7], m);
+    fetch(t + PC_AHEAD - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(PC_AHEAD - 1) : "memory");
+    const Turns turns(sh.turn[t & 7], m);
     const int page = MODE == PC_ROTARY ? -1 : sh.page[t];
 #pragma unroll
     for (int i = 0; i < PC_ROWS; i++) {
       const int r = first + i * ROWS;
       const bool is_q = r < a.H, is_v = r >= a.H + a.KH, here = r < rows && m.any();
-      float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      Pairs x = no_pairs();
       if (here) {
-        unpack_pairs<T>(x, raw[i], m);
-        from[i] += is_q ? a.sq[0] : is_v ? a.sv[0] : a.sk[0];
-        if (t + 1 < nt) load_pairs(raw[i], m, from[i]);
+        const uint2* at = pc_ring + ((t % PC_AHEAD * PC_ROWS + i) * 2) * PC_THREADS + tid;
+        const uint2 lo = at[0], hi = at[PC_THREADS];
+        unpack_pairs<T>(x, Raw<VEC>{{lo.x, lo.y, hi.x, hi.y}}, m);
       }
       if (NORM)   // lanes of rows that have none take part in the sums
         norm_row<LPR>(x, sh.w[is_q ? 0 : is_v ? 2 : 1] + (m.any() ? 8 * m.c : 0), a, is_q ? a.qw != nullptr : !is_v && a.kw);
       if (here) {
-        if (MODE != PC_PAGES16 || !is_v) rotate_pairs(x, cs, m);
+        if (MODE != PC_PAGES16 || !is_v) rotate_pairs<VEC>(x, turns, m);
         if (MODE != PC_PAGES16 || is_q) {
           if (page != -2) store_pairs<T, VEC>(to[i], m, x);
           to[i] += is_q ? a.sqo[0] : a.sko[0];
@@ -327,9 +382,8 @@ __device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, 
 
 // Runs of 8-bit blocks whose first token is one of the `window` packed tokens
 // from t0 on: a warp has one run's keys or values of a key head.  Its values are
-// read (the second time from the L1 cache) and worked out twice, for the largest
-// and for the codes: kept in registers they leave room for one CTA of an SM
-// instead of four (8,192 tokens with q 171 us).
+// worked out twice, for the largest and for the codes: kept in registers they
+// leave room for one CTA of an SM instead of four (8,192 tokens with q 171 us).
 template <typename T, int LPR, bool VEC, bool NORM>
 __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& sh, int t0) {
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
@@ -361,9 +415,28 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
   if (!sh.runs) return;
   const LanePairs m(a, lane % LPR);
   const int items = sh.runs * 2 * a.KH;
+  // an item's rows, in this warp's places of the ring: [row / RPP][half][lane]
+  uint2* ring = pc_ring + wid * (PAGED_BLOCK / RPP * 2 * 32) + lane;
+  auto fetch = [&](int item) {
+    const int i = item / (2 * a.KH), kh = item % (2 * a.KH) >> 1, is_v = item & 1;
+    const long long step = is_v ? a.sv[0] : a.sk[0];
+    const T* from = (is_v ? (const T*)a.v + kh * a.sv[1] : (const T*)a.k + kh * a.sk[1]) + (t0 + sh.run[i] + lane / LPR) * step;
+    for (int u = 0; u * RPP < sh.len[i]; u++, from += RPP * step)
+      if (u * RPP + lane / LPR < sh.len[i] && m.any()) {
+        if (VEC) {
+          cp8(smem_u32(ring + u * 64), from + (m.split ? 4 * m.c : 8 * m.c));
+          cp8(smem_u32(ring + u * 64 + 32), from + (m.split ? m.nf + 4 * m.c : 8 * m.c + 4));
+        } else {
+          Raw<VEC> raw;
+          load_pairs(raw, m, from);
+          ring[u * 64] = make_uint2(raw.w[0], raw.w[1]), ring[u * 64 + 32] = make_uint2(raw.w[2], raw.w[3]);
+        }
+      }
+  };
+  if (wid < items) fetch(wid);
   if (tid % PC_PAIRS < a.nf) {
     const double f = a.freqs[tid % PC_PAIRS];
-    for (int j = tid / PC_PAIRS; j < sh.cover; j += PC_THREADS / PC_PAIRS) sh.turn[j][tid % PC_PAIRS] = rope_angle(sh.at[j], f, a.amp);
+    for (int j = tid / PC_PAIRS; j < sh.cover; j += PC_THREADS / PC_PAIRS) keep_turn(sh.turn[j], tid % PC_PAIRS, sh.at[j], f, a.amp);
   }
   __syncthreads();
   for (int item = wid; item < items; item += PC_WARPS) {
@@ -375,39 +448,30 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
     float* scale_at = is_v ? a.vs + sh.page[i] * a.svs[0] + kh * a.svs[1] + block * a.svs[2]
                            : a.ks + sh.page[i] * a.sks[0] + kh * a.sks[1] + block * a.sks[2];
     const float before = off ? *scale_at : 0.f;
-    const long long step = is_v ? a.sv[0] : a.sk[0];
-    const T* from = (is_v ? (const T*)a.v + kh * a.sv[1] : (const T*)a.k + kh * a.sk[1]) + (t0 + j0 + lane / LPR) * step;
-    auto values = [&](int j, const Raw<VEC>& raw, float (&x)[8]) {   // of row j; zeros where there is none
+    asm volatile("cp.async.wait_all;" ::: "memory");   // each lane reads what it copied itself
+    auto values = [&](int u) {   // of row u RPP + lane / LPR; zeros where there is none
+      const int j = u * RPP + lane / LPR;
       const bool here = j < n && m.any();
-#pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = 0.f;
-      if (here) unpack_pairs<T>(x, raw, m);
-      if (is_v) return;
-      if (NORM) norm_row<LPR>(x, sh.w[1] + (m.any() ? 8 * m.c : 0), a, a.kw != nullptr);
+      Pairs x = no_pairs();
       if (here) {
-        float2 cs[4];
-        load_turns(cs, sh.turn[j0 + j], m);
-        rotate_pairs(x, cs, m);
+        const uint2 lo = ring[u * 64], hi = ring[u * 64 + 32];
+        unpack_pairs<T>(x, Raw<VEC>{{lo.x, lo.y, hi.x, hi.y}}, m);
       }
+      if (is_v) return x;
+      if (NORM) norm_row<LPR>(x, sh.w[1] + (m.any() ? 8 * m.c : 0), a, a.kw != nullptr);
+      if (here) rotate_pairs<VEC>(x, Turns(sh.turn[j0 + j], m), m);
+      return x;
     };
     uint32_t amax = 0;   // bits of the largest finite magnitude
-#pragma unroll 1
-    for (int u = 0; u * RPP < n; u += 4) {
-      Raw<VEC> raw[4];
+#pragma unroll 4
+    for (int u = 0; u * RPP < n; u++) {
+      const Pairs x = values(u);
+      auto most = [&](float v) {
+        const uint32_t y = __float_as_uint(v) & 0x7fffffffu;
+        amax = max(amax, y < 0x7f800000u ? y : 0u);
+      };
 #pragma unroll
-      for (int i4 = 0; i4 < 4; i4++)
-        if ((u + i4) * RPP + lane / LPR < n && m.any()) load_pairs(raw[i4], m, from + (u + i4) * RPP * step);
-#pragma unroll
-      for (int i4 = 0; i4 < 4; i4++) {
-        if ((u + i4) * RPP >= n) break;
-        float x[8];
-        values((u + i4) * RPP + lane / LPR, raw[i4], x);
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const uint32_t y = __float_as_uint(x[e]) & 0x7fffffffu;
-          amax = max(amax, y < 0x7f800000u ? y : 0u);
-        }
-      }
+      for (int e = 0; e < 2; e++) most(x.a[e].x), most(x.a[e].y), most(x.b[e].x), most(x.b[e].y);
     }
     amax = __reduce_max_sync(~0u, amax);
     const float need = __uint_as_float((uint32_t)(paged_scale_exp(amax) + 127) << 23);
@@ -427,29 +491,28 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
 #pragma unroll 2
     for (int u = 0; u * RPP < n; u++) {
       const int j = u * RPP + lane / LPR;
-      Raw<VEC> raw;
-      if (j < n && m.any()) load_pairs(raw, m, from + u * RPP * step);
-      float x[8];
-      values(j, raw, x);
+      Pairs x = values(u);
       if (j < n && m.any()) {
+        const float2 f = make_float2(inv, inv);
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] *= inv;
+        for (int e = 0; e < 2; e++) x.a[e] = pc_mul2(x.a[e], f), x.b[e] = pc_mul2(x.b[e], f);
         store_codes<VEC>(rows + (off + j) * pitch, m, x);
       }
     }
     if (lane == 0) *scale_at = scale;
+    if (item + PC_WARPS < items) fetch(item + PC_WARPS);
   }
 }
 
 template <typename T, int LPR, bool VEC, int MODE, bool NORM>
-__global__ void __launch_bounds__(PC_THREADS, 4) cache_kernel(const CacheArgs a) {
+__global__ void __launch_bounds__(PC_THREADS, PC_PER_SM) cache_kernel(const CacheArgs a) {
   __shared__ CacheShared sh;
   pdl_wait();
-  if (MODE == PC_PAGES8 && blockIdx.x < a.run_ctas)
-    runs_of_blocks<T, LPR, VEC, NORM>(a, sh, blockIdx.x * a.window);
-  else {
-    const int i = blockIdx.x - (MODE == PC_PAGES8 ? a.run_ctas : 0), t0 = i / a.parts * a.tokens;
-    token_rows<T, LPR, VEC, MODE, NORM>(a, sh, t0, min(a.tokens, a.T - t0), i % a.parts);
+  if (MODE == PC_PAGES8 && blockIdx.x >= a.token_ctas) {
+    runs_of_blocks<T, LPR, VEC, NORM>(a, sh, (blockIdx.x - a.token_ctas) * a.window);
+  } else {
+    const int t0 = blockIdx.x / a.parts * a.tokens;
+    token_rows<T, LPR, VEC, MODE, NORM>(a, sh, t0, min(a.tokens, a.T - t0), blockIdx.x % a.parts);
   }
 }
 
@@ -526,14 +589,17 @@ __global__ void __launch_bounds__(PC_THREADS) gather_pages_kernel(const GatherAr
   }
 }
 
+template <typename T, int LPR, bool VEC, int MODE, bool NORM>
+static cudaError_t launch_cache(const CacheArgs& a, int grid, cudaStream_t s) {
+  static std::atomic<unsigned long long> set{0};
+  const cudaError_t e = attn_smem(cache_kernel<T, LPR, VEC, MODE, NORM>, PC_RING, set);
+  return e == cudaSuccess ? launch_pdl(cache_kernel<T, LPR, VEC, MODE, NORM>, dim3(grid), PC_THREADS, PC_RING, s, a) : e;
+}
 template <typename T, int MODE, bool NORM>
 static cudaError_t launch_cache(const CacheArgs& a, int grid, cudaStream_t s) {
-  const bool vec = a.interleaved || a.nf % 4 == 0, narrow = a.hd <= 64;
-  if (narrow)
-    return vec ? launch_pdl(cache_kernel<T, 8, true, MODE, NORM>, dim3(grid), PC_THREADS, 0, s, a)
-               : launch_pdl(cache_kernel<T, 8, false, MODE, NORM>, dim3(grid), PC_THREADS, 0, s, a);
-  return vec ? launch_pdl(cache_kernel<T, 16, true, MODE, NORM>, dim3(grid), PC_THREADS, 0, s, a)
-             : launch_pdl(cache_kernel<T, 16, false, MODE, NORM>, dim3(grid), PC_THREADS, 0, s, a);
+  const bool vec = a.nf % 4 == 0;
+  if (a.hd <= 64) return vec ? launch_cache<T, 8, true, MODE, NORM>(a, grid, s) : launch_cache<T, 8, false, MODE, NORM>(a, grid, s);
+  return vec ? launch_cache<T, 16, true, MODE, NORM>(a, grid, s) : launch_cache<T, 16, false, MODE, NORM>(a, grid, s);
 }
 template <typename T, int MODE>
 static cudaError_t launch_cache(const CacheArgs& a, int grid, cudaStream_t s) {
@@ -548,11 +614,12 @@ using namespace tg;
 namespace tg {
 
 // The CTAs that rotate: shares of `rows` rows of a token, and tokens of a CTA so
-// that all of them are there at once where PC_TOKENS allow it.
+// that the SMs have them all at once, or as few times in a row as PC_TOKENS allow.
 static long long token_ctas(CacheArgs& a, long long rows, int per_sm) {
   const int share = PC_ROWS * PC_THREADS / (a.hd <= 64 ? 8 : 16), most = attn_sms() * per_sm;
   a.parts = (int)((rows + share - 1) / share);
-  a.tokens = (int)std::min((long long)PC_TOKENS, ((long long)a.T * a.parts + most - 1) / most);
+  const long long work = (long long)a.T * a.parts, waves = (work + (long long)most * PC_TOKENS - 1) / ((long long)most * PC_TOKENS);
+  a.tokens = (int)((work + most * waves - 1) / (most * waves));
   return (long long)((a.T + a.tokens - 1) / a.tokens) * a.parts;
 }
 
@@ -585,7 +652,7 @@ static int rotary(ArgCheck& c, const RotaryRecord& r) {
   a.T = (int)r.n_tokens, a.H = (int)r.n_heads, a.KH = (int)r.n_kv_heads, a.hd = (int)r.head_dim, a.nf = (int)r.n_freqs;
   a.interleaved = r.interleaved != 0, a.amp = (float)r.amplitude, a.eps = (float)r.eps, a.inv_hd = 1.f / a.hd;
   cudaStream_t s = static_cast<cudaStream_t>(r.stream);
-  const long long grid = token_ctas(a, (long long)a.H + a.KH, 4);
+  const long long grid = token_ctas(a, (long long)a.H + a.KH, PC_PER_SM);
   if (!c.need(grid < 1ll << 31, "too many rows")) return c.rc;
   return c.done(r.dtype == ATTN_BF16 ? launch_cache<__nv_bfloat16, PC_ROTARY>(a, (int)grid, s) : launch_cache<__half, PC_ROTARY>(a, (int)grid, s));
 }
@@ -631,11 +698,12 @@ static int append(ArgCheck& c, const AppendRecord& r) {
   a.T = (int)r.n_tokens, a.B = (int)r.batch, a.per = a.T / a.B, a.H = (int)r.n_heads, a.KH = (int)r.n_kv_heads, a.hd = (int)r.head_dim;
   a.nf = (int)r.n_freqs, a.n_pages = (int)r.n_pages, a.cols = (int)r.table_cols, a.shift = pool.shift;
   a.interleaved = r.interleaved != 0, a.amp = (float)r.amplitude, a.eps = (float)r.eps, a.inv_hd = 1.f / a.hd;
-  long long ctas = r.page_bits == 16 ? token_ctas(a, (long long)a.H + 2 * a.KH, 4) : a.H ? token_ctas(a, a.H, 4) : 0;
-  if (r.page_bits == 8) {
-    a.window = a.T / a.B >= PC_WINDOW ? PC_WINDOW : 1;
-    a.run_ctas = (a.T + a.window - 1) / a.window;
-    ctas += a.run_ctas;
+  long long ctas = r.page_bits == 16 ? token_ctas(a, (long long)a.H + 2 * a.KH, PC_PER_SM) : a.H ? token_ctas(a, a.H, PC_PER_SM - 1) : 0;
+  if (r.page_bits == 8) {   // the runs' CTAs behind: one of them beside those that rotate, on each SM
+    a.token_ctas = (int)ctas;
+    a.window = 1;
+    while (a.window < PC_WINDOW && (a.T + a.window - 1) / a.window > attn_sms() * PC_PER_SM) a.window *= 2;   // all CTAs there at once
+    ctas += (a.T + a.window - 1) / a.window;
   }
   if (!c.need(ctas < 1ll << 31, "too many rows")) return c.rc;
   const int grid = (int)ctas;
