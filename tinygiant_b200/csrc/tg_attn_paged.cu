@@ -36,7 +36,6 @@
 
 namespace tg {
 
-constexpr int PG_UNIT = 4;   // what a unit's start and end cost, in tiles of a warp
 constexpr int PG_JOIN_THREADS = 256;
 
 struct PagedArgs {
@@ -57,6 +56,7 @@ struct PagedArgs {
   unsigned by_g;  // 2^32 / G, rounded up (G > 1)
   int whole;      // units are not cut
   int team;       // warps of a group: 1, 2 or 4
+  int unit;       // what a unit's start and end cost, in tiles of a warp
   float c;        // scale log2(e)
 };
 
@@ -100,12 +100,10 @@ __device__ __forceinline__ void pg_mma(float (&d)[4], const uint32_t (&a)[4], ui
 // The query of row r = query G + head of the group: r / G for r < 2^25 (by_g G is
 // less than 2^32 + 128).
 __device__ __forceinline__ int query_of(const PagedArgs& a, int r) { return a.G == 1 ? r : (int)__umulhi((unsigned)r, a.by_g); }
-// A pair of accumulators over the sum L, whose reference is 2^up of theirs.
-template <typename T>
-__device__ __forceinline__ uint32_t paged_result(float2 v, float L, float up) {
-  const float s = at_exp2(up);
-  auto one = [&](float x) { return L == 0.f ? 0.f : x == 0.f ? x / L : x / L * s; };
-  return at_pack<T>(one(v.x), one(v.y));
+// What accumulators are multiplied by: 1 over the sum L, whose reference is 2^up of
+// theirs; 0 for a row without a key.
+__device__ __forceinline__ float paged_factor(float L, float up) {
+  return L == 0.f ? 0.f : up == -INFINITY ? 0.f * L : at_exp2(up) / L;
 }
 // Four e4m3 codes, the lowest byte first, as two pairs of fp16.
 __device__ __forceinline__ void pg_codes(uint32_t four, uint32_t& lo, uint32_t& hi) {
@@ -150,7 +148,7 @@ struct PagedShape {
 };
 
 // The tiles of a group as segments: consecutive tiles of one unit (sequence,
-// key head, 16 rows).  Units lie in a row, PG_UNIT places longer than their tiles
+// key head, 16 rows).  Units lie in a row, `unit` places longer than their tiles
 // (none for one without keys), and the places are cut evenly; where units are
 // not cut, a place is a unit.
 struct PagedWalk {
@@ -168,7 +166,7 @@ struct PagedWalk {
   // On to the next segment with keys.
   template <int KEYS>
   __device__ __forceinline__ void next(const PagedArgs& a) {
-    if (!a.whole) x += n + PG_UNIT;
+    if (!a.whole) x += n + a.unit;
     do {
       if (a.whole) x++;
       if (x >= x1) return;
@@ -237,7 +235,7 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
     long long round = 0, mine, before;
     auto scan = [&](int b) {
       const int n = b < a.B ? paged_tiles(min(max(a.lens[b], 0), a.max_len), a.n, a.window, KEYS) : 0;
-      mine = n ? (long long)(n + PG_UNIT) * HU : 0;
+      mine = n ? (long long)(n + a.unit) * HU : 0;
       long long y = mine;
       for (int o = 1; o < 32; o <<= 1) {
         const long long z = __shfl_up_sync(~0u, y, o);
@@ -258,7 +256,7 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
     for (int first = 0; first < a.B; first += S::THREADS) scan(first + tid);
     total = round;
     // a group has two tiles for each warp at least
-    parts = (int)max(1ll, min((long long)groups, paged_div(total, 2 * a.team + PG_UNIT)));
+    parts = (int)max(1ll, min((long long)groups, paged_div(total, 2 * a.team + a.unit)));
     const bool some = group < parts && total > 0;
     wk.x = some ? paged_div(total * group, parts) : total;
     wk.x1 = some ? paged_div(total * (group + 1), parts) : total;
@@ -278,9 +276,9 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
     if (some) {
       wk.b = sh.b0[wid - mate];
       wk.seq<KEYS>(a, wk.len_of(a, wk.b));
-      const long long r = wk.x - sh.before[wid - mate], hu = paged_div(r, wk.n + PG_UNIT);
+      const long long r = wk.x - sh.before[wid - mate], hu = paged_div(r, wk.n + a.unit);
       wk.kh = (int)hu / a.rt, wk.ri = (int)hu % a.rt;
-      wk.j = (int)(r - hu * (wk.n + PG_UNIT));
+      wk.j = (int)(r - hu * (wk.n + a.unit));
       wk.x -= wk.j;
       if (wk.j < wk.n)
         wk.j1 = (int)min((long long)wk.n, wk.x1 - wk.x);
@@ -307,6 +305,13 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
     lk = a.kp + 16 * ((uint64_t)lw.kh * a.skp[1] + (uint64_t)r0 * a.skp[2] + c0);
     lv = a.vp + 16 * ((uint64_t)lw.kh * a.svp[1] + (uint64_t)r0 * a.svp[2] + c0);
     if (CODES) ls = lane & 1 ? a.vs + (uint64_t)lw.kh * a.svs[1] : a.ks + (uint64_t)lw.kh * a.sks[1];
+    // and its queries, for begin() in a tile or two: a lane has a line
+    const int row = lw.ri * (8 * NT) + lane % (8 * NT);
+    if (row < a.rows && (HD > 64 || lane < 8 * NT)) {
+      const int i = query_of(a, row);
+      const T* q = (const T*)a.q + lw.b * a.sq[0] + i * a.sq[1] + (lw.kh * a.G + row - i * a.G) * a.sq[2];
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(q + (lane >= 8 * NT && a.hd > 64 ? 64 : 0)));
+    }
   };
   auto load = [&]() {
     if (lw.more()) {
@@ -627,11 +632,44 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
   auto end = [&]() {
     const bool all = wk.j == 0 && wk.j1 == wk.n;
     const size_t slot = 2 * group + (wk.j == 0);
+    if (!all && wk.j == 0 && mate == 0 && lane == 0)
+      a.desc[group] = make_int4(wk.b, wk.kh * a.rt + wk.ri, paged_group(wk.x + wk.n - 1, total, parts), 0);
+    if (a.team == 1) {   // from the registers
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int z = 0; z < 2; z++) {
+          float L = l[t][z], mm = m[t][z] - OFF;
+#pragma unroll
+          for (int sft = 4; sft < 32; sft <<= 1) L += __shfl_xor_sync(~0u, L, sft);
+          const int h = t * 8 + t4 * 2 + z, row = row0 + h;
+          if (row >= a.rows) continue;
+          if (all) {
+            const int head = wk.kh * a.G + row - tok[t][z] * a.G;
+            if (a.sinks) {
+              const float sink = a.sinks[head] * LOG2E, top = fmaxf(mm, sink);
+              if (sink != -INFINITY) L = (L == 0.f ? 0.f : L * at_exp2(mm - top)) + at_exp2(sink - top), mm = top;
+            }
+            const float f = paged_factor(L, r[t][z] - OFF - mm);
+            T* out = (T*)a.out + wk.b * a.so[0] + tok[t][z] * a.so[1] + head * a.so[2];
+#pragma unroll
+            for (int k = 0; k < S::STEPS; k += 4) {   // eight dimensions in a row
+              const int d = S::dim(k, g);
+              if (d < a.hd)
+                *reinterpret_cast<uint4*>(out + d) = make_uint4(at_pack<T>(o[t][k][z] * f, o[t][k][z + 2] * f), at_pack<T>(o[t][k + 1][z] * f, o[t][k + 1][z + 2] * f),
+                                                                at_pack<T>(o[t][k + 2][z] * f, o[t][k + 2][z + 2] * f), at_pack<T>(o[t][k + 3][z] * f, o[t][k + 3][z + 2] * f));
+            }
+          } else {
+            const size_t at = slot * (8 * NT) + h;
+#pragma unroll
+            for (int k = 0; k < S::STEPS; k++) *reinterpret_cast<float2*>(a.po + at * HD + 16 * k + 2 * g) = make_float2(o[t][k][z], o[t][k][z + 2]);
+            if (g == 0) a.pml[at] = make_float4(mm, L, r[t][z] - OFF, 0.f);
+          }
+        }
+      return;
+    }
     auto meet = [&]() {   // the group's warps
-      if (a.team == 1)
-        __syncwarp();
-      else
-        asm volatile("bar.sync %0, %1;" ::"r"(1 + wid / a.team), "r"(32 * a.team) : "memory");
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + wid / a.team), "r"(32 * a.team) : "memory");
     };
     // each warp's accumulators lie in the place of its ring that is free
     float* red = reinterpret_cast<float*>(ring + put * S::SLOT);
@@ -647,38 +685,49 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
           *reinterpret_cast<float2*>(&red[(t4 * 2 + z) * S::RP + 16 * k + 2 * g]) = make_float2(o[t][k][z], o[t][k][z + 2]);
       }
       meet();
+      // Each warp: lane 8 w + h has warp w's share of row h, then the row's factors.
+      const int w0 = wid - mate, h8 = row0 + t * 8 + (lane & 7), mine = lane >> 3;
+      const float4 ml = mine < a.team ? sh.ml[w0 + mine][lane & 7] : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+      const bool has = ml.y != 0.f;   // a warp with keys
+      float sink = -INFINITY;
+      if (a.sinks && all && h8 < a.rows) sink = a.sinks[wk.kh * a.G + h8 - query_of(a, h8) * a.G] * LOG2E;
+      float mm = has ? ml.x : -INFINITY, rr = has ? ml.z : -INFINITY;
+#pragma unroll
+      for (int sft = 8; sft < 32; sft <<= 1) mm = fmaxf(mm, __shfl_xor_sync(~0u, mm, sft)), rr = fmaxf(rr, __shfl_xor_sync(~0u, rr, sft));
+      mm = fmaxf(mm, sink);
+      const float fr = has && ml.z != -INFINITY ? at_exp2(ml.z - rr) : 0.f;
+      float L = has ? ml.y * at_exp2(ml.x - mm) : 0.f;
+#pragma unroll
+      for (int sft = 8; sft < 32; sft <<= 1) L += __shfl_xor_sync(~0u, L, sft);
+      if (sink != -INFINITY) L += at_exp2(sink - mm);
+      const float fin = paged_factor(L, rr - mm);
+      uint32_t from[4];   // this lane's first pair of each warp
+#pragma unroll
+      for (int w = 0; w < 4; w++)
+        from[w] = smem_u32(dsm) + ((w0 + (w < a.team ? w : 0)) * S::D + __shfl_sync(~0u, __float_as_int(ml.w), w < a.team ? 8 * w : 0)) * S::SLOT + 8 * lane;
 #pragma unroll 1
-      for (int i = mate * 32 + lane; i < 4 * HD; i += 32 * a.team) {
-        const int h = i / (HD / 2), at = i % (HD / 2), row = row0 + t * 8 + h;   // pair `at` of row h
+      for (int i = mate * 32; i < 4 * HD; i += 32 * a.team) {
+        const int h = i / (HD / 2), at = i % (HD / 2), row = row0 + t * 8 + h;   // pairs from `at` on of row h
         if (row >= a.rows) break;
-        const int query = query_of(a, row), head = wk.kh * a.G + row - query * a.G, d = S::dim(at / 8, at % 8);
-        const float sink = a.sinks && all ? a.sinks[head] * LOG2E : -INFINITY;
-        float mm = sink, rr = -INFINITY, L = 0.f;
         float2 v = make_float2(0.f, 0.f);
-#pragma unroll 4
-        for (int w = wid - mate; w < wid - mate + a.team; w++) mm = fmaxf(mm, sh.ml[w][h].x), rr = fmaxf(rr, sh.ml[w][h].z);
-#pragma unroll 4
-        for (int w = wid - mate; w < wid - mate + a.team; w++) {
-          const float4 ml = sh.ml[w][h];
-          const float2 y = *reinterpret_cast<const float2*>(dsm + (w * S::D + __float_as_int(ml.w)) * S::SLOT + (h * S::RP + 2 * at) * 4);
-          if (ml.y == 0.f) continue;   // a warp without keys
-          L = fmaf(ml.y, at_exp2(ml.x - mm), L);
-          const float fr = ml.z != -INFINITY ? at_exp2(ml.z - rr) : 0.f;
-          if (fr != 0.f) v.x = fmaf(y.x, fr, v.x), v.y = fmaf(y.y, fr, v.y);
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+          const float f = __shfl_sync(~0u, fr, 8 * w + h);   // 0 where there is no warp w
+          const uint2 y = lds8(from[w] + (h * S::RP + 2 * at) * 4);
+          if (f != 0.f) v.x = fmaf(__uint_as_float(y.x), f, v.x), v.y = fmaf(__uint_as_float(y.y), f, v.y);
         }
         if (all) {
-          if (sink != -INFINITY) L += at_exp2(sink - mm);
+          const int query = query_of(a, row), d = S::dim((at + lane) / 8, lane % 8);
+          const float f = __shfl_sync(~0u, fin, h);
           if (d < a.hd)
-            *reinterpret_cast<uint32_t*>((T*)a.out + wk.b * a.so[0] + query * a.so[1] + head * a.so[2] + d) = paged_result<T>(v, L, rr - mm);
+            *reinterpret_cast<uint32_t*>((T*)a.out + wk.b * a.so[0] + query * a.so[1] + (wk.kh * a.G + row - query * a.G) * a.so[2] + d) = at_pack<T>(v.x * f, v.y * f);
         } else {
-          *reinterpret_cast<float2*>(a.po + (slot * (8 * NT) + t * 8 + h) * HD + 2 * at) = v;
-          if (at == 0) a.pml[slot * (8 * NT) + t * 8 + h] = make_float4(mm, L, rr, 0.f);
+          *reinterpret_cast<float2*>(a.po + (slot * (8 * NT) + t * 8 + h) * HD + 2 * (at + lane)) = v;
         }
       }
+      if (!all && mate == 0 && lane < 8) a.pml[slot * (8 * NT) + t * 8 + lane] = make_float4(mm, L, rr, 0.f);
       meet();
     }
-    if (!all && wk.j == 0 && mate == 0 && lane == 0)
-      a.desc[group] = make_int4(wk.b, wk.kh * a.rt + wk.ri, paged_group(wk.x + wk.n - 1, total, parts), 0);
   };
 
   // D - 1 loads, then for each tile one load more; whoever has no tile left in
@@ -762,17 +811,18 @@ __global__ void __launch_bounds__(PG_JOIN_THREADS) paged_join_kernel(const Paged
 #pragma unroll
       for (int e = 0; e < HD / 64; e++) v[e].x = fmaf(y[e].x, fr, v[e].x), v[e].y = fmaf(y[e].y, fr, v[e].y);
     }
+    const float fin = paged_factor(L, rr - mm);
 #pragma unroll
     for (int e = 0; e < HD / 64; e++) {
       const int pair = lane + 32 * e, to = PagedShape<T, CODES, HD, NT>::dim(pair / 8, pair % 8);
-      if (to < a.hd) *reinterpret_cast<uint32_t*>((T*)a.out + d.x * a.so[0] + query * a.so[1] + head * a.so[2] + to) = paged_result<T>(v[e], L, rr - mm);
+      if (to < a.hd) *reinterpret_cast<uint32_t*>((T*)a.out + d.x * a.so[0] + query * a.so[1] + head * a.so[2] + to) = at_pack<T>(v[e].x * fin, v[e].y * fin);
     }
   }
 }
 
 // What the host settles before the lengths are known.
 struct PagedSpace {
-  int nt, rt, whole, team = 4, grid, groups;
+  int nt, rt, whole, team = 4, unit, grid, groups;
   size_t po = 0, pml = 0, desc = 0, bytes = 0;
   PagedSpace(int bits, int batch, int queries, int max_len, int window, int H, int KH, int hd, int sms) {
     const int rows = queries * (H / KH), HD = hd <= 64 ? 64 : 128, keys = HD * bits / 8 <= 128 ? 32 : 16;
@@ -783,8 +833,14 @@ struct PagedSpace {
     // keys that a unit's queries read, at most, from a whole block on
     const long long most = window > 0 ? std::min((long long)max_len, (long long)window + queries + 14) : max_len, tiles = (most + keys - 1) / keys;
     whole = tiles <= 16;
+    // A group of four shares a unit's tiles and joins at its end, which costs each
+    // of them two to three tiles' time; a warp by itself has no one to wait for,
+    // but leaves more pieces to the second kernel.
     if (whole)
       while (team > 1 && (long long)sms * warps / team < units) team /= 2;
+    else if (units * tiles >= 8ll * sms * warps)
+      team = 1;
+    unit = team == 1 ? 1 : 5 * team / 2;
     const long long want = whole ? units : units * tiles / 2;   // groups that can have work
     grid = (int)std::max(1ll, std::min((long long)sms, (want * team + warps - 1) / warps));
     groups = grid * warps / team;
@@ -878,7 +934,7 @@ int tg::attention_paged(ArgCheck& c, const AttendRecord& r) {
   a.st = pool.st, a.B = batch, a.n = queries, a.G = H / KH, a.KH = KH, a.rows = queries * a.G, a.rt = sp.rt;
   a.by_g = (unsigned)(((1ull << 32) + a.G - 1) / a.G);
   a.hd = hd, a.cols = (int)r.table_cols, a.n_pages = (int)r.n_pages, a.shift = pool.shift, a.max_len = max_len, a.window = (int)r.window;
-  a.whole = sp.whole, a.team = sp.team, a.c = (float)r.scale * LOG2E;
+  a.whole = sp.whole, a.team = sp.team, a.unit = sp.unit, a.c = (float)r.scale * LOG2E;
   cudaStream_t s = static_cast<cudaStream_t>(r.stream);
   if (r.dtype == ATTN_BF16)
     return c.done(r.page_bits == 8 ? run_paged<__nv_bfloat16, true>(a, sp, s) : run_paged<__nv_bfloat16, false>(a, sp, s));
