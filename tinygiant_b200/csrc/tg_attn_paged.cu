@@ -774,49 +774,64 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
   }
 }
 
-// Block i: the unit that begins in group i and ends in a later one, its pieces'
-// weighted sum.
+// Block (i, y): rows 2 y and 2 y + 1 of the unit that begins in group i and ends
+// in a later one, the pieces' weighted sum: four warps have every fourth piece
+// each (a long sequence by itself lies in a hundred of them).
 template <typename T, bool CODES, int HD, int NT>
 __global__ void __launch_bounds__(PG_JOIN_THREADS) paged_join_kernel(const PagedArgs a) {
+  __shared__ float2 part[PG_JOIN_THREADS / 32][HD / 2];
+  __shared__ float sums[PG_JOIN_THREADS / 32];
   pdl_wait();
-  const int i = blockIdx.x, lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const int i = blockIdx.x, lane = threadIdx.x & 31, wid = threadIdx.x >> 5, w4 = wid & 3, h = 2 * blockIdx.y + (wid >> 2);
   const int4 d = a.desc[i];
   if (d.x < 0) return;
-  const int kh = d.y / a.rt, row0 = d.y % a.rt * (8 * NT), pieces = d.z - i + 1;
-  auto at = [&](int p, int h) { return (size_t)(p ? 2 * (i + p) : 2 * i + 1) * (8 * NT) + h; };
-  for (int h = wid; h < 8 * NT && row0 + h < a.rows; h += PG_JOIN_THREADS / 32) {
-    const int row = row0 + h, query = query_of(a, row), head = kh * a.G + row - query * a.G;
-    const float sink = a.sinks ? a.sinks[head] * LOG2E : -INFINITY;
-    float mm = sink, rr = -INFINITY;
+  const int kh = d.y / a.rt, row = d.y % a.rt * (8 * NT) + h, pieces = d.z - i + 1;
+  const bool here = row < a.rows;
+  const int query = query_of(a, here ? row : 0), head = kh * a.G + (here ? row : 0) - query * a.G;
+  auto at = [&](int p) { return (size_t)(p ? 2 * (i + p) : 2 * i + 1) * (8 * NT) + h; };
+  const float sink = a.sinks ? a.sinks[head] * LOG2E : -INFINITY;
+  float mm = sink, rr = -INFINITY;
+  if (here)
     for (int p = lane; p < pieces; p += 32) {
-      const float4 ml = a.pml[at(p, h)];
+      const float4 ml = a.pml[at(p)];
       mm = fmaxf(mm, ml.x), rr = fmaxf(rr, ml.z);
     }
 #pragma unroll
-    for (int sft = 16; sft; sft >>= 1) mm = fmaxf(mm, __shfl_xor_sync(~0u, mm, sft)), rr = fmaxf(rr, __shfl_xor_sync(~0u, rr, sft));
-    float L = sink != -INFINITY ? at_exp2(sink - mm) : 0.f;
-    float2 v[HD / 64];
+  for (int sft = 16; sft; sft >>= 1) mm = fmaxf(mm, __shfl_xor_sync(~0u, mm, sft)), rr = fmaxf(rr, __shfl_xor_sync(~0u, rr, sft));
+  float L = 0.f;
+  float2 v[HD / 64];
 #pragma unroll
-    for (int e = 0; e < HD / 64; e++) v[e] = make_float2(0.f, 0.f);
+  for (int e = 0; e < HD / 64; e++) v[e] = make_float2(0.f, 0.f);
+  if (here)
 #pragma unroll 4
-    for (int p = 0; p < pieces; p++) {
-      const float4 ml = a.pml[at(p, h)];
+    for (int p = w4; p < pieces; p += 4) {
+      const float4 ml = a.pml[at(p)];
       float2 y[HD / 64];
 #pragma unroll
-      for (int e = 0; e < HD / 64; e++) y[e] = *reinterpret_cast<const float2*>(a.po + at(p, h) * HD + 2 * lane + 64 * e);
-      if (ml.y == 0.f) continue;
-      L = fmaf(ml.y, at_exp2(ml.x - mm), L);
-      const float fr = ml.z != -INFINITY ? at_exp2(ml.z - rr) : 0.f;
-      if (fr == 0.f) continue;
+      for (int e = 0; e < HD / 64; e++) y[e] = *reinterpret_cast<const float2*>(a.po + at(p) * HD + 2 * lane + 64 * e);
+      const float fm = ml.y == 0.f ? 0.f : at_exp2(ml.x - mm), fr = ml.y == 0.f || ml.z == -INFINITY ? 0.f : at_exp2(ml.z - rr);
+      if (fm != 0.f) L = fmaf(ml.y, fm, L);   // not 0 x inf
+      if (fr != 0.f)
 #pragma unroll
-      for (int e = 0; e < HD / 64; e++) v[e].x = fmaf(y[e].x, fr, v[e].x), v[e].y = fmaf(y[e].y, fr, v[e].y);
+        for (int e = 0; e < HD / 64; e++) v[e].x = fmaf(y[e].x, fr, v[e].x), v[e].y = fmaf(y[e].y, fr, v[e].y);
     }
-    const float fin = paged_factor(L, rr - mm);
 #pragma unroll
-    for (int e = 0; e < HD / 64; e++) {
-      const int pair = lane + 32 * e, to = PagedShape<T, CODES, HD, NT>::dim(pair / 8, pair % 8);
-      if (to < a.hd) *reinterpret_cast<uint32_t*>((T*)a.out + d.x * a.so[0] + query * a.so[1] + head * a.so[2] + to) = at_pack<T>(v[e].x * fin, v[e].y * fin);
-    }
+  for (int e = 0; e < HD / 64; e++) part[wid][lane + 32 * e] = v[e];
+  if (lane == 0) sums[wid] = L;
+  __syncthreads();
+  if (w4 || !here) return;
+#pragma unroll
+  for (int w = 1; w < 4; w++) {
+    L += sums[wid + w];
+#pragma unroll
+    for (int e = 0; e < HD / 64; e++) v[e].x += part[wid + w][lane + 32 * e].x, v[e].y += part[wid + w][lane + 32 * e].y;
+  }
+  if (sink != -INFINITY) L += at_exp2(sink - mm);
+  const float fin = paged_factor(L, rr - mm);
+#pragma unroll
+  for (int e = 0; e < HD / 64; e++) {
+    const int pair = lane + 32 * e, to = PagedShape<T, CODES, HD, NT>::dim(pair / 8, pair % 8);
+    if (to < a.hd) *reinterpret_cast<uint32_t*>((T*)a.out + d.x * a.so[0] + query * a.so[1] + head * a.so[2] + to) = at_pack<T>(v[e].x * fin, v[e].y * fin);
   }
 }
 
@@ -834,13 +849,12 @@ struct PagedSpace {
     const long long most = window > 0 ? std::min((long long)max_len, (long long)window + queries + 14) : max_len, tiles = (most + keys - 1) / keys;
     whole = tiles <= 16;
     // A group of four shares a unit's tiles and joins at its end, which costs each
-    // of them two to three tiles' time; a warp by itself has no one to wait for,
-    // but leaves more pieces to the second kernel.
+    // of them two to three tiles' time; a warp by itself has no one to wait for, but
+    // where units are cut it leaves four times the pieces to the second kernel (64
+    // sequences 41 us, with groups of two 38, of four 36).
     if (whole)
       while (team > 1 && (long long)sms * warps / team < units) team /= 2;
-    else if (units * tiles >= 8ll * sms * warps)
-      team = 1;
-    unit = team == 1 ? 1 : 5 * team / 2;
+    unit = 7 * team / 2;
     const long long want = whole ? units : units * tiles / 2;   // groups that can have work
     grid = (int)std::max(1ll, std::min((long long)sms, (want * team + warps - 1) / warps));
     groups = grid * warps / team;
@@ -864,7 +878,7 @@ static cudaError_t run_paged(const PagedArgs& a, const PagedSpace& sp, cudaStrea
   if (e == cudaSuccess) e = launch_pdl(paged_kernel<T, CODES, HD, NT, MANY>, dim3(sp.grid), PagedShape<T, CODES, HD, NT>::THREADS, smem, s, a);
   count_launches(1);
   if (e == cudaSuccess && !a.whole && sp.groups > 1) {
-    e = launch_pdl(paged_join_kernel<T, CODES, HD, NT>, dim3(sp.groups - 1), PG_JOIN_THREADS, 0, s, a);
+    e = launch_pdl(paged_join_kernel<T, CODES, HD, NT>, dim3(sp.groups - 1, 4 * NT), PG_JOIN_THREADS, 0, s, a);
     count_launches(1);
   }
   return e;
