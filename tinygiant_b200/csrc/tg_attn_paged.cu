@@ -183,8 +183,11 @@ struct PagedWalk {
   }
 };
 
-// 64-bit quotients in one place: a few hundred bytes of code each.
-__device__ __noinline__ long long paged_div(long long x, long long y) { return x / y; }
+// Quotients of numbers that are not negative, in one place: that of 64 bits is long
+// in code and time, and seldom needed.
+__device__ __noinline__ long long paged_div(long long x, long long y) {
+  return (unsigned long long)(x | y) >> 32 ? x / y : (long long)((unsigned)x / (unsigned)y);
+}
 
 // The group of n that place x of `total` falls to: group i has [i total / n, (i + 1) total / n).
 __device__ __forceinline__ int paged_group(long long x, long long total, int n) { return (int)paged_div((x + 1) * n - 1, total); }

@@ -34,7 +34,8 @@ static_assert(PC_THREADS == 4 * PC_PAIRS, "angles of four tokens at a time");
 constexpr int PC_CU = 1024;       // sequences whose offsets are kept in shared memory
 constexpr int PC_WINDOW = 16;     // packed tokens that a CTA looks through for blocks' first ones, at most
 constexpr int PC_TOKENS = 32;     // tokens of a CTA that rotates, at most
-constexpr int PC_GATHER = 64;     // tokens of a gather CTA, at most
+constexpr int PC_GATHERS = 5;     // gather CTAs of an SM
+constexpr int PC_GATHER = 128;    // tokens of a gather CTA, at most
 constexpr int PC_ROWS = 3;        // rows of a token that a thread has
 constexpr int PC_AHEAD = 3;       // tokens whose rows are there or on their way
 constexpr int PC_RING = PC_AHEAD * PC_ROWS * 2 * 8 * PC_THREADS;
@@ -529,7 +530,7 @@ struct GatherArgs {
 // Rows of the packed outputs, 16 bytes of a page's row at a time, four of them
 // loaded before the first is stored.  A CTA has `per` tokens.
 template <typename T, bool CODES>
-__global__ void __launch_bounds__(PC_THREADS) gather_pages_kernel(const GatherArgs a, int lpr, int per) {
+__global__ void __launch_bounds__(PC_THREADS, PC_GATHERS) gather_pages_kernel(const GatherArgs a, int lpr, int per) {
   constexpr int N = 4;
   __shared__ int s_cu[PC_CU + 1], s_page[PC_GATHER], s_row[PC_GATHER];
   pdl_wait();
@@ -742,7 +743,10 @@ static int gather(ArgCheck& c, const GatherRecord& r) {
   a.wide = ((uintptr_t)r.k_out | (uintptr_t)r.v_out) % 32 == 0 && (t[0] | t[1] | t[2] | t[3]) % 16 == 0;
   int lpr = 1;
   while (lpr < a.hd / (r.page_bits == 8 ? 16 : 8)) lpr *= 2;
-  const int per = a.T >= 64 * attn_sms() * 4 ? 64 : 16;   // tokens of a CTA
+  // tokens of a CTA, so that the SMs have all CTAs at once, or as few times in a
+  // row as PC_GATHER allows (62,342 rows, 191 MB: 64 tokens, 1.3 times as many
+  // CTAs as fit, 38 us)
+  const int most = attn_sms() * PC_GATHERS, waves = (int)(((long long)a.T + most * PC_GATHER - 1) / (most * PC_GATHER)), per = (int)std::max(4ll, ((long long)a.T + (long long)most * waves - 1) / ((long long)most * waves));
   const dim3 grid((a.T + per - 1) / per);
   cudaStream_t s = static_cast<cudaStream_t>(r.stream);
   const bool bf = r.dtype == ATTN_BF16;

@@ -48,29 +48,28 @@ from .attention import _DTYPES, _MOST, ArgumentError, _empty, _no_backward, _raw
 __all__ = ["rotary_frequencies", "rotary", "cache_append", "attention_paged", "cache_gather", "ArgumentError"]
 
 _CODES = torch.float8_e4m3fn
+_F32, _F64, _I32 = torch.float32, torch.float64, torch.int32
+_current = torch._C._cuda_getDevice
 _MISFITS = (AttributeError, IndexError, KeyError, TypeError, ValueError)   # of what is no tensor, or of other dimensions
 # The calls' arguments as tg_paged_call's records: a call of 30 arguments through ctypes takes 7 us, a record of them 1.
 _ROTARY, _APPEND, _ATTEND, _GATHER = (struct.Struct(f).pack for f in ("24q2dq", "49q2dq", "41qd3q", "36q"))
 
 
-def _run(device, pack, *args):
-    """One library call on torch's current stream of `device` (an index)."""
-    if device != torch._C._cuda_getDevice():
+def _run(device, record):
+    """One library call on the tensors' device (an index)."""
+    if device != _current():
         with torch.cuda.device(device):
-            return _run(device, pack, *args)
-    try:
-        record = pack(*args, _raw_stream(device))
-    except struct.error as e:                      # a number that is none, or beyond 64 bits
-        raise ValueError(f"bad argument: {e}") from None
-    rc = load().tg_paged_call(record)
+            rc = load().tg_paged_call(record)
+    else:
+        rc = load().tg_paged_call(record)
     if rc:
         code, msg = last_error()
         raise (ArgumentError if rc == 3 else TinyGiantCudaError)(f"[{code}] {msg}")
 
 
-def _at(t):
-    """Where a tensor lies, or 0."""
-    return 0 if t is None else t.data_ptr()
+def _no_number(e):
+    """What struct cannot pack: a number that is none, or beyond 64 bits."""
+    raise ValueError(f"bad argument: {e}") from None
 
 
 def rotary_frequencies(dim, theta=10000.0, *, scaling=None, factor=1.0, original_len=None, beta_fast=32.0, beta_slow=1.0,
@@ -143,10 +142,10 @@ def _pool(dev, dtype, k_pages, v_pages, tables, k_scales, v_scales, KH, hd):
     v0, v1, v2, v3 = v_pages.stride()
     t0, t1 = tables.stride()
     if not (kh == KH and d == hd and v_pages.shape == shape and v_pages.dtype is kind and k3 == v3 == t1 == 1
-            and tables.dtype is torch.int32 and k_pages.get_device() == v_pages.get_device() == tables.get_device() == dev):
+            and tables.dtype is _I32 and k_pages.get_device() == v_pages.get_device() == tables.get_device() == dev):
         return None
     if kind is _CODES:
-        if not (k_scales.shape == v_scales.shape == (N, kh, page // 16) and k_scales.dtype is v_scales.dtype is torch.float32
+        if not (k_scales.shape == v_scales.shape == (N, kh, page // 16) and k_scales.dtype is v_scales.dtype is _F32
                 and k_scales.get_device() == v_scales.get_device() == dev):
             return None
         return (k0, k1, k2, v0, v1, v2, *k_scales.stride(), *v_scales.stride(), t0)
@@ -169,10 +168,6 @@ def _pool_named(dtype, k_pages, v_pages, tables, k_scales, v_scales, B, KH, hd):
             codes and ("k_scales", k_scales, (torch.float32,), (shape[0], KH, shape[2] // 16)),
             codes and ("v_scales", v_scales, (torch.float32,), (shape[0], KH, shape[2] // 16)),
             ("tables", tables, (torch.int32,), (B, -1))]
-
-
-def _bits(k_pages):
-    return 8 if k_pages.dtype is _CODES else 16
 
 
 def rotary(q, k, positions, freqs, *, interleaved=False, amplitude=1.0, q_norm=None, k_norm=None, eps=1e-6, out=None):
@@ -209,9 +204,9 @@ def rotary(q, k, positions, freqs, *, interleaved=False, amplitude=1.0, q_norm=N
                 ko = _empty((T, KH, hd), (p0, p1, 1), dtype=dtype, device=q.device)
             fit = fit and k.dtype is dtype and k.get_device() == dev and k.shape == (T, KH, hd)
         n, = freqs.shape
-        fit = (fit and dev >= 0 and q2 == k2 == o2 == p2 == 1 and positions is not None and _vector(positions, dev, torch.int32, T)
-               and _vector(freqs, dev, torch.float64, n) and (q_norm is None or _vector(q_norm, dev, torch.float32, hd))
-               and (k_norm is None or _vector(k_norm, dev, torch.float32, hd)))
+        fit = (fit and dev >= 0 and q2 == k2 == o2 == p2 == 1 and positions is not None and _vector(positions, dev, _I32, T)
+               and _vector(freqs, dev, _F64, n) and (q_norm is None or _vector(q_norm, dev, _F32, hd))
+               and (k_norm is None or _vector(k_norm, dev, _F32, hd)))
     except _MISFITS:
         fit = False
     if not fit:
@@ -219,8 +214,14 @@ def rotary(q, k, positions, freqs, *, interleaved=False, amplitude=1.0, q_norm=N
     if (q.requires_grad or (k is not None and (k.requires_grad or ko.requires_grad)) or freqs.requires_grad or qo.requires_grad
             or (q_norm is not None and q_norm.requires_grad) or (k_norm is not None and k_norm.requires_grad)):
         _no_backward()
-    _run(dev, _ROTARY, 0, kind, q.data_ptr(), _at(k), qo.data_ptr(), _at(ko), positions.data_ptr(), freqs.data_ptr(), _at(q_norm),
-         _at(k_norm), T, H, KH, hd, n, interleaved, q0, q1, k0, k1, o0, o1, p0, p1, amplitude, eps)
+    try:
+        record = _ROTARY(0, kind, q.data_ptr(), 0 if k is None else k.data_ptr(), qo.data_ptr(), 0 if k is None else ko.data_ptr(),
+                         positions.data_ptr(), freqs.data_ptr(), 0 if q_norm is None else q_norm.data_ptr(),
+                         0 if k_norm is None else k_norm.data_ptr(), T, H, KH, hd, n, interleaved, q0, q1, k0, k1, o0, o1, p0, p1,
+                         amplitude, eps, _raw_stream(dev))
+    except (struct.error, OverflowError) as e:
+        _no_number(e)
+    _run(dev, record)
     if given:
         _written(qo)
         if ko is not None:
@@ -269,8 +270,8 @@ def cache_append(k, v, k_pages, v_pages, tables, lens, cu=None, *, k_scales=None
         N, _, page, _ = k_pages.shape
         rows, cols = tables.shape
         fit = (pool and dev >= 0 and k2 == v2 == 1 and v.shape == shape and v.dtype is dtype and v.get_device() == dev and rows == B
-               and _vector(lens, dev, torch.int32, B)
-               and ((T % B == 0 if B else T == 0) if cu is None else _vector(cu, dev, torch.int32, B + 1)))
+               and _vector(lens, dev, _I32, B)
+               and ((T % B == 0 if B else T == 0) if cu is None else _vector(cu, dev, _I32, B + 1)))
         if q is None:
             H, q0, q1, o0, o1, fit = 0, 8, 8, 8, 8, fit and out is None
         else:
@@ -285,9 +286,9 @@ def cache_append(k, v, k_pages, v_pages, tables, lens, cu=None, *, k_scales=None
         n = 0
         if freqs is not None:
             n, = freqs.shape
-            fit = fit and _vector(freqs, dev, torch.float64, n)
-        fit = (fit and (positions is None or _vector(positions, dev, torch.int32, T))
-               and (q_norm is None or _vector(q_norm, dev, torch.float32, hd)) and (k_norm is None or _vector(k_norm, dev, torch.float32, hd)))
+            fit = fit and _vector(freqs, dev, _F64, n)
+        fit = (fit and (positions is None or _vector(positions, dev, _I32, T))
+               and (q_norm is None or _vector(q_norm, dev, _F32, hd)) and (k_norm is None or _vector(k_norm, dev, _F32, hd)))
     except _MISFITS:
         fit = False
     if not fit:
@@ -298,9 +299,17 @@ def cache_append(k, v, k_pages, v_pages, tables, lens, cu=None, *, k_scales=None
             or (q is not None and (q.requires_grad or out.requires_grad)) or (q_norm is not None and q_norm.requires_grad)
             or (k_norm is not None and k_norm.requires_grad)):
         _no_backward()
-    _run(dev, _APPEND, 1, kind, _bits(k_pages), _at(q), k.data_ptr(), v.data_ptr(), _at(out), k_pages.data_ptr(), v_pages.data_ptr(),
-         _at(k_scales), _at(v_scales), tables.data_ptr(), lens.data_ptr(), _at(cu), _at(positions), _at(freqs), _at(q_norm), _at(k_norm),
-         T, B, N, page, cols, H, KH, hd, n, interleaved, q0, q1, k0, k1, v0, v1, o0, o1, *pool, amplitude, eps)
+    try:
+        record = _APPEND(1, kind, 16 if k_scales is None else 8, 0 if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                         0 if q is None else out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                         0 if k_scales is None else k_scales.data_ptr(), 0 if k_scales is None else v_scales.data_ptr(), tables.data_ptr(),
+                         lens.data_ptr(), 0 if cu is None else cu.data_ptr(), 0 if positions is None else positions.data_ptr(),
+                         0 if freqs is None else freqs.data_ptr(), 0 if q_norm is None else q_norm.data_ptr(),
+                         0 if k_norm is None else k_norm.data_ptr(), T, B, N, page, cols, H, KH, hd, n, interleaved, q0, q1, k0, k1, v0,
+                         v1, o0, o1, *pool, amplitude, eps, _raw_stream(dev))
+    except (struct.error, OverflowError) as e:
+        _no_number(e)
+    _run(dev, record)
     _written((k_pages, v_pages) if k_scales is None else (k_pages, v_pages, k_scales, v_scales))
     if given:
         _written(out)
@@ -361,9 +370,9 @@ def attention_paged(q, k_pages, v_pages, tables, lens, *, k_scales=None, v_scale
         N, KH, page, _ = k_pages.shape
         pool = _pool(dev, dtype, k_pages, v_pages, tables, k_scales, v_scales, KH, hd)
         rows, cols = tables.shape
-        fit = (pool and dev >= 0 and q3 == o3 == 1 and rows == B and lens is not None and _vector(lens, dev, torch.int32, B)
+        fit = (pool and dev >= 0 and q3 == o3 == 1 and rows == B and lens is not None and _vector(lens, dev, _I32, B)
                and (not given or (out.shape == shape and out.dtype is dtype and out.get_device() == dev))
-               and (sinks is None or _vector(sinks, dev, torch.float32, H)))
+               and (sinks is None or _vector(sinks, dev, _F32, H)))
     except _MISFITS:
         fit = False
     if not fit:
@@ -373,12 +382,17 @@ def attention_paged(q, k_pages, v_pages, tables, lens, *, k_scales=None, v_scale
         _no_backward()
     most = cols * page
     max_len = most if max_len is None or max_len > most else max_len
-    bits, window = _bits(k_pages), _window(window)
+    bits, window = 16 if k_scales is None else 8, _window(window)
     nbytes = load().tg_attention_paged_workspace(bits, B, n, max_len, window, H, KH, hd) if 0 < max_len < _MOST else 0
     ws = _empty((nbytes,), (1,), dtype=torch.uint8, device=q.device) if nbytes else None
-    _run(dev, _ATTEND, 2, kind, bits, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _at(k_scales), _at(v_scales),
-         out.data_ptr(), tables.data_ptr(), lens.data_ptr(), _at(sinks), B, n, N, page, cols, max_len, H, KH, hd, window, q0, q1, q2,
-         o0, o1, o2, *pool, hd ** -0.5 if scale is None else scale, _at(ws), nbytes)
+    try:
+        record = _ATTEND(2, kind, bits, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), 0 if k_scales is None else k_scales.data_ptr(),
+                         0 if k_scales is None else v_scales.data_ptr(), out.data_ptr(), tables.data_ptr(), lens.data_ptr(),
+                         0 if sinks is None else sinks.data_ptr(), B, n, N, page, cols, max_len, H, KH, hd, window, q0, q1, q2, o0, o1, o2,
+                         *pool, hd ** -0.5 if scale is None else scale, 0 if ws is None else ws.data_ptr(), nbytes, _raw_stream(dev))
+    except (struct.error, OverflowError) as e:
+        _no_number(e)
+    _run(dev, record)
     if given:
         _written(out)
     return out
@@ -422,7 +436,7 @@ def cache_gather(k_pages, v_pages, tables, cu, total, *, k_scales=None, v_scales
             fit = True
         pool = _pool(dev, dtype, k_pages, v_pages, tables, k_scales, v_scales, KH, hd)
         B, cols = tables.shape
-        fit = fit and pool and dev >= 0 and cu is not None and _vector(cu, dev, torch.int32, B + 1)
+        fit = fit and pool and dev >= 0 and cu is not None and _vector(cu, dev, _I32, B + 1)
     except (*_MISFITS, RuntimeError):
         fit = False
     if not fit:
@@ -430,8 +444,13 @@ def cache_gather(k_pages, v_pages, tables, cu, total, *, k_scales=None, v_scales
     if (k_pages.requires_grad or v_pages.requires_grad or ko.requires_grad or vo.requires_grad
             or (k_scales is not None and (k_scales.requires_grad or v_scales.requires_grad))):
         _no_backward()
-    _run(dev, _GATHER, 3, kind, _bits(k_pages), k_pages.data_ptr(), v_pages.data_ptr(), _at(k_scales), _at(v_scales), tables.data_ptr(),
-         cu.data_ptr(), ko.data_ptr(), vo.data_ptr(), total, B, N, page, cols, KH, hd, k0, k1, v0, v1, *pool)
+    try:
+        record = _GATHER(3, kind, 16 if k_scales is None else 8, k_pages.data_ptr(), v_pages.data_ptr(),
+                         0 if k_scales is None else k_scales.data_ptr(), 0 if k_scales is None else v_scales.data_ptr(), tables.data_ptr(),
+                         cu.data_ptr(), ko.data_ptr(), vo.data_ptr(), total, B, N, page, cols, KH, hd, k0, k1, v0, v1, *pool, _raw_stream(dev))
+    except (struct.error, OverflowError) as e:
+        _no_number(e)
+    _run(dev, record)
     if given:
         _written(ko)
         _written(vo)
