@@ -20,12 +20,21 @@
 // weights and one for the accumulators; each warp moves its own only when a
 // score exceeds it by LIFT in base 2.
 //
-// Work: tiles of keys of one (sequence, key head, 16 rows), all in one row cut
-// evenly among persistent CTAs; a CTA's tiles go to its eight warps in turn.
-// Each warp loads its own tiles ahead with cp.async (pages end anywhere, rows
-// that nobody may read come as zeros) and needs no barrier until a unit ends,
-// where the warps' results join in shared memory, and those of units that lie in
-// several CTAs in a second kernel.
+// Work: units are a sequence, a key head and up to 16 rows, their tiles 32 keys
+// (16 of 256-byte rows).  A group of warps walks the tiles of its units, which
+// lie in a row and are cut evenly among the groups, or short ones dealt out whole;
+// a group's tiles go to its warps in turn.  Each warp loads its own tiles ahead
+// with cp.async (pages end anywhere, and rows that nobody may read come as zeros)
+// into places of its own, so no warp waits for another until a unit ends.  There
+// the warps' results join in shared memory, and those of units that lie in
+// several groups in a second kernel.  Nothing spins, and nothing is summed in an
+// order that may change.
+//
+// What bounds it (32 / 4 heads of 128, codes): 256 sequences of 2,048 to 8,192
+// keys, 1.35 GB: 230 us, 0.89 of a copy's rate; a tile takes a warp about 770
+// instructions (loads 160, codes to fp16 130, products 32, softmax 120), 3 of 4
+// issue slots at that rate.  64 sequences of 1 to 4,096: 34 us where the bytes
+// take 20: start and cut 4, units' starts and ends 4, the second kernel 5.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -136,7 +145,7 @@ struct PagedShape {
     return k / 4 * 64 + g * 8 + k % 4 * 2;
   }
   static constexpr int SMEM = WARPS * D * SLOT;
-  static_assert(8 * RP * 4 <= SLOT && D >= 2, "");
+  static_assert(8 * RP * 4 <= SLOT && D >= 2, "8 rows of accumulators lie in a place of the ring");
   // Place of 16-byte word c of row r.  A quarter of a warp reads rows 2 i and
   // 2 i + 1, four words each (K), or words 2 q and 2 q + 1 of rows of one
   // parity (V; half a warp, words of 8 bytes, where rows are 64 bytes): all on
@@ -215,7 +224,7 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
   pdl_wait();
   pdl_trigger();
   // Where this group's tiles begin.
-  PagedWalk wk;
+  PagedWalk wk{};
   long long total;
   int parts;   // the groups that have any
   wk.j = wk.j1 = 0;

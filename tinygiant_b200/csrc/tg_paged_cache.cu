@@ -28,18 +28,21 @@ namespace tg {
 
 constexpr int PC_THREADS = 256;
 constexpr int PC_WARPS = PC_THREADS / 32;
-constexpr int PC_PER_SM = 3;      // CTAs of an SM (4 leave 64 registers, and norms spill: 8,192 tokens x 32 heads rotated in 25 us instead of 22, with norms 37 instead of 33)
+constexpr int PC_PER_SM = 3;      // CTAs of an SM (with 4, and 64 registers: 8,192 tokens x 36 heads rotated in 31 us instead of 26, 2,100 tokens to 8-bit pages 18 instead of 15; keys and values alone 14 instead of 18)
 constexpr int PC_PAIRS = ATTN_MAX_HD / 2;   // pairs of a head, at most
 static_assert(PC_THREADS == 4 * PC_PAIRS, "angles of four tokens at a time");
 constexpr int PC_CU = 1024;       // sequences whose offsets are kept in shared memory
 constexpr int PC_WINDOW = 16;     // packed tokens that a CTA looks through for blocks' first ones, at most
 constexpr int PC_TOKENS = 32;     // tokens of a CTA that rotates, at most
 constexpr int PC_GATHERS = 5;     // gather CTAs of an SM
-constexpr int PC_GATHER = 128;    // tokens of a gather CTA, at most
-constexpr int PC_ROWS = 3;        // rows of a token that a thread has
-constexpr int PC_AHEAD = 3;       // tokens whose rows are there or on their way
-constexpr int PC_RING = PC_AHEAD * PC_ROWS * 2 * 8 * PC_THREADS;
-static_assert(PC_RING >= PAGED_BLOCK * ATTN_MAX_HD * 2 * PC_WARPS, "a warp's run of a head");
+constexpr int PC_GATHER = 32;     // tokens of a gather CTA, at most
+// A thread has R = 2 or 3 rows of a token; pc_ahead tokens' rows are there or on
+// their way.
+template <int R>
+constexpr int pc_ahead = R == 2 ? 4 : 3;
+template <int R>
+constexpr int pc_ring_bytes = pc_ahead<R>* R * 16 * PC_THREADS;
+static_assert(std::min(pc_ring_bytes<2>, pc_ring_bytes<3>) >= PAGED_BLOCK * ATTN_MAX_HD * 2 * PC_WARPS, "a warp's run of a head");
 
 enum { PC_ROTARY, PC_PAGES16, PC_PAGES8 };
 
@@ -55,7 +58,7 @@ struct CacheArgs {
   long long skp[3], svp[3];   // page, head, row; bytes
   long long sks[3], svs[3];   // page, head, block
   long long st;               // tables' row
-  int T, B, per, H, KH, hd, nf, n_pages, cols, shift, token_ctas, window, tokens, parts;
+  int T, B, per, H, KH, hd, nf, n_pages, cols, shift, token_ctas, window, tokens, parts, each;
   int interleaved;
   float amp, eps, inv_hd;   // inv_hd: 1 / hd
 };
@@ -96,33 +99,27 @@ __device__ __forceinline__ float2 pc_mul2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
-template <bool VEC>
-struct Raw {
-  uint32_t w[4];
-};
-template <bool VEC>
-__device__ __forceinline__ void load_pairs(Raw<VEC>& r, const LanePairs& m, const void* row) {
-  const uint16_t* p = static_cast<const uint16_t*>(row);
-  if (VEC) {
-    const uint2 lo = *reinterpret_cast<const uint2*>(p + (m.split ? 4 * m.c : 8 * m.c));
-    const uint2 hi = *reinterpret_cast<const uint2*>(p + (m.split ? m.nf + 4 * m.c : 8 * m.c + 4));
-    r.w[0] = lo.x, r.w[1] = lo.y, r.w[2] = hi.x, r.w[3] = hi.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; i++) r.w[i] = (uint32_t)p[m.low(i)] | (uint32_t)p[m.high(i)] << 16;
-  }
-}
 template <typename T>
 __device__ __forceinline__ float2 halves(uint32_t w) {
   const uint16_t lo = w & 0xffffu, hi = w >> 16;
   return make_float2(to_f32<T>(*reinterpret_cast<const T*>(&lo)), to_f32<T>(*reinterpret_cast<const T*>(&hi)));
 }
+// A lane's pairs of a row in shared memory.
 template <typename T, bool VEC>
-__device__ __forceinline__ void unpack_pairs(Pairs& x, const Raw<VEC>& r, const LanePairs& m) {
-  const float2 y[4] = {halves<T>(r.w[0]), halves<T>(r.w[1]), halves<T>(r.w[2]), halves<T>(r.w[3])};
+__device__ __forceinline__ void read_pairs(Pairs& x, const LanePairs& m, const uint4* row) {
+  const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
   if (VEC && m.split) {
-    x.a[0] = y[0], x.a[1] = y[1], x.b[0] = y[2], x.b[1] = y[3];
+    const uint2 lo = *reinterpret_cast<const uint2*>(p + 4 * m.c), hi = *reinterpret_cast<const uint2*>(p + m.nf + 4 * m.c);
+    x.a[0] = halves<T>(lo.x), x.a[1] = halves<T>(lo.y), x.b[0] = halves<T>(hi.x), x.b[1] = halves<T>(hi.y);
   } else {
+    uint4 w;
+    if (VEC) {
+      w = row[m.c];
+    } else {
+      w.x = (uint32_t)p[m.low(0)] | (uint32_t)p[m.high(0)] << 16, w.y = (uint32_t)p[m.low(1)] | (uint32_t)p[m.high(1)] << 16;
+      w.z = (uint32_t)p[m.low(2)] | (uint32_t)p[m.high(2)] << 16, w.w = (uint32_t)p[m.low(3)] | (uint32_t)p[m.high(3)] << 16;
+    }
+    const float2 y[4] = {halves<T>(w.x), halves<T>(w.y), halves<T>(w.z), halves<T>(w.w)};
     x.a[0] = make_float2(y[0].x, y[1].x), x.b[0] = make_float2(y[0].y, y[1].y);
     x.a[1] = make_float2(y[2].x, y[3].x), x.b[1] = make_float2(y[2].y, y[3].y);
   }
@@ -147,11 +144,9 @@ __device__ __forceinline__ void store_pairs(void* row, const LanePairs& m, const
     }
   }
 }
-// e4m3 codes of a pair, the first in the low byte; NaN where a value is not finite.
+// e4m3 codes of a pair, the first in the low byte; NaN stays, infinities must be gone.
 __device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
   uint16_t d;
-  lo = lo - lo == 0.f ? lo : NAN;
-  hi = hi - hi == 0.f ? hi : NAN;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(hi), "f"(lo));
   return d;
 }
@@ -181,27 +176,39 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const LanePairs& m, cons
   }
 }
 
-// The norm over the LPR lanes of a row (lanes without values have zeros), where
-// `on`; w: the weights in the lanes' order, ones where the norm is off.
-template <int LPR>
-__device__ __forceinline__ void norm_row(Pairs& x, const float* w, const CacheArgs& a, bool on) {
-  float2 q = pc_mul2(x.a[0], x.a[0]);
-  q = at_fma2(x.a[1], x.a[1], q);
-  q = at_fma2(x.b[0], x.b[0], q);
-  q = at_fma2(x.b[1], x.b[1], q);
-  float s = q.x + q.y;
+// `instead` in place of what is not finite.
+__device__ __forceinline__ void only_finite(Pairs& x, float instead) {
+  auto one = [&](float& v) { v = v - v == 0.f ? v : instead; };
 #pragma unroll
-  for (int o = LPR / 2; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-  s = fmaf(s, a.inv_hd, a.eps);
-  float r = rsqrtf(s);
-  r = s > 0.f && r < INFINITY ? fmaf(0.5f * r, fmaf(-s * r, r, 1.f), r) : r;   // a Newton step: half an ulp more exact
-  r = on ? r : 1.f;
-  const float2 rr = make_float2(r, r);
-  const float4 u = reinterpret_cast<const float4*>(w)[0], v = reinterpret_cast<const float4*>(w)[1];
-  x.a[0] = pc_mul2(x.a[0], pc_mul2(rr, make_float2(u.x, u.y)));
-  x.a[1] = pc_mul2(x.a[1], pc_mul2(rr, make_float2(u.z, u.w)));
-  x.b[0] = pc_mul2(x.b[0], pc_mul2(rr, make_float2(v.x, v.y)));
-  x.b[1] = pc_mul2(x.b[1], pc_mul2(rr, make_float2(v.z, v.w)));
+  for (int e = 0; e < 2; e++) one(x.a[e].x), one(x.a[e].y), one(x.b[e].x), one(x.b[e].y);
+}
+// The norm over the LPR lanes of N rows (lanes without values have zeros), where
+// `on` is all ones; where it is 0, w (the weights in the lanes' order) has ones.
+template <int LPR, int N>
+__device__ __forceinline__ void norm_rows(Pairs (&x)[N], const float* w, uint32_t on, const CacheArgs& a) {
+  float s[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    float2 q = pc_mul2(x[i].a[0], x[i].a[0]);
+    q = at_fma2(x[i].a[1], x[i].a[1], q);
+    q = at_fma2(x[i].b[0], x[i].b[0], q);
+    q = at_fma2(x[i].b[1], x[i].b[1], q);
+    s[i] = q.x + q.y;
+  }
+#pragma unroll
+  for (int o = LPR / 2; o; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; i++) s[i] += __shfl_xor_sync(~0u, s[i], o);
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const float r = __uint_as_float((__float_as_uint(rsqrtf(fmaf(s[i], a.inv_hd, a.eps))) & on) | (0x3f800000u & ~on));
+    const float2 rr = make_float2(r, r);
+    const float4 u = *reinterpret_cast<const float4*>(w), v = *reinterpret_cast<const float4*>(w + PC_PAIRS);
+    x[i].a[0] = pc_mul2(x[i].a[0], pc_mul2(rr, make_float2(u.x, u.y)));
+    x[i].a[1] = pc_mul2(x[i].a[1], pc_mul2(rr, make_float2(u.z, u.w)));
+    x[i].b[0] = pc_mul2(x[i].b[0], pc_mul2(rr, make_float2(v.x, v.y)));
+    x[i].b[1] = pc_mul2(x[i].b[1], pc_mul2(rr, make_float2(v.z, v.w)));
+  }
 }
 // cos and sin of a lane's four pairs.
 struct Turns {
@@ -240,8 +247,8 @@ __device__ __forceinline__ const int* keep_offsets(const int* cu, int B, int* s_
   return s_cu;
 }
 
-__device__ __forceinline__ void cp8(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+__device__ __forceinline__ void cp16(uint4* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 static_assert(PC_TOKENS >= PC_WINDOW + PAGED_BLOCK - 1, "both kinds of CTAs' tokens");
 struct CacheShared {
@@ -253,11 +260,11 @@ struct CacheShared {
   int runs, cover;
 };
 __device__ __forceinline__ void keep_weights(const CacheArgs& a, CacheShared& sh) {
-  for (int i = threadIdx.x; i < a.hd; i += PC_THREADS) {   // value i % 8 of lane i / 8: four first ones, four second
-    const int j = i / 8 * 4 + i % 4, second = i % 8 / 4, d = j >= a.nf || a.interleaved ? 2 * j + second : second ? j + a.nf : j;
-    sh.w[0][i] = a.qw ? a.qw[d] : 1.f;
-    sh.w[1][i] = a.kw ? a.kw[d] : 1.f;
-    sh.w[2][i] = 1.f;
+  for (int i = threadIdx.x; i < a.hd; i += PC_THREADS) {   // pairs' first values, and from PC_PAIRS on their second ones
+    const int second = i >= a.hd / 2, j = i - second * (a.hd / 2), at = j + second * PC_PAIRS, d = j >= a.nf || a.interleaved ? 2 * j + second : second ? j + a.nf : j;
+    sh.w[0][at] = a.qw ? a.qw[d] : 1.f;
+    sh.w[1][at] = a.kw ? a.kw[d] : 1.f;
+    sh.w[2][at] = 1.f;
   }
 }
 __device__ __forceinline__ void keep_turn(float (*turn)[PC_PAIRS], int pair, int pos, double f, float amp) {
@@ -266,46 +273,40 @@ __device__ __forceinline__ void keep_turn(float (*turn)[PC_PAIRS], int pair, int
 }
 
 // Rows of nt tokens from t0 on: q, and (tg_rotary, 16-bit pages) k and v.  A row
-// is LPR lanes of 8 values; a thread has the same PC_ROWS rows of every token, of
+// is LPR lanes of 8 values; a thread has the same R rows of every token, of
 // the `part`-th share of a token's rows, and copies those of the next tokens into
 // its own places of a ring in shared memory as it turns this one's.  The angles
 // of four tokens are made together, by all threads, while the four before are
 // turned.
-extern __shared__ uint2 pc_ring[];   // [token % PC_AHEAD][row][half][thread]
-template <typename T, int LPR, bool VEC, int MODE, bool NORM>
+extern __shared__ uint4 pc_ring[];   // [token % pc_ahead][row][thread]: a row is LPR pieces
+template <typename T, int LPR, bool VEC, int MODE, bool NORM, int R>
 __device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, int t0, int nt, int part) {
   const int tid = threadIdx.x;
-  constexpr int ROWS = PC_THREADS / LPR;
+  constexpr int ROWS = PC_THREADS / LPR, AHEAD = pc_ahead<R>;
   const LanePairs m(a, tid % LPR);
   const int rows = a.H + (MODE == PC_PAGES8 ? 0 : a.KH) + (MODE == PC_PAGES16 ? a.KH : 0);
-  const int first = part * PC_ROWS * ROWS + tid / LPR;   // its rows: first, first + ROWS, ..
-  const T* from[PC_ROWS];
-  T* to[PC_ROWS];   // q, tg_rotary's k; the head's place in a page
+  const int first = part * R * ROWS + tid / LPR;   // its rows: first, first + ROWS, ..
+  const T* from[R];
+  T* to[R];   // q, tg_rotary's k; the head's place in a page
+  const float* w[R];
+  uint32_t on[R];
   auto fetch = [&](int t) {
     if (t < nt)
 #pragma unroll
-      for (int i = 0; i < PC_ROWS; i++) {
+      for (int i = 0; i < R; i++) {
         const int r = first + i * ROWS;
-        if (r < rows && m.any()) {
-          const uint32_t at = smem_u32(pc_ring + ((t % PC_AHEAD * PC_ROWS + i) * 2) * PC_THREADS + tid);
-          if (VEC) {
-            cp8(at, from[i] + (m.split ? 4 * m.c : 8 * m.c));
-            cp8(at + 8 * PC_THREADS, from[i] + (m.split ? m.nf + 4 * m.c : 8 * m.c + 4));
-          } else {   // in 2-byte pieces
-            Raw<VEC> raw;
-            load_pairs(raw, m, from[i]);
-            pc_ring[((t % PC_AHEAD * PC_ROWS + i) * 2) * PC_THREADS + tid] = make_uint2(raw.w[0], raw.w[1]);
-            pc_ring[((t % PC_AHEAD * PC_ROWS + i) * 2 + 1) * PC_THREADS + tid] = make_uint2(raw.w[2], raw.w[3]);
-          }
-        }
+        if (r < rows && m.any()) cp16(pc_ring + (t % AHEAD * R + i) * PC_THREADS + tid, from[i] + 8 * m.c);
         from[i] += r < a.H ? a.sq[0] : r < a.H + a.KH ? a.sk[0] : a.sv[0];
       }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
-  for (int i = 0; i < PC_ROWS; i++) {
+  for (int i = 0; i < R; i++) {
     const int r = first + i * ROWS;
     const long long t = t0;
+    const int which = MODE == PC_PAGES8 || r < a.H ? 0 : r < a.H + a.KH ? 1 : 2;
+    w[i] = sh.w[which] + (m.any() ? 4 * m.c : 0);
+    on[i] = (which == 0 && a.qw) || (which == 1 && a.kw) ? ~0u : 0;
     if (r < a.H) {
       from[i] = (const T*)a.q + t * a.sq[0] + r * a.sq[1];
       to[i] = (T*)a.qo + t * a.sqo[0] + r * a.sqo[1];
@@ -318,7 +319,7 @@ __device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, 
     }
   }
 #pragma unroll
-  for (int t = 0; t < PC_AHEAD - 1; t++) fetch(t);
+  for (int t = 0; t < AHEAD - 1; t++) fetch(t);
   const int* cu = MODE == PC_ROTARY ? nullptr : keep_offsets(a.cu, a.B, sh.cu);
   if (NORM) keep_weights(a, sh);
   if (MODE != PC_ROTARY) __syncthreads();
@@ -351,30 +352,28 @@ __device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, 
       __syncthreads();
       angles(t + 4);
     }
-    fetch(t + PC_AHEAD - 1);
-    asm volatile("cp.async.wait_group %0;" ::"n"(PC_AHEAD - 1) : "memory");
+    asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 2) : "memory");
+    __syncwarp();   // the warp's copies of this token are there, the last one's are read
+    fetch(t + AHEAD - 1);
     const Turns turns(sh.turn[t & 7], m);
     const int page = MODE == PC_ROTARY ? -1 : sh.page[t];
 #pragma unroll
-    for (int i = 0; i < PC_ROWS; i++) {
+    for (int i = 0; i < R; i++) {
       const int r = first + i * ROWS;
+      if (r - tid % 32 / LPR >= rows) break;   // none of the warp's
       const bool is_q = r < a.H, is_v = r >= a.H + a.KH, here = r < rows && m.any();
-      Pairs x = no_pairs();
-      if (here) {
-        const uint2* at = pc_ring + ((t % PC_AHEAD * PC_ROWS + i) * 2) * PC_THREADS + tid;
-        const uint2 lo = at[0], hi = at[PC_THREADS];
-        unpack_pairs<T>(x, Raw<VEC>{{lo.x, lo.y, hi.x, hi.y}}, m);
-      }
+      Pairs x[1] = {no_pairs()};
+      if (here) read_pairs<T, VEC>(x[0], m, pc_ring + (t % AHEAD * R + i) * PC_THREADS + tid - m.c);
       if (NORM)   // lanes of rows that have none take part in the sums
-        norm_row<LPR>(x, sh.w[is_q ? 0 : is_v ? 2 : 1] + (m.any() ? 8 * m.c : 0), a, is_q ? a.qw != nullptr : !is_v && a.kw);
+        norm_rows<LPR, 1>(x, w[i], on[i], a);
       if (here) {
-        if (MODE != PC_PAGES16 || !is_v) rotate_pairs<VEC>(x, turns, m);
+        if (MODE != PC_PAGES16 || !is_v) rotate_pairs<VEC>(x[0], turns, m);
         if (MODE != PC_PAGES16 || is_q) {
-          if (page != -2) store_pairs<T, VEC>(to[i], m, x);
+          if (page != -2) store_pairs<T, VEC>(to[i], m, x[0]);
           to[i] += is_q ? a.sqo[0] : a.sko[0];
         } else if (page >= 0) {
           const long long at = is_v ? page * a.svp[0] + sh.row[t] * a.svp[2] : page * a.skp[0] + sh.row[t] * a.skp[2];
-          store_pairs<T, VEC>((uint8_t*)to[i] + at, m, x);
+          store_pairs<T, VEC>((uint8_t*)to[i] + at, m, x[0]);
         }
       }
     }
@@ -384,7 +383,11 @@ __device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, 
 // Runs of 8-bit blocks whose first token is one of the `window` packed tokens
 // from t0 on: a warp has one run's keys or values of a key head.  Its values are
 // worked out twice, for the largest and for the codes: kept in registers they
-// leave room for one CTA of an SM instead of four (8,192 tokens with q 171 us).
+// leave room for one CTA of an SM instead of three (8,192 tokens with q 171 us
+// instead of 47).  Two rows at a time, for their sums' shuffles to overlap.  Keys
+// and values of 4 heads, 8,192 tokens, normed: 18 us; 25 MB to read and write take
+// 4.  As many CTAs as there are SMs' places take 12: what bounds it is how long one
+// takes from its offsets to its scales, and that 512 are one round and a bit.
 template <typename T, int LPR, bool VEC, bool NORM>
 __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& sh, int t0) {
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
@@ -416,23 +419,14 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
   if (!sh.runs) return;
   const LanePairs m(a, lane % LPR);
   const int items = sh.runs * 2 * a.KH;
-  // an item's rows, in this warp's places of the ring: [row / RPP][half][lane]
-  uint2* ring = pc_ring + wid * (PAGED_BLOCK / RPP * 2 * 32) + lane;
+  const uint32_t on = a.kw ? ~0u : 0;
+  uint4* ring = pc_ring + wid * PAGED_BLOCK * LPR;   // an item's rows
   auto fetch = [&](int item) {
     const int i = item / (2 * a.KH), kh = item % (2 * a.KH) >> 1, is_v = item & 1;
     const long long step = is_v ? a.sv[0] : a.sk[0];
     const T* from = (is_v ? (const T*)a.v + kh * a.sv[1] : (const T*)a.k + kh * a.sk[1]) + (t0 + sh.run[i] + lane / LPR) * step;
     for (int u = 0; u * RPP < sh.len[i]; u++, from += RPP * step)
-      if (u * RPP + lane / LPR < sh.len[i] && m.any()) {
-        if (VEC) {
-          cp8(smem_u32(ring + u * 64), from + (m.split ? 4 * m.c : 8 * m.c));
-          cp8(smem_u32(ring + u * 64 + 32), from + (m.split ? m.nf + 4 * m.c : 8 * m.c + 4));
-        } else {
-          Raw<VEC> raw;
-          load_pairs(raw, m, from);
-          ring[u * 64] = make_uint2(raw.w[0], raw.w[1]), ring[u * 64 + 32] = make_uint2(raw.w[2], raw.w[3]);
-        }
-      }
+      if (u * RPP + lane / LPR < sh.len[i] && m.any()) cp16(ring + u * 32 + lane, from + 8 * m.c);
   };
   if (wid < items) fetch(wid);
   if (tid % PC_PAIRS < a.nf) {
@@ -449,32 +443,42 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
     float* scale_at = is_v ? a.vs + sh.page[i] * a.svs[0] + kh * a.svs[1] + block * a.svs[2]
                            : a.ks + sh.page[i] * a.sks[0] + kh * a.sks[1] + block * a.sks[2];
     const float before = off ? *scale_at : 0.f;
-    asm volatile("cp.async.wait_all;" ::: "memory");   // each lane reads what it copied itself
-    auto values = [&](int u) {   // of row u RPP + lane / LPR; zeros where there is none
-      const int j = u * RPP + lane / LPR;
-      const bool here = j < n && m.any();
-      Pairs x = no_pairs();
-      if (here) {
-        const uint2 lo = ring[u * 64], hi = ring[u * 64 + 32];
-        unpack_pairs<T>(x, Raw<VEC>{{lo.x, lo.y, hi.x, hi.y}}, m);
-      }
-      if (is_v) return x;
-      if (NORM) norm_row<LPR>(x, sh.w[1] + (m.any() ? 8 * m.c : 0), a, a.kw != nullptr);
-      if (here) rotate_pairs<VEC>(x, Turns(sh.turn[j0 + j], m), m);
-      return x;
-    };
-    uint32_t amax = 0;   // bits of the largest finite magnitude
-#pragma unroll 4
-    for (int u = 0; u * RPP < n; u++) {
-      const Pairs x = values(u);
-      auto most = [&](float v) {
-        const uint32_t y = __float_as_uint(v) & 0x7fffffffu;
-        amax = max(amax, y < 0x7f800000u ? y : 0u);
-      };
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();
+    auto values = [&](int u, Pairs (&x)[2]) {   // of the rows u RPP + lane / LPR and RPP on; zeros where there is none
 #pragma unroll
-      for (int e = 0; e < 2; e++) most(x.a[e].x), most(x.a[e].y), most(x.b[e].x), most(x.b[e].y);
+      for (int i = 0; i < 2; i++) {
+        x[i] = no_pairs();
+        if ((u + i) * RPP + lane / LPR < n && m.any()) read_pairs<T, VEC>(x[i], m, ring + ((u + i) * RPP + lane / LPR) * LPR);
+      }
+      if (is_v) return;
+      if (NORM) norm_rows<LPR, 2>(x, sh.w[1] + (m.any() ? 4 * m.c : 0), on, a);
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const int j = (u + i) * RPP + lane / LPR;
+        if (j < n && m.any()) rotate_pairs<VEC>(x[i], Turns(sh.turn[j0 + j], m), m);
+      }
+    };
+    uint32_t amax;      // bits of the largest finite magnitude
+    bool odd = false;   // a value is infinite
+    for (;;) {
+      float most = 0.f;   // NaN is less than any number here
+#pragma unroll 1
+      for (int u = 0; u * RPP < n; u += 2) {
+        Pairs x[2];
+        values(u, x);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          if (odd) only_finite(x[i], 0.f);
+#pragma unroll
+          for (int e = 0; e < 2; e++)
+            most = fmaxf(fmaxf(most, fmaxf(fabsf(x[i].a[e].x), fabsf(x[i].a[e].y))), fmaxf(fabsf(x[i].b[e].x), fabsf(x[i].b[e].y)));
+        }
+      }
+      amax = __reduce_max_sync(~0u, __float_as_uint(most));
+      if (odd || amax < 0x7f800000u) break;
+      odd = true;
     }
-    amax = __reduce_max_sync(~0u, amax);
     const float need = __uint_as_float((uint32_t)(paged_scale_exp(amax) + 127) << 23);
     const float scale = fmaxf(need, before), inv = 1.f / scale;
     if (off && scale > before) {   // the earlier tokens' codes under the larger scale
@@ -489,23 +493,35 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
         *at = make_uint2(four(w.x), four(w.y));
       }
     }
-#pragma unroll 2
-    for (int u = 0; u * RPP < n; u++) {
-      const int j = u * RPP + lane / LPR;
-      Pairs x = values(u);
-      if (j < n && m.any()) {
-        const float2 f = make_float2(inv, inv);
+#pragma unroll 1
+    for (int u = 0; u * RPP < n; u += 2) {
+      Pairs x[2];
+      values(u, x);
 #pragma unroll
-        for (int e = 0; e < 2; e++) x.a[e] = pc_mul2(x.a[e], f), x.b[e] = pc_mul2(x.b[e], f);
-        store_codes<VEC>(rows + (off + j) * pitch, m, x);
+      for (int i = 0; i < 2; i++) {
+        const int j = (u + i) * RPP + lane / LPR;
+        if (j < n && m.any()) {
+          const float2 f = make_float2(inv, inv);
+          if (odd) only_finite(x[i], NAN);
+#pragma unroll
+          for (int e = 0; e < 2; e++) x[i].a[e] = pc_mul2(x[i].a[e], f), x[i].b[e] = pc_mul2(x[i].b[e], f);
+          store_codes<VEC>(rows + (off + j) * pitch, m, x[i]);
+        }
       }
     }
     if (lane == 0) *scale_at = scale;
+    __syncwarp();   // all have read the rows
     if (item + PC_WARPS < items) fetch(item + PC_WARPS);
   }
 }
 
-template <typename T, int LPR, bool VEC, int MODE, bool NORM>
+// Rows of tokens and, beside them in the same launch, runs of 8-bit blocks, so that
+// the copies of the one overlap the instructions of the other.  Measured in a
+// replayed graph, bf16, heads of 128: 8,192 tokens x 32 heads rotated 21 us (0.97 of
+// a copy's rate, part of it from L2: bytes bound it), with norms 27 (instructions);
+// the same with 4 key heads to 8-bit pages 39, without norms 29, where 160 MB take
+// 24.  A chunk of 2,100 tokens 15; two tokens 4, of which an empty kernel is 2.
+template <typename T, int LPR, bool VEC, int MODE, bool NORM, int R>
 __global__ void __launch_bounds__(PC_THREADS, PC_PER_SM) cache_kernel(const CacheArgs a) {
   __shared__ CacheShared sh;
   pdl_wait();
@@ -513,7 +529,7 @@ __global__ void __launch_bounds__(PC_THREADS, PC_PER_SM) cache_kernel(const Cach
     runs_of_blocks<T, LPR, VEC, NORM>(a, sh, (blockIdx.x - a.token_ctas) * a.window);
   } else {
     const int t0 = blockIdx.x / a.parts * a.tokens;
-    token_rows<T, LPR, VEC, MODE, NORM>(a, sh, t0, min(a.tokens, a.T - t0), blockIdx.x % a.parts);
+    token_rows<T, LPR, VEC, MODE, NORM, R>(a, sh, t0, min(a.tokens, a.T - t0), blockIdx.x % a.parts);
   }
 }
 
@@ -521,17 +537,23 @@ struct GatherArgs {
   const uint8_t *kp, *vp;
   const float *ks, *vs;
   const int *tables, *cu;
-  void *ko, *vo;
-  long long skp[3], svp[3], sks[3], svs[3], sko[2], svo[2], st;
+  uint8_t *ko, *vo;
+  unsigned skp[3], svp[3];    // page, head, row; 16-byte words
+  unsigned sks[3], svs[3];    // page, head, block
+  unsigned sko[2], svo[2];    // token, head; 16-byte words
+  long long st;
   int T, B, KH, hd, n_pages, cols, shift;
   int wide;   // outputs in 32-byte pieces: rows start on 32-byte boundaries
 };
 
-// Rows of the packed outputs, 16 bytes of a page's row at a time, four of them
-// loaded before the first is stored.  A CTA has `per` tokens.
+// Rows of the packed outputs, 16 bytes of a page's row at a time, three of them
+// loaded before the first is stored.  A CTA has `per` tokens; a thread goes
+// through their rows (K of all heads, then V, of each token) without divisions,
+// and strides are 32-bit numbers of 16-byte words: with 64-bit products the
+// kernel was bound by its instructions (185 for 32 x 16 values, 38 us).
 template <typename T, bool CODES>
 __global__ void __launch_bounds__(PC_THREADS, PC_GATHERS) gather_pages_kernel(const GatherArgs a, int lpr, int per) {
-  constexpr int N = 4;
+  constexpr int N = 3;
   __shared__ int s_cu[PC_CU + 1], s_page[PC_GATHER], s_row[PC_GATHER];
   pdl_wait();
   const int tid = threadIdx.x, t0 = blockIdx.x * per;
@@ -544,28 +566,35 @@ __global__ void __launch_bounds__(PC_THREADS, PC_GATHERS) gather_pages_kernel(co
     s_row[tid] = p & ((1 << a.shift) - 1);
   }
   __syncthreads();
-  const int c = tid % lpr, chunks = a.hd / (CODES ? 16 : 8);
-  if (c >= chunks) return;
-  const int rows = min(per, a.T - t0) * 2 * a.KH, step = PC_THREADS / lpr;
-  for (int r0 = tid / lpr; r0 < rows; r0 += N * step) {
+  const int c = tid % lpr, heads = 2 * a.KH, tokens = min(per, a.T - t0), step = PC_THREADS / lpr;
+  if (c * (CODES ? 16 : 8) >= a.hd) return;
+  const int dj = step / heads, dh = step % heads;
+  int j = tid / lpr / heads, h = tid / lpr % heads;   // the thread's row: token and head
+  while (j < tokens) {
     uint4 w[N];
     float scale[N];
-    T* to[N];
+    uint8_t* to[N];
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      const int r = r0 + i * step;
       to[i] = nullptr;
-      w[i] = make_uint4(0, 0, 0, 0);
-      scale[i] = 0.f;
-      if (r >= rows) continue;
-      const int j = r / (2 * a.KH), h = r % (2 * a.KH), is_v = h >= a.KH, kh = is_v ? h - a.KH : h, page = s_page[j], row = s_row[j];
-      if (page == -2) continue;
-      to[i] = (is_v ? (T*)a.vo + (t0 + j) * a.svo[0] + kh * a.svo[1] : (T*)a.ko + (t0 + j) * a.sko[0] + kh * a.sko[1]) + c * (CODES ? 16 : 8);
-      if (page < 0) continue;
-      w[i] = *reinterpret_cast<const uint4*>(is_v ? a.vp + page * a.svp[0] + kh * a.svp[1] + row * a.svp[2] + c * 16
-                                                  : a.kp + page * a.skp[0] + kh * a.skp[1] + row * a.skp[2] + c * 16);
-      if (CODES) scale[i] = is_v ? a.vs[page * a.svs[0] + kh * a.svs[1] + row / PAGED_BLOCK * a.svs[2]]
-                                 : a.ks[page * a.sks[0] + kh * a.sks[1] + row / PAGED_BLOCK * a.sks[2]];
+      if (j < tokens && s_page[j] != -2) {
+        const int page = s_page[j];
+        const bool is_v = h >= a.KH;
+        const unsigned kh = is_v ? h - a.KH : h, row = s_row[j];
+        to[i] = (is_v ? a.vo : a.ko) + 16 * ((uint64_t)(unsigned)(t0 + j) * (is_v ? a.svo[0] : a.sko[0]) + (uint64_t)kh * (is_v ? a.svo[1] : a.sko[1]) +
+                                             c * (CODES ? 2 : 1));
+        w[i] = make_uint4(0, 0, 0, 0);
+        scale[i] = 0.f;
+        if (page >= 0) {
+          w[i] = *reinterpret_cast<const uint4*>((is_v ? a.vp : a.kp) + 16 * ((uint64_t)(unsigned)page * (is_v ? a.svp[0] : a.skp[0]) +
+                                                                              (uint64_t)row * (is_v ? a.svp[2] : a.skp[2]) + (uint64_t)kh * (is_v ? a.svp[1] : a.skp[1]) + c));
+          if (CODES)
+            scale[i] = (is_v ? a.vs : a.ks)[(uint64_t)(unsigned)page * (is_v ? a.svs[0] : a.sks[0]) + (uint64_t)(row / PAGED_BLOCK) * (is_v ? a.svs[2] : a.sks[2]) +
+                                            (uint64_t)kh * (is_v ? a.svs[1] : a.sks[1])];
+        }
+      }
+      j += dj, h += dh;
+      if (h >= heads) h -= heads, j++;
     }
 #pragma unroll
     for (int i = 0; i < N; i++) {
@@ -573,9 +602,10 @@ __global__ void __launch_bounds__(PC_THREADS, PC_GATHERS) gather_pages_kernel(co
       if (!CODES) {
         *reinterpret_cast<uint4*>(to[i]) = w[i];
       } else {
+        const float2 f = make_float2(scale[i], scale[i]);
         auto two = [&](uint32_t code) {
-          const float2 v = e4m3_values(code);
-          return at_pack<T>(v.x * scale[i], v.y * scale[i]);
+          const float2 v = pc_mul2(e4m3_values(code), f);
+          return at_pack<T>(v.x, v.y);
         };
         const uint32_t y[8] = {two(w[i].x), two(w[i].x >> 16), two(w[i].y), two(w[i].y >> 16),
                                two(w[i].z), two(w[i].z >> 16), two(w[i].w), two(w[i].w >> 16)};
@@ -590,22 +620,23 @@ __global__ void __launch_bounds__(PC_THREADS, PC_GATHERS) gather_pages_kernel(co
   }
 }
 
-template <typename T, int LPR, bool VEC, int MODE, bool NORM>
+template <typename T, int LPR, bool VEC, int MODE, bool NORM, int R>
 static cudaError_t launch_cache(const CacheArgs& a, int grid, cudaStream_t s) {
   static std::atomic<unsigned long long> set{0};
-  const cudaError_t e = attn_smem(cache_kernel<T, LPR, VEC, MODE, NORM>, PC_RING, set);
-  return e == cudaSuccess ? launch_pdl(cache_kernel<T, LPR, VEC, MODE, NORM>, dim3(grid), PC_THREADS, PC_RING, s, a) : e;
+  const cudaError_t e = attn_smem(cache_kernel<T, LPR, VEC, MODE, NORM, R>, pc_ring_bytes<R>, set);
+  return e == cudaSuccess ? launch_pdl(cache_kernel<T, LPR, VEC, MODE, NORM, R>, dim3(grid), PC_THREADS, pc_ring_bytes<R>, s, a) : e;
 }
-template <typename T, int MODE, bool NORM>
+template <typename T, int MODE, bool NORM, int R>
 static cudaError_t launch_cache(const CacheArgs& a, int grid, cudaStream_t s) {
   const bool vec = a.nf % 4 == 0;
-  if (a.hd <= 64) return vec ? launch_cache<T, 8, true, MODE, NORM>(a, grid, s) : launch_cache<T, 8, false, MODE, NORM>(a, grid, s);
-  return vec ? launch_cache<T, 16, true, MODE, NORM>(a, grid, s) : launch_cache<T, 16, false, MODE, NORM>(a, grid, s);
+  if (a.hd <= 64) return vec ? launch_cache<T, 8, true, MODE, NORM, R>(a, grid, s) : launch_cache<T, 8, false, MODE, NORM, R>(a, grid, s);
+  return vec ? launch_cache<T, 16, true, MODE, NORM, R>(a, grid, s) : launch_cache<T, 16, false, MODE, NORM, R>(a, grid, s);
 }
 template <typename T, int MODE>
 static cudaError_t launch_cache(const CacheArgs& a, int grid, cudaStream_t s) {
   count_launches(1);
-  return a.qw || a.kw ? launch_cache<T, MODE, true>(a, grid, s) : launch_cache<T, MODE, false>(a, grid, s);
+  if (a.qw || a.kw) return a.each == 2 ? launch_cache<T, MODE, true, 2>(a, grid, s) : launch_cache<T, MODE, true, 3>(a, grid, s);
+  return a.each == 2 ? launch_cache<T, MODE, false, 2>(a, grid, s) : launch_cache<T, MODE, false, 3>(a, grid, s);
 }
 
 }  // namespace tg
@@ -614,11 +645,15 @@ using namespace tg;
 
 namespace tg {
 
-// The CTAs that rotate: shares of `rows` rows of a token, and tokens of a CTA so
-// that the SMs have them all at once, or as few times in a row as PC_TOKENS allow.
+// The CTAs that rotate: rows of a thread (two, where that takes no more rounds over
+// a token's rows: 32 heads of 128, 8,192 tokens, normed 27 us instead of 29; 36 in
+// two shares of two 33 instead of 28), shares of a token's rows, and tokens of a CTA
+// so that the SMs have them all at once, or as few times in a row as PC_TOKENS allow.
 static long long token_ctas(CacheArgs& a, long long rows, int per_sm) {
-  const int share = PC_ROWS * PC_THREADS / (a.hd <= 64 ? 8 : 16), most = attn_sms() * per_sm;
-  a.parts = (int)((rows + share - 1) / share);
+  const int once = PC_THREADS / (a.hd <= 64 ? 8 : 16), most = attn_sms() * per_sm;
+  const long long by2 = (rows + 2 * once - 1) / (2 * once), by3 = (rows + 3 * once - 1) / (3 * once);
+  a.each = 2 * by2 <= 3 * by3 ? 2 : 3;
+  a.parts = (int)(a.each == 2 ? by2 : by3);
   const long long work = (long long)a.T * a.parts, waves = (work + (long long)most * PC_TOKENS - 1) / ((long long)most * PC_TOKENS);
   a.tokens = (int)((work + most * waves - 1) / (most * waves));
   return (long long)((a.T + a.tokens - 1) / a.tokens) * a.parts;
@@ -700,6 +735,7 @@ static int append(ArgCheck& c, const AppendRecord& r) {
   a.nf = (int)r.n_freqs, a.n_pages = (int)r.n_pages, a.cols = (int)r.table_cols, a.shift = pool.shift;
   a.interleaved = r.interleaved != 0, a.amp = (float)r.amplitude, a.eps = (float)r.eps, a.inv_hd = 1.f / a.hd;
   long long ctas = r.page_bits == 16 ? token_ctas(a, (long long)a.H + 2 * a.KH, PC_PER_SM) : a.H ? token_ctas(a, a.H, PC_PER_SM - 1) : 0;
+  if (!ctas) a.each = 2;
   if (r.page_bits == 8) {   // the runs' CTAs behind: one of them beside those that rotate, on each SM
     a.token_ctas = (int)ctas;
     a.window = 1;
@@ -725,7 +761,10 @@ static int gather(ArgCheck& c, const GatherRecord& r) {
   const PoolCheck pool(c, (int)r.page_bits, (int)r.n_pages, (int)r.page, (int)r.table_cols, (int)r.batch, (int)r.n_kv_heads, (int)r.head_dim,
                        r.strides + 4);
   long long t[4];
-  for (int i = 0; i < 4; i++) t[i] = c.stride(r.strides[i], i % 2 == 0 ? r.total : r.n_kv_heads);
+  for (int i = 0; i < 4; i++) {
+    t[i] = c.stride(r.strides[i], i % 2 == 0 ? r.total : r.n_kv_heads);
+    c.need(t[i] < 1ll << 35, "strides of the outputs must be below 2^35 elements");
+  }
   if (c.rc || r.total == 0 || r.batch == 0) return c.rc;
   if (!c.device()) return c.rc;
   c.ptr(r.cu, 4, "cu"), c.ptr(r.k_out, 16, "k_out"), c.ptr(r.v_out, 16, "v_out");
@@ -735,18 +774,22 @@ static int gather(ArgCheck& c, const GatherRecord& r) {
   if (c.rc) return c.rc;
   GatherArgs a{};
   a.kp = (const uint8_t*)r.k_pages, a.vp = (const uint8_t*)r.v_pages, a.ks = (const float*)r.k_scales, a.vs = (const float*)r.v_scales;
-  a.tables = (const int*)r.tables, a.cu = (const int*)r.cu, a.ko = r.k_out, a.vo = r.v_out;
-  for (int i = 0; i < 3; i++) a.skp[i] = pool.kp[i], a.svp[i] = pool.vp[i], a.sks[i] = pool.ks[i], a.svs[i] = pool.vs[i];
-  for (int i = 0; i < 2; i++) a.sko[i] = t[i], a.svo[i] = t[2 + i];
+  a.tables = (const int*)r.tables, a.cu = (const int*)r.cu, a.ko = (uint8_t*)r.k_out, a.vo = (uint8_t*)r.v_out;
+  for (int i = 0; i < 3; i++) {
+    a.skp[i] = (unsigned)(pool.kp[i] / 16), a.svp[i] = (unsigned)(pool.vp[i] / 16);
+    a.sks[i] = (unsigned)pool.ks[i], a.svs[i] = (unsigned)pool.vs[i];
+  }
+  for (int i = 0; i < 2; i++) a.sko[i] = (unsigned)(t[i] / 8), a.svo[i] = (unsigned)(t[2 + i] / 8);
   a.st = pool.st, a.T = (int)r.total, a.B = (int)r.batch, a.KH = (int)r.n_kv_heads, a.hd = (int)r.head_dim, a.n_pages = (int)r.n_pages;
   a.cols = (int)r.table_cols, a.shift = pool.shift;
   a.wide = ((uintptr_t)r.k_out | (uintptr_t)r.v_out) % 32 == 0 && (t[0] | t[1] | t[2] | t[3]) % 16 == 0;
   int lpr = 1;
   while (lpr < a.hd / (r.page_bits == 8 ? 16 : 8)) lpr *= 2;
-  // tokens of a CTA, so that the SMs have all CTAs at once, or as few times in a
-  // row as PC_GATHER allows (62,342 rows, 191 MB: 64 tokens, 1.3 times as many
-  // CTAs as fit, 38 us)
-  const int most = attn_sms() * PC_GATHERS, waves = (int)(((long long)a.T + most * PC_GATHER - 1) / (most * PC_GATHER)), per = (int)std::max(4ll, ((long long)a.T + (long long)most * waves - 1) / ((long long)most * waves));
+  // tokens of a CTA, at least 4: as many as give every SM the same number of full
+  // rounds of CTAs (62,342 rows of 8 heads, 191 MB: three rounds of 29 tokens 36
+  // us, one of 85 38; a copy of as many bytes takes 33)
+  const long long most = attn_sms() * PC_GATHERS, waves = (a.T + most * PC_GATHER - 1) / (most * PC_GATHER);
+  const int per = (int)std::max(4ll, (a.T + most * waves - 1) / (most * waves));
   const dim3 grid((a.T + per - 1) / per);
   cudaStream_t s = static_cast<cudaStream_t>(r.stream);
   const bool bf = r.dtype == ATTN_BF16;
