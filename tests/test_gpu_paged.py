@@ -905,3 +905,14 @@ def test_a_batch_from_prompts_to_drafts(P, codes):
     for b in range(B):
         pool.tables[b, :(lens[b] - 50) // page] = -1
     assert torch.equal(P.attention_paged(q, pool.k, pool.v, pool.tables, pool.lens, **pool.kw, window=50), before)
+
+
+@pytest.mark.parametrize("bits,window", [("8", "0"), ("16", "0"), ("8", "200")])
+def test_serving_example(gpu, bits, window):
+    """Prompts in chunks, drafts, pages given back and the experts' steps through examples/serve_paged.py, the last attention checked."""
+    import importlib.util
+    from pathlib import Path
+    spec = importlib.util.spec_from_file_location("serve_paged", Path(__file__).resolve().parents[1] / "examples" / "serve_paged.py")
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    assert mod.main(["--batch", "3", "--chunk", "200", "--steps", "12", "--page", "32", "--bits", bits, "--window", window]) < 2e-2
