@@ -916,3 +916,52 @@ def test_serving_example(gpu, bits, window):
     mod = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(mod)
     assert mod.main(["--batch", "3", "--chunk", "200", "--steps", "12", "--page", "32", "--bits", bits, "--window", window]) < 2e-2
+
+
+# heads, kv heads, head_dim: two and three rows of a thread, in one share of a token's rows and in several
+@pytest.mark.parametrize("norms", [False, True])
+@pytest.mark.parametrize("codes", [True, False], ids=["8bit", "16bit"])
+@pytest.mark.parametrize("H,KH,hd", [(8, 2, 64), (32, 4, 128), (40, 4, 128), (140, 4, 96), (0, 2, 128)])
+def test_many_tokens_equal_few_at_a_time(P, H, KH, hd, codes, norms):
+    """Thousands of tokens in one call give the bits of calls that each hold a token or two of a CTA."""
+    g, T, step = gen(31), 2803, 160
+    pool = Pool(g, torch.bfloat16, codes, KH, hd, 32, [T + 48])
+    few = pool.clone()
+    q, k, v = rand(g, T, H + 2 * KH, hd, dtype=torch.bfloat16, scale=3.0).split([H, KH, KH], 1)
+    w = [1 + 0.3 * torch.randn(hd, generator=g, device="cuda") if norms else None for _ in range(2)]
+    kw = {"freqs": P.rotary_frequencies(hd, device="cuda")[0], "q_norm": w[0] if H else None, "k_norm": w[1]}
+    out = P.cache_append(k, v, pool.k, pool.v, pool.tables, pool.lens, **pool.kw, **kw, q=q if H else None)
+    pos = torch.arange(48, T + 48, device="cuda").int()
+    turned = P.rotary(q, k, pos, **kw) if H else P.rotary(k, None, pos, kw["freqs"], q_norm=w[1])[::-1]
+    assert not H or torch.equal(out, turned[0])
+    for a in range(0, T, step):
+        b = min(T, a + step)
+        y = P.cache_append(k[a:b], v[a:b], few.k, few.v, few.tables, ints(b + 48), **few.kw, **kw, q=q[a:b] if H else None)
+        z = P.rotary(k[a:b], None, pos[a:b], kw["freqs"], q_norm=w[1])[0]
+        assert (not H or torch.equal(y, out[a:b])) and torch.equal(z, turned[1][a:b])
+    assert torch.equal(bits(pool.k), bits(few.k)) and torch.equal(bits(pool.v), bits(few.v))
+    assert not codes or (torch.equal(pool.ks, few.ks) and torch.equal(pool.vs, few.vs))
+    if not codes:
+        row = (pool.tables[0].long()[pos.long() // 32], pos.long() % 32)
+        assert torch.equal(pool.k.transpose(1, 2)[row], turned[1]) and torch.equal(pool.v.transpose(1, 2)[row], v)
+
+
+@pytest.mark.parametrize("codes", [True, False], ids=["8bit", "16bit"])
+def test_more_sequences_than_a_cta_keeps_offsets_of(P, codes):
+    """1,500 sequences of none to three new tokens, in one call and in two; and read back."""
+    g, B, KH, hd = gen(32), 1500, 2, 64
+    new = [(7 * b) % 4 for b in range(B)]
+    lens = [16 * (b % 3) + n for b, n in enumerate(new)]
+    pool = Pool(g, torch.bfloat16, codes, KH, hd, 16, lens)
+    two, T, half = pool.clone(), sum(new), sum(new[:B // 2])
+    k, v = rand(g, T, KH, hd, dtype=torch.bfloat16), rand(g, T, KH, hd, dtype=torch.bfloat16)
+    f = P.rotary_frequencies(hd, device="cuda")[0]
+    P.cache_append(k, v, pool.k, pool.v, pool.tables, pool.lens, ends(new), **pool.kw, freqs=f)
+    for rows, seqs in ((slice(0, half), slice(0, B // 2)), (slice(half, T), slice(B // 2, B))):
+        P.cache_append(k[rows], v[rows], two.k, two.v, two.tables[seqs], two.lens[seqs], ends(new[seqs]), **two.kw, freqs=f)
+    assert torch.equal(bits(pool.k), bits(two.k)) and torch.equal(bits(pool.v), bits(two.v))
+    keys, vals = P.cache_gather(pool.k, pool.v, pool.tables, ends(lens), sum(lens), **pool.kw)
+    at = [0, *np.cumsum(lens).tolist()]
+    for b in range(0, B, 97):
+        assert torch.equal(keys[at[b]:at[b + 1]].double(), pool.values("k", b, lens[b]).transpose(0, 1).to(torch.bfloat16).double())
+        assert torch.equal(vals[at[b]:at[b + 1]].double(), pool.values("v", b, lens[b]).transpose(0, 1).to(torch.bfloat16).double())
