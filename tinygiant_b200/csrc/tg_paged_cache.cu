@@ -28,7 +28,7 @@ namespace tg {
 
 constexpr int PC_THREADS = 256;
 constexpr int PC_WARPS = PC_THREADS / 32;
-constexpr int PC_PER_SM = 3;      // CTAs of an SM (with 4, and 64 registers: 8,192 tokens x 36 heads rotated in 31 us instead of 26, 2,100 tokens to 8-bit pages 18 instead of 15; keys and values alone 14 instead of 18)
+constexpr int PC_PER_SM = 3;      // CTAs of an SM (with 4, and 64 registers: 8,192 tokens x 36 heads rotated in 31 us instead of 26, 2,048 tokens to 8-bit pages 18 instead of 15; keys and values alone 14 instead of 18)
 constexpr int PC_PAIRS = ATTN_MAX_HD / 2;   // pairs of a head, at most
 static_assert(PC_THREADS == 4 * PC_PAIRS, "angles of four tokens at a time");
 constexpr int PC_CU = 1024;       // sequences whose offsets are kept in shared memory
@@ -520,7 +520,7 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
 // replayed graph, bf16, heads of 128: 8,192 tokens x 32 heads rotated 21 us (0.97 of
 // a copy's rate, part of it from L2: bytes bound it), with norms 27 (instructions);
 // the same with 4 key heads to 8-bit pages 39, without norms 29, where 160 MB take
-// 24.  A chunk of 2,100 tokens 15; two tokens 4, of which an empty kernel is 2.
+// 24.  A chunk of 2,048 tokens 15; two tokens 4, of which an empty kernel is 2.
 template <typename T, int LPR, bool VEC, int MODE, bool NORM, int R>
 __global__ void __launch_bounds__(PC_THREADS, PC_PER_SM) cache_kernel(const CacheArgs a) {
   __shared__ CacheShared sh;
@@ -786,7 +786,7 @@ static int gather(ArgCheck& c, const GatherRecord& r) {
   int lpr = 1;
   while (lpr < a.hd / (r.page_bits == 8 ? 16 : 8)) lpr *= 2;
   // tokens of a CTA, at least 4: as many as give every SM the same number of full
-  // rounds of CTAs (62,342 rows of 8 heads, 191 MB: three rounds of 29 tokens 36
+  // rounds of CTAs (62,346 rows of 4 key heads, 191 MB: three rounds of 29 tokens 36
   // us, one of 85 38; a copy of as many bytes takes 33)
   const long long most = attn_sms() * PC_GATHERS, waves = (a.T + most * PC_GATHER - 1) / (most * PC_GATHER);
   const int per = (int)std::max(4ll, (a.T + most * waves - 1) / (most * waves));
