@@ -965,3 +965,25 @@ def test_more_sequences_than_a_cta_keeps_offsets_of(P, codes):
     for b in range(0, B, 97):
         assert torch.equal(keys[at[b]:at[b + 1]].double(), pool.values("k", b, lens[b]).transpose(0, 1).to(torch.bfloat16).double())
         assert torch.equal(vals[at[b]:at[b + 1]].double(), pool.values("v", b, lens[b]).transpose(0, 1).to(torch.bfloat16).double())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("hd,n,inter,norm", [(128, 64, False, True), (64, 32, True, False), (80, 20, False, True), (96, 47, False, False), (128, 0, False, True)])
+def test_codes_are_the_exact_values_rounded(P, hd, n, inter, norm, dtype):
+    """Hundreds of thousands of codes of normed and rotated keys: the 64-bit values' nearest, none decided by fp32's rounding."""
+    g, T, KH = gen(41), 1024, 4
+    pool = Pool(g, DT[dtype], True, KH, hd, 64, [T])
+    k = rand(g, T, KH, hd, dtype=DT[dtype], scale=2.0)
+    f = P.rotary_frequencies(2 * n, 1e6, device="cuda")[0] if n else None
+    w = 1 + 0.3 * torch.randn(hd, generator=g, device="cuda") if norm else None
+    P.cache_append(k, k, pool.k, pool.v, pool.tables, pool.lens, **pool.kw, freqs=f, interleaved=inter, k_norm=w)
+    want, _ = rotate64(k, torch.arange(T, device="cuda"), f, inter, 1.0, w)
+    scale, _ = P.cache_gather(torch.ones_like(pool.k.float()).to(E4M3), pool.v, pool.tables, ints(0, T), T, k_scales=pool.ks, v_scales=pool.vs,
+                              dtype=torch.bfloat16)
+    y = want / scale.double()
+    y32 = y.float()
+    short = torch.where(y32.double().abs() > y.abs(), torch.nextafter(y32, torch.zeros_like(y32)), y32)      # towards zero
+    odd = torch.where(short.double() == y, short.view(torch.int32), short.view(torch.int32) | 1).view(torch.float32)
+    p = torch.arange(T, device="cuda")
+    codes = pool.k.transpose(1, 2)[pool.tables[0].long()[p // 64], p % 64]
+    assert torch.equal(bits(codes), bits(odd.to(E4M3)))

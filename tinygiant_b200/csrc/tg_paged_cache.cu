@@ -63,16 +63,16 @@ struct CacheArgs {
   float amp, eps, inv_hd;   // inv_hd: 1 / hd
 };
 
-// cos and sin of p f radians, times amp, rounded once: Taylor's series at an
-// eighth of a turn at most, off by 2^-33.
-__device__ __forceinline__ float2 rope_angle(int p, double f, float amp) {
+// cos and sin of p f radians, times amp: Taylor's series at an eighth of a turn at
+// most, off by 2^-33.
+__device__ __forceinline__ double2 rope_angle(int p, double f, float amp) {
   const double t = (double)p * (f * 0.15915494309189533577);   // turns
   const double n = rint(4.0 * t), x = 6.2831853071795864769 * (t - 0.25 * n), y = x * x;
   const double s = amp * x * (1 + y * (-1.0 / 6 + y * (1.0 / 120 + y * (-1.0 / 5040 + y * (1.0 / 362880)))));
   const double c = amp * (1 + y * (-1.0 / 2 + y * (1.0 / 24 + y * (-1.0 / 720 + y * (1.0 / 40320 - y * (1.0 / 3628800))))));
   const int quarter = (int)((long long)n & 3);
-  const float cs = (float)(quarter & 1 ? -s : c), sn = (float)(quarter & 1 ? c : s);
-  return quarter & 2 ? make_float2(-cs, -sn) : make_float2(cs, sn);
+  const double cs = quarter & 1 ? -s : c, sn = quarter & 1 ? c : s;
+  return quarter & 2 ? make_double2(-cs, -sn) : make_double2(cs, sn);
 }
 
 // Eight values of a row are a lane's: the pairs 4 c .. 4 c + 3 of the row's hd / 2.
@@ -155,24 +155,23 @@ __device__ __forceinline__ float2 e4m3_values(uint32_t two) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)two));
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
+// A lane's codes: of its pairs' first values, and of their second ones.
+struct Codes {
+  uint32_t a, b;
+};
+__device__ __forceinline__ Codes codes_of(const Pairs& x) {
+  return {e4m3_pair(x.a[0].x, x.a[0].y) | e4m3_pair(x.a[1].x, x.a[1].y) << 16, e4m3_pair(x.b[0].x, x.b[0].y) | e4m3_pair(x.b[1].x, x.b[1].y) << 16};
+}
 template <bool VEC>
-__device__ __forceinline__ void store_codes(uint8_t* p, const LanePairs& m, const Pairs& x) {
+__device__ __forceinline__ void store_codes(uint8_t* p, const LanePairs& m, const Codes& y) {
   if (VEC && m.split) {
-    *reinterpret_cast<uint32_t*>(p + 4 * m.c) = e4m3_pair(x.a[0].x, x.a[0].y) | e4m3_pair(x.a[1].x, x.a[1].y) << 16;
-    *reinterpret_cast<uint32_t*>(p + m.nf + 4 * m.c) = e4m3_pair(x.b[0].x, x.b[0].y) | e4m3_pair(x.b[1].x, x.b[1].y) << 16;
+    *reinterpret_cast<uint32_t*>(p + 4 * m.c) = y.a;
+    *reinterpret_cast<uint32_t*>(p + m.nf + 4 * m.c) = y.b;
+  } else if (VEC) {
+    *reinterpret_cast<uint2*>(p + 8 * m.c) = make_uint2(__byte_perm(y.a, y.b, 0x5140), __byte_perm(y.a, y.b, 0x7362));
   } else {
-    const uint32_t w[2] = {e4m3_pair(x.a[0].x, x.b[0].x) | e4m3_pair(x.a[0].y, x.b[0].y) << 16,
-                           e4m3_pair(x.a[1].x, x.b[1].x) | e4m3_pair(x.a[1].y, x.b[1].y) << 16};
-    if (VEC) {
-      *reinterpret_cast<uint2*>(p + 8 * m.c) = make_uint2(w[0], w[1]);
-    } else {
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const uint32_t two = w[i / 2] >> 16 * (i & 1);
-        p[m.low(i)] = (uint8_t)two;
-        p[m.high(i)] = (uint8_t)(two >> 8);
-      }
-    }
+    for (int i = 0; i < 4; i++) p[m.low(i)] = (uint8_t)(y.a >> 8 * i), p[m.high(i)] = (uint8_t)(y.b >> 8 * i);
   }
 }
 
@@ -183,9 +182,9 @@ __device__ __forceinline__ void only_finite(Pairs& x, float instead) {
   for (int e = 0; e < 2; e++) one(x.a[e].x), one(x.a[e].y), one(x.b[e].x), one(x.b[e].y);
 }
 // The norm over the LPR lanes of N rows (lanes without values have zeros), where
-// `on` is all ones; where it is 0, w (the weights in the lanes' order) has ones.
+// on[i] is all ones; where it is 0, w[i] (the weights in the lanes' order) has ones.
 template <int LPR, int N>
-__device__ __forceinline__ void norm_rows(Pairs (&x)[N], const float* w, uint32_t on, const CacheArgs& a) {
+__device__ __forceinline__ void norm_rows(Pairs (&x)[N], const float* const (&w)[N], const uint32_t (&on)[N], const CacheArgs& a) {
   float s[N];
 #pragma unroll
   for (int i = 0; i < N; i++) {
@@ -201,9 +200,9 @@ __device__ __forceinline__ void norm_rows(Pairs (&x)[N], const float* w, uint32_
     for (int i = 0; i < N; i++) s[i] += __shfl_xor_sync(~0u, s[i], o);
 #pragma unroll
   for (int i = 0; i < N; i++) {
-    const float r = __uint_as_float((__float_as_uint(rsqrtf(fmaf(s[i], a.inv_hd, a.eps))) & on) | (0x3f800000u & ~on));
+    const float r = __uint_as_float((__float_as_uint(rsqrtf(fmaf(s[i], a.inv_hd, a.eps))) & on[i]) | (0x3f800000u & ~on[i]));
     const float2 rr = make_float2(r, r);
-    const float4 u = *reinterpret_cast<const float4*>(w), v = *reinterpret_cast<const float4*>(w + PC_PAIRS);
+    const float4 u = *reinterpret_cast<const float4*>(w[i]), v = *reinterpret_cast<const float4*>(w[i] + PC_PAIRS);
     x[i].a[0] = pc_mul2(x[i].a[0], pc_mul2(rr, make_float2(u.x, u.y)));
     x[i].a[1] = pc_mul2(x[i].a[1], pc_mul2(rr, make_float2(u.z, u.w)));
     x[i].b[0] = pc_mul2(x[i].b[0], pc_mul2(rr, make_float2(v.x, v.y)));
@@ -268,8 +267,8 @@ __device__ __forceinline__ void keep_weights(const CacheArgs& a, CacheShared& sh
   }
 }
 __device__ __forceinline__ void keep_turn(float (*turn)[PC_PAIRS], int pair, int pos, double f, float amp) {
-  const float2 t = rope_angle(pos, f, amp);
-  turn[0][pair] = t.x, turn[1][pair] = t.y;
+  const double2 t = rope_angle(pos, f, amp);
+  turn[0][pair] = (float)t.x, turn[1][pair] = (float)t.y;
 }
 
 // Rows of nt tokens from t0 on: q, and (tg_rotary, 16-bit pages) k and v.  A row
@@ -357,27 +356,101 @@ __device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, 
     fetch(t + AHEAD - 1);
     const Turns turns(sh.turn[t & 7], m);
     const int page = MODE == PC_ROTARY ? -1 : sh.page[t];
-#pragma unroll
-    for (int i = 0; i < R; i++) {
+    auto read = [&](int i, Pairs& x) {   // lanes of rows that have none take part in the sums
+      x = no_pairs();
+      if (first + i * ROWS < rows && m.any()) read_pairs<T, VEC>(x, m, pc_ring + (t % AHEAD * R + i) * PC_THREADS + tid - m.c);
+    };
+    auto write = [&](int i, Pairs& x) {
       const int r = first + i * ROWS;
-      if (r - tid % 32 / LPR >= rows) break;   // none of the warp's
-      const bool is_q = r < a.H, is_v = r >= a.H + a.KH, here = r < rows && m.any();
-      Pairs x[1] = {no_pairs()};
-      if (here) read_pairs<T, VEC>(x[0], m, pc_ring + (t % AHEAD * R + i) * PC_THREADS + tid - m.c);
-      if (NORM)   // lanes of rows that have none take part in the sums
-        norm_rows<LPR, 1>(x, w[i], on[i], a);
-      if (here) {
-        if (MODE != PC_PAGES16 || !is_v) rotate_pairs<VEC>(x[0], turns, m);
-        if (MODE != PC_PAGES16 || is_q) {
-          if (page != -2) store_pairs<T, VEC>(to[i], m, x[0]);
-          to[i] += is_q ? a.sqo[0] : a.sko[0];
-        } else if (page >= 0) {
-          const long long at = is_v ? page * a.svp[0] + sh.row[t] * a.svp[2] : page * a.skp[0] + sh.row[t] * a.skp[2];
-          store_pairs<T, VEC>((uint8_t*)to[i] + at, m, x[0]);
-        }
+      const bool is_q = r < a.H, is_v = r >= a.H + a.KH;
+      if (r >= rows || !m.any()) return;
+      if (MODE != PC_PAGES16 || !is_v) rotate_pairs<VEC>(x, turns, m);
+      if (MODE != PC_PAGES16 || is_q) {
+        if (page != -2) store_pairs<T, VEC>(to[i], m, x);
+        to[i] += is_q ? a.sqo[0] : a.sko[0];
+      } else if (page >= 0) {
+        const long long at = is_v ? page * a.svp[0] + sh.row[t] * a.svp[2] : page * a.skp[0] + sh.row[t] * a.skp[2];
+        store_pairs<T, VEC>((uint8_t*)to[i] + at, m, x);
+      }
+    };
+    if (NORM) {   // the rows' sums side by side: 8,192 tokens x 32 heads 25.4 us, one after another 27; without norms that is slower
+      Pairs x[R];
+#pragma unroll
+      for (int i = 0; i < R; i++) read(i, x[i]);
+      norm_rows<LPR, R>(x, w, on, a);
+#pragma unroll
+      for (int i = 0; i < R; i++) write(i, x[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < R; i++) {
+        Pairs x;
+        read(i, x);
+        write(i, x);
       }
     }
   }
+}
+
+// Codes are what the formulas' exact values round to, so that they do not depend on
+// how a sum was taken.  In fp32 the sum of squares is 9 roundings deep, half of
+// which reach its root, which has 4 2^-24 of its own; with the mean, two products
+// and a rotation a value y is off by at most 14.5 2^-24 |(a, b)| <= PC_OFF (|y_a| +
+// |y_b|) of its pair.  Where both ends of that interval round to one code, that is
+// it; the rows of the others, one value in 7,000, are worked out in 64 bits by the
+// whole warp.  The test for doubt takes 2 of 8,192 tokens' 42 us and those rows 3.
+constexpr float PC_OFF = 0x1p-20f;
+__device__ __forceinline__ Codes codes_within(const Pairs& x, float off, bool& doubt) {
+  Pairs lo, hi;
+#pragma unroll
+  for (int e = 0; e < 2; e++) {
+    float2 d = make_float2(off * (fabsf(x.a[e].x) + fabsf(x.b[e].x)), off * (fabsf(x.a[e].y) + fabsf(x.b[e].y)));
+    d.x = fminf(d.x, 1e30f), d.y = fminf(d.y, 1e30f);   // beside a NaN: any doubt
+    const float2 one = make_float2(1.f, 1.f), less = make_float2(-1.f, -1.f);
+    lo.a[e] = at_fma2(d, less, x.a[e]), lo.b[e] = at_fma2(d, less, x.b[e]);
+    hi.a[e] = at_fma2(d, one, x.a[e]), hi.b[e] = at_fma2(d, one, x.b[e]);
+  }
+  const Codes y = codes_of(lo), z = codes_of(hi);
+  doubt = y.a != z.a || y.b != z.b;
+  return y;
+}
+__device__ __forceinline__ float to_odd(double x) {   // rounds to any fewer bits as x does; NaN where x is not finite
+  const float y = __double2float_rz(x);
+  return x - x != 0 ? NAN : (double)y == x ? y : __uint_as_float(__float_as_uint(y) | 1);
+}
+// row: null for lanes without values; eps: negative where there is no norm.
+template <typename T, int LPR, bool VEC, bool NORM>
+__device__ __noinline__ Codes exact_codes(const LanePairs m, const uint4* row, const float* w, const double* freqs, int pos, float amp, float eps,
+                                          float inv, double per_hd) {
+  Pairs x = no_pairs();
+  if (row) read_pairs<T, VEC>(x, m, row);
+  double r = inv;   // a power of two
+  if (NORM) {
+    double part[2], sum;
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+      part[e] = ((double)x.a[e].x * x.a[e].x + (double)x.a[e].y * x.a[e].y) + ((double)x.b[e].x * x.b[e].x + (double)x.b[e].y * x.b[e].y);
+    sum = part[0] + part[1];
+#pragma unroll
+    for (int o = LPR / 2; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    if (eps >= 0.f) {   // 2^-22 after the function, 2^-43 after a Newton step
+      const double z = sum * per_hd + (double)eps, r0 = rsqrtf((float)z);
+      r *= r0 * (1.5 - 0.5 * z * r0 * r0);
+    }
+  }
+  Pairs y;
+  auto pair = [&](int i, float xa, float xb, float& ya, float& yb) {
+    double u = xa * r, v = xb * r;
+    if (NORM) u *= w[i], v *= w[PC_PAIRS + i];
+    if (m.turns(i)) {
+      const double2 t = rope_angle(pos, freqs[4 * m.c + i], amp);
+      const double z = u * t.x - v * t.y;
+      v = v * t.x + u * t.y, u = z;
+    }
+    ya = to_odd(u), yb = to_odd(v);
+  };
+  pair(0, x.a[0].x, x.b[0].x, y.a[0].x, y.b[0].x), pair(1, x.a[0].y, x.b[0].y, y.a[0].y, y.b[0].y);
+  pair(2, x.a[1].x, x.b[1].x, y.a[1].x, y.b[1].x), pair(3, x.a[1].y, x.b[1].y, y.a[1].y, y.b[1].y);
+  return codes_of(y);
 }
 
 // Runs of 8-bit blocks whose first token is one of the `window` packed tokens
@@ -385,8 +458,8 @@ __device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, 
 // worked out twice, for the largest and for the codes: kept in registers they
 // leave room for one CTA of an SM instead of three (8,192 tokens with q 171 us
 // instead of 47).  Two rows at a time, for their sums' shuffles to overlap.  Keys
-// and values of 4 heads, 8,192 tokens, normed: 18 us; 25 MB to read and write take
-// 4.  As many CTAs as there are SMs' places take 12: what bounds it is how long one
+// and values of 4 heads, 8,192 tokens, normed: 23 us; 25 MB to read and write take
+// 4.  As many CTAs as there are SMs' places take 15: what bounds it is how long one
 // takes from its offsets to its scales, and that 512 are one round and a bit.
 template <typename T, int LPR, bool VEC, bool NORM>
 __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& sh, int t0) {
@@ -419,7 +492,9 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
   if (!sh.runs) return;
   const LanePairs m(a, lane % LPR);
   const int items = sh.runs * 2 * a.KH;
-  const uint32_t on = a.kw ? ~0u : 0;
+  const float* const w[2] = {sh.w[1] + (m.any() ? 4 * m.c : 0), sh.w[1] + (m.any() ? 4 * m.c : 0)};
+  const uint32_t on[2] = {a.kw ? ~0u : 0, a.kw ? ~0u : 0};
+  const float off_by = (NORM && a.kw) || 4 * m.c < a.nf ? PC_OFF : 0.f;   // values that no one touches are exact
   uint4* ring = pc_ring + wid * PAGED_BLOCK * LPR;   // an item's rows
   auto fetch = [&](int item) {
     const int i = item / (2 * a.KH), kh = item % (2 * a.KH) >> 1, is_v = item & 1;
@@ -452,7 +527,7 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
         if ((u + i) * RPP + lane / LPR < n && m.any()) read_pairs<T, VEC>(x[i], m, ring + ((u + i) * RPP + lane / LPR) * LPR);
       }
       if (is_v) return;
-      if (NORM) norm_rows<LPR, 2>(x, sh.w[1] + (m.any() ? 4 * m.c : 0), on, a);
+      if (NORM) norm_rows<LPR, 2>(x, w, on, a);
 #pragma unroll
       for (int i = 0; i < 2; i++) {
         const int j = (u + i) * RPP + lane / LPR;
@@ -482,17 +557,18 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
     const float need = __uint_as_float((uint32_t)(paged_scale_exp(amax) + 127) << 23);
     const float scale = fmaxf(need, before), inv = 1.f / scale;
     if (off && scale > before) {   // the earlier tokens' codes under the larger scale
-      const float again = before * inv;
+      const float less = before * inv;
       for (int i8 = lane; i8 < off * (a.hd / 8); i8 += 32) {
         uint2* at = reinterpret_cast<uint2*>(rows + i8 / (a.hd / 8) * pitch + i8 % (a.hd / 8) * 8);
         const uint2 w = *at;
         auto four = [&](uint32_t c) {
           const float2 lo = e4m3_values(c), hi = e4m3_values(c >> 16);
-          return e4m3_pair(lo.x * again, lo.y * again) | e4m3_pair(hi.x * again, hi.y * again) << 16;
+          return e4m3_pair(lo.x * less, lo.y * less) | e4m3_pair(hi.x * less, hi.y * less) << 16;
         };
         *at = make_uint2(four(w.x), four(w.y));
       }
     }
+    unsigned again = 0;   // rows with codes in doubt
 #pragma unroll 1
     for (int u = 0; u * RPP < n; u += 2) {
       Pairs x[2];
@@ -500,14 +576,23 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
 #pragma unroll
       for (int i = 0; i < 2; i++) {
         const int j = (u + i) * RPP + lane / LPR;
-        if (j < n && m.any()) {
-          const float2 f = make_float2(inv, inv);
-          if (odd) only_finite(x[i], NAN);
+        const bool there = j < n && m.any();
+        const float2 f = make_float2(inv, inv);
+        if (odd) only_finite(x[i], NAN);
 #pragma unroll
-          for (int e = 0; e < 2; e++) x[i].a[e] = pc_mul2(x[i].a[e], f), x[i].b[e] = pc_mul2(x[i].b[e], f);
-          store_codes<VEC>(rows + (off + j) * pitch, m, x[i]);
-        }
+        for (int e = 0; e < 2; e++) x[i].a[e] = pc_mul2(x[i].a[e], f), x[i].b[e] = pc_mul2(x[i].b[e], f);
+        bool doubt = false;
+        const Codes y = is_v ? codes_of(x[i]) : codes_within(x[i], off_by, doubt);
+        if (there) store_codes<VEC>(rows + (off + j) * pitch, m, y);
+        if (there && doubt) again |= 1u << (u + i);
       }
+    }
+    for (again = __reduce_or_sync(~0u, again); again; again &= again - 1) {
+      const int j = (__ffs(again) - 1) * RPP + lane / LPR;
+      const bool there = j < n && m.any();
+      const Codes y = exact_codes<T, LPR, VEC, NORM>(m, there ? ring + j * LPR : nullptr, w[0], a.freqs, sh.at[j0 + min(j, n - 1)], a.amp,
+                                                     a.kw ? a.eps : -1.f, inv, 1.0 / a.hd);
+      if (there) store_codes<VEC>(rows + (off + j) * pitch, m, y);
     }
     if (lane == 0) *scale_at = scale;
     __syncwarp();   // all have read the rows
@@ -518,9 +603,9 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
 // Rows of tokens and, beside them in the same launch, runs of 8-bit blocks, so that
 // the copies of the one overlap the instructions of the other.  Measured in a
 // replayed graph, bf16, heads of 128: 8,192 tokens x 32 heads rotated 21 us (0.97 of
-// a copy's rate, part of it from L2: bytes bound it), with norms 27 (instructions);
-// the same with 4 key heads to 8-bit pages 39, without norms 29, where 160 MB take
-// 24.  A chunk of 2,048 tokens 15; two tokens 4, of which an empty kernel is 2.
+// a copy's rate, part of it from L2: bytes bound it), with norms 25.4 (instructions);
+// the same with 4 key heads to 8-bit pages 42, without norms 34, where 160 MB take
+// 24.  A chunk of 2,048 tokens 18; two tokens 4, of which an empty kernel is 2.
 template <typename T, int LPR, bool VEC, int MODE, bool NORM, int R>
 __global__ void __launch_bounds__(PC_THREADS, PC_PER_SM) cache_kernel(const CacheArgs a) {
   __shared__ CacheShared sh;

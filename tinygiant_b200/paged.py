@@ -259,8 +259,8 @@ def cache_append(k, v, k_pages, v_pages, tables, lens, cu=None, *, k_scales=None
     its query is rotated all the same.  Rows of no sequence are left out, the
     query's too.  No place may be written twice in a call, and in pages of 8
     bits no two sequences may write to one block: its values would be undefined.
-    A value that is not finite becomes NaN in 8 bits and does not count for
-    the scale.  Returns the rotated q, or None."""
+    In 8 bits a code is the nearest to what the formulas give exactly, and a
+    value that is not finite becomes NaN and does not count for the scale.  Returns the rotated q, or None."""
     given = out is not None
     try:
         dtype, dev, shape, (k0, k1, k2), (v0, v1, v2) = k.dtype, k.get_device(), k.shape, k.stride(), v.stride()
