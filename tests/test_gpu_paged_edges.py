@@ -1,0 +1,55 @@
+"""The paged cache where it can go wrong: values that are not finite beside cuts, codes and scales next to a border,
+earlier scales of any kind, the C entries by their argument lists, and what is refused beside the ordinary.
+
+Tolerances: none.  Codes, scales and NaN are compared for equality; expected codes are worked out on the host in
+numpy's long doubles (64 bits of mantissa; angles reduced in decimals), from inputs chosen so that the exact value is 2^-44
+of itself or more away from the border between two codes, which that arithmetic (2^-58 of a pair) and fp64's (2^-50)
+resolve."""
+import ctypes
+import decimal
+import math
+
+import numpy as np
+import pytest
+
+import tinygiant_b200 as tg
+from test_gpu_paged import DT, E4M3, Pool, bits, check, ends, gen, ints, paged_ref, rand
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+L = np.longdouble
+
+
+@pytest.fixture(scope="module")
+def P(gpu):
+    from tinygiant_b200 import paged
+    return paged
+
+
+# ---- attention: what is not finite
+
+def put(pool, x, b, j, value, kh=0, d=slice(None)):
+    """A value at position j of sequence b."""
+    pages = getattr(pool, x)
+    pages[int(pool.tables[b, j // pool.page]), kh, j % pool.page, d] = torch.tensor(value, device="cuda").to(pages.dtype)
+
+
+@pytest.mark.parametrize("codes", [True, False], ids=["8bit", "16bit"])
+@pytest.mark.parametrize("with_sinks", [False, True], ids=["plain", "sinks"])
+def test_a_key_of_nan_wherever_units_are_cut(P, codes, with_sinks):
+    """The newest key, alone in its tile or not, alone in its sequence's last piece or not: its sequence is NaN, the other as it was."""
+    g, H, hd = gen(51), 4, 128
+    sinks = torch.randn(H, generator=g, device="cuda") if with_sinks else None
+    for m in [897, 898, *range(513, 1600, 32), 3009, 8193]:
+        pool = Pool(g, torch.bfloat16, codes, 1, hd, 64, [m, m])
+        q = rand(g, 2, H, hd, dtype=torch.bfloat16)
+        for window in (0, 300):
+            call = lambda: P.attention_paged(q, pool.k, pool.v, pool.tables, pool.lens, **pool.kw, sinks=sinks, max_len=m, window=window)  # noqa: E731
+            clean = call()
+            assert bool(torch.isfinite(clean).all())
+            kept = pool.k.clone()
+            for b in (0, 1):
+                put(pool, "k", b, m - 1, math.nan)
+                got = call()
+                assert bool(torch.isnan(got[b]).all()) and torch.equal(got[1 - b], clean[1 - b]), (m, b, window)
+                pool.k.copy_(kept)

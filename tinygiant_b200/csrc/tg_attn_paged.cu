@@ -822,7 +822,7 @@ __global__ void __launch_bounds__(PG_JOIN_THREADS) paged_join_kernel(const Paged
 #pragma unroll
       for (int e = 0; e < HD / 64; e++) y[e] = *reinterpret_cast<const float2*>(a.po + at(p) * HD + 2 * lane + 64 * e);
       const float fm = ml.y == 0.f ? 0.f : at_exp2(ml.x - mm), fr = ml.y == 0.f || ml.z == -INFINITY ? 0.f : at_exp2(ml.z - rr);
-      if (fm != 0.f) L = fmaf(ml.y, fm, L);   // not 0 x inf
+      L = fmaf(ml.y, fm, L);   // a sum of NaN, which the maxima pass by, stays one
       if (fr != 0.f)
 #pragma unroll
         for (int e = 0; e < HD / 64; e++) v[e].x = fmaf(y[e].x, fr, v[e].x), v[e].y = fmaf(y[e].y, fr, v[e].y);
