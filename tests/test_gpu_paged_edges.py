@@ -53,3 +53,41 @@ def test_a_key_of_nan_wherever_units_are_cut(P, codes, with_sinks):
                 got = call()
                 assert bool(torch.isnan(got[b]).all()) and torch.equal(got[1 - b], clean[1 - b]), (m, b, window)
                 pool.k.copy_(kept)
+
+
+@pytest.mark.parametrize("codes", [True, False], ids=["8bit", "16bit"])
+def test_a_key_of_nan_alone_before_a_cut(P, codes):
+    """A window that begins with the last key of a tile, which is NaN: the first piece may see no other."""
+    g, H, hd, n = gen(52), 4, 128, 2
+    for m in range(1500, 1500 + 64, 5):
+        pool = Pool(g, torch.float16, codes, 1, hd, 64, [m, m])
+        q = rand(g, 2, n, H, hd, dtype=torch.float16)
+        for first in (15, 31, 47):                                  # the first key that the last query sees
+            window = m - first
+            call = lambda: P.attention_paged(q, pool.k, pool.v, pool.tables, pool.lens, **pool.kw, max_len=m, window=window)  # noqa: E731
+            clean, kept = call(), pool.k.clone()
+            put(pool, "k", 1, first, math.nan)
+            got = call()
+            assert bool(torch.isnan(got[1]).all()) and torch.equal(got[0], clean[0]), (m, first)
+            pool.k.copy_(kept)
+            put(pool, "k", 1, first - 1, math.nan)                  # which the first query sees alone
+            got = call()
+            assert bool(torch.isnan(got[1, 0]).all()) and torch.equal(got[1, 1:], clean[1, 1:]) and torch.equal(got[0], clean[0])
+            pool.k.copy_(kept)
+
+
+@pytest.mark.parametrize("codes", [True, False], ids=["8bit", "16bit"])
+def test_a_query_of_nan_over_long_sequences(P, codes):
+    g, H, KH, hd, lens = gen(53), 8, 2, 64, [5000, 700, 2048, 33]
+    pool = Pool(g, torch.bfloat16, codes, KH, hd, 16, lens)
+    q = rand(g, 4, 1, H, hd, dtype=torch.bfloat16)
+    for sinks in (None, torch.randn(H, generator=g, device="cuda")):
+        call = lambda: P.attention_paged(q, pool.k, pool.v, pool.tables, pool.lens, **pool.kw, sinks=sinks)  # noqa: E731
+        q[:, 0, 3] = 1.0
+        clean = call()
+        check(clean, *paged_ref(pool, q, lens, 0, sinks), codes)
+        q[:, 0, 3, 5] = math.nan
+        got = call()
+        assert bool(torch.isnan(got[:, 0, 3]).all())
+        keep = [h for h in range(H) if h != 3]
+        assert torch.equal(got[:, :, keep], clean[:, :, keep])

@@ -531,8 +531,9 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
             if (CODES) w = fmaxf(w, __shfl_xor_sync(~0u, w, sft));
           }
           if (!CODES) w = v;
-          const float mn = fmaxf(m[t][z], v), rn = fmaxf(r[t][z], w);
-          const float fm = mn > m[t][z] ? at_exp2(m[t][z] - mn) : 1.f, fr = rn > r[t][z] ? at_exp2(r[t][z] - rn) : 1.f;
+          const bool um = v > limm[t][z], ur = CODES ? w > limr[t][z] : um;   // rows move by their own scores alone
+          const float mn = um ? v : m[t][z], rn = ur ? w : r[t][z];
+          const float fm = um ? at_exp2(m[t][z] - mn) : 1.f, fr = ur ? at_exp2(r[t][z] - rn) : 1.f;
           m[t][z] = mn, r[t][z] = rn;
           nm[t][z] = mn == -INFINITY ? 0.f : OFF - mn;
           nr[t][z] = rn == -INFINITY ? 0.f : OFF - rn;
