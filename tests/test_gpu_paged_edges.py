@@ -91,3 +91,30 @@ def test_a_query_of_nan_over_long_sequences(P, codes):
         assert bool(torch.isnan(got[:, 0, 3]).all())
         keep = [h for h in range(H) if h != 3]
         assert torch.equal(got[:, :, keep], clean[:, :, keep])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("codes", [True, False], ids=["8bit", "16bit"])
+@pytest.mark.parametrize("m", [90, 400, 3000, 20000])
+def test_values_of_nan_under_weights_that_vanish(P, m, codes, dtype):
+    """A value of NaN whose weight is 2^-300 of the largest reaches its dimension, whichever warp, piece or tile has it."""
+    g, hd, dt = gen(54), 64, DT[dtype]
+    pool = Pool(g, dt, codes, 1, hd, 16, [m])
+    pool.k.copy_(torch.zeros_like(pool.k, dtype=torch.float32).to(pool.k.dtype))
+    if codes:
+        pool.ks[:] = 1.0
+    q = torch.zeros(1, 1, 2, hd, dtype=dt, device="cuda")
+    q[..., 0] = 20.0
+    top = m // 3
+    put(pool, "k", 0, top, 15.0, d=0)
+    call = lambda: P.attention_paged(q, pool.k, pool.v, pool.tables, pool.lens, **pool.kw, scale=math.log(2.0), max_len=m)  # noqa: E731
+    clean = call()
+    assert bool(torch.isfinite(clean).all())
+    for j in sorted({0, 1, 33, 64, top - 1, top + 1, top + 40, m // 2, m - 40, m - 1}):
+        kept = pool.v.clone()
+        put(pool, "v", 0, j, math.nan, d=7)
+        got = call()
+        want = torch.zeros_like(got, dtype=torch.bool)
+        want[..., 7] = True
+        assert torch.equal(torch.isnan(got), want) and torch.equal(got[~want], clean[~want]), j
+        pool.v.copy_(kept)

@@ -725,9 +725,9 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
         float2 v = make_float2(0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < 4; w++) {
-          const float f = __shfl_sync(~0u, fr, 8 * w + h);   // 0 where there is no warp w
+          const float f = __shfl_sync(~0u, fr, 8 * w + h);
           const uint2 y = lds8(from[w] + (h * S::RP + 2 * at) * 4);
-          if (f != 0.f) v.x = fmaf(__uint_as_float(y.x), f, v.x), v.y = fmaf(__uint_as_float(y.y), f, v.y);
+          if (w < a.team) v.x = fmaf(__uint_as_float(y.x), f, v.x), v.y = fmaf(__uint_as_float(y.y), f, v.y);   // NaN under a weight of 0 too
         }
         if (all) {
           const int query = query_of(a, row), d = S::dim((at + lane) / 8, lane % 8);
@@ -824,9 +824,8 @@ __global__ void __launch_bounds__(PG_JOIN_THREADS) paged_join_kernel(const Paged
       for (int e = 0; e < HD / 64; e++) y[e] = *reinterpret_cast<const float2*>(a.po + at(p) * HD + 2 * lane + 64 * e);
       const float fm = ml.y == 0.f ? 0.f : at_exp2(ml.x - mm), fr = ml.y == 0.f || ml.z == -INFINITY ? 0.f : at_exp2(ml.z - rr);
       L = fmaf(ml.y, fm, L);   // a sum of NaN, which the maxima pass by, stays one
-      if (fr != 0.f)
 #pragma unroll
-        for (int e = 0; e < HD / 64; e++) v[e].x = fmaf(y[e].x, fr, v[e].x), v[e].y = fmaf(y[e].y, fr, v[e].y);
+      for (int e = 0; e < HD / 64; e++) v[e].x = fmaf(y[e].x, fr, v[e].x), v[e].y = fmaf(y[e].y, fr, v[e].y);
     }
 #pragma unroll
   for (int e = 0; e < HD / 64; e++) part[wid][lane + 32 * e] = v[e];
