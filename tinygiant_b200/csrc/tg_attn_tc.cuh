@@ -43,6 +43,7 @@
 #include <cuda.h>
 
 #include <atomic>
+#include <cfloat>
 #include <type_traits>
 
 #include "tg_attn.h"
@@ -1026,6 +1027,7 @@ __device__ __forceinline__ float2 join_scale(int n, const float2* pml, float sin
     M = m;
   }
   if (L == 0.f) return make_float2(0.f, 0.f);
+  if (sink2 == INFINITY) sink2 = FLT_MAX;   // all the weight is the sink's, not inf - inf
   const float m = fmaxf(M, sink2);
   return make_float2(m, 1.f / (L * at_exp2(M - m) + at_exp2(sink2 - m)));
 }
