@@ -118,3 +118,24 @@ def test_values_of_nan_under_weights_that_vanish(P, m, codes, dtype):
         want[..., 7] = True
         assert torch.equal(torch.isnan(got), want) and torch.equal(got[~want], clean[~want]), j
         pool.v.copy_(kept)
+
+
+@pytest.mark.parametrize("codes", [True, False], ids=["8bit", "16bit"])
+def test_sinks_of_any_size(P, codes):
+    """A sink of +inf, or beyond what fp32 holds in base 2, takes all the weight, one of -inf or as far below none, one of NaN is NaN;
+    as attention_prompt has it."""
+    from tinygiant_b200 import attention as A
+    g, H, hd = gen(55), 8, 64
+    top = torch.finfo(torch.float32).max
+    sinks = torch.tensor([math.inf, top, -math.inf, -top, math.nan, 0.5, 3e38, -3e38], device="cuda")
+    for lens in ([40, 3, 0], [3000, 900, 0]):
+        pool = Pool(g, torch.bfloat16, codes, H, hd, 16, lens)
+        q = rand(g, 3, 1, H, hd, dtype=torch.bfloat16)
+        got = P.attention_paged(q, pool.k, pool.v, pool.tables, pool.lens, **pool.kw, sinks=sinks)
+        plain = P.attention_paged(q, pool.k, pool.v, pool.tables, pool.lens, **pool.kw)
+        assert not bool(got[:2, 0, [0, 1, 6]].any()) and torch.equal(got[:2, 0, [2, 3, 7]], plain[:2, 0, [2, 3, 7]])
+        assert bool(torch.isnan(got[:2, 0, 4]).all()) and not bool(got[2].any())
+        check(got[:2, :, 5], *(x[:2, :, 5] for x in paged_ref(pool, q, lens, 0, torch.full_like(sinks, 0.5))), codes)
+        k, v = P.cache_gather(pool.k, pool.v, pool.tables, ends(lens), sum(lens), **pool.kw)
+        prompt = A.attention_prompt(q[:, 0], k, v, ints(0, 1, 2, 3), ends(lens), sinks=sinks)
+        assert torch.equal(torch.isnan(prompt[:2]), torch.isnan(got[:2, 0])) and not bool(prompt[:2, [0, 1, 6]].any())

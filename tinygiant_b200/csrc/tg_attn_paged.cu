@@ -36,6 +36,7 @@
 // issue slots at that rate.  64 sequences of 1 to 4,096: 34 us where the bytes
 // take 20: start and cut 4, units' starts and ends 4, the second kernel 5.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -113,6 +114,12 @@ __device__ __forceinline__ int query_of(const PagedArgs& a, int r) { return a.G 
 // theirs; 0 for a row without a key.
 __device__ __forceinline__ float paged_factor(float L, float up) {
   return L == 0.f ? 0.f : up == -INFINITY ? 0.f * L : at_exp2(up) / L;
+}
+// A head's sink in base 2.  +inf, or what leaves fp32 here, is fp32's largest, so that
+// it takes all the weight instead of meeting itself as inf - inf.
+__device__ __forceinline__ float sink_of(const PagedArgs& a, int head) {
+  const float x = a.sinks[head] * LOG2E;
+  return x == INFINITY ? FLT_MAX : x;
 }
 // Four e4m3 codes, the lowest byte first, as two pairs of fp16.
 __device__ __forceinline__ void pg_codes(uint32_t four, uint32_t& lo, uint32_t& hi) {
@@ -660,7 +667,7 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
           if (all) {
             const int head = wk.kh * a.G + row - tok[t][z] * a.G;
             if (a.sinks) {
-              const float sink = a.sinks[head] * LOG2E, top = fmaxf(mm, sink);
+              const float sink = sink_of(a, head), top = fmaxf(mm, sink);
               if (sink != -INFINITY) L = (L == 0.f ? 0.f : L * at_exp2(mm - top)) + at_exp2(sink - top), mm = top;
             }
             const float f = paged_factor(L, r[t][z] - OFF - mm);
@@ -703,7 +710,7 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
       const float4 ml = mine < a.team ? sh.ml[w0 + mine][lane & 7] : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
       const bool has = ml.y != 0.f;   // a warp with keys
       float sink = -INFINITY;
-      if (a.sinks && all && h8 < a.rows) sink = a.sinks[wk.kh * a.G + h8 - query_of(a, h8) * a.G] * LOG2E;
+      if (a.sinks && all && h8 < a.rows) sink = sink_of(a, wk.kh * a.G + h8 - query_of(a, h8) * a.G);
       float mm = has ? ml.x : -INFINITY, rr = has ? ml.z : -INFINITY;
 #pragma unroll
       for (int sft = 8; sft < 32; sft <<= 1) mm = fmaxf(mm, __shfl_xor_sync(~0u, mm, sft)), rr = fmaxf(rr, __shfl_xor_sync(~0u, rr, sft));
@@ -802,7 +809,7 @@ __global__ void __launch_bounds__(PG_JOIN_THREADS) paged_join_kernel(const Paged
   const bool here = row < a.rows;
   const int query = query_of(a, here ? row : 0), head = kh * a.G + (here ? row : 0) - query * a.G;
   auto at = [&](int p) { return (size_t)(p ? 2 * (i + p) : 2 * i + 1) * (8 * NT) + h; };
-  const float sink = a.sinks ? a.sinks[head] * LOG2E : -INFINITY;
+  const float sink = a.sinks ? sink_of(a, head) : -INFINITY;
   float mm = sink, rr = -INFINITY;
   if (here)
     for (int p = lane; p < pieces; p += 32) {
