@@ -139,3 +139,65 @@ def test_sinks_of_any_size(P, codes):
         k, v = P.cache_gather(pool.k, pool.v, pool.tables, ends(lens), sum(lens), **pool.kw)
         prompt = A.attention_prompt(q[:, 0], k, v, ints(0, 1, 2, 3), ends(lens), sinks=sinks)
         assert torch.equal(torch.isnan(prompt[:2]), torch.isnan(got[:2, 0])) and not bool(prompt[:2, [0, 1, 6]].any())
+
+
+@pytest.mark.parametrize("hd,n,interleaved", [(128, 16, False), (64, 8, True), (64, 0, False), (96, 5, False)])
+def test_codes_of_infinities_under_a_norm(P, hd, n, interleaved):
+    """A key with an infinity is NaN where that reaches and zero elsewhere, whatever the tokens beside it hold; one call and one by one."""
+    g, T, KH = gen(65), 1024, 4
+    pool = Pool(g, torch.bfloat16, True, KH, hd, 64, [T])
+    one = pool.clone()
+    k, v = (rand(g, T, KH, hd, dtype=torch.bfloat16, scale=2.0) for _ in range(2))
+    at = torch.arange(T, device="cuda") % 16 == 5
+    k[at, :, 3] = math.inf
+    k[at, 1, hd - 1] = -math.inf
+    f = P.rotary_frequencies(2 * n, 1e4, device="cuda")[0] if n else None
+    kw = {"freqs": f, "interleaved": interleaved, "k_norm": 1 + 0.3 * torch.randn(hd, generator=g, device="cuda")}
+    P.cache_append(k, v, pool.k, pool.v, pool.tables, pool.lens, **pool.kw, **kw)
+    p = torch.arange(T, device="cuda")
+    codes = pool.k.transpose(1, 2)[pool.tables[0].long()[p // 64], p % 64].float()       # [T, KH, hd]
+    want = torch.zeros(KH, hd, dtype=torch.bool, device="cuda")
+    want[:, 3] = True
+    want[1, hd - 1] = True
+    if n > 3:
+        want[:, 3 + n if not interleaved else 2] = True
+    assert torch.equal(torch.isnan(codes[at]), want.expand(int(at.sum()), KH, hd))
+    assert not bool(codes[at].nan_to_num(0.0).any()) and bool(torch.isfinite(codes[~at]).all())
+    for t in range(0, T):
+        P.cache_append(k[t:t + 1], v[t:t + 1], one.k, one.v, one.tables, ints(t + 1), **one.kw, **kw)
+    # the scale of a block that grows token by token ends as that of the whole block; the last token's codes were written under it
+    assert torch.equal(one.ks, pool.ks)
+    last = torch.arange(15, T, 16, device="cuda")
+    rows = lambda x: bits(x.transpose(1, 2)[pool.tables[0].long()[last // 64], last % 64])  # noqa: E731
+    assert torch.equal(rows(one.k), rows(pool.k))
+
+
+def test_codes_beyond_fp32(P):
+    """Turned values that fp32 does not hold are NaN and do not count for the scale, heads whose sum of squares it does not hold are
+    normed to zero, whatever the tokens beside them hold."""
+    g, T, KH, hd, top = gen(67), 1024, 4, 64, torch.finfo(torch.float32).max
+    pool = Pool(g, torch.bfloat16, True, KH, hd, 64, [T])
+    k = (torch.randn(T, KH, hd, generator=g, device="cuda") * 1.2e38).clamp(-3.3e38, 3.3e38).to(torch.bfloat16)
+    f, p = P.rotary_frequencies(hd, 1e4, device="cuda")[0], torch.arange(T, device="cuda")
+    P.cache_append(k, k, pool.k, pool.v, pool.tables, pool.lens, **pool.kw, freqs=f)
+    t, (a, b) = (p.double()[:, None] * f)[:, None], k.double().split(hd // 2, -1)
+    y = torch.cat([a * t.cos() - b * t.sin(), b * t.cos() + a * t.sin()], -1)
+    page, row = pool.tables[0].long()[p // 64], p % 64
+    codes, scale = pool.k.transpose(1, 2)[page, row].double(), pool.ks[page, :, row // 16].double()
+    # sine, cosine, product and sum: off by (|a| + |b|) 3 2^-24 <= 2 (3.3e38) 3 2^-24 < 2^-21 of fp32's largest
+    over, fits = y.abs() > top * (1 + 2.0 ** -21), y.abs() < top * (1 - 2.0 ** -21)
+    assert int(over.sum()) > 20 and bool((over | fits).all()) and torch.equal(torch.isnan(codes), over)
+    need = torch.exp2(torch.ceil(torch.log2(torch.where(fits, y.abs(), 0.0).view(T // 16, 16, KH, hd).amax((1, 3)) / 448)))
+    assert torch.equal(scale, need.repeat_interleave(16, 0))
+    step = torch.exp2(torch.clamp(torch.floor(torch.log2((y / scale[..., None]).abs().clamp(min=2.0 ** -30))), min=-6) - 3)
+    u = y / scale[..., None] / step
+    clear = fits & (((u - u.floor()) - 0.5).abs() > 2.0 ** -33 * torch.hypot(a, b).repeat(1, 1, 2) / scale[..., None] / step)
+    # (token 0 is not turned, and of bf16's values, of 8 bits, one in 16 lies between two codes)
+    assert torch.equal(codes[clear], (torch.round(u) * step)[clear]) and int((fits & ~clear)[1:].sum()) < 8
+    # heads of 2^70 beside ordinary ones
+    k = rand(g, T, KH, hd, dtype=torch.bfloat16)
+    large = p % 16 == 9
+    k[large] = (k[large].float() * 2.0 ** 70).to(torch.bfloat16)
+    P.cache_append(k, k, pool.k, pool.v, pool.tables, pool.lens, **pool.kw, freqs=f, k_norm=torch.ones(hd, device="cuda"))
+    codes = pool.k.transpose(1, 2)[page, row].double()
+    assert not bool(codes[large].any()) and bool(torch.isfinite(codes).all()) and bool((codes[~large].abs().amax(-1) > 0).all())

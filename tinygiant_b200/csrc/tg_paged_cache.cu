@@ -18,6 +18,7 @@
 // scale grows when a larger token comes keeps its earlier codes' bits (but for
 // those that fall below the format's least normal value).
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 #include "../../include/tinygiant.h"
@@ -174,6 +175,16 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const LanePairs& m, cons
     for (int i = 0; i < 4; i++) p[m.low(i)] = (uint8_t)(y.a >> 8 * i), p[m.high(i)] = (uint8_t)(y.b >> 8 * i);
   }
 }
+template <bool VEC>
+__device__ __forceinline__ Codes load_codes(const uint8_t* p, const LanePairs& m) {
+  if (VEC && m.split) return {*reinterpret_cast<const uint32_t*>(p + 4 * m.c), *reinterpret_cast<const uint32_t*>(p + m.nf + 4 * m.c)};
+  Codes y{0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; i++) y.a |= (uint32_t)p[m.low(i)] << 8 * i, y.b |= (uint32_t)p[m.high(i)] << 8 * i;
+  return y;
+}
+// All ones in the bytes of four codes that are NaN.
+__device__ __forceinline__ uint32_t e4m3_nans(uint32_t four) { return (((four & 0x7f7f7f7fu) + 0x01010101u & 0x80808080u) >> 7) * 0xffu; }
 
 // `instead` in place of what is not finite.
 __device__ __forceinline__ void only_finite(Pairs& x, float instead) {
@@ -432,10 +443,7 @@ __device__ __noinline__ Codes exact_codes(const LanePairs m, const uint4* row, c
     sum = part[0] + part[1];
 #pragma unroll
     for (int o = LPR / 2; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    if (eps >= 0.f) {   // 2^-22 after the function, 2^-43 after a Newton step
-      const double z = sum * per_hd + (double)eps, r0 = rsqrtf((float)z);
-      r *= r0 * (1.5 - 0.5 * z * r0 * r0);
-    }
+    if (eps >= 0.f) r *= sum > FLT_MAX ? 0.0 : rsqrt(sum * per_hd + (double)eps);   // what fp32 does not hold counts as infinite there too
   }
   Pairs y;
   auto pair = [&](int i, float xa, float xb, float& ya, float& yb) {
@@ -592,7 +600,12 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
       const bool there = j < n && m.any();
       const Codes y = exact_codes<T, LPR, VEC, NORM>(m, there ? ring + j * LPR : nullptr, w[0], a.freqs, sh.at[j0 + min(j, n - 1)], a.amp,
                                                      a.kw ? a.eps : -1.f, inv, 1.0 / a.hd);
-      if (there) store_codes<VEC>(rows + (off + j) * pitch, m, y);
+      if (there) {
+        uint8_t* const at = rows + (off + j) * pitch;
+        const Codes z = load_codes<VEC>(at, m);   // what fp32 does not hold stays NaN
+        const uint32_t na = e4m3_nans(z.a), nb = e4m3_nans(z.b);
+        store_codes<VEC>(at, m, Codes{(y.a & ~na) | (z.a & na), (y.b & ~nb) | (z.b & nb)});
+      }
     }
     if (lane == 0) *scale_at = scale;
     __syncwarp();   // all have read the rows
