@@ -141,6 +141,94 @@ def test_sinks_of_any_size(P, codes):
         assert torch.equal(torch.isnan(prompt[:2]), torch.isnan(got[:2, 0])) and not bool(prompt[:2, [0, 1, 6]].any())
 
 
+# ---- codes next to a border
+
+E4M3_VALUES = np.array([0.0, *(m / 512 for m in range(1, 8)), *((8 + m) / 8 * 2.0 ** e for e in range(-6, 9) for m in range(8))][:127], dtype=L)
+
+
+def nearest(y):
+    """The nearest values of e4m3 of long doubles, |y| <= 448, none a tie."""
+    y = np.asarray(y, dtype=L)
+    d = np.abs(np.abs(y)[..., None] - E4M3_VALUES)
+    i = d.argmin(-1)
+    two = np.partition(d, 1, axis=-1)
+    assert bool((two[..., 1] - two[..., 0] > np.abs(y) * L(2) ** -44).all()), "an input of this test is too near a tie"
+    return np.sign(y) * E4M3_VALUES[i]
+
+
+def border(y):
+    """The border between two codes that is nearest to y > 0, in [16, 448)."""
+    step = 2.0 ** (math.floor(math.log2(y)) - 3)
+    return (math.floor(y / step) + 0.5) * step
+
+
+def bf16(rng, low, high, n):
+    x = torch.from_numpy(rng.uniform(low, high, n)).to(torch.bfloat16)
+    return x, x.double().numpy()
+
+
+def one_token(P, rows, freqs, position=None, ctx=0, before=None, **kw):
+    """One token of one sequence (rows [KH, hd] bf16: key and value) after ctx others, in pages of 8 bits: its codes of K as numbers,
+    and the scales of K and V [KH].  before: the block's scales there."""
+    KH, hd = rows.shape
+    k_pages, v_pages = (torch.zeros(1, KH, 16, hd, device="cuda").to(E4M3) for _ in range(2))
+    ks, vs = (torch.full((1, KH, 1), 1.0, device="cuda") if before is None else before.clone().view(1, KH, 1) for _ in range(2))
+    x = rows.cuda()[None]
+    P.cache_append(x, x, k_pages, v_pages, ints(0).view(1, 1), ints(ctx + 1), k_scales=ks, v_scales=vs,
+                   freqs=None if freqs is None else torch.from_numpy(freqs).cuda(), positions=None if position is None else ints(position), **kw)
+    f = lambda t: t[0, :, ctx].float().cpu().numpy().astype(L)  # noqa: E731
+    return f(k_pages), f(v_pages), ks[0, :, 0].cpu().numpy().astype(L), vs[0, :, 0].cpu().numpy().astype(L)
+
+
+def turned(a, b, p, f):
+    with decimal.localcontext(decimal.Context(prec=60)):
+        around = decimal.Decimal("6.28318530717958647692528676655900576839433879875021164")
+        t = np.array([L(str(decimal.Decimal(p) * decimal.Decimal(float(x)) % around)) for x in f], dtype=L)
+    c, s = np.cos(t), np.sin(t)
+    return a * c - b * s, b * c + a * s
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("p,low,high", [(1, 0.70, 0.7853), (1, 0.0, 6.28), (1048573, 0.0, 6.28), (2000003, 0.0, 6.28)])
+def test_codes_of_angles_next_to_a_border(P, p, low, high, interleaved):
+    """Frequencies that take a pair's first value to a border between two codes, 2^-32 of it to either side (at far positions as near
+    as a frequency in fp64 gets)."""
+    rng, n = np.random.default_rng(61 + p), 32
+    for _ in range(12):
+        a, b, f = np.zeros(n), np.zeros(n), np.zeros(n)
+        a[0] = 300.0                                               # the scale is 1
+        for j in range(1, n):
+            while True:
+                (_, x), (_, y) = bf16(rng, -250, 250, 1), bf16(rng, -250, 250, 1)
+                r, phi, t0 = np.sqrt(L(x[0]) ** 2 + L(y[0]) ** 2), np.arctan2(L(y[0]), L(x[0])), rng.uniform(low, high)
+                y0 = float(r) * math.cos(t0 + float(phi))
+                if not 20 < abs(y0) < 0.9 * float(r):
+                    continue
+                aim = L(border(abs(y0)) * math.copysign(1, y0)) * (1 + L(2) ** -32 * (1 if rng.random() < 0.5 else -1))
+                for theta in (np.arccos(aim / r), -np.arccos(aim / r)):
+                    t = theta - phi
+                    t += L("6.28318530717958647692528676655900577") * np.round((t0 - t) / (L("6.28318530717958647692528676655900577")))
+                    if abs(t - t0) < 0.1 and low <= t <= high:
+                        break
+                else:
+                    continue
+                # a far position: as many whole turns more as make the frequency one of 0.5 to 1
+                turns = 0 if p == 1 else int(rng.uniform(0.5, 1) * p / 6.3)
+                f[j] = np.float64((t + turns * L("6.28318530717958647692528676655900577")) / p)
+                ya, yb = turned(L(x[0]), L(y[0]), p, f[j:j + 1])
+                near_tie = min(abs(abs(v) / L(border(float(abs(v)))) - 1) if abs(v) >= 16 else 1 for v in (ya[0], yb[0]))
+                if near_tie > L(2) ** -41 and abs(yb[0]) > 16:
+                    a[j], b[j] = x[0], y[0]
+                    break
+        ya, yb = turned(a.astype(L), b.astype(L), p, f)
+        row = np.empty(2 * n)
+        want = np.empty(2 * n, dtype=L)
+        lo, hi = (slice(0, None, 2), slice(1, None, 2)) if interleaved else (slice(0, n), slice(n, None))
+        row[lo], row[hi], want[lo], want[hi] = a, b, nearest(ya), nearest(yb)
+        got, _, ks, _ = one_token(P, torch.from_numpy(row).to(torch.bfloat16)[None], f, position=p, interleaved=interleaved)
+        assert ks[0] == 1 and np.array_equal(got[0], want), int((got[0] != want).sum())
+
+
 @pytest.mark.parametrize("hd,n,interleaved", [(128, 16, False), (64, 8, True), (64, 0, False), (96, 5, False)])
 def test_codes_of_infinities_under_a_norm(P, hd, n, interleaved):
     """A key with an infinity is NaN where that reaches and zero elsewhere, whatever the tokens beside it hold; one call and one by one."""
@@ -201,3 +289,36 @@ def test_codes_beyond_fp32(P):
     P.cache_append(k, k, pool.k, pool.v, pool.tables, pool.lens, **pool.kw, freqs=f, k_norm=torch.ones(hd, device="cuda"))
     codes = pool.k.transpose(1, 2)[page, row].double()
     assert not bool(codes[large].any()) and bool(torch.isfinite(codes).all()) and bool((codes[~large].abs().amax(-1) > 0).all())
+
+
+@pytest.mark.parametrize("ctx", [0, 5, 15])
+def test_codes_are_the_64_bit_values_rounded(P, ctx):
+    """Half a million codes under an amplitude and an eps that fp32 does not hold, at far positions and in blocks begun before: those
+    that 64 bits give, but for values within 2^-33 of their pair of a border."""
+    g, T, KH, hd, amp, eps = gen(66), 1024, 4, 128, 1.1, 1.1e-5
+    pool = Pool(g, torch.bfloat16, True, KH, hd, 64, [T + ctx])
+    k = rand(g, T, KH, hd, dtype=torch.bfloat16, scale=2.0)
+    f = P.rotary_frequencies(hd, 1e6, device="cuda")[0]
+    w = 1 + 0.3 * torch.randn(hd, generator=g, device="cuda")
+    pos = torch.randint(0, 1 << 17, (T,), generator=g, device="cuda").int()
+    old = pool.ks[int(pool.tables[0, 0]), :, 0].double()
+    P.cache_append(k, k, pool.k, pool.v, pool.tables, pool.lens, **pool.kw, freqs=f, k_norm=w, amplitude=amp, eps=eps, positions=pos)
+    x = k.double()
+    x = x / torch.sqrt((x * x).mean(-1, keepdim=True) + eps) * w.double()
+    t = (pos.double()[:, None] * f)[:, None]
+    a, b = x[..., :hd // 2], x[..., hd // 2:]
+    y = amp * torch.cat([a * t.cos() - b * t.sin(), b * t.cos() + a * t.sin()], -1)
+    p = torch.arange(ctx, T + ctx, device="cuda")
+    page, row = pool.tables[0].long()[p // 64], p % 64
+    scale = pool.ks[page, :, row // 16].double()
+    for blk in range(p[0] // 16, p[-1] // 16 + 1):
+        m = p // 16 == blk
+        need = torch.exp2(torch.ceil(torch.log2(y[m].abs().amax((0, 2)) / 448)))
+        assert torch.equal(scale[m][0], torch.maximum(need, old) if ctx and blk == 0 else need)
+    y = y / scale[..., None]
+    step = torch.exp2(torch.clamp(torch.floor(torch.log2(y.abs().clamp(min=2.0 ** -30))), min=-6) - 3)
+    u, pair = y / step, amp * torch.hypot(a, b).repeat(1, 1, 2) / scale[..., None] / step
+    clear = ((u - u.floor()) - 0.5).abs() > 2.0 ** -33 * pair        # t is off by 2^17 2^-53 radians at most here
+    got = pool.k.transpose(1, 2)[page, row].double()
+    want = torch.round(u) * step
+    assert torch.equal(got[clear], want[clear]) and int((~clear).sum()) < 8

@@ -8,9 +8,9 @@
 // Rotation:  a head's first 2 n dimensions are n pairs, (j, j + n) or
 //            (2 j, 2 j + 1); pair j of position p turns by p f_j:
 //            a <- s (a cos - b sin), b <- s (b cos + a sin).
-// All in fp32 and rounded once.  The angle is taken in turns in 64 bits,
-// reduced there to an eighth of a turn: in 32 bits a position of 100,000 would
-// leave a sine 7 bits.
+// All in fp32 and rounded once.  The angle is taken in turns in 64 bits, its product
+// with the position whole, and reduced there to an eighth of a turn: in 32 bits a
+// position of 100,000 would leave a sine 7 bits.
 //
 // Pages of 8 bits (e4m3) have a scale for each key head and block of 16 tokens,
 // a power of two: e4m3 keeps 4 bits of every value whatever the factor, so a
@@ -64,16 +64,38 @@ struct CacheArgs {
   float amp, eps, inv_hd;   // inv_hd: 1 / hd
 };
 
-// cos and sin of p f radians, times amp: Taylor's series at an eighth of a turn at
-// most, off by 2^-33.
+// p f radians in turns, as whole quarters and a rest of an eighth at most.  f / 2 pi is
+// a sum of two doubles and the product with p is kept whole, so the rest is off by
+// 2^-56 of a turn however far p is.
+struct Turn {
+  double quarters, rest;
+  __device__ __forceinline__ Turn(int p, double f) {
+    const double per = 0.15915494309189535, per_low = -9.839338337591243e-18;   // 1 / 2 pi
+    const double h = f * per, l = fma(f, per_low, fma(f, per, -h)), t = p * h;
+    quarters = rint(4.0 * t);
+    rest = fma(-0.25, quarters, t) + fma((double)p, l, fma((double)p, h, -t));
+  }
+  __device__ __forceinline__ double2 whole(double s, double c) const {   // of the rest's sine and cosine: cosine, sine
+    const int q = (int)((long long)quarters & 3);
+    const double cs = q & 1 ? -s : c, sn = q & 1 ? c : s;
+    return q & 2 ? make_double2(-cs, -sn) : make_double2(cs, sn);
+  }
+};
+// cos and sin of p f radians, times amp, for fp32: Taylor's series at an eighth of a
+// turn at most, the sine off by 2^-29, the cosine by 2^-33.
 __device__ __forceinline__ double2 rope_angle(int p, double f, float amp) {
-  const double t = (double)p * (f * 0.15915494309189533577);   // turns
-  const double n = rint(4.0 * t), x = 6.2831853071795864769 * (t - 0.25 * n), y = x * x;
+  const Turn t(p, f);
+  const double x = 6.2831853071795864769 * t.rest, y = x * x;
   const double s = amp * x * (1 + y * (-1.0 / 6 + y * (1.0 / 120 + y * (-1.0 / 5040 + y * (1.0 / 362880)))));
   const double c = amp * (1 + y * (-1.0 / 2 + y * (1.0 / 24 + y * (-1.0 / 720 + y * (1.0 / 40320 - y * (1.0 / 3628800))))));
-  const int quarter = (int)((long long)n & 3);
-  const double cs = quarter & 1 ? -s : c, sn = quarter & 1 ? c : s;
-  return quarter & 2 ? make_double2(-cs, -sn) : make_double2(cs, sn);
+  return t.whole(s, c);
+}
+// The same for fp64.
+__device__ __forceinline__ double2 rope_angle64(int p, double f, float amp) {
+  const Turn t(p, f);
+  double s, c;
+  sincospi(2.0 * t.rest, &s, &c);
+  return t.whole(amp * s, amp * c);
 }
 
 // Eight values of a row are a lane's: the pairs 4 c .. 4 c + 3 of the row's hd / 2.
@@ -450,7 +472,7 @@ __device__ __noinline__ Codes exact_codes(const LanePairs m, const uint4* row, c
     double u = xa * r, v = xb * r;
     if (NORM) u *= w[i], v *= w[PC_PAIRS + i];
     if (m.turns(i)) {
-      const double2 t = rope_angle(pos, freqs[4 * m.c + i], amp);
+      const double2 t = rope_angle64(pos, freqs[4 * m.c + i], amp);
       const double z = u * t.x - v * t.y;
       v = v * t.x + u * t.y, u = z;
     }
