@@ -229,6 +229,29 @@ def test_codes_of_angles_next_to_a_border(P, p, low, high, interleaved):
         assert ks[0] == 1 and np.array_equal(got[0], want), int((got[0] != want).sum())
 
 
+def test_codes_of_amplitudes_and_eps_next_to_a_border(P):
+    """An amplitude and an eps that fp32 does not hold decide codes."""
+    rng, n = np.random.default_rng(62), 32
+    for _ in range(8):
+        (_, x) = bf16(rng, 20, 200, 1)
+        for side in (1, -1):
+            amp = float(L(border(x[0] * 1.1)) / L(x[0]) * (1 + side * L(2) ** -30))
+            row = np.full(2 * n, x[0])
+            row[0] = 256.0                                         # the scale is 1
+            got = one_token(P, torch.from_numpy(row).to(torch.bfloat16)[None], np.zeros(n), amplitude=amp)[0]
+            assert np.array_equal(got[0, 1:n], nearest(L(x[0]) * L(amp) * np.ones(n - 1, dtype=L)))
+            # x w / sqrt(x^2 / hd + eps)
+            w = np.float32(rng.uniform(30, 60))
+            y = border(float(w) / math.sqrt(1 / 64 + 0.1 * rng.uniform(0.5, 2)))
+            eps = float((L(w) / (L(y) * (1 + side * L(2) ** -31))) ** 2 - L(1) / 64)
+            one = torch.zeros(1, 64, dtype=torch.bfloat16)
+            one[0, 5] = 1.0
+            wk = torch.full((64,), float(w), device="cuda")
+            got, _, ks, _ = one_token(P, one, None, eps=eps, k_norm=wk)
+            want = nearest(L(w) / np.sqrt(L(1) / 64 + L(eps)) / ks[0])
+            assert got[0, 5] == want and not np.delete(got[0], 5).any()
+
+
 @pytest.mark.parametrize("hd,n,interleaved", [(128, 16, False), (64, 8, True), (64, 0, False), (96, 5, False)])
 def test_codes_of_infinities_under_a_norm(P, hd, n, interleaved):
     """A key with an infinity is NaN where that reaches and zero elsewhere, whatever the tokens beside it hold; one call and one by one."""

@@ -61,7 +61,8 @@ struct CacheArgs {
   long long st;               // tables' row
   int T, B, per, H, KH, hd, nf, n_pages, cols, shift, token_ctas, window, tokens, parts, each;
   int interleaved;
-  float amp, eps, inv_hd;   // inv_hd: 1 / hd
+  double amp, eps64;        // as they were given
+  float eps, inv_hd;        // inv_hd: 1 / hd
 };
 
 // p f radians in turns, as whole quarters and a rest of an eighth at most.  f / 2 pi is
@@ -83,7 +84,7 @@ struct Turn {
 };
 // cos and sin of p f radians, times amp, for fp32: Taylor's series at an eighth of a
 // turn at most, the sine off by 2^-29, the cosine by 2^-33.
-__device__ __forceinline__ double2 rope_angle(int p, double f, float amp) {
+__device__ __forceinline__ double2 rope_angle(int p, double f, double amp) {
   const Turn t(p, f);
   const double x = 6.2831853071795864769 * t.rest, y = x * x;
   const double s = amp * x * (1 + y * (-1.0 / 6 + y * (1.0 / 120 + y * (-1.0 / 5040 + y * (1.0 / 362880)))));
@@ -91,7 +92,7 @@ __device__ __forceinline__ double2 rope_angle(int p, double f, float amp) {
   return t.whole(s, c);
 }
 // The same for fp64.
-__device__ __forceinline__ double2 rope_angle64(int p, double f, float amp) {
+__device__ __forceinline__ double2 rope_angle64(int p, double f, double amp) {
   const Turn t(p, f);
   double s, c;
   sincospi(2.0 * t.rest, &s, &c);
@@ -299,7 +300,7 @@ __device__ __forceinline__ void keep_weights(const CacheArgs& a, CacheShared& sh
     sh.w[2][at] = 1.f;
   }
 }
-__device__ __forceinline__ void keep_turn(float (*turn)[PC_PAIRS], int pair, int pos, double f, float amp) {
+__device__ __forceinline__ void keep_turn(float (*turn)[PC_PAIRS], int pair, int pos, double f, double amp) {
   const double2 t = rope_angle(pos, f, amp);
   turn[0][pair] = (float)t.x, turn[1][pair] = (float)t.y;
 }
@@ -452,7 +453,7 @@ __device__ __forceinline__ float to_odd(double x) {   // rounds to any fewer bit
 }
 // row: null for lanes without values; eps: negative where there is no norm.
 template <typename T, int LPR, bool VEC, bool NORM>
-__device__ __noinline__ Codes exact_codes(const LanePairs m, const uint4* row, const float* w, const double* freqs, int pos, float amp, float eps,
+__device__ __noinline__ Codes exact_codes(const LanePairs m, const uint4* row, const float* w, const double* freqs, int pos, double amp, double eps,
                                           float inv, double per_hd) {
   Pairs x = no_pairs();
   if (row) read_pairs<T, VEC>(x, m, row);
@@ -465,7 +466,7 @@ __device__ __noinline__ Codes exact_codes(const LanePairs m, const uint4* row, c
     sum = part[0] + part[1];
 #pragma unroll
     for (int o = LPR / 2; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    if (eps >= 0.f) r *= sum > FLT_MAX ? 0.0 : rsqrt(sum * per_hd + (double)eps);   // what fp32 does not hold counts as infinite there too
+    if (eps >= 0) r *= sum > FLT_MAX ? 0.0 : rsqrt(sum * per_hd + eps);   // what fp32 does not hold counts as infinite there too
   }
   Pairs y;
   auto pair = [&](int i, float xa, float xb, float& ya, float& yb) {
@@ -621,7 +622,7 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
       const int j = (__ffs(again) - 1) * RPP + lane / LPR;
       const bool there = j < n && m.any();
       const Codes y = exact_codes<T, LPR, VEC, NORM>(m, there ? ring + j * LPR : nullptr, w[0], a.freqs, sh.at[j0 + min(j, n - 1)], a.amp,
-                                                     a.kw ? a.eps : -1.f, inv, 1.0 / a.hd);
+                                                     a.kw ? a.eps64 : -1.0, inv, 1.0 / a.hd);
       if (there) {
         uint8_t* const at = rows + (off + j) * pitch;
         const Codes z = load_codes<VEC>(at, m);   // what fp32 does not hold stays NaN
@@ -806,7 +807,7 @@ static int rotary(ArgCheck& c, const RotaryRecord& r) {
   a.qw = (const float*)r.q_norm, a.kw = (const float*)r.k_norm;
   for (int i = 0; i < 2; i++) a.sq[i] = t[i], a.sk[i] = t[2 + i], a.sqo[i] = t[4 + i], a.sko[i] = t[6 + i];
   a.T = (int)r.n_tokens, a.H = (int)r.n_heads, a.KH = (int)r.n_kv_heads, a.hd = (int)r.head_dim, a.nf = (int)r.n_freqs;
-  a.interleaved = r.interleaved != 0, a.amp = (float)r.amplitude, a.eps = (float)r.eps, a.inv_hd = 1.f / a.hd;
+  a.interleaved = r.interleaved != 0, a.amp = r.amplitude, a.eps64 = r.eps, a.eps = (float)r.eps, a.inv_hd = 1.f / a.hd;
   cudaStream_t s = static_cast<cudaStream_t>(r.stream);
   const long long grid = token_ctas(a, (long long)a.H + a.KH, PC_PER_SM);
   if (!c.need(grid < 1ll << 31, "too many rows")) return c.rc;
@@ -853,7 +854,7 @@ static int append(ArgCheck& c, const AppendRecord& r) {
   a.st = pool.st;
   a.T = (int)r.n_tokens, a.B = (int)r.batch, a.per = a.T / a.B, a.H = (int)r.n_heads, a.KH = (int)r.n_kv_heads, a.hd = (int)r.head_dim;
   a.nf = (int)r.n_freqs, a.n_pages = (int)r.n_pages, a.cols = (int)r.table_cols, a.shift = pool.shift;
-  a.interleaved = r.interleaved != 0, a.amp = (float)r.amplitude, a.eps = (float)r.eps, a.inv_hd = 1.f / a.hd;
+  a.interleaved = r.interleaved != 0, a.amp = r.amplitude, a.eps64 = r.eps, a.eps = (float)r.eps, a.inv_hd = 1.f / a.hd;
   long long ctas = r.page_bits == 16 ? token_ctas(a, (long long)a.H + 2 * a.KH, PC_PER_SM) : a.H ? token_ctas(a, a.H, PC_PER_SM - 1) : 0;
   if (!ctas) a.each = 2;
   if (r.page_bits == 8) {   // the runs' CTAs behind: one of them beside those that rotate, on each SM
