@@ -252,6 +252,29 @@ def test_codes_of_amplitudes_and_eps_next_to_a_border(P):
             assert got[0, 5] == want and not np.delete(got[0], 5).any()
 
 
+def test_scales_next_to_a_border(P):
+    """Blocks whose largest value is 448 times a power of two, 2^-31 of it more or less: the scale goes by the exact value."""
+    rng, KH, n = np.random.default_rng(63), 16, 32
+    for _ in range(12):
+        rows, f, top = np.zeros((KH, 2 * n)), np.zeros(n), np.zeros(KH, dtype=L)
+        for h in range(KH):
+            while True:
+                (_, x), (_, y) = bf16(rng, 300, 640, 1), bf16(rng, -400, 400, 1)
+                phi = np.arctan2(L(y[0]), L(x[0]))
+                r = np.sqrt(L(x[0]) ** 2 + L(y[0]) ** 2)
+                if 448 / math.cos(0.3) < r < 448 / math.cos(0.7):
+                    break
+            t = np.arccos(448 * (1 + L(2) ** -31 * (1 if h % 2 else -1)) / r) - phi
+            f[h] = np.float64(t)
+            rows[h, h], rows[h, n + h] = x[0], y[0]
+            top[h] = np.abs(turned(L(x[0]), L(y[0]), 1, f[h:h + 1])).max()
+        assert bool((np.abs(top / 448 - 1) > L(2) ** -33).all())
+        got, _, ks, vs = one_token(P, torch.from_numpy(rows).to(torch.bfloat16), f, position=1)
+        assert np.array_equal(ks, np.where(top > 448, 2, 1).astype(L)), (ks, top - 448)
+        want = np.where(top > 448, 224, 448)
+        assert np.array_equal(np.abs(got).max(1), want.astype(L))
+
+
 @pytest.mark.parametrize("hd,n,interleaved", [(128, 16, False), (64, 8, True), (64, 0, False), (96, 5, False)])
 def test_codes_of_infinities_under_a_norm(P, hd, n, interleaved):
     """A key with an infinity is NaN where that reaches and zero elsewhere, whatever the tokens beside it hold; one call and one by one."""

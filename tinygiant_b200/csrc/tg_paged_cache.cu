@@ -61,8 +61,8 @@ struct CacheArgs {
   long long st;               // tables' row
   int T, B, per, H, KH, hd, nf, n_pages, cols, shift, token_ctas, window, tokens, parts, each;
   int interleaved;
-  double amp, eps64;        // as they were given
-  float eps, inv_hd;        // inv_hd: 1 / hd
+  double amp, eps64, inv_hd64;   // as they were given; 1 / hd
+  float eps, inv_hd;
 };
 
 // p f radians in turns, as whole quarters and a rest of an eighth at most.  f / 2 pi is
@@ -425,14 +425,16 @@ __device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, 
   }
 }
 
-// Codes are what the formulas' exact values round to, so that they do not depend on
-// how a sum was taken.  In fp32 the sum of squares is 9 roundings deep, half of
+// Codes are what the formulas' values in 64 bits round to, so that they do not depend
+// on how a sum was taken.  In fp32 the sum of squares is 9 roundings deep, half of
 // which reach its root, which has 4 2^-24 of its own; with the mean, two products
 // and a rotation a value y is off by at most 14.5 2^-24 |(a, b)| <= PC_OFF (|y_a| +
 // |y_b|) of its pair.  Where both ends of that interval round to one code, that is
 // it; the rows of the others, one value in 7,000, are worked out in 64 bits by the
 // whole warp.  The test for doubt takes 2 of 8,192 tokens' 42 us and those rows 3.
-constexpr float PC_OFF = 0x1p-20f;
+// So it is with the scale, where the largest value, off by at most 2 PC_OFF of
+// itself, may lie on either side of a border (one block in 100,000).
+constexpr float PC_OFF = 0x1p-20f, PC_OFF_MOST = 0x1p-18f;
 __device__ __forceinline__ Codes codes_within(const Pairs& x, float off, bool& doubt) {
   Pairs lo, hi;
 #pragma unroll
@@ -447,17 +449,18 @@ __device__ __forceinline__ Codes codes_within(const Pairs& x, float off, bool& d
   doubt = y.a != z.a || y.b != z.b;
   return y;
 }
-__device__ __forceinline__ float to_odd(double x) {   // rounds to any fewer bits as x does; NaN where x is not finite
+__device__ __forceinline__ float to_odd(double x) {   // rounds to any fewer bits as x does; NaN where fp32 does not hold x
   const float y = __double2float_rz(x);
-  return x - x != 0 ? NAN : (double)y == x ? y : __uint_as_float(__float_as_uint(y) | 1);
+  return !(fabs(x) <= FLT_MAX) ? NAN : (double)y == x ? y : __uint_as_float(__float_as_uint(y) | 1);
 }
-// row: null for lanes without values; eps: negative where there is no norm.
+// A key row's values times inv, a power of two, to_odd.  row: null for lanes without
+// values; w: the lane's weights.
 template <typename T, int LPR, bool VEC, bool NORM>
-__device__ __noinline__ Codes exact_codes(const LanePairs m, const uint4* row, const float* w, const double* freqs, int pos, double amp, double eps,
-                                          float inv, double per_hd) {
+__device__ __noinline__ Pairs exact_pairs(const CacheArgs& a, const uint4* row, const float* w, int pos, float inv) {
+  const LanePairs m(a, threadIdx.x % LPR);
   Pairs x = no_pairs();
   if (row) read_pairs<T, VEC>(x, m, row);
-  double r = inv;   // a power of two
+  double r = inv;
   if (NORM) {
     double part[2], sum;
 #pragma unroll
@@ -466,14 +469,14 @@ __device__ __noinline__ Codes exact_codes(const LanePairs m, const uint4* row, c
     sum = part[0] + part[1];
 #pragma unroll
     for (int o = LPR / 2; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    if (eps >= 0) r *= sum > FLT_MAX ? 0.0 : rsqrt(sum * per_hd + eps);   // what fp32 does not hold counts as infinite there too
+    if (a.kw) r *= sum > FLT_MAX ? 0.0 : rsqrt(sum * a.inv_hd64 + a.eps64);   // what fp32 does not hold counts as infinite there too
   }
   Pairs y;
   auto pair = [&](int i, float xa, float xb, float& ya, float& yb) {
     double u = xa * r, v = xb * r;
     if (NORM) u *= w[i], v *= w[PC_PAIRS + i];
     if (m.turns(i)) {
-      const double2 t = rope_angle64(pos, freqs[4 * m.c + i], amp);
+      const double2 t = rope_angle64(pos, a.freqs[4 * m.c + i], a.amp);
       const double z = u * t.x - v * t.y;
       v = v * t.x + u * t.y, u = z;
     }
@@ -481,7 +484,7 @@ __device__ __noinline__ Codes exact_codes(const LanePairs m, const uint4* row, c
   };
   pair(0, x.a[0].x, x.b[0].x, y.a[0].x, y.b[0].x), pair(1, x.a[0].y, x.b[0].y, y.a[0].y, y.b[0].y);
   pair(2, x.a[1].x, x.b[1].x, y.a[1].x, y.b[1].x), pair(3, x.a[1].y, x.b[1].y, y.a[1].y, y.b[1].y);
-  return codes_of(y);
+  return y;
 }
 
 // Runs of 8-bit blocks whose first token is one of the `window` packed tokens
@@ -525,6 +528,7 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
   const int items = sh.runs * 2 * a.KH;
   const float* const w[2] = {sh.w[1] + (m.any() ? 4 * m.c : 0), sh.w[1] + (m.any() ? 4 * m.c : 0)};
   const uint32_t on[2] = {a.kw ? ~0u : 0, a.kw ? ~0u : 0};
+  const bool touched = (NORM && a.kw) || a.nf > 0;
   const float off_by = (NORM && a.kw) || 4 * m.c < a.nf ? PC_OFF : 0.f;   // values that no one touches are exact
   uint4* ring = pc_ring + wid * PAGED_BLOCK * LPR;   // an item's rows
   auto fetch = [&](int item) {
@@ -585,6 +589,23 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
       if (odd || amax < 0x7f800000u) break;
       odd = true;
     }
+    auto exact = [&](int u, float times) {   // of the rows u RPP + lane / LPR
+      const int j = u * RPP + lane / LPR;
+      return exact_pairs<T, LPR, VEC, NORM>(a, j < n && m.any() ? ring + j * LPR : nullptr, w[0], sh.at[j0 + min(j, n - 1)], times);
+    };
+    const float top = __uint_as_float(amax);
+    if (!is_v && touched &&
+        paged_scale_exp(__float_as_uint(top - PC_OFF_MOST * top)) != paged_scale_exp(__float_as_uint(top + PC_OFF_MOST * top))) {
+      float most = 0.f;
+#pragma unroll 1
+      for (int u = 0; u * RPP < n; u++) {
+        const Pairs x = exact(u, 1.f);
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+          most = fmaxf(fmaxf(most, fmaxf(fabsf(x.a[e].x), fabsf(x.a[e].y))), fmaxf(fabsf(x.b[e].x), fabsf(x.b[e].y)));
+      }
+      amax = __reduce_max_sync(~0u, __float_as_uint(most));
+    }
     const float need = __uint_as_float((uint32_t)(paged_scale_exp(amax) + 127) << 23);
     const float scale = fmaxf(need, before), inv = 1.f / scale;
     if (off && scale > before) {   // the earlier tokens' codes under the larger scale
@@ -619,11 +640,9 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
       }
     }
     for (again = __reduce_or_sync(~0u, again); again; again &= again - 1) {
-      const int j = (__ffs(again) - 1) * RPP + lane / LPR;
-      const bool there = j < n && m.any();
-      const Codes y = exact_codes<T, LPR, VEC, NORM>(m, there ? ring + j * LPR : nullptr, w[0], a.freqs, sh.at[j0 + min(j, n - 1)], a.amp,
-                                                     a.kw ? a.eps64 : -1.0, inv, 1.0 / a.hd);
-      if (there) {
+      const int u = __ffs(again) - 1, j = u * RPP + lane / LPR;
+      const Codes y = codes_of(exact(u, inv));
+      if (j < n && m.any()) {
         uint8_t* const at = rows + (off + j) * pitch;
         const Codes z = load_codes<VEC>(at, m);   // what fp32 does not hold stays NaN
         const uint32_t na = e4m3_nans(z.a), nb = e4m3_nans(z.b);
@@ -643,7 +662,7 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
 // the same with 4 key heads to 8-bit pages 42, without norms 34, where 160 MB take
 // 24.  A chunk of 2,048 tokens 18; two tokens 4, of which an empty kernel is 2.
 template <typename T, int LPR, bool VEC, int MODE, bool NORM, int R>
-__global__ void __launch_bounds__(PC_THREADS, PC_PER_SM) cache_kernel(const CacheArgs a) {
+__global__ void __launch_bounds__(PC_THREADS, PC_PER_SM) cache_kernel(const __grid_constant__ CacheArgs a) {
   __shared__ CacheShared sh;
   pdl_wait();
   if (MODE == PC_PAGES8 && blockIdx.x >= a.token_ctas) {
@@ -807,7 +826,7 @@ static int rotary(ArgCheck& c, const RotaryRecord& r) {
   a.qw = (const float*)r.q_norm, a.kw = (const float*)r.k_norm;
   for (int i = 0; i < 2; i++) a.sq[i] = t[i], a.sk[i] = t[2 + i], a.sqo[i] = t[4 + i], a.sko[i] = t[6 + i];
   a.T = (int)r.n_tokens, a.H = (int)r.n_heads, a.KH = (int)r.n_kv_heads, a.hd = (int)r.head_dim, a.nf = (int)r.n_freqs;
-  a.interleaved = r.interleaved != 0, a.amp = r.amplitude, a.eps64 = r.eps, a.eps = (float)r.eps, a.inv_hd = 1.f / a.hd;
+  a.interleaved = r.interleaved != 0, a.amp = r.amplitude, a.eps64 = r.eps, a.eps = (float)r.eps, a.inv_hd64 = 1.0 / a.hd, a.inv_hd = 1.f / a.hd;
   cudaStream_t s = static_cast<cudaStream_t>(r.stream);
   const long long grid = token_ctas(a, (long long)a.H + a.KH, PC_PER_SM);
   if (!c.need(grid < 1ll << 31, "too many rows")) return c.rc;
@@ -854,7 +873,7 @@ static int append(ArgCheck& c, const AppendRecord& r) {
   a.st = pool.st;
   a.T = (int)r.n_tokens, a.B = (int)r.batch, a.per = a.T / a.B, a.H = (int)r.n_heads, a.KH = (int)r.n_kv_heads, a.hd = (int)r.head_dim;
   a.nf = (int)r.n_freqs, a.n_pages = (int)r.n_pages, a.cols = (int)r.table_cols, a.shift = pool.shift;
-  a.interleaved = r.interleaved != 0, a.amp = r.amplitude, a.eps64 = r.eps, a.eps = (float)r.eps, a.inv_hd = 1.f / a.hd;
+  a.interleaved = r.interleaved != 0, a.amp = r.amplitude, a.eps64 = r.eps, a.eps = (float)r.eps, a.inv_hd64 = 1.0 / a.hd, a.inv_hd = 1.f / a.hd;
   long long ctas = r.page_bits == 16 ? token_ctas(a, (long long)a.H + 2 * a.KH, PC_PER_SM) : a.H ? token_ctas(a, a.H, PC_PER_SM - 1) : 0;
   if (!ctas) a.each = 2;
   if (r.page_bits == 8) {   // the runs' CTAs behind: one of them beside those that rotate, on each SM
