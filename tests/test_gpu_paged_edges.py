@@ -275,6 +275,49 @@ def test_scales_next_to_a_border(P):
         assert np.array_equal(np.abs(got).max(1), want.astype(L))
 
 
+def test_codes_under_an_earlier_scale_of_any_kind(P):
+    """Earlier tokens' scales that are no powers of two: they stay if they are larger, and the new codes are the nearest under them."""
+    rng, KH, hd = np.random.default_rng(64), 32, 64
+    for _ in range(6):
+        rows = np.zeros((KH, hd))
+        scale = np.zeros(KH, dtype=np.float32)
+        for h in range(KH):
+            x = torch.from_numpy(rng.uniform(0.5, 1, hd)).to(torch.bfloat16).double().numpy()
+            near = np.float32(x[0] / border(rng.uniform(60, 105)))   # the largest value is below 224 scales, so this scale stays
+            while True:   # a scale that takes the first value next to a border, and none to a tie
+                near = np.nextafter(near, np.float32(2))
+                y = x.astype(L) / L(near)
+                step = L(2) ** (np.floor(np.log2(y)) - 3)
+                if bool((np.abs(y / step % 1 - 0.5) > L(2) ** -40).all()):
+                    break
+            rows[h], scale[h] = x, near
+        before = torch.from_numpy(scale).cuda()
+        k, v, ks, vs = one_token(P, torch.from_numpy(rows).to(torch.bfloat16), None, ctx=3, before=before)
+        assert np.array_equal(ks, scale.astype(L)) and np.array_equal(vs, scale.astype(L))
+        want = nearest(rows.astype(L) / scale.astype(L)[:, None])
+        assert np.array_equal(k, want) and np.array_equal(v, want), (int((k != want).sum()), int((v != want).sum()))
+    # and where they grow, the earlier codes are the nearest to what they were
+    codes = torch.arange(127, device="cuda").to(torch.uint8)[:112].view(1, 1, 1, 112).expand(1, KH, 16, 112).contiguous()
+    k_pages, v_pages = codes.view(E4M3).clone(), codes.view(E4M3).clone()
+    old = np.zeros(KH, dtype=np.float32)
+    for h in range(KH):   # code 36 (3.0 = 1.5 x 2) or so times old is next to a border under the scale 1
+        c = E4M3_VALUES[rng.integers(60, 100)]
+        y = border(float(c) * rng.uniform(16.5 / float(c), 0.99)) if c > 17 else None
+        old[h] = np.nextafter(np.float32(0.7 if y is None else y / float(c)), np.float32(2))
+    ks, vs = (torch.from_numpy(old).cuda().view(1, KH, 1).clone() for _ in range(2))
+    x = torch.full((1, KH, 112), 300.0, dtype=torch.bfloat16, device="cuda")
+    P.cache_append(x, x, k_pages, v_pages, ints(0).view(1, 1), ints(16), k_scales=ks, v_scales=vs)
+    assert bool((ks == 1).all())
+    y = E4M3_VALUES[:112][None] * old.astype(L)[:, None]
+    d = np.abs(y[..., None] - E4M3_VALUES)
+    want = E4M3_VALUES[d.argmin(-1)]
+    two = np.partition(d, 1, axis=-1)
+    clear = two[..., 1] - two[..., 0] > np.abs(y) * L(2) ** -44     # ties aside
+    for pages in (k_pages, v_pages):
+        got = pages[0, :, 0].float().cpu().numpy().astype(L)
+        assert np.array_equal(got[clear], want[clear])
+
+
 @pytest.mark.parametrize("hd,n,interleaved", [(128, 16, False), (64, 8, True), (64, 0, False), (96, 5, False)])
 def test_codes_of_infinities_under_a_norm(P, hd, n, interleaved):
     """A key with an infinity is NaN where that reaches and zero elsewhere, whatever the tokens beside it hold; one call and one by one."""

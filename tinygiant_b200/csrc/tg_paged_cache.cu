@@ -453,10 +453,10 @@ __device__ __forceinline__ float to_odd(double x) {   // rounds to any fewer bit
   const float y = __double2float_rz(x);
   return !(fabs(x) <= FLT_MAX) ? NAN : (double)y == x ? y : __uint_as_float(__float_as_uint(y) | 1);
 }
-// A key row's values times inv, a power of two, to_odd.  row: null for lanes without
-// values; w: the lane's weights.
+// A row's values times inv, to_odd.  row: null for lanes without values; w: the lane's
+// weights of a key's norm, null for a row of v.
 template <typename T, int LPR, bool VEC, bool NORM>
-__device__ __noinline__ Pairs exact_pairs(const CacheArgs& a, const uint4* row, const float* w, int pos, float inv) {
+__device__ __noinline__ Pairs exact_pairs(const CacheArgs& a, const uint4* row, const float* w, int pos, double inv) {
   const LanePairs m(a, threadIdx.x % LPR);
   Pairs x = no_pairs();
   if (row) read_pairs<T, VEC>(x, m, row);
@@ -469,13 +469,13 @@ __device__ __noinline__ Pairs exact_pairs(const CacheArgs& a, const uint4* row, 
     sum = part[0] + part[1];
 #pragma unroll
     for (int o = LPR / 2; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    if (a.kw) r *= sum > FLT_MAX ? 0.0 : rsqrt(sum * a.inv_hd64 + a.eps64);   // what fp32 does not hold counts as infinite there too
+    if (w && a.kw) r *= sum > FLT_MAX ? 0.0 : rsqrt(sum * a.inv_hd64 + a.eps64);   // what fp32 does not hold counts as infinite there too
   }
   Pairs y;
   auto pair = [&](int i, float xa, float xb, float& ya, float& yb) {
     double u = xa * r, v = xb * r;
-    if (NORM) u *= w[i], v *= w[PC_PAIRS + i];
-    if (m.turns(i)) {
+    if (NORM && w) u *= w[i], v *= w[PC_PAIRS + i];
+    if (w && m.turns(i)) {
       const double2 t = rope_angle64(pos, a.freqs[4 * m.c + i], a.amp);
       const double z = u * t.x - v * t.y;
       v = v * t.x + u * t.y, u = z;
@@ -589,9 +589,9 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
       if (odd || amax < 0x7f800000u) break;
       odd = true;
     }
-    auto exact = [&](int u, float times) {   // of the rows u RPP + lane / LPR
+    auto exact = [&](int u, double times) {   // of the rows u RPP + lane / LPR
       const int j = u * RPP + lane / LPR;
-      return exact_pairs<T, LPR, VEC, NORM>(a, j < n && m.any() ? ring + j * LPR : nullptr, w[0], sh.at[j0 + min(j, n - 1)], times);
+      return exact_pairs<T, LPR, VEC, NORM>(a, j < n && m.any() ? ring + j * LPR : nullptr, is_v ? nullptr : w[0], sh.at[j0 + min(j, n - 1)], times);
     };
     const float top = __uint_as_float(amax);
     if (!is_v && touched &&
@@ -599,7 +599,7 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
       float most = 0.f;
 #pragma unroll 1
       for (int u = 0; u * RPP < n; u++) {
-        const Pairs x = exact(u, 1.f);
+        const Pairs x = exact(u, 1.0);
 #pragma unroll
         for (int e = 0; e < 2; e++)
           most = fmaxf(fmaxf(most, fmaxf(fabsf(x.a[e].x), fabsf(x.a[e].y))), fmaxf(fabsf(x.b[e].x), fabsf(x.b[e].y)));
@@ -608,16 +608,21 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
     }
     const float need = __uint_as_float((uint32_t)(paged_scale_exp(amax) + 127) << 23);
     const float scale = fmaxf(need, before), inv = 1.f / scale;
+    const bool fine = __float_as_uint(scale) & 0x7fffffu;   // an earlier scale that is no power of two: two roundings more, v's values too
+    const float off_scaled = (is_v ? 0.f : off_by) + (fine ? 0x1p-22f : 0.f);
     if (off && scale > before) {   // the earlier tokens' codes under the larger scale
-      const float less = before * inv;
+      const float less = before * inv;   // has 24 bits, a code 4
+      auto two = [&](float2 c) {
+        auto odd = [&](float x) {
+          const float y = __fmul_rz(x, less);
+          return fmaf(x, less, -y) == 0.f ? y : __uint_as_float(__float_as_uint(y) | 1);
+        };
+        return e4m3_pair(odd(c.x), odd(c.y));
+      };
       for (int i8 = lane; i8 < off * (a.hd / 8); i8 += 32) {
         uint2* at = reinterpret_cast<uint2*>(rows + i8 / (a.hd / 8) * pitch + i8 % (a.hd / 8) * 8);
         const uint2 w = *at;
-        auto four = [&](uint32_t c) {
-          const float2 lo = e4m3_values(c), hi = e4m3_values(c >> 16);
-          return e4m3_pair(lo.x * less, lo.y * less) | e4m3_pair(hi.x * less, hi.y * less) << 16;
-        };
-        *at = make_uint2(four(w.x), four(w.y));
+        *at = make_uint2(two(e4m3_values(w.x)) | two(e4m3_values(w.x >> 16)) << 16, two(e4m3_values(w.y)) | two(e4m3_values(w.y >> 16)) << 16);
       }
     }
     unsigned again = 0;   // rows with codes in doubt
@@ -634,14 +639,14 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
 #pragma unroll
         for (int e = 0; e < 2; e++) x[i].a[e] = pc_mul2(x[i].a[e], f), x[i].b[e] = pc_mul2(x[i].b[e], f);
         bool doubt = false;
-        const Codes y = is_v ? codes_of(x[i]) : codes_within(x[i], off_by, doubt);
+        const Codes y = is_v && !fine ? codes_of(x[i]) : codes_within(x[i], off_scaled, doubt);
         if (there) store_codes<VEC>(rows + (off + j) * pitch, m, y);
         if (there && doubt) again |= 1u << (u + i);
       }
     }
     for (again = __reduce_or_sync(~0u, again); again; again &= again - 1) {
       const int u = __ffs(again) - 1, j = u * RPP + lane / LPR;
-      const Codes y = codes_of(exact(u, inv));
+      const Codes y = codes_of(exact(u, 1.0 / scale));
       if (j < n && m.any()) {
         uint8_t* const at = rows + (off + j) * pitch;
         const Codes z = load_codes<VEC>(at, m);   // what fp32 does not hold stays NaN
