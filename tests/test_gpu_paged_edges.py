@@ -411,3 +411,80 @@ def test_codes_are_the_64_bit_values_rounded(P, ctx):
     got = pool.k.transpose(1, 2)[page, row].double()
     want = torch.round(u) * step
     assert torch.equal(got[clear], want[clear]) and int((~clear).sum()) < 8
+
+
+# ---- how they are called
+
+def stride_words(*tensors):
+    return (ctypes.c_int64 * 32)(*[s for t, n in tensors for s in t.stride()[:n]])
+
+
+def test_entries_by_their_argument_lists(P, gpu):
+    """The four C entries, every argument of a type another one: the bits of the Python calls."""
+    g, H, KH, hd, page, T, B, n = gen(71), 6, 2, 64, 32, 9, 3, 2
+    f = P.rotary_frequencies(48, 1e4, device="cuda")[0]
+    wq, wk, sinks = (1 + 0.3 * torch.randn(m, generator=g, device="cuda") for m in (hd, hd, H))
+    y = rand(g, T, H + 2 * KH, hd, dtype=torch.float16, scale=2.0)
+    q, k, v = y[:, :H], y[:, H:H + KH], y[:, H + KH:]
+    pos, stream = torch.randint(0, 9999, (T,), generator=g, device="cuda").int(), torch.cuda.current_stream().cuda_stream
+    at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    amp, eps = 1.25, 0.5 ** 10                                      # of fp32
+    # rotation
+    want = P.rotary(q, k, pos, f, interleaved=True, amplitude=amp, q_norm=wq, k_norm=wk, eps=eps)
+    got = torch.full_like(y, 9.0)[:, :H], torch.full((KH, T, hd), 9.0, dtype=torch.float16, device="cuda").transpose(0, 1)
+    st = stride_words((q, 2), (k, 2), (got[0], 2), (got[1], 2))
+    assert gpu.tg_rotary(1, at(q), at(k), at(got[0]), at(got[1]), at(pos), at(f), at(wq), at(wk), T, H, KH, hd, len(f), 1, amp, eps, st, stream) == 0
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for codes in (True, False):
+        a = Pool(g, torch.float16, codes, KH, hd, page, [100, 70, 41])
+        if codes:
+            a.vs = a.vs.permute(2, 0, 1).contiguous().permute(1, 2, 0)
+        a.v = a.v.view(torch.uint8 if codes else torch.int16).transpose(1, 2).contiguous().transpose(1, 2).view(a.v.dtype)
+        wide = torch.full((B, a.tables.shape[1] + 3), -1, dtype=torch.int32, device="cuda")
+        wide[:, :a.tables.shape[1]] = a.tables
+        a.tables = wide[:, :a.tables.shape[1]]
+        b, cu = a.clone(), ints(0, 4, 5, 9)
+        b.v = b.v.view(torch.uint8 if codes else torch.int16).transpose(1, 2).contiguous().transpose(1, 2).view(b.v.dtype)
+        b.tables = wide[:, :a.tables.shape[1]]
+        none = torch.empty_strided((1, 1, 1), (1, 1, 1))
+        cache = lambda p: ((p.k, 3), (p.v, 3), (none if p.ks is None else p.ks, 3), (none if p.vs is None else p.vs, 3), (p.tables, 1))  # noqa: E731
+        pb, cols = 8 if codes else 16, a.tables.shape[1]
+        # appending
+        want = P.cache_append(k, v, a.k, a.v, a.tables, a.lens, cu, **a.kw, freqs=f, positions=pos, amplitude=amp, q=q, q_norm=wq, k_norm=wk,
+                              eps=eps)
+        out = torch.full_like(y, 9.0)[:, :H]
+        st = stride_words((q, 2), (k, 2), (v, 2), (out, 2), *cache(b))
+        assert gpu.tg_paged_append(1, pb, at(q), at(k), at(v), at(out), at(b.k), at(b.v), at(b.ks), at(b.vs), at(b.tables), at(b.lens), at(cu), at(pos),
+                                   at(f), at(wq), at(wk), T, B, b.n, page, cols, H, KH, hd, len(f), 0, amp, eps, st, stream) == 0
+        assert torch.equal(out, want) and torch.equal(bits(a.k), bits(b.k)) and torch.equal(bits(a.v), bits(b.v))
+        assert not codes or (torch.equal(a.ks, b.ks) and torch.equal(a.vs, b.vs))
+        # attention, whole and cut
+        x = rand(g, B, n, H, hd, dtype=torch.float16)
+        for max_len, window in ((128, 30), (128, 0), (99, 0)):
+            want = P.attention_paged(x, a.k, a.v, a.tables, a.lens, **a.kw, max_len=max_len, window=window, sinks=sinks, scale=0.25)
+            out = torch.full((H, B, n, hd), 9.0, dtype=torch.float16, device="cuda").permute(1, 2, 0, 3)
+            size = gpu.tg_attention_paged_workspace(pb, B, n, max_len, window, H, KH, hd)
+            ws = torch.empty(max(size, 1), dtype=torch.uint8, device="cuda")
+            st = stride_words((x, 3), (out, 3), *cache(b))
+            assert gpu.tg_attention_paged(1, pb, at(x), at(b.k), at(b.v), at(b.ks), at(b.vs), at(out), at(b.tables), at(b.lens), at(sinks), B, n, b.n, page,
+                                          cols, max_len, H, KH, hd, st, window, 0.25, at(ws), size, stream) == 0
+            assert torch.equal(out, want)
+        # a unit's tiles in several pieces
+        long = Pool(g, torch.float16, codes, KH, hd, page, [2000, 70, 1500])
+        want = P.attention_paged(x, long.k, long.v, long.tables, long.lens, **long.kw, sinks=sinks, scale=0.25, max_len=2000)
+        size = gpu.tg_attention_paged_workspace(pb, B, n, 2000, 0, H, KH, hd)
+        assert size > 0
+        ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+        st = stride_words((x, 3), (out, 3), *cache(long))
+        assert gpu.tg_attention_paged(1, pb, at(x), at(long.k), at(long.v), at(long.ks), at(long.vs), at(out), at(long.tables), at(long.lens), at(sinks), B, n,
+                                      long.n, page, long.tables.shape[1], 2000, H, KH, hd, st, 0, 0.25, at(ws), size, stream) == 0
+        assert torch.equal(out, want)
+        # reading back
+        cu = ints(0, 40, 70, 111)
+        want = P.cache_gather(a.k, a.v, a.tables, cu, 111, **a.kw, dtype=torch.float16)
+        ko, vo = torch.full((111, KH, hd), 9.0, dtype=torch.float16, device="cuda"), torch.full((KH, 111, hd), 9.0, dtype=torch.float16, device="cuda").transpose(0, 1)
+        st = stride_words((ko, 2), (vo, 2), *cache(b))
+        assert gpu.tg_paged_gather(1, pb, at(b.k), at(b.v), at(b.ks), at(b.vs), at(b.tables), at(cu), at(ko), at(vo), 111, B, b.n, page, cols, KH, hd, st,
+                                   stream) == 0
+        assert torch.equal(ko, want[0]) and torch.equal(vo, want[1])
+    assert tg.last_error(gpu)[0] in (0, 3)
