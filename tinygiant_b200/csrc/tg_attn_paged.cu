@@ -65,7 +65,7 @@ struct PagedArgs {
   int B, n, rows, rt, KH, G, hd, cols, n_pages, shift, max_len, window;
   unsigned by_g;  // 2^32 / G, rounded up (G > 1)
   int whole;      // units are not cut
-  int team;       // warps of a group: 1, 2 or 4
+  int team;       // warps of a group: 4, or 1 or 2 where units are not cut
   int unit;       // what a unit's start and end cost, in tiles of a warp
   float c;        // scale log2(e)
 };
@@ -654,7 +654,7 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
     const size_t slot = 2 * group + (wk.j == 0);
     if (!all && wk.j == 0 && mate == 0 && lane == 0)
       a.desc[group] = make_int4(wk.b, wk.kh * a.rt + wk.ri, paged_group(wk.x + wk.n - 1, total, parts), 0);
-    if (a.team == 1) {   // from the registers
+    if (a.team == 1) {   // a unit that was not cut, from the registers
 #pragma unroll
       for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -662,28 +662,21 @@ __global__ void __launch_bounds__((PagedShape<T, CODES, HD, NT>::THREADS), 1) pa
           float L = l[t][z], mm = m[t][z] - OFF;
 #pragma unroll
           for (int sft = 4; sft < 32; sft <<= 1) L += __shfl_xor_sync(~0u, L, sft);
-          const int h = t * 8 + t4 * 2 + z, row = row0 + h;
+          const int row = row0 + t * 8 + t4 * 2 + z;
           if (row >= a.rows) continue;
-          if (all) {
-            const int head = wk.kh * a.G + row - tok[t][z] * a.G;
-            if (a.sinks) {
-              const float sink = sink_of(a, head), top = fmaxf(mm, sink);
-              if (sink != -INFINITY) L = (L == 0.f ? 0.f : L * at_exp2(mm - top)) + at_exp2(sink - top), mm = top;
-            }
-            const float f = paged_factor(L, r[t][z] - OFF - mm);
-            T* out = (T*)a.out + wk.b * a.so[0] + tok[t][z] * a.so[1] + head * a.so[2];
+          const int head = wk.kh * a.G + row - tok[t][z] * a.G;
+          if (a.sinks) {
+            const float sink = sink_of(a, head), top = fmaxf(mm, sink);
+            if (sink != -INFINITY) L = (L == 0.f ? 0.f : L * at_exp2(mm - top)) + at_exp2(sink - top), mm = top;
+          }
+          const float f = paged_factor(L, r[t][z] - OFF - mm);
+          T* out = (T*)a.out + wk.b * a.so[0] + tok[t][z] * a.so[1] + head * a.so[2];
 #pragma unroll
-            for (int k = 0; k < S::STEPS; k += 4) {   // eight dimensions in a row
-              const int d = S::dim(k, g);
-              if (d < a.hd)
-                *reinterpret_cast<uint4*>(out + d) = make_uint4(at_pack<T>(o[t][k][z] * f, o[t][k][z + 2] * f), at_pack<T>(o[t][k + 1][z] * f, o[t][k + 1][z + 2] * f),
-                                                                at_pack<T>(o[t][k + 2][z] * f, o[t][k + 2][z + 2] * f), at_pack<T>(o[t][k + 3][z] * f, o[t][k + 3][z + 2] * f));
-            }
-          } else {
-            const size_t at = slot * (8 * NT) + h;
-#pragma unroll
-            for (int k = 0; k < S::STEPS; k++) *reinterpret_cast<float2*>(a.po + at * HD + 16 * k + 2 * g) = make_float2(o[t][k][z], o[t][k][z + 2]);
-            if (g == 0) a.pml[at] = make_float4(mm, L, r[t][z] - OFF, 0.f);
+          for (int k = 0; k < S::STEPS; k += 4) {   // eight dimensions in a row
+            const int d = S::dim(k, g);
+            if (d < a.hd)
+              *reinterpret_cast<uint4*>(out + d) = make_uint4(at_pack<T>(o[t][k][z] * f, o[t][k][z + 2] * f), at_pack<T>(o[t][k + 1][z] * f, o[t][k + 1][z + 2] * f),
+                                                              at_pack<T>(o[t][k + 2][z] * f, o[t][k + 2][z + 2] * f), at_pack<T>(o[t][k + 3][z] * f, o[t][k + 3][z + 2] * f));
           }
         }
       return;
