@@ -412,7 +412,8 @@ int tg_cache_evict(const void *k, const void *v, const float *weights, const int
 /* ---- A paged cache on device tensors ------------------------------------ *
  * No counterpart in the reference.  Pointers, types, streams, alignment and
  * errors as for the attention above; strides in elements, positive multiples
- * of 16 bytes but for scales and tables.
+ * of 16 bytes but for scales and tables, whose are positive.  Counts of tokens and
+ * rows are below 2^30.
  *
  * A cache is k_pages, v_pages [n_pages][n_kv_heads][page][head_dim], page a power
  * of two of at least 16, and tables [batch][table_cols]: position p of sequence

@@ -901,6 +901,7 @@ static int gather(ArgCheck& c, const GatherRecord& r) {
   need_ints(c, &r.total, 7);
   c.need(r.total >= 0 && r.batch >= 0 && r.n_kv_heads > 0, "n_kv_heads must be positive, the other counts not negative");
   c.need(r.n_kv_heads < 1 << 20, "too many heads");
+  c.need(r.total < 1 << 30, "total must be below 2^30");
   c.need(r.head_dim > 0 && r.head_dim % 8 == 0 && r.head_dim <= ATTN_MAX_HD, "head_dim must be a multiple of 8, at most 128");
   if (c.rc) return c.rc;
   const PoolCheck pool(c, (int)r.page_bits, (int)r.n_pages, (int)r.page, (int)r.table_cols, (int)r.batch, (int)r.n_kv_heads, (int)r.head_dim,
