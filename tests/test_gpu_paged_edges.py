@@ -488,3 +488,25 @@ def test_entries_by_their_argument_lists(P, gpu):
                                    stream) == 0
         assert torch.equal(ko, want[0]) and torch.equal(vo, want[1])
     assert tg.last_error(gpu)[0] in (0, 3)
+
+
+def refusal_tensors():
+    z = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt, device="cuda")  # noqa: E731
+    return {"q": z(4, 4, 64), "k": z(4, 2, 64), "f": z(32, dt=torch.float64), "i": ints(1, 2, 3, 4), "pages": z(3, 2, 32, 64),
+            "codes": z(3, 2, 32, 64, dt=E4M3), "scales": z(3, 2, 2, dt=torch.float32) + 1, "tables": z(4, 2, dt=torch.int32)}
+
+
+def test_broadcast_scales_and_tables_are_refused(P):
+    t = refusal_tensors()
+    q, k, i, codes, scales, tables = (t[n] for n in ("q", "k", "i", "codes", "scales", "tables"))
+    for s in (scales[:1].expand(3, 2, 2), scales[:, :1].expand(3, 2, 2), scales[..., :1].expand(3, 2, 2)):
+        for kw in ({"k_scales": s, "v_scales": scales}, {"k_scales": scales, "v_scales": s}):
+            for call in (lambda: P.attention_paged(q, codes, codes, tables, i, **kw), lambda: P.cache_append(k, k, codes, codes, tables, i, **kw),
+                         lambda: P.cache_gather(codes, codes, tables, ints(0, 1, 2, 3, 4), 4, **kw)):
+                with pytest.raises(ValueError, match="strides of scales"):
+                    call()
+    kw, one = {"k_scales": scales, "v_scales": scales}, tables[:1].expand(4, 2)
+    for call in (lambda: P.attention_paged(q, codes, codes, one, i, **kw), lambda: P.cache_append(k, k, codes, codes, one, i, **kw),
+                 lambda: P.cache_gather(codes, codes, one, ints(0, 1, 2, 3, 4), 4, **kw)):
+        with pytest.raises(ValueError, match="stride of tables"):
+            call()

@@ -32,7 +32,8 @@ stream of the tensors' device, take workspace and outputs from torch's
 allocator, can be captured in a CUDA graph, give the same bits each time, and
 read lengths and tables on the device.  Tensors may be strided views: the last
 dimension is contiguous, the other strides are multiples of 16 bytes (scales
-and tables: any), and data start on 16-byte boundaries.  head_dim is a
+and tables: any, all dimensions of scales), none is broadcast, and data start
+on 16-byte boundaries.  head_dim is a
 multiple of 8 (16 for pages of 8 bits), at most 128.  Norms, angles, rotations,
 softmax statistics and accumulators are fp32 or more.  Bad arguments raise
 ValueError before anything runs; there is no backward pass.
