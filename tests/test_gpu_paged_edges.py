@@ -510,3 +510,24 @@ def test_broadcast_scales_and_tables_are_refused(P):
                  lambda: P.cache_gather(codes, codes, one, ints(0, 1, 2, 3, 4), 4, **kw)):
         with pytest.raises(ValueError, match="stride of tables"):
             call()
+
+
+def test_numbers_that_are_none_are_refused(P):
+    """max_len, window, scale, total, eps and amplitude of other kinds: ValueError, and numpy's whole numbers count as such."""
+    t = refusal_tensors()
+    q, k, f, i, pages, tables = (t[n] for n in ("q", "k", "f", "i", "pages", "tables"))
+    for kw in ({"max_len": 2.5}, {"max_len": "9"}, {"max_len": math.nan}, {"max_len": [3]}, {"window": 1.5}, {"window": "2"}, {"window": None},
+               {"scale": "1"}, {"scale": [1.0]}, {"scale": math.inf}):
+        with pytest.raises(ValueError):
+            P.attention_paged(q, pages, pages, tables, i, **kw)
+    for kw in ({"eps": "x"}, {"eps": None}, {"amplitude": [1.0]}, {"interleaved": "yes"}):
+        with pytest.raises(ValueError):
+            P.rotary(q, k, i, f, **kw)
+        with pytest.raises(ValueError):
+            P.cache_append(k, k, pages, pages, tables, i, freqs=f, **kw)
+    for total in (4.0, "4", None, -1):
+        with pytest.raises(ValueError):
+            P.cache_gather(pages, pages, tables, ints(0, 1, 2, 3, 4), total)
+    want = P.attention_paged(q, pages, pages, tables, i, max_len=40, window=3)
+    assert torch.equal(P.attention_paged(q, pages, pages, tables, i, max_len=np.int64(40), window=np.int32(3)), want)
+    assert P.cache_gather(pages, pages, tables, ints(0, 1, 2, 3, 4), np.int64(4))[0].shape == (4, 2, 64)

@@ -38,6 +38,7 @@ multiple of 8 (16 for pages of 8 bits), at most 128.  Norms, angles, rotations,
 softmax statistics and accumulators are fp32 or more.  Bad arguments raise
 ValueError before anything runs; there is no backward pass.
 """
+import ctypes
 import math
 import struct
 
@@ -69,7 +70,7 @@ def _run(device, record):
 
 
 def _no_number(e):
-    """What struct cannot pack: a number that is none, or beyond 64 bits."""
+    """What struct cannot pack or ctypes pass: a number that is none, or beyond 64 bits."""
     raise ValueError(f"bad argument: {e}") from None
 
 
@@ -382,16 +383,16 @@ def attention_paged(q, k_pages, v_pages, tables, lens, *, k_scales=None, v_scale
             or (k_scales is not None and (k_scales.requires_grad or v_scales.requires_grad)) or (sinks is not None and sinks.requires_grad)):
         _no_backward()
     most = cols * page
-    max_len = most if max_len is None or max_len > most else max_len
-    bits, window = 16 if k_scales is None else 8, _window(window)
-    nbytes = load().tg_attention_paged_workspace(bits, B, n, max_len, window, H, KH, hd) if 0 < max_len < _MOST else 0
-    ws = _empty((nbytes,), (1,), dtype=torch.uint8, device=q.device) if nbytes else None
     try:
+        max_len = most if max_len is None or max_len > most else max_len
+        bits, window = 16 if k_scales is None else 8, _window(window)
+        nbytes = load().tg_attention_paged_workspace(bits, B, n, max_len, window, H, KH, hd) if 0 < max_len < _MOST else 0
+        ws = _empty((nbytes,), (1,), dtype=torch.uint8, device=q.device) if nbytes else None
         record = _ATTEND(2, kind, bits, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), 0 if k_scales is None else k_scales.data_ptr(),
                          0 if k_scales is None else v_scales.data_ptr(), out.data_ptr(), tables.data_ptr(), lens.data_ptr(),
                          0 if sinks is None else sinks.data_ptr(), B, n, N, page, cols, max_len, H, KH, hd, window, q0, q1, q2, o0, o1, o2,
                          *pool, hd ** -0.5 if scale is None else scale, 0 if ws is None else ws.data_ptr(), nbytes, _raw_stream(dev))
-    except (struct.error, OverflowError) as e:
+    except (struct.error, OverflowError, TypeError, ctypes.ArgumentError) as e:
         _no_number(e)
     _run(dev, record)
     if given:
