@@ -531,3 +531,29 @@ def test_numbers_that_are_none_are_refused(P):
     want = P.attention_paged(q, pages, pages, tables, i, max_len=40, window=3)
     assert torch.equal(P.attention_paged(q, pages, pages, tables, i, max_len=np.int64(40), window=np.int32(3)), want)
     assert P.cache_gather(pages, pages, tables, ints(0, 1, 2, 3, 4), np.int64(4))[0].shape == (4, 2, 64)
+
+
+def test_dual_tensors_are_refused(P):
+    """Forward-mode derivatives would be lost without a word: refused, here and by the attention operators beside."""
+    from torch.autograd import forward_ad as fw
+
+    from tinygiant_b200 import attention as A
+    t = refusal_tensors()
+    q, k, f, i, pages, tables = (t[n] for n in ("q", "k", "f", "i", "pages", "tables"))
+    cache, lens = torch.zeros(4, 2, 8, 64, dtype=torch.bfloat16, device="cuda"), ints(1, 2, 3, 4)
+    w = torch.zeros(4, 2, 8, device="cuda")
+    calls = [(q, lambda d: P.rotary(d, k, i, f)), (k, lambda d: P.rotary(q, d, i, f)), (f, lambda d: P.rotary(q, k, i, d)),
+             (q, lambda d: P.rotary(q, k, i, f, out=(d, k))),
+             (k, lambda d: P.cache_append(d, k, pages, pages, tables, i)), (k, lambda d: P.cache_append(k, d, pages, pages, tables, i)),
+             (pages, lambda d: P.cache_append(k, k, d, pages, tables, i)), (q, lambda d: P.cache_append(k, k, pages, pages, tables, i, q=d)),
+             (q, lambda d: P.attention_paged(d, pages, pages, tables, i)), (pages, lambda d: P.attention_paged(q, pages, d, tables, i)),
+             (pages, lambda d: P.cache_gather(pages, d, tables, ints(0, 1, 2, 3, 4), 4)),
+             (q, lambda d: A.attention_prompt(d, k, k, ints(0, 4))), (k, lambda d: A.attention_prompt(q, k, d, ints(0, 4))),
+             (q, lambda d: A.attention_shared(d, None, None, cache, cache, lens)), (cache, lambda d: A.attention_shared(q, None, None, cache, d, lens)),
+             (cache, lambda d: A.cache_evict(cache, d, w, lens, 4, 1))]
+    for x, call in calls:
+        call(x.clone())
+        with fw.dual_level():
+            call(x.clone())                                        # no tangent, no refusal
+            with pytest.raises(ValueError, match="no backward pass"):
+                call(fw.make_dual(x.clone(), torch.ones_like(x)))

@@ -22,11 +22,12 @@ and NaN too.  Bad arguments raise ValueError before anything runs
 (ArgumentError, a TinyGiantCudaError too, where the library sees them); other
 errors of the library raise TinyGiantCudaError.  There is no backward pass:
 where autograd would record the call (gradients on, and a tensor that requires
-them), it is refused.  Writes into out and weights count as changes in place.
+them, or a forward-mode dual tensor), it is refused.  Writes into out and weights count as changes in place.
 """
 import ctypes
 
 import torch
+from torch.autograd import forward_ad as _forward
 
 from . import TinyGiantCudaError, last_error, load
 
@@ -119,6 +120,12 @@ def _no_backward():
         raise ValueError("the attention operators have no backward pass: call them under torch.no_grad(), or detach the tensors")
 
 
+def _no_tangents(*tensors):
+    """Within a forward-mode level: refuses tensors with a tangent, which the call would lose."""
+    if any(t is not None and _forward.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError("the attention operators have no backward pass, and no forward-mode derivative: call them on the tensors' primals")
+
+
 def _need_out(out, q):
     if not isinstance(out, torch.Tensor) or out.shape != q.shape:
         raise ValueError(f"out must have the shape of q, {tuple(q.shape)}")
@@ -164,6 +171,8 @@ def attention_prompt(q, k, v, cu_q, cu_k=None, *, max_k=None, window=0, sinks=No
     if (q.requires_grad or k.requires_grad or v.requires_grad or (given and out.requires_grad)
             or (sinks is not None and sinks.requires_grad)):
         _no_backward()
+    if _forward._current_level >= 0:
+        _no_tangents(q, k, v, out, sinks)
     max_k = tk if max_k is None or max_k > tk else max_k
     lib = load()
     nbytes = lib.tg_attention_prompt_workspace(n, tq, max_k, H, KH, hd)
@@ -225,6 +234,8 @@ def attention_shared(q, prefix_k, prefix_v, k, v, lens, *, max_len=None, window=
             or (P and (prefix_k.requires_grad or prefix_v.requires_grad)) or (sinks is not None and sinks.requires_grad)
             or (weights is not None and weights.requires_grad)):
         _no_backward()
+    if _forward._current_level >= 0:
+        _no_tangents(q, prefix_k, prefix_v, k, v, sinks, weights, out)
     cap = k.shape[2]
     max_len = cap if max_len is None or max_len > cap else max_len
     lib = load()
@@ -273,6 +284,8 @@ def cache_evict(k, v, weights, lens, keep, recent):
                 [("weights", weights, torch.float32, k.shape[:3]), ("lens", lens, torch.int32, k.shape[:1])] if tensors else ())
     if k.requires_grad or v.requires_grad or weights.requires_grad:
         _no_backward()
+    if _forward._current_level >= 0:
+        _no_tangents(k, v, weights)
     B, KH, cap, hd = shape
     where = k.device
     if not (0 < keep <= cap and 0 <= recent <= keep):

@@ -45,7 +45,7 @@ import struct
 import torch
 
 from . import TinyGiantCudaError, last_error, load
-from .attention import _DTYPES, _MOST, ArgumentError, _empty, _no_backward, _raw_stream, _window, _written
+from .attention import _DTYPES, _MOST, ArgumentError, _empty, _forward, _no_backward, _no_tangents, _raw_stream, _window, _written
 
 __all__ = ["rotary_frequencies", "rotary", "cache_append", "attention_paged", "cache_gather", "ArgumentError"]
 
@@ -216,6 +216,8 @@ def rotary(q, k, positions, freqs, *, interleaved=False, amplitude=1.0, q_norm=N
     if (q.requires_grad or (k is not None and (k.requires_grad or ko.requires_grad)) or freqs.requires_grad or qo.requires_grad
             or (q_norm is not None and q_norm.requires_grad) or (k_norm is not None and k_norm.requires_grad)):
         _no_backward()
+    if _forward._current_level >= 0:
+        _no_tangents(q, k, freqs, q_norm, k_norm, qo, ko)
     try:
         record = _ROTARY(0, kind, q.data_ptr(), 0 if k is None else k.data_ptr(), qo.data_ptr(), 0 if k is None else ko.data_ptr(),
                          positions.data_ptr(), freqs.data_ptr(), 0 if q_norm is None else q_norm.data_ptr(),
@@ -301,6 +303,8 @@ def cache_append(k, v, k_pages, v_pages, tables, lens, cu=None, *, k_scales=None
             or (q is not None and (q.requires_grad or out.requires_grad)) or (q_norm is not None and q_norm.requires_grad)
             or (k_norm is not None and k_norm.requires_grad)):
         _no_backward()
+    if _forward._current_level >= 0:
+        _no_tangents(k, v, k_pages, v_pages, k_scales, v_scales, freqs, q, q_norm, k_norm, out)
     try:
         record = _APPEND(1, kind, 16 if k_scales is None else 8, 0 if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(),
                          0 if q is None else out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
@@ -382,6 +386,8 @@ def attention_paged(q, k_pages, v_pages, tables, lens, *, k_scales=None, v_scale
     if (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad or out.requires_grad
             or (k_scales is not None and (k_scales.requires_grad or v_scales.requires_grad)) or (sinks is not None and sinks.requires_grad)):
         _no_backward()
+    if _forward._current_level >= 0:
+        _no_tangents(q, k_pages, v_pages, k_scales, v_scales, sinks, out)
     most = cols * page
     try:
         max_len = most if max_len is None or max_len > most else max_len
@@ -446,6 +452,8 @@ def cache_gather(k_pages, v_pages, tables, cu, total, *, k_scales=None, v_scales
     if (k_pages.requires_grad or v_pages.requires_grad or ko.requires_grad or vo.requires_grad
             or (k_scales is not None and (k_scales.requires_grad or v_scales.requires_grad))):
         _no_backward()
+    if _forward._current_level >= 0:
+        _no_tangents(k_pages, v_pages, k_scales, v_scales, ko, vo)
     try:
         record = _GATHER(3, kind, 16 if k_scales is None else 8, k_pages.data_ptr(), v_pages.data_ptr(),
                          0 if k_scales is None else k_scales.data_ptr(), 0 if k_scales is None else v_scales.data_ptr(), tables.data_ptr(),
