@@ -462,8 +462,8 @@ int tg_paged_append(int dtype, int page_bits, const void *q, const void *k, cons
  * the positions up to it, with window > 0 to the last `window` of those.
  * lens[b] outside 0 .. max_len counts as the nearest inside; max_len is at
  * most table_cols x page.  sinks, and queries without a key: as
- * tg_attention_prompt.  With page_bits 8 the softmax weights meet the codes in
- * fp16.  strides: q, out (sequence, token, head), then the cache's: 19 values.
+ * tg_attention_prompt.  The softmax weights keep 22 bits, with pages of bf16 16.
+ * strides: q, out (sequence, token, head), then the cache's: 19 values.
  * workspace: 256-byte aligned, tg_attention_paged_workspace bytes. */
 size_t tg_attention_paged_workspace(int page_bits, int batch, int n_queries, int max_len, int window, int n_heads,
                                     int n_kv_heads, int head_dim);

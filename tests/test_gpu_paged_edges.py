@@ -141,6 +141,39 @@ def test_sinks_of_any_size(P, codes):
         assert torch.equal(torch.isnan(prompt[:2]), torch.isnan(got[:2, 0])) and not bool(prompt[:2, [0, 1, 6]].any())
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("codes", [True, False], ids=["8bit", "16bit"])
+@pytest.mark.parametrize("m", [7, 60, 3000])
+def test_weights_keep_more_bits_than_the_values(P, m, codes, dtype):
+    """Three keys of weight 1 and values of 1 against four of weight r and -1, r = 0.75 and 2^-12.2 (bf16 pages: 2^-9.2) more, which one
+    fp16 (or bf16) weight would round to 0.75: the output is what that drops.
+
+    Tolerance: u |o| for the output, and of A = 1 at most the weights' 2^-22 (2^-16), twice delta = (hd + 16) 2^-23 S + 2^-18 with S = scale
+    < 0.3, and fp32's sums."""
+    g, dt, hd = gen(56), DT[dtype], 16
+    pool = Pool(g, dt, codes, 1, hd, 16, [m])
+    for x, fill in (("k", -448.0), ("v", 0.0)):                     # the other keys' weights are e^-128
+        pages = getattr(pool, x)
+        pages.copy_(torch.full(pages.shape, fill, device="cuda").to(pages.dtype))
+        if codes:
+            getattr(pool, x + "s").fill_(1.0)
+    at = [round(i * (m - 1) / 6) for i in range(7)]
+    for i, j in enumerate(at):
+        put(pool, "k", 0, j, -1.0 if i % 2 == 0 else 0.0)
+        put(pool, "v", 0, j, -1.0 if i % 2 == 0 else 1.0)
+    q = torch.zeros(1, 1, 3, hd, dtype=dt, device="cuda")
+    q[..., 0] = 1.0
+    one, w = (2.0 ** -9.2, 2.0 ** -16) if dtype == "bf16" and not codes else (2.0 ** -12.2, 2.0 ** -22)
+    for more in (one, -one):
+        scale = float(np.float32(-math.log(0.75 * (1 + more))))
+        r = math.exp(-scale)
+        want = (3 - 4 * r) / (3 + 4 * r)
+        got = P.attention_paged(q, pool.k, pool.v, pool.tables, pool.lens, **pool.kw, scale=scale, max_len=m).double()
+        u = 2.0 ** -8 if dtype == "bf16" else 2.0 ** -11
+        tol = u * abs(want) + w + 2 * (32 * 2.0 ** -23 * scale + 2.0 ** -18)
+        assert abs(want) > 4 * tol and bool(((got - want).abs() <= tol).all()), (got[0, 0, 0, 0].item(), want)
+
+
 # ---- codes next to a border
 
 E4M3_VALUES = np.array([0.0, *(m / 512 for m in range(1, 8)), *((8 + m) / 8 * 2.0 ** e for e in range(-6, 9) for m in range(8))][:127], dtype=L)

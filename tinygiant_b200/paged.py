@@ -356,9 +356,8 @@ def attention_paged(q, k_pages, v_pages, tables, lens, *, k_scales=None, v_scale
     A query without a key gives zeros.  Rows behind lens or before every
     query's window are not read, and nothing that a query does not attend to
     reaches it, infinities and NaN neither; a score of NaN or +inf among its keys
-    makes its outputs NaN, one of -inf has no weight.  With pages of 8 bits the
-    softmax weights meet the codes in fp16, else in the tensors' type.
-    Returns out, of q's shape."""
+    makes its outputs NaN, one of -inf has no weight.  The softmax weights keep
+    22 bits, with bfloat16 pages 16.  Returns out, of q's shape."""
     given = out is not None
     try:
         dtype, dev, shape = q.dtype, q.get_device(), q.shape
