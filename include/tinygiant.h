@@ -447,10 +447,10 @@ int tg_rotary(int dtype, const void *q, const void *k, void *q_out, void *k_out,
  * written, rows of no sequence are left out.  With page_bits 8 a block's scale is
  * the least power of two (2^-117 at least) under which its values are at most
  * 448, or larger if its earlier tokens' is; if it grows, their codes are
- * rounded again; a block's first token starts it anew.  A code is the nearest
- * to what the formulas give exactly; values that are not finite become NaN.  No place may be written twice in a call, and no 8-bit block
- * by two sequences.  strides: q, k, v, q_out (token, head), then the cache's: 21
- * values. */
+ * rounded again; a block's first token starts it anew.  Scales and codes are those
+ * of the formulas in 64 bits; values that are not finite in fp32 become NaN.  No
+ * place may be written twice in a call, and no 8-bit block by two sequences.
+ * strides: q, k, v, q_out (token, head), then the cache's: 21 values. */
 int tg_paged_append(int dtype, int page_bits, const void *q, const void *k, const void *v, void *q_out, void *k_pages,
                     void *v_pages, float *k_scales, float *v_scales, const int *tables, const int *lens, const int *cu,
                     const int *positions, const double *freqs, const float *q_norm, const float *k_norm, int n_tokens,

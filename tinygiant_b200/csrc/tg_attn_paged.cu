@@ -10,8 +10,9 @@
 //
 // Bound by HBM: each key is read once for the rows (query, head of the group)
 // of its key head, up to 16 at a time, so S^T = K Q^T and O^T += V^T P^T run on
-// mma.m16n8k16 with keys and dimensions as the 16 and the rows as the 8 columns
-// (the tensor-memory path has 128 rows to fill).  Codes are exact in fp16, so
+// mma.m16n8k16 with keys and dimensions as the 16 and the rows as the 8 columns.
+// (With 128 keys as the tensor memory's rows one token would be bound by HBM all the
+// same; more than 16 rows would read their keys once.)  Codes are exact in fp16, so
 // with them both products are fp16's: q in fp16 as it is, in bf16 times a power
 // of two that takes its row's largest value to 2^14 (what falls below fp16's
 // least normal value is 2^-28 of that).  A weight meets the values in two parts, its
@@ -36,10 +37,15 @@
 // order that may change.
 //
 // What bounds it (32 / 4 heads of 128, codes): 256 sequences of 2,048 to 8,192
-// keys, 1.35 GB: 230 us, 0.89 of a copy's rate; a tile takes a warp about 770
-// instructions (loads 160, codes to fp16 130, products 32, softmax 120), 3 of 4
-// issue slots at that rate.  64 sequences of 1 to 4,096: 34 us where the bytes
-// take 20: start and cut 4, units' starts and ends 4, the second kernel 5.
+// keys, 1.35 GB: 225 us at the full clock, 0.91 of a copy's rate; a tile takes a warp
+// about 810 instructions (loads 160, codes to fp16 130, products 48, softmax 140), 0.6
+// of the issue slots at that rate.  Call after call the chip's power limit takes the
+// clock to 1,560 MHz, and instructions bound it: 259 us.  64 sequences of 1 to 4,096:
+// 36 us where the bytes take 20: start and cut 4, units' starts and ends 4, the second
+// kernel 5.
+//
+// Registers: 168 of a thread with 8 rows a unit, up to 255 with 16; with heads of 128
+// and codes 24 to 68 bytes are spilled.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>

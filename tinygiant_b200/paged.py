@@ -25,7 +25,9 @@ head.  cache_append makes scales that are powers of two, the least (but 2^-117
 at least) under which a block's values reach no further than 448; a larger
 token raises its block's scale, and the codes before it in the block are
 rounded again.  A first token of a block starts its scale anew, whatever was
-there.  attention_paged and cache_gather take any positive scales.
+there.  attention_paged and cache_gather take any positive scales, and
+cache_append keeps one that it finds before a block's new tokens where it is
+the larger.
 
 As in tinygiant_b200.attention: calls are asynchronous on torch's current
 stream of the tensors' device, take workspace and outputs from torch's
@@ -263,8 +265,10 @@ def cache_append(k, v, k_pages, v_pages, tables, lens, cu=None, *, k_scales=None
     its query is rotated all the same.  Rows of no sequence are left out, the
     query's too.  No place may be written twice in a call, and in pages of 8
     bits no two sequences may write to one block: its values would be undefined.
-    In 8 bits a code is the nearest to what the formulas give exactly, and a
-    value that is not finite becomes NaN and does not count for the scale.  Returns the rotated q, or None."""
+    In 8 bits scales and codes are those of the formulas in 64 bits, whatever
+    order fp32 would have summed in; a value that is not finite in fp32 becomes
+    NaN and does not count for the scale, and heads whose sum of squares fp32
+    does not hold are normed to zero.  Returns the rotated q, or None."""
     given = out is not None
     try:
         dtype, dev, shape, (k0, k1, k2), (v0, v1, v2) = k.dtype, k.get_device(), k.shape, k.stride(), v.stride()
