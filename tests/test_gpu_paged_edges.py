@@ -262,6 +262,23 @@ def test_codes_of_angles_next_to_a_border(P, p, low, high, interleaved):
         assert ks[0] == 1 and np.array_equal(got[0], want), int((got[0] != want).sum())
 
 
+@pytest.mark.parametrize("f", [0.7, 1e3, 1.7e7, 1.3e9, 2.1e12, 1e18, 1e40])
+def test_frequencies_of_any_size(P, f):
+    """Angles of more turns than fp64 counts: to 2^-20 as long as a position's turns are below 2^60, and a rotation always."""
+    pos = ints(0, 1, -1, 77777, 123456789, -987654321, 2147483647, -2147483647)
+    freqs = torch.tensor([f * 2.0 ** -i for i in range(32)], dtype=torch.float64, device="cuda")
+    q = torch.zeros(8, 1, 64, dtype=torch.float16, device="cuda")
+    q[..., :32] = 1.0
+    got = P.rotary(q, None, pos, freqs)[0][:, 0].double()
+    # fp16 rounds by 2^-11 at most, fp32's sine and cosine by 2^-25, twice
+    assert bool(((got[:, :32].square() + got[:, 32:].square() - 1).abs() <= 2.0 ** -9).all())
+    if f < 2e9:
+        for i, p in enumerate(pos.tolist()):
+            c, s = turned(L(1), L(0), p, freqs.cpu().numpy())
+            want = torch.tensor([float(x) for x in (*c, *s)], dtype=torch.float64, device="cuda")
+            assert bool(((got[i] - want).abs() <= 2.0 ** -12 + 2.0 ** -20).all()), (p, float((got[i] - want).abs().max()))
+
+
 def test_codes_of_amplitudes_and_eps_next_to_a_border(P):
     """An amplitude and an eps that fp32 does not hold decide codes."""
     rng, n = np.random.default_rng(62), 32

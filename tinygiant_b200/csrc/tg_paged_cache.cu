@@ -67,19 +67,21 @@ struct CacheArgs {
 
 // p f radians in turns, as whole quarters and a rest of an eighth at most.  f / 2 pi is
 // a sum of two doubles and the product with p is kept whole, so the rest is off by
-// 2^-56 of a turn however far p is.
+// 2^-56 of a turn as long as there are 2^50 of them at most, beyond by 2^-106 of all.
 struct Turn {
-  double quarters, rest;
+  int quarters;   // modulo 4
+  double rest;
   __device__ __forceinline__ Turn(int p, double f) {
     const double per = 0.15915494309189535, per_low = -9.839338337591243e-18;   // 1 / 2 pi
     const double h = f * per, l = fma(f, per_low, fma(f, per, -h)), t = p * h;
-    quarters = rint(4.0 * t);
-    rest = fma(-0.25, quarters, t) + fma((double)p, l, fma((double)p, h, -t));
+    const double n = rint(4.0 * t), r = fma(-0.25, n, t) + fma((double)p, l, fma((double)p, h, -t));
+    const double m = rint(4.0 * r);   // the second double's, where there are so many turns
+    rest = fma(-0.25, m, r);
+    quarters = (int)fma(-4.0, rint(0.25 * n), n) + (int)fma(-4.0, rint(0.25 * m), m) & 3;
   }
   __device__ __forceinline__ double2 whole(double s, double c) const {   // of the rest's sine and cosine: cosine, sine
-    const int q = (int)((long long)quarters & 3);
-    const double cs = q & 1 ? -s : c, sn = q & 1 ? c : s;
-    return q & 2 ? make_double2(-cs, -sn) : make_double2(cs, sn);
+    const double cs = quarters & 1 ? -s : c, sn = quarters & 1 ? c : s;
+    return quarters & 2 ? make_double2(-cs, -sn) : make_double2(cs, sn);
   }
 };
 // cos and sin of p f radians, times amp, for fp32: Taylor's series at an eighth of a
