@@ -430,7 +430,8 @@ int tg_cache_evict(const void *k, const void *v, const float *weights, const int
  * n_freqs), or (2 j, 2 j + 1) if interleaved; it turns by position x freqs[j]
  * radians and is multiplied by amplitude; dimensions from 2 n_freqs on stay.
  * q_norm, k_norm [head_dim] (or NULL): each head is first divided by
- * sqrt(mean(x^2) + eps) and multiplied by these.  q_out and k_out may be q and k.
+ * sqrt(mean(x^2) + eps) and multiplied by these, the squares summed in fp32 (heads
+ * of 2^64 come out as zero).  q_out and k_out may be q and k.
  * n_heads or n_kv_heads may be 0.  strides: q, k, q_out, k_out (token, head): 8
  * values. */
 int tg_rotary(int dtype, const void *q, const void *k, void *q_out, void *k_out, const int *positions,
@@ -463,6 +464,8 @@ int tg_paged_append(int dtype, int page_bits, const void *q, const void *k, cons
  * lens[b] outside 0 .. max_len counts as the nearest inside; max_len is at
  * most table_cols x page.  sinks, and queries without a key: as
  * tg_attention_prompt.  The softmax weights keep 22 bits, with pages of bf16 16.
+ * With page_bits 8 values of bf16 queries below 2^-31 of their head's largest may
+ * lose bits, below 2^-40 they count as zero.
  * strides: q, out (sequence, token, head), then the cache's: 19 values.
  * workspace: 256-byte aligned, tg_attention_paged_workspace bytes. */
 size_t tg_attention_paged_workspace(int page_bits, int batch, int n_queries, int max_len, int window, int n_heads,

@@ -174,6 +174,22 @@ def test_weights_keep_more_bits_than_the_values(P, m, codes, dtype):
         assert abs(want) > 4 * tol and bool(((got - want).abs() <= tol).all()), (got[0, 0, 0, 0].item(), want)
 
 
+@pytest.mark.parametrize("power", [-110, -20, 0, 20, 97])
+def test_queries_of_a_wide_range_over_codes(P, power):
+    """bf16 queries one value of which is 2^30 times the others and meets keys of zero: the others keep all their bits."""
+    g, m, hd = gen(57), 300, 64
+    pool = Pool(g, torch.bfloat16, True, 1, hd, 16, [m])
+    k = pool.k.float()
+    k[..., 9] = 0.0
+    pool.k.copy_(k.to(E4M3))
+    q = rand(g, 1, 1, 8, hd, dtype=torch.bfloat16).abs().clamp(0.51, 0.99)
+    q[..., 9] = 2.0 ** 30
+    scale = 2.0 ** -power / 8
+    q = (q.float() * 2.0 ** power).to(torch.bfloat16)
+    got = P.attention_paged(q, pool.k, pool.v, pool.tables, pool.lens, **pool.kw, scale=scale)
+    check(got, *paged_ref(pool, q, [m], scale=scale), True)
+
+
 # ---- codes next to a border
 
 E4M3_VALUES = np.array([0.0, *(m / 512 for m in range(1, 8)), *((8 + m) / 8 * 2.0 ** e for e in range(-6, 9) for m in range(8))][:127], dtype=L)

@@ -14,8 +14,8 @@
 // (With 128 keys as the tensor memory's rows one token would be bound by HBM all the
 // same; more than 16 rows would read their keys once.)  Codes are exact in fp16, so
 // with them both products are fp16's: q in fp16 as it is, in bf16 times a power
-// of two that takes its row's largest value to 2^14 (what falls below fp16's
-// least normal value is 2^-28 of that).  A weight meets the values in two parts, its
+// of two that takes its row's largest value to 2^14 or more (fp16 keeps bf16's 8 bits
+// down to 2^-31 of that, and nothing below 2^-40).  A weight meets the values in two parts, its
 // rounding to 16 bits and what that drops, 22 bits together in fp16 and 16 in bf16:
 // of 64 sequences' bf16 outputs one in 1,600 is not the exact value's rounding, with
 // one part one in 12 (drafts in fp16: one in 460, and one in 3).  The second product

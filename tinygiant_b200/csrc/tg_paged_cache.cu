@@ -433,7 +433,7 @@ __device__ __forceinline__ void token_rows(const CacheArgs& a, CacheShared& sh, 
 // and a rotation a value y is off by at most 14.5 2^-24 |(a, b)| <= PC_OFF (|y_a| +
 // |y_b|) of its pair.  Where both ends of that interval round to one code, that is
 // it; the rows of the others, one value in 7,000, are worked out in 64 bits by the
-// whole warp.  The test for doubt takes 2 of 8,192 tokens' 45 us and those rows 5.
+// whole warp.  The test for doubt takes 2 of 8,192 tokens' 46 us and those rows 6.
 // So it is with the scale, where the largest value, off by at most 2 PC_OFF of
 // itself, may lie on either side of a border (one block in 100,000).
 constexpr float PC_OFF = 0x1p-20f, PC_OFF_MOST = 0x1p-18f;
@@ -664,9 +664,9 @@ __device__ __forceinline__ void runs_of_blocks(const CacheArgs& a, CacheShared& 
 
 // Rows of tokens and, beside them in the same launch, runs of 8-bit blocks, so that
 // the copies of the one overlap the instructions of the other.  Measured in a
-// replayed graph, bf16, heads of 128: 8,192 tokens x 32 heads rotated 21 us (0.97 of
-// a copy's rate, part of it from L2: bytes bound it), with norms 25.7 (instructions);
-// the same with 4 key heads to 8-bit pages 45, without norms 36, where 160 MB take
+// replayed graph, bf16, heads of 128: 8,192 tokens x 32 heads rotated 22 us (0.94 of
+// a copy's rate, part of it from L2: bytes bound it), with norms 26 (instructions);
+// the same with 4 key heads to 8-bit pages 46, without norms 37, where 160 MB take
 // 24, and to 16-bit pages 37.  A chunk of 2,048 tokens 20; two tokens 5, to 16-bit pages
 // 4, of which an empty kernel is 2.
 template <typename T, int LPR, bool VEC, int MODE, bool NORM, int R>

@@ -182,7 +182,9 @@ def rotary(q, k, positions, freqs, *, interleaved=False, amplitude=1.0, q_norm=N
     Pair j of a head is its dimensions (j, j + n), or (2 j, 2 j + 1) if
     interleaved; dimensions from 2 n on stay as they are.  The pairs are
     multiplied by amplitude.  q_norm, k_norm [hd] fp32: each head is first
-    divided by sqrt(mean(x^2) + eps) and multiplied by these.
+    divided by sqrt(mean(x^2) + eps) and multiplied by these; the squares are
+    summed in fp32, so heads of 2^64 are normed to zero, and with an eps of
+    nothing heads below 2^-60 lose bits.
     out: (q, k) to write, which may be q and k themselves but must not overlap
     them in any other way.  Returns (q, k), k None if it was."""
     given = out is not None
@@ -266,9 +268,9 @@ def cache_append(k, v, k_pages, v_pages, tables, lens, cu=None, *, k_scales=None
     query's too.  No place may be written twice in a call, and in pages of 8
     bits no two sequences may write to one block: its values would be undefined.
     In 8 bits scales and codes are those of the formulas in 64 bits, whatever
-    order fp32 would have summed in; a value that is not finite in fp32 becomes
-    NaN and does not count for the scale, and heads whose sum of squares fp32
-    does not hold are normed to zero.  Returns the rotated q, or None."""
+    order fp32 would have summed in (rotary's limits of a head's squares hold
+    here too); a value that is not finite in fp32 becomes NaN and does not count
+    for the scale.  Returns the rotated q, or None."""
     given = out is not None
     try:
         dtype, dev, shape, (k0, k1, k2), (v0, v1, v2) = k.dtype, k.get_device(), k.shape, k.stride(), v.stride()
@@ -361,7 +363,10 @@ def attention_paged(q, k_pages, v_pages, tables, lens, *, k_scales=None, v_scale
     query's window are not read, and nothing that a query does not attend to
     reaches it, infinities and NaN neither; a score of NaN or +inf among its keys
     makes its outputs NaN, one of -inf has no weight.  The softmax weights keep
-    22 bits, with bfloat16 pages 16.  Returns out, of q's shape."""
+    22 bits, with bfloat16 pages 16.  Over 8-bit pages bfloat16 queries are taken
+    in fp16 times a power of two of their head's own: values below 2^-31 of the
+    head's largest may lose bits, below 2^-40 they count as zero.  Returns out, of
+    q's shape."""
     given = out is not None
     try:
         dtype, dev, shape = q.dtype, q.get_device(), q.shape
