@@ -623,3 +623,32 @@ def test_dual_tensors_are_refused(P):
             call(x.clone())                                        # no tangent, no refusal
             with pytest.raises(ValueError, match="no backward pass"):
                 call(fw.make_dual(x.clone(), torch.ones_like(x)))
+
+
+@pytest.mark.parametrize("codes", [True, False], ids=["8bit", "16bit"])
+def test_two_calls_at_once(P, codes):
+    """Two streams append to and attend over one pool, each for its own sequences, under inference mode: the bits of one after the other."""
+    g, H, KH, hd, n = gen(72), 16, 2, 128, 6
+    lens = [1500, 700, 33, 2100, 16, 900]
+    pool = Pool(g, torch.bfloat16, codes, KH, hd, 16, lens)
+    q, k, v = (rand(g, n, h, hd, dtype=torch.bfloat16) for h in (H, KH, KH))
+    f = P.rotary_frequencies(hd, device="cuda")[0]
+
+    def half(p, rows):
+        outs = []
+        for _ in range(20):
+            y = P.cache_append(k[rows], v[rows], p.k, p.v, p.tables[rows], p.lens[rows], **p.kw, freqs=f, q=q[rows])
+            outs.append(P.attention_paged(y, p.k, p.v, p.tables[rows], p.lens[rows], **p.kw))
+        return outs
+
+    with torch.inference_mode():
+        one, both = pool.clone(), pool.clone()
+        want = half(one, slice(0, 3)) + half(one, slice(3, 6))
+        streams, got = [torch.cuda.Stream() for _ in range(2)], []
+        for s, rows in zip(streams, (slice(0, 3), slice(3, 6))):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got += half(both, rows)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert torch.equal(bits(one.k), bits(both.k)) and torch.equal(bits(one.v), bits(both.v))
