@@ -1,7 +1,7 @@
 """The paged cache where it can go wrong: values that are not finite beside cuts, codes and scales next to a border,
 earlier scales of any kind, the C entries by their argument lists, and what is refused beside the ordinary.
 
-Tolerances: none.  Codes, scales and NaN are compared for equality; expected codes are worked out on the host in
+Tolerances: none, but where a test derives its own.  Codes, scales and NaN are compared for equality; expected codes are worked out on the host in
 numpy's long doubles (64 bits of mantissa; angles reduced in decimals), from inputs chosen so that the exact value is 2^-44
 of itself or more away from the border between two codes, which that arithmetic (2^-58 of a pair) and fp64's (2^-50)
 resolve."""
